@@ -181,7 +181,7 @@ def _logits(case, g):
     rows, n, kind = case["rows"], case["n"], case["kind"]
     x = 2.5 * torch.randn(rows, n, generator=g, device=DEV)
     likely = torch.randint(0, n, (rows, 24), generator=g, device=DEV)
-    x.scatter_(1, likely, 9.0 + 3.0 * torch.randn(rows, 24, generator=g, device=DEV))
+    x.scatter_reduce_(1, likely, 9.0 + 3.0 * torch.randn(rows, 24, generator=g, device=DEV), "amax")      # the same place twice: the larger, whichever comes first
     x.scatter_(1, torch.randint(0, n, (rows, 8), generator=g, device=DEV), -math.inf)
     r = torch.rand(rows, 5, generator=g, device=DEV)
     one = torch.ones(rows, device=DEV)
