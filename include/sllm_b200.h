@@ -143,6 +143,15 @@ int sllm_store_kv_row(const float* src, void* cache_row, int32_t kv_dtype, int32
 int sllm_sample_f32(const float* logits, int32_t n, float temperature, int32_t top_k, float top_p, uint64_t seed,
                     uint64_t step, int32_t* idx_dev, sllm_stream_t stream);
 
+/* The same for all rows of a step in one launch, with settings of each row's own and from random numbers the caller gives. Row r of `rows`: n logits at logits + r * ld.
+ * temperature, top_k, top_p, min_p, u: device arrays of one value per row (temperature NULL = 1, the next three NULL = all logits). w_i = exp((x_i - max x) / temperature);
+ * kept are the top_k largest logits (0 = all), of these the smallest set of largest ones whose mass reaches top_p of theirs (0 or 1 = all), of these those with w_i >= min_p
+ * (0 = all); equal logits are in or out together. Drawn is the first i whose running kept mass exceeds u * (kept mass), u in [0, 1). temperature <= 0: the first of the largest
+ * logits. NaN counts as -infinity, which is never drawn (a row of nothing else gives 0); where logits are +infinity, one of those is drawn. Weights are held as multiples of 2^-44, so
+ * that sums are exact and the result is a function of the row alone. idx_dev [rows] int32; prob_dev [rows] or NULL: the drawn one's share of the kept mass. Up to 786432 logits a row. */
+int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, int32_t n, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                     const float* u, int32_t* idx_dev, float* prob_dev, sllm_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------------------
  * Synthetic weights (device side of oracle/synth_weights.h: same integer hash, bit-identical values).
  * Fills `count` elements [first, first+count) of blob segment `segment` (0 E, 1 norms, 2 wq, 3 wk, 4 wv,
@@ -524,6 +533,26 @@ int sllm_seq_attention_out(const sllm_seq_batch* b, const float* q, int32_t ldq,
 int sllm_seq_attention_finish(const sllm_seq_batch* b, const float* ws, int32_t nsplit, int32_t heads, int32_t dv, const double* vfreq,
                               int32_t layout, const float* gate, int32_t ldg, int32_t gate_channels, const float* sink, float* out,
                               int32_t ldo, void* out16, sllm_stream_t stream);
+/* The 8-bit cache. Pools [pages][kv_heads][page_len][width] of e4m3 codes beside scales [pages][kv_heads][page_len / 32] of fp32: a value is code * scale. The scale of 32 positions
+ * of one head (SLLM_KV8_BLOCK) is the smallest power of two, 2^-100 at least, under which their largest magnitude is at most 448. Head widths are multiples of 16 up to 256, pools
+ * start at a multiple of 16 bytes and have n_pages pages: the kernels touch no others, whatever the block table says. */
+#define SLLM_KV8_BLOCK 32
+/* Rotary positions on q (to q_out, which may be q) and k, and the append: the first 2 * n_freq dimensions of every head turn by the angles of sllm_seq_angles (layout as in
+ * sllm_seq_rotary_kv); k and v go to the cache as codes. A block that a segment begins or that it fills from its first row on takes the scale of the new rows; a block that holds earlier
+ * rows takes the larger of its scale and theirs, and the earlier rows' codes move to it (exact but for codes that become subnormal). Rows behind a segment's last position count as
+ * empty, their codes stay as they are. NaN and infinite values become NaN codes and do not count for the scale. A sequence brings one segment a step. Tokens with tok_slot < 0
+ * are skipped. Where the table has no page, and for two segments of one sequence, nothing is written and the library's next call returns SLLM_EINVAL. */
+int sllm_seq_rotary_kv8(const sllm_seq_batch* b, const float* q, int32_t ldq, int32_t heads, int32_t dk, const float* k, int32_t ldk, int32_t kv_heads, const float* v,
+                        int32_t ldv, int32_t dv, const float* angles, int32_t n_freq, int32_t layout, float* q_out, int32_t ldqo, void* k_pool, float* k_scale,
+                        void* v_pool, float* v_scale, int32_t n_pages, sllm_stream_t stream);
+/* Causal softmax attention of the listed tiles' tokens over the 8-bit cache: score = (q . k) * scale, query head h reads key/value head h / (heads / kv_heads). Options: window,
+ * keep_first, softcap, slopes, chunk; the others are SLLM_ENOTSUP. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16); rows of tokens in no tile stay as
+ * they are. Keys whose page the table does not have are hidden; a token that sees none gives zeros. ws: at least sllm_seq_attention8_ws_bytes bytes, 16-byte aligned, zeros
+ * before its first use; every call leaves its counters zero, so calls one behind the other may share it, calls that run side by side may not. */
+int64_t sllm_seq_attention8_ws_bytes(const sllm_seq_batch* b, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv);
+int sllm_seq_attention8(const sllm_seq_batch* b, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, float scale, const void* k_pool,
+                        const float* k_scale, const void* v_pool, const float* v_scale, int32_t n_pages, void* ws, int64_t ws_bytes, const sllm_seq_attn_opts* opts, float* out,
+                        int32_t ldo, void* out16, sllm_stream_t stream);
 /* Softmax attention whose SCORES are mixed over the heads before the softmax: own_g = (q_g . k of g's key head) * scale for every query
  * head g, then score_h = sum_g talk[h][g] own_g (talk [heads][heads] fp32); values of head h's own value head. The keys of all heads of a
  * token lie side by side in ONE pool row, k_pool [pages][1][page_len][kv_heads * dk]; v_pool [pages][kv_heads][page_len][dv]. Window,

@@ -60,6 +60,8 @@ int status_take() {
     const int32_t what = g_status ? __atomic_exchange_n(g_status, 0, __ATOMIC_ACQ_REL) : 0;
     if (what == 0) return SLLM_OK;
     SLLM_REQUIRE(what != kStatusBatch, SLLM_EINVAL, "seq_ssd_blocks: n_qtiles of an earlier launch does not count the tiles of all its tokens; its results are incomplete");
+    SLLM_REQUIRE(what != kStatusPages, SLLM_EINVAL, "seq_rotary_kv8: a position of an earlier launch has no page in the block table; nothing was written there");
+    SLLM_REQUIRE(what != kStatusTwice, SLLM_EINVAL, "seq_rotary_kv8: an earlier launch had two segments of one sequence; their keys and values were not written");
     set_error("a kernel gave up waiting for its copies or products: the results of an earlier launch are incomplete");
     return SLLM_ETIMEOUT;
 }

@@ -131,6 +131,25 @@ class Ops:
     def attention_talk_takes_mixed(self, heads, kv_heads, dk, dv):
         return bool(self.lib.sllm_seq_attention_talk_takes_mixed(heads, kv_heads, dk, dv, self.kv_dtype))
 
+    # ---- the 8-bit cache: e4m3 pools with a power of two as scale per 32 positions and head ----
+    def rotary_kv8(self, b, q_ptr, ldq, heads, dk, k_ptr, ldk, kv_heads, v_ptr, ldv, dv, angles, n_freq, layout, q_out, ldqo, k_pool, k_scale, v_pool, v_scale, n_pages, st):
+        """Keys turned and, with the values, appended to the 8-bit cache; the turned queries go to ``q_out`` (an address, the queries' own for in place).
+        ``angles``: the table ``angles`` makes. Pools [pages][kv_heads][page_len][width] of float8_e4m3fn, scales [pages][kv_heads][page_len / 32] of float32."""
+        self._ck(self.lib.sllm_seq_rotary_kv8(C.byref(b), q_ptr, ldq, heads, dk, k_ptr, ldk, kv_heads, v_ptr, ldv, dv, _p(angles), n_freq, layout, q_out, ldqo, _p(k_pool),
+                                              _p(k_scale), _p(v_pool), _p(v_scale), n_pages, st))
+
+    def attention8_ws_bytes(self, b, heads, kv_heads, dk, dv):
+        """Bytes of workspace ``attention8`` needs for a step like this; it starts as zeros and every call leaves its counters zero."""
+        n = self.lib.sllm_seq_attention8_ws_bytes(C.byref(b), heads, kv_heads, dk, dv)
+        if n < 0:
+            self._ck(int(n))
+        return int(n)
+
+    def attention8(self, b, q_ptr, ldq, heads, kv_heads, dk, dv, scale, k_pool, k_scale, v_pool, v_scale, n_pages, ws, st, out=None, ldo=0, out16=None, opts=None):
+        """Attention over the 8-bit cache: the result as fp32 rows (``out``) and / or dense bf16 rows (``out16``)."""
+        self._ck(self.lib.sllm_seq_attention8(C.byref(b), q_ptr, ldq, heads, kv_heads, dk, dv, scale, _p(k_pool), _p(k_scale), _p(v_pool), _p(v_scale), n_pages, _p(ws),
+                                              0 if ws is None else ws.numel() * ws.element_size(), C.byref(opts) if opts is not None else None, _p(out), ldo, _p(out16), st))
+
     @staticmethod
     def attention_options(window=0, keep_first=0, softcap=0.0, slopes=None, values_in_keys=False, logdist=None, cross_values=False, chunk=0):
         """The options structure of ``attention``; the caller keeps the ``slopes`` and ``logdist`` tensors alive."""
@@ -286,3 +305,8 @@ class Ops:
     # ---- sampling (the op of the one-sequence path: temperature <= 0 = first maximum) ----
     def sample(self, logits_ptr, n, temperature, top_k, top_p, seed, step, idx_ptr, st):
         self._ck(self.lib.sllm_sample_f32(logits_ptr, n, temperature, top_k, top_p, seed, step, idx_ptr, st))
+
+    def sample_rows(self, logits_ptr, ld, rows, n, temperature, top_k, top_p, min_p, u, idx, st, prob=None):
+        """The next token of every row, drawn from the given numbers ``u`` in [0, 1) with settings per row (device arrays, None = 1 / all / all / all);
+        ``prob``: the probability of what was drawn among what was kept."""
+        self._ck(self.lib.sllm_sample_rows(logits_ptr, ld, rows, n, _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(u), _p(idx), _p(prob), st))
