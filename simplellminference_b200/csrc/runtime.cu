@@ -62,6 +62,7 @@ int status_take() {
     SLLM_REQUIRE(what != kStatusBatch, SLLM_EINVAL, "seq_ssd_blocks: n_qtiles of an earlier launch does not count the tiles of all its tokens; its results are incomplete");
     SLLM_REQUIRE(what != kStatusPages, SLLM_EINVAL, "seq_rotary_kv8: a position of an earlier launch has no page in the block table; nothing was written there");
     SLLM_REQUIRE(what != kStatusTwice, SLLM_EINVAL, "seq_rotary_kv8: an earlier launch had two segments of one sequence; their keys and values were not written");
+    SLLM_REQUIRE(what != kStatusSingle, SLLM_EINVAL, "seq_attention8: an earlier step of as many segments as tokens had a tile of several tokens; its results are incomplete");
     set_error("a kernel gave up waiting for its copies or products: the results of an earlier launch are incomplete");
     return SLLM_ETIMEOUT;
 }

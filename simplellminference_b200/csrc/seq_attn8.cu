@@ -12,13 +12,14 @@ namespace sllm {
 constexpr int kA8Warps = 4;
 
 template <int kGroups>       // groups of 128 value columns
-__global__ void __launch_bounds__(kA8Warps * 32) seq_attention8_kernel(Attn8Args p) {
+__global__ void __launch_bounds__(kA8Warps * 32) seq_attention8_kernel(Attn8Args p, int least) {
     after_previous();
     __shared__ __align__(16) float s_q[kA8Warps][256];
     const sllm_seq_batch& b = p.b;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, g = h / (p.heads / p.kv_heads);
     const int seg = b.qt_seg[blockIdx.x], off = b.qt_off[blockIdx.x], n = min(kBQ, b.seg_len[seg] - off), slot = b.seg_slot[seg];
     const float slope = p.slopes ? p.slopes[h] : 0.0f;
+    if (n < least) return;                                     // another kernel's
     for (int i = warp; i < n; i += kA8Warps) {
         const int t = b.seg_start[seg] + off + i, pos = b.seg_pos0[seg] + off + i, wnd = seq_row_window(pos, p.window, p.chunk);
         const float* q = p.q + (size_t)t * p.ldq + (size_t)h * p.dk;
@@ -92,7 +93,7 @@ extern "C" {
 
 int64_t sllm_seq_attention8_ws_bytes(const sllm_seq_batch* b, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv) {
     SLLM_REQUIRE(b && b->T > 0 && b->nseg > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && dk > 0 && dv > 0, SLLM_EINVAL, "seq_attention8_ws_bytes: bad argument");
-    return 256;
+    return (int64_t)kA8Ws;
 }
 
 int sllm_seq_attention8(const sllm_seq_batch* b, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, float scale, const void* k_pool,
@@ -126,9 +127,17 @@ int sllm_seq_attention8(const sllm_seq_batch* b, const float* q, int32_t ldq, in
         p.slopes = opts->slopes;
     }
     if (int rc = status_check()) return rc;
+    cudaStream_t st = as_stream(stream);
+    const bool narrow = dk <= 128 && dv <= 128 && (unsigned long long)n_pages * kv_heads * b->page_len < 1ull << 31;
+    if (narrow) {
+        const bool single = b->T == b->nseg;
+        if (int rc = launch_attention8_decode(p, single, ws, st)) return rc;
+        if (single) return SLLM_OK;
+    }
     const dim3 grid(b->n_qtiles, heads);
-    if (dv <= 128) overlapping(seq_attention8_kernel<1>)<<<grid, kA8Warps * 32, 0, as_stream(stream)>>>(p);
-    else overlapping(seq_attention8_kernel<2>)<<<grid, kA8Warps * 32, 0, as_stream(stream)>>>(p);
+    const int least = narrow ? 2 : 1;
+    if (dv <= 128) overlapping(seq_attention8_kernel<1>)<<<grid, kA8Warps * 32, 0, st>>>(p, least);
+    else overlapping(seq_attention8_kernel<2>)<<<grid, kA8Warps * 32, 0, st>>>(p, least);
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;

@@ -10,6 +10,9 @@ namespace sllm {
 // tensor map of bf16 elements, boxes with 128-byte rows in the 128B swizzle, zeros outside the tensor (prefill_gemm.cu)
 int tc_encode_bf16(CUtensorMap* tm, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides_bytes, const cuuint32_t* box);
 
+// tensor map of rows of `width` bytes one behind the other, boxes of `box_rows` rows of 64 or 128 bytes in the swizzle of that span, zeros outside the tensor (prefill_gemm.cu)
+int tc_encode_bytes(CUtensorMap* tm, const void* base, uint64_t rows, int width, int box_rows, int box_width);
+
 extern int g_tune_tc_polls;   // runtime.cu: polls after which the kernels below give up a wait
 
 #ifdef __CUDACC__

@@ -253,3 +253,31 @@ def test_append_then_attention_then_draw():
     assert off(fresh, keys) < 2.0 ** -4
     p = torch.softmax(logits.double(), -1).cumsum(-1)
     assert idx.tolist() == [(p[i] <= float(u[i])).sum().item() for i in range(3)]
+
+
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 29, 2.0 ** 34, 2.0 ** 60])
+@pytest.mark.parametrize("segs", [[(700, 1), (64, 1)], [(700, 40), (64, 1)]], ids=["decode", "portions"])
+def test_scores_of_any_size(size, segs):
+    """Scores of up to 2^60: fp32 gives each to 2^-22 of itself, so that the largest wins by more than its error wherever it is 2^-20 of itself ahead; it takes all the weight."""
+    heads, kv_heads, dim = 8, 2, 128
+    step, q, k, v = _case(segs, heads, kv_heads, dim)
+    got, at = _run(step, q * size, k, v, heads).double(), 0
+    for i, (p, n) in enumerate(segs):
+        kk, vv = cache_rows(step, *k, i), cache_rows(step, *v, i)
+        for j in range(n):
+            for h in range(heads):
+                s = kk[h // 4][:p + j + 1] @ q[at + j, h * dim:(h + 1) * dim].double() * dim ** -0.5
+                best, second = s.topk(2).values.tolist()
+                if (best - second) * size > max(40.0, 2.0 ** -18 * abs(best) * size):
+                    assert off(got[at + j, h * dim:(h + 1) * dim], vv[h // 4][int(s.argmax())]) < F32_BOUND, (i, j, h)
+        at += n
+
+
+def test_a_step_that_is_not_of_single_tokens_is_reported():
+    """Two segments, two tokens, but both in one of them."""
+    from simplellminference_b200 import _lib
+    heads, kv_heads, dim = 4, 2, 64
+    step, q, k, v = _case([(100, 1), (5, 1)], heads, kv_heads, dim)
+    step.dev["seg_len"].copy_(torch.tensor([2, 0]))
+    got = _run(step, q, k, v, heads)
+    assert _lib.load().sllm_status() == _lib.EINVAL and got.isnan().all()
