@@ -19,11 +19,14 @@
 
 namespace sllm {
 
-constexpr int kD8Warps = 4, kD8Least = 8;       // warps of a CTA; units of a CTA's share at least
+constexpr int kD8Warps = 4, kD8Ctas = 3;        // warps of a CTA, CTAs of an SM
+// Beginning and ending an item takes a CTA as long as some eight units (queries to fragments, four warps' sums together): every item counts that many more, in front of its first one.
+// Without them a CTA with 34 short items took 208 us where others took 76 (64 requests of up to 8192 positions).
+constexpr int kD8Extra = 8, kD8Least = 8;       // units that an item counts more; units of a CTA's share at least
 
 template <int D>
 struct D8Tile {
-    static constexpr int kRows = kKv8Block * D, kStage = 2 * kRows, kRing = D == 128 ? 3 : 6;      // bytes of a unit's keys; of keys and values; stages of a warp
+    static constexpr int kRows = kKv8Block * D, kStage = 2 * kRows, kRing = D == 128 ? 2 : 4;      // bytes of a unit's keys; of keys and values; stages of a warp
     static constexpr int kSmem = 1024 + kD8Warps * kRing * kStage;
 };
 
@@ -31,6 +34,7 @@ struct D8Args {
     Attn8Args a;
     int only;                    // the launch is the step's only one: it has no tiles of more than one query
     int sets, per_set;           // groups of query heads that a kv head's are divided into, and how many of them one holds
+    int vec_q;                   // rows of queries can be read 16 bytes at a time
     int* counters;
     float* records;
     int32_t* status;
@@ -82,18 +86,19 @@ __device__ __forceinline__ float d8_factor(float from, float to) {        // 2^(
     return from == to ? 1.0f : tc_exp2((from - (float)d8_whole(from)) - (to - (float)d8_whole(to)));
 }
 
-// What a tile of the list has to do here: units of one head set, 0 when it holds more than one query (or none)
-__device__ __forceinline__ int d8_units(const D8Args& da, int tile) {
+// A tile of the list as this kernel sees it: its query, and how many units a head set of it has; none when it holds more than one query (or none).
+struct D8Tile1 { int t, pos, slot, units; };
+__device__ __forceinline__ D8Tile1 d8_tile(const D8Args& da, int tile) {
     const Attn8Args& p = da.a;
-    const int seg = p.b.qt_seg[tile], off = p.b.qt_off[tile], n = p.b.seg_len[seg] - off;
+    const int seg = p.b.qt_seg[tile], off = p.b.qt_off[tile], n = p.b.seg_len[seg] - off, pos = p.b.seg_pos0[seg] + off;
+    D8Tile1 r{p.b.seg_start[seg] + off, pos, p.b.seg_slot[seg], 0};
     if (n > 1 && da.only) *reinterpret_cast<volatile int32_t*>(da.status) = kStatusSingle;
-    if (n != 1) return 0;
-    const int pos = p.b.seg_pos0[seg] + off;
-    return pos < 0 ? 0 : TileList(pos, pos, seq_row_window(pos, p.window, p.chunk), p.keep_first, kKv8Block).n;
+    if (n == 1 && pos >= 0) r.units = TileList(pos, pos, seq_row_window(pos, p.window, p.chunk), p.keep_first, kKv8Block).n;
+    return r;
 }
 
 template <int D, int NT>       // column width of a head, rounded up; groups of four query heads
-__global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const D8Args da) {
+__global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const D8Args da) {
     using Tile = D8Tile<D>;
     constexpr int kRing = Tile::kRing, kChunk = D / 8, kSteps = D / 16, kMt = D / 16, kHeads = 4 * NT;   // bytes of a value row a lane reads; k-steps of a score; 16-column tiles of a result
     const Attn8Args& p = da.a;
@@ -101,13 +106,12 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
     extern __shared__ uint8_t d8_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(d8_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t bars[kD8Warps][kRing];
-    __shared__ int s_page[kD8Warps][kRing];
-    __shared__ float2 s_scale[kD8Warps][kRing];
     __shared__ long long s_sum[kD8Warps];
+    constexpr int kKnown = 128;            // tiles kept at hand
+    __shared__ D8Tile1 s_known[kKnown];
     __shared__ int s_tile, s_gave_up, s_last;
     __shared__ long long s_before;
-    __shared__ float s_ref[kD8Warps][kHeads], s_l[kD8Warps][kHeads];
-    __shared__ int s_R[kD8Warps][kHeads];
+    __shared__ float4 s_head[kD8Warps + 1][kHeads];      // of a warp and head, and of all: reference, sum, exponent
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     volatile int* gave_up = &s_gave_up;
     if (threadIdx.x == 0) {
@@ -122,7 +126,12 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
     const int per_tile = p.kv_heads * da.sets, n_tiles = b.n_qtiles;
     const int per_thread = (n_tiles + kD8Warps * 32 - 1) / (kD8Warps * 32), t0 = min(n_tiles, (int)threadIdx.x * per_thread), t1 = min(n_tiles, t0 + per_thread);
     long long mine = 0;
-    for (int i = t0; i < t1; ++i) mine += d8_units(da, i);
+    auto count = [&](int units) { return units > 0 ? units + kD8Extra : 0; };
+    for (int i = t0; i < t1; ++i) {
+        const D8Tile1 x = d8_tile(da, i);
+        if (n_tiles <= kKnown) s_known[i] = x;
+        mine += count(x.units);
+    }
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -147,7 +156,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
     if (begin >= before && begin < before + mine * per_tile) {
         long long at = before;
         for (int i = t0; i < t1; ++i) {
-            const long long n = (long long)d8_units(da, i) * per_tile;
+            const long long n = (long long)count((n_tiles <= kKnown ? s_known[i] : d8_tile(da, i)).units) * per_tile;
             if (begin < at + n) {
                 s_tile = i;
                 s_before = at;
@@ -165,54 +174,60 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
     int fresh = 1;                         // no shared memory written by ordinary stores since the last copies
     // ---- pieces: this CTA's part of one head set of one tile ----
     for (long long u = begin; u < end;) {
-        const int seg = b.qt_seg[tile], off = b.qt_off[tile], t = b.seg_start[seg] + off, pos = b.seg_pos0[seg] + off, slot = b.seg_slot[seg];
-        const int wnd = seq_row_window(pos, p.window, p.chunk);
-        const TileList blocks(pos, pos, wnd, p.keep_first, kKv8Block);
-        if (u >= tile0 + (long long)blocks.n * per_tile || b.seg_len[seg] - off != 1 || pos < 0) {       // the next tile (this one may have nothing to do here)
-            if (b.seg_len[seg] - off == 1 && pos >= 0) tile0 += (long long)blocks.n * per_tile;
+        const D8Tile1 known = n_tiles <= kKnown ? s_known[tile] : d8_tile(da, tile);
+        const int t = known.t, pos = known.pos, slot = known.slot, each = count(known.units);
+        if (u >= tile0 + (long long)each * per_tile) {               // the next tile
+            tile0 += (long long)each * per_tile;
             ++tile;
             continue;
         }
-        const int set = (int)((u - tile0) / blocks.n), gkv = set / da.sets, h0 = gkv * (p.heads / p.kv_heads) + (set % da.sets) * da.per_set;
+        const int wnd = seq_row_window(pos, p.window, p.chunk);
+        const TileList blocks(pos, pos, wnd, p.keep_first, kKv8Block);
+        const int set = (int)((u - tile0) / each), gkv = set / da.sets, h0 = gkv * (p.heads / p.kv_heads) + (set % da.sets) * da.per_set;
         const int G = min(da.per_set, (gkv + 1) * (p.heads / p.kv_heads) - h0);                       // query heads of this set
-        const long long item0 = tile0 + (long long)set * blocks.n, item1 = item0 + blocks.n;
-        const int j0 = (int)(u - item0), j1 = (int)(min(end, item1) - item0), n_mine = max(0, (j1 - j0 - warp + kD8Warps - 1) / kD8Warps);
+        const long long item0 = tile0 + (long long)set * each + kD8Extra, item1 = item0 + blocks.n;    // its units
+        const int j0 = max(0, (int)(u - item0)), j1 = (int)(min(end, item1) - item0), n_mine = max(0, (j1 - j0 - warp + kD8Warps - 1) / kD8Warps);
+        if (j1 <= 0) break;                // the share ends before the first of them
         if (!fresh) {                      // the last piece's sums were written where copies land: in front of them for everybody
             fence_async_smem();
             __syncthreads();
             fresh = 1;
         }
-        // ---- loads: unit i of this warp ----
-        int ahead_page = -1;               // lane l: page of unit 32 * x + l
-        auto issue = [&](int i) {
-            if ((i & 31) == 0) {
-                const int at = i + lane;
-                ahead_page = at < n_mine ? kv8_page(b, p.n_pages, slot, blocks.tile_of(j0 + warp + at * kD8Warps) * kKv8Block) : -1;
-            }
-            const int page = __shfl_sync(0xffffffffu, ahead_page, i & 31);
-            if (i < n_mine) {
-                const int stage = (int)((turns + i) % kRing), in_page = blocks.tile_of(j0 + warp + i * kD8Warps) * kKv8Block % b.page_len;
-                if (lane == 0) {
-                    s_page[warp][stage] = page;
-                    if (page >= 0) {
-                        const int row = (page * p.kv_heads + gkv) * b.page_len + in_page;
-                        uint8_t* dst = smem + (warp * kRing + stage) * Tile::kStage;
-                        mb_expect(&bars[warp][stage], Tile::kStage);
-                        tma_load_2d(dst, &tmK, 0, row, &bars[warp][stage]);
-                        tma_load_2d(dst + Tile::kRows, &tmV, 0, row, &bars[warp][stage]);
-                    } else {
-                        mb_arrive(&bars[warp][stage]);
-                    }
-                } else if (lane <= 2 && page >= 0) {
-                    const float* src = (lane == 1 ? p.k_scale : p.v_scale) + kv8_scale_at(page, p.kv_heads, gkv, b.page_len, in_page);
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s_addr(&s_scale[warp][stage]) + (lane - 1) * 4), "l"(src) : "memory");
+        // ---- loads: unit i of this warp; lane l knows the pool row (-1: no page) and the scales of unit 32 * x + l ----
+        int rows = -1;
+        float ks_l = 0.0f, vs_l = 0.0f, ks_before = 0.0f, vs_before = 0.0f;
+        auto look_up = [&](int i) {
+            const int at = i + lane;
+            ks_before = ks_l;
+            vs_before = vs_l;
+            rows = -1;
+            if (at < n_mine) {
+                const int key0 = blocks.tile_of(j0 + warp + at * kD8Warps) * kKv8Block, page = kv8_page(b, p.n_pages, slot, key0);
+                if (page >= 0) {
+                    rows = (page * p.kv_heads + gkv) * b.page_len + key0 % b.page_len;
+                    ks_l = p.k_scale[rows / kKv8Block];
+                    vs_l = p.v_scale[rows / kKv8Block];
+                } else {
+                    ks_l = -1.0f;
                 }
             }
-            cp_async_commit();
         };
-#pragma unroll
-        for (int i = 0; i < kRing - 1; ++i) issue(i);
-        // ---- queries: two fp16 terms of q * 2^-e, e from the head's largest ----
+        auto issue = [&](int i) {
+            const int row = __shfl_sync(0xffffffffu, rows, i & 31);
+            if (i < n_mine && lane == 0) {
+                const int stage = (int)((turns + i) % kRing);
+                if (row >= 0) {
+                    uint8_t* dst = smem + (warp * kRing + stage) * Tile::kStage;
+                    mb_expect(&bars[warp][stage], Tile::kStage);
+                    tma_load_2d(dst, &tmK, 0, row, &bars[warp][stage]);
+                    tma_load_2d(dst + Tile::kRows, &tmV, 0, row, &bars[warp][stage]);
+                } else {
+                    mb_arrive(&bars[warp][stage]);
+                }
+            }
+        };
+        look_up(0);
+        // ---- queries: asked for before the table has answered; then two fp16 terms of q * 2^-e, e from the head's largest ----
         uint32_t qb[NT][kSteps][2];
         float factor[NT];                  // what a sum of products times a key scale is multiplied by
         float slope[NT];
@@ -225,12 +240,23 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
 #pragma unroll
             for (int ks = 0; ks < kSteps; ++ks) {
                 const int col = 16 * (c + 4 * (ks / 4)) + 4 * (ks % 4);
+                const bool take = live && col < p.dk;
+                if (da.vec_q) {
+                    const float4 y = take ? *reinterpret_cast<const float4*>(q + col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    v[ks][0] = y.x; v[ks][1] = y.y; v[ks][2] = y.z; v[ks][3] = y.w;
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[ks][e] = live && col < p.dk ? q[col + e] : 0.0f;
-                    top = fmaxf(top, fabsf(v[ks][e]));
+                    for (int e = 0; e < 4; ++e) v[ks][e] = take ? q[col + e] : 0.0f;
                 }
             }
+            if (x == 0) {
+#pragma unroll
+                for (int i = 0; i < kRing - 1; ++i) issue(i);
+            }
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[ks][e]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int ex = top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127, -100) : 0;
@@ -246,8 +272,8 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
                 qb[x][ks][0] = pack_f16(w[0], w[1]);
                 qb[x][ks][1] = pack_f16(w[2], w[3]);
             }
-            // scores are head c's on this lane: its scale comes from the lanes that hold its queries
-            factor[x] = p.scale * __shfl_sync(0xffffffffu, up, 8 * c + c);
+            // scores are head c's on this lane: its scale comes from a lane that holds its queries
+            factor[x] = p.scale * __shfl_sync(0xffffffffu, up, 8 * c);
             slope[x] = p.slopes && 4 * x + c < G ? p.slopes[h0 + 4 * x + c] : 0.0f;
         }
         float ref[NT], l[NT], o[NT][kMt][2];
@@ -261,16 +287,18 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
             for (int i = 0; i < kMt; ++i) o[x][i][0] = o[x][i][1] = 0.0f;
         }
         const int fg = g ^ ((g & 1) << 2);                          // key of row g: rows of a read lie in different banks
+        const int va = 2 * c, vo = (2 * c + 1) ^ 4;      // and of k 2c, 2c + 1
         bool ok = true;
         for (int i = 0; i < n_mine; ++i) {
+            if (((i + kRing - 1) & 31) == 0) look_up(i + kRing - 1);
             issue(i + kRing - 1);                                   // (the stage of unit i - 1, which every lane has read)
             const int stage = (int)((turns + i) % kRing);
-            cp_async_wait<kRing - 1>();
             ok = tc_wait_warp(&bars[warp][stage], (uint32_t)((turns + i) / kRing) & 1, gave_up, da.polls);
             if (!ok) break;
-            __syncwarp();
-            if (s_page[warp][stage] < 0) continue;
-            const float ks_ = s_scale[warp][stage].x, vs_ = s_scale[warp][stage].y;
+            // (the batch of units that is being issued may be the one behind this unit's)
+            const bool older = ((i + kRing - 1) & ~31) != (i & ~31);
+            const float ks_ = __shfl_sync(0xffffffffu, older ? ks_before : ks_l, i & 31), vs_ = __shfl_sync(0xffffffffu, older ? vs_before : vs_l, i & 31);
+            if (ks_ < 0.0f) continue;                               // no page: its keys are hidden
             const uint32_t kb = ring + stage * Tile::kStage, vb = kb + Tile::kRows;
             const int key0 = blocks.tile_of(j0 + warp + i * kD8Warps) * kKv8Block;
             // ---- scores: two tiles of 16 keys ----
@@ -285,19 +313,20 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
                     const int r0 = 16 * mt + fg;
                     const uint4 lo = lds16(kb + d8_at<D>(r0, c + 4 * half)), hi = lds16(kb + d8_at<D>(r0 + 8, c + 4 * half));
                     const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, d[4] = {hi.x, hi.y, hi.z, hi.w};
+                    float part[NT][4];
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        float part[NT][4];
-                        const uint32_t f0[4] = {kv8_half2(a[e] & 0xffffu), kv8_half2(d[e] & 0xffffu), kv8_half2(a[e] >> 16), kv8_half2(d[e] >> 16)};
-                        const uint32_t f1[4] = {kv8_half2(a[e + 1] & 0xffffu), kv8_half2(d[e + 1] & 0xffffu), kv8_half2(a[e + 1] >> 16), kv8_half2(d[e + 1] >> 16)};
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t f[4] = {kv8_half2(a[e] & 0xffffu), kv8_half2(d[e] & 0xffffu), kv8_half2(a[e] >> 16), kv8_half2(d[e] >> 16)};
 #pragma unroll
                         for (int x = 0; x < NT; ++x) {
-                            mma_f16_zero(part[x], f0, qb[x][4 * half + e][0], qb[x][4 * half + e][1]);
-                            mma_f16(part[x], f1, qb[x][4 * half + e + 1][0], qb[x][4 * half + e + 1][1]);
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) s[x][y] += part[x][y];
+                            if (e == 0) mma_f16_zero(part[x], f, qb[x][4 * half][0], qb[x][4 * half][1]);
+                            else mma_f16(part[x], f, qb[x][4 * half + e][0], qb[x][4 * half + e][1]);
                         }
                     }
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) s[x][y] += part[x][y];
                 }
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
@@ -357,38 +386,40 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
                     pb[x][e] = movmatrix_trans(pack_f16(hi, y - hi));
                 }
             }
-            // ---- values: two runs of 16 keys ----
+            // ---- values: two runs of 16 keys, one chain ----
+            uint32_t v[8][kChunk / 4];
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                uint32_t v[4][kChunk / 4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = 2 * c + (e & 1), key = 16 * ks + 8 * (e >> 1) + (row ^ ((row & 1) << 2));
-                    if constexpr (D == 128) {
-                        const uint4 y = lds16(vb + d8_at<D>(key, g));
-                        v[e][0] = y.x; v[e][1] = y.y; v[e][2] = y.z; v[e][3] = y.w;
-                    } else {
-                        const uint2 y = lds8(vb + d8_at<D>(key, g >> 1) + 8 * (g & 1));
-                        v[e][0] = y.x; v[e][1] = y.y;
-                    }
-                    if (masked && !seq_sees(pos, key0 + key, wnd, p.keep_first)) {                   // a hidden row may hold anything
-#pragma unroll
-                        for (int k = 0; k < kChunk / 4; ++k) v[e][k] = 0u;
-                    }
+            for (int e = 0; e < 8; ++e) {
+                const int key = 8 * (e >> 1) + (e & 1 ? vo : va);
+                if constexpr (D == 128) {
+                    const uint4 y = lds16(vb + d8_at<D>(key, g));
+                    v[e][0] = y.x; v[e][1] = y.y; v[e][2] = y.z; v[e][3] = y.w;
+                } else {
+                    const uint2 y = lds8(vb + d8_at<D>(key, g >> 1) + 8 * (g & 1));
+                    v[e][0] = y.x; v[e][1] = y.y;
                 }
+                if (masked && !seq_sees(pos, key0 + key, wnd, p.keep_first)) {                       // a hidden row may hold anything
 #pragma unroll
-                for (int k = 0; k < kChunk / 4; ++k) {
+                    for (int k = 0; k < kChunk / 4; ++k) v[e][k] = 0u;
+                }
+            }
 #pragma unroll
-                    for (int odd = 0; odd < 2; ++odd) {
-                        const uint32_t sel = odd ? 0x7362u : 0x5140u, y = __byte_perm(v[0][k], v[1][k], sel), z = __byte_perm(v[2][k], v[3][k], sel);
-                        const uint32_t a[4] = {kv8_half2(y & 0xffffu), kv8_half2(y >> 16), kv8_half2(z & 0xffffu), kv8_half2(z >> 16)};
+            for (int k = 0; k < kChunk / 4; ++k) {
 #pragma unroll
-                        for (int x = 0; x < NT; ++x) {
-                            float part[4];
-                            mma_f16_zero(part, a, pb[x][2 * ks], pb[x][2 * ks + 1]);
-                            o[x][2 * k + odd][0] += part[0] + part[1];
-                            o[x][2 * k + odd][1] += part[2] + part[3];
-                        }
+                for (int odd = 0; odd < 2; ++odd) {
+                    const uint32_t sel = odd ? 0x7362u : 0x5140u;
+                    uint32_t y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = __byte_perm(v[2 * e][k], v[2 * e + 1][k], sel);
+                    const uint32_t a0[4] = {kv8_half2(y[0] & 0xffffu), kv8_half2(y[0] >> 16), kv8_half2(y[1] & 0xffffu), kv8_half2(y[1] >> 16)};
+                    const uint32_t a1[4] = {kv8_half2(y[2] & 0xffffu), kv8_half2(y[2] >> 16), kv8_half2(y[3] & 0xffffu), kv8_half2(y[3] >> 16)};
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        float part[4];
+                        mma_f16_zero(part, a0, pb[x][0], pb[x][1]);
+                        mma_f16(part, a1, pb[x][2], pb[x][3]);
+                        o[x][2 * k + odd][0] += part[0] + part[1];
+                        o[x][2 * k + odd][1] += part[2] + part[3];
                     }
                 }
             }
@@ -396,7 +427,6 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
         }
         turns += n_mine;
         // ---- the four warps' sums together ----
-        cp_async_wait<0>();
         __syncthreads();                   // every stage has been read
         if (s_gave_up) break;
         float* sums = reinterpret_cast<float*>(smem);                       // [warp][head][D]
@@ -405,85 +435,105 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) seq_attention8_decode_kernel
 #pragma unroll
             for (int s = 4; s < 32; s <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], s);
             const int h = 4 * x + c;
-            if (g == 0) {
-                s_ref[warp][h] = ref[x];
-                s_l[warp][h] = l[x];
-                s_R[warp][h] = R[x];
-            }
+            if (g == 0) s_head[warp][h] = make_float4(ref[x], l[x], __int_as_float(R[x]), 0.0f);
             float* dst = sums + (warp * kHeads + h) * D + kChunk * g;
 #pragma unroll
             for (int i = 0; i < kMt; i += 2) *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[x][i][0], o[x][i][1], o[x][i + 1][0], o[x][i + 1][1]);
         }
         fresh = 0;
         __syncthreads();
-        // reference, sum and exponent of a head over `n` parts; then a column's value from them
         const int first_cta = owner(item0), last_cta = owner(item1 - 1), parts = last_cta - first_cta + 1;
         float* record = da.records + (size_t)(2 * blockIdx.x + (begin >= item0 ? 0 : 1)) * kA8Record;
         constexpr int kTail = kA8MaxHeads * 128;                               // where a record's references, sums and exponents begin
-        auto store = [&](int h, int col, float v) {
-            if (p.out) p.out[(size_t)t * p.ldo + (size_t)(h0 + h) * p.dv + col] = v;
-            if (p.out16) p.out16[((size_t)t * p.heads + h0 + h) * p.dv + col] = f32_to_bf16_bits(v);
+        // Sums of parts with references and exponents of their own, brought to the largest of each. A column's result: sum * 2^e / (den * 2^r); a query that sees no key gives 0.
+        auto store = [&](int h, int col, float4 sum, float r, float den, int e) {
+            const float f = den == 0.0f ? 0.0f : kv8_pow2(max(-126, min(126, e - d8_whole(r)))) / den;
+            const float y[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
+            if (col >= p.dv) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (p.out) p.out[(size_t)t * p.ldo + (size_t)(h0 + h) * p.dv + col + i] = y[i];
+                if (p.out16) p.out16[((size_t)t * p.heads + h0 + h) * p.dv + col + i] = f32_to_bf16_bits(y[i]);
+            }
         };
-        auto result = [&](float sum, float den, float r, int e) {              // sum * 2^e / (den * 2^r); a query that sees no key gives 0
-            if (den == 0.0f) return 0.0f;
-            const int d = e - d8_whole(r);
-            return sum / den * kv8_pow2(max(-126, min(126, d)));
+        auto weight = [&](float4 part, float r, int e) {
+            const int d = __float_as_int(part.z) - e;
+            return d < -126 ? 0.0f : kv8_pow2(d) * d8_factor(part.x, r);
         };
-        for (int i = threadIdx.x; i < G * D; i += kD8Warps * 32) {
-            const int h = i / D, col = i % D;
-            float r = -INFINITY, den = 0.0f, sum = 0.0f;
+        auto add = [](float4& sum, float4 v, float f) {
+            sum.x = fmaf(v.x, f, sum.x); sum.y = fmaf(v.y, f, sum.y); sum.z = fmaf(v.z, f, sum.z); sum.w = fmaf(v.w, f, sum.w);
+        };
+        for (int i = threadIdx.x; i < G * (D / 4); i += kD8Warps * 32) {
+            const int h = i / (D / 4), col = i % (D / 4) * 4;
+            float r = -INFINITY, den = 0.0f;
             int e = kD8None;
 #pragma unroll
             for (int w = 0; w < kD8Warps; ++w) {
-                r = fmaxf(r, s_ref[w][h]);
-                e = max(e, s_R[w][h]);
+                r = fmaxf(r, s_head[w][h].x);
+                e = max(e, __float_as_int(s_head[w][h].z));
             }
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < kD8Warps; ++w) {
-                const int d = s_R[w][h] - e;
-                den += s_l[w][h] * (s_ref[w][h] == r ? 1.0f : tc_exp2(s_ref[w][h] - r));
-                sum += sums[(w * kHeads + h) * D + col] * (d < -126 ? 0.0f : kv8_pow2(d) * d8_factor(s_ref[w][h], r));
+                const float4 part = s_head[w][h];
+                den += part.y * (part.x == r ? 1.0f : tc_exp2(part.x - r));
+                add(sum, *reinterpret_cast<const float4*>(sums + (w * kHeads + h) * D + col), weight(part, r, e));
             }
             if (parts == 1) {
-                if (col < p.dv) store(h, col, result(sum, den, r, e));
+                store(h, col, sum, r, den, e);
             } else {
-                record[h * 128 + col] = sum;
-                if (col == 0) {
-                    record[kTail + 4 * h] = r;
-                    record[kTail + 4 * h + 1] = den;
-                    record[kTail + 4 * h + 2] = __int_as_float(e);
-                }
+                *reinterpret_cast<float4*>(record + h * 128 + col) = sum;
+                if (col == 0) *reinterpret_cast<float4*>(record + kTail + 4 * h) = make_float4(r, den, __int_as_float(e), 0.0f);
             }
         }
         if (parts > 1) {
-            __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) {
-                s_last = atomicAdd(da.counters + first_cta, 1) == parts - 1;
+            if (threadIdx.x == 0) {        // what the CTA has stored before the barrier comes before this, and what others have stored before theirs, before what follows
+                int before_me;
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before_me) : "l"(da.counters + first_cta) : "memory");
+                s_last = before_me == parts - 1;
                 if (s_last) da.counters[first_cta] = 0;
-                __threadfence();
             }
             __syncthreads();
             if (s_last) {                  // all parts are there: in the order of the units, whoever was last
+                const int later = share(first_cta) < item0;
                 const float* rest = da.records + (size_t)2 * first_cta * kA8Record;
-                auto part = [&](int i) { return rest + (size_t)(2 * i + (i == 0 && share(first_cta) < item0 ? 1 : 0)) * kA8Record; };
-                for (int i = threadIdx.x; i < G * D; i += kD8Warps * 32) {
-                    const int h = i / D, col = i % D;
-                    float r = -INFINITY, den = 0.0f, sum = 0.0f;
+                __threadfence();
+                auto part = [&](int x) { return reinterpret_cast<const float4*>(rest + (size_t)(2 * x + (x == 0 ? later : 0)) * kA8Record); };
+                float* weights = sums;     // [head][part]: at most 8 x 512 of them, the ring holds more
+                for (int h = warp; h < G; h += kD8Warps) {
+                    float r = -INFINITY, den = 0.0f;
                     int e = kD8None;
-#pragma unroll 8
-                    for (int x = 0; x < parts; ++x) {
-                        r = fmaxf(r, __ldcg(part(x) + kTail + 4 * h));
-                        e = max(e, __float_as_int(__ldcg(part(x) + kTail + 4 * h + 2)));
+                    for (int x = lane; x < parts; x += 32) {
+                        const float4 v = __ldcg(part(x) + kTail / 4 + h);
+                        r = fmaxf(r, v.x);
+                        e = max(e, __float_as_int(v.z));
                     }
-#pragma unroll 8
-                    for (int x = 0; x < parts; ++x) {
-                        const float rx = __ldcg(part(x) + kTail + 4 * h);
-                        const int d = __float_as_int(__ldcg(part(x) + kTail + 4 * h + 2)) - e;
-                        den += __ldcg(part(x) + kTail + 4 * h + 1) * (rx == r ? 1.0f : tc_exp2(rx - r));
-                        sum += __ldcg(part(x) + h * 128 + col) * (d < -126 ? 0.0f : kv8_pow2(d) * d8_factor(rx, r));
+                    r = warp_max(r);
+                    e = __reduce_max_sync(0xffffffffu, e);
+                    for (int x = lane; x < parts; x += 32) {
+                        const float4 v = __ldcg(part(x) + kTail / 4 + h);
+                        den += v.y * (v.x == r ? 1.0f : tc_exp2(v.x - r));
+                        weights[h * kA8Workers + x] = weight(v, r, e);
                     }
-                    if (col < p.dv) store(h, col, result(sum, den, r, e));
+                    den = warp_sum(den);
+                    if (lane == 0) s_head[kD8Warps][h] = make_float4(r, den, __int_as_float(e), 0.0f);
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < G * (D / 4); i += kD8Warps * 32) {
+                    const int h = i / (D / 4), col = i % (D / 4) * 4;
+                    const float4 head = s_head[kD8Warps][h];
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    int x = 0;
+                    for (; x + 8 <= parts; x += 8) {
+                        float4 v[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) v[y] = __ldcg(part(x + y) + (h * 128 + col) / 4);
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) add(sum, v[y], weights[h * kA8Workers + x + y]);
+                    }
+                    for (; x < parts; ++x) add(sum, __ldcg(part(x) + (h * 128 + col) / 4), weights[h * kA8Workers + x]);
+                    store(h, col, sum, head.x, head.y, __float_as_int(head.z));
                 }
             }
         }
@@ -501,7 +551,7 @@ static int d8_launch(D8Args& a, const CUtensorMap& tmK, const CUtensorMap& tmV, 
         SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, D8Tile<D>::kSmem));
         ready = true;
     }
-    overlapping(kernel)<<<std::min(kA8Workers, 2 * sm_count()), kD8Warps * 32, D8Tile<D>::kSmem, st>>>(tmK, tmV, a);
+    overlapping(kernel)<<<std::min(kA8Workers, kD8Ctas * sm_count()), kD8Warps * 32, D8Tile<D>::kSmem, st>>>(tmK, tmV, a);
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
@@ -515,6 +565,7 @@ int launch_attention8_decode(const Attn8Args& p, bool only, void* ws, cudaStream
     a.sets = (group + kA8MaxHeads - 1) / kA8MaxHeads;
     a.per_set = (group + a.sets - 1) / a.sets;
     a.sets = (group + a.per_set - 1) / a.per_set;
+    a.vec_q = p.ldq % 4 == 0 && ((uintptr_t)p.q % 16) == 0;
     a.counters = (int*)ws;
     a.records = (float*)(a.counters + kA8Workers);
     if (int rc = status_word(&a.status)) return rc;
