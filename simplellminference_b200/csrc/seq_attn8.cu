@@ -133,6 +133,7 @@ int sllm_seq_attention8(const sllm_seq_batch* b, const float* q, int32_t ldq, in
         const bool single = b->T == b->nseg;
         if (int rc = launch_attention8_decode(p, single, ws, st)) return rc;
         if (single) return SLLM_OK;
+        if (attention8_tc_takes(p)) return launch_attention8_tc(p, ws, st);
     }
     const dim3 grid(b->n_qtiles, heads);
     const int least = narrow ? 2 : 1;

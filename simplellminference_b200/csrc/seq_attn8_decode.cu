@@ -567,7 +567,7 @@ int launch_attention8_decode(const Attn8Args& p, bool only, void* ws, cudaStream
     a.sets = (group + a.per_set - 1) / a.per_set;
     a.vec_q = p.ldq % 4 == 0 && ((uintptr_t)p.q % 16) == 0;
     a.counters = (int*)ws;
-    a.records = (float*)(a.counters + kA8Workers);
+    a.records = (float*)((uint8_t*)ws + kA8RecordsAt);
     if (int rc = status_word(&a.status)) return rc;
     a.polls = (unsigned)g_tune_tc_polls;
     const int D = std::max(p.dk, p.dv) <= 64 ? 64 : 128;
