@@ -26,18 +26,8 @@ namespace sllm {
 constexpr int kT8Rows = 128, kT8Keys = 64, kT8Threads = 512, kT8Raw = 4;      // rows of a tile, keys of a tile, stages of the codes' ring
 constexpr int kT8Extra = 4, kT8Least = 4;       // key tiles that an item's beginning and end count for; key tiles of a CTA's share at least
 constexpr int kT8Flush = 16;
+constexpr int kT8Known = 16;                    // key tiles whose scales are kept at hand: more than the producer is ever ahead of the softmax (the rings' stages and two)
 constexpr uint32_t kT8Tmem = 512, kT8S = 0, kT8Q = 128, kT8O = 256;           // columns: S0 S1 | Q0 Q1 | O0 O1
-
-template <int HD, int kTerms>
-struct T8Shape {
-    static constexpr int kBlocks = HD / 64, kStages = kTerms == 1 ? 3 : 2;
-    static constexpr int kBlock = kT8Keys * 128, kTile = kBlocks * kBlock;    // fp16: 64 columns of all keys; all columns
-    static constexpr int kCodes = kT8Keys * HD;                              // bytes of a tile of codes
-    static constexpr int kQBlock = kT8Rows * 128, kQTile = kTerms == 2 ? kBlocks * kQBlock : 0;
-    static constexpr int kSmem = 1024 + 2 * kStages * kTile + 2 * kT8Raw * kCodes + 2 * kQTile + 512 + 8 * kT8Rows * (int)sizeof(float);
-};
-constexpr int kT8PartTile = kT8Rows * (128 + 2), kT8Part = 2 * kT8PartTile;   // floats of a part: per tile O as [HD / 4][128][4], references, sums
-static_assert(kT8Part == kA8Part, "the workspace's parts");
 
 struct T8Args {
     Attn8Args a;
@@ -106,101 +96,125 @@ __global__ void __launch_bounds__(1024) seq_attention8_plan_kernel(Attn8Args p, 
     }
     __syncthreads();
     __threadfence_block();
-    int all = 0;
+    int all = 0, kept = 0;
     for (int r0 = 0; r0 < runs; r0 += 1024) {
         const int r = r0 + threadIdx.x;
-        int units = 0;
+        int units = 0, seg = 0, first = 0;
+        uint32_t m[8];
         if (r < runs) {
             int lo = -1, hi = -1;
+#pragma unroll
             for (int w = 0; w < 8; ++w) {
-                const uint32_t m = *reinterpret_cast<volatile uint32_t*>(&plan->mask[r][w]);
-                if (!m) continue;
-                if (lo < 0) lo = 32 * w + __ffs(m) - 1;
-                hi = 32 * w + 31 - __clz(m);
+                m[w] = *reinterpret_cast<volatile uint32_t*>(&plan->mask[r][w]);
+                if (!m[w]) continue;
+                if (lo < 0) lo = 32 * w + __ffs(m[w]) - 1;
+                hi = 32 * w + 31 - __clz(m[w]);
             }
-            const int seg = plan->seg[r], pos0 = b.seg_pos0[seg] + plan->first[r];
+            seg = plan->seg[r];
+            first = plan->first[r];
+            const int pos0 = b.seg_pos0[seg] + first;
             if (lo >= 0 && pos0 >= 0) units = TileList(pos0 + lo, pos0 + hi, seq_row_window(pos0 + lo, p.window, p.chunk), p.keep_first, kT8Keys).n + kT8Extra;
         }
-        int total;
-        const int at = scan(units, total);
-        if (r < runs) plan->before[r] = all + at;
+        int total, kept_here;
+        const int at = scan(units, total), to = kept + scan(units > 0, kept_here);      // (behind its barriers every run of this round has been read)
+        if (units > 0) {                         // a run without listed tiles is left out
+            plan->before[to] = all + at;
+            plan->seg[to] = seg;
+            plan->first[to] = first;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) plan->mask[to][w] = m[w];
+        }
         all += total;
+        kept += kept_here;
+        __syncthreads();
     }
     if (threadIdx.x == 0) {
-        plan->before[runs] = all;
-        plan->runs = runs;
+        plan->before[kept] = all;
+        plan->runs = kept;
     }
 }
 
-// What a role knows of the item it is at. Every role walks its CTA's share by itself.
+// An item of a CTA's share, as all its roles see it.
 struct T8Item {
-    int x, y;                                // run, head set
     int k0, k1, n;                           // its key tiles that are this CTA's, of so many
     int tok0, pos0, slot, gkv, h0;           // first token and position of the run; kv head, first query head
     int lo, hi;                              // first and last listed query of the run
-    uint32_t m[8];
+    int keys[2];                             // how many of k0 .. k1 either tile has to see: those up to its last listed query's
+    int first_cta, parts, slot_of, later;    // the CTAs that share it; which of this CTA's two places its part takes, and the first CTA's
+    uint32_t m[8];                           // listed queries
+    __device__ __forceinline__ bool listed(int q) const { return m[q >> 5] >> (q & 31) & 1; }
 };
+constexpr int kT8Items = 48;                 // of a share, kept in shared memory; the ones behind are worked out where they are needed
 
-struct T8Walk {
+// A CTA's share of the row of all key tiles: items first_item, first_item + 1, ... of the step (run by run, head set by head set)
+struct T8Share {
     const T8Args& p;
-    long long begin, end, u;
-    int x, ctas;
-    long long total;
-    __device__ __forceinline__ T8Walk(const T8Args& args, int start_run, int n_ctas, long long all) : p(args), x(start_run), ctas(n_ctas), total(all) {
-        begin = share(blockIdx.x);
-        end = share(blockIdx.x + 1);
-        u = begin;
-    }
+    long long total, begin, end;
+    int ctas, first_item, count;
     __device__ __forceinline__ long long share(int c) const { return (long long)c * total / ctas; }
     __device__ __forceinline__ int owner(long long v) const { return (int)(((v + 1) * ctas - 1) / total); }
-    __device__ __forceinline__ bool next(T8Item& it) {
-        for (; u < end;) {
-            const int b0 = p.plan->before[x], each = p.plan->before[x + 1] - b0;
-            const long long at = (long long)b0 * p.sets;
-            if (u >= at + (long long)each * p.sets) { ++x; continue; }
-            it.x = x;
-            it.y = (int)((u - at) / each);
-            it.n = each - kT8Extra;
-            const long long item0 = at + (long long)it.y * each + kT8Extra;
-            it.k0 = (int)max(0ll, u - item0);
-            it.k1 = (int)(min(end, item0 + it.n) - item0);
-            if (it.k1 <= 0) return false;        // the share ends before the item's first tile
-            u = item0 + it.k1;
-            const sllm_seq_batch& b = p.a.b;
-            const int seg = p.plan->seg[x], first = p.plan->first[x], group = p.a.heads / p.a.kv_heads, per = group / p.hpc;
-            it.tok0 = b.seg_start[seg] + first;
-            it.pos0 = b.seg_pos0[seg] + first;
-            it.slot = b.seg_slot[seg];
-            it.gkv = it.y / per;
-            it.h0 = it.gkv * group + it.y % per * p.hpc;
-            it.lo = it.hi = -1;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                it.m[w] = p.plan->mask[x][w];
-                if (it.m[w]) {
-                    if (it.lo < 0) it.lo = 32 * w + __ffs(it.m[w]) - 1;
-                    it.hi = 32 * w + 31 - __clz(it.m[w]);
-                }
-            }
-            return true;
+    __device__ __forceinline__ T8Share(const T8Args& args, int n_ctas, long long all) : p(args), total(all), ctas(n_ctas) {
+        begin = share(blockIdx.x);
+        end = share(blockIdx.x + 1);
+    }
+    __device__ __forceinline__ int item_of(long long u) const {          // the item that unit u (beginnings counted) belongs to
+        int lo = 0, hi = p.plan->runs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if ((long long)p.plan->before[mid] * p.sets <= u) lo = mid; else hi = mid;
         }
-        return false;
+        const int b0 = p.plan->before[lo], each = p.plan->before[lo + 1] - b0;
+        return lo * p.sets + (int)((u - (long long)b0 * p.sets) / each);
     }
-    __device__ __forceinline__ TileList tiles(const T8Item& it) const {
-        return TileList(it.pos0 + it.lo, it.pos0 + it.hi, seq_row_window(it.pos0 + it.lo, p.a.window, p.a.chunk), p.a.keep_first, kT8Keys);
-    }
-    // how many of its key tiles k0 .. k1 a tile has to see: those up to its last listed query's
-    __device__ __forceinline__ int keys(const T8Item& it, int j) const {
-        int last = -1;
-        const int q0 = j * p.queries, q1 = q0 + p.queries;
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-            if (32 * w >= q0 && 32 * w < q1 && it.m[w]) last = 32 * w + 31 - __clz(it.m[w]);
-        if (last < 0) return 0;
-        const int n = it.n - ((it.pos0 + it.hi) / kT8Keys - (it.pos0 + last) / kT8Keys);
-        return max(0, min(it.k1, n) - it.k0);
+    __device__ __noinline__ void work_out(int i, T8Item& it) const {     // k1 <= 0: the share ends before its first tile
+        const int x = (first_item + i) / p.sets, y = (first_item + i) % p.sets;
+        const int b0 = p.plan->before[x], each = p.plan->before[x + 1] - b0;
+        const long long item0 = (long long)b0 * p.sets + (long long)y * each + kT8Extra;
+        it.n = each - kT8Extra;
+        it.k0 = (int)max(0ll, begin - item0);
+        it.k1 = (int)(min(end, item0 + it.n) - item0);
+        const sllm_seq_batch& b = p.a.b;
+        const int seg = p.plan->seg[x], first = p.plan->first[x], group = p.a.heads / p.a.kv_heads, per = group / p.hpc;
+        it.tok0 = b.seg_start[seg] + first;
+        it.pos0 = b.seg_pos0[seg] + first;
+        it.slot = b.seg_slot[seg];
+        it.gkv = y / per;
+        it.h0 = it.gkv * group + y % per * p.hpc;
+        it.lo = it.hi = -1;
+        int last[2] = {-1, -1};
+        for (int w = 0; w < 8; ++w) {
+            it.m[w] = p.plan->mask[x][w];
+            if (!it.m[w]) continue;
+            if (it.lo < 0) it.lo = 32 * w + __ffs(it.m[w]) - 1;
+            it.hi = 32 * w + 31 - __clz(it.m[w]);
+            last[32 * w >= p.queries] = it.hi;
+        }
+        for (int j = 0; j < 2; ++j) {
+            const int n = last[j] < 0 ? 0 : it.n - ((it.pos0 + it.hi) / kT8Keys - (it.pos0 + last[j]) / kT8Keys);
+            it.keys[j] = max(0, min(it.k1, n) - it.k0);
+        }
+        it.first_cta = owner(item0);
+        it.parts = owner(item0 + it.n - 1) - it.first_cta + 1;
+        it.slot_of = begin >= item0 ? 0 : 1;
+        it.later = share(it.first_cta) < item0;
     }
 };
+
+template <int HD, int kTerms>
+struct T8Shape {
+    static constexpr int kBlocks = HD / 64, kStages = kTerms == 1 ? 3 : 2;
+    static constexpr int kBlock = kT8Keys * 128, kTile = kBlocks * kBlock;    // fp16: 64 columns of all keys; all columns
+    static constexpr int kCodes = kT8Keys * HD;                              // bytes of a tile of codes
+    static constexpr int kQBlock = kT8Rows * 128, kQTile = kTerms == 2 ? kBlocks * kQBlock : 0;
+    static constexpr int kStaging = kTerms == 1 ? 8 * 32 * 128 : 0;           // queries on their way to TMEM: 32 rows of 32 columns a warp (with two terms the second one's place)
+    static constexpr int kItems = (kT8Items * (int)sizeof(T8Item) + 127) / 128 * 128;
+    static constexpr int kSmem = 1024 + 2 * kStages * kTile + 2 * kT8Raw * kCodes + 2 * kQTile + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems + kStaging;
+};
+constexpr int kT8PartTile = kT8Rows * (128 + 2), kT8Part = 2 * kT8PartTile;   // floats of a part: per tile O as [HD / 4][128][4], references, sums
+static_assert(kT8Part == kA8Part, "the workspace's parts");
+
+// what the producer knows of a key tile: per 32 keys the key scale, log2 of the value scale, the pool row (-1: no page)
+struct T8Tile { float ks[2], ev[2]; int row[2], pad[2]; };
 
 // pool row of 32 keys, or -1 where they have no page (or lie behind the last listed query)
 __device__ __forceinline__ int t8_row(const Attn8Args& p, int slot, int gkv, int key0, int last_pos) {
@@ -245,11 +259,14 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
     uint64_t* meet = lread + 2;              // of warps 12-15
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet + 1);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* s_start = reinterpret_cast<int*>(tmem_slot + 2);
-    int* s_last = reinterpret_cast<int*>(tmem_slot + 3);
-    volatile int* s_nan = reinterpret_cast<volatile int*>(tmem_slot + 4);        // [8]: at i % 8 the number (from 1) of an item that had NaN among its values; the converters are fewer items ahead
+    int* s_start = reinterpret_cast<int*>(tmem_slot + 2);                        // the first item and how many
+    int* s_last = reinterpret_cast<int*>(tmem_slot + 4);
+    volatile int* s_nan = reinterpret_cast<volatile int*>(tmem_slot + 5);        // [8]: at i % 8 the number (from 1) of an item that had NaN among its values; the converters are fewer items ahead
     float* factor = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);        // [2][128]
     float *s_ref = factor + 2 * kT8Rows, *s_sum = s_ref + 2 * kT8Rows;                        // [2][128] each
+    T8Tile* s_tile = reinterpret_cast<T8Tile*>(s_sum + 2 * kT8Rows);                           // [kT8Known]
+    T8Item* s_items = reinterpret_cast<T8Item*>(factor + 8 * kT8Rows);                         // [kT8Items]
+    uint8_t* s_stage = reinterpret_cast<uint8_t*>(factor + 8 * kT8Rows) + Sh::kItems;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Attn8Args& a = p.a;
 
@@ -266,41 +283,64 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
     }
     if (warp == 1) tc_alloc(tmem_slot, kT8Tmem);
     after_previous();
-    // this CTA's share: the run it begins in
-    const int runs = p.plan->runs;
-    const long long total = (long long)p.plan->before[runs] * p.sets;
+    // this CTA's share of the row of all key tiles, and its items
+    const long long total = (long long)p.plan->before[p.plan->runs] * p.sets;
     const int ctas = (int)min((long long)gridDim.x, (total + kT8Least - 1) / kT8Least);
     const bool work = (int)blockIdx.x < ctas;
-    if (work && threadIdx.x == 0) {
-        const long long first = (long long)blockIdx.x * total / ctas;
-        int lo = 0, hi = runs;                   // before[lo] * sets <= first < before[hi] * sets
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if ((long long)p.plan->before[mid] * p.sets <= first) lo = mid; else hi = mid;
-        }
-        *s_start = lo;
+    T8Share w(p, ctas, total);
+    if (work && warp >= 2 && warp < 4) {
+        w.first_item = w.item_of(w.begin);
+        const int n = w.item_of(w.end - 1) - w.first_item + 1, i = threadIdx.x - 64;
+        if (i < min(n, kT8Items)) w.work_out(i, s_items[i]);
+        if (i == 0) { s_start[0] = w.first_item; s_start[1] = n; }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    w.first_item = s_start[0];
+    w.count = s_start[1];
+    // the i-th item, or false behind the last one (whose first tile the share may end before)
+    auto item_at = [&](int i, T8Item& more) -> const T8Item* {
+        if (i >= w.count) return nullptr;
+        const T8Item* it = s_items + i;
+        if (i >= kT8Items) {
+            w.work_out(i, more);
+            it = &more;
+        }
+        return it->k1 > 0 ? it : nullptr;
+    };
+    auto tiles_of = [&](const T8Item& it) { return TileList(it.pos0 + it.lo, it.pos0 + it.hi, seq_row_window(it.pos0 + it.lo, a.window, a.chunk), a.keep_first, kT8Keys); };
 
     if (!work) {
-    } else if (warp == 0) {
-        if (elect_one()) {   // ===== TMA producer =====
-            T8Walk w(p, *s_start, ctas, total);
-            T8Item it;
-            int g = 0;                           // key tiles so far
-            bool ok = true;
-            while (ok && w.next(it)) {
-                const TileList tiles = w.tiles(it);
-                for (int k = it.k0; k < it.k1; ++k, ++g) {
-                    const int s = g % RS, key0 = tiles.tile_of(k) * kT8Keys;
-                    int row[2];
+    } else if (warp == 0) {   // ===== TMA producer: lane l knows key tile 32 * x + l of the item =====
+        T8Item more;
+        int g = 0;                               // key tiles so far
+        bool ok = true;
+        for (int n_item = 0; ok; ++n_item) {
+            const T8Item* at = item_at(n_item, more);
+            if (!at) break;
+            const T8Item& it = *at;
+            const TileList tiles = tiles_of(it);
+            T8Tile mine{};
+            for (int k = it.k0, k1 = it.k1; k < k1; ++k, ++g) {
+                if (((k - it.k0) & 31) == 0 && k + lane < it.k1) {
+                    const int key0 = tiles.tile_of(k + lane) * kT8Keys;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) row[x] = t8_row(a, it.slot, it.gkv, key0 + x * kKv8Block, it.pos0 + it.hi);
-                    ok = tc_wait(rempty + s, ((uint32_t)(g / RS) & 1) ^ 1, gave_up, p.polls);
-                    if (!ok) break;
+                    for (int x = 0; x < 2; ++x) {
+                        const int row = t8_row(a, it.slot, it.gkv, key0 + x * kKv8Block, it.pos0 + it.hi);
+                        mine.row[x] = row;
+                        mine.ks[x] = row >= 0 ? a.k_scale[row / kKv8Block] : 1.0f;
+                        mine.ev[x] = row >= 0 ? t8_log2(a.v_scale[row / kKv8Block]) : 0.0f;
+                    }
+                }
+                const int s = g % RS, from = (k - it.k0) & 31;
+                const int row[2] = {__shfl_sync(0xffffffffu, mine.row[0], from), __shfl_sync(0xffffffffu, mine.row[1], from)};
+                ok = tc_wait_warp(rempty + s, ((uint32_t)(g / RS) & 1) ^ 1, gave_up, p.polls);
+                if (!ok) break;
+                if (lane == from) s_tile[g % kT8Known] = mine;
+                __syncwarp();
+                if (lane == 0) {
                     const int boxes = (row[0] >= 0) + (row[1] >= 0);
                     if (boxes) mb_expect(rfull + s, (uint32_t)(boxes * 2 * kKv8Block * HD));
                     else mb_arrive(rfull + s);
@@ -336,13 +376,14 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     tc_mma_bf16_ts(tmem + kT8O + 128 * j, tmem + kT8S + 64 * j + 8 * ks, v + (uint32_t)((ks % (kT8Keys / 16)) * 128), idesc_o, more || ks != 0);
                 tc_commit(odone + j);
             };
-            T8Walk w(p, *s_start, ctas, total);
-            T8Item it;
+            T8Item more;
             int g = 0;                           // key tiles so far; products and items of either tile
             uint32_t done[2] = {0, 0}, items[2] = {0, 0};
             bool ok = true;
-            while (ok && w.next(it)) {
-                const int n = it.k1 - it.k0, nkt[2] = {w.keys(it, 0), w.keys(it, 1)};
+            for (int i = 0; ok; ++i) {
+                const T8Item* at = item_at(i, more);
+                if (!at) break;
+                const int n = at->k1 - at->k0, nkt[2] = {at->keys[0], at->keys[1]};
                 ok = tc_wait(kfull + g % ST, (uint32_t)(g / ST) & 1, gave_up, p.polls);
                 if (!ok) break;
                 tc_fence_after();
@@ -390,79 +431,79 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             }
         }
     } else if (warp < 4) {   // ===== codes to fp16 =====
-        T8Walk w(p, *s_start, ctas, total);
-        T8Item it;
-        int g = 0, item = 0;
+        T8Item more;
+        int g = 0;
         bool ok = true;
         const int me = (warp - 2) * 32 + lane, r8 = me & 7, c0 = me >> 3;       // row of eight, first chunk: neighbouring lanes' chunks lie in different banks, read and written
         constexpr int kChunks = HD / 16, kPer = 8 / kChunks;                    // chunks of a row; rows of eight that 64 threads take at a time: 1 or 2
-        while (ok && w.next(it)) {
-            ++item;
-            const TileList tiles = w.tiles(it);
-            const int last_pos = it.pos0 + it.hi;
-            bool bad = false;
-            for (int k = it.k0; k < it.k1; ++k, ++g) {
+        for (int n_item = 0; ok; ++n_item) {
+            const T8Item* at = item_at(n_item, more);
+            if (!at) break;
+            const TileList tiles = tiles_of(*at);
+            const int last_pos = at->pos0 + at->hi;
+            for (int k = at->k0, k1 = at->k1; k < k1; ++k, ++g) {
                 const int s = g % RS, t = g % ST, key0 = tiles.tile_of(k) * kT8Keys;
                 const uint32_t par = (uint32_t)(g / ST) & 1;
                 ok = tc_wait_warp(rfull + s, (uint32_t)(g / RS) & 1, gave_up, p.polls) && tc_wait_warp(kempty + t, par ^ 1, gave_up, p.polls);
                 if (!ok) break;
-                auto convert = [&](const uint8_t* raw, uint8_t* tile, auto values_) {
-                    constexpr bool values = decltype(values_)::value;
+                // kWild: rows that the run must not see become zeros, and NaN codes, which are reported
+                auto convert = [&](const uint8_t* raw, uint8_t* tile, auto values_, auto wild_) {
+                    constexpr bool values = decltype(values_)::value, wild = decltype(wild_)::value;
                     const uint32_t from = s_addr(raw), to = s_addr(tile);
-                    bool there[2];                 // (keys without a page are hidden by the softmax, whatever they are)
-                    if (values) {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) there[x] = t8_row(a, it.slot, it.gkv, key0 + x * kKv8Block, last_pos) >= 0;
-                    }
+                    uint32_t any = 0;
 #pragma unroll
                     for (int r0 = 0; r0 < kT8Keys; r0 += 8 * kPer) {
                         const int row = r0 + r8 + 8 * (c0 / kChunks), chunk = c0 % kChunks;
                         uint4 v = t8_lds(from + row * HD + ((HD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
                         if (values) {
-                            const bool take = there[r0 + 8 * (c0 / kChunks) >= kKv8Block] && key0 + row <= last_pos;
-                            uint32_t* y = &v.x;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                y[e] = take ? y[e] : 0u;
-                                const uint32_t n = ((y[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;       // the top bit of every NaN
-                                if (n) {
-                                    bad = true;
-                                    y[e] &= ~((n >> 7) * 0xffu);
-                                }
-                            }
+                            const bool take = !wild || (key0 + row <= last_pos && s_tile[g % kT8Known].row[row >= kKv8Block] >= 0);
+                            auto look = [&](uint32_t y) {
+                                if (wild && !take) y = 0u;
+                                const uint32_t n = (y & 0x7f7f7f7fu) + 0x01010101u;                  // the top bit of every NaN
+                                any |= n;
+                                return wild ? y & ~(((n & 0x80808080u) >> 7) * 0xffu) : y;
+                            };
+                            v.x = look(v.x); v.y = look(v.y); v.z = look(v.z); v.w = look(v.w);
                         }
                         const uint32_t at = to + (chunk / 4) * Sh::kBlock + row * 128, c = (chunk % 4) * 2;
                         t8_sts(at + ((c ^ (row & 7)) << 4), kv8_half2(v.x & 0xffffu), kv8_half2(v.x >> 16), kv8_half2(v.y & 0xffffu), kv8_half2(v.y >> 16));
                         t8_sts(at + (((c + 1) ^ (row & 7)) << 4), kv8_half2(v.z & 0xffffu), kv8_half2(v.z >> 16), kv8_half2(v.w & 0xffffu), kv8_half2(v.w >> 16));
                     }
+                    return __any_sync(0xffffffffu, any & 0x80808080u);
+                };
+                auto publish = [&]() {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 };
-                convert(sRaw + 2 * s * Sh::kCodes, sK + t * Sh::kTile, std::false_type{});
+                convert(sRaw + 2 * s * Sh::kCodes, sK + t * Sh::kTile, std::false_type{}, std::false_type{});
+                publish();
                 if (lane == 0) mb_arrive(kfull + t);
                 ok = tc_wait_warp(vempty + t, par ^ 1, gave_up, p.polls);
                 if (!ok) break;
-                convert(sRaw + (2 * s + 1) * Sh::kCodes, sV + t * Sh::kTile, std::true_type{});
-                if (bad) s_nan[item & 7] = item;   // read behind the product with these values
-                __threadfence_block();
-                __syncwarp();
+                const uint8_t* codes = sRaw + (2 * s + 1) * Sh::kCodes;
+                bool whole = key0 + kT8Keys - 1 <= last_pos && s_tile[g % kT8Known].row[0] >= 0 && s_tile[g % kT8Known].row[1] >= 0;
+                if (whole) whole = !convert(codes, sV + t * Sh::kTile, std::true_type{}, std::false_type{});
+                if (!whole && convert(codes, sV + t * Sh::kTile, std::true_type{}, std::true_type{})) {
+                    s_nan[n_item & 7] = n_item + 1;          // read behind the product with these values
+                    __threadfence_block();
+                }
+                publish();
                 if (lane == 0) { mb_arrive(vfull + t); mb_arrive(rempty + s); }
             }
         }
     } else if (warp >= 12) {   // ===== O of both tiles =====
         const int quad = warp & 3, row = quad * 32 + lane;
-        T8Walk w(p, *s_start, ctas, total);
-        T8Item it;
+        T8Item more;
         uint32_t done[2] = {0, 0}, items[2] = {0, 0};
-        int item = 0;
         uint32_t met = 0;
         bool ok = true;
-        while (ok && w.next(it)) {
-            ++item;
-            const int n = it.k1 - it.k0, nkt[2] = {w.keys(it, 0), w.keys(it, 1)};
-            const bool whole = it.k0 == 0 && it.k1 == it.n;
-            const long long item0 = w.u - it.k1;                               // its first key tile in the row of all
-            float* part = p.parts + (size_t)(2 * blockIdx.x + (w.begin >= item0 ? 0 : 1)) * kT8Part;
+        for (int n_item = 0; ok; ++n_item) {
+            const T8Item* at = item_at(n_item, more);
+            if (!at) break;
+            const T8Item& it = *at;
+            const int n = it.k1 - it.k0, nkt[2] = {it.keys[0], it.keys[1]};
+            const bool whole = it.parts == 1;
+            float* part = p.parts + (size_t)(2 * blockIdx.x + it.slot_of) * kT8Part;
             float since[2] = {1.0f, 1.0f};                                     // what the references have grown by since O was flushed
             for (int kt = 0; ok && kt < n; ++kt)
 #pragma unroll
@@ -513,13 +554,10 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 }
             if (!ok) break;
             // ---- results, or this CTA's part of them ----
-            const bool nan_here = s_nan[item & 7] == item;
+            const bool nan_here = s_nan[n_item & 7] == n_item + 1;
             auto query = [&](int j, int& q) {                                  // this row's query, and whether it is listed
                 q = j * p.queries + (row >> p.hpc_log2);
-                uint32_t m = 0;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) m = q / 32 == x ? it.m[x] : m;
-                return (m >> (q & 31) & 1) != 0;
+                return it.listed(q);
             };
             // columns c .. c + 31 of this row: o * inv; `hit`: columns that a NaN value reaches
             auto store = [&](int j, int c, const float (&o)[32], float inv, const uint32_t (&hit)[4]) {
@@ -639,7 +677,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             if (!ok) break;
             tc_fence_before();
             if (!whole) {
-                const int c_first = w.owner(item0), parts = w.owner(item0 + it.n - 1) - c_first + 1;
+                const int c_first = it.first_cta, parts = it.parts;
                 auto together = [&]() {              // these four warps; a wait like the others, which ends
                     mb_arrive(meet);
                     ok = tc_wait_warp(meet, met++ & 1, gave_up, p.polls);
@@ -655,7 +693,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 if (!together()) break;
                 if (*s_last) {                       // all parts are there: in the order of the key tiles, whoever was last
                     __threadfence();
-                    const int later = w.share(c_first) < item0;
+                    const int later = it.later;
                     auto from = [&](int x, int j) { return p.parts + (size_t)(2 * (c_first + x) + (x == 0 ? later : 0)) * kT8Part + j * kT8PartTile; };
 #pragma unroll 1
                     for (int j = 0; j < 2; ++j) {
@@ -698,70 +736,96 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
         const int j = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_tmem = tmem + lanes + kT8S + 64 * j, q_tmem = tmem + lanes + kT8Q + 64 * j;
         const int q = j * p.queries + (row >> p.hpc_log2);
-        T8Walk w(p, *s_start, ctas, total);
-        T8Item it;
+        T8Item more;
         uint32_t done = 0, items = 0;
+        int g0 = 0, g1 = 0;                      // key tiles of the CTA in front of this item, and of the next
         bool ok = true;
-        while (ok && w.next(it)) {
-            const int n = w.keys(it, j);
+        for (int n_item = 0; ok; ++n_item) {
+            const T8Item* at = item_at(n_item, more);
+            if (!at) break;
+            const T8Item& it = *at;
+            const int n = it.keys[j];
+            g0 = g1;
+            g1 += it.k1 - it.k0;
             if (n == 0) continue;
-            uint32_t m = 0;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) m = q / 32 == x ? it.m[x] : m;
-            const bool live = m >> (q & 31) & 1;
-            const int qpos = it.pos0 + (live ? q : it.hi), h = it.h0 + (row & (p.hpc - 1)), last_pos = it.pos0 + it.hi;
-            const TileList tiles = w.tiles(it);
+            const bool live = it.listed(q);
+            const int qpos = it.pos0 + (live ? q : it.hi), h = it.h0 + (row & (p.hpc - 1));
+            const TileList tiles = tiles_of(it);
             // ---- queries: fp16 in TMEM, brought to 1 .. 2 by a power of two of the row's largest; every score of the item before has been read ----
             float up;
             {
-                const float* src = a.q + (size_t)(it.tok0 + (live ? q : it.hi)) * a.ldq + (size_t)h * a.dk;
-                float top = 0.0f;
-                auto load = [&](int c, float (&x)[32]) {
+                // A row is read by neighbouring lanes: once for its largest, once more for its terms, which go through shared memory to the row's own lane.
+                const long long mine = (long long)(it.tok0 + (live ? q : it.hi)) * a.ldq + (long long)h * a.dk;       // (a row without a query reads another)
+                auto row_at = [&](int r, int col) {                        // 16 bytes of row r of this warp's
+                    const float* src = a.q + __shfl_sync(0xffffffffu, mine, r) + col;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (col < a.dk) {
+                        if (p.vec_q) v = *reinterpret_cast<const float4*>(src);
+                        else v = make_float4(src[0], src[1], src[2], src[3]);
+                    }
+                    return v;
+                };
+                constexpr int kLanes = HD / 4, kPer = 32 / kLanes;         // lanes of a row, rows of a load
+                uint32_t top = 0;
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += 16) {
+                    float4 v[16 / kPer];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const bool take = c + i < a.dk;
-                        if (p.vec_q) {
-                            const float4 v = take ? *reinterpret_cast<const float4*>(src + c + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+                    for (int i = 0; i < 16 / kPer; ++i) v[i] = row_at(r0 + i * kPer + lane / kLanes, (lane % kLanes) * 4);
+#pragma unroll
+                    for (int i = 0; i < 16 / kPer; ++i) {
+                        uint32_t t = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu), max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
+                        if constexpr (kPer == 1) {
+                            t = __reduce_max_sync(0xffffffffu, t);
+                            if (lane == r0 + i) top = t;
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[i + e] = take ? src[c + i + e] : 0.0f;
+                            for (int o = 1; o < 16; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+                            const uint32_t first = __shfl_sync(0xffffffffu, t, 0), second = __shfl_sync(0xffffffffu, t, 16);
+                            if (lane == r0 + 2 * i) top = first;
+                            if (lane == r0 + 2 * i + 1) top = second;
                         }
                     }
-                };
-#pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                    float x[32];
-                    load(c, x);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(x[i]));
                 }
-                const int ex = top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127, -100) : 0;
+                const int ex = top < 0x7f800000u ? max((int)(top >> 23) - 127, -100) : 0;
                 const float down = kv8_pow2(-ex);
                 up = kv8_pow2(ex);
                 if (items) tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                    float x[32];
-                    uint32_t hi[16];
-                    load(c, x);
+                for (int pair = 0; pair < HD / 64; ++pair) {
+                    const uint32_t place = s_addr(kTerms == 1 ? s_stage + (warp - 4) * 4096 : sQ + j * Sh::kQTile + pair * Sh::kQBlock + quad * 4096);      // 32 rows of 128 bytes, chunk i of row r at i ^ (r % 8)
+                    uint32_t lo[kTerms == 2 ? 32 : 1];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        x[2 * i] *= down;
-                        x[2 * i + 1] *= down;
-                        hi[i] = t8_pack(x[2 * i], x[2 * i + 1]);
-                    }
-                    tc_st16(q_tmem + c / 2, hi);
-                    if constexpr (kTerms == 2) {
-                        uint32_t lo[16];
+                    for (int half = 0; half < 2; ++half) {
+                        float4 v[8];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 y = t8_unpack(hi[i]);
-                            lo[i] = t8_pack(x[2 * i] - y.x, x[2 * i + 1] - y.y);
+                        for (int i = 0; i < 8; ++i) v[i] = row_at(4 * i + lane / 8, 64 * pair + 32 * half + (lane % 8) * 4);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = 4 * i + lane / 8;
+                            t8_sts(place + r * 128 + (((lane % 8) ^ (r & 7)) << 4), __float_as_uint(v[i].x), __float_as_uint(v[i].y), __float_as_uint(v[i].z), __float_as_uint(v[i].w));
                         }
-                        const uint32_t at = s_addr(sQ) + j * Sh::kQTile + (c / 64) * Sh::kQBlock + row * 128;
+                        __syncwarp();
+                        uint32_t hi[16];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) t8_sts(at + (((c % 64 / 8 + i) ^ (row & 7)) << 4), lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 y = t8_lds(place + lane * 128 + ((i ^ (lane & 7)) << 4));
+                            const float x[4] = {__uint_as_float(y.x) * down, __uint_as_float(y.y) * down, __uint_as_float(y.z) * down, __uint_as_float(y.w) * down};
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                hi[2 * i + e] = t8_pack(x[2 * e], x[2 * e + 1]);
+                                if constexpr (kTerms == 2) {
+                                    const float2 z = t8_unpack(hi[2 * i + e]);
+                                    lo[16 * half + 2 * i + e] = t8_pack(x[2 * e] - z.x, x[2 * e + 1] - z.y);
+                                }
+                            }
+                        }
+                        tc_st16(q_tmem + 32 * pair + 16 * half, hi);
+                        __syncwarp();
+                    }
+                    if constexpr (kTerms == 2) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) t8_sts(place + lane * 128 + ((i ^ (lane & 7)) << 4), lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
                     }
                 }
                 tc_wait_st();
@@ -772,24 +836,8 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             const int wnd = seq_row_window(qpos, a.window, a.chunk);
             const float slope = kOpts && a.slopes ? a.slopes[h] : 0.0f, mul = a.scale * up * (kOpts ? 1.0f : 1.4426950408889634f);
             float ref = -INFINITY, l = 0.0f;
-            // scales of the next tile's blocks, asked for a tile ahead
-            int rows[2];
-            float ks[2], vs[2];
-            auto look_up = [&](int k) {
-                const int key0 = tiles.tile_of(k) * kT8Keys;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    rows[x] = t8_row(a, it.slot, it.gkv, key0 + x * kKv8Block, last_pos);
-                    ks[x] = rows[x] >= 0 ? a.k_scale[rows[x] / kKv8Block] : 1.0f;
-                    vs[x] = rows[x] >= 0 ? a.v_scale[rows[x] / kKv8Block] : 1.0f;
-                }
-            };
-            look_up(it.k0);
             for (int kt = 0; kt < n; ++kt) {
                 const int key0 = tiles.tile_of(it.k0 + kt) * kT8Keys;
-                const bool gone[2] = {rows[0] < 0, rows[1] < 0};
-                const float f0[2] = {ks[0] * mul, ks[1] * mul}, v0[2] = {vs[0], vs[1]};
-                if (kt + 1 < n) look_up(it.k0 + kt + 1);
                 ok = tc_wait_warp(sfull + j, done & 1, gave_up, p.polls);
                 if (!ok) break;
                 ++done;
@@ -797,17 +845,19 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 uint32_t s[64];
                 tc_ld32_async(s_tmem, s);
                 tc_ld32_async(s_tmem + 32, s + 32);
-                float ev[2] = {t8_log2(v0[0]), t8_log2(v0[1])};
+                const T8Tile known = s_tile[(g0 + kt) % kT8Known];
+                const bool gone[2] = {known.row[0] < 0, known.row[1] < 0};
+                const float ev[2] = {known.ev[0], known.ev[1]};
                 // every key of the tile is visible to every row of the warp
                 const bool all = __all_sync(0xffffffffu, !gone[0] && !gone[1] && key0 + kT8Keys - 1 <= qpos && (qpos - key0 < wnd || key0 + kT8Keys <= a.keep_first));
                 tc_arrived(s);
                 tc_arrived(s + 32);
-                float f[2] = {f0[0], f0[1]};
+                float f[2] = {known.ks[0] * mul, known.ks[1] * mul};
                 if (kOpts) {
                     const float dist = (float)(qpos - key0), inv = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 #pragma unroll
                     for (int e = 0; e < 64; ++e) {
-                        float v = __uint_as_float(s[e]) * f0[e / 32];
+                        float v = __uint_as_float(s[e]) * f[e / 32];
                         if (a.softcap > 0.0f) v = a.softcap * tanhf(v * inv);
                         v = fmaf(-slope, dist - (float)e, v);
                         s[e] = __float_as_uint(v);
