@@ -48,6 +48,9 @@ __global__ void __launch_bounds__(1024) seq_attention8_plan_kernel(Attn8Args p, 
     const sllm_seq_batch& b = p.b;
     __shared__ int s_base[kA8Segs + 1];
     __shared__ int s_warp[32];
+    constexpr int kFew = 640;
+    __shared__ uint32_t s_mask[kFew * 8];
+    __shared__ int s_seg[kFew], s_first[kFew];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto scan = [&](int v, int& total) {         // exclusive sum over the CTA
         int upto = v;
@@ -76,13 +79,16 @@ __global__ void __launch_bounds__(1024) seq_attention8_plan_kernel(Attn8Args p, 
         runs += total;
     }
     runs = min(runs, kA8Runs);                   // (the host has made sure)
-    for (int i = threadIdx.x; i < runs * 8; i += 1024) plan->mask[i / 8][i % 8] = 0;
+    const bool few = runs <= kFew;               // their masks fit shared memory
+    for (int i = threadIdx.x; i < runs * 8; i += 1024) {
+        if (few) s_mask[i] = 0; else plan->mask[i / 8][i % 8] = 0;
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < b.nseg; i += 1024) {
         const int len = b.seg_len[i], n = len > 1 ? (len + width - 1) / width : 0;
         for (int r = 0; r < n && s_base[i] + r < runs; ++r) {
-            plan->seg[s_base[i] + r] = i;
-            plan->first[s_base[i] + r] = r * width;
+            const int at = s_base[i] + r;
+            if (few) { s_seg[at] = i; s_first[at] = r * width; } else { plan->seg[at] = i; plan->first[at] = r * width; }
         }
     }
     for (int i = threadIdx.x; i < b.n_qtiles; i += 1024) {
@@ -90,7 +96,7 @@ __global__ void __launch_bounds__(1024) seq_attention8_plan_kernel(Attn8Args p, 
         if (n <= 1 || off < 0) continue;
         for (int q = off; q < off + n;) {        // a word of a run's mask at a time
             const int run = s_base[seg] + q / width, bit = q % width, count = min(off + n - q, 32 - bit % 32);
-            if (run < runs) atomicOr(&plan->mask[run][bit / 32], (count == 32 ? 0xffffffffu : (1u << count) - 1) << (bit % 32));
+            if (run < runs) atomicOr(few ? &s_mask[run * 8 + bit / 32] : &plan->mask[run][bit / 32], (count == 32 ? 0xffffffffu : (1u << count) - 1) << (bit % 32));
             q += count;
         }
     }
@@ -105,13 +111,13 @@ __global__ void __launch_bounds__(1024) seq_attention8_plan_kernel(Attn8Args p, 
             int lo = -1, hi = -1;
 #pragma unroll
             for (int w = 0; w < 8; ++w) {
-                m[w] = *reinterpret_cast<volatile uint32_t*>(&plan->mask[r][w]);
+                m[w] = few ? s_mask[r * 8 + w] : *reinterpret_cast<volatile uint32_t*>(&plan->mask[r][w]);
                 if (!m[w]) continue;
                 if (lo < 0) lo = 32 * w + __ffs(m[w]) - 1;
                 hi = 32 * w + 31 - __clz(m[w]);
             }
-            seg = plan->seg[r];
-            first = plan->first[r];
+            seg = few ? s_seg[r] : plan->seg[r];
+            first = few ? s_first[r] : plan->first[r];
             const int pos0 = b.seg_pos0[seg] + first;
             if (lo >= 0 && pos0 >= 0) units = TileList(pos0 + lo, pos0 + hi, seq_row_window(pos0 + lo, p.window, p.chunk), p.keep_first, kT8Keys).n + kT8Extra;
         }
@@ -756,22 +762,27 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             {
                 // A row is read by neighbouring lanes: once for its largest, once more for its terms, which go through shared memory to the row's own lane.
                 const long long mine = (long long)(it.tok0 + (live ? q : it.hi)) * a.ldq + (long long)h * a.dk;       // (a row without a query reads another)
-                auto row_at = [&](int r, int col) {                        // 16 bytes of row r of this warp's
-                    const float* src = a.q + __shfl_sync(0xffffffffu, mine, r) + col;
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (col < a.dk) {
-                        if (p.vec_q) v = *reinterpret_cast<const float4*>(src);
-                        else v = make_float4(src[0], src[1], src[2], src[3]);
+                auto rows_at = [&](auto& v, auto r_of, int col) {          // 16 bytes of a row of this warp's, for each of v
+                    if (p.vec_q) {
+#pragma unroll
+                        for (int i = 0; i < (int)(sizeof(v) / 16); ++i) {
+                            const float* src = a.q + __shfl_sync(0xffffffffu, mine, r_of(i)) + col;
+                            v[i] = col < a.dk ? *reinterpret_cast<const float4*>(src) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < (int)(sizeof(v) / 16); ++i) {
+                            const float* src = a.q + __shfl_sync(0xffffffffu, mine, r_of(i)) + col;
+                            v[i] = col < a.dk ? make_float4(src[0], src[1], src[2], src[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        }
                     }
-                    return v;
                 };
                 constexpr int kLanes = HD / 4, kPer = 32 / kLanes;         // lanes of a row, rows of a load
                 uint32_t top = 0;
 #pragma unroll 1
                 for (int r0 = 0; r0 < 32; r0 += 16) {
                     float4 v[16 / kPer];
-#pragma unroll
-                    for (int i = 0; i < 16 / kPer; ++i) v[i] = row_at(r0 + i * kPer + lane / kLanes, (lane % kLanes) * 4);
+                    rows_at(v, [&](int i) { return r0 + i * kPer + lane / kLanes; }, (lane % kLanes) * 4);
 #pragma unroll
                     for (int i = 0; i < 16 / kPer; ++i) {
                         uint32_t t = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu), max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
@@ -798,8 +809,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float4 v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = row_at(4 * i + lane / 8, 64 * pair + 32 * half + (lane % 8) * 4);
+                        rows_at(v, [&](int i) { return 4 * i + lane / 8; }, 64 * pair + 32 * half + (lane % 8) * 4);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int r = 4 * i + lane / 8;
@@ -834,7 +844,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 mb_arrive(qready + j);
             }
             const int wnd = seq_row_window(qpos, a.window, a.chunk);
-            const float slope = kOpts && a.slopes ? a.slopes[h] : 0.0f, mul = a.scale * up * (kOpts ? 1.0f : 1.4426950408889634f);
+            const float slope = kOpts && a.slopes ? a.slopes[h] : 0.0f, mul = a.scale * up * (kOpts ? 1.0f : kTcLog2e);
             float ref = -INFINITY, l = 0.0f;
             for (int kt = 0; kt < n; ++kt) {
                 const int key0 = tiles.tile_of(it.k0 + kt) * kT8Keys;
@@ -854,24 +864,54 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 tc_arrived(s + 32);
                 float f[2] = {known.ks[0] * mul, known.ks[1] * mul};
                 if (kOpts) {
-                    const float dist = (float)(qpos - key0), inv = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+                    if (a.softcap > 0.0f) {
+                        const float inv[2] = {f[0] / a.softcap, f[1] / a.softcap};
+                        float most = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) {
-                        float v = __uint_as_float(s[e]) * f[e / 32];
-                        if (a.softcap > 0.0f) v = a.softcap * tanhf(v * inv);
-                        v = fmaf(-slope, dist - (float)e, v);
-                        s[e] = __float_as_uint(v);
+                        for (int e = 0; e < 64; e += 2) {
+                            const float x = __uint_as_float(s[e]) * inv[e / 32], y = __uint_as_float(s[e + 1]) * inv[e / 32];
+                            s[e] = __float_as_uint(x);
+                            s[e + 1] = __float_as_uint(y);
+                            most = tc_max3(most, fabsf(x), fabsf(y));
+                        }
+                        // scores within a quarter of the cap, as nearly all are: the series that tc_tanh takes for them, two at a time
+                        if (__any_sync(0xffffffffu, most >= 0.25f)) {
+#pragma unroll
+                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(a.softcap * tc_tanh(__uint_as_float(s[e])));
+                        } else {
+                            auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
+                            const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), one = both(1.0f), cap2 = both(a.softcap);
+#pragma unroll
+                            for (int e = 0; e < 64; e += 2) {
+                                const uint64_t x = tc_two(s[e], s[e + 1]), x2 = tc_mul2(x, x);
+                                float y, z;
+                                tc_split(tc_mul2(cap2, tc_mul2(x, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, c4, c3), c2), c1), one))), y, z);
+                                s[e] = __float_as_uint(y);
+                                s[e + 1] = __float_as_uint(z);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f[e / 32]);
                     }
-                    f[0] = f[1] = 1.4426950408889634f;
+                    if (a.slopes) {
+                        const float dist = (float)(qpos - key0);
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(fmaf(-slope, dist - (float)e, __uint_as_float(s[e])));
+                    }
+                    f[0] = f[1] = kTcLog2e;
                 }
-                auto step = [&](auto masked) {
-                    constexpr bool kMasked = decltype(masked)::value;
-                    if (kMasked) {
-                        const int hi = qpos - key0, lo = wnd > qpos ? INT_MIN : qpos - wnd - key0, keep = a.keep_first - key0;
+                if (!all) {        // the columns this row sees, as bits
+                    const int hi = qpos - key0, lo = wnd > qpos ? -1 : qpos - wnd - key0, keep = a.keep_first - key0;
+                    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };       // bits 0 .. n - 1
 #pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            if (e > hi || (e <= lo && e >= keep) || gone[e / 32]) s[e] = 0xff800000u;       // -inf
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t seen = gone[x] ? 0u : below(hi + 1 - 32 * x) & (~below(lo + 1 - 32 * x) | below(keep - 32 * x));
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[32 * x + e] = seen & (1u << e) ? s[32 * x + e] : 0xff800000u;        // -inf
                     }
+                }
+                {
                     float top[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -935,9 +975,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         tc_split(sum, s0, s1);
                         l = fmaf(s0 + s1, tc_exp2(-ev[x] - far), l);         // without the value scale
                     }
-                };
-                if (all) step(std::false_type{});
-                else step(std::true_type{});
+                }
                 tc_wait_st();
                 tc_fence_before();
                 mb_arrive(pready + j);
@@ -969,7 +1007,8 @@ static int t8_launch(const T8Args& a, const CUtensorMap& tmK, const CUtensorMap&
         SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
         ready = true;
     }
-    overlapping(kernel)<<<std::min(kA8TcWorkers, sm_count()), kT8Threads, Sh::kSmem, st>>>(tmK, tmV, a);
+    LaunchCfg lc(dim3(std::min(kA8TcWorkers, sm_count())), dim3(kT8Threads), Sh::kSmem, st, true);        // its beginning while the plan is made
+    SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(kernel), tmK, tmV, a));
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;

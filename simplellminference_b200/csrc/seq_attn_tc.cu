@@ -26,17 +26,7 @@ namespace sllm {
 constexpr int kSaRows = 128, kSaKeys = 64, kSaThreads = 256, kSaBox = 32;
 constexpr int kSaFlush = 12;             // tiles between two flushes of O: from there on three terms' products would be further off than that body's two
 constexpr uint32_t kSaTmem = 256;        // scores at 0 .. 63, then the weights' terms at 0 .. 95, O at 128; two CTAs share an SM's 512 columns
-constexpr float kSaLog2e = 1.4426950408889634f;
 
-// tanh to 1e-6 of its value without a branch: 1 - 2 / (1 + e^2|x|), and below 1/4, where that cancels, the Taylor series to x^9 (remainder 0.0089 x^11). The worst
-// place is just above 1/4: the documented errors of ex2.approx (2^-22) and rcp.approx (1 ulp) and the rounding of 1 + e leave 2.2e-7 of a result of 0.245.
-__device__ __forceinline__ float sa_tanh(float x) {
-    const float a = fabsf(x), x2 = x * x;
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + tc_exp2(a * (2.0f * kSaLog2e))));
-    const float small = x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    return a < 0.25f ? small : copysignf(fmaf(-2.0f, r, 1.0f), x);
-}
 __device__ __forceinline__ float sa_log2(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -234,7 +224,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) seq_attention_tc_kernel(const _
         const float slope = kOpts && p.slopes ? p.slopes[h] : 0.0f, r1 = kOpts && p.logdist ? p.logdist[h] : 0.0f, r2 = kOpts && p.logdist ? p.logdist[p.heads + h] : 0.0f;
         // Weights are 2^(score * mul - ref): one rounding between a score and its exponential. Without caps or charges mul holds the scale, too.
         const bool plain = !kOpts && p.scale > 0.0f;
-        const float mul = plain ? p.scale * kSaLog2e : kSaLog2e;
+        const float mul = plain ? p.scale * kTcLog2e : kTcLog2e;
         float ref = -INFINITY, l = 0.0f, flushed = -INFINITY;      // what the weights are relative to; their sum; the reference of what has been flushed
         const int rows = parts >> ((warp * 32 >> sa.hpc_log2) / kBQ) & 1 ? min(32, (nq << sa.hpc_log2) - warp * 32) : 0;      // a warp's rows belong to one tile
         // the records of this warp's rows, and how far the next head's and the next query's are
@@ -310,11 +300,11 @@ __global__ void __launch_bounds__(kSaThreads, 2) seq_attention_tc_kernel(const _
                     if (e & 2) top1 = tc_max3(top1, fabsf(x), fabsf(y));
                     else top0 = tc_max3(top0, fabsf(x), fabsf(y));
                 }
-                // Scores within a quarter of the cap, as nearly all are: the series alone, two at a time. It is the one sa_tanh takes for them, so which of the two loops a tile
+                // Scores within a quarter of the cap, as nearly all are: the series alone, two at a time. It is the one tc_tanh takes for them, so which of the two loops a tile
                 // goes through shows in no bit (NaN stays NaN in both).
                 if (__any_sync(0xffffffffu, fmaxf(top0, top1) >= 0.25f)) {
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(p.softcap * sa_tanh(__uint_as_float(s[e])));
+                    for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(p.softcap * tc_tanh(__uint_as_float(s[e])));
                 } else {
                     auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
                     const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), c0 = both(1.0f), cap2 = both(p.softcap);

@@ -126,6 +126,16 @@ __device__ __forceinline__ float tc_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+constexpr float kTcLog2e = 1.4426950408889634f;
+// tanh to 1e-6 of its value without a branch: 1 - 2 / (1 + e^2|x|), and below 1/4, where that cancels, the Taylor series to x^9 (remainder 0.0089 x^11). The worst
+// place is just above 1/4: the documented errors of ex2.approx (2^-22) and rcp.approx (1 ulp) and the rounding of 1 + e leave 2.2e-7 of a result of 0.245.
+__device__ __forceinline__ float tc_tanh(float x) {
+    const float a = fabsf(x), x2 = x * x;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + tc_exp2(a * (2.0f * kTcLog2e))));
+    const float small = x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return a < 0.25f ? small : copysignf(fmaf(-2.0f, r, 1.0f), x);
+}
 __device__ __forceinline__ float tc_max3(float a, float b, float c) {      // fmaxf(fmaxf(a, b), c) in one instruction
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
