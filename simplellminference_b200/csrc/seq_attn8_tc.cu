@@ -4,11 +4,11 @@
 // tiles of 64 keys and values. fp16 operands, since fp16 holds every e4m3 code: keys and values enter exactly, and block scales multiply scores and weights.
 //   warp 0 (one lane)   TMA producer: boxes of 32 rows of codes, looked up in the block table, into a ring;
 //   warps 2, 3          codes to fp16 rows in the 128B swizzle (keys K-major, values as they lie); value rows that the run must not see, and NaN codes among values, become zeros;
-//   warp 1 (one lane)   MMA issuer: S = Q K^T with Q read from TMEM (shared memory has to feed the codes' conversion, too: from there Q alone would take its bandwidth), O += P V with P over S;
-//   warps 4-7, 8-11     softmax of tile 0 / 1, a thread per row: queries to fp16 in TMEM once an item, then per key tile maximum, weights and their sum;
+//   warp 1 (one lane)   MMA issuer: S = Q K^T, O += P V with P read from TMEM; P has columns of its own, so that the next scores are made while the softmax takes its exponentials;
+//   warps 4-7, 8-11     softmax of tile 0 / 1: queries to fp16 once an item; then, a thread per row, maximum, weights and their sum of every key tile;
 //   warps 12-15         O of both tiles: rescaled where a maximum has grown, results written, parts of shared items put together.
 // Results in bf16 (kTerms = 1): queries and weights are one fp16 number each (2^-12 of a value on average less than the 2^-9 of the result's own rounding). Results in fp32 (kTerms = 2): both are
-// the sum of two (22 bits; the second query term is read from shared memory), and O is added to an fp32 copy of the CTA's own every kT8Flush tiles, because the tensor core truncates as it
+// the sum of two (22 bits), and O is added to an fp32 copy of the CTA's own every kT8Flush tiles, because the tensor core truncates as it
 // accumulates.
 // Weights are relative to the largest of score + log2(value scale) so far, rounded up to a whole number: differences of exponents are exact then, and O is rescaled by powers of two, and
 // seldom. The denominator takes the value scale out again, block by block.
@@ -23,11 +23,11 @@
 
 namespace sllm {
 
-constexpr int kT8Rows = 128, kT8Keys = 64, kT8Threads = 512, kT8Raw = 4;      // rows of a tile, keys of a tile, stages of the codes' ring
+constexpr int kT8Rows = 128, kT8Keys = 64, kT8Threads = 512;      // rows of a tile, keys of a tile
 constexpr int kT8Extra = 4, kT8Least = 4;       // key tiles that an item's beginning and end count for; key tiles of a CTA's share at least
 constexpr int kT8Flush = 16;
 constexpr int kT8Known = 16;                    // key tiles whose scales are kept at hand: more than the producer is ever ahead of the softmax (the rings' stages and two)
-constexpr uint32_t kT8Tmem = 512, kT8S = 0, kT8Q = 128, kT8O = 256;           // columns: S0 S1 | Q0 Q1 | O0 O1
+constexpr uint32_t kT8Tmem = 512, kT8S = 0, kT8P = 128, kT8O = 256;           // columns: S0 S1 | P0 P1 | O0 O1
 
 struct T8Args {
     Attn8Args a;
@@ -208,13 +208,12 @@ struct T8Share {
 
 template <int HD, int kTerms>
 struct T8Shape {
-    static constexpr int kBlocks = HD / 64, kStages = kTerms == 1 ? 3 : 2;
+    static constexpr int kBlocks = HD / 64, kK = 2, kV = kTerms == 1 ? 2 : 1, kRaw = kTerms == 1 ? 4 : 2;      // stages of keys, of values, of codes
     static constexpr int kBlock = kT8Keys * 128, kTile = kBlocks * kBlock;    // fp16: 64 columns of all keys; all columns
     static constexpr int kCodes = kT8Keys * HD;                              // bytes of a tile of codes
-    static constexpr int kQBlock = kT8Rows * 128, kQTile = kTerms == 2 ? kBlocks * kQBlock : 0;
-    static constexpr int kStaging = kTerms == 1 ? 8 * 32 * 128 : 0;           // queries on their way to TMEM: 32 rows of 32 columns a warp (with two terms the second one's place)
+    static constexpr int kQBlock = kT8Rows * 128, kQTerm = kBlocks * kQBlock, kQTile = kTerms * kQTerm;
     static constexpr int kItems = (kT8Items * (int)sizeof(T8Item) + 127) / 128 * 128;
-    static constexpr int kSmem = 1024 + 2 * kStages * kTile + 2 * kT8Raw * kCodes + 2 * kQTile + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems + kStaging;
+    static constexpr int kSmem = 1024 + (kK + kV) * kTile + 2 * kRaw * kCodes + 2 * kQTile + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems;
 };
 constexpr int kT8PartTile = kT8Rows * (128 + 2), kT8Part = 2 * kT8PartTile;   // floats of a part: per tile O as [HD / 4][128][4], references, sums
 static_assert(kT8Part == kA8Part, "the workspace's parts");
@@ -248,20 +247,127 @@ __device__ __forceinline__ uint4 t8_lds(uint32_t at) {
 __device__ __forceinline__ void t8_sts(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// The roles' code together has to stay near what the instruction caches hold (with everything in line it was 172 KB, and an item's beginning took 14000 clocks): what is seldom run is a function.
+__device__ __noinline__ bool t8_wait_long(uint64_t* bar, uint32_t parity, volatile int* gave_up, unsigned polls) { return tc_wait(bar, parity, gave_up, polls); }
+__device__ __forceinline__ bool t8_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, unsigned polls) {
+    uint32_t done = 0;
+    if (polls)
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(s_addr(bar)), "r"(parity) : "memory");
+    return done || t8_wait_long(bar, parity, gave_up, polls);
+}
+__device__ __forceinline__ bool t8_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up, unsigned polls) {
+    return __all_sync(0xffffffffu, t8_wait(bar, parity, gave_up, polls));
+}
+__device__ __noinline__ float4 t8_four(const float* x, bool take) { return take ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); }      // (an address of any alignment)
 // fp16 operands: the bf16 descriptor without its types
 __host__ __device__ constexpr uint32_t t8_idesc(int M, int N) { return umma_idesc_bf16(M, N) & ~((1u << 7) | (1u << 10)); }
+
+// Where the result of a row of tile j goes, or whether it has none
+struct T8Out { float* out; uint16_t* out16; bool listed, wide; };
+__device__ __forceinline__ T8Out t8_out(const T8Args& p, const T8Item& it, int j, int row) {
+    const Attn8Args& a = p.a;
+    const int q = j * p.queries + (row >> p.hpc_log2), h = it.h0 + (row & (p.hpc - 1));
+    const size_t t = it.tok0 + q;
+    T8Out r{a.out ? a.out + t * a.ldo + (size_t)h * a.dv : nullptr, a.out16 ? a.out16 + (t * a.heads + h) * a.dv : nullptr, it.listed(q), false};
+    r.wide = ((reinterpret_cast<uintptr_t>(r.out) | reinterpret_cast<uintptr_t>(r.out16)) & 15) == 0;
+    return r;
+}
+__device__ __noinline__ void t8_store_narrow(float* out, uint16_t* out16, float4 x, float4 y) {
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (out) out[e] = v[e];
+        if (out16) out16[e] = f32_to_bf16_bits(v[e]);
+    }
+}
+// eight columns
+__device__ __forceinline__ void t8_store(const T8Out& to, int c, float4 x, float4 y) {
+    if (!to.wide) {
+        t8_store_narrow(to.out ? to.out + c : nullptr, to.out16 ? to.out16 + c : nullptr, x, y);
+        return;
+    }
+    if (to.out) {
+        *reinterpret_cast<float4*>(to.out + c) = x;
+        *reinterpret_cast<float4*>(to.out + c + 4) = y;
+    }
+    if (to.out16) *reinterpret_cast<uint4*>(to.out16 + c) = make_uint4(tc_pack(x.x, x.y), tc_pack(x.z, x.w), tc_pack(y.x, y.y), tc_pack(y.z, y.w));
+}
+// Rare: a row whose keys' values may hold NaN codes has its result; it becomes NaN in the columns where one of the values that it sees is.
+__device__ __noinline__ void t8_poison(const T8Args& p, const T8Item& it, int j, int row) {
+    const Attn8Args& a = p.a;
+    const T8Out to = t8_out(p, it, j, row);
+    if (!to.listed) return;
+    const int pos = it.pos0 + j * p.queries + (row >> p.hpc_log2), wnd = seq_row_window(pos, a.window, a.chunk);
+    const TileList mine(pos, pos, wnd, a.keep_first, kKv8Block);
+    for (int x = 0; x < mine.n; ++x) {
+        const int key0 = mine.tile_of(x) * kKv8Block, r = t8_row(a, it.slot, it.gkv, key0, pos);
+        if (r < 0) continue;
+        for (int e = 0; e < kKv8Block; ++e) {
+            if (!seq_sees(pos, key0 + e, wnd, a.keep_first)) continue;
+            const uint8_t* v = a.v_pool + (size_t)(r + e) * a.dv;
+            for (int c = 0; c < a.dv; ++c) {
+                if ((v[c] & 0x7f) != 0x7f) continue;
+                if (to.out) to.out[c] = __int_as_float(0x7fffffff);
+                if (to.out16) to.out16[c] = 0x7fff;
+            }
+        }
+    }
+}
+// An item whose parts are all there, row `row` of both tiles: its parts brought to one reference and added, in the order of the key tiles.
+__device__ __noinline__ void t8_merge(const T8Args& p, const T8Item& it, int row) {
+    const int parts = it.parts;
+#pragma unroll 1
+    for (int j = 0; j < 2; ++j) {
+        const float* first = p.parts + (size_t)(2 * it.first_cta + it.later) * kT8Part + j * kT8PartTile;
+        const float* rest = p.parts + (size_t)(2 * it.first_cta) * kT8Part + j * kT8PartTile;
+        auto from = [&](int x) { return x == 0 ? first : rest + (size_t)(2 * x) * kT8Part; };
+        float top = -INFINITY, l = 0.0f;
+        bool wild = false;
+#pragma unroll 4
+        for (int x = 0; x < parts; ++x) top = fmaxf(top, __ldcg(from(x) + 128 * kT8Rows + row));
+#pragma unroll 4
+        for (int x = 0; x < parts; ++x) {
+            const float r = __ldcg(from(x) + 128 * kT8Rows + row), s = __ldcg(from(x) + 129 * kT8Rows + row);
+            wild |= __float_as_uint(s) >> 31;
+            l += fabsf(s) * (r == top ? 1.0f : tc_exp2(r - top));
+        }
+        const T8Out to = t8_out(p, it, j, row);
+        if (!to.listed) continue;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (int c = 0; c < p.a.dv; c += 16) {
+            float4 y[4] = {};
+#pragma unroll 2
+            for (int x = 0; x < parts; ++x) {
+                const float r = __ldcg(from(x) + 128 * kT8Rows + row);
+                if (r == -INFINITY && __ldcg(from(x) + 129 * kT8Rows + row) == 0.0f) continue;       // none of this part's keys is visible: its O may never have been written
+                const float f = r == top ? 1.0f : tc_exp2(r - top);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(from(x)) + (c / 4 + i) * kT8Rows + row);
+                    y[i].x = fmaf(v.x, f, y[i].x); y[i].y = fmaf(v.y, f, y[i].y); y[i].z = fmaf(v.z, f, y[i].z); y[i].w = fmaf(v.w, f, y[i].w);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = make_float4(y[i].x * inv, y[i].y * inv, y[i].z * inv, y[i].w * inv);
+            t8_store(to, c, y[0], y[1]);
+            t8_store(to, c + 8, y[2], y[3]);
+        }
+        if (wild) t8_poison(p, it, j, row);
+    }
+}
 
 template <int HD, int kTerms, bool kOpts>
 __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ T8Args p) {
     using Sh = T8Shape<HD, kTerms>;
-    constexpr int ST = Sh::kStages, RS = kT8Raw;
+    constexpr int SK = Sh::kK, SV = Sh::kV, RS = Sh::kRaw;
     extern __shared__ uint8_t t8_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(t8_smem) + 1023) & ~(uintptr_t)1023);
-    uint8_t *sK = smem, *sV = sK + ST * Sh::kTile, *sQ = sV + ST * Sh::kTile, *sRaw = sQ + 2 * Sh::kQTile;      // sRaw: keys, then values, of each stage
+    uint8_t *sK = smem, *sV = sK + SK * Sh::kTile, *sQ = sV + SV * Sh::kTile, *sRaw = sQ + 2 * Sh::kQTile;      // sRaw: keys, then values, of each stage
     uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + 2 * RS * Sh::kCodes);
-    uint64_t *rfull = bars, *rempty = rfull + RS, *kfull = rempty + RS, *kempty = kfull + ST, *vfull = kempty + ST, *vempty = vfull + ST;
-    // per tile: queries written / scores written / factors for O written / weights written and O rescaled / product with the values done / sums written, and read
-    uint64_t *qready = vempty + ST, *sfull = qready + 2, *factors = sfull + 2, *pready = factors + 2, *odone = pready + 2, *lready = odone + 2, *lread = lready + 2;
+    uint64_t *rfull = bars, *rempty = rfull + RS, *kfull = rempty + RS, *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV;
+    // per tile: queries written / scores written / scores read / factors for O written / weights written and O rescaled / product with the values done / sums written, and read
+    uint64_t *qready = vempty + SV, *sfull = qready + 2, *sread = sfull + 2, *factors = sread + 2, *pready = factors + 2, *odone = pready + 2, *lready = odone + 2, *lread = lready + 2;
     uint64_t* meet = lread + 2;              // of warps 12-15
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet + 1);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -272,15 +378,15 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
     float *s_ref = factor + 2 * kT8Rows, *s_sum = s_ref + 2 * kT8Rows;                        // [2][128] each
     T8Tile* s_tile = reinterpret_cast<T8Tile*>(s_sum + 2 * kT8Rows);                           // [kT8Known]
     T8Item* s_items = reinterpret_cast<T8Item*>(factor + 8 * kT8Rows);                         // [kT8Items]
-    uint8_t* s_stage = reinterpret_cast<uint8_t*>(factor + 8 * kT8Rows) + Sh::kItems;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Attn8Args& a = p.a;
 
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < RS; ++i) { mb_init(rfull + i, 1); mb_init(rempty + i, 2); }
-        for (int i = 0; i < ST; ++i) { mb_init(kfull + i, 2); mb_init(kempty + i, 1); mb_init(vfull + i, 2); mb_init(vempty + i, 1); }
+        for (int i = 0; i < SK; ++i) { mb_init(kfull + i, 2); mb_init(kempty + i, 1); }
+        for (int i = 0; i < SV; ++i) { mb_init(vfull + i, 2); mb_init(vempty + i, 1); }
         for (int j = 0; j < 2; ++j) {
-            mb_init(qready + j, 128); mb_init(sfull + j, 1); mb_init(factors + j, 128); mb_init(pready + j, 256); mb_init(odone + j, 1); mb_init(lready + j, 128); mb_init(lread + j, 128);
+            mb_init(qready + j, 128); mb_init(sfull + j, 1); mb_init(sread + j, 128); mb_init(factors + j, 128); mb_init(pready + j, 256); mb_init(odone + j, 1); mb_init(lready + j, 128); mb_init(lread + j, 128);
         }
         *gave_up = 0;
         for (int i = 0; i < 8; ++i) s_nan[i] = 0;
@@ -342,7 +448,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 }
                 const int s = g % RS, from = (k - it.k0) & 31;
                 const int row[2] = {__shfl_sync(0xffffffffu, mine.row[0], from), __shfl_sync(0xffffffffu, mine.row[1], from)};
-                ok = tc_wait_warp(rempty + s, ((uint32_t)(g / RS) & 1) ^ 1, gave_up, p.polls);
+                ok = t8_wait_warp(rempty + s, ((uint32_t)(g / RS) & 1) ^ 1, gave_up, p.polls);
                 if (!ok) break;
                 if (lane == from) s_tile[g % kT8Known] = mine;
                 __syncwarp();
@@ -363,76 +469,62 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
         if (elect_one()) {   // ===== MMA issuer =====
             constexpr uint32_t idesc_s = t8_idesc(kT8Rows, kT8Keys), idesc_o = t8_idesc(kT8Rows, HD) | (1u << 16);      // B MN-major
             const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, Sh::kBlock);     // + bytes / 16: another place
-            auto scores = [&](int j, int g) {
-                const uint64_t k = k_desc + (uint32_t)(g % ST) * (Sh::kTile / 16), q = q_desc + (uint32_t)j * (Sh::kQTile / 16);
+            uint32_t made[2] = {0, 0}, done[2] = {0, 0}, items[2] = {0, 0};     // scores, products and items of either tile
+            auto scores = [&](int j, int g) {    // behind the softmax's reading of the ones before
+                if (made[j] && !t8_wait(sread + j, (made[j] - 1) & 1, gave_up, p.polls)) return false;
+                ++made[j];
+                tc_fence_after();
+                const uint64_t k = k_desc + (uint32_t)(g % SK) * (Sh::kTile / 16);
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks)
-                    tc_mma_bf16_ts(tmem + kT8S + 64 * j, tmem + kT8Q + 64 * j + 8 * ks, k + (uint32_t)((ks / 4) * (Sh::kBlock / 16) + 2 * (ks % 4)), idesc_s, ks != 0);
-                if constexpr (kTerms == 2) {
+                for (int term = 0; term < kTerms; ++term) {
+                    const uint64_t q = q_desc + (uint32_t)j * (Sh::kQTile / 16) + (uint32_t)term * (Sh::kQTerm / 16);
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks)
-                        tc_mma_bf16(tmem + kT8S + 64 * j, q + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kBlock / 16) + 2 * (ks % 4)), idesc_s, 1);
+                        tc_mma_bf16(tmem + kT8S + 64 * j, q + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kBlock / 16) + 2 * (ks % 4)), idesc_s,
+                                    term != 0 || ks != 0);
                 }
                 tc_commit(sfull + j);
+                return true;
             };
             auto values = [&](int j, int g, bool more) {
-                const uint64_t v = v_desc + (uint32_t)(g % ST) * (Sh::kTile / 16);
+                const uint64_t v = v_desc + (uint32_t)(g % SV) * (Sh::kTile / 16);
 #pragma unroll
                 for (int ks = 0; ks < kTerms * kT8Keys / 16; ++ks)       // first terms, then second ones, against the same values
-                    tc_mma_bf16_ts(tmem + kT8O + 128 * j, tmem + kT8S + 64 * j + 8 * ks, v + (uint32_t)((ks % (kT8Keys / 16)) * 128), idesc_o, more || ks != 0);
+                    tc_mma_bf16_ts(tmem + kT8O + 128 * j, tmem + kT8P + 64 * j + 8 * ks, v + (uint32_t)((ks % (kT8Keys / 16)) * 128), idesc_o, more || ks != 0);
                 tc_commit(odone + j);
             };
             T8Item more;
-            int g = 0;                           // key tiles so far; products and items of either tile
-            uint32_t done[2] = {0, 0}, items[2] = {0, 0};
+            int g = 0;                           // key tiles so far
             bool ok = true;
-            for (int i = 0; ok; ++i) {
-                const T8Item* at = item_at(i, more);
+            for (int n_item = 0; ok; ++n_item) {
+                const T8Item* at = item_at(n_item, more);
                 if (!at) break;
                 const int n = at->k1 - at->k0, nkt[2] = {at->keys[0], at->keys[1]};
-                ok = tc_wait(kfull + g % ST, (uint32_t)(g / ST) & 1, gave_up, p.polls);
-                if (!ok) break;
-                tc_fence_after();
+                ok = t8_wait(kfull + g % SK, (uint32_t)(g / SK) & 1, gave_up, p.polls);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (!ok || nkt[j] == 0) continue;
-                    ok = tc_wait(qready + j, items[j]++ & 1, gave_up, p.polls);
-                    // they land where the last weights of the item before lie
-                    if (ok && done[j]) ok = tc_wait(odone + j, (done[j] - 1) & 1, gave_up, p.polls);
-                    if (!ok) continue;
-                    tc_fence_after();
-                    scores(j, g);
-                }
+                for (int j = 0; j < 2; ++j)
+                    if (ok && nkt[j]) ok = t8_wait(qready + j, items[j]++ & 1, gave_up, p.polls) && scores(j, g);
                 if (!ok) break;
-                tc_commit(kempty + g % ST);
-                for (int kt = 0; kt < n; ++kt, ++g) {
-                    ok = tc_wait(vfull + g % ST, (uint32_t)(g / ST) & 1, gave_up, p.polls);
-                    bool keys = false;
+                tc_commit(kempty + g % SK);
+                for (int kt = 0; ok && kt < n; ++kt, ++g) {
+                    if (kt + 1 < n) ok = t8_wait(kfull + (g + 1) % SK, (uint32_t)((g + 1) / SK) & 1, gave_up, p.polls);
+                    // Either tile's next scores, then its product with these values: so the tiles come to lie half a step apart, and one's exponentials run during the other's products.
+                    bool values_there = false;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
+                        if (ok && kt + 1 < nkt[j]) ok = scores(j, g + 1);
                         if (!ok || kt >= nkt[j]) continue;
-                        ok = tc_wait(pready + j, done[j] & 1, gave_up, p.polls);
+                        if (!values_there) ok = t8_wait(vfull + g % SV, (uint32_t)(g / SV) & 1, gave_up, p.polls);
+                        values_there = true;
+                        ok = ok && t8_wait(pready + j, done[j] & 1, gave_up, p.polls);
                         if (!ok) continue;
+                        ++done[j];
                         tc_fence_after();
                         values(j, g, kTerms == 1 ? kt != 0 : kt % kT8Flush != 0);
-                        ++done[j];
-                        if (kt + 1 >= nkt[j]) continue;
-                        if (!keys) {
-                            ok = tc_wait(kfull + (g + 1) % ST, (uint32_t)((g + 1) / ST) & 1, gave_up, p.polls);
-                            keys = true;
-                        }
-                        // the next scores land where the weights lie that this product is still reading
-                        ok = ok && tc_wait(odone + j, (done[j] - 1) & 1, gave_up, p.polls);
-                        if (!ok) continue;
-                        tc_fence_after();
-                        scores(j, g + 1);
                     }
                     if (!ok) break;
-                    tc_commit(vempty + g % ST);
-                    if (kt + 1 < n) {
-                        if (!keys) ok = tc_wait(kfull + (g + 1) % ST, (uint32_t)((g + 1) / ST) & 1, gave_up, p.polls);     // (nobody needed these keys; never so while a tile goes on)
-                        tc_commit(kempty + (g + 1) % ST);
-                    }
+                    tc_commit(vempty + g % SV);
+                    if (kt + 1 < n) tc_commit(kempty + (g + 1) % SK);
                 }
             }
         }
@@ -442,65 +534,69 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
         bool ok = true;
         const int me = (warp - 2) * 32 + lane, r8 = me & 7, c0 = me >> 3;       // row of eight, first chunk: neighbouring lanes' chunks lie in different banks, read and written
         constexpr int kChunks = HD / 16, kPer = 8 / kChunks;                    // chunks of a row; rows of eight that 64 threads take at a time: 1 or 2
+        // wild: rows that the run must not see become zeros, and NaN codes, which are reported
+        auto convert = [&](int key0, int last_pos, int x, const uint8_t* raw, uint8_t* tile, auto values_, auto wild_) {
+            constexpr bool values = decltype(values_)::value, wild = decltype(wild_)::value;
+            const uint32_t from = s_addr(raw), to = s_addr(tile);
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int r0 = 0; r0 < kT8Keys; r0 += 8 * kPer) {
+                const int row = r0 + r8 + 8 * (c0 / kChunks), chunk = c0 % kChunks;
+                uint4 v = t8_lds(from + row * HD + ((HD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
+                if (values) {
+                    const bool take = !wild || (key0 + row <= last_pos && s_tile[x % kT8Known].row[row >= kKv8Block] >= 0);
+                    auto look = [&](uint32_t y) {
+                        if (wild && !take) y = 0u;
+                        const uint32_t n = (y & 0x7f7f7f7fu) + 0x01010101u;                  // the top bit of every NaN
+                        any |= n;
+                        return wild ? y & ~(((n & 0x80808080u) >> 7) * 0xffu) : y;
+                    };
+                    v.x = look(v.x); v.y = look(v.y); v.z = look(v.z); v.w = look(v.w);
+                }
+                const uint32_t at = to + (chunk / 4) * Sh::kBlock + row * 128, c = (chunk % 4) * 2;
+                t8_sts(at + ((c ^ (row & 7)) << 4), kv8_half2(v.x & 0xffffu), kv8_half2(v.x >> 16), kv8_half2(v.y & 0xffffu), kv8_half2(v.y >> 16));
+                t8_sts(at + (((c + 1) ^ (row & 7)) << 4), kv8_half2(v.z & 0xffffu), kv8_half2(v.z >> 16), kv8_half2(v.w & 0xffffu), kv8_half2(v.w >> 16));
+            }
+            return __any_sync(0xffffffffu, any & 0x80808080u);
+        };
+        auto publish = [&]() {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
         for (int n_item = 0; ok; ++n_item) {
             const T8Item* at = item_at(n_item, more);
             if (!at) break;
             const TileList tiles = tiles_of(*at);
             const int last_pos = at->pos0 + at->hi;
-            for (int k = at->k0, k1 = at->k1; k < k1; ++k, ++g) {
-                const int s = g % RS, t = g % ST, key0 = tiles.tile_of(k) * kT8Keys;
-                const uint32_t par = (uint32_t)(g / ST) & 1;
-                ok = tc_wait_warp(rfull + s, (uint32_t)(g / RS) & 1, gave_up, p.polls) && tc_wait_warp(kempty + t, par ^ 1, gave_up, p.polls);
-                if (!ok) break;
-                // kWild: rows that the run must not see become zeros, and NaN codes, which are reported
-                auto convert = [&](const uint8_t* raw, uint8_t* tile, auto values_, auto wild_) {
-                    constexpr bool values = decltype(values_)::value, wild = decltype(wild_)::value;
-                    const uint32_t from = s_addr(raw), to = s_addr(tile);
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int r0 = 0; r0 < kT8Keys; r0 += 8 * kPer) {
-                        const int row = r0 + r8 + 8 * (c0 / kChunks), chunk = c0 % kChunks;
-                        uint4 v = t8_lds(from + row * HD + ((HD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
-                        if (values) {
-                            const bool take = !wild || (key0 + row <= last_pos && s_tile[g % kT8Known].row[row >= kKv8Block] >= 0);
-                            auto look = [&](uint32_t y) {
-                                if (wild && !take) y = 0u;
-                                const uint32_t n = (y & 0x7f7f7f7fu) + 0x01010101u;                  // the top bit of every NaN
-                                any |= n;
-                                return wild ? y & ~(((n & 0x80808080u) >> 7) * 0xffu) : y;
-                            };
-                            v.x = look(v.x); v.y = look(v.y); v.z = look(v.z); v.w = look(v.w);
-                        }
-                        const uint32_t at = to + (chunk / 4) * Sh::kBlock + row * 128, c = (chunk % 4) * 2;
-                        t8_sts(at + ((c ^ (row & 7)) << 4), kv8_half2(v.x & 0xffffu), kv8_half2(v.x >> 16), kv8_half2(v.y & 0xffffu), kv8_half2(v.y >> 16));
-                        t8_sts(at + (((c + 1) ^ (row & 7)) << 4), kv8_half2(v.z & 0xffffu), kv8_half2(v.z >> 16), kv8_half2(v.w & 0xffffu), kv8_half2(v.w >> 16));
-                    }
-                    return __any_sync(0xffffffffu, any & 0x80808080u);
-                };
-                auto publish = [&]() {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                };
-                convert(sRaw + 2 * s * Sh::kCodes, sK + t * Sh::kTile, std::false_type{}, std::false_type{});
+            auto keys = [&](int x) {               // keys of this CTA's tile x
+                ok = t8_wait_warp(rfull + x % RS, (uint32_t)(x / RS) & 1, gave_up, p.polls) && t8_wait_warp(kempty + x % SK, ((uint32_t)(x / SK) & 1) ^ 1, gave_up, p.polls);
+                if (!ok) return;
+                convert(0, 0, 0, sRaw + 2 * (x % RS) * Sh::kCodes, sK + x % SK * Sh::kTile, std::false_type{}, std::false_type{});
                 publish();
-                if (lane == 0) mb_arrive(kfull + t);
-                ok = tc_wait_warp(vempty + t, par ^ 1, gave_up, p.polls);
+                if (lane == 0) mb_arrive(kfull + x % SK);
+            };
+            keys(g);
+            for (int k = at->k0, k1 = at->k1; ok && k < k1; ++k, ++g) {
+                const int s = g % RS, tv = g % SV, key0 = tiles.tile_of(k) * kT8Keys;
+                if (k + 1 < k1) keys(g + 1);       // a tile ahead of the values: the scores come first
+                if (!ok) break;
+                ok = t8_wait_warp(vempty + tv, ((uint32_t)(g / SV) & 1) ^ 1, gave_up, p.polls);
                 if (!ok) break;
                 const uint8_t* codes = sRaw + (2 * s + 1) * Sh::kCodes;
                 bool whole = key0 + kT8Keys - 1 <= last_pos && s_tile[g % kT8Known].row[0] >= 0 && s_tile[g % kT8Known].row[1] >= 0;
-                if (whole) whole = !convert(codes, sV + t * Sh::kTile, std::true_type{}, std::false_type{});
-                if (!whole && convert(codes, sV + t * Sh::kTile, std::true_type{}, std::true_type{})) {
+                if (whole) whole = !convert(key0, last_pos, g, codes, sV + tv * Sh::kTile, std::true_type{}, std::false_type{});
+                if (!whole && convert(key0, last_pos, g, codes, sV + tv * Sh::kTile, std::true_type{}, std::true_type{})) {
                     s_nan[n_item & 7] = n_item + 1;          // read behind the product with these values
                     __threadfence_block();
                 }
                 publish();
-                if (lane == 0) { mb_arrive(vfull + t); mb_arrive(rempty + s); }
+                if (lane == 0) { mb_arrive(vfull + tv); mb_arrive(rempty + s); }
             }
         }
     } else if (warp >= 12) {   // ===== O of both tiles =====
         const int quad = warp & 3, row = quad * 32 + lane;
         T8Item more;
-        uint32_t done[2] = {0, 0}, items[2] = {0, 0};
+        uint32_t done0 = 0, done1 = 0, items0 = 0, items1 = 0;
         uint32_t met = 0;
         bool ok = true;
         for (int n_item = 0; ok; ++n_item) {
@@ -510,21 +606,23 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             const int n = it.k1 - it.k0, nkt[2] = {it.keys[0], it.keys[1]};
             const bool whole = it.parts == 1;
             float* part = p.parts + (size_t)(2 * blockIdx.x + it.slot_of) * kT8Part;
-            float since[2] = {1.0f, 1.0f};                                     // what the references have grown by since O was flushed
+            float since0 = 1.0f, since1 = 1.0f;                                // what the references have grown by since O was flushed
             for (int kt = 0; ok && kt < n; ++kt)
-#pragma unroll
+#pragma unroll 1
                 for (int j = 0; j < 2; ++j) {
-                    if (!ok || kt >= nkt[j]) continue;
-                    ok = tc_wait_warp(factors + j, done[j] & 1, gave_up, p.polls);
-                    if (ok && kt > 0) ok = tc_wait_warp(odone + j, (done[j] - 1) & 1, gave_up, p.polls);     // long since: the scores follow that product
+                    if (!ok || kt >= (j ? nkt[1] : nkt[0])) continue;
+                    float since = j ? since1 : since0;
+                    const uint32_t so_far = j ? done1 : done0;
+                    ok = t8_wait_warp(factors + j, so_far & 1, gave_up, p.polls);       // (the softmax has waited for the product before)
+                    if (ok && kt > 0) ok = t8_wait_warp(odone + j, (so_far - 1) & 1, gave_up, p.polls);
                     if (!ok) continue;
-                    ++done[j];
+                    (j ? done1 : done0) = so_far + 1;
                     tc_fence_after();
                     const float f = factor[j * kT8Rows + row];
                     const uint32_t o_tmem = tmem + ((uint32_t)(quad * 32) << 16) + kT8O + 128 * j;
                     if (kTerms == 2 && kt > 0 && kt % kT8Flush == 0) {         // O so far, relative to the reference before this tile's
                         uint4* acc = reinterpret_cast<uint4*>(part + j * kT8PartTile);
-                        const float s = kt > kT8Flush ? since[j] : 0.0f;
+                        const float s = kt > kT8Flush ? since : 0.0f;
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
                             uint32_t o[32];
@@ -539,9 +637,9 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                                 acc[(c / 4 + i) * kT8Rows + row] = make_uint4(sum(v[i].x, o[4 * i]), sum(v[i].y, o[4 * i + 1]), sum(v[i].z, o[4 * i + 2]), sum(v[i].w, o[4 * i + 3]));
                             }
                         }
-                        since[j] = f;
+                        since = f;
                     } else {
-                        since[j] *= f;
+                        since *= f;
                         if (kt > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
 #pragma unroll 1
                             for (int c = 0; c < HD; c += 32) {
@@ -555,102 +653,39 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                             tc_wait_st();
                         }
                     }
+                    (j ? since1 : since0) = since;
                     tc_fence_before();
                     mb_arrive(pready + j);
                 }
             if (!ok) break;
             // ---- results, or this CTA's part of them ----
-            const bool nan_here = s_nan[n_item & 7] == n_item + 1;
-            auto query = [&](int j, int& q) {                                  // this row's query, and whether it is listed
-                q = j * p.queries + (row >> p.hpc_log2);
-                return it.listed(q);
-            };
-            // columns c .. c + 31 of this row: o * inv; `hit`: columns that a NaN value reaches
-            auto store = [&](int j, int c, const float (&o)[32], float inv, const uint32_t (&hit)[4]) {
-                int q;
-                if (!query(j, q) || c >= a.dv) return;
-                const size_t t = it.tok0 + q;
-                const int h = it.h0 + (row & (p.hpc - 1)), cols = min(32, a.dv - c);
-                float y[32];
-                uint32_t hits = 0;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) hits = c / 32 == x ? hit[x] : hits;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = hits >> i & 1 ? __int_as_float(0x7fffffff) : o[i] * inv;
-                if (a.out) {
-                    float* dst = a.out + t * a.ldo + (size_t)h * a.dv + c;
-                    if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            if (i < cols) *reinterpret_cast<float4*>(dst + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i < cols) dst[i] = y[i];
-                    }
-                }
-                if (a.out16) {
-                    uint16_t* dst = a.out16 + (t * a.heads + h) * a.dv + c;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        if (i < cols) {
-                            if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-                                *reinterpret_cast<uint4*>(dst + i) = make_uint4(tc_pack(y[i], y[i + 1]), tc_pack(y[i + 2], y[i + 3]), tc_pack(y[i + 4], y[i + 5]), tc_pack(y[i + 6], y[i + 7]));
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) dst[i + e] = f32_to_bf16_bits(y[i + e]);
-                            }
-                        }
-                }
-            };
-            // the columns in which a value that this row sees is NaN (rare: a walk over all its keys)
-            auto search = [&](int j, uint32_t (&hit)[4]) {
-                int q;
-                if (!query(j, q)) return;
-                const int pos = it.pos0 + q, wnd = seq_row_window(pos, a.window, a.chunk);
-                const TileList mine(pos, pos, wnd, a.keep_first, kKv8Block);
-                for (int x = 0; x < mine.n; ++x) {
-                    const int key0 = mine.tile_of(x) * kKv8Block, r = t8_row(a, it.slot, it.gkv, key0, pos);
-                    if (r < 0) continue;
-                    for (int e = 0; e < kKv8Block; ++e) {
-                        if (!seq_sees(pos, key0 + e, wnd, a.keep_first)) continue;
-                        const uint32_t* v = reinterpret_cast<const uint32_t*>(a.v_pool + (size_t)(r + e) * a.dv);
-                        for (int c = 0; c < a.dv / 4; ++c) {
-                            const uint32_t m = ((v[c] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                            if (m) {
-                                const uint32_t bits = (m >> 7 & 1) | (m >> 14 & 2) | (m >> 21 & 4) | (m >> 28 & 8);
-#pragma unroll
-                                for (int y = 0; y < 4; ++y)
-                                    if (c / 8 == y) hit[y] |= bits << (4 * (c % 8));
-                            }
-                        }
-                    }
-                }
-            };
 #pragma unroll 1
             for (int j = 0; ok && j < 2; ++j) {
-                if (nkt[j] == 0) {
+                const int mine = j ? nkt[1] : nkt[0];
+                const float since = j ? since1 : since0;
+                if (mine == 0) {
                     if (!whole) {                                              // none of this part's keys is visible to this tile
                         part[j * kT8PartTile + 128 * kT8Rows + row] = -INFINITY;
                         part[j * kT8PartTile + 129 * kT8Rows + row] = 0.0f;
                     }
                     continue;
                 }
-                ok = tc_wait_warp(lready + j, items[j]++ & 1, gave_up, p.polls) && tc_wait_warp(odone + j, (done[j] - 1) & 1, gave_up, p.polls);
+                ok = t8_wait_warp(lready + j, (j ? items1 : items0) & 1, gave_up, p.polls) && t8_wait_warp(odone + j, ((j ? done1 : done0) - 1) & 1, gave_up, p.polls);
+                if (j) ++items1; else ++items0;
                 if (!ok) break;
                 tc_fence_after();
                 const float ref = s_ref[j * kT8Rows + row], l = s_sum[j * kT8Rows + row], inv = l == 0.0f ? 0.0f : 1.0f / l;
                 mb_arrive(lread + j);
-                uint32_t hit[4] = {0u, 0u, 0u, 0u};
-                if (whole && nan_here) search(j, hit);
+                const bool nan_here = s_nan[n_item & 7] == n_item + 1;         // (behind the last product: every value has been converted)
                 const uint32_t o_tmem = tmem + ((uint32_t)(quad * 32) << 16) + kT8O + 128 * j;
                 uint4* acc = reinterpret_cast<uint4*>(part + j * kT8PartTile);
-                const bool flushed = kTerms == 2 && nkt[j] > kT8Flush;
+                const bool flushed = kTerms == 2 && mine > kT8Flush;
+                const T8Out to = t8_out(p, it, j, row);
+                const float f = whole ? inv : 1.0f;
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t o[32];
                     tc_ld32_async(o_tmem + c, o);
-                    float y[32];
                     if (flushed) {
                         uint4 v[8];
 #pragma unroll
@@ -658,23 +693,26 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         tc_arrived(o);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float s = since[j];
-                            y[4 * i] = fmaf(__uint_as_float(v[i].x), s, __uint_as_float(o[4 * i])); y[4 * i + 1] = fmaf(__uint_as_float(v[i].y), s, __uint_as_float(o[4 * i + 1]));
-                            y[4 * i + 2] = fmaf(__uint_as_float(v[i].z), s, __uint_as_float(o[4 * i + 2])); y[4 * i + 3] = fmaf(__uint_as_float(v[i].w), s, __uint_as_float(o[4 * i + 3]));
+                            auto sum = [&](uint32_t x, uint32_t& y) { y = __float_as_uint(fmaf(__uint_as_float(x), since, __uint_as_float(y))); };
+                            sum(v[i].x, o[4 * i]); sum(v[i].y, o[4 * i + 1]); sum(v[i].z, o[4 * i + 2]); sum(v[i].w, o[4 * i + 3]);
                         }
                     } else {
                         tc_arrived(o);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]);
                     }
-                    if (whole) {
-                        store(j, c, y, inv, hit);
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) acc[(c / 4 + i) * kT8Rows + row] = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), __float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]));
+                    for (int i = 0; i < 32; i += 8) {
+                        auto four = [&](int e) { return make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f); };
+                        const float4 x = four(i), y = four(i + 4);
+                        if (!whole) {
+                            reinterpret_cast<float4*>(acc)[((c + i) / 4) * kT8Rows + row] = x;
+                            reinterpret_cast<float4*>(acc)[((c + i) / 4 + 1) * kT8Rows + row] = y;
+                        } else if (to.listed && c + i < a.dv) {
+                            t8_store(to, c + i, x, y);
+                        }
                     }
                     __syncwarp();
                 }
+                if (whole && nan_here) t8_poison(p, it, j, row);
                 if (!whole) {
                     part[j * kT8PartTile + 128 * kT8Rows + row] = ref;
                     part[j * kT8PartTile + 129 * kT8Rows + row] = nan_here ? -l : l;      // (sums are not negative: the sign says that there was NaN)
@@ -686,7 +724,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 const int c_first = it.first_cta, parts = it.parts;
                 auto together = [&]() {              // these four warps; a wait like the others, which ends
                     mb_arrive(meet);
-                    ok = tc_wait_warp(meet, met++ & 1, gave_up, p.polls);
+                    ok = t8_wait_warp(meet, met++ & 1, gave_up, p.polls);
                     return ok;
                 };
                 if (!together()) break;
@@ -697,50 +735,16 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     if (before_me == parts - 1) p.counters[c_first] = 0;
                 }
                 if (!together()) break;
-                if (*s_last) {                       // all parts are there: in the order of the key tiles, whoever was last
+                if (*s_last) {
                     __threadfence();
-                    const int later = it.later;
-                    auto from = [&](int x, int j) { return p.parts + (size_t)(2 * (c_first + x) + (x == 0 ? later : 0)) * kT8Part + j * kT8PartTile; };
-#pragma unroll 1
-                    for (int j = 0; j < 2; ++j) {
-                        int q;
-                        float top = -INFINITY, l = 0.0f;
-                        bool wild = false;
-                        for (int x = 0; x < parts; ++x) top = fmaxf(top, __ldcg(from(x, j) + 128 * kT8Rows + row));
-                        for (int x = 0; x < parts; ++x) {
-                            const float r = __ldcg(from(x, j) + 128 * kT8Rows + row), s = __ldcg(from(x, j) + 129 * kT8Rows + row);
-                            wild |= __float_as_uint(s) >> 31;
-                            l += fabsf(s) * (r == top ? 1.0f : tc_exp2(r - top));
-                        }
-                        uint32_t hit[4] = {0u, 0u, 0u, 0u};
-                        if (__any_sync(0xffffffffu, wild)) search(j, hit);
-                        if (!query(j, q)) continue;
-                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll 1
-                        for (int c = 0; c < HD; c += 32) {
-                            float y[32] = {};
-#pragma unroll 2
-                            for (int x = 0; x < parts; ++x) {
-                                const float r = __ldcg(from(x, j) + 128 * kT8Rows + row);
-                                const bool none = r == -INFINITY && __ldcg(from(x, j) + 129 * kT8Rows + row) == 0.0f;       // its O may never have been written
-                                if (none) continue;
-                                const float f = r == top ? 1.0f : tc_exp2(r - top);
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const float4 v = __ldcg(reinterpret_cast<const float4*>(from(x, j)) + (c / 4 + i) * kT8Rows + row);
-                                    y[4 * i] = fmaf(v.x, f, y[4 * i]); y[4 * i + 1] = fmaf(v.y, f, y[4 * i + 1]); y[4 * i + 2] = fmaf(v.z, f, y[4 * i + 2]); y[4 * i + 3] = fmaf(v.w, f, y[4 * i + 3]);
-                                }
-                            }
-                            store(j, c, y, inv, hit);
-                        }
-                    }
+                    t8_merge(p, it, row);
                 }
                 if (!together()) break;              // s_last has been read
             }
         }
     } else {   // ===== softmax: TMEM lane quadrant = warp % 4 =====
         const int j = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
-        const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_tmem = tmem + lanes + kT8S + 64 * j, q_tmem = tmem + lanes + kT8Q + 64 * j;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_tmem = tmem + lanes + kT8S + 64 * j, p_tmem = tmem + lanes + kT8P + 64 * j;
         const int q = j * p.queries + (row >> p.hpc_log2);
         T8Item more;
         uint32_t done = 0, items = 0;
@@ -757,90 +761,54 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             const bool live = it.listed(q);
             const int qpos = it.pos0 + (live ? q : it.hi), h = it.h0 + (row & (p.hpc - 1));
             const TileList tiles = tiles_of(it);
-            // ---- queries: fp16 in TMEM, brought to 1 .. 2 by a power of two of the row's largest; every score of the item before has been read ----
+            // ---- queries: fp16, brought to 1 .. 2 by a power of two of the row's largest; every score of the item before has been made ----
             float up;
             {
-                // A row is read by neighbouring lanes: once for its largest, once more for its terms, which go through shared memory to the row's own lane.
                 const long long mine = (long long)(it.tok0 + (live ? q : it.hi)) * a.ldq + (long long)h * a.dk;       // (a row without a query reads another)
-                auto rows_at = [&](auto& v, auto r_of, int col) {          // 16 bytes of a row of this warp's, for each of v
+                constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 8;       // lanes of a row, rows of a load, loads on their way
+                const int col = (lane % kLanes) * 4;
+                const uint32_t to = s_addr(sQ) + j * Sh::kQTile + (col / 64) * Sh::kQBlock + (col % 8) * 2;
+                int ex = 0;
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += kAhead * kPer) {
+                    float4 v[kAhead];
                     if (p.vec_q) {
 #pragma unroll
-                        for (int i = 0; i < (int)(sizeof(v) / 16); ++i) {
-                            const float* src = a.q + __shfl_sync(0xffffffffu, mine, r_of(i)) + col;
+                        for (int i = 0; i < kAhead; ++i) {
+                            const float* src = a.q + __shfl_sync(0xffffffffu, mine, r0 + i * kPer + lane / kLanes) + col;
                             v[i] = col < a.dk ? *reinterpret_cast<const float4*>(src) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < (int)(sizeof(v) / 16); ++i) {
-                            const float* src = a.q + __shfl_sync(0xffffffffu, mine, r_of(i)) + col;
-                            v[i] = col < a.dk ? make_float4(src[0], src[1], src[2], src[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        }
+                        for (int i = 0; i < kAhead; ++i) v[i] = t8_four(a.q + __shfl_sync(0xffffffffu, mine, r0 + i * kPer + lane / kLanes) + col, col < a.dk);
                     }
-                };
-                constexpr int kLanes = HD / 4, kPer = 32 / kLanes;         // lanes of a row, rows of a load
-                uint32_t top = 0;
-#pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += 16) {
-                    float4 v[16 / kPer];
-                    rows_at(v, [&](int i) { return r0 + i * kPer + lane / kLanes; }, (lane % kLanes) * 4);
 #pragma unroll
-                    for (int i = 0; i < 16 / kPer; ++i) {
+                    for (int i = 0; i < kAhead; ++i) {
+                        const int r = r0 + i * kPer + lane / kLanes, rr = quad * 32 + r;
                         uint32_t t = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu), max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
                         if constexpr (kPer == 1) {
                             t = __reduce_max_sync(0xffffffffu, t);
-                            if (lane == r0 + i) top = t;
                         } else {
 #pragma unroll
-                            for (int o = 1; o < 16; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
-                            const uint32_t first = __shfl_sync(0xffffffffu, t, 0), second = __shfl_sync(0xffffffffu, t, 16);
-                            if (lane == r0 + 2 * i) top = first;
-                            if (lane == r0 + 2 * i + 1) top = second;
+                            for (int o = 1; o < kLanes; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+                        }
+                        const int e = t < 0x7f800000u ? max((int)(t >> 23) - 127, -100) : 0;
+#pragma unroll
+                        for (int x = 0; x < kPer; ++x) {
+                            const int of = kPer == 1 ? e : __shfl_sync(0xffffffffu, e, x * kLanes);
+                            if (lane == r0 + i * kPer + x) ex = of;
+                        }
+                        const float down = kv8_pow2(-e), x0 = v[i].x * down, x1 = v[i].y * down, x2 = v[i].z * down, x3 = v[i].w * down;
+                        const uint32_t h0 = t8_pack(x0, x1), h1 = t8_pack(x2, x3), dst = to + rr * 128 + (((col % 64 / 8) ^ (rr & 7)) << 4);
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(dst), "r"(h0), "r"(h1) : "memory");
+                        if constexpr (kTerms == 2) {
+                            const float2 y0 = t8_unpack(h0), y1 = t8_unpack(h1);
+                            asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(dst + Sh::kQTerm), "r"(t8_pack(x0 - y0.x, x1 - y0.y)), "r"(t8_pack(x2 - y1.x, x3 - y1.y)) : "memory");
                         }
                     }
                 }
-                const int ex = top < 0x7f800000u ? max((int)(top >> 23) - 127, -100) : 0;
-                const float down = kv8_pow2(-ex);
                 up = kv8_pow2(ex);
-                if (items) tc_fence_after();
-#pragma unroll 1
-                for (int pair = 0; pair < HD / 64; ++pair) {
-                    const uint32_t place = s_addr(kTerms == 1 ? s_stage + (warp - 4) * 4096 : sQ + j * Sh::kQTile + pair * Sh::kQBlock + quad * 4096);      // 32 rows of 128 bytes, chunk i of row r at i ^ (r % 8)
-                    uint32_t lo[kTerms == 2 ? 32 : 1];
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        float4 v[8];
-                        rows_at(v, [&](int i) { return 4 * i + lane / 8; }, 64 * pair + 32 * half + (lane % 8) * 4);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int r = 4 * i + lane / 8;
-                            t8_sts(place + r * 128 + (((lane % 8) ^ (r & 7)) << 4), __float_as_uint(v[i].x), __float_as_uint(v[i].y), __float_as_uint(v[i].z), __float_as_uint(v[i].w));
-                        }
-                        __syncwarp();
-                        uint32_t hi[16];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint4 y = t8_lds(place + lane * 128 + ((i ^ (lane & 7)) << 4));
-                            const float x[4] = {__uint_as_float(y.x) * down, __uint_as_float(y.y) * down, __uint_as_float(y.z) * down, __uint_as_float(y.w) * down};
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                hi[2 * i + e] = t8_pack(x[2 * e], x[2 * e + 1]);
-                                if constexpr (kTerms == 2) {
-                                    const float2 z = t8_unpack(hi[2 * i + e]);
-                                    lo[16 * half + 2 * i + e] = t8_pack(x[2 * e] - z.x, x[2 * e + 1] - z.y);
-                                }
-                            }
-                        }
-                        tc_st16(q_tmem + 32 * pair + 16 * half, hi);
-                        __syncwarp();
-                    }
-                    if constexpr (kTerms == 2) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) t8_sts(place + lane * 128 + ((i ^ (lane & 7)) << 4), lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-                    }
-                }
-                tc_wait_st();
-                if constexpr (kTerms == 2) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                tc_fence_before();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mb_arrive(qready + j);
             }
             const int wnd = seq_row_window(qpos, a.window, a.chunk);
@@ -848,7 +816,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             float ref = -INFINITY, l = 0.0f;
             for (int kt = 0; kt < n; ++kt) {
                 const int key0 = tiles.tile_of(it.k0 + kt) * kT8Keys;
-                ok = tc_wait_warp(sfull + j, done & 1, gave_up, p.polls);
+                ok = t8_wait_warp(sfull + j, done & 1, gave_up, p.polls);
                 if (!ok) break;
                 ++done;
                 tc_fence_after();
@@ -862,6 +830,8 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 const bool all = __all_sync(0xffffffffu, !gone[0] && !gone[1] && key0 + kT8Keys - 1 <= qpos && (qpos - key0 < wnd || key0 + kT8Keys <= a.keep_first));
                 tc_arrived(s);
                 tc_arrived(s + 32);
+                tc_fence_before();
+                mb_arrive(sread + j);              // the next scores may be made
                 float f[2] = {known.ks[0] * mul, known.ks[1] * mul};
                 if (kOpts) {
                     if (a.softcap > 0.0f) {
@@ -934,6 +904,10 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         f[0] = f[1] = 1.0f;
                     }
                     const float nr = fmaxf(ref, ceilf(mx)), less = kt == 0 || nr == ref ? 1.0f : tc_exp2(ref - nr);
+                    // the product with the last weights has been made: their place is free, and their factors have been used
+                    if (done > 1) ok = t8_wait_warp(odone + j, (done - 2) & 1, gave_up, p.polls);
+                    if (!ok) break;
+                    tc_fence_after();
                     factor[j * kT8Rows + row] = less;
                     mb_arrive(factors + j);
                     l = kt == 0 ? 0.0f : l * less;
@@ -969,8 +943,8 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                                 if constexpr (kTerms == 2) lo[e] = far != 0.0f ? 0u : lo[e];
                             }
                         }
-                        tc_st16(s_tmem + 16 * x, hi);
-                        if constexpr (kTerms == 2) tc_st16(s_tmem + 32 + 16 * x, lo);
+                        tc_st16(p_tmem + 16 * x, hi);
+                        if constexpr (kTerms == 2) tc_st16(p_tmem + 32 + 16 * x, lo);
                         float s0, s1;
                         tc_split(sum, s0, s1);
                         l = fmaf(s0 + s1, tc_exp2(-ev[x] - far), l);         // without the value scale
@@ -981,7 +955,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 mb_arrive(pready + j);
             }
             if (!ok) break;
-            if (items) ok = tc_wait_warp(lread + j, (items - 1) & 1, gave_up, p.polls);
+            if (items) ok = t8_wait_warp(lread + j, (items - 1) & 1, gave_up, p.polls);
             if (!ok) break;
             s_ref[j * kT8Rows + row] = ref;
             s_sum[j * kT8Rows + row] = l;
