@@ -258,7 +258,6 @@ __device__ __forceinline__ bool t8_wait(uint64_t* bar, uint32_t parity, volatile
 __device__ __forceinline__ bool t8_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up, unsigned polls) {
     return __all_sync(0xffffffffu, t8_wait(bar, parity, gave_up, polls));
 }
-__device__ __noinline__ float4 t8_four(const float* x, bool take) { return take ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); }      // (an address of any alignment)
 // fp16 operands: the bf16 descriptor without its types
 __host__ __device__ constexpr uint32_t t8_idesc(int M, int N) { return umma_idesc_bf16(M, N) & ~((1u << 7) | (1u << 10)); }
 
@@ -764,42 +763,54 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             // ---- queries: fp16, brought to 1 .. 2 by a power of two of the row's largest; every score of the item before has been made ----
             float up;
             {
-                const long long mine = (long long)(it.tok0 + (live ? q : it.hi)) * a.ldq + (long long)h * a.dk;       // (a row without a query reads another)
-                constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 8;       // lanes of a row, rows of a load, loads on their way
-                const int col = (lane % kLanes) * 4;
-                const uint32_t to = s_addr(sQ) + j * Sh::kQTile + (col / 64) * Sh::kQBlock + (col % 8) * 2;
+                constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 16;       // lanes of a row, rows of a load, loads on their way
+                const int mine = it.tok0 + (live ? q : it.hi), col = (lane % kLanes) * 4, sub = lane / kLanes;      // (a row without a query reads another)
+                const float* src = a.q + (size_t)it.h0 * a.dk + col;
+                // row 8 i + r of a block lies 1024 i + 128 r further, its chunks exchanged by r
+                const uint32_t to = s_addr(sQ) + j * Sh::kQTile + (col / 64) * Sh::kQBlock + quad * 4096 + (col % 8) * 2, chunk = col % 64 / 8;
+                const bool take = col < a.dk;
                 int ex = 0;
 #pragma unroll 1
                 for (int r0 = 0; r0 < 32; r0 += kAhead * kPer) {
                     float4 v[kAhead];
+                    auto address = [&](int i) {
+                        const int r = i * kPer + sub;
+                        return src + (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, r0 + r) * (uint32_t)a.ldq + (uint32_t)((r & (p.hpc - 1)) * a.dk);
+                    };
                     if (p.vec_q) {
 #pragma unroll
                         for (int i = 0; i < kAhead; ++i) {
-                            const float* src = a.q + __shfl_sync(0xffffffffu, mine, r0 + i * kPer + lane / kLanes) + col;
-                            v[i] = col < a.dk ? *reinterpret_cast<const float4*>(src) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            const float* at = address(i);
+                            v[i] = take ? *reinterpret_cast<const float4*>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < kAhead; ++i) v[i] = t8_four(a.q + __shfl_sync(0xffffffffu, mine, r0 + i * kPer + lane / kLanes) + col, col < a.dk);
+                        for (int i = 0; i < kAhead; ++i) {
+                            const float* at = address(i);
+                            v[i] = take ? make_float4(at[0], at[1], at[2], at[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < kAhead; ++i) {
-                        const int r = r0 + i * kPer + lane / kLanes, rr = quad * 32 + r;
-                        uint32_t t = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu), max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
+                        const int r = i * kPer + sub;
+                        uint32_t t = __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
                         if constexpr (kPer == 1) {
                             t = __reduce_max_sync(0xffffffffu, t);
                         } else {
 #pragma unroll
                             for (int o = 1; o < kLanes; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
                         }
-                        const int e = t < 0x7f800000u ? max((int)(t >> 23) - 127, -100) : 0;
-#pragma unroll
-                        for (int x = 0; x < kPer; ++x) {
-                            const int of = kPer == 1 ? e : __shfl_sync(0xffffffffu, e, x * kLanes);
-                            if (lane == r0 + i * kPer + x) ex = of;
+                        int e = max((int)(t >> 23), 27);           // exponent + 127, 27 at least: the reciprocal stays a normal number
+                        if (e == 255) e = 127;                     // an infinity among them
+                        if constexpr (kPer == 1) {
+                            if (lane == r0 + i) ex = e;
+                        } else {
+                            const int e0 = __shfl_sync(0xffffffffu, e, 0), e1 = __shfl_sync(0xffffffffu, e, 16);
+                            if (lane == r0 + 2 * i) ex = e0;
+                            if (lane == r0 + 2 * i + 1) ex = e1;
                         }
-                        const float down = kv8_pow2(-e), x0 = v[i].x * down, x1 = v[i].y * down, x2 = v[i].z * down, x3 = v[i].w * down;
-                        const uint32_t h0 = t8_pack(x0, x1), h1 = t8_pack(x2, x3), dst = to + rr * 128 + (((col % 64 / 8) ^ (rr & 7)) << 4);
+                        const float down = __uint_as_float((uint32_t)(254 - e) << 23), x0 = v[i].x * down, x1 = v[i].y * down, x2 = v[i].z * down, x3 = v[i].w * down;
+                        const uint32_t h0 = t8_pack(x0, x1), h1 = t8_pack(x2, x3), dst = to + (r0 + r) * 128 + ((chunk ^ (r & 7)) << 4);
                         asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(dst), "r"(h0), "r"(h1) : "memory");
                         if constexpr (kTerms == 2) {
                             const float2 y0 = t8_unpack(h0), y1 = t8_unpack(h1);
@@ -807,9 +818,19 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         }
                     }
                 }
-                up = kv8_pow2(ex);
+                up = __uint_as_float((uint32_t)ex << 23);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mb_arrive(qready + j);
+                // the next item's queries come into the L2 meanwhile: each lane asks for a row's
+                if (n_item + 1 < min(w.count, kT8Items)) {
+                    const T8Item& after = s_items[n_item + 1];
+                    if (after.k1 > 0 && after.keys[j] > 0) {
+                        const char* at = reinterpret_cast<const char*>(a.q + (size_t)(after.tok0 + (after.listed(q) ? q : after.hi)) * a.ldq + (size_t)(after.h0 + (row & (p.hpc - 1))) * a.dk);
+#pragma unroll
+                        for (int c = 0; c < HD * 4; c += 128)
+                            if (c < a.dk * 4) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + c));
+                    }
+                }
             }
             const int wnd = seq_row_window(qpos, a.window, a.chunk);
             const float slope = kOpts && a.slopes ? a.slopes[h] : 0.0f, mul = a.scale * up * (kOpts ? 1.0f : kTcLog2e);
@@ -834,42 +855,45 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 mb_arrive(sread + j);              // the next scores may be made
                 float f[2] = {known.ks[0] * mul, known.ks[1] * mul};
                 if (kOpts) {
-                    if (a.softcap > 0.0f) {
+                    if (a.softcap > 0.0f) {        // s becomes what times f is the capped score
                         const float inv[2] = {f[0] / a.softcap, f[1] / a.softcap};
-                        float most = 0.0f;
+                        float most[2];
 #pragma unroll
-                        for (int e = 0; e < 64; e += 2) {
-                            const float x = __uint_as_float(s[e]) * inv[e / 32], y = __uint_as_float(s[e + 1]) * inv[e / 32];
-                            s[e] = __float_as_uint(x);
-                            s[e + 1] = __float_as_uint(y);
-                            most = tc_max3(most, fabsf(x), fabsf(y));
+                        for (int x = 0; x < 2; ++x) {
+                            float t0 = 0.0f, t1 = 0.0f;
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                t0 = tc_max3(t0, fabsf(__uint_as_float(s[32 * x + e])), fabsf(__uint_as_float(s[32 * x + e + 1])));
+                                t1 = tc_max3(t1, fabsf(__uint_as_float(s[32 * x + e + 2])), fabsf(__uint_as_float(s[32 * x + e + 3])));
+                            }
+                            most[x] = fmaxf(t0, t1);
                         }
                         // scores within a quarter of the cap, as nearly all are: the series that tc_tanh takes for them, two at a time
-                        if (__any_sync(0xffffffffu, most >= 0.25f)) {
+                        if (__any_sync(0xffffffffu, fmaxf(most[0] * inv[0], most[1] * inv[1]) >= 0.25f)) {
+                            const float back[2] = {a.softcap / f[0], a.softcap / f[1]};
 #pragma unroll
-                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(a.softcap * tc_tanh(__uint_as_float(s[e])));
+                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(back[e / 32] * tc_tanh(__uint_as_float(s[e]) * inv[e / 32]));
                         } else {
                             auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
-                            const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), one = both(1.0f), cap2 = both(a.softcap);
+                            const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), one = both(1.0f);
 #pragma unroll
                             for (int e = 0; e < 64; e += 2) {
-                                const uint64_t x = tc_two(s[e], s[e + 1]), x2 = tc_mul2(x, x);
+                                const uint64_t v = tc_two(s[e], s[e + 1]), x = tc_mul2(v, both(inv[e / 32])), x2 = tc_mul2(x, x);
                                 float y, z;
-                                tc_split(tc_mul2(cap2, tc_mul2(x, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, c4, c3), c2), c1), one))), y, z);
+                                tc_split(tc_mul2(v, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, c4, c3), c2), c1), one)), y, z);
                                 s[e] = __float_as_uint(y);
                                 s[e + 1] = __float_as_uint(z);
                             }
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f[e / 32]);
                     }
                     if (a.slopes) {
                         const float dist = (float)(qpos - key0);
 #pragma unroll
-                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(fmaf(-slope, dist - (float)e, __uint_as_float(s[e])));
+                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(fmaf(-slope, dist - (float)e, __uint_as_float(s[e]) * f[e / 32]));
+                        f[0] = f[1] = 1.0f;
                     }
-                    f[0] = f[1] = kTcLog2e;
+                    f[0] *= kTcLog2e;
+                    f[1] *= kTcLog2e;
                 }
                 if (!all) {        // the columns this row sees, as bits
                     const int hi = qpos - key0, lo = wnd > qpos ? -1 : qpos - wnd - key0, keep = a.keep_first - key0;
@@ -885,23 +909,36 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     float top[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float m0 = -INFINITY, m1 = -INFINITY;
+                        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
-                            m0 = tc_max3(m0, __uint_as_float(s[32 * x + e]), __uint_as_float(s[32 * x + e + 1]));
-                            m1 = tc_max3(m1, __uint_as_float(s[32 * x + e + 2]), __uint_as_float(s[32 * x + e + 3]));
+                            t0 = tc_max3(t0, __uint_as_float(s[32 * x + e]), __uint_as_float(s[32 * x + e + 1]));
+                            t1 = tc_max3(t1, __uint_as_float(s[32 * x + e + 2]), __uint_as_float(s[32 * x + e + 3]));
                         }
-                        top[x] = fmaxf(m0, m1);
+                        top[x] = fmaxf(t0, t1);
                     }
-                    float mx = fmaxf(fmaf(top[0], f[0], ev[0]), fmaf(top[1], f[1], ev[1]));
-                    // Scores so large that a rounded product and one inside a multiply-add are far apart: every product is rounded, so that no weight is above 1
-                    if (__any_sync(0xffffffffu, fabsf(mx) > 65536.0f && mx != -INFINITY)) {
+                    const float m0 = fmaf(top[0], f[0], ev[0]), m1 = fmaf(top[1], f[1], ev[1]);
+                    float mx = fmaxf(m0, m1);
+                    // Rare, with one vote for both: scores so large that a rounded product and one inside a multiply-add are far apart (every product is rounded then, so that no weight is
+                    // above 1), and a block whose weights come out below 2^-60 because its value scale is that much smaller than others' (`far`).
+                    float far[2] = {0.0f, 0.0f};
+                    const bool rare = __any_sync(0xffffffffu, fabsf(mx) > 65536.0f ? mx != -INFINITY : fminf(m0, m1) < fmaxf(ref, mx) - 60.0f);
+                    if (rare) {
+                        if (__any_sync(0xffffffffu, fabsf(mx) > 65536.0f && mx != -INFINITY)) {
 #pragma unroll
-                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f[e / 32]);
-                        mx = fmaxf(__fadd_rn(__fmul_rn(top[0], f[0]), ev[0]), __fadd_rn(__fmul_rn(top[1], f[1]), ev[1]));
-                        top[0] *= f[0];
-                        top[1] *= f[1];
-                        f[0] = f[1] = 1.0f;
+                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f[e / 32]);
+                            top[0] *= f[0];
+                            top[1] *= f[1];
+                            f[0] = f[1] = 1.0f;
+                            mx = fmaxf(__fadd_rn(top[0], ev[0]), __fadd_rn(top[1], ev[1]));
+                        }
+                        // Nothing to O, but the denominator has their weights without the scale: they are taken 2^far larger, so that they do not vanish.
+                        const float base = fmaxf(ref, ceilf(mx));
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float most = fmaf(top[x], f[x], ev[x]) - base;
+                            far[x] = most < -60.0f && most > -1e6f ? floorf(-most) : 0.0f;
+                        }
                     }
                     const float nr = fmaxf(ref, ceilf(mx)), less = kt == 0 || nr == ref ? 1.0f : tc_exp2(ref - nr);
                     // the product with the last weights has been made: their place is free, and their factors have been used
@@ -916,10 +953,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     const float base = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        // A block whose weights come out below 2^-60 because its value scale is that much smaller than others': nothing to O, but the denominator has its weights without the
-                        // scale. They are taken 2^far larger, so that they do not vanish.
-                        const float most = fmaf(top[x], f[x], ev[x]) - base, far = most < -60.0f && most > -1e6f ? floorf(-most) : 0.0f;
-                        const float neg = ev[x] - base + far;
+                        const float neg = ev[x] - base + far[x];
                         const uint64_t f2 = tc_two(__float_as_uint(f[x]), __float_as_uint(f[x])), neg2 = tc_two(__float_as_uint(neg), __float_as_uint(neg));
                         uint64_t sum = 0;
                         uint32_t hi[16], lo[16];
@@ -936,18 +970,18 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                                 lo[e] = t8_pack(y - u.x, z - u.y);
                             }
                         }
-                        if (__any_sync(0xffffffffu, far != 0.0f)) {
+                        if (rare) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
-                                hi[e] = far != 0.0f ? 0u : hi[e];
-                                if constexpr (kTerms == 2) lo[e] = far != 0.0f ? 0u : lo[e];
+                                hi[e] = far[x] != 0.0f ? 0u : hi[e];
+                                if constexpr (kTerms == 2) lo[e] = far[x] != 0.0f ? 0u : lo[e];
                             }
                         }
                         tc_st16(p_tmem + 16 * x, hi);
                         if constexpr (kTerms == 2) tc_st16(p_tmem + 32 + 16 * x, lo);
                         float s0, s1;
                         tc_split(sum, s0, s1);
-                        l = fmaf(s0 + s1, tc_exp2(-ev[x] - far), l);         // without the value scale
+                        l = fmaf(s0 + s1, tc_exp2(-ev[x] - far[x]), l);         // without the value scale
                     }
                 }
                 tc_wait_st();

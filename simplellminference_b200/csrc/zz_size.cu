@@ -1,0 +1,1000 @@
+// csrc/seq_attn8_tc.cu — attention of prompt portions over the 8-bit paged cache on the 5th-generation tensor cores, heads of up to 128 columns.
+//
+// 128 rows = the query heads of a kv head (four, two or one) x 32, 64 or 128 neighbouring queries are a tile; a CTA has two tiles at a time, neighbours in the sequence (a run), that share
+// tiles of 64 keys and values. fp16 operands, since fp16 holds every e4m3 code: keys and values enter exactly, and block scales multiply scores and weights.
+//   warp 0 (one lane)   TMA producer: boxes of 32 rows of codes, looked up in the block table, into a ring;
+//   warps 2, 3          codes to fp16 rows in the 128B swizzle (keys K-major, values as they lie); value rows that the run must not see, and NaN codes among values, become zeros;
+//   warp 1 (one lane)   MMA issuer: S = Q K^T, O += P V with P read from TMEM; P has columns of its own, so that the next scores are made while the softmax takes its exponentials;
+//   warps 4-7, 8-11     softmax of tile 0 / 1: queries to fp16 once an item; then, a thread per row, maximum, weights and their sum of every key tile;
+//   warps 12-15         O of both tiles: rescaled where a maximum has grown, results written, parts of shared items put together.
+// Results in bf16 (kTerms = 1): queries and weights are one fp16 number each (2^-12 of a value on average less than the 2^-9 of the result's own rounding). Results in fp32 (kTerms = 2): both are
+// the sum of two (22 bits), and O is added to an fp32 copy of the CTA's own every kT8Flush tiles, because the tensor core truncates as it
+// accumulates.
+// Weights are relative to the largest of score + log2(value scale) so far, rounded up to a whole number: differences of exponents are exact then, and O is rescaled by powers of two, and
+// seldom. The denominator takes the value scale out again, block by block.
+// A value's NaN code must reach exactly the rows that see it, but 0 * NaN is NaN: the converters replace it and say so, and rows of such an item look for NaN among their keys' values
+// at the end.
+// Shares. A CTA per item would leave most SMs idle where few queries follow a long context. The key tiles of all items lie in one row, made by a small kernel in front from what the
+// device knows (contexts, listed tiles); every CTA takes an equal run of it. Items that a cut goes through leave O, reference and sum as parts for the one of their CTAs that is done last.
+#include <type_traits>
+
+#include "seq_attn8.cuh"
+#include "tcgen05.cuh"
+
+namespace sllm {
+
+constexpr int kT8Rows = 128, kT8Keys = 64, kT8Threads = 512;      // rows of a tile, keys of a tile
+constexpr int kT8Extra = 4, kT8Least = 4;       // key tiles that an item's beginning and end count for; key tiles of a CTA's share at least
+constexpr int kT8Flush = 16;
+constexpr int kT8Known = 16;                    // key tiles whose scales are kept at hand: more than the producer is ever ahead of the softmax (the rings' stages and two)
+constexpr uint32_t kT8Tmem = 512, kT8S = 0, kT8P = 128, kT8O = 256;           // columns: S0 S1 | P0 P1 | O0 O1
+
+struct T8Args {
+    Attn8Args a;
+    int hpc, hpc_log2, queries;          // query heads and queries of a tile: hpc * queries = 128
+    int sets;                            // head sets of a step: kv_heads * (group / hpc)
+    int vec_q;
+    const A8Plan* plan;
+    int* counters;
+    float* parts;
+    int32_t* status;
+    unsigned polls;
+};
+
+// ---- the plan: which runs of 2 * queries neighbouring queries have listed tiles, and how many key tiles each ----
+// One CTA. Tiles of one query are the other kernel's.
+__global__ void __launch_bounds__(1024) seq_attention8_plan_kernel(Attn8Args p, int width, A8Plan* plan) {
+    after_previous();
+    const sllm_seq_batch& b = p.b;
+    __shared__ int s_base[kA8Segs + 1];
+    __shared__ int s_warp[32];
+    constexpr int kFew = 640;
+    __shared__ uint32_t s_mask[kFew * 8];
+    __shared__ int s_seg[kFew], s_first[kFew];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto scan = [&](int v, int& total) {         // exclusive sum over the CTA
+        int upto = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        __syncthreads();
+        if (lane == 31) s_warp[warp] = upto;
+        __syncthreads();
+        int before = 0;
+        total = 0;
+        for (int w = 0; w < 32; ++w) {
+            if (w < warp) before += s_warp[w];
+            total += s_warp[w];
+        }
+        return before + upto - v;
+    };
+    int runs = 0;
+    for (int s0 = 0; s0 < b.nseg; s0 += 1024) {
+        const int s = s0 + threadIdx.x, len = s < b.nseg ? b.seg_len[s] : 0;
+        int total;
+        const int at = scan(len > 1 ? (len + width - 1) / width : 0, total);
+        if (s < b.nseg) s_base[s] = runs + at;
+        runs += total;
+    }
+    runs = min(runs, kA8Runs);                   // (the host has made sure)
+    const bool few = runs <= kFew;               // their masks fit shared memory
+    for (int i = threadIdx.x; i < runs * 8; i += 1024) {
+        if (few) s_mask[i] = 0; else plan->mask[i / 8][i % 8] = 0;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < b.nseg; i += 1024) {
+        const int len = b.seg_len[i], n = len > 1 ? (len + width - 1) / width : 0;
+        for (int r = 0; r < n && s_base[i] + r < runs; ++r) {
+            const int at = s_base[i] + r;
+            if (few) { s_seg[at] = i; s_first[at] = r * width; } else { plan->seg[at] = i; plan->first[at] = r * width; }
+        }
+    }
+    for (int i = threadIdx.x; i < b.n_qtiles; i += 1024) {
+        const int seg = b.qt_seg[i], off = b.qt_off[i], n = min(kBQ, b.seg_len[seg] - off);
+        if (n <= 1 || off < 0) continue;
+        for (int q = off; q < off + n;) {        // a word of a run's mask at a time
+            const int run = s_base[seg] + q / width, bit = q % width, count = min(off + n - q, 32 - bit % 32);
+            if (run < runs) atomicOr(few ? &s_mask[run * 8 + bit / 32] : &plan->mask[run][bit / 32], (count == 32 ? 0xffffffffu : (1u << count) - 1) << (bit % 32));
+            q += count;
+        }
+    }
+    __syncthreads();
+    __threadfence_block();
+    int all = 0, kept = 0;
+    for (int r0 = 0; r0 < runs; r0 += 1024) {
+        const int r = r0 + threadIdx.x;
+        int units = 0, seg = 0, first = 0;
+        uint32_t m[8];
+        if (r < runs) {
+            int lo = -1, hi = -1;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                m[w] = few ? s_mask[r * 8 + w] : *reinterpret_cast<volatile uint32_t*>(&plan->mask[r][w]);
+                if (!m[w]) continue;
+                if (lo < 0) lo = 32 * w + __ffs(m[w]) - 1;
+                hi = 32 * w + 31 - __clz(m[w]);
+            }
+            seg = few ? s_seg[r] : plan->seg[r];
+            first = few ? s_first[r] : plan->first[r];
+            const int pos0 = b.seg_pos0[seg] + first;
+            if (lo >= 0 && pos0 >= 0) units = TileList(pos0 + lo, pos0 + hi, seq_row_window(pos0 + lo, p.window, p.chunk), p.keep_first, kT8Keys).n + kT8Extra;
+        }
+        int total, kept_here;
+        const int at = scan(units, total), to = kept + scan(units > 0, kept_here);      // (behind its barriers every run of this round has been read)
+        if (units > 0) {                         // a run without listed tiles is left out
+            plan->before[to] = all + at;
+            plan->seg[to] = seg;
+            plan->first[to] = first;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) plan->mask[to][w] = m[w];
+        }
+        all += total;
+        kept += kept_here;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        plan->before[kept] = all;
+        plan->runs = kept;
+    }
+}
+
+// An item of a CTA's share, as all its roles see it.
+struct T8Item {
+    int k0, k1, n;                           // its key tiles that are this CTA's, of so many
+    int tok0, pos0, slot, gkv, h0;           // first token and position of the run; kv head, first query head
+    int lo, hi;                              // first and last listed query of the run
+    int keys[2];                             // how many of k0 .. k1 either tile has to see: those up to its last listed query's
+    int first_cta, parts, slot_of, later;    // the CTAs that share it; which of this CTA's two places its part takes, and the first CTA's
+    uint32_t m[8];                           // listed queries
+    __device__ __forceinline__ bool listed(int q) const { return m[q >> 5] >> (q & 31) & 1; }
+};
+constexpr int kT8Items = 48;                 // of a share, kept in shared memory; the ones behind are worked out where they are needed
+
+// A CTA's share of the row of all key tiles: items first_item, first_item + 1, ... of the step (run by run, head set by head set)
+struct T8Share {
+    const T8Args& p;
+    long long total, begin, end;
+    int ctas, first_item, count;
+    __device__ __forceinline__ long long share(int c) const { return (long long)c * total / ctas; }
+    __device__ __forceinline__ int owner(long long v) const { return (int)(((v + 1) * ctas - 1) / total); }
+    __device__ __forceinline__ T8Share(const T8Args& args, int n_ctas, long long all) : p(args), total(all), ctas(n_ctas) {
+        begin = share(blockIdx.x);
+        end = share(blockIdx.x + 1);
+    }
+    __device__ __forceinline__ int item_of(long long u) const {          // the item that unit u (beginnings counted) belongs to
+        int lo = 0, hi = p.plan->runs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if ((long long)p.plan->before[mid] * p.sets <= u) lo = mid; else hi = mid;
+        }
+        const int b0 = p.plan->before[lo], each = p.plan->before[lo + 1] - b0;
+        return lo * p.sets + (int)((u - (long long)b0 * p.sets) / each);
+    }
+    __device__ __noinline__ void work_out(int i, T8Item& it) const {     // k1 <= 0: the share ends before its first tile
+        const int x = (first_item + i) / p.sets, y = (first_item + i) % p.sets;
+        const int b0 = p.plan->before[x], each = p.plan->before[x + 1] - b0;
+        const long long item0 = (long long)b0 * p.sets + (long long)y * each + kT8Extra;
+        it.n = each - kT8Extra;
+        it.k0 = (int)max(0ll, begin - item0);
+        it.k1 = (int)(min(end, item0 + it.n) - item0);
+        const sllm_seq_batch& b = p.a.b;
+        const int seg = p.plan->seg[x], first = p.plan->first[x], group = p.a.heads / p.a.kv_heads, per = group / p.hpc;
+        it.tok0 = b.seg_start[seg] + first;
+        it.pos0 = b.seg_pos0[seg] + first;
+        it.slot = b.seg_slot[seg];
+        it.gkv = y / per;
+        it.h0 = it.gkv * group + y % per * p.hpc;
+        it.lo = it.hi = -1;
+        int last[2] = {-1, -1};
+        for (int w = 0; w < 8; ++w) {
+            it.m[w] = p.plan->mask[x][w];
+            if (!it.m[w]) continue;
+            if (it.lo < 0) it.lo = 32 * w + __ffs(it.m[w]) - 1;
+            it.hi = 32 * w + 31 - __clz(it.m[w]);
+            last[32 * w >= p.queries] = it.hi;
+        }
+        for (int j = 0; j < 2; ++j) {
+            const int n = last[j] < 0 ? 0 : it.n - ((it.pos0 + it.hi) / kT8Keys - (it.pos0 + last[j]) / kT8Keys);
+            it.keys[j] = max(0, min(it.k1, n) - it.k0);
+        }
+        it.first_cta = owner(item0);
+        it.parts = owner(item0 + it.n - 1) - it.first_cta + 1;
+        it.slot_of = begin >= item0 ? 0 : 1;
+        it.later = share(it.first_cta) < item0;
+    }
+};
+
+template <int HD, int kTerms>
+struct T8Shape {
+    static constexpr int kBlocks = HD / 64, kK = 2, kV = kTerms == 1 ? 2 : 1, kRaw = kTerms == 1 ? 4 : 2;      // stages of keys, of values, of codes
+    static constexpr int kBlock = kT8Keys * 128, kTile = kBlocks * kBlock;    // fp16: 64 columns of all keys; all columns
+    static constexpr int kCodes = kT8Keys * HD;                              // bytes of a tile of codes
+    static constexpr int kQBlock = kT8Rows * 128, kQTerm = kBlocks * kQBlock, kQTile = kTerms * kQTerm;
+    static constexpr int kItems = (kT8Items * (int)sizeof(T8Item) + 127) / 128 * 128;
+    static constexpr int kSmem = 1024 + (kK + kV) * kTile + 2 * kRaw * kCodes + 2 * kQTile + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems;
+};
+constexpr int kT8PartTile = kT8Rows * (128 + 2), kT8Part = 2 * kT8PartTile;   // floats of a part: per tile O as [HD / 4][128][4], references, sums
+static_assert(kT8Part == kA8Part, "the workspace's parts");
+
+// what the producer knows of a key tile: per 32 keys the key scale, log2 of the value scale, the pool row (-1: no page)
+struct T8Tile { float ks[2], ev[2]; int row[2], pad[2]; };
+
+// pool row of 32 keys, or -1 where they have no page (or lie behind the last listed query)
+__device__ __forceinline__ int t8_row(const Attn8Args& p, int slot, int gkv, int key0, int last_pos) {
+    if (key0 > last_pos) return -1;
+    const int page = kv8_page(p.b, p.n_pages, slot, key0);
+    return page < 0 ? -1 : (page * p.kv_heads + gkv) * p.b.page_len + key0 % p.b.page_len;
+}
+__device__ __forceinline__ uint32_t t8_pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 t8_unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+// of a scale; exact for powers of two, as the append leaves them
+__device__ __forceinline__ float t8_log2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__uint_as_float((__float_as_uint(x) & 0x7fffffu) | 0x3f800000u)));
+    return y + (float)((int)(__float_as_uint(x) >> 23 & 0xff) - 127);
+}
+__device__ __forceinline__ uint4 t8_lds(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void t8_sts(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// The roles' code together has to stay near what the instruction caches hold (with everything in line it was 172 KB, and an item's beginning took 14000 clocks): what is seldom run is a function.
+__device__ __noinline__ bool t8_wait_long(uint64_t* bar, uint32_t parity, volatile int* gave_up, unsigned polls) { return tc_wait(bar, parity, gave_up, polls); }
+__device__ __forceinline__ bool t8_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, unsigned polls) {
+    uint32_t done = 0;
+    if (polls)
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(s_addr(bar)), "r"(parity) : "memory");
+    return done || t8_wait_long(bar, parity, gave_up, polls);
+}
+__device__ __forceinline__ bool t8_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up, unsigned polls) {
+    return __all_sync(0xffffffffu, t8_wait(bar, parity, gave_up, polls));
+}
+__device__ __noinline__ float4 t8_four(const float* x, bool take) { return take ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); }      // (an address of any alignment)
+// fp16 operands: the bf16 descriptor without its types
+__host__ __device__ constexpr uint32_t t8_idesc(int M, int N) { return umma_idesc_bf16(M, N) & ~((1u << 7) | (1u << 10)); }
+
+// Where the result of a row of tile j goes, or whether it has none
+struct T8Out { float* out; uint16_t* out16; bool listed, wide; };
+__device__ __forceinline__ T8Out t8_out(const T8Args& p, const T8Item& it, int j, int row) {
+    const Attn8Args& a = p.a;
+    const int q = j * p.queries + (row >> p.hpc_log2), h = it.h0 + (row & (p.hpc - 1));
+    const size_t t = it.tok0 + q;
+    T8Out r{a.out ? a.out + t * a.ldo + (size_t)h * a.dv : nullptr, a.out16 ? a.out16 + (t * a.heads + h) * a.dv : nullptr, it.listed(q), false};
+    r.wide = ((reinterpret_cast<uintptr_t>(r.out) | reinterpret_cast<uintptr_t>(r.out16)) & 15) == 0;
+    return r;
+}
+__device__ __noinline__ void t8_store_narrow(float* out, uint16_t* out16, float4 x, float4 y) {
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (out) out[e] = v[e];
+        if (out16) out16[e] = f32_to_bf16_bits(v[e]);
+    }
+}
+// eight columns
+__device__ __forceinline__ void t8_store(const T8Out& to, int c, float4 x, float4 y) {
+    if (!to.wide) {
+        t8_store_narrow(to.out ? to.out + c : nullptr, to.out16 ? to.out16 + c : nullptr, x, y);
+        return;
+    }
+    if (to.out) {
+        *reinterpret_cast<float4*>(to.out + c) = x;
+        *reinterpret_cast<float4*>(to.out + c + 4) = y;
+    }
+    if (to.out16) *reinterpret_cast<uint4*>(to.out16 + c) = make_uint4(tc_pack(x.x, x.y), tc_pack(x.z, x.w), tc_pack(y.x, y.y), tc_pack(y.z, y.w));
+}
+// Rare: a row whose keys' values may hold NaN codes has its result; it becomes NaN in the columns where one of the values that it sees is.
+__device__ __noinline__ void t8_poison(const T8Args& p, const T8Item& it, int j, int row) {
+    const Attn8Args& a = p.a;
+    const T8Out to = t8_out(p, it, j, row);
+    if (!to.listed) return;
+    const int pos = it.pos0 + j * p.queries + (row >> p.hpc_log2), wnd = seq_row_window(pos, a.window, a.chunk);
+    const TileList mine(pos, pos, wnd, a.keep_first, kKv8Block);
+    for (int x = 0; x < mine.n; ++x) {
+        const int key0 = mine.tile_of(x) * kKv8Block, r = t8_row(a, it.slot, it.gkv, key0, pos);
+        if (r < 0) continue;
+        for (int e = 0; e < kKv8Block; ++e) {
+            if (!seq_sees(pos, key0 + e, wnd, a.keep_first)) continue;
+            const uint8_t* v = a.v_pool + (size_t)(r + e) * a.dv;
+            for (int c = 0; c < a.dv; ++c) {
+                if ((v[c] & 0x7f) != 0x7f) continue;
+                if (to.out) to.out[c] = __int_as_float(0x7fffffff);
+                if (to.out16) to.out16[c] = 0x7fff;
+            }
+        }
+    }
+}
+// An item whose parts are all there, row `row` of both tiles: its parts brought to one reference and added, in the order of the key tiles.
+__device__ __noinline__ void t8_merge(const T8Args& p, const T8Item& it, int row) {
+    const int parts = it.parts;
+#pragma unroll 1
+    for (int j = 0; j < 2; ++j) {
+        const float* first = p.parts + (size_t)(2 * it.first_cta + it.later) * kT8Part + j * kT8PartTile;
+        const float* rest = p.parts + (size_t)(2 * it.first_cta) * kT8Part + j * kT8PartTile;
+        auto from = [&](int x) { return x == 0 ? first : rest + (size_t)(2 * x) * kT8Part; };
+        float top = -INFINITY, l = 0.0f;
+        bool wild = false;
+#pragma unroll 4
+        for (int x = 0; x < parts; ++x) top = fmaxf(top, __ldcg(from(x) + 128 * kT8Rows + row));
+#pragma unroll 4
+        for (int x = 0; x < parts; ++x) {
+            const float r = __ldcg(from(x) + 128 * kT8Rows + row), s = __ldcg(from(x) + 129 * kT8Rows + row);
+            wild |= __float_as_uint(s) >> 31;
+            l += fabsf(s) * (r == top ? 1.0f : tc_exp2(r - top));
+        }
+        const T8Out to = t8_out(p, it, j, row);
+        if (!to.listed) continue;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (int c = 0; c < p.a.dv; c += 16) {
+            float4 y[4] = {};
+#pragma unroll 2
+            for (int x = 0; x < parts; ++x) {
+                const float r = __ldcg(from(x) + 128 * kT8Rows + row);
+                if (r == -INFINITY && __ldcg(from(x) + 129 * kT8Rows + row) == 0.0f) continue;       // none of this part's keys is visible: its O may never have been written
+                const float f = r == top ? 1.0f : tc_exp2(r - top);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(from(x)) + (c / 4 + i) * kT8Rows + row);
+                    y[i].x = fmaf(v.x, f, y[i].x); y[i].y = fmaf(v.y, f, y[i].y); y[i].z = fmaf(v.z, f, y[i].z); y[i].w = fmaf(v.w, f, y[i].w);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = make_float4(y[i].x * inv, y[i].y * inv, y[i].z * inv, y[i].w * inv);
+            t8_store(to, c, y[0], y[1]);
+            t8_store(to, c + 8, y[2], y[3]);
+        }
+        if (wild) t8_poison(p, it, j, row);
+    }
+}
+
+template <int HD, int kTerms, bool kOpts>
+__global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ T8Args p) {
+    using Sh = T8Shape<HD, kTerms>;
+    constexpr int SK = Sh::kK, SV = Sh::kV, RS = Sh::kRaw;
+    extern __shared__ uint8_t t8_smem[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(t8_smem) + 1023) & ~(uintptr_t)1023);
+    uint8_t *sK = smem, *sV = sK + SK * Sh::kTile, *sQ = sV + SV * Sh::kTile, *sRaw = sQ + 2 * Sh::kQTile;      // sRaw: keys, then values, of each stage
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + 2 * RS * Sh::kCodes);
+    uint64_t *rfull = bars, *rempty = rfull + RS, *kfull = rempty + RS, *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV;
+    // per tile: queries written / scores written / scores read / factors for O written / weights written and O rescaled / product with the values done / sums written, and read
+    uint64_t *qready = vempty + SV, *sfull = qready + 2, *sread = sfull + 2, *factors = sread + 2, *pready = factors + 2, *odone = pready + 2, *lready = odone + 2, *lread = lready + 2;
+    uint64_t* meet = lread + 2;              // of warps 12-15
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet + 1);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* s_start = reinterpret_cast<int*>(tmem_slot + 2);                        // the first item and how many
+    int* s_last = reinterpret_cast<int*>(tmem_slot + 4);
+    volatile int* s_nan = reinterpret_cast<volatile int*>(tmem_slot + 5);        // [8]: at i % 8 the number (from 1) of an item that had NaN among its values; the converters are fewer items ahead
+    float* factor = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);        // [2][128]
+    float *s_ref = factor + 2 * kT8Rows, *s_sum = s_ref + 2 * kT8Rows;                        // [2][128] each
+    T8Tile* s_tile = reinterpret_cast<T8Tile*>(s_sum + 2 * kT8Rows);                           // [kT8Known]
+    T8Item* s_items = reinterpret_cast<T8Item*>(factor + 8 * kT8Rows);                         // [kT8Items]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Attn8Args& a = p.a;
+
+    if (warp == 0 && lane == 0) {
+        for (int i = 0; i < RS; ++i) { mb_init(rfull + i, 1); mb_init(rempty + i, 2); }
+        for (int i = 0; i < SK; ++i) { mb_init(kfull + i, 2); mb_init(kempty + i, 1); }
+        for (int i = 0; i < SV; ++i) { mb_init(vfull + i, 2); mb_init(vempty + i, 1); }
+        for (int j = 0; j < 2; ++j) {
+            mb_init(qready + j, 128); mb_init(sfull + j, 1); mb_init(sread + j, 128); mb_init(factors + j, 128); mb_init(pready + j, 256); mb_init(odone + j, 1); mb_init(lready + j, 128); mb_init(lread + j, 128);
+        }
+        *gave_up = 0;
+        for (int i = 0; i < 8; ++i) s_nan[i] = 0;
+        mb_init(meet, 128);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tc_alloc(tmem_slot, kT8Tmem);
+    after_previous();
+    // this CTA's share of the row of all key tiles, and its items
+    const long long total = (long long)p.plan->before[p.plan->runs] * p.sets;
+    const int ctas = (int)min((long long)gridDim.x, (total + kT8Least - 1) / kT8Least);
+    const bool work = (int)blockIdx.x < ctas;
+    T8Share w(p, ctas, total);
+    if (work && warp >= 2 && warp < 4) {
+        w.first_item = w.item_of(w.begin);
+        const int n = w.item_of(w.end - 1) - w.first_item + 1, i = threadIdx.x - 64;
+        if (i < min(n, kT8Items)) w.work_out(i, s_items[i]);
+        if (i == 0) { s_start[0] = w.first_item; s_start[1] = n; }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    w.first_item = s_start[0];
+    w.count = s_start[1];
+    // the i-th item, or false behind the last one (whose first tile the share may end before)
+    auto item_at = [&](int i, T8Item& more) -> const T8Item* {
+        if (i >= w.count) return nullptr;
+        const T8Item* it = s_items + i;
+        if (i >= kT8Items) {
+            w.work_out(i, more);
+            it = &more;
+        }
+        return it->k1 > 0 ? it : nullptr;
+    };
+    auto tiles_of = [&](const T8Item& it) { return TileList(it.pos0 + it.lo, it.pos0 + it.hi, seq_row_window(it.pos0 + it.lo, a.window, a.chunk), a.keep_first, kT8Keys); };
+
+    if (!work) {
+    } else if (warp == 0) {   // ===== TMA producer
+    } else if (warp == 1) {
+        if (elect_one()) {   // ===== MMA issuer =====
+            constexpr uint32_t idesc_s = t8_idesc(kT8Rows, kT8Keys), idesc_o = t8_idesc(kT8Rows, HD) | (1u << 16);      // B MN-major
+            const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, Sh::kBlock);     // + bytes / 16: another place
+            uint32_t made[2] = {0, 0}, done[2] = {0, 0}, items[2] = {0, 0};     // scores, products and items of either tile
+            auto scores = [&](int j, int g) {    // behind the softmax's reading of the ones before
+                if (made[j] && !t8_wait(sread + j, (made[j] - 1) & 1, gave_up, p.polls)) return false;
+                ++made[j];
+                tc_fence_after();
+                const uint64_t k = k_desc + (uint32_t)(g % SK) * (Sh::kTile / 16);
+#pragma unroll
+                for (int term = 0; term < kTerms; ++term) {
+                    const uint64_t q = q_desc + (uint32_t)j * (Sh::kQTile / 16) + (uint32_t)term * (Sh::kQTerm / 16);
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        tc_mma_bf16(tmem + kT8S + 64 * j, q + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kBlock / 16) + 2 * (ks % 4)), idesc_s,
+                                    term != 0 || ks != 0);
+                }
+                tc_commit(sfull + j);
+                return true;
+            };
+            auto values = [&](int j, int g, bool more) {
+                const uint64_t v = v_desc + (uint32_t)(g % SV) * (Sh::kTile / 16);
+#pragma unroll
+                for (int ks = 0; ks < kTerms * kT8Keys / 16; ++ks)       // first terms, then second ones, against the same values
+                    tc_mma_bf16_ts(tmem + kT8O + 128 * j, tmem + kT8P + 64 * j + 8 * ks, v + (uint32_t)((ks % (kT8Keys / 16)) * 128), idesc_o, more || ks != 0);
+                tc_commit(odone + j);
+            };
+            T8Item more;
+            int g = 0;                           // key tiles so far
+            bool ok = true;
+            for (int n_item = 0; ok; ++n_item) {
+                const T8Item* at = item_at(n_item, more);
+                if (!at) break;
+                const int n = at->k1 - at->k0, nkt[2] = {at->keys[0], at->keys[1]};
+                ok = t8_wait(kfull + g % SK, (uint32_t)(g / SK) & 1, gave_up, p.polls);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (ok && nkt[j]) ok = t8_wait(qready + j, items[j]++ & 1, gave_up, p.polls) && scores(j, g);
+                if (!ok) break;
+                tc_commit(kempty + g % SK);
+                for (int kt = 0; ok && kt < n; ++kt, ++g) {
+                    if (kt + 1 < n) ok = t8_wait(kfull + (g + 1) % SK, (uint32_t)((g + 1) / SK) & 1, gave_up, p.polls);
+                    // Either tile's next scores, then its product with these values: so the tiles come to lie half a step apart, and one's exponentials run during the other's products.
+                    bool values_there = false;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if (ok && kt + 1 < nkt[j]) ok = scores(j, g + 1);
+                        if (!ok || kt >= nkt[j]) continue;
+                        if (!values_there) ok = t8_wait(vfull + g % SV, (uint32_t)(g / SV) & 1, gave_up, p.polls);
+                        values_there = true;
+                        ok = ok && t8_wait(pready + j, done[j] & 1, gave_up, p.polls);
+                        if (!ok) continue;
+                        ++done[j];
+                        tc_fence_after();
+                        values(j, g, kTerms == 1 ? kt != 0 : kt % kT8Flush != 0);
+                    }
+                    if (!ok) break;
+                    tc_commit(vempty + g % SV);
+                    if (kt + 1 < n) tc_commit(kempty + (g + 1) % SK);
+                }
+            }
+        }
+    } else if (warp < 4) {   // ===== codes to fp16 =====
+        T8Item more;
+        int g = 0;
+        bool ok = true;
+        const int me = (warp - 2) * 32 + lane, r8 = me & 7, c0 = me >> 3;       // row of eight, first chunk: neighbouring lanes' chunks lie in different banks, read and written
+        constexpr int kChunks = HD / 16, kPer = 8 / kChunks;                    // chunks of a row; rows of eight that 64 threads take at a time: 1 or 2
+        // wild: rows that the run must not see become zeros, and NaN codes, which are reported
+        auto convert = [&](int key0, int last_pos, int x, const uint8_t* raw, uint8_t* tile, auto values_, auto wild_) {
+            constexpr bool values = decltype(values_)::value, wild = decltype(wild_)::value;
+            const uint32_t from = s_addr(raw), to = s_addr(tile);
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int r0 = 0; r0 < kT8Keys; r0 += 8 * kPer) {
+                const int row = r0 + r8 + 8 * (c0 / kChunks), chunk = c0 % kChunks;
+                uint4 v = t8_lds(from + row * HD + ((HD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
+                if (values) {
+                    const bool take = !wild || (key0 + row <= last_pos && s_tile[x % kT8Known].row[row >= kKv8Block] >= 0);
+                    auto look = [&](uint32_t y) {
+                        if (wild && !take) y = 0u;
+                        const uint32_t n = (y & 0x7f7f7f7fu) + 0x01010101u;                  // the top bit of every NaN
+                        any |= n;
+                        return wild ? y & ~(((n & 0x80808080u) >> 7) * 0xffu) : y;
+                    };
+                    v.x = look(v.x); v.y = look(v.y); v.z = look(v.z); v.w = look(v.w);
+                }
+                const uint32_t at = to + (chunk / 4) * Sh::kBlock + row * 128, c = (chunk % 4) * 2;
+                t8_sts(at + ((c ^ (row & 7)) << 4), kv8_half2(v.x & 0xffffu), kv8_half2(v.x >> 16), kv8_half2(v.y & 0xffffu), kv8_half2(v.y >> 16));
+                t8_sts(at + (((c + 1) ^ (row & 7)) << 4), kv8_half2(v.z & 0xffffu), kv8_half2(v.z >> 16), kv8_half2(v.w & 0xffffu), kv8_half2(v.w >> 16));
+            }
+            return __any_sync(0xffffffffu, any & 0x80808080u);
+        };
+        auto publish = [&]() {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        for (int n_item = 0; ok; ++n_item) {
+            const T8Item* at = item_at(n_item, more);
+            if (!at) break;
+            const TileList tiles = tiles_of(*at);
+            const int last_pos = at->pos0 + at->hi;
+            auto keys = [&](int x) {               // keys of this CTA's tile x
+                ok = t8_wait_warp(rfull + x % RS, (uint32_t)(x / RS) & 1, gave_up, p.polls) && t8_wait_warp(kempty + x % SK, ((uint32_t)(x / SK) & 1) ^ 1, gave_up, p.polls);
+                if (!ok) return;
+                convert(0, 0, 0, sRaw + 2 * (x % RS) * Sh::kCodes, sK + x % SK * Sh::kTile, std::false_type{}, std::false_type{});
+                publish();
+                if (lane == 0) mb_arrive(kfull + x % SK);
+            };
+            keys(g);
+            for (int k = at->k0, k1 = at->k1; ok && k < k1; ++k, ++g) {
+                const int s = g % RS, tv = g % SV, key0 = tiles.tile_of(k) * kT8Keys;
+                if (k + 1 < k1) keys(g + 1);       // a tile ahead of the values: the scores come first
+                if (!ok) break;
+                ok = t8_wait_warp(vempty + tv, ((uint32_t)(g / SV) & 1) ^ 1, gave_up, p.polls);
+                if (!ok) break;
+                const uint8_t* codes = sRaw + (2 * s + 1) * Sh::kCodes;
+                bool whole = key0 + kT8Keys - 1 <= last_pos && s_tile[g % kT8Known].row[0] >= 0 && s_tile[g % kT8Known].row[1] >= 0;
+                if (whole) whole = !convert(key0, last_pos, g, codes, sV + tv * Sh::kTile, std::true_type{}, std::false_type{});
+                if (!whole && convert(key0, last_pos, g, codes, sV + tv * Sh::kTile, std::true_type{}, std::true_type{})) {
+                    s_nan[n_item & 7] = n_item + 1;          // read behind the product with these values
+                    __threadfence_block();
+                }
+                publish();
+                if (lane == 0) { mb_arrive(vfull + tv); mb_arrive(rempty + s); }
+            }
+        }
+    } else if (warp >= 12) {   // ===== O of both tiles =====
+        const int quad = warp & 3, row = quad * 32 + lane;
+        T8Item more;
+        uint32_t done0 = 0, done1 = 0, items0 = 0, items1 = 0;
+        uint32_t met = 0;
+        bool ok = true;
+        for (int n_item = 0; ok; ++n_item) {
+            const T8Item* at = item_at(n_item, more);
+            if (!at) break;
+            const T8Item& it = *at;
+            const int n = it.k1 - it.k0, nkt[2] = {it.keys[0], it.keys[1]};
+            const bool whole = it.parts == 1;
+            float* part = p.parts + (size_t)(2 * blockIdx.x + it.slot_of) * kT8Part;
+            float since0 = 1.0f, since1 = 1.0f;                                // what the references have grown by since O was flushed
+            for (int kt = 0; ok && kt < n; ++kt)
+#pragma unroll 1
+                for (int j = 0; j < 2; ++j) {
+                    if (!ok || kt >= (j ? nkt[1] : nkt[0])) continue;
+                    float since = j ? since1 : since0;
+                    const uint32_t so_far = j ? done1 : done0;
+                    ok = t8_wait_warp(factors + j, so_far & 1, gave_up, p.polls);       // (the softmax has waited for the product before)
+                    if (ok && kt > 0) ok = t8_wait_warp(odone + j, (so_far - 1) & 1, gave_up, p.polls);
+                    if (!ok) continue;
+                    (j ? done1 : done0) = so_far + 1;
+                    tc_fence_after();
+                    const float f = factor[j * kT8Rows + row];
+                    const uint32_t o_tmem = tmem + ((uint32_t)(quad * 32) << 16) + kT8O + 128 * j;
+                    if (kTerms == 2 && kt > 0 && kt % kT8Flush == 0) {         // O so far, relative to the reference before this tile's
+                        uint4* acc = reinterpret_cast<uint4*>(part + j * kT8PartTile);
+                        const float s = kt > kT8Flush ? since : 0.0f;
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            uint4 v[8];
+                            tc_ld32_async(o_tmem + c, o);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v[i] = kt > kT8Flush ? acc[(c / 4 + i) * kT8Rows + row] : make_uint4(0u, 0u, 0u, 0u);
+                            tc_arrived(o);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                auto sum = [&](uint32_t x, uint32_t y) { return __float_as_uint(fmaf(__uint_as_float(x), s, __uint_as_float(y))); };
+                                acc[(c / 4 + i) * kT8Rows + row] = make_uint4(sum(v[i].x, o[4 * i]), sum(v[i].y, o[4 * i + 1]), sum(v[i].z, o[4 * i + 2]), sum(v[i].w, o[4 * i + 3]));
+                            }
+                        }
+                        since = f;
+                    } else {
+                        since *= f;
+                        if (kt > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+#pragma unroll 1
+                            for (int c = 0; c < HD; c += 32) {
+                                uint32_t o[32];
+                                tc_ld32_async(o_tmem + c, o);
+                                tc_arrived(o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tc_st32(o_tmem + c, o);
+                            }
+                            tc_wait_st();
+                        }
+                    }
+                    (j ? since1 : since0) = since;
+                    tc_fence_before();
+                    mb_arrive(pready + j);
+                }
+            if (!ok) break;
+            // ---- results, or this CTA's part of them ----
+#pragma unroll 1
+            for (int j = 0; ok && j < 2; ++j) {
+                const int mine = j ? nkt[1] : nkt[0];
+                const float since = j ? since1 : since0;
+                if (mine == 0) {
+                    if (!whole) {                                              // none of this part's keys is visible to this tile
+                        part[j * kT8PartTile + 128 * kT8Rows + row] = -INFINITY;
+                        part[j * kT8PartTile + 129 * kT8Rows + row] = 0.0f;
+                    }
+                    continue;
+                }
+                ok = t8_wait_warp(lready + j, (j ? items1 : items0) & 1, gave_up, p.polls) && t8_wait_warp(odone + j, ((j ? done1 : done0) - 1) & 1, gave_up, p.polls);
+                if (j) ++items1; else ++items0;
+                if (!ok) break;
+                tc_fence_after();
+                const float ref = s_ref[j * kT8Rows + row], l = s_sum[j * kT8Rows + row], inv = l == 0.0f ? 0.0f : 1.0f / l;
+                mb_arrive(lread + j);
+                const bool nan_here = s_nan[n_item & 7] == n_item + 1;         // (behind the last product: every value has been converted)
+                const uint32_t o_tmem = tmem + ((uint32_t)(quad * 32) << 16) + kT8O + 128 * j;
+                uint4* acc = reinterpret_cast<uint4*>(part + j * kT8PartTile);
+                const bool flushed = kTerms == 2 && mine > kT8Flush;
+                const T8Out to = t8_out(p, it, j, row);
+                const float f = whole ? inv : 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    tc_ld32_async(o_tmem + c, o);
+                    if (flushed) {
+                        uint4 v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = acc[(c / 4 + i) * kT8Rows + row];
+                        tc_arrived(o);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            auto sum = [&](uint32_t x, uint32_t& y) { y = __float_as_uint(fmaf(__uint_as_float(x), since, __uint_as_float(y))); };
+                            sum(v[i].x, o[4 * i]); sum(v[i].y, o[4 * i + 1]); sum(v[i].z, o[4 * i + 2]); sum(v[i].w, o[4 * i + 3]);
+                        }
+                    } else {
+                        tc_arrived(o);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        auto four = [&](int e) { return make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f); };
+                        const float4 x = four(i), y = four(i + 4);
+                        if (!whole) {
+                            reinterpret_cast<float4*>(acc)[((c + i) / 4) * kT8Rows + row] = x;
+                            reinterpret_cast<float4*>(acc)[((c + i) / 4 + 1) * kT8Rows + row] = y;
+                        } else if (to.listed && c + i < a.dv) {
+                            t8_store(to, c + i, x, y);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (whole && nan_here) t8_poison(p, it, j, row);
+                if (!whole) {
+                    part[j * kT8PartTile + 128 * kT8Rows + row] = ref;
+                    part[j * kT8PartTile + 129 * kT8Rows + row] = nan_here ? -l : l;      // (sums are not negative: the sign says that there was NaN)
+                }
+            }
+            if (!ok) break;
+            tc_fence_before();
+            if (!whole) {
+                const int c_first = it.first_cta, parts = it.parts;
+                auto together = [&]() {              // these four warps; a wait like the others, which ends
+                    mb_arrive(meet);
+                    ok = t8_wait_warp(meet, met++ & 1, gave_up, p.polls);
+                    return ok;
+                };
+                if (!together()) break;
+                if (threadIdx.x == 12 * 32) {        // what these warps have stored before the barrier comes before this, and what others have stored before theirs, before what follows
+                    int before_me;
+                    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before_me) : "l"(p.counters + c_first) : "memory");
+                    *s_last = before_me == parts - 1;
+                    if (before_me == parts - 1) p.counters[c_first] = 0;
+                }
+                if (!together()) break;
+                if (*s_last) {
+                    __threadfence();
+                    t8_merge(p, it, row);
+                }
+                if (!together()) break;              // s_last has been read
+            }
+        }
+    } else {   // ===== softmax: TMEM lane quadrant = warp % 4 =====
+        const int j = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_tmem = tmem + lanes + kT8S + 64 * j, p_tmem = tmem + lanes + kT8P + 64 * j;
+        const int q = j * p.queries + (row >> p.hpc_log2);
+        T8Item more;
+        uint32_t done = 0, items = 0;
+        int g0 = 0, g1 = 0;                      // key tiles of the CTA in front of this item, and of the next
+        bool ok = true;
+        for (int n_item = 0; ok; ++n_item) {
+            const T8Item* at = item_at(n_item, more);
+            if (!at) break;
+            const T8Item& it = *at;
+            const int n = it.keys[j];
+            g0 = g1;
+            g1 += it.k1 - it.k0;
+            if (n == 0) continue;
+            const bool live = it.listed(q);
+            const int qpos = it.pos0 + (live ? q : it.hi), h = it.h0 + (row & (p.hpc - 1));
+            const TileList tiles = tiles_of(it);
+            // ---- queries: fp16, brought to 1 .. 2 by a power of two of the row's largest; every score of the item before has been made ----
+            float up;
+            {
+                constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 8;        // lanes of a row, rows of a load, loads on their way
+                const int mine = it.tok0 + (live ? q : it.hi), col = (lane % kLanes) * 4, sub = lane / kLanes;      // (a row without a query reads another)
+                const float* src = a.q + (size_t)it.h0 * a.dk + col;
+                // row 8 i + r of a block lies 1024 i + 128 r further, its chunks exchanged by r
+                const uint32_t to = s_addr(sQ) + j * Sh::kQTile + (col / 64) * Sh::kQBlock + quad * 4096 + (col % 8) * 2, chunk = col % 64 / 8;
+                const bool take = col < a.dk;
+                int ex = 0;
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += kAhead * kPer) {
+                    float4 v[kAhead];
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) {
+                        const int r = i * kPer + sub;
+                        const float* at = src + (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, r0 + r) * (uint32_t)a.ldq + (uint32_t)((r & (p.hpc - 1)) * a.dk);
+                        if (p.vec_q) v[i] = take ? *reinterpret_cast<const float4*>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        else v[i] = t8_four(at, take);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) {
+                        const int r = i * kPer + sub;
+                        uint32_t t = __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+                        if constexpr (kPer == 1) {
+                            t = __reduce_max_sync(0xffffffffu, t);
+                        } else {
+#pragma unroll
+                            for (int o = 1; o < kLanes; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+                        }
+                        int e = max((int)(t >> 23), 27);           // exponent + 127, 27 at least: the reciprocal stays a normal number
+                        if (e == 255) e = 127;                     // an infinity among them
+                        if constexpr (kPer == 1) {
+                            if (lane == r0 + i) ex = e;
+                        } else {
+                            const int e0 = __shfl_sync(0xffffffffu, e, 0), e1 = __shfl_sync(0xffffffffu, e, 16);
+                            if (lane == r0 + 2 * i) ex = e0;
+                            if (lane == r0 + 2 * i + 1) ex = e1;
+                        }
+                        const float down = __uint_as_float((uint32_t)(254 - e) << 23), x0 = v[i].x * down, x1 = v[i].y * down, x2 = v[i].z * down, x3 = v[i].w * down;
+                        const uint32_t h0 = t8_pack(x0, x1), h1 = t8_pack(x2, x3), dst = to + (r0 + r) * 128 + ((chunk ^ (r & 7)) << 4);
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(dst), "r"(h0), "r"(h1) : "memory");
+                        if constexpr (kTerms == 2) {
+                            const float2 y0 = t8_unpack(h0), y1 = t8_unpack(h1);
+                            asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(dst + Sh::kQTerm), "r"(t8_pack(x0 - y0.x, x1 - y0.y)), "r"(t8_pack(x2 - y1.x, x3 - y1.y)) : "memory");
+                        }
+                    }
+                }
+                up = __uint_as_float((uint32_t)ex << 23);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mb_arrive(qready + j);
+            }
+            const int wnd = seq_row_window(qpos, a.window, a.chunk);
+            const float slope = kOpts && a.slopes ? a.slopes[h] : 0.0f, mul = a.scale * up * (kOpts ? 1.0f : kTcLog2e);
+            float ref = -INFINITY, l = 0.0f;
+            for (int kt = 0; kt < n; ++kt) {
+                const int key0 = tiles.tile_of(it.k0 + kt) * kT8Keys;
+                ok = t8_wait_warp(sfull + j, done & 1, gave_up, p.polls);
+                if (!ok) break;
+                ++done;
+                tc_fence_after();
+                uint32_t s[64];
+                tc_ld32_async(s_tmem, s);
+                tc_ld32_async(s_tmem + 32, s + 32);
+                const T8Tile known = s_tile[(g0 + kt) % kT8Known];
+                const bool gone[2] = {known.row[0] < 0, known.row[1] < 0};
+                const float ev[2] = {known.ev[0], known.ev[1]};
+                // every key of the tile is visible to every row of the warp
+                const bool all = __all_sync(0xffffffffu, !gone[0] && !gone[1] && key0 + kT8Keys - 1 <= qpos && (qpos - key0 < wnd || key0 + kT8Keys <= a.keep_first));
+                tc_arrived(s);
+                tc_arrived(s + 32);
+                tc_fence_before();
+                mb_arrive(sread + j);              // the next scores may be made
+                float f[2] = {known.ks[0] * mul, known.ks[1] * mul};
+                if (kOpts) {
+                    if (a.softcap > 0.0f) {
+                        const float inv[2] = {f[0] / a.softcap, f[1] / a.softcap};
+                        float most = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 64; e += 2) {
+                            const float x = __uint_as_float(s[e]) * inv[e / 32], y = __uint_as_float(s[e + 1]) * inv[e / 32];
+                            s[e] = __float_as_uint(x);
+                            s[e + 1] = __float_as_uint(y);
+                            most = tc_max3(most, fabsf(x), fabsf(y));
+                        }
+                        // scores within a quarter of the cap, as nearly all are: the series that tc_tanh takes for them, two at a time
+                        if (__any_sync(0xffffffffu, most >= 0.25f)) {
+#pragma unroll
+                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(a.softcap * tc_tanh(__uint_as_float(s[e])));
+                        } else {
+                            auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
+                            const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), one = both(1.0f), cap2 = both(a.softcap);
+#pragma unroll
+                            for (int e = 0; e < 64; e += 2) {
+                                const uint64_t x = tc_two(s[e], s[e + 1]), x2 = tc_mul2(x, x);
+                                float y, z;
+                                tc_split(tc_mul2(cap2, tc_mul2(x, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, c4, c3), c2), c1), one))), y, z);
+                                s[e] = __float_as_uint(y);
+                                s[e + 1] = __float_as_uint(z);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f[e / 32]);
+                    }
+                    if (a.slopes) {
+                        const float dist = (float)(qpos - key0);
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(fmaf(-slope, dist - (float)e, __uint_as_float(s[e])));
+                    }
+                    f[0] = f[1] = kTcLog2e;
+                }
+                if (!all) {        // the columns this row sees, as bits
+                    const int hi = qpos - key0, lo = wnd > qpos ? -1 : qpos - wnd - key0, keep = a.keep_first - key0;
+                    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };       // bits 0 .. n - 1
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t seen = gone[x] ? 0u : below(hi + 1 - 32 * x) & (~below(lo + 1 - 32 * x) | below(keep - 32 * x));
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[32 * x + e] = seen & (1u << e) ? s[32 * x + e] : 0xff800000u;        // -inf
+                    }
+                }
+                {
+                    float top[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            t0 = tc_max3(t0, __uint_as_float(s[32 * x + e]), __uint_as_float(s[32 * x + e + 1]));
+                            t1 = tc_max3(t1, __uint_as_float(s[32 * x + e + 2]), __uint_as_float(s[32 * x + e + 3]));
+                        }
+                        top[x] = fmaxf(t0, t1);
+                    }
+                    const float m0 = fmaf(top[0], f[0], ev[0]), m1 = fmaf(top[1], f[1], ev[1]);
+                    float mx = fmaxf(m0, m1);
+                    // Rare, with one vote for both: scores so large that a rounded product and one inside a multiply-add are far apart (every product is rounded then, so that no weight is
+                    // above 1), and a block whose weights come out below 2^-60 because its value scale is that much smaller than others' (`far`).
+                    float far[2] = {0.0f, 0.0f};
+                    const bool rare = __any_sync(0xffffffffu, fabsf(mx) > 65536.0f ? mx != -INFINITY : fminf(m0, m1) < fmaxf(ref, mx) - 60.0f);
+                    if (rare) {
+                        if (__any_sync(0xffffffffu, fabsf(mx) > 65536.0f && mx != -INFINITY)) {
+#pragma unroll
+                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f[e / 32]);
+                            top[0] *= f[0];
+                            top[1] *= f[1];
+                            f[0] = f[1] = 1.0f;
+                            mx = fmaxf(__fadd_rn(top[0], ev[0]), __fadd_rn(top[1], ev[1]));
+                        }
+                        // Nothing to O, but the denominator has their weights without the scale: they are taken 2^far larger, so that they do not vanish.
+                        const float base = fmaxf(ref, ceilf(mx));
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float most = fmaf(top[x], f[x], ev[x]) - base;
+                            far[x] = most < -60.0f && most > -1e6f ? floorf(-most) : 0.0f;
+                        }
+                    }
+                    const float nr = fmaxf(ref, ceilf(mx)), less = kt == 0 || nr == ref ? 1.0f : tc_exp2(ref - nr);
+                    // the product with the last weights has been made: their place is free, and their factors have been used
+                    if (done > 1) ok = t8_wait_warp(odone + j, (done - 2) & 1, gave_up, p.polls);
+                    if (!ok) break;
+                    tc_fence_after();
+                    factor[j * kT8Rows + row] = less;
+                    mb_arrive(factors + j);
+                    l = kt == 0 ? 0.0f : l * less;
+                    ref = nr;
+                    // where every score so far is -inf, -inf - ref were no number: relative to 0 their weights are 0
+                    const float base = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float neg = ev[x] - base + far[x];
+                        const uint64_t f2 = tc_two(__float_as_uint(f[x]), __float_as_uint(f[x])), neg2 = tc_two(__float_as_uint(neg), __float_as_uint(neg));
+                        uint64_t sum = 0;
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float y, z;
+                            tc_split(tc_fma2(tc_two(s[32 * x + 2 * e], s[32 * x + 2 * e + 1]), f2, neg2), y, z);
+                            y = tc_exp2(y);
+                            z = tc_exp2(z);
+                            sum = tc_add2(sum, tc_two(__float_as_uint(y), __float_as_uint(z)));
+                            hi[e] = t8_pack(y, z);
+                            if constexpr (kTerms == 2) {
+                                const float2 u = t8_unpack(hi[e]);
+                                lo[e] = t8_pack(y - u.x, z - u.y);
+                            }
+                        }
+                        if (rare) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                hi[e] = far[x] != 0.0f ? 0u : hi[e];
+                                if constexpr (kTerms == 2) lo[e] = far[x] != 0.0f ? 0u : lo[e];
+                            }
+                        }
+                        tc_st16(p_tmem + 16 * x, hi);
+                        if constexpr (kTerms == 2) tc_st16(p_tmem + 32 + 16 * x, lo);
+                        float s0, s1;
+                        tc_split(sum, s0, s1);
+                        l = fmaf(s0 + s1, tc_exp2(-ev[x] - far[x]), l);         // without the value scale
+                    }
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mb_arrive(pready + j);
+            }
+            if (!ok) break;
+            if (items) ok = t8_wait_warp(lread + j, (items - 1) & 1, gave_up, p.polls);
+            if (!ok) break;
+            s_ref[j * kT8Rows + row] = ref;
+            s_sum[j * kT8Rows + row] = l;
+            ++items;
+            mb_arrive(lready + j);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*gave_up) tc_gave_up(p.status);
+    if (warp == 1) {
+        tc_fence_after();
+        tc_dealloc(tmem, kT8Tmem);
+    }
+}
+
+template <int HD, int kTerms, bool kOpts>
+static int t8_launch(const T8Args& a, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t st) {
+    using Sh = T8Shape<HD, kTerms>;
+    auto* kernel = seq_attention8_tc_kernel<HD, kTerms, kOpts>;
+    static bool ready = false;
+    if (!ready) {
+        SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+        ready = true;
+    }
+    LaunchCfg lc(dim3(std::min(kA8TcWorkers, sm_count())), dim3(kT8Threads), Sh::kSmem, st, true);        // its beginning while the plan is made
+    SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(kernel), tmK, tmV, a));
+    ++g_launches;
+    SLLM_LAUNCH_CHECK_ONLY();
+    return SLLM_OK;
+}
+
+static int t8_hpc(const Attn8Args& p) {
+    const int group = p.heads / p.kv_heads;
+    return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+}
+
+bool attention8_tc_takes(const Attn8Args& p) {
+    const int width = 2 * kT8Rows / t8_hpc(p);
+    return p.dk <= 128 && p.dv <= 128 && p.b.nseg <= kA8Segs && p.b.T / width + p.b.nseg <= kA8Runs;
+}
+
+int launch_attention8_tc(const Attn8Args& p, void* ws, cudaStream_t st) {
+    T8Args a{};
+    a.a = p;
+    a.hpc = t8_hpc(p);
+    a.hpc_log2 = a.hpc / 2;
+    a.queries = kT8Rows / a.hpc;
+    a.sets = p.heads / a.hpc;
+    a.vec_q = p.ldq % 4 == 0 && ((uintptr_t)p.q % 16) == 0;
+    A8Plan* plan = reinterpret_cast<A8Plan*>((uint8_t*)ws + kA8PlanAt);
+    a.plan = plan;
+    a.counters = (int*)ws + kA8Workers;
+    a.parts = (float*)((uint8_t*)ws + kA8PartsAt);
+    if (int rc = status_word(&a.status)) return rc;
+    a.polls = (unsigned)g_tune_tc_polls;
+    const int HD = std::max(p.dk, p.dv) <= 64 ? 64 : 128;
+    CUtensorMap tmK, tmV;
+    const uint64_t rows = (uint64_t)p.n_pages * p.kv_heads * p.b.page_len;
+    if (int rc = tc_encode_bytes(&tmK, p.k_pool, rows, p.dk, kKv8Block, HD)) return rc;
+    if (int rc = tc_encode_bytes(&tmV, p.v_pool, rows, p.dv, kKv8Block, HD)) return rc;
+    overlapping(seq_attention8_plan_kernel)<<<1, 1024, 0, st>>>(p, 2 * a.queries, plan);
+    ++g_launches;
+    SLLM_LAUNCH_CHECK_ONLY();
+    const bool opts = p.softcap > 0.0f || p.slopes;
+return t8_launch<128,1,false>(a,tmK,tmV,st);
+}
+
+}  // namespace sllm
