@@ -148,7 +148,7 @@ int sllm_sample_f32(const float* logits, int32_t n, float temperature, int32_t t
  * kept are the top_k largest logits (0 = all), of these the smallest set of largest ones whose mass reaches top_p of theirs (0 or 1 = all), of these those with w_i >= min_p
  * (0 = all); equal logits are in or out together. Drawn is the first i whose running kept mass exceeds u * (kept mass), u in [0, 1). temperature <= 0: the first of the largest
  * logits. NaN counts as -infinity, which is never drawn (a row of nothing else gives 0); where logits are +infinity, one of those is drawn. Weights are held as multiples of 2^-44, so
- * that sums are exact and the result is a function of the row alone. idx_dev [rows] int32; prob_dev [rows] or NULL: the drawn one's share of the kept mass. Up to 786432 logits a row. */
+ * that sums are exact and the result is a function of the row alone. idx_dev [rows] int32; prob_dev [rows] or NULL: the drawn one's share of the kept mass. Up to 720896 logits a row. */
 int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, int32_t n, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                      const float* u, int32_t* idx_dev, float* prob_dev, sllm_stream_t stream);
 
