@@ -6,10 +6,10 @@
 // thousands over a large vocabulary. Weights are computed in double and held as multiples of 2^-44: sums of these integers are exact, so nothing depends on the order of threads, and
 // what is left is the rounding of a weight, 2^-45 of the largest.
 // A cluster of CTAs shares a row and keeps it in shared memory: the logits are read once, whatever the settings ask for.
-// The last value that stays (top_k, top_p) is found without sorting: a histogram of the distance to the largest logit, 1024 bins of 1/8 (integers: sums of counts, or of weights in three
+// The last value that stays (top_k, top_p) is found without sorting: a histogram of the distance to the largest logit, 1024 bins of 1/22 of a bit of weight (integers: sums of counts, or of weights in three
 // parts of 16 bits, so that shared memory's 32-bit additions do), added over the cluster; if the bin that holds the border is full, once more over its 1024 parts. What is left goes to one
 // CTA, which compares it pair by pair. Where a top_k leaves no more than kSrFew candidates all of them go there, and the draw ends there. Only parts too full for that (hundreds of logits
-// within 2^-13 that are not all equal, or beyond the last bin) are halved bit by bit.
+// within 2^-14 of a bit that are not all equal, or beyond the last bin) are halved bit by bit.
 // Bound: barriers of the cluster and what lies between them; bytes (4 a logit) and double arithmetic (some 20 instructions a weight) come to about a quarter of it over large batches.
 #include <cooperative_groups.h>
 
@@ -32,29 +32,20 @@ struct SampleRows {
     int ld, n, slice;
 };
 
-// 2^t for -64 <= t <= 0 to 1e-14 of its value: 2^round(t) times the Taylor series of 2^f, |f| <= 1/2 (remainder 0.3466^12 / 12! = 6e-15)
-__device__ __forceinline__ double sr_exp2(double t) {
-    const double magic = 6755399441055744.0;                       // 1.5 * 2^52: adding it rounds to an integer, which the low bits then hold
-    const double r = t + magic, f = t - (r - magic);
-    const int n = __double2loint(r);
-    constexpr double l = 0.693147180559945309417;
-    constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7, c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
-    double p = c11;
-    p = fma(p, f, c10); p = fma(p, f, c9); p = fma(p, f, c8); p = fma(p, f, c7); p = fma(p, f, c6); p = fma(p, f, c5); p = fma(p, f, c4); p = fma(p, f, c3); p = fma(p, f, c2);
-    p = fma(p, f, l);
-    p = fma(p, f, 1.0);
-    return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
-}
-
 // The weight of a row's logits, in 2^-44
 struct SrRow {
     float top;                 // the largest logit
-    double rate;               // log2(e) / temperature
+    double top_d, rate;        // and as a double; 32 log2(e) / temperature
+    const double* powers;      // 2^(i / 32), i < 32
+    // of one no further below the largest than some 46 bits: exp(z) = 2^(k / 32) e^g with |g| <= ln 2 / 64, the Taylor series of e^g (remainder 0.0109^6 / 6! = 2e-15), rounded by adding 2^52
     __device__ __forceinline__ uint64_t weight_of(float x) const {
-        if (x == top) return (uint64_t)kSrOne;
-        if (x == -INFINITY || top == INFINITY) return 0;
-        const double t = ((double)x - (double)top) * rate;
-        return t < -64.0 ? 0 : (uint64_t)__double2ll_rn(sr_exp2(t) * kSrOne);
+        if (top == INFINITY) return x == top ? (uint64_t)kSrOne : 0;
+        const double magic = 6755399441055744.0;                       // 1.5 * 2^52: adding it rounds to an integer, which the low bits then hold
+        const double z = (double)x - top_d, r = fma(z, rate, magic), f = fma(z, rate, -(r - magic));
+        const int k = __double2loint(r);
+        constexpr double l = 0.693147180559945309417 / 32, c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5;
+        const double g = f * f, a = fma(fma(c5, f, c4), g, fma(c3, f, c2)), p = fma(a, g, fma(l, f, 1.0)) * powers[k & 31];
+        return (uint64_t)__double_as_longlong(__hiloint2double(__double2hiint(p) + (((k >> 5) + 44) << 20), __double2loint(p)) + 4503599627370496.0) & 0xfffffffffffffull;
     }
 };
 
@@ -64,7 +55,10 @@ __device__ __forceinline__ uint32_t sr_key(float f) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-struct SrShared {
+__device__ __forceinline__ float sr_float(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+struct alignas(16) SrShared {
+    double powers[32];
     uint64_t slot[2][kSrCluster];        // what the CTAs of the cluster have sent, two sums in turn
     uint64_t warp[kSrWarps], before[kSrWarps];
     // bins: counts and weights of this CTA's logits; sums over the cluster for the bins this CTA adds up, and of all CTAs' bins
@@ -78,11 +72,12 @@ struct SrShared {
     int at[kSrFew];
     uint64_t w[kSrFew];
     uint32_t listed, lowest;
+    float tops[kSrCluster * kSrWarps];   // the largest logit of every warp of the cluster
     // where a border lies: the bin, and what lies in bins before it and in it
     int bin;
     uint64_t mass_before;
     uint32_t count_before, count_in;
-    uint32_t threshold;
+    float threshold;
 };
 
 __device__ __forceinline__ uint64_t sr_warp_sum(uint64_t v) {
@@ -149,12 +144,19 @@ struct SrWork {
     cg::cluster_group& cluster;
     SrRow r;
     const float* s_x;
-    int count, rank, size, turn;
-    float far;                           // distances to the largest logit beyond which a weight is 0
+    int lo, hi, rank, size, turn;        // this warp's run
+    float mine;                          // its largest logit
+    float far, scale;                    // distances to the largest logit beyond which a weight is 0; bins in a distance of 1: the last one begins there
+    // f(logit, place in the CTA's slice) for every logit of this warp's run, if one of them is not below `least`
+    template <typename F>
+    __device__ __forceinline__ void each(float least, F f) const {
+        if (mine < least) return;
+        for (int i = lo + (int)(threadIdx.x & 31); i < hi; i += 32) f(s_x[i], i);
+    }
 
     __device__ __forceinline__ void barrier() { if (size == 1) __syncthreads(); else cluster.sync(); }
     __device__ __forceinline__ uint64_t weight(float x) const { return r.top - x > far ? 0 : r.weight_of(x); }      // (inf - inf is no number: not beyond)
-    static __device__ __forceinline__ int bin_of(float d) { return (int)fminf(d * 8.0f, (float)(kSrBins - 1)); }
+    __device__ __forceinline__ int bin_of(float d) const { return (int)fminf(d * scale, (float)(kSrBins - 1)); }
     __device__ __forceinline__ void clear() {
         for (int i = threadIdx.x; i < kSrBins; i += kSrThreads) sh.count[i] = sh.part[0][i] = sh.part[1][i] = sh.part[2][i] = 0;
         if (threadIdx.x == 0) { sh.listed = 0; sh.lowest = 0xffffffffu; }
@@ -193,27 +195,26 @@ struct SrWork {
         __syncthreads();
     }
 
-    // which bin of 1/8 (outer < 0), or which part of bin `outer`, a logit belongs to; -1: none
+    // which bin (outer < 0), or which part of bin `outer`, a logit belongs to; -1: none
     __device__ __forceinline__ int place(float x, int outer) const {
         const float d = r.top - x;
         if (outer < 0) return bin_of(d);
-        return bin_of(d) == outer ? (int)fminf(fmaxf((d - outer * 0.125f) * (8.0f * kSrBins), 0.0f), (float)(kSrBins - 1)) : -1;
+        return bin_of(d) == outer ? (int)fminf(fmaxf(fmaf(d, scale, -(float)outer) * kSrBins, 0.0f), (float)(kSrBins - 1)) : -1;
     }
 
-    // The least value that stays, as a key: top_k of them (by_mass false), or those that reach `share` of the mass of the logits with keys from `above` on. small: a border by count that
+    // The least value that stays: of top_k of them (by_mass false), or of those that reach `share` of the mass of the logits from `above` on. small: a border by count that
     // leaves no more than kSrFew candidates is not looked for; they are all in the first CTA's list then, and the answer is 0.
-    __device__ uint32_t find(bool by_mass, uint64_t top_k, double share, uint32_t above, bool& small) {
+    __device__ float find(bool by_mass, uint64_t top_k, double share, float above, bool& small) {
         double need = (double)top_k;
         uint64_t m0 = 0;
         uint32_t n0 = 0;
         int outer = -1;
         for (;;) {
             clear();
-            for (int i = threadIdx.x; i < count; i += kSrThreads) {
-                const float x = s_x[i];
-                const int bin = sr_key(x) >= above ? place(x, outer) : -1;
+            each(above, [&](float x, int) {
+                const int bin = x >= above ? place(x, outer) : -1;
                 if (bin >= 0) add(bin, by_mass ? weight(x) : 0, by_mass);
-            }
+            });
             barrier();                                                   // every CTA's bins are there
             const int own = kSrBins / size, b0 = rank * own;
             uint64_t mass = 0;
@@ -276,17 +277,16 @@ struct SrWork {
             }
             // candidates to the first CTA: the border's bin, or everything up to it
             SrShared* first = cluster.map_shared_rank(&sh, 0);
-            for (int i = threadIdx.x; i < count; i += kSrThreads) {
-                const float x = s_x[i];
-                const int b = sr_key(x) >= above ? place(x, outer) : -1;
+            each(above, [&](float x, int i) {
+                const int b = x >= above ? place(x, outer) : -1;
                 if (b >= 0 && (small ? b <= bin : b == bin)) {
                     const uint32_t to = atomicAdd(&first->listed, 1u);
                     first->x[to] = x;
                     first->at[to] = (rank << 20) | i;
                 }
-            }
+            });
             barrier();
-            if (small) return 0;
+            if (small) return 0.0f;
             if (rank == 0) {                                             // pair by pair: one stays when what lies above it is not yet enough
                 const bool is = threadIdx.x < in;
                 const float x = is ? sh.x[threadIdx.x] : 0.0f;
@@ -296,22 +296,52 @@ struct SrWork {
                 for (uint32_t k = 0; k < in; ++k) v += sh.x[k] > x ? sh.w[k] : 0;
                 if (is && (double)v < need) atomicMin(&sh.lowest, sr_key(x));
                 __syncthreads();
-                if (threadIdx.x == 0) sh.threshold = sh.lowest;
+                if (threadIdx.x == 0) sh.threshold = sr_float(sh.lowest);
             }
             barrier();
             return cluster.map_shared_rank(&sh, 0)->threshold;
         }
     }
 
+    // A top_k below the number of the cluster's warps: the top_k-th largest of the warps' largest logits is no larger than the top_k-th largest of all, so that the candidates lie from there
+    // on; as a rule not many more than top_k. True when the first CTA's list holds all of them.
+    __device__ __forceinline__ bool few(int top_k, int groups) {
+        if (top_k * 8 > groups * 7) return false;
+        if (threadIdx.x == 0) { sh.listed = 0; sh.lowest = 0xffffffffu; }
+        __syncthreads();
+        if ((int)threadIdx.x < groups) {
+            const float x = sh.tops[threadIdx.x];
+            int above = 0;
+            for (int k = 0; k < groups; ++k) above += sh.tops[k] > x;
+            if (above < top_k) atomicMin(&sh.lowest, sr_key(x));
+        }
+        __syncthreads();
+        const float bound = sr_float(sh.lowest);
+        barrier();                                                       // the first CTA's list is empty
+        SrShared* first = cluster.map_shared_rank(&sh, 0);
+        each(bound, [&](float x, int i) {
+            if (x >= bound) {
+                const uint32_t to = atomicAdd(&first->listed, 1u);
+                if (to < kSrFew) {
+                    first->x[to] = x;
+                    first->at[to] = (rank << 20) | i;
+                }
+            }
+        });
+        barrier();
+        const bool all = cluster.map_shared_rank(&sh, 0)->listed <= kSrFew;
+        barrier();                                                       // (it has been read, before the first CTA goes on)
+        return all;
+    }
+
     // The border lies among more candidates than the list holds: all alike, or halved bit by bit
-    __device__ __noinline__ uint32_t crowded(bool by_mass, double need, uint32_t above, int outer, int bin) {
+    __device__ __noinline__ float crowded(bool by_mass, double need, float above, int outer, int bin) {
         uint64_t high = 0, low = 0;
-        for (int i = threadIdx.x; i < count; i += kSrThreads) {
-            const float x = s_x[i];
-            if (sr_key(x) < above || place(x, outer) != bin) continue;
+        each(above, [&](float x, int) {
+            if (x < above || place(x, outer) != bin) return;
             high = max(high, (uint64_t)sr_key(x));
             low = max(low, (uint64_t)~sr_key(x));
-        }
+        });
         high = sr_all<true>(high, sh, turn, cluster);
         low = (uint32_t)~(uint32_t)sr_all<true>(low, sh, turn, cluster);
         // the largest key from `low` on at which there is enough; at `low` there is
@@ -319,13 +349,12 @@ struct SrWork {
         while (from < to) {
             const uint32_t mid = from + (to - from + 1) / 2;
             uint64_t v = 0;
-            for (int i = threadIdx.x; i < count; i += kSrThreads) {
-                const float x = s_x[i];
-                if (sr_key(x) >= mid && sr_key(x) >= above) v += by_mass ? weight(x) : 1;
-            }
+            each(above, [&](float x, int) {
+                if (sr_key(x) >= mid && x >= above) v += by_mass ? weight(x) : 1;
+            });
             if ((double)sr_all<false>(v, sh, turn, cluster) >= need) from = mid; else to = mid - 1;
         }
-        return from;
+        return sr_float(from);
     }
 };
 
@@ -339,60 +368,79 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p
     const int first = min(p.n, rank * p.slice), count = min(p.n, first + p.slice) - first;
     const float* x = p.logits + (size_t)row * p.ld + first;
     int turn = 0;
-    // the largest logit and the first place that has it, as one number; NaN counts as -infinity
-    uint64_t best = 0;
-    auto take = [&](float v, int i) {
+    // NaN counts as -infinity
+    float best = -INFINITY;
+    auto take = [&](float v) {
         v = v == v ? v : -INFINITY;
-        const uint64_t k = ((uint64_t)sr_key(v) << 32) | (uint32_t)~(first + i);
-        best = k > best ? k : best;
+        best = fmaxf(best, v);
         return v;
     };
+    // a warp owns a run of neighbouring logits
+    const int run = ((count + kSrWarps - 1) / kSrWarps + 3) / 4 * 4, lo = min(count, warp * run), hi = min(count, lo + run);
+    if (threadIdx.x < 32) sh.powers[threadIdx.x] = exp2(threadIdx.x / 32.0);
     {
-        const int head = min(count, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 4), body = (count - head) / 4;      // up to a multiple of 16 bytes; 16 bytes a load
-        if ((int)threadIdx.x < head) s_x[threadIdx.x] = take(x[threadIdx.x], threadIdx.x);
+        const int off = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 4, head = min(hi - lo, off), body = (hi - lo - head) / 4;      // up to a multiple of 16 bytes; 16 bytes a load
+        s_x += (4 - off) & 3;                                        // so that they are stored 16 bytes at a time, too
+        const float* from = x + lo + head;
+        float* to = s_x + lo + head;
+        if (lane < head) s_x[lo + lane] = take(x[lo + lane]);
         constexpr int kAhead = 4;
-        for (int c = threadIdx.x; c < body; c += kAhead * kSrThreads) {
+        for (int c = lane; c < body; c += kAhead * 32) {
             float4 v[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
-                if (c + k * kSrThreads < body) v[k] = *reinterpret_cast<const float4*>(x + head + 4 * (c + k * kSrThreads));
+                if (c + k * 32 < body) v[k] = *reinterpret_cast<const float4*>(from + 4 * (c + k * 32));
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const int at = head + 4 * (c + k * kSrThreads);
-                if (c + k * kSrThreads >= body) break;
-                s_x[at] = take(v[k].x, at);
-                s_x[at + 1] = take(v[k].y, at + 1);
-                s_x[at + 2] = take(v[k].z, at + 2);
-                s_x[at + 3] = take(v[k].w, at + 3);
+                if (c + k * 32 >= body) break;
+                *reinterpret_cast<float4*>(to + 4 * (c + k * 32)) = make_float4(take(v[k].x), take(v[k].y), take(v[k].z), take(v[k].w));
             }
         }
-        for (int i = head + 4 * body + threadIdx.x; i < count; i += kSrThreads) s_x[i] = take(x[i], i);
+        for (int i = lo + head + 4 * body + lane; i < hi; i += 32) s_x[i] = take(x[i]);
     }
     const float temperature = p.temperature ? p.temperature[row] : 1.0f, top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.0f, u = p.u[row];
     const int top_k = p.top_k ? p.top_k[row] : 0;
-    best = sr_all<true>(best, sh, turn, cluster);
-    const int arg = (int)~(uint32_t)best;
-    const uint32_t top_key = (uint32_t)(best >> 32);
+    // the largest of every warp to all CTAs: the largest of all, and (below) a bound for the top_k largest
+    best = warp_max(best);
+    if (size == 1) {
+        if (lane == 0) sh.tops[warp] = best;
+        __syncthreads();
+    } else {
+        if (lane < size) cluster.map_shared_rank(&sh, lane)->tops[rank * kSrWarps + warp] = best;
+        cluster.sync();
+    }
+    const int groups = size * kSrWarps;
     SrRow r;
-    r.top = __uint_as_float(top_key & 0x80000000u ? top_key & 0x7fffffffu : ~top_key);
+    r.top = -INFINITY;
+    for (int i = lane; i < groups; i += 32) r.top = fmaxf(r.top, sh.tops[i]);
+    r.top = warp_max(r.top);
+    r.top_d = (double)r.top;
     if (!(temperature > 0.0f) || r.top == -INFINITY) {
+        // the first place that has it
+        uint64_t place = 0;
+        if (best == r.top)
+            for (int i = lo + lane; i < hi; i += 32)
+                if (s_x[i] == r.top) place = max(place, (uint64_t)(uint32_t)~(first + i));
+        place = sr_all<true>(place, sh, turn, cluster);
         if (rank == 0 && threadIdx.x == 0) {
-            p.idx[row] = r.top == -INFINITY ? 0 : arg;
+            p.idx[row] = r.top == -INFINITY ? 0 : (int)~(uint32_t)place;
             if (p.prob) p.prob[row] = r.top == -INFINITY ? 0.0f : 1.0f;
         }
         return;
     }
-    r.rate = 1.4426950408889634074 / (double)temperature;
+    r.rate = 32 * 1.4426950408889634074 / (double)temperature;
+    r.powers = sh.powers;
     const uint64_t least = min_p > 0.0f ? (uint64_t)__double2ll_ru(fmin((double)min_p, 1.0) * kSrOne) : 0;
     // beyond this distance a weight is below 2^-45 (or well below min_p: log2 in fp32 is off by less than a thousandth of that here)
     const float bits = min_p > 0.0f ? fminf(46.0f, -log2f(fminf(min_p, 1.0f)) + 0.01f) : 46.0f;
-    SrWork w{sh, cluster, r, s_x, count, rank, size, turn, 46.0f * 0.6931472f * temperature * 1.0001f};
+    const float reach = 46.0f * 0.6931472f * temperature * 1.0001f;
+    SrWork w{sh, cluster, r, s_x, lo, hi, rank, size, turn, best, reach, (float)(kSrBins - 1) / reach};
     const float far = bits * 0.6931472f * temperature * 1.0001f;
-    uint32_t thr = 0;                                               // kept: key >= thr
+    float thr = -INFINITY;                                          // kept: from there on
     if (r.top < INFINITY) {                                         // (of infinite logits all are kept, and nothing else weighs anything)
         if (top_k > 0 && top_k < p.n) {
             bool small = true;
-            thr = w.find(false, (uint64_t)top_k, 0.0, 0, small);
+            thr = w.few(top_k, groups) ? 0.0f : w.find(false, (uint64_t)top_k, 0.0, -INFINITY, small);
             if (small) {                                            // the first CTA has all that may stay
                 if (rank != 0) return;
                 const int n = (int)sh.listed, i = threadIdx.x;
@@ -434,19 +482,19 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p
         }
         if (top_p > 0.0f && top_p < 1.0f) {
             bool small = false;
-            thr = max(thr, w.find(true, 0, (double)top_p, thr, small));
+            thr = fmaxf(thr, w.find(true, 0, (double)top_p, thr, small));
         }
     }
     turn = w.turn;
     auto kept = [&](float v) -> uint64_t {
-        if (sr_key(v) < thr || r.top - v > far) return 0;
+        if (v < thr || r.top - v > far) return 0;
         const uint64_t y = r.weight_of(v);
         return y >= least ? y : 0;
     };
-    // a warp owns a run of neighbouring logits: its mass first, then the one in whose run the target lies walks it
-    const int run = (count + kSrWarps - 1) / kSrWarps, lo = min(count, warp * run), hi = min(count, lo + run);
+    // the mass of the warp's run first, then the warp in whose run the target lies walks it
     uint64_t mine = 0;
-    for (int i = lo + lane; i < hi; i += 32) mine += kept(s_x[i]);
+    if (best >= thr && !(r.top - best > far))
+        for (int i = lo + lane; i < hi; i += 32) mine += kept(s_x[i]);
     mine = sr_warp_sum(mine);
     if (lane == 0) sh.before[warp] = mine;
     const uint64_t all = sr_all<false>(lane == 0 ? mine : 0, sh, turn, cluster);
@@ -490,7 +538,7 @@ extern "C" int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, i
     static bool ready = false;
     if (!ready) {
         SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SrShared) + kSrSlice * 4));
+        SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SrShared) + kSrSlice * 4 + 16));
         ready = true;
     }
     int cs = 1;
@@ -500,7 +548,7 @@ extern "C" int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, i
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)rows * cs);
     cfg.blockDim = dim3(kSrThreads);
-    cfg.dynamicSmemBytes = sizeof(SrShared) + (size_t)p.slice * 4;
+    cfg.dynamicSmemBytes = sizeof(SrShared) + (size_t)p.slice * 4 + 16;
     cfg.stream = as_stream(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
