@@ -16,44 +16,44 @@ struct Kv8Args {
     const float *q, *k, *v, *angles;
     float *q_out, *k_scale, *v_scale;
     uint8_t *k_pool, *v_pool;
-    int ldq, ldk, ldv, ldqo, heads, kv_heads, dk, dv, n_freq, layout, n_pages;
+    int ldq, ldk, ldv, ldqo, heads, kv_heads, dk, dv, n_freq, n_pages;
     int units, q_split;              // (segment, block) pairs the grid has room for; CTAs that share a token's queries
     int32_t* status;
 };
 
 constexpr int kKv8Threads = 128;
 
-// A job is eight columns of a row: four neighbouring pairs of a turned row (both halves of each), eight neighbouring columns elsewhere. `at`: the first column of its two runs of four.
+// A job is eight columns of a row: four neighbouring pairs of a turned row (both halves of each), eight neighbouring columns elsewhere. The first column of its two runs of four:
+template <bool kVec, int kLayout>
+__device__ __forceinline__ int kv8_column(int job, int n_freq, int run) {
+    return kVec && kLayout == 1 && job < n_freq / 4 ? (run ? n_freq + 4 * job : 4 * job) : 8 * job + 4 * run;
+}
 // kVec: rows are 16-byte aligned and n_freq is a multiple of four, so that a run is one load; else every column for itself.
-template <bool kVec>
-__device__ __forceinline__ void kv8_load(const float* row, const float* angles, int n_freq, int layout, int job, int (&at)[2], float (&x)[8]) {
+template <bool kVec, int kLayout>
+__device__ __forceinline__ void kv8_load(const float* row, const float* angles, int n_freq, int job, float (&x)[8]) {
     if constexpr (kVec) {
-        const bool turned = job < n_freq / 4;
-        if (turned && layout) { at[0] = 4 * job; at[1] = n_freq + 4 * job; } else { at[0] = 8 * job; at[1] = 8 * job + 4; }
-        const float4 a = *reinterpret_cast<const float4*>(row + at[0]), c = *reinterpret_cast<const float4*>(row + at[1]);
+        const float4 a = *reinterpret_cast<const float4*>(row + kv8_column<kVec, kLayout>(job, n_freq, 0)), c = *reinterpret_cast<const float4*>(row + kv8_column<kVec, kLayout>(job, n_freq, 1));
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
-        if (turned) {
+        if (job < n_freq / 4) {
             const float4 t0 = *reinterpret_cast<const float4*>(angles + 8 * job), t1 = *reinterpret_cast<const float4*>(angles + 8 * job + 4);
             const float cs[4] = {t0.x, t0.z, t1.x, t1.z}, sn[4] = {t0.y, t0.w, t1.y, t1.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float &u = layout ? x[i] : x[2 * i], &w = layout ? x[4 + i] : x[2 * i + 1];
-                const float u0 = u, w0 = w;
+                constexpr int kStep = kLayout ? 1 : 2, kOther = kLayout ? 4 : 1;
+                const float u = x[kStep * i], w = x[kStep * i + kOther];
                 // products and sums rounded one by one: a code does not depend on where a compiler contracts
-                u = __fsub_rn(__fmul_rn(u0, cs[i]), __fmul_rn(w0, sn[i]));
-                w = __fadd_rn(__fmul_rn(w0, cs[i]), __fmul_rn(u0, sn[i]));
+                x[kStep * i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(w, sn[i]));
+                x[kStep * i + kOther] = __fadd_rn(__fmul_rn(w, cs[i]), __fmul_rn(u, sn[i]));
             }
         }
     } else {
-        at[0] = 8 * job;
-        at[1] = 8 * job + 4;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int c = 8 * job + i;
             x[i] = row[c];
             if (c < 2 * n_freq) {
-                const bool first = layout ? c < n_freq : !(c & 1);
-                const int m = layout ? (first ? c : c - n_freq) : c >> 1, other = layout ? (first ? c + n_freq : c - n_freq) : c ^ 1;
+                const bool first = kLayout ? c < n_freq : !(c & 1);
+                const int m = kLayout ? (first ? c : c - n_freq) : c >> 1, other = kLayout ? (first ? c + n_freq : c - n_freq) : c ^ 1;
                 const float cs = angles[2 * m], sn = angles[2 * m + 1], o = row[other];
                 x[i] = first ? __fsub_rn(__fmul_rn(x[i], cs), __fmul_rn(o, sn)) : __fadd_rn(__fmul_rn(x[i], cs), __fmul_rn(o, sn));
             }
@@ -62,7 +62,7 @@ __device__ __forceinline__ void kv8_load(const float* row, const float* angles, 
 }
 
 // The part of one segment's rows that lies in the block at `lo` (a multiple of 32), for one head of one pool, by the whole CTA.
-template <bool kVec, int kJobs>
+template <bool kVec, int kLayout, int kJobs>
 __device__ __forceinline__ void kv8_block(const Kv8Args& p, int tok0, int pos0, int len, int slot, int lo, int g, const float* src, int ld, int width, int n_freq, uint8_t* pool,
                                           float* scales, float* red) {
     const sllm_seq_batch& b = p.b;
@@ -77,13 +77,12 @@ __device__ __forceinline__ void kv8_block(const Kv8Args& p, int tok0, int pos0, 
     uint8_t* dst = pool + seq_pool_row(page, p.kv_heads, g, b.page_len, in_page, width);
     const float was = first > lo ? *scale : 0.0f;                          // without earlier rows the block begins anew
     float x[kJobs][8], top = 0.0f;
-    int at[kJobs][2];
 #pragma unroll
     for (int j = 0; j < kJobs; ++j) {
         const int i = threadIdx.x + j * kKv8Threads;
         if (i >= jobs) break;
         const int t = tok + i / per_row;
-        kv8_load<kVec>(src + (size_t)t * ld + (size_t)g * width, p.angles + (size_t)t * 2 * n_freq, n_freq, p.layout, i % per_row, at[j], x[j]);
+        kv8_load<kVec, kLayout>(src + (size_t)t * ld + (size_t)g * width, p.angles + (size_t)t * 2 * n_freq, n_freq, i % per_row, x[j]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float a = fabsf(x[j][e]);
@@ -113,15 +112,15 @@ __device__ __forceinline__ void kv8_block(const Kv8Args& p, int tok0, int pos0, 
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const float* y = x[j] + 4 * h;
-            *reinterpret_cast<uint32_t*>(row + at[j][h]) = kv8_pack4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+            *reinterpret_cast<uint32_t*>(row + kv8_column<kVec, kLayout>(i % per_row, n_freq, h)) = kv8_pack4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
         }
     }
     __syncthreads();                                                       // red is used again
 }
 
 // kJobs: jobs of a thread for 32 rows
-template <bool kVec, int kJobs>
-__global__ void __launch_bounds__(kKv8Threads) seq_rotary_kv8_kernel(Kv8Args p) {
+template <bool kVec, int kLayout, int kJobs>
+__global__ void __launch_bounds__(kKv8Threads, kJobs == 4 ? 8 : 4) seq_rotary_kv8_kernel(Kv8Args p) {
     after_previous();
     __shared__ float red[kKv8Threads / 32];
     const sllm_seq_batch& b = p.b;
@@ -166,13 +165,13 @@ __global__ void __launch_bounds__(kKv8Threads) seq_rotary_kv8_kernel(Kv8Args p) 
         }
         const int lo0 = pos0 / kKv8Block * kKv8Block + from * kKv8Block;
         for (int i = 0; i < n_blocks && lo0 + i * kKv8Block < pos0 + len; ++i) {
-            if (values) kv8_block<kVec, kJobs>(p, tok0, pos0, len, slot, lo0 + i * kKv8Block, g, p.v, p.ldv, p.dv, 0, p.v_pool, p.v_scale, red);
-            else kv8_block<kVec, kJobs>(p, tok0, pos0, len, slot, lo0 + i * kKv8Block, g, p.k, p.ldk, p.dk, p.n_freq, p.k_pool, p.k_scale, red);
+            if (values) kv8_block<kVec, kLayout, kJobs>(p, tok0, pos0, len, slot, lo0 + i * kKv8Block, g, p.v, p.ldv, p.dv, 0, p.v_pool, p.v_scale, red);
+            else kv8_block<kVec, kLayout, kJobs>(p, tok0, pos0, len, slot, lo0 + i * kKv8Block, g, p.k, p.ldk, p.dk, p.n_freq, p.k_pool, p.k_scale, red);
         }
         return;
     }
     const int t = (blockIdx.x - cache) / p.q_split, part = (blockIdx.x - cache) % p.q_split;
-    if (b.tok_slot[t] < 0) return;                                         // a place without a token
+    const bool token = b.tok_slot[t] >= 0;                                 // or a place without one: its row is read, but nothing is stored (asked for beside the rows, not in front)
     const float *q = p.q + (size_t)t * p.ldq, *angles = p.angles + (size_t)t * 2 * p.n_freq;
     float* out = p.q_out + (size_t)t * p.ldqo;
     // in place only what turns has to move
@@ -181,25 +180,26 @@ __global__ void __launch_bounds__(kKv8Threads) seq_rotary_kv8_kernel(Kv8Args p) 
     if constexpr (kVec) {
         for (int i0 = part * kKv8Threads + threadIdx.x; i0 < jobs; i0 += kAhead * p.q_split * kKv8Threads) {
             float x[kAhead][8];
-            int at[kAhead][2];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 const int i = i0 + j * p.q_split * kKv8Threads;
-                if (i < jobs) kv8_load<true>(q + (size_t)(i / per_head) * p.dk, angles, p.n_freq, p.layout, i % per_head, at[j], x[j]);
+                if (i < jobs) kv8_load<true, kLayout>(q + (size_t)(i / per_head) * p.dk, angles, p.n_freq, i % per_head, x[j]);
             }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 const int i = i0 + j * p.q_split * kKv8Threads;
-                if (i >= jobs) break;
+                if (i >= jobs || !token) break;
                 float* row = out + (size_t)(i / per_head) * p.dk;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(row + at[j][h]) = make_float4(x[j][4 * h], x[j][4 * h + 1], x[j][4 * h + 2], x[j][4 * h + 3]);
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<float4*>(row + kv8_column<true, kLayout>(i % per_head, p.n_freq, h)) = make_float4(x[j][4 * h], x[j][4 * h + 1], x[j][4 * h + 2], x[j][4 * h + 3]);
             }
         }
     } else {                                                               // pair by pair: both halves belong to one thread, so that rows may be turned in place
+        if (!token) return;
         const int pairs = p.heads * p.n_freq;
         for (int i = part * kKv8Threads + threadIdx.x; i < pairs; i += p.q_split * kKv8Threads) {
-            const int h = i / p.n_freq, m = i % p.n_freq, ia = p.layout ? m : 2 * m, ib = p.layout ? m + p.n_freq : 2 * m + 1;
+            const int h = i / p.n_freq, m = i % p.n_freq, ia = kLayout ? m : 2 * m, ib = kLayout ? m + p.n_freq : 2 * m + 1;
             const float u = q[(size_t)h * p.dk + ia], w = q[(size_t)h * p.dk + ib], cs = angles[2 * m], sn = angles[2 * m + 1];
             out[(size_t)h * p.dk + ia] = __fsub_rn(__fmul_rn(u, cs), __fmul_rn(w, sn));
             out[(size_t)h * p.dk + ib] = __fadd_rn(__fmul_rn(w, cs), __fmul_rn(u, sn));
@@ -213,10 +213,10 @@ __global__ void __launch_bounds__(kKv8Threads) seq_rotary_kv8_kernel(Kv8Args p) 
     }
 }
 
-template <bool kVec>
+template <bool kVec, int kLayout>
 static void launch_rotary_kv8(const Kv8Args& p, unsigned grid, cudaStream_t st) {
-    if (max(p.dk, p.dv) <= 128) overlapping(seq_rotary_kv8_kernel<kVec, 4>)<<<grid, kKv8Threads, 0, st>>>(p);
-    else overlapping(seq_rotary_kv8_kernel<kVec, 8>)<<<grid, kKv8Threads, 0, st>>>(p);
+    if (max(p.dk, p.dv) <= 128) overlapping(seq_rotary_kv8_kernel<kVec, kLayout, 4>)<<<grid, kKv8Threads, 0, st>>>(p);
+    else overlapping(seq_rotary_kv8_kernel<kVec, kLayout, 8>)<<<grid, kKv8Threads, 0, st>>>(p);
 }
 
 }  // namespace sllm
@@ -237,7 +237,7 @@ extern "C" int sllm_seq_rotary_kv8(const sllm_seq_batch* b, const float* q, int3
     SLLM_REQUIRE(ldq >= heads * dk && ldqo >= heads * dk && ldk >= kv_heads * dk && ldv >= kv_heads * dv, SLLM_EINVAL, "seq_rotary_kv8: a row is shorter than its heads");
     SLLM_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) % 16) == 0, SLLM_EINVAL, "seq_rotary_kv8: pools have to start at a multiple of 16 bytes");
     SLLM_REQUIRE(q != q_out || ldq == ldqo, SLLM_EINVAL, "seq_rotary_kv8: queries in place keep their row stride");
-    Kv8Args p{*b, q, k, v, angles, q_out, k_scale, v_scale, (uint8_t*)k_pool, (uint8_t*)v_pool, ldq, ldk, ldv, ldqo, heads, kv_heads, dk, dv, n_freq, layout, n_pages, 0, 1, nullptr};
+    Kv8Args p{*b, q, k, v, angles, q_out, k_scale, v_scale, (uint8_t*)k_pool, (uint8_t*)v_pool, ldq, ldk, ldv, ldqo, heads, kv_heads, dk, dv, n_freq, n_pages, 0, 1, nullptr};
     // a segment of n tokens touches (n + 62) / 32 blocks at most, and no more than it has tokens
     p.units = b->T == b->nseg ? b->nseg : (int)std::min<long long>(b->T, (b->T + 62LL * b->nseg) / kKv8Block);
     constexpr int kMostSplit = 8;
@@ -249,8 +249,9 @@ extern "C" int sllm_seq_rotary_kv8(const sllm_seq_batch* b, const float* q, int3
     p.q_split = b->T >= 2 * sm_count() ? 1 : std::max(1, std::min(kMostSplit, (jobs + kKv8Threads - 1) / kKv8Threads));
     const unsigned grid = (unsigned)(p.units * 2 * kv_heads + b->T * p.q_split);
     const bool vec = ((ldq | ldqo | ldk | ldv | n_freq) % 4) == 0 && (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)angles) % 16) == 0;
-    if (vec) launch_rotary_kv8<true>(p, grid, as_stream(stream));
-    else launch_rotary_kv8<false>(p, grid, as_stream(stream));
+    cudaStream_t st = as_stream(stream);
+    if (layout) vec ? launch_rotary_kv8<true, 1>(p, grid, st) : launch_rotary_kv8<false, 1>(p, grid, st);
+    else vec ? launch_rotary_kv8<true, 0>(p, grid, st) : launch_rotary_kv8<false, 0>(p, grid, st);
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
