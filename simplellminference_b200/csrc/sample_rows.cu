@@ -21,7 +21,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kSrThreads = 512, kSrWarps = kSrThreads / 32, kSrCluster = 16;
 constexpr int kSrSlice = 44 * 1024;              // logits of a CTA at most (176 KB)
-constexpr int kSrBins = 1024, kSrFew = 512;      // bins; logits that one CTA compares pair by pair
+constexpr int kSrBins = 1024, kSrFew = 512, kSrPairs = 128;   // bins; logits that one CTA can hold; up to which it compares them pair by pair rather than have their bins divided
 constexpr double kSrOne = 17592186044416.0;      // 2^44: the weights of 720896 logits add up to less than 2^64
 
 struct SampleRows {
@@ -61,23 +61,19 @@ struct alignas(16) SrShared {
     double powers[32];
     uint64_t slot[2][kSrCluster];        // what the CTAs of the cluster have sent, two sums in turn
     uint64_t warp[kSrWarps], before[kSrWarps];
-    // bins: counts and weights of this CTA's logits; sums over the cluster for the bins this CTA adds up, and of all CTAs' bins
-    uint32_t count[kSrBins], part[3][kSrBins];
-    uint64_t all_mass[kSrBins];
-    uint32_t all_count[kSrBins];
-    uint64_t cta_mass[kSrCluster];
-    uint32_t cta_count[kSrCluster];
+    uint32_t count[2][kSrBins];          // this CTA's logits by bin, and by part of the bins around the border
+    double2 span[kSrWarps];
+    uint32_t span_n[kSrWarps];
+    uint64_t aside[2][kSrCluster][2];    // weights of every CTA's logits before and behind the window
     // candidates, in the first CTA
     float x[kSrFew];
     int at[kSrFew];
     uint64_t w[kSrFew];
-    uint32_t listed, lowest;
+    uint32_t listed, lowest, top_key;
     float tops[kSrCluster * kSrWarps];   // the largest logit of every warp of the cluster
-    // where a border lies: the bin, and what lies in bins before it and in it
-    int bin;
-    uint64_t mass_before;
-    uint32_t count_before, count_in;
-    float threshold;
+    int bins[2];                         // the first and the last bin that may hold the border
+    uint32_t counts[2];                  // logits in the bins before the first, and up to the last
+    float threshold, highest;            // the last value that stays, and the largest logit that was compared for it
 };
 
 __device__ __forceinline__ uint64_t sr_warp_sum(uint64_t v) {
@@ -115,27 +111,58 @@ __device__ __forceinline__ uint64_t sr_all(uint64_t v, SrShared& sh, int& turn, 
     return v;
 }
 
-// exclusive sum over the CTA, and the total
-template <typename T>
-__device__ __forceinline__ T sr_scan(T v, T* warps, T& total) {
-    T upto = v;
+// sums over the threads in front, and over all
+struct SrSpan {
+    double low, high;          // of bounds of the weights
+    uint32_t n;
+};
+__device__ __forceinline__ SrSpan sr_scan(SrSpan v, SrShared& sh, bool mass, SrSpan& total) {
+    SrSpan upto = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const T x = __shfl_up_sync(0xffffffffu, upto, o);
-        if ((int)(threadIdx.x & 31) >= o) upto += x;
+        const bool in = (int)(threadIdx.x & 31) >= o;
+        const uint32_t n = __shfl_up_sync(0xffffffffu, upto.n, o);
+        upto.n += in ? n : 0;
+        if (mass) {
+            const double l = __shfl_up_sync(0xffffffffu, upto.low, o), h = __shfl_up_sync(0xffffffffu, upto.high, o);
+            upto.low += in ? l : 0.0;
+            upto.high += in ? h : 0.0;
+        }
+    }
+    if ((threadIdx.x & 31) == 31) {
+        sh.span_n[threadIdx.x >> 5] = upto.n;
+        sh.span[threadIdx.x >> 5] = make_double2(upto.low, upto.high);
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 31) warps[threadIdx.x >> 5] = upto;
-    __syncthreads();
-    T before = 0;
-    total = 0;
+    SrSpan before{0.0, 0.0, 0};
+    total = before;
 #pragma unroll
     for (int i = 0; i < kSrWarps; ++i) {
-        const T x = warps[i];
-        if (i < (int)(threadIdx.x >> 5)) before += x;
-        total += x;
+        const bool in = i < (int)(threadIdx.x >> 5);
+        const uint32_t n = sh.span_n[i];
+        total.n += n;
+        before.n += in ? n : 0;
+        if (mass) {
+            const double2 x = sh.span[i];
+            total.low += x.x;
+            total.high += x.y;
+            before.low += in ? x.x : 0.0;
+            before.high += in ? x.y : 0.0;
+        }
     }
-    return before + upto - v;
+    return SrSpan{before.low + upto.low - v.low, before.high + upto.high - v.high, before.n + upto.n - v.n};
+}
+
+// n candidates, each looked at by so many neighbouring threads that all have work
+__device__ __forceinline__ int sr_share(int n) {
+    int s = 32;
+    while (s * n > kSrThreads) s >>= 1;
+    return s;
+}
+template <typename T>
+__device__ __forceinline__ T sr_share_sum(T v, int share) {
+    for (int o = share >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 // One row, by the CTAs of a cluster.
@@ -146,161 +173,243 @@ struct SrWork {
     const float* s_x;
     int lo, hi, rank, size, turn;        // this warp's run
     float mine;                          // its largest logit
+    uint64_t front;                      // after a search by weight that ended with a list: the weights of this thread's logits larger than all on it,
+    float highest;                       // the largest one on it; else 0 and infinity
     float far, scale;                    // distances to the largest logit beyond which a weight is 0; bins in a distance of 1: the last one begins there
-    // f(logit, place in the CTA's slice) for every logit of this warp's run, if one of them is not below `least`
+    // f(logit, place in the CTA's slice) for every logit of this warp's run, if one of them is not below `least`; four at a time
     template <typename F>
     __device__ __forceinline__ void each(float least, F f) const {
         if (mine < least) return;
-        for (int i = lo + (int)(threadIdx.x & 31); i < hi; i += 32) f(s_x[i], i);
+        int i = lo + (int)(threadIdx.x & 31);
+        for (; i + 96 < hi; i += 128) {
+            const float x[4] = {s_x[i], s_x[i + 32], s_x[i + 64], s_x[i + 96]};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f(x[k], i + 32 * k);
+        }
+        for (; i < hi; i += 32) f(s_x[i], i);
+    }
+    // f(weight, place) of those for which is(logit); four weights at a time: their arithmetic is one long chain each
+    template <typename G, typename F>
+    __device__ __forceinline__ void weigh(float least, G is, F f) const {
+        if (mine < least || r.top - mine > far) return;
+        for (int i = lo + (int)(threadIdx.x & 31); i < hi; i += 128) {
+            float x[4];
+            bool in[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                x[k] = i + 32 * k < hi ? s_x[i + 32 * k] : -INFINITY;
+                in[k] = !(r.top - x[k] > far) && x[k] > -INFINITY && is(x[k]);
+            }
+            if (in[0] || in[1] || in[2] || in[3]) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t w = r.weight_of(x[k]);
+                    f(in[k] ? w : 0, x[k]);
+                }
+            }
+        }
     }
 
     __device__ __forceinline__ void barrier() { if (size == 1) __syncthreads(); else cluster.sync(); }
-    __device__ __forceinline__ uint64_t weight(float x) const { return r.top - x > far ? 0 : r.weight_of(x); }      // (inf - inf is no number: not beyond)
+    __device__ __forceinline__ uint64_t weight(float x) const { return r.top - x > far || x == -INFINITY ? 0 : r.weight_of(x); }      // (inf - inf is no number: not beyond)
     __device__ __forceinline__ int bin_of(float d) const { return (int)fminf(d * scale, (float)(kSrBins - 1)); }
-    __device__ __forceinline__ void clear() {
-        for (int i = threadIdx.x; i < kSrBins; i += kSrThreads) sh.count[i] = sh.part[0][i] = sh.part[1][i] = sh.part[2][i] = 0;
-        if (threadIdx.x == 0) { sh.listed = 0; sh.lowest = 0xffffffffu; }
+    // The bins (parts of bins [b0, b0 + width), kSrBins of them, where inner) that may hold the border, and the logits in front and up to the last one, into sh.bins and sh.counts; the counts
+    // are complete, m0 and m1 lie in front of and behind the bins. By count the border is known. By weight, the mass in front of it is less than `share` of all, and that up to its end is not:
+    // (1 - share) * front < share * rest. A bin's logits weigh between what its two ends do (3 % apart, or that by the number of parts), so that the border lies in one of very few bins.
+    __device__ __forceinline__ void border(const uint32_t* count, bool by_mass, uint64_t top_k, double share, bool inner, int b0, int width, uint64_t m0, uint64_t m1, uint32_t n0) {
+        uint32_t n[2] = {0, 0};
+        constexpr int kAhead = 8;                                        // CTAs asked at once
+        for (int k0 = 0; k0 < size; k0 += kAhead) {
+            uint2 c[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) c[k] = reinterpret_cast<const uint2*>(cluster.map_shared_rank(count, min(k0 + k, size - 1)))[threadIdx.x];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                n[0] += k0 + k < size ? c[k].x : 0;
+                n[1] += k0 + k < size ? c[k].y : 0;
+            }
+        }
+        double low[2] = {0.0, 0.0}, high[2] = {0.0, 0.0};
+        if (by_mass) {
+            // bits of weight a bin; places are rounded to 2^-12 of a bin at most, weights to whole numbers
+            const float bits = 46.0f * 1.0001f / (kSrBins - 1), step = inner ? (float)width / kSrBins : 1.0f, slack = 1.0f / 1024;
+            const bool even = scale > 0.0f && scale < INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = 2 * (int)threadIdx.x + i;
+                const float d = (float)b0 + at * step;
+                // the last bin holds everything beyond it; a temperature whose bins have no width in fp32 (or no end) tells nothing
+                const float h = even ? exp2f(-bits * (d - slack)) * 1.00001f : 1.0f, l = even && !(at == kSrBins - 1 && b0 + width == kSrBins) ? exp2f(-bits * (d + step + slack)) * 0.99999f : 0.0f;
+                high[i] = n[i] * ((double)h * kSrOne + 1.0);
+                low[i] = n[i] * fmax((double)l * kSrOne - 1.0, 0.0);
+            }
+        }
+        SrSpan all;
+        SrSpan v = sr_scan(SrSpan{low[0] + low[1], high[0] + high[1], n[0] + n[1]}, sh, by_mass, all);
+        const double front = (double)m0, behind = (double)m1, tiny = 1e-12 * (front + behind + all.high);
+        if (threadIdx.x == 0) { sh.bins[0] = kSrBins; sh.bins[1] = -1; }
         __syncthreads();
-    }
-    __device__ __forceinline__ void add(int bin, uint64_t w, bool mass) {
-        atomicAdd(&sh.count[bin], 1u);
-        if (!mass) return;
-        const uint32_t a = (uint32_t)w & 0xffffu, b = (uint32_t)(w >> 16) & 0xffffu, c = (uint32_t)(w >> 32);
-        if (a) atomicAdd(&sh.part[0][bin], a);
-        if (b) atomicAdd(&sh.part[1][bin], b);
-        if (c) atomicAdd(&sh.part[2][bin], c);
-    }
-    static __device__ __forceinline__ uint64_t join(uint32_t a, uint32_t b, uint32_t c) { return (uint64_t)a + ((uint64_t)b << 16) + ((uint64_t)c << 32); }
-
-    // The bin at which what has been counted (or weighed) reaches `need`, of two neighbouring bins a thread (the first one those from first_bin on): into sh.bin and what lies before it
-    __device__ __forceinline__ void border(const uint64_t (&mass)[2], const uint32_t (&n)[2], int first_bin, uint64_t mass0, uint32_t n0, bool by_mass, double need) {
-        uint64_t all_m;
-        uint32_t all_n;
-        const uint64_t m = mass0 + sr_scan(mass[0] + mass[1], sh.warp, all_m);
-        const uint32_t c = n0 + sr_scan(n[0] + n[1], reinterpret_cast<uint32_t*>(sh.before), all_n);
-        uint64_t mb = m;
-        uint32_t cb = c;
+        bool may[2];
+        uint32_t before[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const double from = by_mass ? (double)mb : (double)cb, to = by_mass ? (double)(mb + mass[i]) : (double)(cb + n[i]);
-            if (from < need && to >= need) {
-                sh.bin = first_bin + 2 * (int)threadIdx.x + i;
-                sh.mass_before = mb;
-                sh.count_before = cb;
-                sh.count_in = n[i];
+            before[i] = v.n;
+            if (by_mass) {
+                const double least = front + v.low, rest = behind + (all.high - v.high);                   // in front of it at least, and from it on at most
+                v.low += low[i];
+                v.high += high[i];
+                may[i] = (1.0 - share) * (least - tiny) < share * (rest + tiny) && (1.0 - share) * (front + v.high + tiny) >= share * (behind + (all.low - v.low) - tiny);
+            } else {
+                may[i] = n0 + v.n < top_k && n0 + v.n + n[i] >= top_k;
             }
-            mb += mass[i];
-            cb += n[i];
+            v.n += n[i];
+            may[i] = may[i] && n[i] > 0;
+            if (may[i]) {
+                atomicMin(&sh.bins[0], 2 * (int)threadIdx.x + i);
+                atomicMax(&sh.bins[1], 2 * (int)threadIdx.x + i);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int at = 2 * (int)threadIdx.x + i;
+            if (at == sh.bins[0]) sh.counts[0] = before[i];
+            if (at == sh.bins[1]) sh.counts[1] = before[i] + n[i];
         }
         __syncthreads();
     }
 
-    // which bin (outer < 0), or which part of bin `outer`, a logit belongs to; -1: none
-    __device__ __forceinline__ int place(float x, int outer) const {
-        const float d = r.top - x;
-        if (outer < 0) return bin_of(d);
-        return bin_of(d) == outer ? (int)fminf(fmaxf(fmaf(d, scale, -(float)outer) * kSrBins, 0.0f), (float)(kSrBins - 1)) : -1;
+    // this CTA's weights before and behind the window to every CTA
+    __device__ __forceinline__ void send_aside(uint64_t front, uint64_t behind, int buffer) {
+        front = sr_warp_sum(front);
+        behind = sr_warp_sum(behind);
+        if ((threadIdx.x & 31) == 0) { sh.warp[threadIdx.x >> 5] = front; sh.before[threadIdx.x >> 5] = behind; }
+        __syncthreads();
+        if ((int)threadIdx.x < 2 * size) {
+            const uint64_t* from = threadIdx.x & 1 ? sh.before : sh.warp;
+            uint64_t v = 0;
+#pragma unroll
+            for (int i = 0; i < kSrWarps; ++i) v += from[i];
+            cluster.map_shared_rank(&sh, threadIdx.x >> 1)->aside[buffer][rank][threadIdx.x & 1] = v;
+        }
+    }
+    __device__ __forceinline__ void take_aside(uint64_t& front, uint64_t& behind, int buffer) const {
+        for (int k = 0; k < size; ++k) { front += sh.aside[buffer][k][0]; behind += sh.aside[buffer][k][1]; }
     }
 
     // The least value that stays: of top_k of them (by_mass false), or of those that reach `share` of the mass of the logits from `above` on. small: a border by count that
     // leaves no more than kSrFew candidates is not looked for; they are all in the first CTA's list then, and the answer is 0.
     __device__ float find(bool by_mass, uint64_t top_k, double share, float above, bool& small) {
-        double need = (double)top_k;
-        uint64_t m0 = 0;
-        uint32_t n0 = 0;
-        int outer = -1;
-        for (;;) {
-            clear();
-            each(above, [&](float x, int) {
-                const int bin = x >= above ? place(x, outer) : -1;
-                if (bin >= 0) add(bin, by_mass ? weight(x) : 0, by_mass);
-            });
-            barrier();                                                   // every CTA's bins are there
-            const int own = kSrBins / size, b0 = rank * own;
-            uint64_t mass = 0;
-            uint32_t n = 0;
-            for (int i = threadIdx.x; i < own; i += kSrThreads) {
-                uint32_t c = 0;
-                uint64_t m = 0;
-                for (int k = 0; k < size; ++k) {
-                    const SrShared* o = cluster.map_shared_rank(&sh, k);
-                    c += o->count[b0 + i];
-                    if (by_mass) m += join(o->part[0][b0 + i], o->part[1][b0 + i], o->part[2][b0 + i]);
-                }
-                sh.all_count[i] = c;
-                sh.all_mass[i] = m;
-                mass += m;
-                n += c;
-            }
-            uint64_t all_m;
-            uint32_t all_n;
-            sr_scan(mass, sh.warp, all_m);
-            sr_scan(n, reinterpret_cast<uint32_t*>(sh.before), all_n);
-            if ((int)threadIdx.x < size) {
-                SrShared* o = cluster.map_shared_rank(&sh, threadIdx.x);
-                o->cta_mass[rank] = all_m;
-                o->cta_count[rank] = all_n;
-            }
-            barrier();
-            if (by_mass && outer < 0) {
-                uint64_t total = 0;
-                for (int k = 0; k < size; ++k) total += sh.cta_mass[k];
-                need = share * (double)total;
-            }
-            // the CTA whose bins hold the border; everybody looks at them
-            int owner = 0;
-            for (; owner < size - 1; ++owner) {
-                const double to = by_mass ? (double)(m0 + sh.cta_mass[owner]) : (double)(n0 + sh.cta_count[owner]);
-                if (to >= need) break;
-                m0 += sh.cta_mass[owner];
-                n0 += sh.cta_count[owner];
-            }
-            const SrShared* o = cluster.map_shared_rank(&sh, owner);
-            uint64_t mm[2];
-            uint32_t nn[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int at = 2 * threadIdx.x + i;
-                mm[i] = at < own ? o->all_mass[at] : 0;
-                nn[i] = at < own ? o->all_count[at] : 0;
-            }
-            border(mm, nn, owner * own, m0, n0, by_mass, need);
-            const int bin = sh.bin;
-            const uint32_t in = sh.count_in;
-            m0 = sh.mass_before;
-            n0 = sh.count_before;
-            small = small && !by_mass && outer < 0 && n0 + in <= kSrFew;
-            if (!small && in > kSrFew) {
-                if (outer >= 0 || bin == kSrBins - 1) return crowded(by_mass, need, above, outer, bin);
-                outer = bin;
-                continue;
-            }
-            // candidates to the first CTA: the border's bin, or everything up to it
-            SrShared* first = cluster.map_shared_rank(&sh, 0);
+        for (int i = threadIdx.x; i < 2 * kSrBins; i += kSrThreads) (&sh.count[0][0])[i] = 0;
+        if (threadIdx.x == 0) { sh.listed = 0; sh.lowest = 0xffffffffu; }
+        __syncthreads();
+        each(above, [&](float x, int) {
+            if (x >= above) atomicAdd(&sh.count[0][bin_of(r.top - x)], 1u);
+        });
+        barrier();                                                       // every CTA's bins are there, its list is empty
+        uint64_t m0 = 0, m1 = 0;
+        highest = INFINITY;
+        border(sh.count[0], by_mass, top_k, share, false, 0, kSrBins, 0, 0, 0);
+        const int b0 = sh.bins[0], b1 = sh.bins[1];
+        uint32_t n0 = sh.counts[0], upto = sh.counts[1];
+        small = small && !by_mass && upto <= kSrFew;
+        SrShared* first = cluster.map_shared_rank(&sh, 0);
+        auto list = [&](float x, int i) {
+            const uint32_t to = atomicAdd(&first->listed, 1u);
+            first->x[to] = x;
+            first->at[to] = (rank << 20) | i;
+        };
+        front = 0;
+        uint64_t behind = 0;
+        if (small || upto - n0 <= kSrPairs) {                            // everything up to the border, or what lies around it
             each(above, [&](float x, int i) {
-                const int b = x >= above ? place(x, outer) : -1;
-                if (b >= 0 && (small ? b <= bin : b == bin)) {
-                    const uint32_t to = atomicAdd(&first->listed, 1u);
-                    first->x[to] = x;
-                    first->at[to] = (rank << 20) | i;
-                }
+                const int b = bin_of(r.top - x);
+                if (x >= above && b <= b1 && (small || b >= b0)) list(x, i);
             });
+            if (by_mass) {
+                weigh(above, [&](float x) { const int b = bin_of(r.top - x); return x >= above && (b < b0 || b > b1); }, [&](uint64_t y, float x) {
+                    front += bin_of(r.top - x) < b0 ? y : 0;
+                    behind += y;
+                });
+                send_aside(front, behind - front, 0);
+            }
             barrier();
             if (small) return 0.0f;
-            if (rank == 0) {                                             // pair by pair: one stays when what lies above it is not yet enough
-                const bool is = threadIdx.x < in;
-                const float x = is ? sh.x[threadIdx.x] : 0.0f;
-                if (is) sh.w[threadIdx.x] = by_mass ? weight(x) : 1;
-                __syncthreads();
-                uint64_t v = by_mass ? m0 : n0;
-                for (uint32_t k = 0; k < in; ++k) v += sh.x[k] > x ? sh.w[k] : 0;
-                if (is && (double)v < need) atomicMin(&sh.lowest, sr_key(x));
-                __syncthreads();
-                if (threadIdx.x == 0) sh.threshold = sr_float(sh.lowest);
+            if (by_mass) take_aside(m0, m1, 0);
+        } else {
+            const float parts = (float)kSrBins / (b1 - b0 + 1);
+            auto part_of = [&](float d) { return (int)fminf(fmaxf(fmaf(d, scale, -(float)b0) * parts, 0.0f), (float)(kSrBins - 1)); };
+            each(above, [&](float x, int) {
+                const int b = bin_of(r.top - x);
+                if (x >= above && b >= b0 && b <= b1) atomicAdd(&sh.count[1][part_of(r.top - x)], 1u);
+            });
+            if (by_mass) {
+                weigh(above, [&](float x) { const int b = bin_of(r.top - x); return x >= above && (b < b0 || b > b1); }, [&](uint64_t y, float x) {
+                    front += bin_of(r.top - x) < b0 ? y : 0;
+                    behind += y;
+                });
+                send_aside(front, behind - front, 0);
             }
             barrier();
-            return cluster.map_shared_rank(&sh, 0)->threshold;
+            if (by_mass) take_aside(m0, m1, 0);
+            const uint32_t outside = n0;
+            border(sh.count[1], by_mass, top_k, share, true, b0, b1 - b0 + 1, m0, m1, n0);
+            const int c0 = sh.bins[0], c1 = sh.bins[1];
+            n0 = outside + sh.counts[0];
+            upto = outside + sh.counts[1];
+            if (upto - n0 > kSrFew) {
+                front = 0;
+                SrWork copy = *this;                                     // (its address is taken: the fields of this one stay in registers)
+                const float found = copy.crowded(by_mass, top_k, share, above);
+                turn = copy.turn;
+                return found;
+            }
+            uint64_t inner = 0;
+            behind = 0;
+            each(above, [&](float x, int i) {
+                const int b = bin_of(r.top - x);
+                if (x < above || b < b0 || b > b1) return;
+                const int c = part_of(r.top - x);
+                if (c >= c0 && c <= c1) list(x, i);
+                else if (by_mass) {
+                    const uint64_t y = weight(x);
+                    inner += c < c0 ? y : 0;
+                    behind += c > c1 ? y : 0;
+                }
+            });
+            if (by_mass) send_aside(inner, behind, 1);
+            front += inner;
+            barrier();
+            if (by_mass) take_aside(m0, m1, 1);
         }
+        if (rank == 0) {                                                 // pair by pair: one stays when what lies above it is not yet enough
+            const int in = (int)(upto - n0), split = sr_share(in), at = threadIdx.x / split, part = threadIdx.x % split;
+            const float x = at < in ? sh.x[at] : 0.0f;
+            if (at < in && part == 0) sh.w[at] = by_mass ? weight(x) : 1;
+            if (threadIdx.x == 0) sh.top_key = 0;
+            __syncthreads();
+            uint64_t v = 0, all = 0;
+            if (at < in) {
+#pragma unroll 4
+                for (int k = part; k < in; k += split) {
+                    const uint64_t y = sh.w[k];
+                    all += y;
+                    v += sh.x[k] > x ? y : 0;
+                }
+            }
+            v = (by_mass ? m0 : n0) + sr_share_sum(v, split);
+            all = sr_share_sum(all, split);
+            const double need = by_mass ? share * (double)(m0 + m1 + all) : (double)top_k;
+            if (at < in) {
+                if ((double)v < need) atomicMin(&sh.lowest, sr_key(x));
+                atomicMax(&sh.top_key, sr_key(x));
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) { sh.threshold = sr_float(sh.lowest); sh.highest = sr_float(sh.top_key); }
+        }
+        barrier();
+        if (by_mass) highest = first->highest;
+        return first->threshold;
     }
 
     // A top_k below the number of the cluster's warps: the top_k-th largest of the warps' largest logits is no larger than the top_k-th largest of all, so that the candidates lie from there
@@ -309,11 +418,14 @@ struct SrWork {
         if (top_k * 8 > groups * 7) return false;
         if (threadIdx.x == 0) { sh.listed = 0; sh.lowest = 0xffffffffu; }
         __syncthreads();
-        if ((int)threadIdx.x < groups) {
-            const float x = sh.tops[threadIdx.x];
-            int above = 0;
-            for (int k = 0; k < groups; ++k) above += sh.tops[k] > x;
-            if (above < top_k) atomicMin(&sh.lowest, sr_key(x));
+        const int split = sr_share(groups), at = threadIdx.x / split;
+        if (at < groups) {
+            const float x = sh.tops[at];
+            int larger = 0;
+#pragma unroll 8
+            for (int k = threadIdx.x % split; k < groups; k += split) larger += sh.tops[k] > x;
+            larger = sr_share_sum(larger, split);                        // (kSrThreads / split divides groups: whole warps are here)
+            if (larger < top_k) atomicMin(&sh.lowest, sr_key(x));
         }
         __syncthreads();
         const float bound = sr_float(sh.lowest);
@@ -335,15 +447,17 @@ struct SrWork {
     }
 
     // The border lies among more candidates than the list holds: all alike, or halved bit by bit
-    __device__ __noinline__ float crowded(bool by_mass, double need, float above, int outer, int bin) {
-        uint64_t high = 0, low = 0;
+    __device__ __noinline__ float crowded(bool by_mass, uint64_t top_k, double share, float above) {
+        uint64_t high = 0, low = 0, all = 0;
         each(above, [&](float x, int) {
-            if (x < above || place(x, outer) != bin) return;
+            if (x < above) return;
             high = max(high, (uint64_t)sr_key(x));
             low = max(low, (uint64_t)~sr_key(x));
+            all += by_mass ? weight(x) : 0;
         });
         high = sr_all<true>(high, sh, turn, cluster);
         low = (uint32_t)~(uint32_t)sr_all<true>(low, sh, turn, cluster);
+        const double need = by_mass ? share * (double)sr_all<false>(all, sh, turn, cluster) : (double)top_k;
         // the largest key from `low` on at which there is enough; at `low` there is
         uint32_t from = (uint32_t)low, to = (uint32_t)high;
         while (from < to) {
@@ -434,7 +548,7 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p
     // beyond this distance a weight is below 2^-45 (or well below min_p: log2 in fp32 is off by less than a thousandth of that here)
     const float bits = min_p > 0.0f ? fminf(46.0f, -log2f(fminf(min_p, 1.0f)) + 0.01f) : 46.0f;
     const float reach = 46.0f * 0.6931472f * temperature * 1.0001f;
-    SrWork w{sh, cluster, r, s_x, lo, hi, rank, size, turn, best, reach, (float)(kSrBins - 1) / reach};
+    SrWork w{sh, cluster, r, s_x, lo, hi, rank, size, turn, best, 0, INFINITY, reach, (float)(kSrBins - 1) / reach};
     const float far = bits * 0.6931472f * temperature * 1.0001f;
     float thr = -INFINITY;                                          // kept: from there on
     if (r.top < INFINITY) {                                         // (of infinite logits all are kept, and nothing else weighs anything)
@@ -443,37 +557,54 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p
             thr = w.few(top_k, groups) ? 0.0f : w.find(false, (uint64_t)top_k, 0.0, -INFINITY, small);
             if (small) {                                            // the first CTA has all that may stay
                 if (rank != 0) return;
-                const int n = (int)sh.listed, i = threadIdx.x;
-                const float mine = i < n ? sh.x[i] : -INFINITY;
-                const int at = i < n ? (sh.at[i] >> 20) * p.slice + (sh.at[i] & 0xfffff) : 0x7fffffff;
+                const int n = (int)sh.listed, split = sr_share(n), i = threadIdx.x / split, part = threadIdx.x % split;
+                const bool is = i < n;
+                const float mine = is ? sh.x[i] : -INFINITY;
+                const int at = is ? (sh.at[i] >> 20) * p.slice + (sh.at[i] & 0xfffff) : 0x7fffffff;
                 int above = 0;
-                for (int k = 0; k < n; ++k) above += sh.x[k] > mine;
-                uint64_t mass = i < n && above < top_k ? w.weight(mine) : 0;
+                if (is) {
+#pragma unroll 4
+                    for (int k = part; k < n; k += split) above += sh.x[k] > mine;
+                }
+                above = sr_share_sum(above, split);
+                uint64_t mass = is && above < top_k ? w.weight(mine) : 0;
                 __syncthreads();
-                if (i < n) { sh.w[i] = mass; sh.at[i] = at; }
+                if (is && part == 0) { sh.w[i] = mass; sh.at[i] = at; }
                 __syncthreads();
                 uint64_t all = 0, higher = 0;
-                for (int k = 0; k < n; ++k) {
-                    const uint64_t y = sh.w[k];
-                    all += y;
-                    higher += sh.x[k] > mine ? y : 0;
+                if (top_p > 0.0f && top_p < 1.0f) {
+                    if (is) {
+#pragma unroll 4
+                        for (int k = part; k < n; k += split) {
+                            const uint64_t y = sh.w[k];
+                            all += y;
+                            higher += sh.x[k] > mine ? y : 0;
+                        }
+                    }
+                    all = sr_share_sum(all, split);
+                    higher = sr_share_sum(higher, split);
+                    if (!((double)higher < (double)top_p * (double)all)) mass = 0;
                 }
-                if (top_p > 0.0f && top_p < 1.0f && !((double)higher < (double)top_p * (double)all)) mass = 0;
                 if (mass < least) mass = 0;
                 __syncthreads();
-                if (i < n) sh.w[i] = mass;
+                if (is && part == 0) sh.w[i] = mass;
                 __syncthreads();
                 uint64_t before = 0;
                 all = 0;
-                for (int k = 0; k < n; ++k) {
-                    const uint64_t y = sh.w[k];
-                    all += y;
-                    before += sh.at[k] < at ? y : 0;
+                if (is) {
+#pragma unroll 4
+                    for (int k = part; k < n; k += split) {
+                        const uint64_t y = sh.w[k];
+                        all += y;
+                        before += sh.at[k] < at ? y : 0;
+                    }
                 }
+                all = sr_share_sum(all, split);
+                before = sr_share_sum(before, split);
                 const double to = u > 0.0f ? fmin((double)u, 1.0) * (double)all : 0.0;
                 uint64_t target = (uint64_t)to;
                 if (target >= all) target = all - 1;
-                if (i < n && before <= target && target < before + mass) {
+                if (is && part == 0 && before <= target && target < before + mass) {
                     p.idx[row] = at;
                     if (p.prob) p.prob[row] = (float)((double)mass / (double)all);
                 }
@@ -486,15 +617,17 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p
         }
     }
     turn = w.turn;
+    w.far = far;
     auto kept = [&](float v) -> uint64_t {
-        if (v < thr || r.top - v > far) return 0;
+        if (v < thr || r.top - v > far || v == -INFINITY) return 0;
         const uint64_t y = r.weight_of(v);
         return y >= least ? y : 0;
     };
-    // the mass of the warp's run first, then the warp in whose run the target lies walks it
-    uint64_t mine = 0;
-    if (best >= thr && !(r.top - best > far))
-        for (int i = lo + lane; i < hi; i += 32) mine += kept(s_x[i]);
+    // the mass of the warp's run first (a search for top_p's border has weighed what lies above it already), then the warp in whose run the target lies walks it
+    const bool known = least == 0 && w.highest < INFINITY;
+    uint64_t mine = known ? w.front : 0;
+    const float high = known ? w.highest : INFINITY;
+    w.weigh(thr, [&](float v) { return v >= thr && v <= high; }, [&](uint64_t y, float) { mine += y >= least ? y : 0; });
     mine = sr_warp_sum(mine);
     if (lane == 0) sh.before[warp] = mine;
     const uint64_t all = sr_all<false>(lane == 0 ? mine : 0, sh, turn, cluster);
@@ -505,8 +638,21 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p
     uint64_t target = (uint64_t)at;                                 // running > at is running > floor(at) for whole numbers
     if (target >= all) target = all - 1;
     if (before <= target && target < before + mine) {
-        for (int i = lo; i < hi; i += 32) {
-            const uint64_t y = i + lane < hi ? kept(s_x[i + lane]) : 0;
+        // a lane adds up a run of its own (an odd number of logits: no two lanes meet in a bank) to find the one with the target in it, which is then looked at logit by logit
+        const int each = ((hi - lo + 31) / 32) | 1, from = min(hi, lo + lane * each), to = min(hi, from + each);
+        uint64_t own = 0;
+#pragma unroll 4
+        for (int i = from; i < to; ++i) own += kept(s_x[i]);
+        uint64_t past_own = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t z = __shfl_up_sync(0xffffffffu, past_own, o);
+            if (lane >= o) past_own += z;
+        }
+        const int who = __ffs(__ballot_sync(0xffffffffu, before + past_own > target)) - 1, end = __shfl_sync(0xffffffffu, to, who);
+        before += __shfl_sync(0xffffffffu, past_own - own, who);
+        for (int i = __shfl_sync(0xffffffffu, from, who); i < end; i += 32) {
+            const uint64_t y = i + lane < end ? kept(s_x[i + lane]) : 0;
             uint64_t upto = y;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {

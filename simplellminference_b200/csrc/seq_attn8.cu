@@ -131,9 +131,10 @@ int sllm_seq_attention8(const sllm_seq_batch* b, const float* q, int32_t ldq, in
     const bool narrow = dk <= 128 && dv <= 128 && (unsigned long long)n_pages * kv_heads * b->page_len < 1ull << 31;
     if (narrow) {
         const bool single = b->T == b->nseg;
-        if (int rc = launch_attention8_decode(p, single, ws, st)) return rc;
+        const bool tc = !single && attention8_tc_takes(p);
+        if (int rc = launch_attention8_decode(p, single, tc ? attention8_tc_width(p) : 0, ws, st)) return rc;
         if (single) return SLLM_OK;
-        if (attention8_tc_takes(p)) return launch_attention8_tc(p, ws, st);
+        if (tc) return launch_attention8_tc(p, ws, st);
     }
     const dim3 grid(b->n_qtiles, heads);
     const int least = narrow ? 2 : 1;

@@ -32,6 +32,8 @@ struct D8Tile {
 
 struct D8Args {
     Attn8Args a;
+    int plan_width;              // of the other kernel's plan, which CTA 0 makes (0: it is a worker like the others)
+    A8Plan* plan;
     int only;                    // the launch is the step's only one: it has no tiles of more than one query
     int sets, per_set;           // groups of query heads that a kv head's are divided into, and how many of them one holds
     int vec_q;                   // rows of queries can be read 16 bytes at a time
@@ -98,7 +100,8 @@ __device__ __forceinline__ D8Tile1 d8_tile(const D8Args& da, int tile) {
 }
 
 template <int D, int NT>       // column width of a head, rounded up; groups of four query heads
-__global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const D8Args da) {
+__global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                                                                           const __grid_constant__ D8Args da) {
     using Tile = D8Tile<D>;
     constexpr int kRing = Tile::kRing, kChunk = D / 8, kSteps = D / 16, kMt = D / 16, kHeads = 4 * NT;   // bytes of a value row a lane reads; k-steps of a score; 16-column tiles of a result
     const Attn8Args& p = da.a;
@@ -121,6 +124,12 @@ __global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     after_previous();
+    static_assert(kA8PlanSmem <= Tile::kSmem - 1024, "room for the plan");
+    if (da.plan_width && blockIdx.x == 0) {
+        a8_plan<kD8Warps * 32>(p, da.plan_width, da.plan, smem);
+        return;
+    }
+    const int worker = blockIdx.x - (da.plan_width != 0), workers = gridDim.x - (da.plan_width != 0);
 
     // ---- the row of all units, and this CTA's share of it ----
     const int per_tile = p.kv_heads * da.sets, n_tiles = b.n_qtiles;
@@ -148,11 +157,11 @@ __global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_
     }
     total *= per_tile;
     before *= per_tile;
-    const int ctas = (int)min((long long)gridDim.x, (total + kD8Least - 1) / kD8Least);
-    if ((int)blockIdx.x >= ctas) return;
+    const int ctas = (int)min((long long)workers, (total + kD8Least - 1) / kD8Least);
+    if (worker >= ctas) return;
     auto share = [&](int x) { return (long long)x * total / ctas; };
     auto owner = [&](long long u) { return (int)(((u + 1) * ctas - 1) / total); };
-    const long long begin = share(blockIdx.x), end = share(blockIdx.x + 1);
+    const long long begin = share(worker), end = share(worker + 1);
     if (begin >= before && begin < before + mine * per_tile) {
         long long at = before;
         for (int i = t0; i < t1; ++i) {
@@ -443,7 +452,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_
         fresh = 0;
         __syncthreads();
         const int first_cta = owner(item0), last_cta = owner(item1 - 1), parts = last_cta - first_cta + 1;
-        float* record = da.records + (size_t)(2 * blockIdx.x + (begin >= item0 ? 0 : 1)) * kA8Record;
+        float* record = da.records + (size_t)(2 * worker + (begin >= item0 ? 0 : 1)) * kA8Record;
         constexpr int kTail = kA8MaxHeads * 128;                               // where a record's references, sums and exponents begin
         // Sums of parts with references and exponents of their own, brought to the largest of each. A column's result: sum * 2^e / (den * 2^r); a query that sees no key gives 0.
         auto store = [&](int h, int col, float4 sum, float r, float den, int e) {
@@ -557,10 +566,12 @@ static int d8_launch(D8Args& a, const CUtensorMap& tmK, const CUtensorMap& tmV, 
     return SLLM_OK;
 }
 
-int launch_attention8_decode(const Attn8Args& p, bool only, void* ws, cudaStream_t st) {
+int launch_attention8_decode(const Attn8Args& p, bool only, int plan_width, void* ws, cudaStream_t st) {
     D8Args a{};
     a.a = p;
     a.only = only;
+    a.plan_width = plan_width;
+    a.plan = reinterpret_cast<A8Plan*>((uint8_t*)ws + kA8PlanAt);
     const int group = p.heads / p.kv_heads;
     a.sets = (group + kA8MaxHeads - 1) / kA8MaxHeads;
     a.per_set = (group + a.sets - 1) / a.sets;

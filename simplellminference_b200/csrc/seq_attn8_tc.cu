@@ -6,7 +6,7 @@
 //   warps 2, 3          codes to fp16 rows in the 128B swizzle (keys K-major, values as they lie); value rows that the run must not see, and NaN codes among values, become zeros;
 //   warp 1 (one lane)   MMA issuer: S = Q K^T, O += P V with P read from TMEM; P has columns of its own, so that the next scores are made while the softmax takes its exponentials;
 //   warps 4-7, 8-11     softmax of tile 0 / 1: queries to fp16 once an item; then, a thread per row, maximum, weights and their sum of every key tile;
-//   warps 12-15         O of both tiles: rescaled where a maximum has grown, results written, parts of shared items put together.
+//   warps 12-15         O of both tiles: rescaled where a maximum has grown, results or parts of them written.
 // Results in bf16 (kTerms = 1): queries and weights are one fp16 number each (2^-12 of a value on average less than the 2^-9 of the result's own rounding). Results in fp32 (kTerms = 2): both are
 // the sum of two (22 bits), and O is added to an fp32 copy of the CTA's own every kT8Flush tiles, because the tensor core truncates as it
 // accumulates.
@@ -14,8 +14,9 @@
 // seldom. The denominator takes the value scale out again, block by block.
 // A value's NaN code must reach exactly the rows that see it, but 0 * NaN is NaN: the converters replace it and say so, and rows of such an item look for NaN among their keys' values
 // at the end.
-// Shares. A CTA per item would leave most SMs idle where few queries follow a long context. The key tiles of all items lie in one row, made by a small kernel in front from what the
-// device knows (contexts, listed tiles); every CTA takes an equal run of it. Items that a cut goes through leave O, reference and sum as parts for the one of their CTAs that is done last.
+// Shares. A CTA per item would leave most SMs idle where few queries follow a long context. The key tiles of all items lie in one row, made by a CTA of the kernel in front from what the
+// device knows (contexts, listed tiles); every CTA takes an equal run of it. Items that a cut goes through leave O, reference and sum as parts, which a kernel behind puts together (done by
+// the last of an item's CTAs, one SM reading what up to ten had left, that took as long as all the rest).
 #include <type_traits>
 
 #include "seq_attn8.cuh"
@@ -23,8 +24,8 @@
 
 namespace sllm {
 
-constexpr int kT8Rows = 128, kT8Keys = 64, kT8Threads = 512;      // rows of a tile, keys of a tile
-constexpr int kT8Extra = 4, kT8Least = 4;       // key tiles that an item's beginning and end count for; key tiles of a CTA's share at least
+constexpr int kT8Rows = 128, kT8Keys = kA8Keys, kT8Threads = 512; // rows of a tile, keys of a tile
+constexpr int kT8Extra = kA8Extra, kT8Least = 4;                  // key tiles that an item's beginning and end count for; key tiles of a CTA's share at least
 constexpr int kT8Flush = 16;
 constexpr int kT8Known = 16;                    // key tiles whose scales are kept at hand: more than the producer is ever ahead of the softmax (the rings' stages and two)
 constexpr uint32_t kT8Tmem = 512, kT8S = 0, kT8P = 128, kT8O = 256;           // columns: S0 S1 | P0 P1 | O0 O1
@@ -35,110 +36,11 @@ struct T8Args {
     int sets;                            // head sets of a step: kv_heads * (group / hpc)
     int vec_q;
     const A8Plan* plan;
-    int* counters;
+    struct T8Item* cuts;                 // of every CTA: the item it has the first part of and others the rest (parts 0: none)
     float* parts;
     int32_t* status;
     unsigned polls;
 };
-
-// ---- the plan: which runs of 2 * queries neighbouring queries have listed tiles, and how many key tiles each ----
-// One CTA. Tiles of one query are the other kernel's.
-__global__ void __launch_bounds__(1024) seq_attention8_plan_kernel(Attn8Args p, int width, A8Plan* plan) {
-    after_previous();
-    const sllm_seq_batch& b = p.b;
-    __shared__ int s_base[kA8Segs + 1];
-    __shared__ int s_warp[32];
-    constexpr int kFew = 640;
-    __shared__ uint32_t s_mask[kFew * 8];
-    __shared__ int s_seg[kFew], s_first[kFew];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto scan = [&](int v, int& total) {         // exclusive sum over the CTA
-        int upto = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
-        }
-        __syncthreads();
-        if (lane == 31) s_warp[warp] = upto;
-        __syncthreads();
-        int before = 0;
-        total = 0;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) before += s_warp[w];
-            total += s_warp[w];
-        }
-        return before + upto - v;
-    };
-    int runs = 0;
-    for (int s0 = 0; s0 < b.nseg; s0 += 1024) {
-        const int s = s0 + threadIdx.x, len = s < b.nseg ? b.seg_len[s] : 0;
-        int total;
-        const int at = scan(len > 1 ? (len + width - 1) / width : 0, total);
-        if (s < b.nseg) s_base[s] = runs + at;
-        runs += total;
-    }
-    runs = min(runs, kA8Runs);                   // (the host has made sure)
-    const bool few = runs <= kFew;               // their masks fit shared memory
-    for (int i = threadIdx.x; i < runs * 8; i += 1024) {
-        if (few) s_mask[i] = 0; else plan->mask[i / 8][i % 8] = 0;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < b.nseg; i += 1024) {
-        const int len = b.seg_len[i], n = len > 1 ? (len + width - 1) / width : 0;
-        for (int r = 0; r < n && s_base[i] + r < runs; ++r) {
-            const int at = s_base[i] + r;
-            if (few) { s_seg[at] = i; s_first[at] = r * width; } else { plan->seg[at] = i; plan->first[at] = r * width; }
-        }
-    }
-    for (int i = threadIdx.x; i < b.n_qtiles; i += 1024) {
-        const int seg = b.qt_seg[i], off = b.qt_off[i], n = min(kBQ, b.seg_len[seg] - off);
-        if (n <= 1 || off < 0) continue;
-        for (int q = off; q < off + n;) {        // a word of a run's mask at a time
-            const int run = s_base[seg] + q / width, bit = q % width, count = min(off + n - q, 32 - bit % 32);
-            if (run < runs) atomicOr(few ? &s_mask[run * 8 + bit / 32] : &plan->mask[run][bit / 32], (count == 32 ? 0xffffffffu : (1u << count) - 1) << (bit % 32));
-            q += count;
-        }
-    }
-    __syncthreads();
-    __threadfence_block();
-    int all = 0, kept = 0;
-    for (int r0 = 0; r0 < runs; r0 += 1024) {
-        const int r = r0 + threadIdx.x;
-        int units = 0, seg = 0, first = 0;
-        uint32_t m[8];
-        if (r < runs) {
-            int lo = -1, hi = -1;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                m[w] = few ? s_mask[r * 8 + w] : *reinterpret_cast<volatile uint32_t*>(&plan->mask[r][w]);
-                if (!m[w]) continue;
-                if (lo < 0) lo = 32 * w + __ffs(m[w]) - 1;
-                hi = 32 * w + 31 - __clz(m[w]);
-            }
-            seg = few ? s_seg[r] : plan->seg[r];
-            first = few ? s_first[r] : plan->first[r];
-            const int pos0 = b.seg_pos0[seg] + first;
-            if (lo >= 0 && pos0 >= 0) units = TileList(pos0 + lo, pos0 + hi, seq_row_window(pos0 + lo, p.window, p.chunk), p.keep_first, kT8Keys).n + kT8Extra;
-        }
-        int total, kept_here;
-        const int at = scan(units, total), to = kept + scan(units > 0, kept_here);      // (behind its barriers every run of this round has been read)
-        if (units > 0) {                         // a run without listed tiles is left out
-            plan->before[to] = all + at;
-            plan->seg[to] = seg;
-            plan->first[to] = first;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) plan->mask[to][w] = m[w];
-        }
-        all += total;
-        kept += kept_here;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        plan->before[kept] = all;
-        plan->runs = kept;
-    }
-}
 
 // An item of a CTA's share, as all its roles see it.
 struct T8Item {
@@ -150,6 +52,7 @@ struct T8Item {
     uint32_t m[8];                           // listed queries
     __device__ __forceinline__ bool listed(int q) const { return m[q >> 5] >> (q & 31) & 1; }
 };
+static_assert(sizeof(T8Item) <= kA8Cut, "the workspace's cuts");
 constexpr int kT8Items = 48;                 // of a share, kept in shared memory; the ones behind are worked out where they are needed
 
 // A CTA's share of the row of all key tiles: items first_item, first_item + 1, ... of the step (run by run, head set by head set)
@@ -157,24 +60,25 @@ struct T8Share {
     const T8Args& p;
     long long total, begin, end;
     int ctas, first_item, count;
+    const int* before;                   // of the plan, or a copy of it
     __device__ __forceinline__ long long share(int c) const { return (long long)c * total / ctas; }
     __device__ __forceinline__ int owner(long long v) const { return (int)(((v + 1) * ctas - 1) / total); }
-    __device__ __forceinline__ T8Share(const T8Args& args, int n_ctas, long long all) : p(args), total(all), ctas(n_ctas) {
+    __device__ __forceinline__ T8Share(const T8Args& args, int n_ctas, long long all, const int* plan_before) : p(args), total(all), ctas(n_ctas), before(plan_before) {
         begin = share(blockIdx.x);
         end = share(blockIdx.x + 1);
     }
-    __device__ __forceinline__ int item_of(long long u) const {          // the item that unit u (beginnings counted) belongs to
-        int lo = 0, hi = p.plan->runs;
+    __device__ __forceinline__ int item_of(long long u, int runs) const {          // the item that unit u (beginnings counted) belongs to
+        int lo = 0, hi = runs;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if ((long long)p.plan->before[mid] * p.sets <= u) lo = mid; else hi = mid;
+            if ((long long)before[mid] * p.sets <= u) lo = mid; else hi = mid;
         }
-        const int b0 = p.plan->before[lo], each = p.plan->before[lo + 1] - b0;
+        const int b0 = before[lo], each = before[lo + 1] - b0;
         return lo * p.sets + (int)((u - (long long)b0 * p.sets) / each);
     }
     __device__ __noinline__ void work_out(int i, T8Item& it) const {     // k1 <= 0: the share ends before its first tile
         const int x = (first_item + i) / p.sets, y = (first_item + i) % p.sets;
-        const int b0 = p.plan->before[x], each = p.plan->before[x + 1] - b0;
+        const int b0 = before[x], each = before[x + 1] - b0;
         const long long item0 = (long long)b0 * p.sets + (long long)y * each + kT8Extra;
         it.n = each - kT8Extra;
         it.k0 = (int)max(0ll, begin - item0);
@@ -291,8 +195,8 @@ __device__ __forceinline__ void t8_store(const T8Out& to, int c, float4 x, float
     }
     if (to.out16) *reinterpret_cast<uint4*>(to.out16 + c) = make_uint4(tc_pack(x.x, x.y), tc_pack(x.z, x.w), tc_pack(y.x, y.y), tc_pack(y.z, y.w));
 }
-// Rare: a row whose keys' values may hold NaN codes has its result; it becomes NaN in the columns where one of the values that it sees is.
-__device__ __noinline__ void t8_poison(const T8Args& p, const T8Item& it, int j, int row) {
+// Rare: a row whose keys' values may hold NaN codes has its result; it becomes NaN in the columns c0 .. c1 - 1 where one of the values that it sees is.
+__device__ __noinline__ void t8_poison(const T8Args& p, const T8Item& it, int j, int row, int c0, int c1) {
     const Attn8Args& a = p.a;
     const T8Out to = t8_out(p, it, j, row);
     if (!to.listed) return;
@@ -304,7 +208,7 @@ __device__ __noinline__ void t8_poison(const T8Args& p, const T8Item& it, int j,
         for (int e = 0; e < kKv8Block; ++e) {
             if (!seq_sees(pos, key0 + e, wnd, a.keep_first)) continue;
             const uint8_t* v = a.v_pool + (size_t)(r + e) * a.dv;
-            for (int c = 0; c < a.dv; ++c) {
+            for (int c = c0; c < c1; ++c) {
                 if ((v[c] & 0x7f) != 0x7f) continue;
                 if (to.out) to.out[c] = __int_as_float(0x7fffffff);
                 if (to.out16) to.out16[c] = 0x7fff;
@@ -312,48 +216,44 @@ __device__ __noinline__ void t8_poison(const T8Args& p, const T8Item& it, int j,
         }
     }
 }
-// An item whose parts are all there, row `row` of both tiles: its parts brought to one reference and added, in the order of the key tiles.
-__device__ __noinline__ void t8_merge(const T8Args& p, const T8Item& it, int row) {
-    const int parts = it.parts;
-#pragma unroll 1
-    for (int j = 0; j < 2; ++j) {
-        const float* first = p.parts + (size_t)(2 * it.first_cta + it.later) * kT8Part + j * kT8PartTile;
-        const float* rest = p.parts + (size_t)(2 * it.first_cta) * kT8Part + j * kT8PartTile;
-        auto from = [&](int x) { return x == 0 ? first : rest + (size_t)(2 * x) * kT8Part; };
-        float top = -INFINITY, l = 0.0f;
-        bool wild = false;
-#pragma unroll 4
-        for (int x = 0; x < parts; ++x) top = fmaxf(top, __ldcg(from(x) + 128 * kT8Rows + row));
-#pragma unroll 4
-        for (int x = 0; x < parts; ++x) {
-            const float r = __ldcg(from(x) + 128 * kT8Rows + row), s = __ldcg(from(x) + 129 * kT8Rows + row);
-            wild |= __float_as_uint(s) >> 31;
-            l += fabsf(s) * (r == top ? 1.0f : tc_exp2(r - top));
-        }
-        const T8Out to = t8_out(p, it, j, row);
-        if (!to.listed) continue;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll 1
-        for (int c = 0; c < p.a.dv; c += 16) {
-            float4 y[4] = {};
+// The parts of the items that were cut, brought to one reference and added, in the order of the key tiles. CTA (x, y): the item that CTA x of the kernel in front had the first part of,
+// if there is one; tile y / 4, a thread per row, 32 columns.
+constexpr int kT8JoinCols = 32, kT8JoinCtas = 2 * 128 / kT8JoinCols;
+__global__ void __launch_bounds__(kT8Rows) seq_attention8_join_kernel(const __grid_constant__ T8Args p) {
+    after_previous();
+    const int row = threadIdx.x, j = blockIdx.y / (kT8JoinCtas / 2), c0 = blockIdx.y % (kT8JoinCtas / 2) * kT8JoinCols;
+    const T8Item& it = p.cuts[blockIdx.x];
+    if (it.parts < 2 || c0 >= p.a.dv) return;
+    const T8Out to = t8_out(p, it, j, row);
+    if (!to.listed) return;
+    const float* first = p.parts + (size_t)(2 * it.first_cta + it.later) * kT8Part + j * kT8PartTile;
+    const float* rest = p.parts + (size_t)(2 * it.first_cta) * kT8Part + j * kT8PartTile;
+    auto from = [&](int x) { return x == 0 ? first : rest + (size_t)(2 * x) * kT8Part; };
+    float top = -INFINITY, l = 0.0f;
+#pragma unroll 8
+    for (int x = 0; x < it.parts; ++x) top = fmaxf(top, from(x)[128 * kT8Rows + row]);
+    bool wild = false;
+    float4 y[kT8JoinCols / 4] = {};
 #pragma unroll 2
-            for (int x = 0; x < parts; ++x) {
-                const float r = __ldcg(from(x) + 128 * kT8Rows + row);
-                if (r == -INFINITY && __ldcg(from(x) + 129 * kT8Rows + row) == 0.0f) continue;       // none of this part's keys is visible: its O may never have been written
-                const float f = r == top ? 1.0f : tc_exp2(r - top);
+    for (int x = 0; x < it.parts; ++x) {
+        const float *part = from(x), r = part[128 * kT8Rows + row], sum = part[129 * kT8Rows + row], f = r == top ? 1.0f : tc_exp2(r - top);
+        wild |= __float_as_uint(sum) >> 31;
+        l += fabsf(sum) * f;
+        if (r == -INFINITY && sum == 0.0f) continue;       // none of this part's keys is visible: its O may never have been written
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(from(x)) + (c / 4 + i) * kT8Rows + row);
-                    y[i].x = fmaf(v.x, f, y[i].x); y[i].y = fmaf(v.y, f, y[i].y); y[i].z = fmaf(v.z, f, y[i].z); y[i].w = fmaf(v.w, f, y[i].w);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = make_float4(y[i].x * inv, y[i].y * inv, y[i].z * inv, y[i].w * inv);
-            t8_store(to, c, y[0], y[1]);
-            t8_store(to, c + 8, y[2], y[3]);
+        for (int i = 0; i < kT8JoinCols / 4; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(part)[(c0 / 4 + i) * kT8Rows + row];
+            y[i].x = fmaf(v.x, f, y[i].x); y[i].y = fmaf(v.y, f, y[i].y); y[i].z = fmaf(v.z, f, y[i].z); y[i].w = fmaf(v.w, f, y[i].w);
         }
-        if (wild) t8_poison(p, it, j, row);
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < kT8JoinCols / 4; i += 2) {
+        if (c0 + 4 * i >= p.a.dv) break;
+        const float4 u = y[i], v = y[i + 1];
+        t8_store(to, c0 + 4 * i, make_float4(u.x * inv, u.y * inv, u.z * inv, u.w * inv), make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    }
+    if (wild) t8_poison(p, it, j, row, c0, min(p.a.dv, c0 + kT8JoinCols));
 }
 
 template <int HD, int kTerms, bool kOpts>
@@ -367,8 +267,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
     uint64_t *rfull = bars, *rempty = rfull + RS, *kfull = rempty + RS, *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV;
     // per tile: queries written / scores written / scores read / factors for O written / weights written and O rescaled / product with the values done / sums written, and read
     uint64_t *qready = vempty + SV, *sfull = qready + 2, *sread = sfull + 2, *factors = sread + 2, *pready = factors + 2, *odone = pready + 2, *lready = odone + 2, *lread = lready + 2;
-    uint64_t* meet = lread + 2;              // of warps 12-15
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(lread + 2);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* s_start = reinterpret_cast<int*>(tmem_slot + 2);                        // the first item and how many
     int* s_last = reinterpret_cast<int*>(tmem_slot + 4);
@@ -389,28 +288,42 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
         }
         *gave_up = 0;
         for (int i = 0; i < 8; ++i) s_nan[i] = 0;
-        mb_init(meet, 128);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tc_alloc(tmem_slot, kT8Tmem);
     after_previous();
     // this CTA's share of the row of all key tiles, and its items
-    const long long total = (long long)p.plan->before[p.plan->runs] * p.sets;
+    const int runs = p.plan->runs;
+    int* s_before = reinterpret_cast<int*>(smem);                              // where operands come later
+    static_assert((kA8Runs + 1) * 4 <= (SK + SV) * Sh::kTile + 2 * RS * Sh::kCodes, "room for the plan");
+    for (int i = threadIdx.x; i <= runs; i += kT8Threads) s_before[i] = p.plan->before[i];
+    __syncthreads();
+    const long long total = (long long)s_before[runs] * p.sets;
     const int ctas = (int)min((long long)gridDim.x, (total + kT8Least - 1) / kT8Least);
     const bool work = (int)blockIdx.x < ctas;
-    T8Share w(p, ctas, total);
+    T8Share w(p, ctas, total, s_before);
     if (work && warp >= 2 && warp < 4) {
-        w.first_item = w.item_of(w.begin);
-        const int n = w.item_of(w.end - 1) - w.first_item + 1, i = threadIdx.x - 64;
+        w.first_item = w.item_of(w.begin, runs);
+        const int n = w.item_of(w.end - 1, runs) - w.first_item + 1, i = threadIdx.x - 64;
         if (i < min(n, kT8Items)) w.work_out(i, s_items[i]);
         if (i == 0) { s_start[0] = w.first_item; s_start[1] = n; }
+        if (i == 63) {                           // the last one may go on in the next CTA
+            T8Item last;
+            w.work_out(n - 1, last);
+            if (last.first_cta != (int)blockIdx.x || last.parts == 1) last.parts = 0;
+            p.cuts[blockIdx.x] = last;
+        }
+    } else if (!work && threadIdx.x == 127) {
+        p.cuts[blockIdx.x].parts = 0;
     }
+    fence_async_smem();                                                        // (s_before has been read before the first copy writes there)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     w.first_item = s_start[0];
     w.count = s_start[1];
+    w.before = p.plan->before;
     // the i-th item, or false behind the last one (whose first tile the share may end before)
     auto item_at = [&](int i, T8Item& more) -> const T8Item* {
         if (i >= w.count) return nullptr;
@@ -596,7 +509,6 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
         const int quad = warp & 3, row = quad * 32 + lane;
         T8Item more;
         uint32_t done0 = 0, done1 = 0, items0 = 0, items1 = 0;
-        uint32_t met = 0;
         bool ok = true;
         for (int n_item = 0; ok; ++n_item) {
             const T8Item* at = item_at(n_item, more);
@@ -711,7 +623,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     }
                     __syncwarp();
                 }
-                if (whole && nan_here) t8_poison(p, it, j, row);
+                if (whole && nan_here) t8_poison(p, it, j, row, 0, a.dv);
                 if (!whole) {
                     part[j * kT8PartTile + 128 * kT8Rows + row] = ref;
                     part[j * kT8PartTile + 129 * kT8Rows + row] = nan_here ? -l : l;      // (sums are not negative: the sign says that there was NaN)
@@ -719,27 +631,6 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             }
             if (!ok) break;
             tc_fence_before();
-            if (!whole) {
-                const int c_first = it.first_cta, parts = it.parts;
-                auto together = [&]() {              // these four warps; a wait like the others, which ends
-                    mb_arrive(meet);
-                    ok = t8_wait_warp(meet, met++ & 1, gave_up, p.polls);
-                    return ok;
-                };
-                if (!together()) break;
-                if (threadIdx.x == 12 * 32) {        // what these warps have stored before the barrier comes before this, and what others have stored before theirs, before what follows
-                    int before_me;
-                    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before_me) : "l"(p.counters + c_first) : "memory");
-                    *s_last = before_me == parts - 1;
-                    if (before_me == parts - 1) p.counters[c_first] = 0;
-                }
-                if (!together()) break;
-                if (*s_last) {
-                    __threadfence();
-                    t8_merge(p, it, row);
-                }
-                if (!together()) break;              // s_last has been read
-            }
         }
     } else {   // ===== softmax: TMEM lane quadrant = warp % 4 =====
         const int j = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
@@ -868,19 +759,27 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                             }
                             most[x] = fmaxf(t0, t1);
                         }
-                        // scores within a quarter of the cap, as nearly all are: the series that tc_tanh takes for them, two at a time
-                        if (__any_sync(0xffffffffu, fmaxf(most[0] * inv[0], most[1] * inv[1]) >= 0.25f)) {
+                        // scores below the cap, as nearly all are: tanh x = x g(x^2), g through Chebyshev's eight points of [0, 1] (9e-9 of its value; with its roundings 1.1e-7), two scores
+                        // at a time: 5 instructions a score, where tc_tanh takes 13 and two of the special function unit
+                        if (__any_sync(0xffffffffu, !(fmaxf(most[0] * inv[0], most[1] * inv[1]) < 1.0f))) {
                             const float back[2] = {a.softcap / f[0], a.softcap / f[1]};
 #pragma unroll
                             for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(back[e / 32] * tc_tanh(__uint_as_float(s[e]) * inv[e / 32]));
                         } else {
                             auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
-                            const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), one = both(1.0f);
+                            const uint64_t c7 = both(-0.00035232809f), c6 = both(0.0022786476f), c5 = both(-0.0079124849f), c4 = both(0.0214614104f), c3 = both(-0.0538697056f),
+                                           c2 = both(0.1333213896f), c1 = both(-0.333332777f), one = both(1.0f);
 #pragma unroll
                             for (int e = 0; e < 64; e += 2) {
-                                const uint64_t v = tc_two(s[e], s[e + 1]), x = tc_mul2(v, both(inv[e / 32])), x2 = tc_mul2(x, x);
+                                const uint64_t v = tc_two(s[e], s[e + 1]), x = tc_mul2(v, both(inv[e / 32])), u = tc_mul2(x, x);
+                                uint64_t t = tc_fma2(u, c7, c6);
+                                t = tc_fma2(u, t, c5);
+                                t = tc_fma2(u, t, c4);
+                                t = tc_fma2(u, t, c3);
+                                t = tc_fma2(u, t, c2);
+                                t = tc_fma2(u, t, c1);
                                 float y, z;
-                                tc_split(tc_mul2(v, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, c4, c3), c2), c1), one)), y, z);
+                                tc_split(tc_mul2(v, tc_fma2(u, t, one)), y, z);
                                 s[e] = __float_as_uint(y);
                                 s[e + 1] = __float_as_uint(z);
                             }
@@ -1017,7 +916,9 @@ static int t8_launch(const T8Args& a, const CUtensorMap& tmK, const CUtensorMap&
     }
     LaunchCfg lc(dim3(std::min(kA8TcWorkers, sm_count())), dim3(kT8Threads), Sh::kSmem, st, true);        // its beginning while the plan is made
     SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(kernel), tmK, tmV, a));
-    ++g_launches;
+    LaunchCfg join(dim3(lc.cfg.gridDim.x, kT8JoinCtas), dim3(kT8Rows), 0, st, true);
+    SLLM_CUDA(cudaLaunchKernelEx(&join.cfg, overlapping(seq_attention8_join_kernel), a));
+    g_launches += 2;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
 }
@@ -1027,8 +928,10 @@ static int t8_hpc(const Attn8Args& p) {
     return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
 }
 
+int attention8_tc_width(const Attn8Args& p) { return 2 * kT8Rows / t8_hpc(p); }
+
 bool attention8_tc_takes(const Attn8Args& p) {
-    const int width = 2 * kT8Rows / t8_hpc(p);
+    const int width = attention8_tc_width(p);
     return p.dk <= 128 && p.dv <= 128 && p.b.nseg <= kA8Segs && p.b.T / width + p.b.nseg <= kA8Runs;
 }
 
@@ -1040,9 +943,8 @@ int launch_attention8_tc(const Attn8Args& p, void* ws, cudaStream_t st) {
     a.queries = kT8Rows / a.hpc;
     a.sets = p.heads / a.hpc;
     a.vec_q = p.ldq % 4 == 0 && ((uintptr_t)p.q % 16) == 0;
-    A8Plan* plan = reinterpret_cast<A8Plan*>((uint8_t*)ws + kA8PlanAt);
-    a.plan = plan;
-    a.counters = (int*)ws + kA8Workers;
+    a.plan = reinterpret_cast<const A8Plan*>((uint8_t*)ws + kA8PlanAt);
+    a.cuts = reinterpret_cast<T8Item*>((uint8_t*)ws + kA8CutsAt);
     a.parts = (float*)((uint8_t*)ws + kA8PartsAt);
     if (int rc = status_word(&a.status)) return rc;
     a.polls = (unsigned)g_tune_tc_polls;
@@ -1051,9 +953,6 @@ int launch_attention8_tc(const Attn8Args& p, void* ws, cudaStream_t st) {
     const uint64_t rows = (uint64_t)p.n_pages * p.kv_heads * p.b.page_len;
     if (int rc = tc_encode_bytes(&tmK, p.k_pool, rows, p.dk, kKv8Block, HD)) return rc;
     if (int rc = tc_encode_bytes(&tmV, p.v_pool, rows, p.dv, kKv8Block, HD)) return rc;
-    overlapping(seq_attention8_plan_kernel)<<<1, 1024, 0, st>>>(p, 2 * a.queries, plan);
-    ++g_launches;
-    SLLM_LAUNCH_CHECK_ONLY();
     const bool opts = p.softcap > 0.0f || p.slopes;
 #define SLLM_T8(HD_)                                                                                                                            \
     (p.out ? (opts ? t8_launch<HD_, 2, true>(a, tmK, tmV, st) : t8_launch<HD_, 2, false>(a, tmK, tmV, st))                                        \
