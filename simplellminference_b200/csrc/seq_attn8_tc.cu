@@ -112,12 +112,13 @@ struct T8Share {
 
 template <int HD, int kTerms>
 struct T8Shape {
-    static constexpr int kBlocks = HD / 64, kK = 2, kV = kTerms == 1 ? 2 : 1, kRaw = kTerms == 1 ? 4 : 2;      // stages of keys, of values, of codes
+    static constexpr int kBlocks = HD / 64, kK = 2, kV = kTerms == 1 ? 2 : 1, kRaw = kTerms == 2 ? 2 : HD == 128 ? 3 : 4;      // stages of keys, of values, of codes
     static constexpr int kBlock = kT8Keys * 128, kTile = kBlocks * kBlock;    // fp16: 64 columns of all keys; all columns
     static constexpr int kCodes = kT8Keys * HD;                              // bytes of a tile of codes
     static constexpr int kQBlock = kT8Rows * 128, kQTerm = kBlocks * kQBlock, kQTile = kTerms * kQTerm;
     static constexpr int kItems = (kT8Items * (int)sizeof(T8Item) + 127) / 128 * 128;
-    static constexpr int kSmem = 1024 + (kK + kV) * kTile + 2 * kRaw * kCodes + 2 * kQTile + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems;
+    static constexpr int kSpare = kTerms == 1 ? 2 * kT8Rows * HD : 0;        // where queries wait to be converted
+    static constexpr int kSmem = 1024 + (kK + kV) * kTile + 2 * kRaw * kCodes + 2 * kQTile + kSpare + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems;
 };
 constexpr int kT8PartTile = kT8Rows * (128 + 2), kT8Part = 2 * kT8PartTile;   // floats of a part: per tile O as [HD / 4][128][4], references, sums
 static_assert(kT8Part == kA8Part, "the workspace's parts");
@@ -217,8 +218,8 @@ __device__ __noinline__ void t8_poison(const T8Args& p, const T8Item& it, int j,
     }
 }
 // The parts of the items that were cut, brought to one reference and added, in the order of the key tiles. CTA (x, y): the item that CTA x of the kernel in front had the first part of,
-// if there is one; tile y / 4, a thread per row, 32 columns.
-constexpr int kT8JoinCols = 32, kT8JoinCtas = 2 * 128 / kT8JoinCols;
+// if there is one; a thread per row of one tile, 16 columns.
+constexpr int kT8JoinCols = 16, kT8JoinCtas = 2 * 128 / kT8JoinCols;
 __global__ void __launch_bounds__(kT8Rows) seq_attention8_join_kernel(const __grid_constant__ T8Args p) {
     after_previous();
     const int row = threadIdx.x, j = blockIdx.y / (kT8JoinCtas / 2), c0 = blockIdx.y % (kT8JoinCtas / 2) * kT8JoinCols;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kT8Rows) seq_attention8_join_kernel(const __gr
     for (int x = 0; x < it.parts; ++x) top = fmaxf(top, from(x)[128 * kT8Rows + row]);
     bool wild = false;
     float4 y[kT8JoinCols / 4] = {};
-#pragma unroll 2
+#pragma unroll 4
     for (int x = 0; x < it.parts; ++x) {
         const float *part = from(x), r = part[128 * kT8Rows + row], sum = part[129 * kT8Rows + row], f = r == top ? 1.0f : tc_exp2(r - top);
         wild |= __float_as_uint(sum) >> 31;
@@ -263,7 +264,8 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
     extern __shared__ uint8_t t8_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(t8_smem) + 1023) & ~(uintptr_t)1023);
     uint8_t *sK = smem, *sV = sK + SK * Sh::kTile, *sQ = sV + SV * Sh::kTile, *sRaw = sQ + 2 * Sh::kQTile;      // sRaw: keys, then values, of each stage
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + 2 * RS * Sh::kCodes);
+    uint8_t* sSpare = sRaw + 2 * RS * Sh::kCodes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sSpare + Sh::kSpare);
     uint64_t *rfull = bars, *rempty = rfull + RS, *kfull = rempty + RS, *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV;
     // per tile: queries written / scores written / scores read / factors for O written / weights written and O rescaled / product with the values done / sums written, and read
     uint64_t *qready = vempty + SV, *sfull = qready + 2, *sread = sfull + 2, *factors = sread + 2, *pready = factors + 2, *odone = pready + 2, *lready = odone + 2, *lread = lready + 2;
@@ -654,60 +656,87 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             // ---- queries: fp16, brought to 1 .. 2 by a power of two of the row's largest; every score of the item before has been made ----
             float up;
             {
-                constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 16;       // lanes of a row, rows of a load, loads on their way
+                // Sixteen rows at a time, by copies to where fp16 rows come to lie: theirs, and those of the second term (with one term, those of the rows behind, then a place of their own). Two
+                // lanes convert a row once all of it is in registers: few instructions (by whole rows, each with a reduction, and in line for all of them it was 20 KB of code run once an item,
+                // and took 5000 to 20000 clocks).
+                constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kLoads = 16 / kPer, kChunks = HD / 8;       // lanes of a row, rows of a load, loads of sixteen rows; a lane's chunks of four columns
                 const int mine = it.tok0 + (live ? q : it.hi), col = (lane % kLanes) * 4, sub = lane / kLanes;      // (a row without a query reads another)
                 const float* src = a.q + (size_t)it.h0 * a.dk + col;
-                // row 8 i + r of a block lies 1024 i + 128 r further, its chunks exchanged by r
-                const uint32_t to = s_addr(sQ) + j * Sh::kQTile + (col / 64) * Sh::kQBlock + quad * 4096 + (col % 8) * 2, chunk = col % 64 / 8;
-                const bool take = col < a.dk;
-                int ex = 0;
+                // row 8 i + r of a block lies 1024 i + 128 r further, its chunks of 16 bytes exchanged by r
+                const uint32_t own = s_addr(sQ) + j * Sh::kQTile + quad * 4096, spare = s_addr(sSpare) + (4 * j + quad) * (16 * 2 * HD);
+                auto piece = [&](int x, int n) {                   // 2 KB, a quarter (HD 64: half) of sixteen rows
+                    const uint32_t at = own + (n >> 1) * Sh::kQBlock;
+                    if (kTerms == 2) return at + x * 2048 + (n & 1) * Sh::kQTerm;
+                    return !(n & 1) ? at + x * 2048 : x == 0 ? at + 2048 : spare + (n >> 1) * 2048;
+                };
+                int ex = 127;
 #pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += kAhead * kPer) {
-                    float4 v[kAhead];
-                    auto address = [&](int i) {
-                        const int r = i * kPer + sub;
-                        return src + (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, r0 + r) * (uint32_t)a.ldq + (uint32_t)((r & (p.hpc - 1)) * a.dk);
-                    };
-                    if (p.vec_q) {
+                for (int x = 0; x < 2; ++x) {
+                    if (kTerms == 1 || x == 0) {
+                        auto address = [&](int i) {
+                            const int r = 16 * x + i * kPer + sub;
+                            return src + (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, r) * (uint32_t)a.ldq + (uint32_t)((r & (p.hpc - 1)) * a.dk);
+                        };
+                        auto place = [&](int i) { return piece(x + i / kLoads, i % kLoads / 4) + (i & 3) * 512 + lane * 16; };
+                        const bool take = col < a.dk;
+                        if (p.vec_q) {                             // (no branch between the copies: they go out one behind the other)
 #pragma unroll
-                        for (int i = 0; i < kAhead; ++i) {
-                            const float* at = address(i);
-                            v[i] = take ? *reinterpret_cast<const float4*>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < kAhead; ++i) {
-                            const float* at = address(i);
-                            v[i] = take ? make_float4(at[0], at[1], at[2], at[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < kAhead; ++i) {
-                        const int r = i * kPer + sub;
-                        uint32_t t = __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
-                        if constexpr (kPer == 1) {
-                            t = __reduce_max_sync(0xffffffffu, t);
+                            for (int i = 0; i < kLoads * kTerms; ++i) {
+                                const float* at = address(i);
+                                asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16;\n}\n" ::"r"(place(i)), "l"(at), "r"((uint32_t)take) : "memory");
+                            }
                         } else {
-#pragma unroll
-                            for (int o = 1; o < kLanes; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+#pragma unroll 1
+                            for (int i = 0; i < kLoads * kTerms; ++i) {
+                                const float* at = address(i);
+                                if (take) t8_sts(place(i), __float_as_uint(at[0]), __float_as_uint(at[1]), __float_as_uint(at[2]), __float_as_uint(at[3]));
+                            }
                         }
-                        int e = max((int)(t >> 23), 27);           // exponent + 127, 27 at least: the reciprocal stays a normal number
-                        if (e == 255) e = 127;                     // an infinity among them
-                        if constexpr (kPer == 1) {
-                            if (lane == r0 + i) ex = e;
-                        } else {
-                            const int e0 = __shfl_sync(0xffffffffu, e, 0), e1 = __shfl_sync(0xffffffffu, e, 16);
-                            if (lane == r0 + 2 * i) ex = e0;
-                            if (lane == r0 + 2 * i + 1) ex = e1;
+                        if (!take) {
+#pragma unroll 1
+                            for (int i = 0; i < kLoads * kTerms; ++i) t8_sts(place(i), 0u, 0u, 0u, 0u);
                         }
-                        const float down = __uint_as_float((uint32_t)(254 - e) << 23), x0 = v[i].x * down, x1 = v[i].y * down, x2 = v[i].z * down, x3 = v[i].w * down;
-                        const uint32_t h0 = t8_pack(x0, x1), h1 = t8_pack(x2, x3), dst = to + (r0 + r) * 128 + ((chunk ^ (r & 7)) << 4);
-                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(dst), "r"(h0), "r"(h1) : "memory");
-                        if constexpr (kTerms == 2) {
-                            const float2 y0 = t8_unpack(h0), y1 = t8_unpack(h1);
-                            asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(dst + Sh::kQTerm), "r"(t8_pack(x0 - y0.x, x1 - y0.y)), "r"(t8_pack(x2 - y1.x, x3 - y1.y)) : "memory");
-                        }
+                        asm volatile("cp.async.wait_all;" ::: "memory");
+                        __syncwarp();                              // a copy is seen by its own lane after the wait, by the others behind this
                     }
+                    // lane r of either half takes its chunks of four columns in the order 0 ^ r, 1 ^ r, ...: no two meet in a bank
+                    constexpr int kRow = HD * 4, kOf = 2048 / kRow;                            // bytes of a row, rows of a piece
+                    const int n = lane & 15, r = 16 * x + n, turn = n & (kChunks - 1);
+                    const uint32_t from = piece(x, n / kOf) + n % kOf * kRow + (lane >> 4) * (kRow / 2);
+                    uint32_t v[kChunks][4];
+                    float most = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) {
+                        const uint4 w = t8_lds(from + ((c ^ turn) << 4));
+                        v[c][0] = w.x; v[c][1] = w.y; v[c][2] = w.z; v[c][3] = w.w;
+                        auto of = [](uint32_t y) { return fabsf(__uint_as_float(y)); };
+                        most = tc_max3(tc_max3(most, of(w.x), of(w.y)), of(w.z), of(w.w));
+                    }
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                    int e = max((int)(__float_as_uint(most) >> 23), 27);       // exponent + 127, 27 at least: the reciprocal stays a normal number
+                    if (e == 255) e = 127;                         // an infinity among them
+                    if (lane >> 4 == x) ex = e;
+                    const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                    __syncwarp();                                  // all have read
+#pragma unroll
+                    for (int d = 0; d < kChunks / 2; ++d) {        // eight columns; in an odd lane the second four come first
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float y = __uint_as_float(v[2 * d + k / 2][2 * k & 3]) * down, z = __uint_as_float(v[2 * d + k / 2][(2 * k & 3) + 1]) * down;
+                            hi[k] = t8_pack(y, z);
+                            if constexpr (kTerms == 2) {
+                                const float2 w = t8_unpack(hi[k]);
+                                lo[k] = t8_pack(y - w.x, z - w.y);
+                            }
+                        }
+                        const bool odd = turn & 1;
+                        const int chunk = (lane >> 4) * (kChunks / 2) + (d ^ (turn >> 1));
+                        const uint32_t to = own + (chunk >> 3) * Sh::kQBlock + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+                        t8_sts(to, odd ? hi[2] : hi[0], odd ? hi[3] : hi[1], odd ? hi[0] : hi[2], odd ? hi[1] : hi[3]);
+                        if constexpr (kTerms == 2) t8_sts(to + Sh::kQTerm, odd ? lo[2] : lo[0], odd ? lo[3] : lo[1], odd ? lo[0] : lo[2], odd ? lo[1] : lo[3]);
+                    }
+                    __syncwarp();
                 }
                 up = __uint_as_float((uint32_t)ex << 23);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
