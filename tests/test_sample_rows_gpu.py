@@ -155,3 +155,24 @@ def test_same_every_time_and_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert (idx.tolist(), prob.tolist()) == first
+
+
+@pytest.mark.parametrize("n", [900, 60000])
+def test_temperatures_of_any_size(n):
+    """Up to where a distance over the temperature, or the distance itself, leaves fp32's range; logits of -inf weigh nothing at any."""
+    x = torch.randn(6, n, generator=torch.Generator().manual_seed(n))
+    x[:, ::5] = -math.inf
+    x[3], x[4] = x[3] * 1e37, torch.where(torch.arange(n) % 2 == 0, 3e38, -3e38)
+    for t in (1e-38, 1e-30, 1e30, 1e37, 3e38):
+        for p, m, k in ((1.0, 0.0, 0), (0.7, 0.0, 0), (0.9, 0.01, n // 3)):
+            rows = [0, 1, 3] if t < 1e37 else [0, 1]
+            _check(x[rows], [t] * len(rows), [k] * len(rows), [p] * len(rows), [m] * len(rows), [0.1, 0.6, 0.9][:len(rows)])
+
+
+@pytest.mark.parametrize("n,grain", [(50257, 0.25), (128256, 2.0 ** -9), (20000, 1.0)])
+def test_borders_in_crowded_places(n, grain):
+    """Logits on a grid: hundreds and thousands of equal ones where top_k's and top_p's borders lie, together and with a min_p."""
+    x = (2.5 * torch.randn(12, n, generator=torch.Generator().manual_seed(n)) / grain).round() * grain
+    k = [0, 0, n // 2, n // 2, n // 7, 700, 0, 3000, n // 2, 0, n - 1, 129]
+    p = [0.5, 0.99, 1.0, 0.9, 0.999, 0.8, 0.999999, 1.0, 0.3, 0.01, 0.95, 0.6]
+    _check(x, [0.6 + 0.1 * i for i in range(12)], k, p, [0.0, 0.001, 0.0] * 4, [i / 12 for i in range(12)])
