@@ -545,7 +545,7 @@ int sllm_seq_attention_finish(const sllm_seq_batch* b, const float* ws, int32_t 
 int sllm_seq_rotary_kv8(const sllm_seq_batch* b, const float* q, int32_t ldq, int32_t heads, int32_t dk, const float* k, int32_t ldk, int32_t kv_heads, const float* v,
                         int32_t ldv, int32_t dv, const float* angles, int32_t n_freq, int32_t layout, float* q_out, int32_t ldqo, void* k_pool, float* k_scale,
                         void* v_pool, float* v_scale, int32_t n_pages, sllm_stream_t stream);
-/* Causal softmax attention of the listed tiles' tokens over the 8-bit cache: score = (q . k) * scale, query head h reads key/value head h / (heads / kv_heads). Options: window,
+/* Causal softmax attention of the listed tiles' tokens over the 8-bit cache: score = (q . k) * scale (positive), query head h reads key/value head h / (heads / kv_heads). Options: window,
  * keep_first, softcap, slopes, chunk; the others are SLLM_ENOTSUP. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16); rows of tokens in no tile stay as
  * they are. Keys whose page the table does not have are hidden; a token that sees none gives zeros. ws: at least sllm_seq_attention8_ws_bytes bytes, 16-byte aligned, zeros
  * before its first use and after an SLLM_ETIMEOUT; every call leaves its counters zero, so calls one behind the other may share it, calls that run side by side may not. A step

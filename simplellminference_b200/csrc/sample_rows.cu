@@ -6,11 +6,14 @@
 // thousands over a large vocabulary. Weights are computed in double and held as multiples of 2^-44: sums of these integers are exact, so nothing depends on the order of threads, and
 // what is left is the rounding of a weight, 2^-45 of the largest.
 // A cluster of CTAs shares a row and keeps it in shared memory: the logits are read once, whatever the settings ask for.
-// The last value that stays (top_k, top_p) is found without sorting: a histogram of the distance to the largest logit, 1024 bins of 1/22 of a bit of weight (integers: sums of counts, or of weights in three
-// parts of 16 bits, so that shared memory's 32-bit additions do), added over the cluster; if the bin that holds the border is full, once more over its 1024 parts. What is left goes to one
-// CTA, which compares it pair by pair. Where a top_k leaves no more than kSrFew candidates all of them go there, and the draw ends there. Only parts too full for that (hundreds of logits
-// within 2^-14 of a bit that are not all equal, or beyond the last bin) are halved bit by bit.
-// Bound: barriers of the cluster and what lies between them; bytes (4 a logit) and double arithmetic (some 20 instructions a weight) come to about a quarter of it over large batches.
+// The last value that stays (top_k, top_p) is found without sorting. The logits are counted in 1024 bins by their distance to the largest, 1/22 of a bit of weight each, over the cluster. By count
+// that names the border's bin. By weight it bounds it: the logits of a bin weigh what its two ends do, 3 % apart, so that the borders of one to a few bins are possible; only then are the weights
+// outside them added up, in registers. (Bins of exact weights took four additions in shared memory a logit.) Where more than kSrPairs logits are left, the few bins are counted once more in
+// 1024 parts. The rest goes to one CTA, which compares it pair by pair; parts too full for that (hundreds of logits within 2^-14 of a bit, or beyond the last bin) are halved bit by bit.
+// A top_k below 7/8 of the cluster's warps needs no bins: the top_k-th largest of the warps' largest logits bounds it from below, the candidates from there on are the first CTA's, and the draw ends there.
+// Bound: chains. A row passes 4 to 10 barriers of its cluster (some 1000 clocks each), a weight is a chain of 13 double operations, and 64 rows of 128256 logits fill the shared memory of the
+// machine twice, so that half of them wait for the other half. Floors and times, us (fp32 logits in a captured graph): one row of 32000 0.02 (bytes) and 9.3 (one kernel with nothing in it: 2.2);
+// 64 rows of 128256 5.0, and by settings: top_k of 20 to 100 with top_p 28, top_p alone 92, min_p 19, none 41, a fifth each and a fifth at temperature 0 51 to 56.
 #include <cooperative_groups.h>
 
 #include "seq_common.cuh"
@@ -687,6 +690,8 @@ extern "C" int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, i
         SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SrShared) + kSrSlice * 4 + 16));
         ready = true;
     }
+    // CTAs of a row: until one holds no more than 16384 logits, and then as long as the machine has room for twice as many and they have 2048 each. The five kinds of settings in turn over 128256
+    // logits, with 4, 8 and 16 CTAs, us: 64 rows 63, 55 and 67 (of 16 only 14 clusters fit at once, of the others 33), 16 rows 53, 36 and 33.
     int cs = 1;
     while (cs < kSrCluster && ((n + cs - 1) / cs > 16384 || ((long long)rows * cs < 2 * sm_count() && n / cs >= 2048))) cs *= 2;
     SampleRows p{logits, temperature, top_p, min_p, u, top_k, idx_dev, prob_dev, ld, n, ((n + cs - 1) / cs + 3) / 4 * 4};

@@ -3,6 +3,8 @@
 //   s_j = scale * 2^ek * (q . code_j),  p = softmax over the visible j,  o = sum_j p_j 2^ev code'_j
 // A block's scales are one number each for 32 keys, so they multiply scores and weights, never codes: the codes enter the products as they are.
 // Keys whose page the block table does not have are hidden; a query that sees no key gives zeros.
+#include <cfloat>
+
 #include "seq_attn8.cuh"
 
 namespace sllm {
@@ -107,6 +109,7 @@ int sllm_seq_attention8(const sllm_seq_batch* b, const float* q, int32_t ldq, in
     SLLM_REQUIRE(dk > 0 && dv > 0 && dk % 16 == 0 && dv % 16 == 0 && dk <= 256 && dv <= 256, SLLM_ENOTSUP, "seq_attention8: head widths %d and %d are not multiples of 16 up to 256",
                  dk, dv);
     SLLM_REQUIRE(heads <= 65535, SLLM_ENOTSUP, "seq_attention8: %d heads", heads);
+    SLLM_REQUIRE(scale > 0.0f && scale <= FLT_MAX, SLLM_EINVAL, "seq_attention8: scores need a positive finite scale");
     SLLM_REQUIRE(b->page_len > 0 && b->page_len % kKv8Block == 0, SLLM_ENOTSUP, "seq_attention8: pages of a multiple of %d positions", kKv8Block);
     SLLM_REQUIRE(ldq >= heads * dk && (!out || ldo >= heads * dv), SLLM_EINVAL, "seq_attention8: a row is shorter than its heads");
     SLLM_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) % 16) == 0, SLLM_EINVAL, "seq_attention8: pools have to start at a multiple of 16 bytes");

@@ -53,6 +53,7 @@ def _opts(**kw):
     (dict(out=None), _lib.EINVAL), (dict(n_pages=0), _lib.EINVAL), (dict(ws=None), _lib.EINVAL), (dict(ws=AT[15] + 8), _lib.EINVAL), (dict(ws_bytes=100), _lib.EINVAL),
     (dict(heads=7), _lib.EINVAL), (dict(kv_heads=0), _lib.EINVAL), (dict(dk=100), _lib.ENOTSUP), (dict(dv=264), _lib.ENOTSUP), (dict(ldq=1023), _lib.EINVAL), (dict(ldo=1000), _lib.EINVAL),
     (dict(k_pool=AT[11] + 8), _lib.EINVAL), (dict(v_pool=AT[13] + 1), _lib.EINVAL), (dict(opts=_opts(window=-1)), _lib.EINVAL), (dict(opts=_opts(softcap=-1.0)), _lib.EINVAL),
+    (dict(scale=0.0), _lib.EINVAL), (dict(scale=-0.1), _lib.EINVAL), (dict(scale=float("inf")), _lib.EINVAL), (dict(scale=float("nan")), _lib.EINVAL),
     (dict(opts=_opts(window=5, chunk=7)), _lib.EINVAL), (dict(opts=_opts(values_in_keys=True)), _lib.ENOTSUP), (dict(opts=_opts(cross_values=True)), _lib.ENOTSUP),
     (dict(b=_batch(n_qtiles=0)), _lib.EINVAL), (dict(b=_batch(qt_off=None)), _lib.EINVAL), (dict(b=_batch(page_len=40)), _lib.ENOTSUP), (dict(b=_batch(seg_pos0=None)), _lib.EINVAL)], ids=str)
 def test_attention_refuses(change, code):

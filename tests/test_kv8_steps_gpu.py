@@ -140,3 +140,15 @@ def test_layers_captured_one_behind_the_other(overlap):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(out, want))
+
+
+@pytest.mark.parametrize("opts", [{}, dict(window=40, keep_first=3), dict(softcap=20.0), dict(chunk=50)], ids=str)
+@pytest.mark.parametrize("segs", [[(300, 1), (64, 1), (0, 1)], [(300, 70), (64, 1), (0, 33)]], ids=["decode", "portions"])
+def test_queries_and_keys_of_zero(segs, opts):
+    """Both scales are the least there are, and their product is below fp32's range: every score is 0, every visible value counts the same; with a query of ordinary size, too."""
+    step, q, k, v = _case(segs, 8, 2, 128)
+    for pool in ((torch.zeros_like(k[0].view(torch.uint8)).view(k[0].dtype), torch.full_like(k[1], 2.0 ** -100)), k):
+        for x in (torch.zeros_like(q), q * 2.0 ** -120, q):
+            want = _want(step, x, pool, v, 8, **opts)
+            for bf16, bound in ((False, F32_BOUND), (True, BF16_BOUND)):
+                assert off(_run(step, x, pool, v, 8, bf16=bf16, **opts), want) < bound
