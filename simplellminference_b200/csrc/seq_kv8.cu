@@ -5,7 +5,7 @@
 // No other CTA touches the block, so nothing is atomic and the result does not depend on the order of CTAs. The others turn a token's queries.
 // Angles come as a table (sllm_seq_angles): made once a step for all layers, they cost a layer 8 bytes a pair and token here instead of a sine and a cosine in double per head.
 // Bound: bytes; queries in and out are most of them (32 heads over 8: 32 of 43 KB a token). Prompts of 3896 tokens, 32 heads over 8 of 128: 39.5 us, 26 at the rate of a copy (4.3 TB/s; loads wait
-// for memory); 64 requests of one token 4.0 us, one 2.8 (an empty kernel takes 2.2).
+// for memory); 64 requests of one token 3.9 us, one 2.8 (a kernel that adds to one number takes 1.1).
 #include <climits>
 
 #include "kv8.cuh"
@@ -248,8 +248,9 @@ extern "C" int sllm_seq_rotary_kv8(const sllm_seq_batch* b, const float* q, int3
     if (int rc = status_check()) return rc;
     if (int rc = status_word(&p.status)) return rc;
     const int jobs = heads * (dk / 8);
-    // a token's queries are divided where the tokens alone do not fill the machine: one token of 32 heads of 128 2.8 us with four CTAs, 3.4 with one; 3896 tokens 39.5 with one, 43 with four
-    p.q_split = b->T >= 2 * sm_count() ? 1 : std::max(1, std::min(kMostSplit, (jobs + kKv8Threads - 1) / kKv8Threads));
+    // A token's queries are divided where the tokens alone do not fill the machine, us with 1, 2, 4 and 8 CTAs a token: one token of 32 heads of 128 3.04, 2.97, 2.97, 3.02; 64 of them 4.28, 3.97, 4.06, 4.58;
+    // 664 tokens of 32 heads of 64 5.52, 4.85, 5.05, 5.99; 3896 of 128 39.7, 41.3, 45.7, 50.3
+    p.q_split = b->T >= 8 * sm_count() ? 1 : std::max(1, std::min(b->T >= 2 * sm_count() ? 2 : kMostSplit, (jobs + kKv8Threads - 1) / kKv8Threads));
     const unsigned grid = (unsigned)(p.units * 2 * kv_heads + b->T * p.q_split);
     const bool vec = ((ldq | ldqo | ldk | ldv | n_freq) % 4) == 0 && (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)angles) % 16) == 0;
     cudaStream_t st = as_stream(stream);
