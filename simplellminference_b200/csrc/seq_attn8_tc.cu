@@ -17,9 +17,9 @@
 // Shares. A CTA per item would leave most SMs idle where few queries follow a long context. The key tiles of all items lie in one row, made by a CTA of the kernel in front from what the
 // device knows (contexts, listed tiles); every CTA takes an equal run of it. Items that a cut goes through leave O, reference and sum as parts, which a kernel behind puts together (done by
 // the last of an item's CTAs, one SM reading what up to ten had left, that took as long as all the rest).
-// Bound: the chain of a step (64 keys for 256 rows): 2400 to 3300 clocks, of which the tensor pipe needs 1024 (2048 with two terms) and the exponentials 1024; in front of it some 16000 clocks for
-// launch, plan and the first queries, and 10000 to 20000 for every further item. Prompts of 2048, 1300 behind 700, 311 and 37 behind 4000 tokens, 32 heads over 8 of 128, bf16 results: 185 us, 41 at
-// the rate of a large product. A portion of 256 behind 6000 and 12 decoding requests, capped, fp32: 144 us, 32 with two terms.
+// Bound: the chain of a step (64 keys for 256 rows): 2400 to 3600 clocks, of which the tensor pipe needs 1024 (2048 with two terms) and the exponentials 1024; in front of it some 16000 clocks for
+// launch, plan and the first queries, and 10000 to 20000 for every further item. Prompts of 2048, 1300 behind 700, 311 and 37 behind 4000 tokens, 32 heads over 8 of 128, bf16 results: 168 us, 41 at
+// the rate of a large product. A portion of 256 behind 6000 and 12 decoding requests, capped, fp32: 151 us, 32 with two terms.
 #include <type_traits>
 
 #include "seq_attn8.cuh"
@@ -28,9 +28,10 @@
 namespace sllm {
 
 constexpr int kT8Rows = 128, kT8Keys = kA8Keys, kT8Threads = 512; // rows of a tile, keys of a tile
-// Key tiles that an item's beginning and end count for (4, 6 and 8: 184, 186 and 186 us for the prompts above, 144, 144 and 145 for the portion); key tiles of a CTA's share at least; key tiles
-// after which fp32 results leave tensor memory: it truncates as it adds, by 2^-24 or so a step, all one way.
-constexpr int kT8Extra = kA8Extra, kT8Least = 4, kT8Flush = 16;
+// Key tiles that an item's beginning and end count for (4, 6 and 8: 184, 186 and 186 us for prompts, 144, 144 and 145 for a portion); key tiles of a CTA's share at least; key tiles after which fp32
+// results leave tensor memory, which truncates as it adds, all one way. The portion below, 16, 8, 4 and 2 tiles: 147, 147, 151 and 153 us, off by 2.2e-6, 1.7e-6, 0.8e-6 and 0.7e-6 of the norm (the latter two
+// with the second terms of scores first, which costs nothing); fp32 arithmetic throughout is off by 1.3e-6.
+constexpr int kT8Extra = kA8Extra, kT8Least = 4, kT8Flush = 4;
 constexpr int kT8Known = 16;                    // key tiles whose scales are kept at hand: more than the producer is ever ahead of the softmax (the rings' stages and two)
 constexpr uint32_t kT8Tmem = 512, kT8S = 0, kT8P = 128, kT8O = 256;           // columns: S0 S1 | P0 P1 | O0 O1
 
@@ -394,12 +395,12 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 tc_fence_after();
                 const uint64_t k = k_desc + (uint32_t)(g % SK) * (Sh::kTile / 16);
 #pragma unroll
-                for (int term = 0; term < kTerms; ++term) {
+                for (int term = kTerms - 1; term >= 0; --term) {         // the small products first: the tensor core truncates by the size of what it adds to
                     const uint64_t q = q_desc + (uint32_t)j * (Sh::kQTile / 16) + (uint32_t)term * (Sh::kQTerm / 16);
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks)
                         tc_mma_bf16(tmem + kT8S + 64 * j, q + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kBlock / 16) + 2 * (ks % 4)), idesc_s,
-                                    term != 0 || ks != 0);
+                                    term != kTerms - 1 || ks != 0);
                 }
                 tc_commit(sfull + j);
                 return true;
@@ -457,10 +458,18 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             constexpr bool values = decltype(values_)::value, wild = decltype(wild_)::value;
             const uint32_t from = s_addr(raw), to = s_addr(tile);
             uint32_t any = 0;
-#pragma unroll 4
-            for (int r0 = 0; r0 < kT8Keys; r0 += 8 * kPer) {
-                const int row = r0 + r8 + 8 * (c0 / kChunks), chunk = c0 % kChunks;
-                uint4 v = t8_lds(from + row * HD + ((HD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
+            // all reads in front of all writes: a round's own chain, eight times over, took 1080 clocks a tile of keys and 1380 of values, and the product with the values waited for it
+            constexpr int kRounds = kT8Keys / (8 * kPer);
+            uint4 codes[kRounds];
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+                const int row = i * 8 * kPer + r8 + 8 * (c0 / kChunks), chunk = c0 % kChunks;
+                codes[i] = t8_lds(from + row * HD + ((HD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+                const int row = i * 8 * kPer + r8 + 8 * (c0 / kChunks), chunk = c0 % kChunks;
+                uint4 v = codes[i];
                 if (values) {
                     const bool take = !wild || (key0 + row <= last_pos && s_tile[x % kT8Known].row[row >= kKv8Block] >= 0);
                     auto look = [&](uint32_t y) {
