@@ -18,8 +18,8 @@
 // device knows (contexts, listed tiles); every CTA takes an equal run of it. Items that a cut goes through leave O, reference and sum as parts, which a kernel behind puts together (done by
 // the last of an item's CTAs, one SM reading what up to ten had left, that took as long as all the rest).
 // Bound: the chain of a step (64 keys for 256 rows): 2400 to 3600 clocks, of which the tensor pipe needs 1024 (2048 with two terms) and the exponentials 1024; in front of it some 16000 clocks for
-// launch, plan and the first queries, and 10000 to 20000 for every further item. Prompts of 2048, 1300 behind 700, 311 and 37 behind 4000 tokens, 32 heads over 8 of 128, bf16 results: 168 us, 41 at
-// the rate of a large product. A portion of 256 behind 6000 and 12 decoding requests, capped, fp32: 151 us, 32 with two terms.
+// launch, plan and the first queries, and 10000 to 20000 for every further item. Prompts of 2048, 1300 behind 700, 311 and 37 behind 4000 tokens, 32 heads over 8 of 128, bf16 results: 162 us, 41 at
+// the rate of a large product. A portion of 256 behind 6000 and 12 decoding requests, capped, fp32: 146 us, 32 with two terms.
 #include <type_traits>
 
 #include "seq_attn8.cuh"
@@ -29,7 +29,7 @@ namespace sllm {
 
 constexpr int kT8Rows = 128, kT8Keys = kA8Keys, kT8Threads = 512; // rows of a tile, keys of a tile
 // Key tiles that an item's beginning and end count for (4, 6 and 8: 184, 186 and 186 us for prompts, 144, 144 and 145 for a portion); key tiles of a CTA's share at least; key tiles after which fp32
-// results leave tensor memory, which truncates as it adds, all one way. The portion below, 16, 8, 4 and 2 tiles: 147, 147, 151 and 153 us, off by 2.2e-6, 1.7e-6, 0.8e-6 and 0.7e-6 of the norm (the latter two
+// results leave tensor memory, which truncates as it adds, all one way. The portion below, 16, 8, 4 and 2 tiles: 147, 147, 151 and 153 us (now 146), off by 2.2e-6, 1.7e-6, 0.8e-6 and 0.7e-6 of the norm (the latter two
 // with the second terms of scores first, which costs nothing); fp32 arithmetic throughout is off by 1.3e-6.
 constexpr int kT8Extra = kA8Extra, kT8Least = 4, kT8Flush = 4;
 constexpr int kT8Known = 16;                    // key tiles whose scales are kept at hand: more than the producer is ever ahead of the softmax (the rings' stages and two)
@@ -229,7 +229,8 @@ __global__ void __launch_bounds__(kT8Rows) seq_attention8_join_kernel(const __gr
     after_previous();
     const int row = threadIdx.x, j = blockIdx.y / (kT8JoinCtas / 2), c0 = blockIdx.y % (kT8JoinCtas / 2) * kT8JoinCols;
     const T8Item& it = p.cuts[blockIdx.x];
-    if (it.parts < 2 || c0 >= p.a.dv) return;
+    const int parts = it.parts;
+    if (parts < 2 || c0 >= p.a.dv) return;
     const T8Out to = t8_out(p, it, j, row);
     if (!to.listed) return;
     const float* first = p.parts + (size_t)(2 * it.first_cta + it.later) * kT8Part + j * kT8PartTile;
@@ -237,19 +238,33 @@ __global__ void __launch_bounds__(kT8Rows) seq_attention8_join_kernel(const __gr
     auto from = [&](int x) { return x == 0 ? first : rest + (size_t)(2 * x) * kT8Part; };
     float top = -INFINITY, l = 0.0f;
 #pragma unroll 8
-    for (int x = 0; x < it.parts; ++x) top = fmaxf(top, from(x)[128 * kT8Rows + row]);
+    for (int x = 0; x < parts; ++x) top = fmaxf(top, from(x)[128 * kT8Rows + row]);
     bool wild = false;
     float4 y[kT8JoinCols / 4] = {};
-#pragma unroll 4
-    for (int x = 0; x < it.parts; ++x) {
-        const float *part = from(x), r = part[128 * kT8Rows + row], sum = part[129 * kT8Rows + row], f = r == top ? 1.0f : tc_exp2(r - top);
-        wild |= __float_as_uint(sum) >> 31;
-        l += fabsf(sum) * f;
-        if (r == -INFINITY && sum == 0.0f) continue;       // none of this part's keys is visible: its O may never have been written
+    constexpr int kAhead = 4;                              // parts asked for at once, without a branch between them
+    for (int x0 = 0; x0 < parts; x0 += kAhead) {
+        float r[kAhead], sum[kAhead];
+        float4 v[kAhead][kT8JoinCols / 4];
 #pragma unroll
-        for (int i = 0; i < kT8JoinCols / 4; ++i) {
-            const float4 v = reinterpret_cast<const float4*>(part)[(c0 / 4 + i) * kT8Rows + row];
-            y[i].x = fmaf(v.x, f, y[i].x); y[i].y = fmaf(v.y, f, y[i].y); y[i].z = fmaf(v.z, f, y[i].z); y[i].w = fmaf(v.w, f, y[i].w);
+        for (int x = 0; x < kAhead; ++x) {
+            const float* part = from(min(x0 + x, parts - 1));
+            r[x] = part[128 * kT8Rows + row];
+            sum[x] = part[129 * kT8Rows + row];
+#pragma unroll
+            for (int i = 0; i < kT8JoinCols / 4; ++i) v[x][i] = reinterpret_cast<const float4*>(part)[(c0 / 4 + i) * kT8Rows + row];
+        }
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            // where none of a part's keys is visible its O may never have been written
+            if (x0 + x >= parts) continue;
+            wild |= __float_as_uint(sum[x]) >> 31;
+            if (r[x] == -INFINITY && sum[x] == 0.0f) continue;
+            const float f = r[x] == top ? 1.0f : tc_exp2(r[x] - top);
+            l += fabsf(sum[x]) * f;
+#pragma unroll
+            for (int i = 0; i < kT8JoinCols / 4; ++i) {
+                y[i].x = fmaf(v[x][i].x, f, y[i].x); y[i].y = fmaf(v[x][i].y, f, y[i].y); y[i].z = fmaf(v[x][i].z, f, y[i].z); y[i].w = fmaf(v[x][i].w, f, y[i].w);
+            }
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
