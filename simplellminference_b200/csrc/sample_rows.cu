@@ -319,6 +319,7 @@ struct SrWork {
         SrShared* first = cluster.map_shared_rank(&sh, 0);
         auto list = [&](float x, int i) {
             const uint32_t to = atomicAdd(&first->listed, 1u);
+            if (to >= kSrFew) return;                                    // (the counts say that they fit)
             first->x[to] = x;
             first->at[to] = (rank << 20) | i;
         };
@@ -386,7 +387,7 @@ struct SrWork {
             if (by_mass) take_aside(m0, m1, 1);
         }
         if (rank == 0) {                                                 // pair by pair: one stays when what lies above it is not yet enough
-            const int in = (int)(upto - n0), split = sr_share(in), at = threadIdx.x / split, part = threadIdx.x % split;
+            const int in = min((int)(upto - n0), kSrFew), split = sr_share(in), at = threadIdx.x / split, part = threadIdx.x % split;
             const float x = at < in ? sh.x[at] : 0.0f;
             if (at < in && part == 0) sh.w[at] = by_mass ? weight(x) : 1;
             if (threadIdx.x == 0) sh.top_key = 0;
