@@ -127,7 +127,7 @@ __device__ __noinline__ void a8_plan(const Attn8Args& p, int width, A8Plan* plan
             if (lo >= 0 && pos0 >= 0) units = TileList(pos0 + lo, pos0 + hi, seq_row_window(pos0 + lo, p.window, p.chunk), p.keep_first, kA8Keys).n + kA8Extra;
         }
         int total, kept_here;
-        const int at = scan(units, total), to = kept + scan(units > 0, kept_here);      // (behind its barriers every run of this round has been read)
+        const int at = scan(units, total), to = kept + scan(units > 0, kept_here);      // (behind its barriers every run of this turn has been read)
         if (units > 0) {                         // a run without listed tiles is left out
             plan->before[to] = all + at;
             plan->seg[to] = seg;
