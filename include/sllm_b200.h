@@ -546,8 +546,8 @@ int sllm_seq_rotary_kv8(const sllm_seq_batch* b, const float* q, int32_t ldq, in
                         int32_t ldv, int32_t dv, const float* angles, int32_t n_freq, int32_t layout, float* q_out, int32_t ldqo, void* k_pool, float* k_scale,
                         void* v_pool, float* v_scale, int32_t n_pages, sllm_stream_t stream);
 /* Causal softmax attention of the listed tiles' tokens over the 8-bit cache: score = (q . k) * scale (positive), query head h reads key/value head h / (heads / kv_heads). Options: window,
- * keep_first, softcap, slopes, chunk; the others are SLLM_ENOTSUP. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16); rows of tokens in no tile stay as
- * they are. Keys whose page the table does not have are hidden; a token that sees none gives zeros. ws: at least sllm_seq_attention8_ws_bytes bytes, 16-byte aligned, zeros
+ * keep_first, softcap, slopes, chunk; the others are SLLM_ENOTSUP. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16), which is
+ * the fp32 result rounded, whether or not that is asked for; rows of tokens in no tile stay as they are. Keys whose page the table does not have are hidden; a token that sees none gives zeros. ws: at least sllm_seq_attention8_ws_bytes bytes, 16-byte aligned, zeros
  * before its first use and after an SLLM_ETIMEOUT; every call leaves its counters zero, so calls one behind the other may share it, calls that run side by side may not. A step
  * of as many segments as tokens has one token in each (a tile of more is reported as SLLM_EINVAL by the library's next call). */
 int64_t sllm_seq_attention8_ws_bytes(const sllm_seq_batch* b, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv);

@@ -7,9 +7,9 @@
 //   warp 1 (one lane)   MMA issuer: S = Q K^T, O += P V with P read from TMEM; P has columns of its own, so that the next scores are made while the softmax takes its exponentials;
 //   warps 4-7, 8-11     softmax of tile 0 / 1: queries to fp16 once an item; then, a thread per row, maximum, weights and their sum of every key tile;
 //   warps 12-15         O of both tiles: rescaled where a maximum has grown, results or parts of them written.
-// Results in bf16 (kTerms = 1): queries and weights are one fp16 number each (2^-12 of a value on average less than the 2^-9 of the result's own rounding). Results in fp32 (kTerms = 2): both are
-// the sum of two (22 bits), and O is added to an fp32 copy of the CTA's own every kT8Flush tiles, because the tensor core truncates as it
-// accumulates.
+// Queries and weights are the sum of two fp16 numbers each (22 bits), and O is added to an fp32 copy of the CTA's own every kT8Flush tiles, because the tensor core truncates as it accumulates.
+// Results in bf16 are those in fp32, rounded: with one fp16 number for a query and a weight 15 % of them were another bf16 number (now 0.06 %, as far as fp32 sums let them), and they
+// depended on whether fp32 results were asked for as well; prompts below took 170 us then, 268 now.
 // Weights are relative to the largest of score + log2(value scale) so far, rounded up to a whole number: differences of exponents are exact then, and O is rescaled by powers of two, and
 // seldom. The denominator takes the value scale out again, block by block.
 // A value's NaN code must reach exactly the rows that see it, but 0 * NaN is NaN: the converters replace it and say so, and rows of such an item look for NaN among their keys' values
@@ -115,15 +115,15 @@ struct T8Share {
     }
 };
 
-template <int HD, int kTerms>
+constexpr int kT8Terms = 2;                      // fp16 numbers that a query, or a weight, is the sum of
+template <int HD>
 struct T8Shape {
-    static constexpr int kBlocks = HD / 64, kK = 2, kV = kTerms == 1 ? 2 : 1, kRaw = kTerms == 2 ? 2 : HD == 128 ? 3 : 4;      // stages of keys, of values, of codes
+    static constexpr int kBlocks = HD / 64, kK = 2, kV = 1, kRaw = 2;         // stages of keys, of values, of codes
     static constexpr int kBlock = kT8Keys * 128, kTile = kBlocks * kBlock;    // fp16: 64 columns of all keys; all columns
     static constexpr int kCodes = kT8Keys * HD;                              // bytes of a tile of codes
-    static constexpr int kQBlock = kT8Rows * 128, kQTerm = kBlocks * kQBlock, kQTile = kTerms * kQTerm;
+    static constexpr int kQBlock = kT8Rows * 128, kQTerm = kBlocks * kQBlock, kQTile = kT8Terms * kQTerm;
     static constexpr int kItems = (kT8Items * (int)sizeof(T8Item) + 127) / 128 * 128;
-    static constexpr int kSpare = kTerms == 1 ? 2 * kT8Rows * HD : 0;        // where queries wait to be converted
-    static constexpr int kSmem = 1024 + (kK + kV) * kTile + 2 * kRaw * kCodes + 2 * kQTile + kSpare + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems;
+    static constexpr int kSmem = 1024 + (kK + kV) * kTile + 2 * kRaw * kCodes + 2 * kQTile + 512 + 8 * kT8Rows * (int)sizeof(float) + kItems;
 };
 constexpr int kT8PartTile = kT8Rows * (128 + 2), kT8Part = 2 * kT8PartTile;   // floats of a part: per tile O as [HD / 4][128][4], references, sums
 static_assert(kT8Part == kA8Part, "the workspace's parts");
@@ -277,15 +277,14 @@ __global__ void __launch_bounds__(kT8Rows) seq_attention8_join_kernel(const __gr
     if (wild) t8_poison(p, it, j, row, c0, min(p.a.dv, c0 + kT8JoinCols));
 }
 
-template <int HD, int kTerms, bool kOpts>
+template <int HD, bool kOpts>
 __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ T8Args p) {
-    using Sh = T8Shape<HD, kTerms>;
+    using Sh = T8Shape<HD>;
     constexpr int SK = Sh::kK, SV = Sh::kV, RS = Sh::kRaw;
     extern __shared__ uint8_t t8_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(t8_smem) + 1023) & ~(uintptr_t)1023);
     uint8_t *sK = smem, *sV = sK + SK * Sh::kTile, *sQ = sV + SV * Sh::kTile, *sRaw = sQ + 2 * Sh::kQTile;      // sRaw: keys, then values, of each stage
-    uint8_t* sSpare = sRaw + 2 * RS * Sh::kCodes;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sSpare + Sh::kSpare);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + 2 * RS * Sh::kCodes);
     uint64_t *rfull = bars, *rempty = rfull + RS, *kfull = rempty + RS, *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV;
     // per tile: queries written / scores written / scores read / factors for O written / weights written and O rescaled / product with the values done / sums written, and read
     uint64_t *qready = vempty + SV, *sfull = qready + 2, *sread = sfull + 2, *factors = sread + 2, *pready = factors + 2, *odone = pready + 2, *lready = odone + 2, *lread = lready + 2;
@@ -410,12 +409,12 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 tc_fence_after();
                 const uint64_t k = k_desc + (uint32_t)(g % SK) * (Sh::kTile / 16);
 #pragma unroll
-                for (int term = kTerms - 1; term >= 0; --term) {         // the small products first: the tensor core truncates by the size of what it adds to
+                for (int term = kT8Terms - 1; term >= 0; --term) {         // the small products first: the tensor core truncates by the size of what it adds to
                     const uint64_t q = q_desc + (uint32_t)j * (Sh::kQTile / 16) + (uint32_t)term * (Sh::kQTerm / 16);
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks)
                         tc_mma_bf16(tmem + kT8S + 64 * j, q + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kBlock / 16) + 2 * (ks % 4)), idesc_s,
-                                    term != kTerms - 1 || ks != 0);
+                                    term != kT8Terms - 1 || ks != 0);
                 }
                 tc_commit(sfull + j);
                 return true;
@@ -423,7 +422,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             auto values = [&](int j, int g, bool more) {
                 const uint64_t v = v_desc + (uint32_t)(g % SV) * (Sh::kTile / 16);
 #pragma unroll
-                for (int ks = 0; ks < kTerms * kT8Keys / 16; ++ks)       // first terms, then second ones, against the same values
+                for (int ks = 0; ks < kT8Terms * kT8Keys / 16; ++ks)       // first terms, then second ones, against the same values
                     tc_mma_bf16_ts(tmem + kT8O + 128 * j, tmem + kT8P + 64 * j + 8 * ks, v + (uint32_t)((ks % (kT8Keys / 16)) * 128), idesc_o, more || ks != 0);
                 tc_commit(odone + j);
             };
@@ -454,7 +453,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         if (!ok) continue;
                         ++done[j];
                         tc_fence_after();
-                        values(j, g, kTerms == 1 ? kt != 0 : kt % kT8Flush != 0);
+                        values(j, g, kt % kT8Flush != 0);
                     }
                     if (!ok) break;
                     tc_commit(vempty + g % SV);
@@ -561,7 +560,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     tc_fence_after();
                     const float f = factor[j * kT8Rows + row];
                     const uint32_t o_tmem = tmem + ((uint32_t)(quad * 32) << 16) + kT8O + 128 * j;
-                    if (kTerms == 2 && kt > 0 && kt % kT8Flush == 0) {         // O so far, relative to the reference before this tile's
+                    if (kt > 0 && kt % kT8Flush == 0) {         // O so far, relative to the reference before this tile's
                         uint4* acc = reinterpret_cast<uint4*>(part + j * kT8PartTile);
                         const float s = kt > kT8Flush ? since : 0.0f;
 #pragma unroll 1
@@ -620,7 +619,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 const bool nan_here = s_nan[n_item & 7] == n_item + 1;         // (behind the last product: every value has been converted)
                 const uint32_t o_tmem = tmem + ((uint32_t)(quad * 32) << 16) + kT8O + 128 * j;
                 uint4* acc = reinterpret_cast<uint4*>(part + j * kT8PartTile);
-                const bool flushed = kTerms == 2 && mine > kT8Flush;
+                const bool flushed = mine > kT8Flush;
                 const T8Out to = t8_out(p, it, j, row);
                 const float f = whole ? inv : 1.0f;
 #pragma unroll 1
@@ -684,49 +683,44 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
             // ---- queries: fp16, brought to 1 .. 2 by a power of two of the row's largest; every score of the item before has been made ----
             float up;
             {
-                // Sixteen rows at a time, by copies to where fp16 rows come to lie: theirs, and those of the second term (with one term, those of the rows behind, then a place of their own). Two
-                // lanes convert a row once all of it is in registers: few instructions (by whole rows, each with a reduction, and in line for all of them it was 20 KB of code run once an item,
-                // and took 5000 to 20000 clocks).
+                // By copies to where fp16 rows come to lie: theirs, and those of the second term. Two lanes convert a row, sixteen rows at a time, once all of it is in registers: few instructions
+                // (by whole rows, each with a reduction, and in line for all of them it was 20 KB of code run once an item, and took 5000 to 20000 clocks).
                 constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kLoads = 16 / kPer, kChunks = HD / 8;       // lanes of a row, rows of a load, loads of sixteen rows; a lane's chunks of four columns
                 const int mine = it.tok0 + (live ? q : it.hi), col = (lane % kLanes) * 4, sub = lane / kLanes;      // (a row without a query reads another)
                 const float* src = a.q + (size_t)it.h0 * a.dk + col;
                 // row 8 i + r of a block lies 1024 i + 128 r further, its chunks of 16 bytes exchanged by r
-                const uint32_t own = s_addr(sQ) + j * Sh::kQTile + quad * 4096, spare = s_addr(sSpare) + (4 * j + quad) * (16 * 2 * HD);
-                auto piece = [&](int x, int n) {                   // 2 KB, a quarter (HD 64: half) of sixteen rows
-                    const uint32_t at = own + (n >> 1) * Sh::kQBlock;
-                    if (kTerms == 2) return at + x * 2048 + (n & 1) * Sh::kQTerm;
-                    return !(n & 1) ? at + x * 2048 : x == 0 ? at + 2048 : spare + (n >> 1) * 2048;
-                };
+                const uint32_t own = s_addr(sQ) + j * Sh::kQTile + quad * 4096;
+                auto piece = [&](int x, int n) { return own + (n >> 1) * Sh::kQBlock + x * 2048 + (n & 1) * Sh::kQTerm; };      // 2 KB, a quarter (HD 64: half) of sixteen rows
                 int ex = 127;
+                {
+                    auto address = [&](int i) {
+                        const int r = i * kPer + sub;
+                        return src + (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, r) * (uint32_t)a.ldq + (uint32_t)((r & (p.hpc - 1)) * a.dk);
+                    };
+                    auto place = [&](int i) { return piece(i / kLoads, i % kLoads / 4) + (i & 3) * 512 + lane * 16; };
+                    const bool take = col < a.dk;
+                    if (p.vec_q) {                                 // (no branch between the copies: they go out one behind the other)
+#pragma unroll
+                        for (int i = 0; i < kLoads * 2; ++i) {
+                            const float* at = address(i);
+                            asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16;\n}\n" ::"r"(place(i)), "l"(at), "r"((uint32_t)take) : "memory");
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < kLoads * 2; ++i) {
+                            const float* at = address(i);
+                            if (take) t8_sts(place(i), __float_as_uint(at[0]), __float_as_uint(at[1]), __float_as_uint(at[2]), __float_as_uint(at[3]));
+                        }
+                    }
+                    if (!take) {
+#pragma unroll 1
+                        for (int i = 0; i < kLoads * 2; ++i) t8_sts(place(i), 0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    __syncwarp();                                  // a copy is seen by its own lane after the wait, by the others behind this
+                }
 #pragma unroll 1
                 for (int x = 0; x < 2; ++x) {
-                    if (kTerms == 1 || x == 0) {
-                        auto address = [&](int i) {
-                            const int r = 16 * x + i * kPer + sub;
-                            return src + (size_t)(uint32_t)__shfl_sync(0xffffffffu, mine, r) * (uint32_t)a.ldq + (uint32_t)((r & (p.hpc - 1)) * a.dk);
-                        };
-                        auto place = [&](int i) { return piece(x + i / kLoads, i % kLoads / 4) + (i & 3) * 512 + lane * 16; };
-                        const bool take = col < a.dk;
-                        if (p.vec_q) {                             // (no branch between the copies: they go out one behind the other)
-#pragma unroll
-                            for (int i = 0; i < kLoads * kTerms; ++i) {
-                                const float* at = address(i);
-                                asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16;\n}\n" ::"r"(place(i)), "l"(at), "r"((uint32_t)take) : "memory");
-                            }
-                        } else {
-#pragma unroll 1
-                            for (int i = 0; i < kLoads * kTerms; ++i) {
-                                const float* at = address(i);
-                                if (take) t8_sts(place(i), __float_as_uint(at[0]), __float_as_uint(at[1]), __float_as_uint(at[2]), __float_as_uint(at[3]));
-                            }
-                        }
-                        if (!take) {
-#pragma unroll 1
-                            for (int i = 0; i < kLoads * kTerms; ++i) t8_sts(place(i), 0u, 0u, 0u, 0u);
-                        }
-                        asm volatile("cp.async.wait_all;" ::: "memory");
-                        __syncwarp();                              // a copy is seen by its own lane after the wait, by the others behind this
-                    }
                     // lane r of either half takes its chunks of four columns in the order 0 ^ r, 1 ^ r, ...: no two meet in a bank
                     constexpr int kRow = HD * 4, kOf = 2048 / kRow;                            // bytes of a row, rows of a piece
                     const int n = lane & 15, r = 16 * x + n, turn = n & (kChunks - 1);
@@ -753,16 +747,14 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         for (int k = 0; k < 4; ++k) {
                             const float y = __uint_as_float(v[2 * d + k / 2][2 * k & 3]) * down, z = __uint_as_float(v[2 * d + k / 2][(2 * k & 3) + 1]) * down;
                             hi[k] = t8_pack(y, z);
-                            if constexpr (kTerms == 2) {
-                                const float2 w = t8_unpack(hi[k]);
-                                lo[k] = t8_pack(y - w.x, z - w.y);
-                            }
+                            const float2 w = t8_unpack(hi[k]);
+                            lo[k] = t8_pack(y - w.x, z - w.y);
                         }
                         const bool odd = turn & 1;
                         const int chunk = (lane >> 4) * (kChunks / 2) + (d ^ (turn >> 1));
                         const uint32_t to = own + (chunk >> 3) * Sh::kQBlock + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
                         t8_sts(to, odd ? hi[2] : hi[0], odd ? hi[3] : hi[1], odd ? hi[0] : hi[2], odd ? hi[1] : hi[3]);
-                        if constexpr (kTerms == 2) t8_sts(to + Sh::kQTerm, odd ? lo[2] : lo[0], odd ? lo[3] : lo[1], odd ? lo[0] : lo[2], odd ? lo[1] : lo[3]);
+                        t8_sts(to + Sh::kQTerm, odd ? lo[2] : lo[0], odd ? lo[3] : lo[1], odd ? lo[0] : lo[2], odd ? lo[1] : lo[3]);
                     }
                     __syncwarp();
                 }
@@ -922,20 +914,18 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                             z = tc_exp2(z);
                             sum = tc_add2(sum, tc_two(__float_as_uint(y), __float_as_uint(z)));
                             hi[e] = t8_pack(y, z);
-                            if constexpr (kTerms == 2) {
-                                const float2 u = t8_unpack(hi[e]);
-                                lo[e] = t8_pack(y - u.x, z - u.y);
-                            }
+                            const float2 u = t8_unpack(hi[e]);
+                            lo[e] = t8_pack(y - u.x, z - u.y);
                         }
                         if (rare) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 hi[e] = far[x] != 0.0f ? 0u : hi[e];
-                                if constexpr (kTerms == 2) lo[e] = far[x] != 0.0f ? 0u : lo[e];
+                                lo[e] = far[x] != 0.0f ? 0u : lo[e];
                             }
                         }
                         tc_st16(p_tmem + 16 * x, hi);
-                        if constexpr (kTerms == 2) tc_st16(p_tmem + 32 + 16 * x, lo);
+                        tc_st16(p_tmem + 32 + 16 * x, lo);
                         float s0, s1;
                         tc_split(sum, s0, s1);
                         l = fmaf(s0 + s1, tc_exp2(-ev[x] - far[x]), l);         // without the value scale
@@ -963,10 +953,10 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
     }
 }
 
-template <int HD, int kTerms, bool kOpts>
+template <int HD, bool kOpts>
 static int t8_launch(const T8Args& a, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t st) {
-    using Sh = T8Shape<HD, kTerms>;
-    auto* kernel = seq_attention8_tc_kernel<HD, kTerms, kOpts>;
+    using Sh = T8Shape<HD>;
+    auto* kernel = seq_attention8_tc_kernel<HD, kOpts>;
     static bool ready = false;
     if (!ready) {
         SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
@@ -1012,11 +1002,8 @@ int launch_attention8_tc(const Attn8Args& p, void* ws, cudaStream_t st) {
     if (int rc = tc_encode_bytes(&tmK, p.k_pool, rows, p.dk, kKv8Block, HD)) return rc;
     if (int rc = tc_encode_bytes(&tmV, p.v_pool, rows, p.dv, kKv8Block, HD)) return rc;
     const bool opts = p.softcap > 0.0f || p.slopes;
-#define SLLM_T8(HD_)                                                                                                                            \
-    (p.out ? (opts ? t8_launch<HD_, 2, true>(a, tmK, tmV, st) : t8_launch<HD_, 2, false>(a, tmK, tmV, st))                                        \
-           : (opts ? t8_launch<HD_, 1, true>(a, tmK, tmV, st) : t8_launch<HD_, 1, false>(a, tmK, tmV, st)))
-    return HD == 128 ? SLLM_T8(128) : SLLM_T8(64);
-#undef SLLM_T8
+    if (HD == 128) return opts ? t8_launch<128, true>(a, tmK, tmV, st) : t8_launch<128, false>(a, tmK, tmV, st);
+    return opts ? t8_launch<64, true>(a, tmK, tmV, st) : t8_launch<64, false>(a, tmK, tmV, st);
 }
 
 }  // namespace sllm
