@@ -477,11 +477,12 @@ struct SrWork {
 };
 
 __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p) {
+    cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // waited for before anything is sent: every CTA of the cluster runs by then (nothing is handed over)
     after_previous();
     extern __shared__ __align__(16) uint8_t sr_raw[];
     SrShared& sh = *reinterpret_cast<SrShared*>(sr_raw);
     float* s_x = reinterpret_cast<float*>(sr_raw + sizeof(SrShared));
-    cg::cluster_group cluster = cg::this_cluster();
     const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / size, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int first = min(p.n, rank * p.slice), count = min(p.n, first + p.slice) - first;
     const float* x = p.logits + (size_t)row * p.ld + first;
@@ -520,6 +521,7 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(SampleRows p
     const int top_k = p.top_k ? p.top_k[row] : 0;
     // the largest of every warp to all CTAs: the largest of all, and (below) a bound for the top_k largest
     best = warp_max(best);
+    cluster.barrier_wait();
     if (size == 1) {
         if (lane == 0) sh.tops[warp] = best;
         __syncthreads();

@@ -1,0 +1,28 @@
+"""Draws of whole steps (Ops.sample_rows) by clusters of every size, at the ends of what a row may be; the numbers as in test_sample_rows_gpu.py."""
+import pytest
+import torch
+from test_sample_rows_gpu import _check, _ops, _settings
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n", [2000, 4095, 8191, 16383, 32771])
+def test_rows_while_other_kernels_run(n):
+    """Clusters of 1, 2, 4, 8 and 16 CTAs that start while others' CTAs hold the machine: two streams of draws beside products give what one row after the other gives."""
+    x = 2.5 * torch.randn(12, n, generator=torch.Generator().manual_seed(n))
+    s = _settings(12, n)
+    _check(x, *s)
+    xs, dev = x.cuda(), [torch.tensor(v, dtype=torch.int32 if i == 1 else torch.float32, device="cuda") for i, v in enumerate(s)]
+    ops, a = _ops(), torch.randn(2048, 2048, device="cuda")
+    want = torch.empty(12, dtype=torch.int32, device="cuda")
+    ops.sample_rows(xs.data_ptr(), n, 12, n, *dev, want, torch.cuda.current_stream().cuda_stream)
+    streams, out = [torch.cuda.Stream() for _ in range(3)], torch.full((2, 60, 12), -5, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(60):
+        with torch.cuda.stream(streams[2]):
+            a @ a
+        for j in range(2):
+            for row in range(0, 12, 4):                          # a few rows a launch: large clusters
+                ops.sample_rows(xs[row:].data_ptr(), n, 4, n, *(d[row:] for d in dev), out[j, i, row:], streams[j].cuda_stream)
+    torch.cuda.synchronize()
+    assert (out == want).all()
