@@ -868,25 +868,35 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     }
                     const float m0 = fmaf(top[0], f[0], ev[0]), m1 = fmaf(top[1], f[1], ev[1]);
                     float mx = fmaxf(m0, m1);
-                    // Rare, with one vote for both: scores so large that a rounded product and one inside a multiply-add are far apart (every product is rounded then, so that no weight is
-                    // above 1), and a block whose weights come out below 2^-60 because its value scale is that much smaller than others' (`far`).
+                    // Rare, with one vote for both: scores so large that a rounded product and one inside a multiply-add are far apart, and a value scale's exponent is less than their steps: every
+                    // product is rounded then, its reference, rounded down, taken from it in front of the exponent, and what is above 1 still is 1 (the largest one's weight: rounded to nearest
+                    // the reference could be a step above or below, and the weight out of fp16's range); and a block whose weights come out below 2^-60 because its value scale is that much
+                    // smaller than others' (`far`).
                     float far[2] = {0.0f, 0.0f};
                     const bool rare = __any_sync(0xffffffffu, fabsf(mx) > 65536.0f ? mx != -INFINITY : fminf(m0, m1) < fmaxf(ref, mx) - 60.0f);
+                    bool large = false;
                     if (rare) {
-                        if (__any_sync(0xffffffffu, fabsf(mx) > 65536.0f && mx != -INFINITY)) {
-#pragma unroll
-                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f[e / 32]);
+                        large = __any_sync(0xffffffffu, fabsf(mx) > 65536.0f && mx != -INFINITY);
+                        if (large) {
                             top[0] *= f[0];
                             top[1] *= f[1];
-                            f[0] = f[1] = 1.0f;
-                            mx = fmaxf(__fadd_rn(top[0], ev[0]), __fadd_rn(top[1], ev[1]));
+                            mx = fmaxf(__fadd_rd(top[0], ev[0]), __fadd_rd(top[1], ev[1]));
                         }
                         // Nothing to O, but the denominator has their weights without the scale: they are taken 2^far larger, so that they do not vanish.
-                        const float base = fmaxf(ref, ceilf(mx));
+                        const float base = fmaxf(ref, ceilf(mx)), from = base == -INFINITY ? 0.0f : base;
+                        auto relative = [&](float product, int x) {        // 2^.. of a weight without the value scale, of a large score
+                            const float y = __fsub_rn(product, from);
+                            return y > -ev[x] ? -ev[x] : y;                // (NaN stays)
+                        };
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const float most = fmaf(top[x], f[x], ev[x]) - base;
+                            const float most = large ? relative(top[x], x) + ev[x] : fmaf(top[x], f[x], ev[x]) - base;
                             far[x] = most < -60.0f && most > -1e6f ? floorf(-most) : 0.0f;
+                        }
+                        if (large) {
+#pragma unroll
+                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(relative(__fmul_rn(__uint_as_float(s[e]), f[e / 32]), e / 32));
+                            f[0] = f[1] = 1.0f;
                         }
                     }
                     const float nr = fmaxf(ref, ceilf(mx)), less = kt == 0 || nr == ref ? 1.0f : tc_exp2(ref - nr);
@@ -899,7 +909,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     l = kt == 0 ? 0.0f : l * less;
                     ref = nr;
                     // where every score so far is -inf, -inf - ref were no number: relative to 0 their weights are 0
-                    const float base = ref == -INFINITY ? 0.0f : ref;
+                    const float base = ref == -INFINITY || large ? 0.0f : ref;
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const float neg = ev[x] - base + far[x];

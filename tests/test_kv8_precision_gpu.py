@@ -1,7 +1,10 @@
-"""Bits of the attention over the 8-bit cache (Ops.attention8) where few of them are left: results in bf16, against those in fp32."""
+"""Bits of the attention over the 8-bit cache (Ops.attention8) where few of them are left: results in bf16, against those in fp32; scores of
+any size."""
+import math
+
 import pytest
 import torch
-from kv8_testlib import off
+from kv8_testlib import cache_rows, off
 from test_kv8_attention_gpu import F32_BOUND, _case, _run, _want
 
 pytestmark = pytest.mark.gpu
@@ -18,3 +21,25 @@ def test_bf16_results_are_the_fp32_results_rounded(segs, heads, kv_heads, dim, o
     alone, (both, both16) = _run(step, q, k, v, heads, bf16=True, **opts), _run(step, q, k, v, heads, both=True, **opts)
     assert torch.equal(both, fp32) and torch.equal(alone, both16)
     assert torch.equal(alone, fp32.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("shift", [-40, -8, 0, 8, 9, 40])
+@pytest.mark.parametrize("segs", [[(700, 1), (64, 1)], [(700, 40), (64, 1)]], ids=["decode", "portions"])
+def test_large_scores_beside_scales_of_values(shift, segs):
+    """Scores whose steps are as large as the exponents of value scales: no weight leaves fp16's range, and a key that wins by more than the steps takes all the weight."""
+    heads, kv_heads, dim = 8, 2, 128
+    step, q, k, v = _case(segs, heads, kv_heads, dim)
+    v = (v[0], v[1] * 2.0 ** shift)
+    for size in (2.0 ** e for e in range(18, 32)):
+        got, at = _run(step, q * size, k, v, heads).double(), 0
+        assert got.isfinite().all(), size
+        for i, (p, n) in enumerate(segs):
+            kk, vv = (cache_rows(step, *x, i).repeat_interleave(heads // kv_heads, 0) for x in (k, v))
+            s = q[at:at + n].double().view(n, heads, dim).transpose(0, 1) @ kk.mT * dim ** -0.5
+            s = s.masked_fill(torch.arange(p + n, device="cuda") > torch.arange(p, p + n, device="cuda")[:, None], -math.inf)
+            (best, second), where = s.topk(2).values.unbind(-1), s.argmax(-1)
+            sure = (best - second) * size > torch.clamp(2.0 ** -18 * best.abs() * size, min=60.0)
+            want = vv.gather(1, where[..., None].expand(-1, -1, dim)).transpose(0, 1)
+            have, sure = got[at:at + n].view(n, heads, dim), sure.T
+            assert (((have - want).norm(dim=-1) / want.norm(dim=-1))[sure] < F32_BOUND).all(), (size, i)
+            at += n
