@@ -20,6 +20,10 @@ struct Attn8Args {
     uint16_t* out16;
 };
 
+// Softmax weights are the sum of two fp16 numbers, whose steps end at 2^-24: they are multiplied by 2^14 first (2 of them fit fp16 then), so that a weight is off by 2^-39 of the power of two above
+// the largest at most, or by 2^-22 of itself. As they are they would be off by 2^-25: a key 14 nats below the largest kept five bits of its weight, one 18 nats below none.
+constexpr int kA8Lift = 14;
+
 // The workspace: counters that every call leaves zero, then what CTAs that share an item leave of it. Its layout is the same for every step.
 constexpr int kA8Workers = 512;                                        // CTAs of a launch at most
 constexpr int kA8MaxHeads = 8;                                         // query heads of an item at most

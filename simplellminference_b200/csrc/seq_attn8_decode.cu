@@ -9,7 +9,7 @@
 //   waits for nobody else's.
 //   Products on mma.sync m16n8k16 with fp16 operands: e4m3 codes are fp16 numbers, so keys and values enter exactly, two codes an instruction. Keys are the A operand (16 of them x 16
 //   columns), queries the B operand: its eight columns are four heads twice, a query's value being the sum of two fp16 numbers (22 bits of the head's largest, which a power of two brings to
-//   1 .. 2). Both terms' scores then lie side by side in one lane. The softmax's weights are split the same way, transposed by movmatrix, and are the B operand of the second product, whose A
+//   1 .. 2). Both terms' scores then lie side by side in one lane. The softmax's weights are split the same way (2^14 times as large, kA8Lift), transposed by movmatrix, and are the B operand of the second product, whose A
 //   operand is the values, turned on the way from shared memory by two byte permutations for four codes. Which key is which row, and which column which k, is free as long
 //   as both operands agree: the order is the one in which a lane's 16-byte reads deliver them.
 //   Sums. The tensor core truncates as it accumulates: a chain of scores is four instructions long (64 columns), one of values two, before it is added to fp32 registers with ordinary rounding.
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_
                 }
                 const float base = ref[x] == -INFINITY ? 0.0f : ref[x];                              // nothing seen yet: every weight is 0
                 const int d = ev + d8_whole(ref[x]) - R[x];
-                const float lift = mant * kv8_pow2(max(-126, min(126, d)));
+                const float lift = mant * kv8_pow2(max(-126, min(126, d + kA8Lift)));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float q = tc_exp2(w[x][e] - base);
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_
         constexpr int kTail = kA8MaxHeads * 128;                               // where a record's references, sums and exponents begin
         // Sums of parts with references and exponents of their own, brought to the largest of each. A column's result: sum * 2^e / (den * 2^r); a query that sees no key gives 0.
         auto store = [&](int h, int col, float4 sum, float r, float den, int e) {
-            const float f = den == 0.0f ? 0.0f : kv8_pow2(max(-126, min(126, e - d8_whole(r)))) / den;
+            const float f = den == 0.0f ? 0.0f : kv8_pow2(max(-126, min(126, e - d8_whole(r) - kA8Lift))) / den;
             const float y[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
             if (col >= p.dv) return;
 #pragma unroll

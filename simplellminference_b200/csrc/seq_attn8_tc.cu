@@ -11,7 +11,7 @@
 // Results in bf16 are those in fp32, rounded: with one fp16 number for a query and a weight 15 % of them were another bf16 number (now 0.06 %, as far as fp32 sums let them), and they
 // depended on whether fp32 results were asked for as well; prompts below took 170 us then, 268 now.
 // Weights are relative to the largest of score + log2(value scale) so far, rounded up to a whole number: differences of exponents are exact then, and O is rescaled by powers of two, and
-// seldom. The denominator takes the value scale out again, block by block.
+// seldom; as operands, and in O, they are 2^14 times as large (kA8Lift). The denominator takes the value scale out again, block by block.
 // A value's NaN code must reach exactly the rows that see it, but 0 * NaN is NaN: the converters replace it and say so, and rows of such an item look for NaN among their keys' values
 // at the end.
 // Shares. A CTA per item would leave most SMs idle where few queries follow a long context. The key tiles of all items lie in one row, made by a CTA of the kernel in front from what the
@@ -115,6 +115,7 @@ struct T8Share {
     }
 };
 
+constexpr float kT8Down = 1.0f / (1 << kA8Lift);          // of weights, and of O
 constexpr int kT8Terms = 2;                      // fp16 numbers that a query, or a weight, is the sum of
 template <int HD>
 struct T8Shape {
@@ -614,14 +615,14 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                 if (j) ++items1; else ++items0;
                 if (!ok) break;
                 tc_fence_after();
-                const float ref = s_ref[j * kT8Rows + row], l = s_sum[j * kT8Rows + row], inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float ref = s_ref[j * kT8Rows + row], l = s_sum[j * kT8Rows + row], inv = l == 0.0f ? 0.0f : kT8Down / l;
                 mb_arrive(lread + j);
                 const bool nan_here = s_nan[n_item & 7] == n_item + 1;         // (behind the last product: every value has been converted)
                 const uint32_t o_tmem = tmem + ((uint32_t)(quad * 32) << 16) + kT8O + 128 * j;
                 uint4* acc = reinterpret_cast<uint4*>(part + j * kT8PartTile);
                 const bool flushed = mine > kT8Flush;
                 const T8Out to = t8_out(p, it, j, row);
-                const float f = whole ? inv : 1.0f;
+                const float f = whole ? inv : kT8Down;
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t o[32];
@@ -882,7 +883,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                             top[1] *= f[1];
                             mx = fmaxf(__fadd_rd(top[0], ev[0]), __fadd_rd(top[1], ev[1]));
                         }
-                        // Nothing to O, but the denominator has their weights without the scale: they are taken 2^far larger, so that they do not vanish.
+                        // Nothing to O (2^-60 is far below the last step of fp16, too), but the denominator has their weights without the scale: they are taken 2^far larger, so that they do not vanish.
                         const float base = fmaxf(ref, ceilf(mx)), from = base == -INFINITY ? 0.0f : base;
                         auto relative = [&](float product, int x) {        // 2^.. of a weight without the value scale, of a large score
                             const float y = __fsub_rn(product, from);
@@ -912,7 +913,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                     const float base = ref == -INFINITY || large ? 0.0f : ref;
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float neg = ev[x] - base + far[x];
+                        const float neg = ev[x] - base + (far[x] + (float)kA8Lift);
                         const uint64_t f2 = tc_two(__float_as_uint(f[x]), __float_as_uint(f[x])), neg2 = tc_two(__float_as_uint(neg), __float_as_uint(neg));
                         uint64_t sum = 0;
                         uint32_t hi[16], lo[16];
@@ -938,7 +939,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         tc_st16(p_tmem + 32 + 16 * x, lo);
                         float s0, s1;
                         tc_split(sum, s0, s1);
-                        l = fmaf(s0 + s1, tc_exp2(-ev[x] - far[x]), l);         // without the value scale
+                        l = fmaf((s0 + s1) * kT8Down, tc_exp2(-ev[x] - far[x]), l);         // without the value scale
                     }
                 }
                 tc_wait_st();

@@ -1,11 +1,11 @@
 """Bits of the attention over the 8-bit cache (Ops.attention8) where few of them are left: results in bf16, against those in fp32; scores of
-any size."""
+any size; thousands of weights far below one."""
 import math
 
 import pytest
 import torch
-from kv8_testlib import cache_rows, off
-from test_kv8_attention_gpu import F32_BOUND, _case, _run, _want
+from kv8_testlib import BLOCK, Step, cache_rows, codes_of, off, scale_for
+from test_kv8_attention_gpu import BF16_BOUND, F32_BOUND, _case, _run, _want
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,41 @@ def test_large_scores_beside_scales_of_values(shift, segs):
             have, sure = got[at:at + n].view(n, heads, dim), sure.T
             assert (((have - want).norm(dim=-1) / want.norm(dim=-1))[sure] < F32_BOUND).all(), (size, i)
             at += n
+
+
+def _pool(x, step):
+    """[pages][kv_heads][page][width] as the append leaves it."""
+    x = x.view(*x.shape[:2], step.page // BLOCK, BLOCK, -1)
+    scale = scale_for(x.abs().amax((-1, -2)))
+    return codes_of(x / scale[..., None, None]).flatten(2, 3).cuda(), scale.cuda()
+
+
+@pytest.mark.parametrize("gap", [10.0, 14.0, 18.0])
+@pytest.mark.parametrize("sink", ["ordinary", "zero"])
+@pytest.mark.parametrize("segs", [[(8000, 1), (3000, 1)], [(8000, 40), (3000, 3)]], ids=["decode", "portions"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_key_far_ahead_of_thousands(gap, sink, segs, dim):
+    """A key whose score is `gap` above all others', whose weights are e^-gap then, and add up to N e^-gap: of values that share a sign, they are a part of the result, or all of it where the
+    key's own value is 0. Then the key's score, of size gap, counts for every weight (2^-23 of it), and so does what the weights are rounded to: 2^-39 of the power of two above the largest
+    at most, 2^-38 of the largest, by chance up or down, which N of them have 1 / sqrt(3 N) of on average; four times that."""
+    heads, kv_heads = 8, 2
+    step = Step(segs, 64)
+    g = torch.Generator().manual_seed(int(gap))
+    q = torch.randn(step.T, heads, dim, generator=g)
+    q[..., 0] = gap * dim ** 0.5 / 16
+    k, v = (torch.randn(step.n_pages, kv_heads, step.page, dim, generator=g) for _ in range(2))
+    k, v = 0.1 * k, v.abs() + 0.5
+    k[..., 0] = 0.0
+    for i in range(len(segs)):
+        page, row = int(step.table_np[i, 100 // step.page]), 100 % step.page
+        k[page, :, row] = 0.0
+        k[page, :, row, 0] = 16.0
+        if sink == "zero":
+            v[page, :, row] = 0.0
+    q, k, v = q.flatten(1).cuda(), _pool(k, step), _pool(v, step)
+    want, got, got16, at = _want(step, q, k, v, heads), _run(step, q, k, v, heads), _run(step, q, k, v, heads, bf16=True), 0
+    for p, n in segs:
+        bound = F32_BOUND + (gap * 2.0 ** -23 + 4 * 2.0 ** -38 * math.exp(gap) / math.sqrt(3 * p) if sink == "zero" else 0.0)
+        assert off(got[at:at + n], want[at:at + n]) < bound, (p, n)
+        assert off(got16[at:at + n], want[at:at + n]) < BF16_BOUND, (p, n)
+        at += n
