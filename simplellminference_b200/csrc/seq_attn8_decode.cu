@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_
                 for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[ks][e]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int ex = top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127, -100) : 0;
+            const int ex = top < INFINITY ? min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126) : 0;      // so that 2^-ex is a normal number, too
             const float down = kv8_pow2(-ex), up = kv8_pow2(ex);
 #pragma unroll
             for (int ks = 0; ks < kSteps; ++ks) {

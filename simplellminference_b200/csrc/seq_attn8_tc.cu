@@ -736,8 +736,7 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                         most = tc_max3(tc_max3(most, of(w.x), of(w.y)), of(w.z), of(w.w));
                     }
                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-                    int e = max((int)(__float_as_uint(most) >> 23), 27);       // exponent + 127, 27 at least: the reciprocal stays a normal number
-                    if (e == 255) e = 127;                         // an infinity among them
+                    const int of = (int)(__float_as_uint(most) >> 23), e = of == 255 ? 127 : min(max(of, 27), 253);      // exponent + 127 (an infinity among them: 0), so that its reciprocal is a normal number
                     if (lane >> 4 == x) ex = e;
                     const float down = __uint_as_float((uint32_t)(254 - e) << 23);
                     __syncwarp();                                  // all have read

@@ -4,8 +4,8 @@ import math
 
 import pytest
 import torch
-from kv8_testlib import BLOCK, Step, cache_rows, codes_of, off, scale_for
-from test_kv8_attention_gpu import BF16_BOUND, F32_BOUND, _case, _run, _want
+from kv8_testlib import BLOCK, Step, attention, cache_rows, codes_of, off, scale_for
+from test_kv8_attention_gpu import BF16_BOUND, F32_BOUND, _case, _ops, _run, _want, _workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,22 @@ def test_one_key_far_ahead_of_thousands(gap, sink, segs, dim):
         assert off(got[at:at + n], want[at:at + n]) < bound, (p, n)
         assert off(got16[at:at + n], want[at:at + n]) < BF16_BOUND, (p, n)
         at += n
+
+
+@pytest.mark.parametrize("segs", [[(300, 1), (64, 1)], [(300, 70), (64, 1)]], ids=["decode", "portions"])
+@pytest.mark.parametrize("dim", [64, 128, 192])
+def test_queries_at_the_end_of_fp32(segs, dim):
+    """Queries of 2^126 to 2^128 over keys of the least scale and a score scale of 2^-38: scores of an ordinary size, as if both were scaled by powers of two."""
+    heads, kv_heads = 8, 2
+    step, q, k, v = _case(segs, heads, kv_heads, dim)
+    k = (k[0], torch.full_like(k[1], 2.0 ** -100))
+    q = torch.sign(q) * torch.clamp(q.abs(), 0.25, 0.999)
+    ops, out, out16 = _ops(), torch.empty(step.T, heads * dim, device="cuda"), torch.empty(step.T, heads * dim, device="cuda", dtype=torch.bfloat16)
+    ws = _workspace(ops, step, heads, kv_heads, dim, dim)
+    kv = [(cache_rows(step, *k, i), cache_rows(step, *v, i)) for i in range(len(segs))]
+    for up in (2.0 ** 126, 2.0 ** 127):
+        x = (q * up * 2.0).clamp(-3.4e38, 3.4e38)
+        want = attention(step, x, kv, heads, 2.0 ** -38)
+        ops.attention8(step.b, x.data_ptr(), heads * dim, heads, kv_heads, dim, dim, 2.0 ** -38, *k, *v, step.n_pages, ws, torch.cuda.current_stream().cuda_stream, out=out, ldo=heads * dim,
+                       out16=out16)
+        assert off(out, want) < F32_BOUND and off(out16, want) < BF16_BOUND, up
