@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdio>
 #include <string>
 
@@ -73,6 +74,23 @@ struct LaunchCfg {
         attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
         cfg.attrs = attr;
         cfg.numAttrs = pdl ? 1 : 0;
+    }
+};
+
+// A kernel's attributes belong to a device: what a launcher sets in front of its first launch, it sets on each device that becomes the current one. (Two host threads that both come first both
+// set them, which is the same.)
+class OncePerDevice {
+    std::atomic<uint64_t> done{0};
+  public:
+    template <class F>
+    int operator()(F set) {                // set() returns an SLLM code
+        int dev = 0;
+        SLLM_CUDA(cudaGetDevice(&dev));
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_acquire) & bit) return SLLM_OK;
+        if (int rc = set()) return rc;
+        done.fetch_or(bit, std::memory_order_release);
+        return SLLM_OK;
     }
 };
 

@@ -687,12 +687,13 @@ extern "C" int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, i
     SLLM_REQUIRE(logits && u && idx_dev && rows > 0 && n > 0, SLLM_EINVAL, "sample_rows: null pointer, no rows or no logits");
     SLLM_REQUIRE(ld >= n, SLLM_EINVAL, "sample_rows: rows of %d logits lie %d apart", n, ld);
     SLLM_REQUIRE(n <= kSrCluster * kSrSlice, SLLM_ENOTSUP, "sample_rows: %d logits in a row, %d at most", n, kSrCluster * kSrSlice);
-    static bool ready = false;
-    if (!ready) {
-        SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SrShared) + kSrSlice * 4 + 16));
-        ready = true;
-    }
+    static OncePerDevice ready;
+    if (int rc = ready([&] {
+            SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            SLLM_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SrShared) + kSrSlice * 4 + 16));
+            return SLLM_OK;
+        }))
+        return rc;
     // CTAs of a row: until one holds no more than 16384 logits, and then as long as the machine has room for twice as many and they have 2048 each. The five kinds of settings in turn over 128256
     // logits, with 4, 8 and 16 CTAs, us: 64 rows 63, 55 and 67 (of 16 only 14 clusters fit at once, of the others 33), 16 rows 53, 36 and 33.
     int cs = 1;

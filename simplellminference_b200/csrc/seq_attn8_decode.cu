@@ -556,11 +556,12 @@ __global__ void __launch_bounds__(kD8Warps * 32, kD8Ctas) seq_attention8_decode_
 template <int D, int NT>
 static int d8_launch(D8Args& a, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t st) {
     auto* kernel = seq_attention8_decode_kernel<D, NT>;
-    static bool ready = false;
-    if (!ready) {
-        SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, D8Tile<D>::kSmem));
-        ready = true;
-    }
+    static OncePerDevice ready;
+    if (int rc = ready([&] {
+            SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, D8Tile<D>::kSmem));
+            return SLLM_OK;
+        }))
+        return rc;
     overlapping(kernel)<<<std::min(kA8Workers, kD8Ctas * sm_count()), kD8Warps * 32, D8Tile<D>::kSmem, st>>>(tmK, tmV, a);
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();

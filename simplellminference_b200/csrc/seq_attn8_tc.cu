@@ -967,11 +967,12 @@ template <int HD, bool kOpts>
 static int t8_launch(const T8Args& a, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t st) {
     using Sh = T8Shape<HD>;
     auto* kernel = seq_attention8_tc_kernel<HD, kOpts>;
-    static bool ready = false;
-    if (!ready) {
-        SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
-        ready = true;
-    }
+    static OncePerDevice ready;
+    if (int rc = ready([&] {
+            SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+            return SLLM_OK;
+        }))
+        return rc;
     LaunchCfg lc(dim3(std::min(kA8TcWorkers, sm_count())), dim3(kT8Threads), Sh::kSmem, st, true);        // its beginning while the plan is made
     SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(kernel), tmK, tmV, a));
     LaunchCfg join(dim3(lc.cfg.gridDim.x, kT8JoinCtas), dim3(kT8Rows), 0, st, true);
