@@ -26,3 +26,16 @@ def test_rows_while_other_kernels_run(n):
                 ops.sample_rows(xs[row:].data_ptr(), n, 4, n, *(d[row:] for d in dev), out[j, i, row:], streams[j].cuda_stream)
     torch.cuda.synchronize()
     assert (out == want).all()
+
+
+@pytest.mark.parametrize("n", [720896, 720895, 655360 + 17])
+def test_the_longest_rows(n):
+    """All that a row may hold: 16 CTAs with 44 * 1024 logits each, and, where all are equal, a sum of 720896 * 2^44, as near to 2^64 as it gets. A weight that is not the largest is rounded to
+    2^-45 of that, by chance up or down: sums of all are off by some 2^-45 sqrt(n) = 2^-35 of it at most, where a draw has thousands of them."""
+    g = torch.Generator().manual_seed(n)
+    x = 2.5 * torch.randn(8, n, generator=g)
+    x[0] = x[1] = x[2] = -3.25
+    x[3] = torch.where(torch.arange(n) % 2 == 0, 1.0, 0.5)
+    t, k, p, m = [1.0, 0.7, 1.3, 1.0, 1.0, 0.9, 1.0, 0.8], [0, n // 3, 0, n - 1, 0, 300000, 0, 60], [1.0, 1.0, 0.9, 0.75, 1.0, 1.0, 0.95, 0.9], [0.0] * 6 + [1e-4, 0.0]
+    _check(x, t, k, p, m, [0.999999, 0.5, 0.0, 0.3, 0.77, 0.123456, 0.4, 0.9])
+    _check(x, [1e30] * 8, [0] * 8, [1.0] * 8, [0.0] * 8, [(i + 0.5) / 8 for i in range(8)])
