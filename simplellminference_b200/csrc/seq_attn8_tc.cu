@@ -810,15 +810,20 @@ __global__ void __launch_bounds__(kT8Threads, 1) seq_attention8_tc_kernel(const 
                             most[x] = fmaxf(t0, t1);
                         }
                         // scores below the cap, as nearly all are: tanh x = x g(x^2), g through Chebyshev's eight points of [0, 1] (9e-9 of its value; with its roundings 1.1e-7), two scores
-                        // at a time: 5 instructions a score, where tc_tanh takes 13 and two of the special function unit
+                        // at a time: 5 instructions a score, where tc_tanh takes 13 and two of the special function unit. Where one of the warp's scores is not, that of a hidden key (which may be
+                        // anything) among them, the others still go through the same series: it shows in no bit of theirs.
+                        constexpr float k7 = -0.00035232809f, k6 = 0.0022786476f, k5 = -0.0079124849f, k4 = 0.0214614104f, k3 = -0.0538697056f, k2 = 0.1333213896f, k1 = -0.333332777f;
                         if (__any_sync(0xffffffffu, !(fmaxf(most[0] * inv[0], most[1] * inv[1]) < 1.0f))) {
                             const float back[2] = {a.softcap / f[0], a.softcap / f[1]};
 #pragma unroll
-                            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(back[e / 32] * tc_tanh(__uint_as_float(s[e]) * inv[e / 32]));
+                            for (int e = 0; e < 64; ++e) {
+                                const float v = __uint_as_float(s[e]), x = __fmul_rn(v, inv[e / 32]), u = __fmul_rn(x, x);
+                                const float t = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, k7, k6), k5), k4), k3), k2), k1);
+                                s[e] = __float_as_uint(fabsf(x) < 1.0f ? __fmul_rn(v, fmaf(u, t, 1.0f)) : back[e / 32] * tc_tanh(x));
+                            }
                         } else {
                             auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
-                            const uint64_t c7 = both(-0.00035232809f), c6 = both(0.0022786476f), c5 = both(-0.0079124849f), c4 = both(0.0214614104f), c3 = both(-0.0538697056f),
-                                           c2 = both(0.1333213896f), c1 = both(-0.333332777f), one = both(1.0f);
+                            const uint64_t c7 = both(k7), c6 = both(k6), c5 = both(k5), c4 = both(k4), c3 = both(k3), c2 = both(k2), c1 = both(k1), one = both(1.0f);
 #pragma unroll
                             for (int e = 0; e < 64; e += 2) {
                                 const uint64_t v = tc_two(s[e], s[e + 1]), x = tc_mul2(v, both(inv[e / 32])), u = tc_mul2(x, x);

@@ -100,3 +100,26 @@ def test_queries_at_the_end_of_fp32(segs, dim):
         ops.attention8(step.b, x.data_ptr(), heads * dim, heads, kv_heads, dim, dim, 2.0 ** -38, *k, *v, step.n_pages, ws, torch.cuda.current_stream().cuda_stream, out=out, ldo=heads * dim,
                        out16=out16)
         assert off(out, want) < F32_BOUND and off(out16, want) < BF16_BOUND, up
+
+
+@pytest.mark.parametrize("segs", [[(500, 1), (31, 1)], [(500, 40), (31, 3), (0, 70)]], ids=["decode", "portions"])
+@pytest.mark.parametrize("opts", [dict(softcap=20.0), dict(softcap=20.0, window=50, keep_first=3), dict(softcap=2.0)], ids=str)
+def test_hidden_rows_change_no_bit_of_capped_scores(segs, opts):
+    """Rows behind a sequence or a window that hold zeros, the largest codes there are, or NaN; and what an earlier call has left in shared memory."""
+    heads, kv_heads, dim = 6, 1, 128
+    step, q, k, v = _case(segs, heads, kv_heads, dim)
+    hidden = torch.ones(step.n_pages, step.page, dtype=torch.bool)
+    for i, (p, n) in enumerate(segs):
+        for y in range(p + n):
+            if "window" not in opts or y > p - opts["window"] or y < opts["keep_first"]:
+                hidden[int(step.table_np[i, y // step.page]), y % step.page] = False
+    loud, results = _case([(900, 200)], heads, kv_heads, dim, seed=3), []
+    for code in (0x00, 0x7e, 0x7f, 0x00):
+        pools = []
+        for pool, scale in (k, v):
+            codes = pool.view(torch.uint8).clone()
+            codes[hidden.cuda()[:, None, :, None].expand_as(codes)] = code
+            pools.append((codes.view(torch.float8_e4m3fn), scale))
+        results.append(_run(step, q, *pools, heads, **opts))
+        _run(loud[0], loud[1] * 100, *loud[2:], heads)
+    assert all(torch.equal(r, results[0]) for r in results[1:])
