@@ -147,8 +147,8 @@ int sllm_sample_f32(const float* logits, int32_t n, float temperature, int32_t t
  * temperature, top_k, top_p, min_p, u: device arrays of one value per row (temperature NULL = 1, the next three NULL = all logits). w_i = exp((x_i - max x) / temperature);
  * kept are the top_k largest logits (0 = all), of these the smallest set of largest ones whose mass reaches top_p of theirs (0 or 1 = all), of these those with w_i >= min_p
  * (0 = all); equal logits are in or out together. Drawn is the first i whose running kept mass exceeds u * (kept mass), u in [0, 1). temperature <= 0: the first of the largest
- * logits. NaN counts as -infinity, which is never drawn (a row of nothing else gives 0); where logits are +infinity, one of those is drawn. Weights are held as multiples of 2^-44, so
- * that sums are exact and the result is a function of the row alone. idx_dev [rows] int32; prob_dev [rows] or NULL: the drawn one's share of the kept mass. Up to 720896 logits a row. */
+ * logits. NaN counts as -infinity, which is never drawn (a row of nothing else gives 0); where logits are +infinity, one of those is drawn. Weights are held as multiples of 2^-44 of
+ * the largest, so that sums are exact and the result is a function of the row alone (a logit that weighs less than 2^-45 is never drawn). idx_dev [rows] int32; prob_dev [rows] or NULL: the drawn one's share of the kept mass. Up to 720896 logits a row. */
 int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, int32_t n, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                      const float* u, int32_t* idx_dev, float* prob_dev, sllm_stream_t stream);
 
@@ -546,10 +546,12 @@ int sllm_seq_rotary_kv8(const sllm_seq_batch* b, const float* q, int32_t ldq, in
                         int32_t ldv, int32_t dv, const float* angles, int32_t n_freq, int32_t layout, float* q_out, int32_t ldqo, void* k_pool, float* k_scale,
                         void* v_pool, float* v_scale, int32_t n_pages, sllm_stream_t stream);
 /* Causal softmax attention of the listed tiles' tokens over the 8-bit cache: score = (q . k) * scale (positive), query head h reads key/value head h / (heads / kv_heads). Options: window,
- * keep_first, softcap, slopes, chunk; the others are SLLM_ENOTSUP. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16), which is
- * the fp32 result rounded, whether or not that is asked for; rows of tokens in no tile stay as they are. Keys whose page the table does not have are hidden; a token that sees none gives zeros. ws: at least sllm_seq_attention8_ws_bytes bytes, 16-byte aligned, zeros
- * before its first use and after an SLLM_ETIMEOUT; every call leaves its counters zero, so calls one behind the other may share it, calls that run side by side may not. A step
- * of as many segments as tokens has one token in each (a tile of more is reported as SLLM_EINVAL by the library's next call). */
+ * keep_first, softcap, slopes, chunk; the others are SLLM_ENOTSUP. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16: the fp32 result rounded, whether or
+ * not that is asked for); rows of tokens in no tile stay as they are. Scores and sums are fp32; up to 128 columns a head, queries carry 22 bits of their head's largest, a weight 22 bits or
+ * 2^-38 of the largest one, whichever is coarser. Keys whose page the table does not have are hidden; a token that sees none gives zeros. ws: at least sllm_seq_attention8_ws_bytes bytes
+ * (47 MB, whatever the step), 16-byte aligned, zeros before its first use and after an SLLM_ETIMEOUT; every call leaves its counters zero, so calls one behind the other may share it,
+ * calls that run side by side may not. A step of as many segments as tokens has one token in each (a tile of more is reported as SLLM_EINVAL by the library's next call) and takes one
+ * launch; one with more places (T) than segments takes the portions' launches, too, if none of it is a portion. Heads of more than 128 columns take a slower kernel. */
 int64_t sllm_seq_attention8_ws_bytes(const sllm_seq_batch* b, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv);
 int sllm_seq_attention8(const sllm_seq_batch* b, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv, float scale, const void* k_pool,
                         const float* k_scale, const void* v_pool, const float* v_scale, int32_t n_pages, void* ws, int64_t ws_bytes, const sllm_seq_attn_opts* opts, float* out,

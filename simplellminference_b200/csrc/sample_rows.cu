@@ -12,8 +12,8 @@
 // 1024 parts. The rest goes to one CTA, which compares it pair by pair; parts too full for that (hundreds of logits within 2^-14 of a bit, or beyond the last bin) are halved bit by bit.
 // A top_k below 7/8 of the cluster's warps needs no bins: the top_k-th largest of the warps' largest logits bounds it from below, the candidates from there on are the first CTA's, and the draw ends there.
 // Bound: chains. A row passes 4 to 10 barriers of its cluster (some 1000 clocks each), a weight is a chain of 13 double operations, and 64 rows of 128256 logits fill the shared memory of the
-// machine twice, so that half of them wait for the other half. Floors and times, us (fp32 logits in a captured graph): one row of 32000 0.02 (bytes) and 9.3 (a kernel that adds to one number: 1.1);
-// 64 rows of 128256 5.0, and by settings: top_k of 20 to 100 with top_p 28, top_p alone 92, min_p 19, none 41, a fifth each and a fifth at temperature 0 51 to 56.
+// machine twice, so that half of them wait for the other half. Floors and times, us (fp32 logits in a captured graph): one row of 32000 0.02 (bytes) and 9.5 (a kernel that adds to one number: 1.1);
+// 64 rows of 128256 5.0, and by settings: top_k of 20 to 100 with top_p 30, top_p alone 92, min_p 19, none 41, a fifth each and a fifth at temperature 0 55.
 #include <cooperative_groups.h>
 
 #include "seq_common.cuh"

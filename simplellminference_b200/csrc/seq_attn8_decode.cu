@@ -1,7 +1,8 @@
 // csrc/seq_attn8_decode.cu — attention of single tokens over the 8-bit paged cache, heads of up to 128 columns: one launch, whatever the contexts are.
 //
-// Bound: the cache's bytes. 64 requests of up to 8191 positions, 32 heads over 8 of 128: 97 us, 80 at the rate of a copy (5.4 TB/s); eight of 76 to 8000 17.2, of which 7.3; one of 8000 13.9, of
-// which 2.5: the launch, the look at the contexts, an item's beginning and end and the joining of parts take 11 us whatever the contexts are. Everything else is arranged so that the bytes keep coming:
+// Bound: the cache's bytes. 64 requests of up to 8191 positions, 32 heads over 8 of 128: 98 us, 80 at the rate of a copy (5.3 TB/s); eight of 76 to 8000 17.4, of which 7.3; one of 8000 13.8, of
+// which 2.5: the launch, the look at the contexts, an item's beginning and end and the joining of parts through global memory take 11 us here whatever the contexts are, which is this kernel's way
+// and no floor (the kernel over bf16 pools, whose clusters join parts in shared memory, serves eight requests of 64 positions in 7.0). Everything else is arranged so that the bytes keep coming:
 //   Work. A unit is one block of 32 keys for the query heads of a kv head (up to 8 at a time). All units of a step lie in one row, request by request and head by head, and every CTA
 //   takes an equal share of it, found from the contexts on the device: requests of 77 and of 8000 positions fill the machine alike. A request's head that several CTAs share is put
 //   together by the one of them that is done last (a counter), in the order of its parts.

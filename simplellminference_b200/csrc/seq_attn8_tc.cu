@@ -9,7 +9,7 @@
 //   warps 12-15         O of both tiles: rescaled where a maximum has grown, results or parts of them written.
 // Queries and weights are the sum of two fp16 numbers each (22 bits), and O is added to an fp32 copy of the CTA's own every kT8Flush tiles, because the tensor core truncates as it accumulates.
 // Results in bf16 are those in fp32, rounded: with one fp16 number for a query and a weight 15 % of them were another bf16 number (now 0.06 %, as far as fp32 sums let them), and they
-// depended on whether fp32 results were asked for as well; prompts below took 170 us then, 268 now.
+// depended on whether fp32 results were asked for as well; the prompts below took 170 us then.
 // Weights are relative to the largest of score + log2(value scale) so far, rounded up to a whole number: differences of exponents are exact then, and O is rescaled by powers of two, and
 // seldom; as operands, and in O, they are 2^14 times as large (kA8Lift). The denominator takes the value scale out again, block by block.
 // A value's NaN code must reach exactly the rows that see it, but 0 * NaN is NaN: the converters replace it and say so, and rows of such an item look for NaN among their keys' values
@@ -17,9 +17,10 @@
 // Shares. A CTA per item would leave most SMs idle where few queries follow a long context. The key tiles of all items lie in one row, made by a CTA of the kernel in front from what the
 // device knows (contexts, listed tiles); every CTA takes an equal run of it. Items that a cut goes through leave O, reference and sum as parts, which a kernel behind puts together (done by
 // the last of an item's CTAs, one SM reading what up to ten had left, that took as long as all the rest).
-// Bound: the chain of a step (64 keys for 256 rows): 2400 to 3600 clocks, of which the tensor pipe needs 1024 (2048 with two terms) and the exponentials 1024; in front of it some 16000 clocks for
-// launch, plan and the first queries, and 10000 to 20000 for every further item. Prompts of 2048, 1300 behind 700, 311 and 37 behind 4000 tokens, 32 heads over 8 of 128, bf16 results: 162 us, 41 at
-// the rate of a large product. A portion of 256 behind 6000 and 12 decoding requests, capped, fp32: 146 us, 32 with two terms.
+// Bound: the chain of a step (64 keys for 256 rows): 2.6 us, 3.8 with capped scores (18 portions of 64 queries behind 4000 and 8100 positions), of which the tensor pipe needs 2048 clocks and the
+// exponentials 1024; an item's beginning and end, 10 us (1184 items of one step); some 20 us of launches, plan and first queries. Prompts of 2048, 1300 behind 700, 311 and 37 behind 4000 tokens,
+// 32 heads over 8 of 128, bf16 results: 276 us, 41 at the rate of a large product and 81 with the two terms. A portion of 256 behind 6000 and 12 decoding requests, capped, fp32: 148 us, 32 with two
+// terms.
 #include <type_traits>
 
 #include "seq_attn8.cuh"
@@ -28,9 +29,9 @@
 namespace sllm {
 
 constexpr int kT8Rows = 128, kT8Keys = kA8Keys, kT8Threads = 512; // rows of a tile, keys of a tile
-// Key tiles that an item's beginning and end count for (4, 6 and 8: 184, 186 and 186 us for prompts, 144, 144 and 145 for a portion); key tiles of a CTA's share at least; key tiles after which fp32
-// results leave tensor memory, which truncates as it adds, all one way. The portion below, 16, 8, 4 and 2 tiles: 147, 147, 151 and 153 us (now 146), off by 2.2e-6, 1.7e-6, 0.8e-6 and 0.7e-6 of the norm (the latter two
-// with the second terms of scores first, which costs nothing); fp32 arithmetic throughout is off by 1.3e-6.
+// Key tiles that an item's beginning and end count for (4, 6 and 8: 280, 278 and 280 us for prompts, 151, 152 and 152 for a portion); key tiles of a CTA's share at least; key tiles after which O
+// leaves tensor memory, which truncates as it adds, all one way. Prompts, fp32 results, 16, 8, 4 and 2 tiles: 262, 271, 282 and 299 us, off by 1.4e-6, 1.0e-6, 0.7e-6 and 0.5e-6 of the norm; the portion
+// 141, 143, 147 and 148 us, off by 1.4e-6, 0.9e-6, 0.6e-6 and 0.5e-6, where fp32 arithmetic throughout is off by 1.1e-6.
 constexpr int kT8Extra = kA8Extra, kT8Least = 4, kT8Flush = 4;
 constexpr int kT8Known = 16;                    // key tiles whose scales are kept at hand: more than the producer is ever ahead of the softmax (the rings' stages and two)
 constexpr uint32_t kT8Tmem = 512, kT8S = 0, kT8P = 128, kT8O = 256;           // columns: S0 S1 | P0 P1 | O0 O1

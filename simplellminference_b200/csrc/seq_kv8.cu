@@ -4,8 +4,8 @@
 // keeps them in registers, takes their largest magnitude and stores codes and scale; where the block holds earlier rows and its scale grows, their codes move to the new one.
 // No other CTA touches the block, so nothing is atomic and the result does not depend on the order of CTAs. The others turn a token's queries.
 // Angles come as a table (sllm_seq_angles): made once a step for all layers, they cost a layer 8 bytes a pair and token here instead of a sine and a cosine in double per head.
-// Bound: bytes; queries in and out are most of them (32 heads over 8: 32 of 43 KB a token). Prompts of 3896 tokens, 32 heads over 8 of 128: 39.5 us, 26 at the rate of a copy (4.3 TB/s; loads wait
-// for memory); 64 requests of one token 3.9 us, one 2.8 (a kernel that adds to one number takes 1.1).
+// Bound: bytes; queries in and out are most of them (32 heads over 8: 32 of 43 KB a token). Prompts of 3896 tokens, 32 heads over 8 of 128: 39.4 us, 26 at the rate of a copy (4.3 TB/s; loads wait
+// for memory, and the queries' stream shares registers and block size with the cache's part); 64 requests of one token 3.9 us, one 2.8 (a kernel that adds to one number takes 1.1).
 #include <climits>
 
 #include "kv8.cuh"
@@ -120,7 +120,7 @@ __device__ __forceinline__ void kv8_block(const Kv8Args& p, int tok0, int pos0, 
 }
 
 // kJobs: jobs of a thread for 32 rows
-// Eight CTAs an SM, though 64 registers spill 50 words: 39.5 us for the prompts above, with six of 80 registers and one division a thread instead of one a job 42.3, with the layout an argument 51.7.
+// Eight CTAs an SM, though their 64 registers spill 50 words (as do 128): 39.4 us for the prompts above, with six of 80 registers and one division a thread instead of one a job 42.3, with the layout an argument 51.7.
 template <bool kVec, int kLayout, int kJobs>
 __global__ void __launch_bounds__(kKv8Threads, kJobs == 4 ? 8 : 4) seq_rotary_kv8_kernel(Kv8Args p) {
     after_previous();

@@ -146,7 +146,7 @@ class Ops:
         return int(n)
 
     def attention8(self, b, q_ptr, ldq, heads, kv_heads, dk, dv, scale, k_pool, k_scale, v_pool, v_scale, n_pages, ws, st, out=None, ldo=0, out16=None, opts=None):
-        """Attention over the 8-bit cache: the result as fp32 rows (``out``) and / or dense bf16 rows (``out16``: the same, rounded)."""
+        """Attention over the 8-bit cache: the result as fp32 rows (``out``) and / or dense bf16 rows (``out16``: the same, rounded). ``ws``: of ``attention8_ws_bytes``."""
         self._ck(self.lib.sllm_seq_attention8(C.byref(b), q_ptr, ldq, heads, kv_heads, dk, dv, scale, _p(k_pool), _p(k_scale), _p(v_pool), _p(v_scale), n_pages, _p(ws),
                                               0 if ws is None else ws.numel() * ws.element_size(), C.byref(opts) if opts is not None else None, _p(out), ldo, _p(out16), st))
 
