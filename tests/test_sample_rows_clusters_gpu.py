@@ -39,3 +39,33 @@ def test_the_longest_rows(n):
     t, k, p, m = [1.0, 0.7, 1.3, 1.0, 1.0, 0.9, 1.0, 0.8], [0, n // 3, 0, n - 1, 0, 300000, 0, 60], [1.0, 1.0, 0.9, 0.75, 1.0, 1.0, 0.95, 0.9], [0.0] * 6 + [1e-4, 0.0]
     _check(x, t, k, p, m, [0.999999, 0.5, 0.0, 0.3, 0.77, 0.123456, 0.4, 0.9])
     _check(x, [1e30] * 8, [0] * 8, [1.0] * 8, [0.0] * 8, [(i + 0.5) / 8 for i in range(8)])
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+def test_captured_behind_the_kernel_that_writes_the_rows(overlap):
+    """Draws from what an attention leaves, their kernel resident early or not, the step replayed: what the calls give one by one."""
+    from test_kv8_attention_gpu import _case, _workspace
+    ops, heads, kv_heads, dim = _ops(), 32, 8, 128
+    step, q, k, v = _case([(300, 1), (64, 1), (4000, 1), (7, 1)], heads, kv_heads, dim)
+    ws, out = _workspace(ops, step, heads, kv_heads, dim, dim), torch.empty(4, heads * dim, device="cuda")
+    idx = torch.full((4,), -5, dtype=torch.int32, device="cuda")
+    p, u = torch.full((4,), 0.9, device="cuda"), torch.tensor([0.1, 0.4, 0.7, 0.95], device="cuda")
+
+    def calls(st):
+        ops.attention8(step.b, q.data_ptr(), heads * dim, heads, kv_heads, dim, dim, dim ** -0.5, *k, *v, step.n_pages, ws, st, out=out, ldo=heads * dim)
+        ops.sample_rows(out.data_ptr(), heads * dim, 4, heads * dim, None, None, p, None, u, idx, st)
+
+    calls(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want, side, graph = idx.clone(), torch.cuda.Stream(), torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph, stream=side):
+        calls(side.cuda_stream)
+    if overlap:
+        assert ops.overlap(graph.raw_cuda_graph()) > 0
+    graph.instantiate()
+    for _ in range(20):
+        out.fill_(0.0)
+        idx.fill_(-5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(idx, want)
