@@ -246,8 +246,8 @@ def _attend(s):
     heads, kv_heads, dim = case["heads"], case["kv_heads"], case["dim"]
     if own:
         f32 = case["out"] == "f32"
-        s["ops"].attention_shared(s["batch"], len(s["groups"]), s["group_start"], s["group_len"], s["q"].data_ptr(), heads * dim, heads, kv_heads, dim, dim, dim ** -0.5, s["k_pool"], s["v_pool"], s["ws"],
-                                  torch.cuda.current_stream().cuda_stream, out=s["out"] if f32 else None, ldo=heads * dim, out16=None if f32 else s["out"], opts=s["opts"])
+        s["ops"].attention_shared(s["batch"], len(s["groups"]), s["group_start"], s["group_len"], s["q"].data_ptr(), heads * dim, heads, kv_heads, dim, dim, dim ** -0.5, s["k_pool"], s["v_pool"], s["k_pool"].shape[0],
+                                  s["ws"], torch.cuda.current_stream().cuda_stream, out=s["out"] if f32 else None, ldo=heads * dim, out16=None if f32 else s["out"], opts=s["opts"])
         return s["out"]
     q = s["q"] if case["cache"] == "f32" else s["q"].bfloat16().float()
     per = heads // kv_heads
