@@ -151,6 +151,12 @@ int sllm_sample_f32(const float* logits, int32_t n, float temperature, int32_t t
  * the largest, so that sums are exact and the result is a function of the row alone (a logit that weighs less than 2^-45 is never drawn). idx_dev [rows] int32; prob_dev [rows] or NULL: the drawn one's share of the kept mass. Up to 720896 logits a row. */
 int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, int32_t n, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                      const float* u, int32_t* idx_dev, float* prob_dev, sllm_stream_t stream);
+/* How likely tokens are, for all rows in one launch. Row r of `rows`: n logits at logits + r * ld; p = softmax. token [rows] int32 or NULL: logprob [rows] = ln p(token), rank [rows] int32 =
+ * how many tokens come before it (larger logits, equal ones of a lower index); a token outside 0 .. n - 1 gives NaN and -1. entropy [rows] = -sum p ln p. top > 0 (32 at most): the most likely
+ * tokens in that order, top_idx [rows][top] int32 and top_logprob [rows][top]. Outputs that are not wanted are NULL. A logit of -infinity has no probability; where logits are +infinity, those share
+ * it evenly; a row with NaN, or of nothing but -infinity, gives NaN, its ranks and alternatives stay those of the order, in which NaN comes last. Sums are fp32, relative to the largest logit. */
+int sllm_token_logprobs(const float* logits, int64_t ld, int32_t rows, int32_t n, const int32_t* token, float* logprob, float* entropy, int32_t* rank, int32_t top, int32_t* top_idx,
+                        float* top_logprob, sllm_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------------
  * Synthetic weights (device side of oracle/synth_weights.h: same integer hash, bit-identical values).
@@ -448,6 +454,13 @@ typedef struct {
  * when out is NULL or holds less than that), or SLLM_EINVAL. */
 int64_t sllm_seq_step_fill(int32_t* out, int64_t capacity, int32_t nseg, const int32_t* segments, const int32_t* tokens, const int32_t* rows, int32_t n_rows,
                            const sllm_kvpages* kp, int32_t tile, int64_t* offsets, int32_t* n_qtiles);
+/* Rows of fp32 (x_bf16 != 0: bf16) values to 8-bit integers with a scale a row: scale = max(max |x| / 127, 2^-126), code = x / scale rounded to fp32 and then to the nearest whole number (of two
+ * as near the even one). A row with an infinite value or NaN gets the scale NaN and zeros. x [T][ldx] values, codes [T][ldc] int8 (columns behind K stay as they are), scales [T]. */
+int sllm_seq_quantise_rows(const void* x, int32_t x_bf16, int64_t ldx, void* codes, int64_t ldc, float* scales, int32_t T, int32_t K, sllm_stream_t stream);
+/* C[t][n] = (sum_k a[t][k] * w[n][k]) * a_scale[t] * w_scale[n] + bias[n] (+ C[t][n] if accumulate): int8 codes a [T][lda] and w [N][ldw], rows of both at multiples of 16 bytes and readable up to
+ * lda and ldw (what lies behind column K does not count), bias [N] or NULL, C fp32 [T][ldc]. Sums are exact (K up to 131072), then rounded to fp32; the products follow in this order. */
+int sllm_seq_linear8(const void* a, int64_t lda, const float* a_scale, const void* w, int64_t ldw, const float* w_scale, const float* bias, float* C, int64_t ldc, int32_t T, int32_t N, int32_t K,
+                     int32_t accumulate, sllm_stream_t stream);
 /* out[s][t][:] = table[ids[t]][:] * scale for every stream s (a model with one residual stream passes streams = 1) */
 int sllm_seq_embed(const int32_t* ids, const void* table, int32_t w_dtype, int32_t vocab, int32_t d, int32_t streams, float scale,
                    float* out, int32_t T, sllm_stream_t stream);
@@ -527,6 +540,16 @@ int sllm_seq_attention(const sllm_seq_batch* b, const float* q, int32_t ldq, int
 int sllm_seq_attention_out(const sllm_seq_batch* b, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv,
                            float scale, const void* k_pool, const void* v_pool, int32_t kv_dtype, int32_t nsplit, float* ws,
                            const sllm_seq_attn_opts* opts, float* out, int32_t ldo, void* out16, sllm_stream_t stream);
+/* sllm_seq_attention_out for segments in groups whose first positions are the same. Segments group_start[g] .. group_start[g + 1] - 1 (device arrays; group_start [n_groups + 1] ascends from 0 to
+ * nseg) share their positions 0 .. group_len[g] - 1, which are read once for all their tokens, through the block table of the group's first segment; the positions behind them through each
+ * segment's own. Segments come in the order of their tokens. 0: nothing is shared; a token sees no position behind its own, whatever group_len says. Pools in fp32 or bf16 (queries are then
+ * rounded to bf16) of n_pages pages: no others are touched, keys whose page the table does not have are hidden, and a token that sees none gives zeros. Options: window, keep_first, softcap,
+ * slopes; the others are SLLM_ENOTSUP. Head widths are multiples of 8 up to 256, scale is positive. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16: the fp32 result
+ * rounded); rows of tokens in no listed tile stay as they are. ws: at least sllm_seq_attention_shared_ws_bytes bytes, which need no contents; calls that may run at the same time need one each. */
+int64_t sllm_seq_attention_shared_ws_bytes(const sllm_seq_batch* b, int32_t n_groups, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv);
+int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const int32_t* group_start, const int32_t* group_len, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads,
+                              int32_t dk, int32_t dv, float scale, const void* k_pool, const void* v_pool, int32_t kv_dtype, int32_t n_pages, void* ws, int64_t ws_bytes,
+                              const sllm_seq_attn_opts* opts, float* out, int32_t ldo, void* out16, sllm_stream_t stream);
 /* Merges the shares, normalises (sink [heads] or NULL: the denominator of head h also holds exp(sink[h]), a term without key or value),
  * turns every head's output back by -pos * vfreq[m] (vfreq NULL = not), multiplies head h by sigmoid(gate[t][h]), or with gate_channels
  * column c of head h by sigmoid(gate[t][h*dv + c]) (gate NULL = not), and stores out[t][h*dv ..] and / or out16, dense bf16 rows. */

@@ -61,6 +61,7 @@ SIGNATURES = {
     "sllm_store_kv_row": (C.c_int, [_P, _P, _I, _I, _P]),
     "sllm_sample_f32": (C.c_int, [_P, _I, _F, _I, _F, C.c_uint64, C.c_uint64, _P, _P]),
     "sllm_sample_rows": (C.c_int, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "sllm_token_logprobs": (C.c_int, [_P, _L, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P]),
     "sllm_synth_fill": (C.c_int, [C.POINTER(Shape), C.c_uint64, _I, _L, _L, _L, _L, _L, _P, _I, _P, _I, _P]),
     "sllm_convert_weights": (C.c_int, [_P, _P, _I, _P, _I, _L, _L, _P]),
     "sllm_engine_create": (C.c_int, [C.POINTER(EngineConfig), _P, C.POINTER(_P)]),
@@ -165,6 +166,10 @@ SIGNATURES.update({
     "sllm_seq_rotary_kv8": (C.c_int, [_B, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P]),
     "sllm_seq_attention8_ws_bytes": (_L, [_B, _I, _I, _I, _I]),
     "sllm_seq_attention8": (C.c_int, [_B, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _P, _L, C.POINTER(SeqAttnOpts), _P, _I, _P, _P]),
+    "sllm_seq_attention_shared_ws_bytes": (_L, [_B, _I, _I, _I, _I, _I]),
+    "sllm_seq_attention_shared": (C.c_int, [_B, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _I, _I, _P, _L, C.POINTER(SeqAttnOpts), _P, _I, _P, _P]),
+    "sllm_seq_quantise_rows": (C.c_int, [_P, _I, _L, _P, _L, _P, _I, _I, _P]),
+    "sllm_seq_linear8": (C.c_int, [_P, _L, _P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _P]),
     "sllm_seq_attention_talk": (C.c_int, [_B, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P, _P, _I, _I, _P, C.POINTER(SeqAttnOpts), _P, _I, _P, _P, _I, _P, _P]),
     "sllm_seq_attention_talk_takes_mixed": (C.c_int, [_I, _I, _I, _I, _I]),
     "sllm_seq_angles": (C.c_int, [_B, _P, _I, _P, _P]),
@@ -202,10 +207,10 @@ SIGNATURES.update({
 })
 
 # The ragged-token-batch part of the library can be built and loaded on its own (`make -C csrc seq` -> libsllm_b200_seq.so: the
-# sllm_seq_* kernels, the tensor-core GEMM, the page bookkeeping, the sampler): a model made of those blocks then needs twenty-three
+# sllm_seq_* kernels, the tensor-core GEMM, the page bookkeeping, the sampler): a model made of those blocks then needs twenty-six
 # translation units compiled, not all of them. The full library contains the same objects and is preferred when it exists.
 SEQ_LIB_PATH = os.path.join(HERE, "lib", "libsllm_b200_seq.so")
-SEQ_SYMBOL_PREFIXES = ("sllm_seq_", "sllm_kvpages_", "sllm_sample_", "sllm_last_error", "sllm_status", "sllm_abi_version", "sllm_tune", "sllm_device_info",
+SEQ_SYMBOL_PREFIXES = ("sllm_seq_", "sllm_kvpages_", "sllm_sample_", "sllm_token_", "sllm_last_error", "sllm_status", "sllm_abi_version", "sllm_tune", "sllm_device_info",
                        "sllm_prefill_gemm_", "sllm_graph_")
 
 _lib = None

@@ -1,0 +1,296 @@
+// csrc/seq_attn_shared.cu — softmax attention of requests whose first positions are the same (several answers to one prompt, questions behind a common text).
+//
+//   s_j = scale * (q . k_j),  p = softmax over the visible j,  o = sum_j p_j v_j
+// The keys j below the group's shared length are read once for all tokens of the group: the query heads of a kv head and all the tokens are the rows of one product. The keys from there on are each
+// segment's own. Both leave (reference, sum, weighted values) of every row, and a last kernel puts them together. A hidden key's values may be anything: they reach no row that does not see it.
+#include <cfloat>
+
+#include "seq_attn_shared.cuh"
+
+namespace sllm {
+
+// Any head width, pools in fp32 or bf16: a CTA takes 4 * kRw rows of a (group or segment, kv head) and a share of the keys, 32 at a time through shared memory; a warp has kRw rows, a lane one
+// key of them for the scores and four columns of the values for the sums; fp32 throughout.
+constexpr int kShWarps = 4, kShKeys = 32;
+
+struct ShSpan {                          // rows and keys of a CTA
+    int tok0, n_rows, slot, key0, key1;  // rows: (token, head of the kv head) from tok0 on; keys [key0, key1)
+    int which;                           // of the records
+};
+
+template <typename T, int kRw>
+__device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, int g, float* smem) {
+    constexpr int kRows = kShWarps * kRw, kPer = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = p.heads / p.kv_heads;
+    const int ldk = p.dk + 4, cols = (p.dv + 127) / 128;
+    float *s_q = smem, *s_k = s_q + kRows * p.dk, *s_v = s_k + kShKeys * ldk, *s_p = s_v + kShKeys * p.dv;      // s_p: [warp][key][row]
+    for (int r0 = 0; r0 < sp.n_rows; r0 += kRows) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < kRows * p.dk; i += kShWarps * 32) {
+            const int r = r0 + i / p.dk, c = i % p.dk;
+            float x = 0.0f;
+            if (r < sp.n_rows) {
+                x = p.q[(size_t)(sp.tok0 + r / per) * p.ldq + (size_t)(g * per + r % per) * p.dk + c];
+                if (sizeof(T) == 2) x = seq_round_bf16(x);               // as the products on the tensor cores take it
+            }
+            s_q[i] = x;
+        }
+        int pos[kRw];
+        float m[kRw], l[kRw], o[kRw][2][4], slope[kRw];
+#pragma unroll
+        for (int i = 0; i < kRw; ++i) {
+            const int r = r0 + warp * kRw + i;
+            pos[i] = r < sp.n_rows ? p.b.tok_pos[sp.tok0 + r / per] : -1;
+            slope[i] = p.slopes ? p.slopes[g * per + r % per] : 0.0f;
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] = 0.0f;
+        }
+        for (int j0 = sp.key0 / kShKeys * kShKeys; j0 < sp.key1; j0 += kShKeys) {
+            const int page = sh_page(p, sp.slot, j0), in_page = j0 % p.b.page_len;           // (pages are a multiple of 32 positions)
+            // hidden from every row of the CTA: before its window, or no page
+            int seen = 0;
+#pragma unroll
+            for (int i = 0; i < kRw; ++i) seen |= pos[i] >= j0 && (pos[i] - (j0 + kShKeys - 1) < p.window || j0 < p.keep_first);
+            if (!__syncthreads_or(seen && page >= 0)) continue;          // (behind it the last tile has been read, and the queries are there)
+            int odd = 0;                                                 // a value that is infinite or NaN
+            for (int i = threadIdx.x; i < kShKeys * (p.dk / kPer); i += kShWarps * 32) {
+                const int k = i / (p.dk / kPer), c = i % (p.dk / kPer) * kPer;
+                float x[kPer];
+                seq_ld16(reinterpret_cast<const T*>(p.k_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page + k, p.dk) + c, j0 + k >= sp.key0 && j0 + k < sp.key1, x);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) s_k[k * ldk + c + e] = x[e];
+            }
+            for (int i = threadIdx.x; i < kShKeys * (p.dv / kPer); i += kShWarps * 32) {
+                const int k = i / (p.dv / kPer), c = i % (p.dv / kPer) * kPer;
+                float x[kPer];
+                seq_ld16(reinterpret_cast<const T*>(p.v_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page + k, p.dv) + c, j0 + k >= sp.key0 && j0 + k < sp.key1, x);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    s_v[k * p.dv + c + e] = x[e];
+                    odd |= !(fabsf(x[e]) <= FLT_MAX);
+                }
+            }
+            odd = __syncthreads_or(odd);
+            const int key = j0 + lane;
+            float s[kRw] = {};
+            for (int c = 0; c < p.dk; c += 4) {
+                const float4 k = *reinterpret_cast<const float4*>(s_k + lane * ldk + c);
+#pragma unroll
+                for (int i = 0; i < kRw; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(s_q + (warp * kRw + i) * p.dk + c);
+                    s[i] = fmaf(x.w, k.w, fmaf(x.z, k.z, fmaf(x.y, k.y, fmaf(x.x, k.x, s[i]))));
+                }
+            }
+            unsigned sees[kRw];
+#pragma unroll
+            for (int i = 0; i < kRw; ++i) {
+                const bool here = key >= sp.key0 && key < sp.key1 && seq_sees(pos[i], key, p.window, p.keep_first);
+                sees[i] = __ballot_sync(0xffffffffu, here);
+                const float x = here ? sh_score(s[i] * p.scale, p.softcap, slope[i], pos[i], key) : -INFINITY;
+                const float top = fmaxf(m[i], warp_max(x));
+                const float f = top == -INFINITY ? 1.0f : expf(m[i] - top), w = x == -INFINITY ? 0.0f : expf(x - top);
+                m[i] = top;
+                l[i] = l[i] * f + warp_sum(w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] *= f;
+                s_p[(warp * kShKeys + lane) * kRw + i] = w;
+            }
+            __syncwarp();
+            for (int k = 0; k < kShKeys; ++k) {
+                float w[kRw];
+#pragma unroll
+                for (int i = 0; i < kRw; ++i) w[i] = s_p[(warp * kShKeys + k) * kRw + i];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int col = c * 128 + 4 * lane;
+                    if (c >= cols || col >= p.dv) break;
+                    const float4 v = *reinterpret_cast<const float4*>(s_v + k * p.dv + col);
+#pragma unroll
+                    for (int i = 0; i < kRw; ++i) {
+                        if (odd && !(sees[i] >> k & 1)) continue;
+                        o[i][c][0] = fmaf(w[i], v.x, o[i][c][0]); o[i][c][1] = fmaf(w[i], v.y, o[i][c][1]);
+                        o[i][c][2] = fmaf(w[i], v.z, o[i][c][2]); o[i][c][3] = fmaf(w[i], v.w, o[i][c][3]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < kRw; ++i) {
+            const int r = r0 + warp * kRw + i;
+            if (r >= sp.n_rows) break;
+            float* rec = sh_record(p, sp.tok0 + r / per, g * per + r % per, sp.which);
+            if (lane == 0) {
+                rec[0] = m[i] * 1.4426950408889634f;
+                rec[1] = l[i];
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int col = c * 128 + 4 * lane;
+                if (col < p.dv) *reinterpret_cast<float4*>(rec + kShHead + col) = make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+            }
+        }
+    }
+}
+
+// The grid's x: row tiles of the groups (as many as there can be; the ones there are not have nothing to do), then the listed tiles of queries. y: kv heads; z: shares of the keys.
+template <typename T, int kRw>
+__global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(SharedArgs p, int group_tiles) {
+    after_previous();
+    extern __shared__ __align__(16) float sh_smem[];
+    constexpr int kRows = kShWarps * kRw;
+    const int g = blockIdx.y, per = p.heads / p.kv_heads, z = blockIdx.z, tokens = max(1, kRows / per);      // of a row tile
+    ShSpan sp;
+    if ((int)blockIdx.x < group_tiles) {
+        if (z >= p.shares) return;
+        int tile = blockIdx.x, i = 0, first = 0, n = 0;
+        for (; i < p.n_groups; ++i) {
+            sh_group_tokens(p, i, first, n);
+            const int tiles = (n + tokens - 1) / tokens;
+            if (tile < tiles) break;
+            tile -= tiles;
+        }
+        if (i == p.n_groups) return;
+        const int len = max(0, p.group_len[i]), tiles = (len + kShKeys - 1) / kShKeys;
+        sp.tok0 = first + tile * tokens;
+        sp.n_rows = min(tokens, n - tile * tokens) * per;
+        sp.slot = p.b.seg_slot[p.group_start[i]];
+        sp.key0 = (int)((long long)tiles * z / p.shares) * kShKeys;
+        sp.key1 = min(len, (int)((long long)tiles * (z + 1) / p.shares) * kShKeys);
+        sp.which = z;
+    } else {
+        if (z >= p.own) return;
+        const int x = blockIdx.x - group_tiles, seg = p.b.qt_seg[x], off = p.b.qt_off[x];
+        const int n = min(kBQ, p.b.seg_len[seg] - off), end = p.b.seg_pos0[seg] + off + n, from = min(sh_shared_len(p, seg), end);
+        const int t0 = from / kShKeys, tiles = (end + kShKeys - 1) / kShKeys - t0;
+        sp.tok0 = p.b.seg_start[seg] + off;
+        sp.n_rows = n * per;
+        sp.slot = p.b.seg_slot[seg];
+        sp.key0 = max(from, (t0 + tiles * z / p.own) * kShKeys);
+        sp.key1 = min(end, (t0 + tiles * (z + 1) / p.own) * kShKeys);
+        sp.which = p.shares + z;
+    }
+    sh_rows<T, kRw>(p, sp, g, sh_smem);
+}
+
+// The records of a (token, head) put together: a warp each.
+__global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedArgs p) {
+    after_previous();
+    const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], n = min(kBQ, p.b.seg_len[seg] - off), lane = threadIdx.x & 31, count = p.shares + p.own;
+    for (int i = blockIdx.y * 4 + (threadIdx.x >> 5); i < n * p.heads; i += gridDim.y * 4) {
+        const int t = p.b.seg_start[seg] + off + i / p.heads, h = i % p.heads;
+        const float* rec = sh_record(p, t, h, 0);
+        const int step = p.dv + kShHead;
+        float top = -INFINITY;
+        for (int k = lane; k < count; k += 32) top = fmaxf(top, rec[(size_t)k * step]);
+        top = warp_max(top);
+        float sum = 0.0f;
+        for (int k = lane; k < count; k += 32) {
+            const float m = rec[(size_t)k * step];
+            const float l = rec[(size_t)k * step + 1];
+            sum += m == -INFINITY && l == 0.0f ? 0.0f : exp2f(m - top) * l;        // (nothing seen, or nothing but NaN)
+        }
+        sum = warp_sum(sum);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int c = 4 * lane; c < p.dv; c += 128) {
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < count; ++k) {
+                const float m = rec[(size_t)k * step];
+                if (m == -INFINITY) continue;
+                const float f = exp2f(m - top);
+                const float4 x = *reinterpret_cast<const float4*>(rec + (size_t)k * step + kShHead + c);
+                o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+            }
+            const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (p.out) p.out[(size_t)t * p.ldo + (size_t)h * p.dv + c + e] = y[e];
+                if (p.out16) p.out16[((size_t)t * p.heads + h) * p.dv + c + e] = f32_to_bf16_bits(y[e]);
+            }
+        }
+    }
+}
+
+template <typename T, int kRw>
+static int sh_launch(const SharedArgs& p, cudaStream_t st) {
+    constexpr int kRows = kShWarps * kRw;
+    const int tokens = std::max(1, kRows / (p.heads / p.kv_heads));
+    const size_t smem = ((size_t)kRows * p.dk + (size_t)kShKeys * (p.dk + 4 + p.dv) + kShWarps * kShKeys * kRw) * sizeof(float);
+    static OncePerDevice ready;
+    if (int rc = ready([&] {
+            SLLM_CUDA(cudaFuncSetAttribute(seq_attention_shared_kernel<T, kRw>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024));
+            return SLLM_OK;
+        }))
+        return rc;
+    const long long tiles = (p.b.T + tokens - 1) / tokens + p.n_groups;
+    SLLM_REQUIRE(tiles + p.b.n_qtiles <= 0x7fffffffLL, SLLM_ENOTSUP, "seq_attention_shared: too many tokens");
+    overlapping(seq_attention_shared_kernel<T, kRw>)<<<dim3((unsigned)tiles + p.b.n_qtiles, p.kv_heads, std::max(p.shares, p.own)), kShWarps * 32, smem, st>>>(p, (int)tiles);
+    ++g_launches;
+    SLLM_LAUNCH_CHECK();
+    const int most = (p.b.T == p.b.nseg ? p.heads : kBQ * p.heads) / 4 + 1;
+    overlapping(seq_attention_shared_merge_kernel)<<<dim3(p.b.n_qtiles, std::min(most, 256)), 128, 0, st>>>(p);
+    ++g_launches;
+    SLLM_LAUNCH_CHECK();
+    return SLLM_OK;
+}
+
+}  // namespace sllm
+
+using namespace sllm;
+
+// Shares of the keys, the same for every call with these sizes: enough CTAs for the machine, records of a bounded size.
+static void shared_plan(int64_t T, int n_qtiles, int n_groups, int heads, int kv_heads, int* shares, int* own) {
+    const int64_t rows = T * (heads / kv_heads), tiles = ((rows + 15) / 16 + n_groups) * kv_heads, tiles_own = (int64_t)n_qtiles * kv_heads;
+    *shares = (int)std::min<int64_t>(24, std::max<int64_t>(1, 2 * sm_count() / tiles));
+    *own = (int)std::min<int64_t>(8, std::max<int64_t>(1, 2 * sm_count() / tiles_own));
+}
+
+extern "C" {
+
+int64_t sllm_seq_attention_shared_ws_bytes(const sllm_seq_batch* b, int32_t n_groups, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv) {
+    SLLM_REQUIRE(b && b->T > 0 && b->nseg > 0 && b->n_qtiles > 0 && n_groups > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && dk > 0 && dv > 0, SLLM_EINVAL,
+                 "seq_attention_shared_ws_bytes: bad argument");
+    int shares, own;
+    shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &shares, &own);
+    return (int64_t)b->T * heads * (shares + own) * (dv + kShHead) * (int64_t)sizeof(float);
+}
+
+int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const int32_t* group_start, const int32_t* group_len, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads,
+                              int32_t dk, int32_t dv, float scale, const void* k_pool, const void* v_pool, int32_t kv_dtype, int32_t n_pages, void* ws, int64_t ws_bytes,
+                              const sllm_seq_attn_opts* opts, float* out, int32_t ldo, void* out16, sllm_stream_t stream) {
+    SLLM_REQUIRE(b && b->T > 0 && b->nseg > 0 && b->tok_pos && b->seg_start && b->seg_len && b->seg_slot && b->seg_pos0 && b->block_table && b->max_pages > 0 && b->qt_seg && b->qt_off &&
+                     b->n_qtiles > 0,
+                 SLLM_EINVAL, "seq_attention_shared: incomplete batch description");
+    SLLM_REQUIRE(n_groups > 0 && n_groups <= b->nseg && group_start && group_len, SLLM_EINVAL, "seq_attention_shared: %d groups of %d segments", n_groups, b->nseg);
+    SLLM_REQUIRE(q && k_pool && v_pool && n_pages > 0 && (out || out16), SLLM_EINVAL, "seq_attention_shared: null pointer, no pages or no output");
+    SLLM_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, SLLM_EINVAL, "seq_attention_shared: %d query heads over %d kv heads", heads, kv_heads);
+    SLLM_REQUIRE(kv_dtype == SLLM_F32 || kv_dtype == SLLM_BF16, SLLM_ENOTSUP, "seq_attention_shared: fp32 or bf16 pools");
+    SLLM_REQUIRE(dk > 0 && dv > 0 && dk % 8 == 0 && dv % 8 == 0 && dk <= 256 && dv <= 256, SLLM_ENOTSUP, "seq_attention_shared: head widths %d and %d are not multiples of 8 up to 256", dk, dv);
+    SLLM_REQUIRE(kv_heads <= 65535, SLLM_ENOTSUP, "seq_attention_shared: %d kv heads", kv_heads);
+    SLLM_REQUIRE(scale > 0.0f && scale <= FLT_MAX, SLLM_EINVAL, "seq_attention_shared: scores need a positive finite scale");
+    SLLM_REQUIRE(b->page_len > 0 && b->page_len % kBK == 0, SLLM_ENOTSUP, "seq_attention_shared: pages of a multiple of %d positions", kBK);
+    SLLM_REQUIRE(ldq >= heads * dk && (!out || ldo >= heads * dv), SLLM_EINVAL, "seq_attention_shared: a row is shorter than its heads");
+    SLLM_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) % 16) == 0, SLLM_EINVAL, "seq_attention_shared: pools have to start at a multiple of 16 bytes");
+    SLLM_REQUIRE(ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= sllm_seq_attention_shared_ws_bytes(b, n_groups, heads, kv_heads, dk, dv), SLLM_EINVAL,
+                 "seq_attention_shared: the workspace is too small or not aligned");
+    SLLM_REQUIRE(!opts || (opts->window >= 0 && opts->keep_first >= 0 && opts->softcap >= 0.0f), SLLM_EINVAL, "seq_attention_shared: bad options");
+    SLLM_REQUIRE(!opts || (!opts->values_in_keys && !opts->logdist && !opts->cross_values && !opts->chunk), SLLM_ENOTSUP,
+                 "seq_attention_shared: values in keys, charges on the logarithm of the distance, values of every head and chunks are not part of this form");
+    SharedArgs p{*b, n_groups, group_start, group_len, q, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, INT_MAX, 0, 0.0f, nullptr, 0, 0, (float*)ws, out, ldo, (uint16_t*)out16};
+    if (opts) {
+        if (opts->window > 0) {
+            p.window = opts->window;
+            p.keep_first = opts->keep_first;
+        }
+        p.softcap = opts->softcap;
+        p.slopes = opts->slopes;
+    }
+    shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &p.shares, &p.own);
+    if (int rc = status_check()) return rc;
+    cudaStream_t st = as_stream(stream);
+    return kv_dtype == SLLM_F32 ? sh_launch<float, 4>(p, st) : sh_launch<uint16_t, 4>(p, st);
+}
+
+}  // extern "C"

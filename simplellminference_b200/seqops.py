@@ -78,6 +78,15 @@ class Ops:
                                           self.round_a_fixed if w_fixed else self.round_a, batch, a_bs, w_bs, bias_bs, c_bs,
                                           (scratch if isinstance(scratch, int) else _p(scratch)) if self.tensor_cores else None, int(a16_ready), rows_dev, st))
 
+    # ---- products of 8-bit integers ----
+    def quantise_rows(self, x_ptr, x_bf16, ldx, codes_ptr, ldc, scales, T, K, st):
+        """Rows of fp32 (or bf16) values to int8 codes, ``ldc`` bytes apart, and a scale a row: what ``linear8`` reads, for activations in every step and once for the rows of a matrix."""
+        self._ck(self.lib.sllm_seq_quantise_rows(x_ptr, int(bool(x_bf16)), ldx, codes_ptr, ldc, _p(scales), T, K, st))
+
+    def linear8(self, a_ptr, lda, a_scale, w, ldw, w_scale, bias, c_ptr, ldc, T, N, K, st, accumulate=False):
+        """C = (a . w^T) * a_scale[t] * w_scale[n] (+ bias) (+ C): int8 codes [T][lda] and [N][ldw], rows at multiples of 16 bytes; sums exact, the result fp32."""
+        self._ck(self.lib.sllm_seq_linear8(a_ptr, lda, _p(a_scale), _p(w), ldw, _p(w_scale), _p(bias), c_ptr, ldc, T, N, K, int(bool(accumulate)), st))
+
     def linear_grouped(self, a_ptr, a_bf16, w, c_ptr, counts_ptr, groups, cap, rows_hint, N, K, st):
         """``groups`` products one behind the other in one launch, each over the rows its count (device memory) says are in use."""
         self._ck(self.lib.sllm_seq_linear_grouped(a_ptr, int(bool(a_bf16)), _p(w), self.w_dtype, c_ptr, counts_ptr, groups, cap, rows_hint, N, K, st))
@@ -149,6 +158,21 @@ class Ops:
         """Attention over the 8-bit cache: the result as fp32 rows (``out``) and / or dense bf16 rows (``out16``: the same, rounded). ``ws``: of ``attention8_ws_bytes``."""
         self._ck(self.lib.sllm_seq_attention8(C.byref(b), q_ptr, ldq, heads, kv_heads, dk, dv, scale, _p(k_pool), _p(k_scale), _p(v_pool), _p(v_scale), n_pages, _p(ws),
                                               0 if ws is None else ws.numel() * ws.element_size(), C.byref(opts) if opts is not None else None, _p(out), ldo, _p(out16), st))
+
+    # ---- requests whose first positions are the same ----
+    def attention_shared_ws_bytes(self, b, n_groups, heads, kv_heads, dk, dv):
+        """Bytes of workspace ``attention_shared`` needs for a step like this."""
+        n = self.lib.sllm_seq_attention_shared_ws_bytes(C.byref(b), n_groups, heads, kv_heads, dk, dv)
+        if n < 0:
+            self._ck(int(n))
+        return int(n)
+
+    def attention_shared(self, b, n_groups, group_start, group_len, q_ptr, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, ws, st, out=None, ldo=0, out16=None, opts=None):
+        """``attention_out`` for segments in groups: the first ``group_len[g]`` positions of segments ``group_start[g]`` .. ``group_start[g + 1] - 1`` are the same and are read once for all
+        of them, through the block table of the group's first one (device arrays; 0: nothing is shared). ``ws``: of ``attention_shared_ws_bytes``."""
+        self._ck(self.lib.sllm_seq_attention_shared(C.byref(b), n_groups, _p(group_start), _p(group_len), q_ptr, ldq, heads, kv_heads, dk, dv, scale, _p(k_pool), _p(v_pool), self.kv_dtype,
+                                                    n_pages, _p(ws), 0 if ws is None else ws.numel() * ws.element_size(), C.byref(opts) if opts is not None else None, _p(out), ldo,
+                                                    _p(out16), st))
 
     @staticmethod
     def attention_options(window=0, keep_first=0, softcap=0.0, slopes=None, values_in_keys=False, logdist=None, cross_values=False, chunk=0):
@@ -310,3 +334,9 @@ class Ops:
         """The next token of every row, drawn from the given numbers ``u`` in [0, 1) with settings per row (device arrays, None = 1 / all / all / all);
         ``prob``: the probability of what was drawn among what was kept."""
         self._ck(self.lib.sllm_sample_rows(logits_ptr, ld, rows, n, _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(u), _p(idx), _p(prob), st))
+
+    # ---- how likely tokens are ----
+    def token_logprobs(self, logits_ptr, ld, rows, n, tokens, st, logprob=None, entropy=None, rank=None, top=0, top_idx=None, top_logprob=None):
+        """Of every row of logits: the given token's (``tokens``, device int32, or None) log probability and rank, the entropy in nats, and the ``top`` most likely tokens with their log
+        probabilities ([rows][top]); each of the outputs may be left out."""
+        self._ck(self.lib.sllm_token_logprobs(logits_ptr, ld, rows, n, _p(tokens), _p(logprob), _p(entropy), _p(rank), top, _p(top_idx), _p(top_logprob), st))
