@@ -556,6 +556,17 @@ int tc_encode_bytes(CUtensorMap* tm, const void* base, uint64_t rows, int width,
     return SLLM_OK;
 }
 
+int tc_encode_rows(CUtensorMap* tm, const void* base, uint64_t rows, int64_t width, int64_t stride, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    SLLM_REQUIRE(fn, SLLM_ESTATE, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)width, rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+    const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    SLLM_REQUIRE(r == CUDA_SUCCESS, SLLM_EINVAL, "cuTensorMapEncodeTiled failed (%d): %llu rows of %lld bytes, %lld apart", (int)r, (unsigned long long)rows, (long long)width, (long long)stride);
+    return SLLM_OK;
+}
+
 const char* pf_unsupported_reason(int w_dtype, int hd, int d, int q_loc, int I_loc) {
     if (w_dtype != SLLM_BF16) return "batched prefill needs bf16 weights (tensor-core operands)";
     if (hd != 64 && hd != 128) return "batched prefill attention is instantiated for head_dim 64 and 128";

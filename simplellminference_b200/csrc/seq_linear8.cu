@@ -3,6 +3,7 @@
 //   s_t = max(max_k |x_tk| / 127, 2^-126),  a_tk = round(x_tk / s_t);   C_tn = (sum_k a_tk w_nk) * s_t * v_n + bias_n
 // Sums of codes are exact in 32 bits (127 * 127 * 131072 < 2^31), so a result is three roundings of fp32 away from the formula and does not depend on how a product is cut.
 #include "seq_common.cuh"
+#include "tcgen05.cuh"
 
 namespace sllm {
 
@@ -113,18 +114,18 @@ __device__ __forceinline__ void l8_store(const Linear8Args& p, int t, int n, int
 }
 
 // A warp takes two rows of W and kT tokens: sixteen codes a load, four products an instruction.
-constexpr int kL8Warps = 8, kL8Rows = 2;
+constexpr int kL8Warps = 8, kL8Rows = 2, kL8Few = 4;
 template <int kT>
 __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args p) {
     after_previous();
-    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * kL8Warps + (threadIdx.x >> 5)) * kL8Rows, t0 = blockIdx.y * kT;
+    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * kL8Warps + (threadIdx.x >> 5)) * kL8Rows;
     if (n0 >= p.N) return;
     int sum[kL8Rows][kT] = {};
     const int8_t *w[kL8Rows], *a[kT];
 #pragma unroll
     for (int r = 0; r < kL8Rows; ++r) w[r] = p.w + (size_t)min(n0 + r, p.N - 1) * p.ldw;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) a[t] = p.a + (size_t)min(t0 + t, p.T - 1) * p.lda;
+    for (int t = 0; t < kT; ++t) a[t] = p.a + (size_t)min(t, p.T - 1) * p.lda;
 #pragma unroll 4
     for (int c = lane * 16; c < p.K; c += 512) {
         uint4 x[kL8Rows];
@@ -149,8 +150,233 @@ __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args 
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             const int v = __reduce_add_sync(0xffffffffu, sum[r][t]);
-            if (lane == 0 && n0 + r < p.N && t0 + t < p.T) l8_store(p, t0 + t, n0 + r, v);
+            if (lane == 0 && n0 + r < p.N && t < p.T) l8_store(p, t, n0 + r, v);
         }
+}
+
+// From kL8Few tokens on: tcgen05, products of 8-bit integers with sums in TMEM. The rows of W are the rows of a tile and the tokens its columns, however few there are: a tile is 128 rows of W by up
+// to 256 tokens, and the results of a token, neighbours in memory, lie in neighbouring lanes of a warp.
+//   warp 0 (one lane)  TMA producer: 128 bytes of K of the rows and of the tokens a stage (zeros behind the last of either);
+//   warp 1 (one lane)  MMA issuer, four products of 32 values of K a stage;
+//   warps 2-5          the sums out of TMEM, scales and bias, rows out, while the issuer fills the second accumulator.
+// Where rows and tokens make fewer tiles than the machine has SMs, a cluster shares a tile: its CTAs take a part of K each, leave their sums in shared memory and add up a part of the tokens each
+// (whole numbers: the order does not matter).
+constexpr int kL8TcThreads = 192, kL8Block = 128, kL8Stages = 12;
+constexpr uint32_t kL8RowBytes = 128 * kL8Block;
+constexpr int kL8Ring = 192 * 1024, kL8Smem = 1024 + kL8Ring + 512;
+
+struct Linear8Tc {
+    Linear8Args a;
+    int bn, t_tiles, units, blocks, stages, split, cols;      // tokens of a tile; tiles of tokens and in all; blocks of K; CTAs of a tile; TMEM columns of an accumulator
+    int32_t* status;
+    unsigned polls;
+};
+
+__device__ __forceinline__ int l8_peer(const void* local, uint32_t cta) {      // a word of another CTA of the cluster
+    uint32_t at;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(s_addr(local)), "r"(cta));
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void l8_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const Linear8Tc p) {
+    after_previous();        // in front of the allocation of TMEM: a CTA that waits for another kernel must not hold what that kernel's CTAs may be waiting for
+    extern __shared__ uint8_t l8_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(l8_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t a_bytes = (uint32_t)p.bn * kL8Block, stage_bytes = kL8RowBytes + a_bytes;
+    const int ST = p.stages;
+    uint64_t *full = reinterpret_cast<uint64_t*>(smem + kL8Ring), *empty = full + kL8Stages, *tfull = empty + kL8Stages, *tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmA);
+        for (int i = 0; i < ST; ++i) { mb_init(full + i, 1); mb_init(empty + i, 1); }
+        for (int i = 0; i < 2; ++i) { mb_init(tfull + i, 1); mb_init(tempty + i, 4); }
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tc_alloc(tmem_slot, 2 * p.cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int part = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, step = (int)gridDim.x / p.split;
+    const int k0 = p.blocks * part / p.split, k1 = p.blocks * (part + 1) / p.split;
+    if (warp == 0) {
+        if (elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int unit = first; ok && unit < p.units; unit += step) {
+                const int n0 = unit / p.t_tiles * 128, t0 = unit % p.t_tiles * p.bn;
+                for (int k = k0; k < k1; ++k) {
+                    ok = tc_wait(empty + stage, phase ^ 1, gave_up, p.polls);
+                    if (!ok) break;
+                    uint8_t* at = smem + (uint32_t)stage * stage_bytes;
+                    mb_expect(full + stage, stage_bytes);
+                    tma_load_2d(at, &tmW, k * kL8Block, n0, full + stage);
+                    tma_load_2d(at + kL8RowBytes, &tmA, k * kL8Block, t0, full + stage);
+                    if (++stage == ST) { stage = 0; phase ^= 1; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t idesc = umma_idesc_i8(128, p.bn);
+            const uint64_t w_desc = umma_desc_sw128(smem), a_desc = umma_desc_sw128(smem + kL8RowBytes);
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int unit = first; ok && unit < p.units; unit += step) {
+                ok = tc_wait(tempty + acc, acc_phase ^ 1, gave_up, p.polls);
+                if (!ok) break;
+                tc_fence_after();
+                for (int k = k0; k < k1; ++k) {
+                    ok = tc_wait(full + stage, phase, gave_up, p.polls);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t off = (uint64_t)((uint32_t)stage * (stage_bytes >> 4));
+#pragma unroll
+                    for (int i = 0; i < kL8Block / 32; ++i) tc_mma_i8(tmem + (uint32_t)(acc * p.cols), w_desc + off + 2 * i, a_desc + off + 2 * i, idesc, k > k0 || i);
+                    tc_commit(empty + stage);
+                    if (++stage == ST) { stage = 0; phase ^= 1; }
+                }
+                if (!ok) break;
+                tc_commit(tfull + acc);
+                if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quad = warp & 3;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int unit = first; unit < p.units; unit += step) {
+            if (!tc_wait_warp(tfull + acc, acc_phase, gave_up, p.polls)) break;
+            tc_fence_after();
+            const int n = unit / p.t_tiles * 128 + quad * 32 + lane, t0 = unit % p.t_tiles * p.bn;
+            const bool live = n < p.a.N;
+            const float ws = live ? p.a.w_scale[n] : 0.0f, bias = live && p.a.bias ? p.a.bias[n] : 0.0f;
+            const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * p.cols);
+#pragma unroll 1
+            for (int c = 0; c < p.bn; c += 32) {
+                uint32_t v[32];
+                __syncwarp();
+                tc_ld32(src + (uint32_t)c, v);
+                if (c + 32 >= p.bn) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mb_arrive(tempty + acc);
+                }
+                if (p.split > 1) {               // (every stage has been read: the ring is free)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c + j < p.bn) reinterpret_cast<int*>(smem)[(c + j) * 128 + quad * 32 + lane] = (int)v[j];
+                } else {
+                    const int t = t0 + c, have = min(32, min(p.bn - c, p.a.T - t));
+                    const float s = lane < have ? p.a.a_scale[t + lane] : 0.0f;
+                    float* to = p.a.out + (size_t)t * p.a.ldc + n;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float y = (float)(int)v[j] * __shfl_sync(0xffffffffu, s, j) * ws;
+                        if (j >= have || !live) continue;
+                        if (p.a.bias) y += bias;
+                        float* at = to + (size_t)j * p.a.ldc;
+                        *at = p.a.accumulate ? *at + y : y;
+                    }
+                }
+            }
+            if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        }
+        __syncwarp();
+    }
+    if (p.split > 1) {                           // one tile a cluster
+        l8_cluster_sync();
+        const int unit = first, n = unit / p.t_tiles * 128 + (warp & 3) * 32 + lane, t0 = unit % p.t_tiles * p.bn;
+        if (warp >= 2 && n < p.a.N) {
+            for (int j = part; j < p.bn && t0 + j < p.a.T; j += p.split) {
+                int sum = 0;
+                for (int r = 0; r < p.split; ++r) sum += l8_peer(reinterpret_cast<int*>(smem) + j * 128 + (warp & 3) * 32 + lane, (uint32_t)r);
+                l8_store(p.a, t0 + j, n, sum);
+            }
+        }
+        l8_cluster_sync();                       // nobody leaves while its sums are being read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*gave_up) tc_gave_up(p.status);
+    if (warp == 1) {
+        tc_fence_after();
+        tc_dealloc(tmem, 2 * p.cols);
+    }
+}
+
+// Tokens of a tile and CTAs that share one: the cheapest of all, a stage reckoned at what its products or its bytes take (clocks), a wave of tiles at its beginning and end beside its stages.
+struct Linear8Plan { int bn, split; };
+static Linear8Plan l8_plan(int T, int N, int K) {
+    const int sms = sm_count(), w_tiles = (N + 127) / 128, blocks = (K + kL8Block - 1) / kL8Block, most = std::min(256, (T + 15) / 16 * 16);
+    Linear8Plan best{16, 1};
+    double least = 1e30;
+    for (int bn = 16; bn <= most; bn += 16)
+        for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
+            if (split > 1 && bn > 128) break;
+            const double units = (double)w_tiles * ((T + bn - 1) / bn), waves = (double)(((long long)units * split + sms - 1) / sms);
+            const double stage = std::max(2.0 * bn, (kL8RowBytes + bn * kL8Block) / 50.0);
+            const double cost = waves * (((blocks + split - 1) / split) * stage + (split > 1 ? 4000.0 : 1500.0 + 4.0 * bn));
+            if (cost < least - 1e-9) { least = cost; best = {bn, split}; }
+        }
+    return best;
+}
+
+static int l8_tc(const Linear8Args& a, cudaStream_t st) {
+    static OncePerDevice ready;
+    if (int rc = ready([&] {
+            SLLM_CUDA(cudaFuncSetAttribute(linear8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kL8Smem));
+            return SLLM_OK;
+        }))
+        return rc;
+    const Linear8Plan pl = l8_plan(a.T, a.N, a.K);
+    Linear8Tc p{};
+    p.a = a;
+    p.bn = pl.bn;
+    p.split = pl.split;
+    p.t_tiles = (a.T + pl.bn - 1) / pl.bn;
+    const long long units = (long long)((a.N + 127) / 128) * p.t_tiles;
+    SLLM_REQUIRE(units * pl.split <= 0x7fffffffLL, SLLM_ENOTSUP, "seq_linear8: %d rows for %d tokens", a.N, a.T);
+    p.units = (int)units;
+    p.blocks = (a.K + kL8Block - 1) / kL8Block;
+    p.stages = std::min(kL8Stages, kL8Ring / ((int)kL8RowBytes + pl.bn * kL8Block));
+    p.cols = 32;
+    while (p.cols < pl.bn) p.cols *= 2;
+    if (int rc = status_check()) return rc;
+    if (int rc = status_word(&p.status)) return rc;
+    p.polls = (unsigned)g_tune_tc_polls;
+    CUtensorMap tmW, tmA;
+    if (int rc = tc_encode_rows(&tmW, a.w, (uint64_t)a.N, a.K, a.ldw, 128)) return rc;
+    if (int rc = tc_encode_rows(&tmA, a.a, (uint64_t)a.T, a.K, a.lda, pl.bn)) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(pl.split > 1 ? (unsigned)(p.units * pl.split) : (unsigned)std::min(p.units, sm_count()));
+    cfg.blockDim = dim3(kL8TcThreads);
+    cfg.dynamicSmemBytes = kL8Smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = pl.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pl.split > 1 ? 1 : 0;
+    SLLM_CUDA(cudaLaunchKernelEx(&cfg, overlapping(linear8_tc_kernel), tmW, tmA, p));
+    ++g_launches;
+    SLLM_LAUNCH_CHECK_ONLY();
+    return SLLM_OK;
 }
 
 }  // namespace sllm
@@ -187,12 +413,12 @@ int sllm_seq_linear8(const void* a, int64_t lda, const float* a_scale, const voi
     SLLM_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && (((uintptr_t)a | (uintptr_t)w) % 16) == 0, SLLM_EINVAL, "seq_linear8: rows of codes have to start at multiples of 16 bytes");
     Linear8Args p{(const int8_t*)a, (const int8_t*)w, a_scale, w_scale, bias, C, lda, ldw, ldc, T, N, K, accumulate != 0};
     cudaStream_t st = as_stream(stream);
-    const int wide = (N + kL8Warps * kL8Rows - 1) / (kL8Warps * kL8Rows), per = T > 2 ? 4 : T;
-    SLLM_REQUIRE((T + per - 1) / per <= 65535, SLLM_ENOTSUP, "seq_linear8: %d tokens", T);
-    const dim3 grid(wide, (T + per - 1) / per);
+    if (T > kL8Few) return l8_tc(p, st);
+    const int per = T > 2 ? kL8Few : T;
+    const dim3 grid((N + kL8Warps * kL8Rows - 1) / (kL8Warps * kL8Rows));
     if (per == 1) overlapping(linear8_few_kernel<1>)<<<grid, kL8Warps * 32, 0, st>>>(p);
     else if (per == 2) overlapping(linear8_few_kernel<2>)<<<grid, kL8Warps * 32, 0, st>>>(p);
-    else overlapping(linear8_few_kernel<4>)<<<grid, kL8Warps * 32, 0, st>>>(p);
+    else overlapping(linear8_few_kernel<kL8Few>)<<<grid, kL8Warps * 32, 0, st>>>(p);
     ++g_launches;
     SLLM_LAUNCH_CHECK();
     return SLLM_OK;

@@ -13,6 +13,9 @@ int tc_encode_bf16(CUtensorMap* tm, const void* base, int rank, const cuuint64_t
 // tensor map of rows of `width` bytes one behind the other, boxes of `box_rows` rows of 64 or 128 bytes in the swizzle of that span, zeros outside the tensor (prefill_gemm.cu)
 int tc_encode_bytes(CUtensorMap* tm, const void* base, uint64_t rows, int width, int box_rows, int box_width);
 
+// the same for rows of `width` bytes that lie `stride` bytes apart (a multiple of 16), boxes of 128 bytes (prefill_gemm.cu)
+int tc_encode_rows(CUtensorMap* tm, const void* base, uint64_t rows, int64_t width, int64_t stride, int box_rows);
+
 extern int g_tune_tc_polls;   // runtime.cu: polls after which the kernels below give up a wait
 
 #ifdef __CUDACC__
@@ -54,6 +57,13 @@ __device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t adesc, uin
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// 8-bit integers, sums in 32 bits
+__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // 32 lanes x 32 consecutive fp32 columns: thread i of the warp receives row (lane base + i)
 __device__ __forceinline__ void tc_ld32_async(uint32_t taddr, uint32_t* r) {      // complete after tc_wait_ld
     asm volatile(
@@ -85,6 +95,11 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(const void* tile) {
 // instruction descriptor, kind::f16: D = fp32 (1<<4), A = B = bf16 (1<<7, 1<<10), both K-major, N>>3 at bit 17, M>>4 at bit 24
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// the same for kind::i8: D = s32 (2<<4), A = B = signed (1<<7, 1<<10); an instruction takes 32 values of K
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int M, int N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
 // value operand: [keys][64 columns] blocks of 128-byte rows in the 128B swizzle, read with the columns as the N dimension (MN-major): the next 64

@@ -187,3 +187,19 @@ def test_captured_and_replayed():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(c, -first)
+
+
+@pytest.mark.parametrize("T,n,k", [(200, 700, 1000), (20, 256, 4096)], ids=["tiles", "shared tiles"])
+def test_waits_that_run_out_are_reported(T, n, k):
+    """With no polls allowed the tensor-core kernel gives up its first waits; the library's next call says so, once, and later products are whole again."""
+    from simplellminference_b200 import _lib
+    lib = _lib.load()
+    assert lib.sllm_status() == 0
+    assert lib.sllm_tune(10, 0) == 0
+    try:
+        with pytest.raises(_lib.SllmError) as e:
+            _product(T, n, k)
+    finally:
+        assert lib.sllm_tune(10, 1 << 24) == 0
+    assert e.value.code == _lib.ETIMEOUT and lib.sllm_status() == 0
+    _product(T, n, k)
