@@ -145,31 +145,28 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
     ShSpan sp;
     if ((int)blockIdx.x < group_tiles) {
         if (z >= p.shares) return;
-        int tile = blockIdx.x, i = 0, first = 0, n = 0;
-        for (; i < p.n_groups; ++i) {
-            sh_group_tokens(p, i, first, n);
-            const int tiles = (n + tokens - 1) / tokens;
-            if (tile < tiles) break;
-            tile -= tiles;
-        }
-        if (i == p.n_groups) return;
-        const int len = max(0, p.group_len[i]), tiles = (len + kShKeys - 1) / kShKeys;
+        int tile = blockIdx.x, first, n;
+        const int i = sh_find_group(p, tokens, tile, first, n);
+        if (i < 0) return;
+        const int len = max(0, p.group_len[i]), tiles = (len + kShKeys - 1) / kShKeys, cuts = sh_cuts(len, kShLeast, p.shares);
+        if (z >= cuts) return;
         sp.tok0 = first + tile * tokens;
         sp.n_rows = min(tokens, n - tile * tokens) * per;
         sp.slot = p.b.seg_slot[p.group_start[i]];
-        sp.key0 = (int)((long long)tiles * z / p.shares) * kShKeys;
-        sp.key1 = min(len, (int)((long long)tiles * (z + 1) / p.shares) * kShKeys);
+        sp.key0 = tiles * z / cuts * kShKeys;
+        sp.key1 = min(len, tiles * (z + 1) / cuts * kShKeys);
         sp.which = z;
     } else {
         if (z >= p.own) return;
         const int x = blockIdx.x - group_tiles, seg = p.b.qt_seg[x], off = p.b.qt_off[x];
         const int n = min(kBQ, p.b.seg_len[seg] - off), end = p.b.seg_pos0[seg] + off + n, from = min(sh_shared_len(p, seg), end);
-        const int t0 = from / kShKeys, tiles = (end + kShKeys - 1) / kShKeys - t0;
+        const int t0 = from / kShKeys, tiles = (end + kShKeys - 1) / kShKeys - t0, cuts = sh_cuts(end - from, kShOwnLeast, p.own);
+        if (z >= cuts) return;
         sp.tok0 = p.b.seg_start[seg] + off;
         sp.n_rows = n * per;
         sp.slot = p.b.seg_slot[seg];
-        sp.key0 = max(from, (t0 + tiles * z / p.own) * kShKeys);
-        sp.key1 = min(end, (t0 + tiles * (z + 1) / p.own) * kShKeys);
+        sp.key0 = max(from, (t0 + tiles * z / cuts) * kShKeys);
+        sp.key1 = min(end, (t0 + tiles * (z + 1) / cuts) * kShKeys);
         sp.which = p.shares + z;
     }
     sh_rows<T, kRw>(p, sp, g, sh_smem);
@@ -178,39 +175,50 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
 // The records of a (token, head) put together: a warp each.
 __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedArgs p) {
     after_previous();
-    const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], n = min(kBQ, p.b.seg_len[seg] - off), lane = threadIdx.x & 31, count = p.shares + p.own;
+    const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], n = min(kBQ, p.b.seg_len[seg] - off), lane = threadIdx.x & 31;
+    const int shared = sh_shared_len(p, seg), end = p.b.seg_pos0[seg] + off + n;
+    const int first = sh_cuts(shared, kShLeast, p.shares), count = first + sh_cuts(end - min(shared, end), kShOwnLeast, p.own);
     for (int i = blockIdx.y * 4 + (threadIdx.x >> 5); i < n * p.heads; i += gridDim.y * 4) {
         const int t = p.b.seg_start[seg] + off + i / p.heads, h = i % p.heads;
-        const float* rec = sh_record(p, t, h, 0);
-        const int step = p.dv + kShHead;
         float top = -INFINITY;
-        for (int k = lane; k < count; k += 32) top = fmaxf(top, rec[(size_t)k * step]);
+        for (int k = lane; k < count; k += 32) top = fmaxf(top, sh_record(p, t, h, k < first ? k : p.shares + k - first)[0]);
         top = warp_max(top);
-        float sum = 0.0f;
-        for (int k = lane; k < count; k += 32) {
-            const float m = rec[(size_t)k * step];
-            const float l = rec[(size_t)k * step + 1];
-            sum += m == -INFINITY && l == 0.0f ? 0.0f : exp2f(m - top) * l;        // (nothing seen, or nothing but NaN)
-        }
-        sum = warp_sum(sum);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (int c = 4 * lane; c < p.dv; c += 128) {
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = 0; k < count; ++k) {
-                const float m = rec[(size_t)k * step];
-                if (m == -INFINITY) continue;
-                const float f = exp2f(m - top);
-                const float4 x = *reinterpret_cast<const float4*>(rec + (size_t)k * step + kShHead + c);
-                o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+        float sum = 0.0f, o[2][4] = {};
+        for (int k = 0; k < count; ++k) {
+            const float* rec = sh_record(p, t, h, k < first ? k : p.shares + k - first);
+            const float m = rec[0], l = rec[1];
+            if (m == -INFINITY && l == 0.0f) continue;                   // nothing seen (a weight of NaN goes on)
+            const float f = exp2f(m - top);
+            sum = fmaf(f, l, sum);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int col = c * 128 + 4 * lane;
+                if (col >= p.dv) break;
+                const float4 x = *reinterpret_cast<const float4*>(rec + kShHead + col);
+                o[c][0] = fmaf(f, x.x, o[c][0]); o[c][1] = fmaf(f, x.y, o[c][1]); o[c][2] = fmaf(f, x.z, o[c][2]); o[c][3] = fmaf(f, x.w, o[c][3]);
             }
-            const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int col = c * 128 + 4 * lane;
+            if (col >= p.dv) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (p.out) p.out[(size_t)t * p.ldo + (size_t)h * p.dv + c + e] = y[e];
-                if (p.out16) p.out16[((size_t)t * p.heads + h) * p.dv + c + e] = f32_to_bf16_bits(y[e]);
+                const float y = o[c][e] * inv;
+                if (p.out) p.out[(size_t)t * p.ldo + (size_t)h * p.dv + col + e] = y;
+                if (p.out16) p.out16[((size_t)t * p.heads + h) * p.dv + col + e] = f32_to_bf16_bits(y);
             }
         }
     }
+}
+
+static int sh_merge(const SharedArgs& p, cudaStream_t st) {
+    const int most = (p.b.T == p.b.nseg ? p.heads : kBQ * p.heads) / 4 + 1;
+    overlapping(seq_attention_shared_merge_kernel)<<<dim3(p.b.n_qtiles, std::min(most, 256)), 128, 0, st>>>(p);
+    ++g_launches;
+    SLLM_LAUNCH_CHECK_ONLY();
+    return SLLM_OK;
 }
 
 template <typename T, int kRw>
@@ -228,11 +236,7 @@ static int sh_launch(const SharedArgs& p, cudaStream_t st) {
     SLLM_REQUIRE(tiles + p.b.n_qtiles <= 0x7fffffffLL, SLLM_ENOTSUP, "seq_attention_shared: too many tokens");
     overlapping(seq_attention_shared_kernel<T, kRw>)<<<dim3((unsigned)tiles + p.b.n_qtiles, p.kv_heads, std::max(p.shares, p.own)), kShWarps * 32, smem, st>>>(p, (int)tiles);
     ++g_launches;
-    SLLM_LAUNCH_CHECK();
-    const int most = (p.b.T == p.b.nseg ? p.heads : kBQ * p.heads) / 4 + 1;
-    overlapping(seq_attention_shared_merge_kernel)<<<dim3(p.b.n_qtiles, std::min(most, 256)), 128, 0, st>>>(p);
-    ++g_launches;
-    SLLM_LAUNCH_CHECK();
+    SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
 }
 
@@ -240,11 +244,11 @@ static int sh_launch(const SharedArgs& p, cudaStream_t st) {
 
 using namespace sllm;
 
-// Shares of the keys, the same for every call with these sizes: enough CTAs for the machine, records of a bounded size.
+// Shares of the keys at most, the same for every call with these sizes: enough CTAs for the machine, however few rows there are.
 static void shared_plan(int64_t T, int n_qtiles, int n_groups, int heads, int kv_heads, int* shares, int* own) {
-    const int64_t rows = T * (heads / kv_heads), tiles = ((rows + 15) / 16 + n_groups) * kv_heads, tiles_own = (int64_t)n_qtiles * kv_heads;
-    *shares = (int)std::min<int64_t>(24, std::max<int64_t>(1, 2 * sm_count() / tiles));
-    *own = (int)std::min<int64_t>(8, std::max<int64_t>(1, 2 * sm_count() / tiles_own));
+    const int64_t tiles = (T * (heads / kv_heads) / 128 + n_groups) * kv_heads, tiles_own = (int64_t)n_qtiles * kv_heads;
+    *shares = (int)std::min<int64_t>(32, std::max<int64_t>(1, (4 * sm_count() + tiles - 1) / tiles));
+    *own = (int)std::min<int64_t>(16, std::max<int64_t>(1, (4 * sm_count() + tiles_own - 1) / tiles_own));
 }
 
 extern "C" {
@@ -290,7 +294,11 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &p.shares, &p.own);
     if (int rc = status_check()) return rc;
     cudaStream_t st = as_stream(stream);
-    return kv_dtype == SLLM_F32 ? sh_launch<float, 4>(p, st) : sh_launch<uint16_t, 4>(p, st);
+    int rc;
+    if (kv_dtype == SLLM_F32) rc = sh_launch<float, 4>(p, st);
+    else if (dk == dv && (dk == 64 || dk == 128)) rc = launch_attention_shared_tc(p, st);
+    else rc = sh_launch<uint16_t, 4>(p, st);
+    return rc ? rc : sh_merge(p, st);
 }
 
 }  // extern "C"

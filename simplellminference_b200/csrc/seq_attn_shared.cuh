@@ -4,6 +4,10 @@
 
 namespace sllm {
 
+// the kernel for pools in bf16 and heads of 64 or 128 (seq_attn_shared_tc.cu)
+struct SharedArgs;
+int launch_attention_shared_tc(const SharedArgs& p, cudaStream_t st);
+
 // A step whose segments come in groups: the first group_len[g] positions of all segments group_start[g] .. group_start[g + 1] - 1 are the same and are read through the block table of the group's
 // first segment; the positions behind them through each segment's own.
 struct SharedArgs {
@@ -48,15 +52,42 @@ __device__ __forceinline__ void sh_group_tokens(const SharedArgs& p, int g, int&
     first = p.b.seg_start[s0];
     n = max(0, min(p.b.seg_start[s1 - 1] + p.b.seg_len[s1 - 1], p.b.T) - first);
 }
-// positions that segment `seg` shares with its group
+// positions that segment `seg` shares with its group (by whole warps)
 __device__ __forceinline__ int sh_shared_len(const SharedArgs& p, int seg) {
-    int lo = 0, hi = p.n_groups;         // group_start[lo] <= seg < group_start[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.group_start[mid] <= seg) lo = mid; else hi = mid;
-    }
-    return max(0, p.group_len[lo]);
+    int upto = 0;                        // groups that begin at or before the segment
+    for (int i = threadIdx.x & 31; i - (int)(threadIdx.x & 31) < p.n_groups; i += 32) upto += __popc(__ballot_sync(0xffffffffu, i < p.n_groups && p.group_start[i] <= seg));
+    return upto > 0 ? max(0, p.group_len[upto - 1]) : 0;
 }
+// The group that holds row tile `tile` of tiles of `tokens` tokens, group after group, its first token and how many it has; `tile` becomes the tile's number in it (by whole warps). -1: there
+// are not so many.
+__device__ __forceinline__ int sh_find_group(const SharedArgs& p, int tokens, int& tile, int& first, int& n) {
+    const int lane = threadIdx.x & 31;
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
+        first = n = 0;
+        if (g0 + lane < p.n_groups) sh_group_tokens(p, g0 + lane, first, n);
+        const int tiles = (n + tokens - 1) / tokens;
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, upto > tile);
+        if (past) {
+            const int who = __ffs(past) - 1;
+            tile -= __shfl_sync(0xffffffffu, upto - tiles, who);
+            first = __shfl_sync(0xffffffffu, first, who);
+            n = __shfl_sync(0xffffffffu, n, who);
+            return g0 + who;
+        }
+        tile -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return -1;
+}
+// How many of the step's shares a range of keys is cut into: none smaller than `least` keys.
+__device__ __forceinline__ int sh_cuts(int keys, int least, int most) { return keys <= 0 ? 0 : min(most, (keys + least - 1) / least); }
+constexpr int kShLeast = 256, kShOwnLeast = 512;         // of the shared positions; of a segment's own
+
 // a score after its scale: capped, charged for its distance
 __device__ __forceinline__ float sh_score(float s, float softcap, float slope, int pos, int key) {
     if (softcap > 0.0f) s = softcap * tanhf(s / softcap);

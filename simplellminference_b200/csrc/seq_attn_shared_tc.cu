@@ -1,0 +1,743 @@
+// csrc/seq_attn_shared_tc.cu — attention behind shared first positions over bf16 pools, heads of 64 or 128 columns.
+//
+// One launch, two kinds of CTAs. Where many rows see the same keys (the shared positions of a group, a portion's own positions) a CTA is a tile of 128 rows = the query heads of a kv head x
+// neighbouring tokens, on tcgen05, against a share of the keys, 64 at a time:
+//   warps 0-3  softmax, a thread per row: queries to bf16 rows in shared memory; per key tile the scores from TMEM, capped, charged and masked, fp32 maximum and sum; the weights go back to TMEM as
+//              THREE bf16 terms (24 bits; two leave 2^-18 of a weight, which is more than all the rest). O stays in TMEM, rescaled only where a maximum has grown by more than 2^8; the
+//              tensor core truncates as it adds, so every kStFlush tiles O moves on to the row's record;
+//   warp 4     (one lane) TMA producer: boxes of 32 positions, looked up in the block table; what is behind the last position or in no page reads as zeros;
+//   warp 5     (one lane) MMA issuer: S = Q K^T, O += (hi + mid + lo) V with the weights read from TMEM, V as it lies;
+//   warps 6-7  zero the value rows that are not part of the share, and take infinities and NaN out of the values (0 * NaN is NaN for rows that do not see them, and the terms of a weight times
+//              infinity are NaN for those that do); rows that see them get them back at the end.
+// Where a segment has few rows of its own (a decoding request: the query heads of one token), eight warps take 16 keys in turn on mma.sync, 8 rows at a time as the columns: such a CTA is bound by what
+// it reads, and a tile of 128 rows would be empty but for four. Keys and values go from the pool to registers as the products take them, 16 bytes a load: the columns of a head are contracted in
+// an order of the kernel's own, and those of the values are dealt to the tiles of O so that a lane's eight neighbours are rows of four of them.
+#include <cfloat>
+
+#include "seq_attn_shared.cuh"
+#include "tcgen05.cuh"
+
+namespace sllm {
+
+constexpr int kStRows = 128, kStKeys = 64, kStThreads = 256, kStBox = 32, kStWarps = kStThreads / 32;
+constexpr int kStFlush = 12;
+constexpr uint32_t kStTmem = 256;            // scores at 0 .. 63, then the weights' terms at 0 .. 95, O at 128; two CTAs share an SM's 512 columns
+constexpr int kStFew = 16;                   // rows of a segment up to which its own positions are the eight warps' work
+constexpr float kStLog2e = 1.4426950408889634f;
+
+template <int HD>
+struct StShape {
+    static constexpr int kBlocks = HD / 64, kQBlock = kStRows * 128, kQBytes = kBlocks * kQBlock, kKBlock = kStKeys * 128, kTile = kBlocks * kKBlock;
+    static constexpr int kStages = HD == 128 ? 2 : 4;
+    static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTile + 512;
+};
+
+struct StArgs {
+    SharedArgs a;
+    int hpc, sets, queries;                  // query heads of a tile, tiles' head sets of a kv head, tokens of a tile
+    int subs;                                // tiles that a listed tile of queries may need
+    int group_tiles;                         // row tiles of the groups at most
+    int vec_q;
+    int32_t* status;
+    unsigned polls;
+};
+
+// What a CTA does.
+struct StItem {
+    int tok0, nq, slot, g, h0;               // rows: nq tokens from tok0 on x hpc heads from h0 on, of kv head g
+    int key0, key1, which;                   // keys, and the record that takes the result
+};
+
+__device__ __forceinline__ void st_ld16(uint32_t taddr, uint32_t* o) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]),
+                   "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                 : "r"(taddr)
+                 : "memory");
+    tc_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) asm volatile("" : "+r"(o[e]));
+}
+// whether one of the eight bf16 values is infinite or NaN
+__device__ __forceinline__ bool st_odd(const uint4& v) {
+    auto two = [](uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u; };
+    return two(v.x) || two(v.y) || two(v.z) || two(v.w);
+}
+__device__ __forceinline__ uint32_t st_without(uint32_t x) {            // the pair with those replaced by zero
+    return ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u) | ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu);
+}
+__device__ __forceinline__ uint4 st_without(const uint4& v) { return make_uint4(st_without(v.x), st_without(v.y), st_without(v.z), st_without(v.w)); }
+
+// ---- few rows: eight warps -------------------------------------------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t st_turned(uint32_t x) {              // 8 x 8 values of 16 bits, transposed over the warp
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <int HD>
+__device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
+    const SharedArgs& p = sa.a;
+    constexpr int kSteps = HD / 32, kHalves = HD / 64, kTiles = HD / 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_rows = it.nq * sa.hpc;
+    const uint16_t *kp = reinterpret_cast<const uint16_t*>(p.k_pool), *vp = reinterpret_cast<const uint16_t*>(p.v_pool);
+    for (int r0 = 0; r0 < n_rows; r0 += 8) {
+        // columns of the products: rows r0 .. r0 + 7. As an operand a lane has row g, as a result rows 2t and 2t + 1
+        uint32_t q[kSteps][4];
+        {
+            const int r = min(r0 + g, n_rows - 1);
+            const float* src = p.q + (size_t)(it.tok0 + r / sa.hpc) * p.ldq + (size_t)(it.h0 + r % sa.hpc) * HD + 8 * t;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                float x[8];
+                if (sa.vec_q) {
+                    const float4 a = *reinterpret_cast<const float4*>(src + 32 * s), b = *reinterpret_cast<const float4*>(src + 32 * s + 4);
+                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = src[32 * s + e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[s][e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+            }
+        }
+        int pos[2];
+        float slope[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kTiles][4] = {};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 2 * t + i;
+            pos[i] = r < n_rows ? p.b.tok_pos[it.tok0 + r / sa.hpc] : -1;
+            slope[i] = p.slopes && r < n_rows ? p.slopes[it.h0 + r % sa.hpc] * kStLog2e : 0.0f;
+        }
+        // the keys that any of the rows sees: up to the last position, and from the oldest of a window
+        int last = max(pos[0], pos[1]), least = min(pos[0] < 0 ? INT_MAX : pos[0], pos[1] < 0 ? INT_MAX : pos[1]);
+#pragma unroll
+        for (int w = 1; w < 4; w *= 2) {
+            last = max(last, __shfl_xor_sync(0xffffffffu, last, w));
+            least = min(least, __shfl_xor_sync(0xffffffffu, least, w));
+        }
+        const int end = min(it.key1, last + 1), oldest = p.window > least ? 0 : least - p.window + 1;
+        for (int j0 = it.key0 / 16 * 16 + 16 * warp; j0 < end; j0 += 16 * kStWarps) {
+            if (j0 + 16 <= oldest && j0 >= p.keep_first) continue;
+            const int page = sh_page(p, it.slot, j0), in_page = j0 % p.b.page_len;            // (pages are a multiple of 32 positions)
+            if (page < 0) continue;
+            const uint16_t* kr = kp + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD) + 8 * t;
+            const uint16_t* vr = vp + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD) + 8 * g;
+            auto mine = [&](int key) { return key >= it.key0 && key < end; };
+            const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+            uint4 k[kSteps][2], v[kHalves][4];
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) k[s][i] = mine(j0 + g + 8 * i) ? ld_stream(kr + (g + 8 * i) * HD + 32 * s) : none;
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+                    v[h][i] = mine(j0 + key) ? ld_stream(vr + key * HD + 64 * h) : none;
+                }
+            float s[4] = {};                 // (key g, rows 2t and 2t + 1), (key g + 8, the same)
+#pragma unroll
+            for (int e = 0; e < kSteps; ++e) {
+                const uint32_t a0[4] = {k[e][0].x, k[e][1].x, k[e][0].y, k[e][1].y}, a1[4] = {k[e][0].z, k[e][1].z, k[e][0].w, k[e][1].w};
+                mma_bf16_16816(s, a0, q[e][0], q[e][1]);
+                mma_bf16_16816(s, a1, q[e][2], q[e][3]);
+            }
+            bool sees[4];
+            float top[2] = {m[0], m[1]};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = j0 + g + 8 * (i >> 1), row = i & 1;
+                sees[i] = mine(key) && seq_sees(pos[row], key, p.window, p.keep_first);
+                float x = s[i] * p.scale;
+                if (p.softcap > 0.0f) x = p.softcap * tc_tanh(x / p.softcap);
+                s[i] = sees[i] ? fmaf(-slope[row], (float)(pos[row] - key), x * kStLog2e) : -INFINITY;
+                top[row] = fmaxf(top[row], s[i]);
+            }
+#pragma unroll
+            for (int w = 4; w < 32; w *= 2) {
+                top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], w));
+                top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
+            }
+            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+                const float f0 = top[0] == m[0] ? 1.0f : tc_exp2(m[0] - top[0]), f1 = top[1] == m[1] ? 1.0f : tc_exp2(m[1] - top[1]);
+                l[0] *= f0;
+                l[1] *= f1;
+#pragma unroll
+                for (int c = 0; c < kTiles; ++c) { o[c][0] *= f0; o[c][1] *= f1; o[c][2] *= f0; o[c][3] *= f1; }
+                m[0] = top[0];
+                m[1] = top[1];
+            }
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = s[i] == -INFINITY ? 0.0f : tc_exp2(s[i] - m[i & 1]);
+                l[i & 1] += w[i];
+            }
+            uint32_t b[3][2];
+            split3_bf16(w[0], w[1], b[0][0], b[1][0], b[2][0]);
+            split3_bf16(w[2], w[3], b[0][1], b[1][1], b[2][1]);
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) b[x][i] = st_turned(b[x][i]);
+            bool odd = false;                // a value that is no number: it goes by itself to the rows that see its key
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd |= st_odd(v[h][i]);
+            if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                for (int key = 0; key < 16; ++key) {
+                    if (!mine(j0 + key)) continue;
+                    const bool s0 = seq_sees(pos[0], j0 + key, p.window, p.keep_first), s1 = seq_sees(pos[1], j0 + key, p.window, p.keep_first);
+#pragma unroll
+                    for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {          // columns 64 (c / 4) + 8 g + 2 (c % 4) + i, rows 2t and 2t + 1
+                            const float x = seq_ld(vr + key * HD, 64 * (c / 4) + 2 * (c % 4) + i);
+                            if (fabsf(x) <= FLT_MAX) continue;
+                            if (s0) o[c][2 * i] += x;
+                            if (s1) o[c][2 * i + 1] += x;
+                        }
+                }
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[h][i] = st_without(v[h][i]);
+            }
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    auto word = [&](int i) { return e == 0 ? v[h][i].x : e == 1 ? v[h][i].y : e == 2 ? v[h][i].z : v[h][i].w; };
+                    const uint32_t a[4] = {__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(0), word(1), 0x7632), __byte_perm(word(2), word(3), 0x5410), __byte_perm(word(2), word(3), 0x7632)};
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) mma_bf16_16816(o[4 * h + e], a, b[x][0], b[x][1]);
+                }
+        }
+#pragma unroll
+        for (int w = 4; w < 32; w *= 2) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], w);
+            l[1] += __shfl_xor_sync(0xffffffffu, l[1], w);
+        }
+        // the warps' parts: [warp][row][columns], then references and sums
+        float *part = smem, *ref = part + kStWarps * 8 * HD, *sum = ref + kStWarps * 8;
+        __syncthreads();                     // the rows before these have been read
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<float2*>(part + (warp * 8 + 2 * t + i) * HD + 64 * (c / 4) + 8 * g + 2 * (c % 4)) = make_float2(o[c][i], o[c][2 + i]);
+        if (g == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                ref[warp * 8 + 2 * t + i] = m[i];
+                sum[warp * 8 + 2 * t + i] = l[i];
+            }
+        }
+        __syncthreads();
+        const int r = r0 + warp;             // a warp puts one row together
+        if (r < n_rows) {
+            float mx = -INFINITY, all = 0.0f, f[kStWarps];
+#pragma unroll
+            for (int w = 0; w < kStWarps; ++w) mx = fmaxf(mx, ref[w * 8 + warp]);
+#pragma unroll
+            for (int w = 0; w < kStWarps; ++w) {
+                const float y = sum[w * 8 + warp];
+                f[w] = ref[w * 8 + warp] == -INFINITY && y == 0.0f ? 0.0f : tc_exp2(ref[w * 8 + warp] - mx);
+                all = fmaf(f[w], y, all);
+            }
+            float* rec = sh_record(p, it.tok0 + r / sa.hpc, it.h0 + r % sa.hpc, it.which);
+            if (lane == 0) {
+                rec[0] = mx;
+                rec[1] = all;
+            }
+            if (4 * lane < HD) {
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kStWarps; ++w) {
+                    if (f[w] == 0.0f) continue;
+                    const float4 x = *reinterpret_cast<const float4*>(part + (w * 8 + warp) * HD + 4 * lane);
+                    y.x = fmaf(f[w], x.x, y.x); y.y = fmaf(f[w], x.y, y.y); y.z = fmaf(f[w], x.z, y.z); y.w = fmaf(f[w], x.w, y.w);
+                }
+                *reinterpret_cast<float4*>(rec + kShHead + 4 * lane) = y;
+            }
+        }
+    }
+}
+
+// ---- many rows: tcgen05 ----------------------------------------------------------------------------------------------------------------------------------------------------------------
+// The key tiles of a share that any row may see: those of the first positions that stay visible behind a window, then those from the oldest key in a window on.
+struct StTiles {
+    int first, n_keep, lo, n;
+    __device__ __forceinline__ StTiles(int key0, int key1, int oldest, int keep_first) {
+        first = key0 / kStKeys;
+        const int end = (key1 + kStKeys - 1) / kStKeys;
+        lo = min(max(first, oldest / kStKeys), max(end, first));
+        n_keep = max(0, min(lo, (keep_first + kStKeys - 1) / kStKeys) - first);
+        n = key1 > key0 ? n_keep + max(0, end - lo) : 0;
+    }
+    __device__ __forceinline__ int tile_of(int i) const { return i < n_keep ? first + i : lo + i - n_keep; }
+};
+
+template <int HD, bool kOpts>
+__device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const StArgs& sa, const StItem& it, uint8_t* smem) {
+    using Sh = StShape<HD>;
+    constexpr int ST = Sh::kStages;
+    const SharedArgs& p = sa.a;
+    uint8_t *sK = smem, *sV = sK + ST * Sh::kTile, *sQ = sV + ST * Sh::kTile;
+    uint64_t* kfull = reinterpret_cast<uint64_t*>(sQ + Sh::kQBytes);
+    uint64_t *kempty = kfull + ST, *vfull = kempty + ST, *vready = vfull + ST, *vempty = vready + ST, *qready = vempty + ST, *sfull = qready + 1, *pready = sfull + 1, *odone = pready + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odone + 1);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* extent = reinterpret_cast<int*>(tmem_slot + 2);         // the rows' least and largest position; whether values were taken out
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_rows = it.nq * sa.hpc;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; ++i) { mb_init(kfull + i, 1); mb_init(kempty + i, 1); mb_init(vfull + i, 1); mb_init(vready + i, 2); mb_init(vempty + i, 1); }
+        mb_init(qready, 128); mb_init(sfull, 1); mb_init(pready, 128); mb_init(odone, 1);
+        *gave_up = 0;
+        extent[0] = INT_MAX;
+        extent[1] = -1;
+        extent[2] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 5) tc_alloc(tmem_slot, kStTmem);
+    tc_fence_before();
+    __syncthreads();
+    if (warp < 4) {
+        const int pos = threadIdx.x < it.nq ? p.b.tok_pos[it.tok0 + threadIdx.x] : -1;       // (a tile has at most 128 tokens)
+        const int most = __reduce_max_sync(0xffffffffu, pos), least = __reduce_min_sync(0xffffffffu, pos < 0 ? INT_MAX : pos);
+        if (lane == 0) {
+            atomicMax(extent + 1, most);
+            atomicMin(extent, least);
+        }
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int least = extent[0], most = extent[1], key1 = min(it.key1, most + 1);
+    const StTiles tiles(it.key0, key1, p.window > least ? 0 : least - p.window + 1, p.keep_first);
+    const int n = tiles.n;
+    if (warp == 4) {
+        if (elect_one()) {   // ===== TMA producer =====
+            for (int i = 0; i < n; ++i) {
+                const int s = i % ST, j0 = tiles.tile_of(i) * kStKeys;
+                const uint32_t ph = (uint32_t)(i / ST) & 1;
+                int at[2], row[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int pos = j0 + x * kStBox, page = pos < key1 && pos + kStBox > it.key0 ? sh_page(p, it.slot, pos) : -1;
+                    at[x] = page >= 0 ? pos % p.b.page_len : p.b.page_len;                     // outside the map: zeros
+                    row[x] = page >= 0 ? page * p.kv_heads + it.g : 0;
+                }
+                if (!tc_wait(kempty + s, ph ^ 1, gave_up, sa.polls)) break;
+                mb_expect(kfull + s, Sh::kTile);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    for (int c = 0; c < Sh::kBlocks; ++c) tma_load_3d(sK + s * Sh::kTile + c * Sh::kKBlock + x * kStBox * 128, &tmK, 64 * c, at[x], row[x], kfull + s);
+                if (!tc_wait(vempty + s, ph ^ 1, gave_up, sa.polls)) break;
+                mb_expect(vfull + s, Sh::kTile);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    for (int c = 0; c < Sh::kBlocks; ++c) tma_load_3d(sV + s * Sh::kTile + c * Sh::kKBlock + x * kStBox * 128, &tmV, 64 * c, at[x], row[x], vfull + s);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        if (elect_one()) {   // ===== MMA issuer =====
+            constexpr uint32_t idesc_s = umma_idesc_bf16(kStRows, kStKeys), idesc_o = umma_idesc_bf16(kStRows, HD) | (1u << 16);      // B MN-major
+            const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, Sh::kKBlock);  // + bytes / 16: another place
+            auto scores = [&](int i) {
+                const uint64_t k = k_desc + (uint32_t)(i % ST) * (Sh::kTile / 16);
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks)
+                    tc_mma_bf16(tmem, q_desc + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kKBlock / 16) + 2 * (ks % 4)), idesc_s, ks != 0);
+                tc_commit(sfull);
+                tc_commit(kempty + i % ST);
+            };
+            bool ok = n > 0 && tc_wait(qready, 0, gave_up, sa.polls) && tc_wait(kfull, 0, gave_up, sa.polls);
+            if (ok) {
+                tc_fence_after();
+                scores(0);
+            }
+            for (int i = 0; ok && i < n; ++i) {
+                ok = tc_wait(vready + i % ST, (uint32_t)(i / ST) & 1, gave_up, sa.polls) && tc_wait(pready, (uint32_t)i & 1, gave_up, sa.polls);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t v = v_desc + (uint32_t)(i % ST) * (Sh::kTile / 16);
+#pragma unroll
+                for (int ks = 0; ks < 3 * kStKeys / 16; ++ks)                    // first terms, then second ones, then third ones, against the same values
+                    tc_mma_bf16_ts(tmem + 128, tmem + 8 * ks, v + (uint32_t)((ks % (kStKeys / 16)) * 128), idesc_o, (i % kStFlush | ks) != 0);
+                tc_commit(odone);
+                tc_commit(vempty + i % ST);
+                if (i + 1 < n) {        // the next scores land where the weights lie that this product is still reading
+                    ok = tc_wait(kfull + (i + 1) % ST, (uint32_t)((i + 1) / ST) & 1, gave_up, sa.polls) && tc_wait(odone, (uint32_t)i & 1, gave_up, sa.polls);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(i + 1);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 6) {   // ===== values that are not the share's, or no numbers =====
+        for (int i = 0; i < n; ++i) {
+            const int s = i % ST, j0 = tiles.tile_of(i) * kStKeys, from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
+            if (!tc_wait_warp(vfull + s, (uint32_t)(i / ST) & 1, gave_up, sa.polls)) break;
+            bool odd = false;
+#pragma unroll 8
+            for (int x = (warp - 6) * 32 + lane; x < kStKeys * 8 * Sh::kBlocks; x += 64) {      // (the rows of a block of 64 columns lie one behind the other)
+                const int r = x / 8 % kStKeys;
+                uint4* at = reinterpret_cast<uint4*>(sV + s * Sh::kTile + x * 16);
+                const uint4 v = *at;
+                if (r < from || r >= to) {
+                    *at = make_uint4(0u, 0u, 0u, 0u);
+                } else if (st_odd(v)) {
+                    *at = st_without(v);
+                    odd = true;
+                }
+            }
+            if (odd) extent[2] = 1;
+            if (from > 0 || to < kStKeys || __any_sync(0xffffffffu, odd)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mb_arrive(vready + s);
+        }
+    }
+    bool ok = true;
+    float ref = -INFINITY, l = 0.0f;         // what the weights are relative to; their sum
+    const int row = threadIdx.x, qi = min(row / sa.hpc, it.nq - 1), h = it.h0 + row % sa.hpc;
+    const bool live = row < n_rows;          // (of the first four warps)
+    float* place = sh_record(p, it.tok0 + qi, h, it.which) + kShHead;
+    if (warp < 4) {   // ===== softmax: row = warp * 32 + lane = token * hpc + head =====
+        const int qpos = live ? p.b.tok_pos[it.tok0 + qi] : -1;
+        {   // the warp's 32 rows, one row (or two) per load so that neighbouring lanes read neighbouring columns; sixteen loads on their way before the first of them is stored
+            constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 16;
+            const int col = (lane % kLanes) * 4;
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += kPer * kAhead) {
+                float4 x[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int r = warp * 32 + r0 + k * kPer + lane / kLanes;
+                    const float* src = p.q + (size_t)(it.tok0 + min(r / sa.hpc, it.nq - 1)) * p.ldq + (size_t)(it.h0 + r % sa.hpc) * HD + col;
+                    if (r >= n_rows) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    else if (sa.vec_q) x[k] = *reinterpret_cast<const float4*>(src);
+                    else x[k] = make_float4(src[0], src[1], src[2], src[3]);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int r = warp * 32 + r0 + k * kPer + lane / kLanes;
+                    *reinterpret_cast<uint2*>(sQ + (col / 64) * Sh::kQBlock + r * 128 + ((((col % 64) / 8) ^ (r & 7)) << 4) + (col % 8) * 2) =
+                        make_uint2(tc_pack(x[k].x, x[k].y), tc_pack(x[k].z, x[k].w));
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mb_arrive(qready);
+        }
+        const uint32_t s_tmem = tmem + ((uint32_t)(warp * 32) << 16), o_tmem = s_tmem + 128;
+        const float slope = kOpts && p.slopes && live ? p.slopes[h] : 0.0f;
+        const bool plain = !kOpts;           // weights are 2^(score * mul - ref): one rounding between a score and its exponential. Without caps or charges mul holds the scale, too
+        const float mul = plain ? p.scale * kStLog2e : kStLog2e;
+        float flushed = -INFINITY;           // the reference of what has been flushed
+        auto store_flushed = [&](const uint32_t* o, int c) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(place + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        };
+        auto add_flushed = [&](uint32_t* o, int c) {        // carried over to the present reference
+            const float f = flushed == ref ? 1.0f : tc_exp2(flushed - ref);
+            float4 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const float4*>(place + c + 4 * e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[4 * e] = __float_as_uint(fmaf(w[e].x, f, __uint_as_float(o[4 * e])));
+                o[4 * e + 1] = __float_as_uint(fmaf(w[e].y, f, __uint_as_float(o[4 * e + 1])));
+                o[4 * e + 2] = __float_as_uint(fmaf(w[e].z, f, __uint_as_float(o[4 * e + 2])));
+                o[4 * e + 3] = __float_as_uint(fmaf(w[e].w, f, __uint_as_float(o[4 * e + 3])));
+            }
+        };
+        for (int i = 0; i < n; ++i) {
+            const int j0 = tiles.tile_of(i) * kStKeys;
+            // keys of the tile that are in the share and in a page
+            const int from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
+            uint64_t have = (to >= 64 ? ~0ull : (1ull << to) - 1) & ~((1ull << from) - 1);
+            if (sh_page(p, it.slot, j0) < 0) have &= ~0xffffffffull;
+            if (to > kStBox && sh_page(p, it.slot, j0 + kStBox) < 0) have &= 0xffffffffull;
+            ok = tc_wait_warp(sfull, (uint32_t)i & 1, gave_up, sa.polls);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[64];
+            tc_ld32_async(s_tmem, s);
+            tc_ld32_async(s_tmem + 32, s + 32);
+            tc_arrived(s);
+            tc_arrived(s + 32);
+            // every key of the tile is visible to every row of the warp
+            const bool all = have == ~0ull && __all_sync(0xffffffffu, !live || (j0 + kStKeys - 1 <= qpos && (qpos - j0 < p.window || j0 + kStKeys <= p.keep_first)));
+            if (kOpts && p.softcap > 0.0f) {
+                const float inv = p.scale / p.softcap;
+                const uint64_t inv2 = tc_two(__float_as_uint(inv), __float_as_uint(inv));
+                float top0 = 0.0f, top1 = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 64; e += 2) {
+                    float x, y;
+                    tc_split(tc_mul2(tc_two(s[e], s[e + 1]), inv2), x, y);
+                    s[e] = __float_as_uint(x);
+                    s[e + 1] = __float_as_uint(y);
+                    if (e & 2) top1 = tc_max3(top1, fabsf(x), fabsf(y));
+                    else top0 = tc_max3(top0, fabsf(x), fabsf(y));
+                }
+                // scores within a quarter of the cap, as nearly all are: the series that tc_tanh takes for them, two at a time
+                if (__any_sync(0xffffffffu, fmaxf(top0, top1) >= 0.25f)) {
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(p.softcap * tc_tanh(__uint_as_float(s[e])));
+                } else {
+                    auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
+                    const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), c0 = both(1.0f), cap2 = both(p.softcap);
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) {
+                        const uint64_t x = tc_two(s[e], s[e + 1]), x2 = tc_mul2(x, x);
+                        float a, c;
+                        tc_split(tc_mul2(cap2, tc_mul2(x, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, c4, c3), c2), c1), c0))), a, c);
+                        s[e] = __float_as_uint(a);
+                        s[e + 1] = __float_as_uint(c);
+                    }
+                }
+            } else if (!plain) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * p.scale);
+            }
+            if (kOpts && p.slopes) {
+                const float d0 = (float)(qpos - j0);
+#pragma unroll
+                for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(fmaf(-slope, d0 - (float)e, __uint_as_float(s[e])));
+            }
+            if (!all) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e)
+                    if (!(have >> e & 1) || !seq_sees(qpos, j0 + e, p.window, p.keep_first)) s[e] = 0xff800000u;       // -inf
+            }
+            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) m[(e / 2) & 3] = tc_max3(m[(e / 2) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            const float mx = tc_max3(fmaxf(m[0], m[1]), m[2], m[3]) * mul;
+            if (i % kStFlush == 0 && i > 0) {           // the product before this tile has completed: these scores follow it
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 16) {
+                    uint32_t o[16];
+                    st_ld16(o_tmem + c, o);
+                    if (live) {
+                        if (i > kStFlush) add_flushed(o, c);
+                        store_flushed(o, c);
+                    }
+                    __syncwarp();
+                }
+                flushed = ref;
+            }
+            if (i == 0) {
+                ref = mx;
+            } else if (__any_sync(0xffffffffu, mx > ref + 8.0f)) {
+                const float nr = fmaxf(ref, mx), f = nr == ref ? 1.0f : tc_exp2(ref - nr);
+                l *= f;
+                ref = nr;
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 16) {
+                    uint32_t o[16];
+                    st_ld16(o_tmem + c, o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tc_st16(o_tmem + c, o);
+                }
+            }
+            uint64_t sum = 0;                                                   // (0, 0)
+            const float base = ref == -INFINITY ? 0.0f : ref;                   // nothing seen yet: every weight is exp(-inf) = 0
+            const uint64_t mul2 = tc_two(__float_as_uint(mul), __float_as_uint(mul)), base2 = tc_two(__float_as_uint(-base), __float_as_uint(-base));
+            const uint64_t less = tc_two(__float_as_uint(-1.0f), __float_as_uint(-1.0f));
+            auto terms = [](uint32_t w) { return tc_two(w << 16, w & 0xffff0000u); };
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t hi[16], mid[16], lo[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float x, y;
+                    tc_split(tc_fma2(tc_two(s[half * 32 + 2 * e], s[half * 32 + 2 * e + 1]), mul2, base2), x, y);
+                    x = tc_exp2(x);
+                    y = tc_exp2(y);
+                    const uint64_t w = tc_two(__float_as_uint(x), __float_as_uint(y));
+                    sum = tc_add2(sum, w);
+                    hi[e] = tc_pack(x, y);
+                    const uint64_t r = tc_fma2(terms(hi[e]), less, w);          // what the first terms leave: exact
+                    tc_split(r, x, y);
+                    mid[e] = tc_pack(x, y);
+                    tc_split(tc_fma2(terms(mid[e]), less, r), x, y);
+                    lo[e] = tc_pack(x, y);
+                }
+                tc_st16(s_tmem + half * 16, hi);
+                tc_st16(s_tmem + 32 + half * 16, mid);
+                tc_st16(s_tmem + 64 + half * 16, lo);
+            }
+            float l0, l1;
+            tc_split(sum, l0, l1);
+            l += l0 + l1;
+            tc_wait_st();
+            tc_fence_before();
+            mb_arrive(pready);
+        }
+        if (ok && n > 0) ok = tc_wait_warp(odone, (uint32_t)(n - 1) & 1, gave_up, sa.polls);
+        tc_fence_after();
+        if (ok && live) {
+            place[-kShHead] = ref;
+            place[1 - kShHead] = l;
+        }
+        float* mine = reinterpret_cast<float*>(smem) + warp * (32 * 33);        // the rings' place: every tile has been read
+        const int rows = min(32, n_rows - warp * 32);
+#pragma unroll 1
+        for (int c = 0; ok && c < HD; c += 32) {
+            uint32_t o[32];
+            if (n > 0) {
+                tc_ld32_async(o_tmem + c, o);
+                tc_arrived(o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+            if (n > kStFlush && live) {
+                add_flushed(o, c);
+                add_flushed(o + 16, c + 16);
+            }
+            __syncwarp();        // through shared memory, so that a store covers neighbouring columns of one row
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mine[lane * 33 + e] = __uint_as_float(o[e]);
+            __syncwarp();
+#pragma unroll 1
+            for (int r0 = 0; r0 < rows; r0 += 16) {
+                float x[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[k] = mine[(r0 + k) * 33 + lane];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int rr = warp * 32 + r0 + k;
+                    if (r0 + k < rows) sh_record(p, it.tok0 + rr / sa.hpc, it.h0 + rr % sa.hpc, it.which)[kShHead + c + lane] = x[k];
+                }
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*gave_up) tc_gave_up(sa.status);
+    if (extent[2] && warp < 4 && live) {     // infinities and NaN that were taken out of the values: back to the rows that see them (columns of this row alone, written behind the barrier)
+        const int qpos = p.b.tok_pos[it.tok0 + qi];
+        for (int i = 0; i < n; ++i) {
+            const int j0 = tiles.tile_of(i) * kStKeys;
+            for (int key = max(j0, it.key0); key < min(j0 + kStKeys, key1); ++key) {
+                const int page = sh_page(p, it.slot, key);
+                if (page < 0 || !seq_sees(qpos, key, p.window, p.keep_first)) continue;
+                const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v_pool) + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, key % p.b.page_len, HD);
+                for (int c = 0; c < HD; ++c) {
+                    const float x = seq_ld(v, c);
+                    if (!(fabsf(x) <= FLT_MAX)) place[c] += x;
+                }
+            }
+        }
+    }
+    if (warp == 5) {
+        tc_fence_after();
+        tc_dealloc(tmem, kStTmem);
+    }
+}
+
+template <int HD, bool kOpts>
+__global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const StArgs sa) {
+    after_previous();        // in front of the allocation of TMEM: a CTA that waits for another kernel must not hold what that kernel's CTAs may be waiting for
+    extern __shared__ uint8_t st_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(st_raw) + 1023) & ~(uintptr_t)1023);
+    const SharedArgs& p = sa.a;
+    const int all_sets = p.kv_heads * sa.sets;
+    StItem it;
+    int x = (int)blockIdx.x;
+    if (x < sa.group_tiles * all_sets * p.shares) {      // the group tiles, tiles of one share and head set beside each other
+        int tile = x % sa.group_tiles, first, n;
+        x /= sa.group_tiles;
+        const int z = x % p.shares, set = x / p.shares;
+        const int i = sh_find_group(p, sa.queries, tile, first, n);
+        if (i < 0) return;
+        const int len = max(0, p.group_len[i]), tiles = (len + kStKeys - 1) / kStKeys, cuts = sh_cuts(len, kShLeast, p.shares);
+        if (z >= cuts) return;
+        it.tok0 = first + tile * sa.queries;
+        it.nq = min(sa.queries, n - tile * sa.queries);
+        it.slot = p.b.seg_slot[p.group_start[i]];
+        it.g = set / sa.sets;
+        it.h0 = it.g * (p.heads / p.kv_heads) + set % sa.sets * sa.hpc;
+        it.key0 = tiles * z / cuts * kStKeys;
+        it.key1 = min(len, tiles * (z + 1) / cuts * kStKeys);
+        it.which = z;
+    } else {
+        x -= sa.group_tiles * all_sets * p.shares;
+        const int tile = x % p.b.n_qtiles;
+        x /= p.b.n_qtiles;
+        const int z = x % p.own, sub = x / p.own % sa.subs, set = x / p.own / sa.subs;
+        const int seg = p.b.qt_seg[tile], off = p.b.qt_off[tile], n = min(kBQ, p.b.seg_len[seg] - off);
+        if (sub * sa.queries >= n) return;
+        const int all = p.b.seg_pos0[seg] + off + n, from = min(sh_shared_len(p, seg), all), cuts = sh_cuts(all - from, kShOwnLeast, p.own);
+        if (z >= cuts) return;
+        const int t0 = from / kStKeys, tiles = (all + kStKeys - 1) / kStKeys - t0;
+        it.tok0 = p.b.seg_start[seg] + off + sub * sa.queries;
+        it.nq = min(sa.queries, n - sub * sa.queries);
+        it.slot = p.b.seg_slot[seg];
+        it.g = set / sa.sets;
+        it.h0 = it.g * (p.heads / p.kv_heads) + set % sa.sets * sa.hpc;
+        it.key0 = max(from, (t0 + tiles * z / cuts) * kStKeys);
+        it.key1 = min(all, (t0 + tiles * (z + 1) / cuts) * kStKeys);
+        it.which = p.shares + z;
+        if (it.nq * sa.hpc <= kStFew) {
+            st_few<HD>(sa, it, reinterpret_cast<float*>(smem));
+            return;
+        }
+    }
+    st_many<HD, kOpts>(tmK, tmV, sa, it, smem);
+}
+
+template <int HD, bool kOpts>
+static int st_launch(const SharedArgs& p, cudaStream_t st) {
+    using Sh = StShape<HD>;
+    static_assert(Sh::kSmem - 1024 >= kStWarps * 8 * (HD + 2) * 4, "the warps' parts");
+    auto* kernel = seq_attention_shared_tc_kernel<HD, kOpts>;
+    static OncePerDevice ready;
+    if (int rc = ready([&] {
+            SLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+            return SLLM_OK;
+        }))
+        return rc;
+    StArgs a{};
+    a.a = p;
+    const int per = p.heads / p.kv_heads;
+    for (a.hpc = std::min(per, 16); per % a.hpc; --a.hpc) {}
+    a.sets = per / a.hpc;
+    a.queries = kStRows / a.hpc;
+    a.subs = p.b.T == p.b.nseg ? 1 : (kBQ + a.queries - 1) / a.queries;
+    a.group_tiles = (p.b.T + a.queries - 1) / a.queries + p.n_groups;
+    if (int rc = status_word(&a.status)) return rc;
+    a.polls = (unsigned)g_tune_tc_polls;
+    a.vec_q = p.ldq % 4 == 0 && ((uintptr_t)p.q % 16) == 0;
+    CUtensorMap tmK, tmV;
+    const cuuint64_t dims[3] = {HD, (cuuint64_t)p.b.page_len, (cuuint64_t)p.n_pages * p.kv_heads};
+    const cuuint64_t strides[2] = {HD * 2, (cuuint64_t)p.b.page_len * HD * 2};
+    const cuuint32_t box[3] = {64, kStBox, 1};
+    if (int rc = tc_encode_bf16(&tmK, p.k_pool, 3, dims, strides, box)) return rc;
+    if (int rc = tc_encode_bf16(&tmV, p.v_pool, 3, dims, strides, box)) return rc;
+    const long long all_sets = (long long)p.kv_heads * a.sets, grid = all_sets * ((long long)a.group_tiles * p.shares + (long long)p.b.n_qtiles * p.own * a.subs);
+    SLLM_REQUIRE(grid <= 0x7fffffffLL, SLLM_ENOTSUP, "seq_attention_shared: too many tokens or heads");
+    overlapping(kernel)<<<(unsigned)grid, kStThreads, Sh::kSmem, st>>>(tmK, tmV, a);
+    ++g_launches;
+    SLLM_LAUNCH_CHECK_ONLY();
+    return SLLM_OK;
+}
+
+int launch_attention_shared_tc(const SharedArgs& p, cudaStream_t st) {
+    const bool opts = p.softcap > 0.0f || p.slopes;
+    if (p.dk == 128) return opts ? st_launch<128, true>(p, st) : st_launch<128, false>(p, st);
+    return opts ? st_launch<64, true>(p, st) : st_launch<64, false>(p, st);
+}
+
+}  // namespace sllm

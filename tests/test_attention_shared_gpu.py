@@ -237,3 +237,19 @@ def test_captured_with_lengths_that_grow():
     g.replay()
     torch.cuda.synchronize()
     _close(out.cpu(), late.want())
+
+
+def test_waits_that_run_out_are_reported():
+    """With no polls allowed the tensor-core kernel gives up its first waits; the library's next call says so, once, and later launches are whole again."""
+    from simplellminference_b200 import _lib
+    lib = _lib.load()
+    s = SharedStep([(300, _owns(6, 90)), (20, [(0, 40)])], 8, 2, 128)
+    assert lib.sllm_status() == 0
+    assert lib.sllm_tune(10, 0) == 0
+    try:
+        with pytest.raises(_lib.SllmError) as e:
+            s.run()
+    finally:
+        assert lib.sllm_tune(10, 1 << 24) == 0
+    assert e.value.code == _lib.ETIMEOUT and lib.sllm_status() == 0
+    _close(s.run()[0], s.want())
