@@ -36,6 +36,16 @@ __device__ __forceinline__ bool seq_sees(int qpos, int key, int window, int keep
     return key <= qpos && (qpos - key < window || key < keep_first);
 }
 
+// page of a position and its row there: the product with the rounded-up reciprocal is at most one too large
+__device__ __forceinline__ int page_of(int pos, int page_len, uint32_t magic, int& in_page) {
+    int page = (int)__umulhi((uint32_t)pos, magic);
+    in_page = pos - page * page_len;
+    if (in_page < 0) {
+        --page;
+        in_page += page_len;
+    }
+    return page;
+}
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

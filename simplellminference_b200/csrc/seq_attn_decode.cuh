@@ -41,17 +41,6 @@ __device__ __forceinline__ float seq_score(float dot, float scale, float softcap
     return sc;
 }
 
-// page of a position and its row there: the product with the rounded-up reciprocal is at most one too large
-__device__ __forceinline__ int page_of(int pos, int page_len, uint32_t magic, int& in_page) {
-    int page = (int)__umulhi((uint32_t)pos, magic);
-    in_page = pos - page * page_len;
-    if (in_page < 0) {
-        --page;
-        in_page += page_len;
-    }
-    return page;
-}
-
 // 16 bytes of a cache row as pairs of floats
 __device__ __forceinline__ void cache_pairs(const uint4& u, uint64_t (&p)[2]) {
     p[0] = pair_f32(u.x, u.y);

@@ -48,7 +48,8 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
             for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] = 0.0f;
         }
         for (int j0 = sp.key0 / kShKeys * kShKeys; j0 < sp.key1; j0 += kShKeys) {
-            const int page = sh_page(p, sp.slot, j0), in_page = j0 % p.b.page_len;           // (pages are a multiple of 32 positions)
+            int in_page;
+            const int page = sh_page(p, sp.slot, j0, in_page);           // (pages are a multiple of 32 positions)
             // hidden from every row of the CTA: before its window, or no page
             int seen = 0;
 #pragma unroll
@@ -90,7 +91,7 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
                 sees[i] = __ballot_sync(0xffffffffu, here);
                 const float x = here ? sh_score(s[i] * p.scale, p.softcap, slope[i], pos[i], key) : -INFINITY;
                 const float top = fmaxf(m[i], warp_max(x));
-                const float f = top == -INFINITY ? 1.0f : expf(m[i] - top), w = x == -INFINITY ? 0.0f : expf(x - top);
+                const float f = top == -INFINITY ? 1.0f : fmaxf(expf(m[i] - top), FLT_MIN), w = x == -INFINITY ? 0.0f : expf(x - top);
                 m[i] = top;
                 l[i] = l[i] * f + warp_sum(w);
 #pragma unroll
@@ -110,8 +111,9 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
 #pragma unroll
                     for (int i = 0; i < kRw; ++i) {
                         if (odd && !(sees[i] >> k & 1)) continue;
-                        o[i][c][0] = fmaf(w[i], v.x, o[i][c][0]); o[i][c][1] = fmaf(w[i], v.y, o[i][c][1]);
-                        o[i][c][2] = fmaf(w[i], v.z, o[i][c][2]); o[i][c][3] = fmaf(w[i], v.w, o[i][c][3]);
+                        const float x = odd ? fmaxf(w[i], FLT_MIN) : w[i];
+                        o[i][c][0] = fmaf(x, v.x, o[i][c][0]); o[i][c][1] = fmaf(x, v.y, o[i][c][1]);
+                        o[i][c][2] = fmaf(x, v.z, o[i][c][2]); o[i][c][3] = fmaf(x, v.w, o[i][c][3]);
                     }
                 }
             }
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
         int tile = blockIdx.x, first, n;
         const int i = sh_find_group(p, tokens, tile, first, n);
         if (i < 0) return;
-        const int len = max(0, p.group_len[i]), tiles = (len + kShKeys - 1) / kShKeys, cuts = sh_cuts(len, kShLeast, p.shares);
+        const int len = max(0, p.group_len[i]), tiles = (len + kShKeys - 1) / kShKeys, cuts = sh_cuts(len, p.least, p.shares);
         if (z >= cuts) return;
         sp.tok0 = first + tile * tokens;
         sp.n_rows = min(tokens, n - tile * tokens) * per;
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
         if (z >= p.own) return;
         const int x = blockIdx.x - group_tiles, seg = p.b.qt_seg[x], off = p.b.qt_off[x];
         const int n = min(kBQ, p.b.seg_len[seg] - off), end = p.b.seg_pos0[seg] + off + n, from = min(sh_shared_len(p, seg), end);
-        const int t0 = from / kShKeys, tiles = (end + kShKeys - 1) / kShKeys - t0, cuts = sh_cuts(end - from, kShOwnLeast, p.own);
+        const int t0 = from / kShKeys, tiles = (end + kShKeys - 1) / kShKeys - t0, cuts = sh_cuts(end - from, p.own_least, p.own);
         if (z >= cuts) return;
         sp.tok0 = p.b.seg_start[seg] + off;
         sp.n_rows = n * per;
@@ -177,18 +179,19 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
     after_previous();
     const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], n = min(kBQ, p.b.seg_len[seg] - off), lane = threadIdx.x & 31;
     const int shared = sh_shared_len(p, seg), end = p.b.seg_pos0[seg] + off + n;
-    const int first = sh_cuts(shared, kShLeast, p.shares), count = first + sh_cuts(end - min(shared, end), kShOwnLeast, p.own);
+    const int first = sh_cuts(shared, p.least ? p.least : *p.plan, p.shares), count = first + sh_cuts(end - min(shared, end), p.own_least, p.own);
     for (int i = blockIdx.y * 4 + (threadIdx.x >> 5); i < n * p.heads; i += gridDim.y * 4) {
         const int t = p.b.seg_start[seg] + off + i / p.heads, h = i % p.heads;
         float top = -INFINITY;
         for (int k = lane; k < count; k += 32) top = fmaxf(top, sh_record(p, t, h, k < first ? k : p.shares + k - first)[0]);
         top = warp_max(top);
         float sum = 0.0f, o[2][4] = {};
+#pragma unroll 4
         for (int k = 0; k < count; ++k) {
             const float* rec = sh_record(p, t, h, k < first ? k : p.shares + k - first);
             const float m = rec[0], l = rec[1];
-            if (m == -INFINITY && l == 0.0f) continue;                   // nothing seen (a weight of NaN goes on)
-            const float f = exp2f(m - top);
+            // nothing seen: nothing (a sum of NaN goes on); else never zero, so that an infinity stays one
+            const float f = m == -INFINITY && l == 0.0f ? 0.0f : fmaxf(exp2f(m - top), FLT_MIN);
             sum = fmaf(f, l, sum);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -258,7 +261,7 @@ int64_t sllm_seq_attention_shared_ws_bytes(const sllm_seq_batch* b, int32_t n_gr
                  "seq_attention_shared_ws_bytes: bad argument");
     int shares, own;
     shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &shares, &own);
-    return (int64_t)b->T * heads * (shares + own) * (dv + kShHead) * (int64_t)sizeof(float);
+    return (int64_t)b->T * heads * (shares + own) * (dv + kShHead) * (int64_t)sizeof(float) + kShPlan;
 }
 
 int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const int32_t* group_start, const int32_t* group_len, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads,
@@ -282,7 +285,9 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     SLLM_REQUIRE(!opts || (opts->window >= 0 && opts->keep_first >= 0 && opts->softcap >= 0.0f), SLLM_EINVAL, "seq_attention_shared: bad options");
     SLLM_REQUIRE(!opts || (!opts->values_in_keys && !opts->logdist && !opts->cross_values && !opts->chunk), SLLM_ENOTSUP,
                  "seq_attention_shared: values in keys, charges on the logarithm of the distance, values of every head and chunks are not part of this form");
-    SharedArgs p{*b, n_groups, group_start, group_len, q, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, INT_MAX, 0, 0.0f, nullptr, 0, 0, (float*)ws, out, ldo, (uint16_t*)out16};
+    SharedArgs p{*b, n_groups, group_start, group_len, q, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, INT_MAX, 0, 0.0f, nullptr, 0, 0,
+                 (uint32_t)(((1ull << 32) + b->page_len - 1) / b->page_len), 0, 0, (int*)ws,
+                 (float*)((char*)ws + kShPlan), out, ldo, (uint16_t*)out16};
     if (opts) {
         if (opts->window > 0) {
             p.window = opts->window;
@@ -294,10 +299,10 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &p.shares, &p.own);
     if (int rc = status_check()) return rc;
     cudaStream_t st = as_stream(stream);
-    int rc;
-    if (kv_dtype == SLLM_F32) rc = sh_launch<float, 4>(p, st);
-    else if (dk == dv && (dk == 64 || dk == 128)) rc = launch_attention_shared_tc(p, st);
-    else rc = sh_launch<uint16_t, 4>(p, st);
+    const bool tc = kv_dtype == SLLM_BF16 && dk == dv && (dk == 64 || dk == 128);
+    p.least = tc ? 0 : 64;
+    p.own_least = tc ? 512 : 64;
+    const int rc = tc ? launch_attention_shared_tc(p, st) : kv_dtype == SLLM_F32 ? sh_launch<float, 4>(p, st) : sh_launch<uint16_t, 4>(p, st);
     return rc ? rc : sh_merge(p, st);
 }
 

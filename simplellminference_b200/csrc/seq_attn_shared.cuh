@@ -21,7 +21,10 @@ struct SharedArgs {
     int n_pages, window, keep_first;
     float softcap;
     const float* slopes;
-    int shares, own;                     // records of a (token, head): of the shared positions, of its own
+    int shares, own;                     // records of a (token, head) at most: of the shared positions, of its own
+    uint32_t page_magic;                 // ceil(2^32 / page_len): the page of a position without a division (page_of)
+    int least, own_least;                // keys of a share at least; least 0: as the plan at the workspace's beginning has it
+    int* plan;
     float* ws;
     float* out;
     int ldo;
@@ -31,15 +34,16 @@ struct SharedArgs {
 // What a CTA leaves of the keys it has seen, for a (token, head): the reference of the weights as a power of two, their sum, and the weighted sum of the values. Records lie
 // [token][head][shares + own][dv + 4].
 constexpr int kShHead = 4;               // floats in front of the values (16 bytes, so that these are aligned)
+constexpr int kShPlan = 64;              // bytes in front of the records: the plan, one number
 
 #ifdef __CUDACC__
 
 __device__ __forceinline__ float* sh_record(const SharedArgs& p, int t, int h, int which) {
     return p.ws + (((size_t)t * p.heads + h) * (p.shares + p.own) + which) * (p.dv + kShHead);
 }
-// the page of a position, -1 where the table has none that exists
-__device__ __forceinline__ int sh_page(const SharedArgs& p, int slot, int pos) {
-    const int at = pos / p.b.page_len;
+// the page of a position (-1 where the table has none that exists) and the position's place in it
+__device__ __forceinline__ int sh_page(const SharedArgs& p, int slot, int pos, int& in_page) {
+    const int at = page_of(pos, p.b.page_len, p.page_magic, in_page);
     if (slot < 0 || at >= p.b.max_pages) return -1;
     const int page = p.b.block_table[(size_t)slot * p.b.max_pages + at];
     return page >= 0 && page < p.n_pages ? page : -1;
@@ -86,7 +90,6 @@ __device__ __forceinline__ int sh_find_group(const SharedArgs& p, int tokens, in
 }
 // How many of the step's shares a range of keys is cut into: none smaller than `least` keys.
 __device__ __forceinline__ int sh_cuts(int keys, int least, int most) { return keys <= 0 ? 0 : min(most, (keys + least - 1) / least); }
-constexpr int kShLeast = 256, kShOwnLeast = 512;         // of the shared positions; of a segment's own
 
 // a score after its scale: capped, charged for its distance
 __device__ __forceinline__ float sh_score(float s, float softcap, float slope, int pos, int key) {

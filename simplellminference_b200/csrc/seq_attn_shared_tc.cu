@@ -9,8 +9,8 @@
 //   warp 5     (one lane) MMA issuer: S = Q K^T, O += (hi + mid + lo) V with the weights read from TMEM, V as it lies;
 //   warps 6-7  zero the value rows that are not part of the share, and take infinities and NaN out of the values (0 * NaN is NaN for rows that do not see them, and the terms of a weight times
 //              infinity are NaN for those that do); rows that see them get them back at the end.
-// Where a segment has few rows of its own (a decoding request: the query heads of one token), eight warps take 16 keys in turn on mma.sync, 8 rows at a time as the columns: such a CTA is bound by what
-// it reads, and a tile of 128 rows would be empty but for four. Keys and values go from the pool to registers as the products take them, 16 bytes a load: the columns of a head are contracted in
+// Where a segment has few rows of its own (a decoding request: the query heads of one token), four warps take 16 keys in turn on mma.sync, 8 rows at a time as the columns: such work is bound by what
+// it reads, and a tile of 128 rows would be empty but for four. A CTA does two items at once, since one is a chain (queries, pages, keys and values, maximum, sums, four parts put together). Keys and values go from the pool to registers as the products take them, 16 bytes a load: the columns of a head are contracted in
 // an order of the kernel's own, and those of the values are dealt to the tiles of O so that a lane's eight neighbours are rows of four of them.
 #include <cfloat>
 
@@ -22,21 +22,29 @@ namespace sllm {
 constexpr int kStRows = 128, kStKeys = 64, kStThreads = 256, kStBox = 32, kStWarps = kStThreads / 32;
 constexpr int kStFlush = 12;
 constexpr uint32_t kStTmem = 256;            // scores at 0 .. 63, then the weights' terms at 0 .. 95, O at 128; two CTAs share an SM's 512 columns
-constexpr int kStFew = 16;                   // rows of a segment up to which its own positions are the eight warps' work
+constexpr int kStFew = 16, kStTeam = 4;      // rows of a segment up to which its own positions are a team's work; warps of a team, of which a CTA has two
 constexpr float kStLog2e = 1.4426950408889634f;
 
 template <int HD>
 struct StShape {
     static constexpr int kBlocks = HD / 64, kQBlock = kStRows * 128, kQBytes = kBlocks * kQBlock, kKBlock = kStKeys * 128, kTile = kBlocks * kKBlock;
     static constexpr int kStages = HD == 128 ? 2 : 4;
-    static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTile + 512;
+    static constexpr int kBars = kQBytes + 2 * kStages * kTile, kPlan = kBars + 512, kSmem = 1024 + kPlan + 10 * 1024;
 };
+
+// The step's work as a CTA sees it: entries (groups, then listed tiles of queries), as many at a time as it has threads, and how many items each and those before it are.
+constexpr int kStEntries = kStThreads;
+struct StPlan {
+    int tok0[kStEntries], n[kStEntries], slot[kStEntries], from[kStEntries], end[kStEntries], cuts[kStEntries], tiles[kStEntries], upto[kStEntries];
+    int warp[kStWarps];
+    int least, total;
+};
+static_assert(sizeof(StPlan) <= 10 * 1024, "its place");
 
 struct StArgs {
     SharedArgs a;
     int hpc, sets, queries;                  // query heads of a tile, tiles' head sets of a kv head, tokens of a tile
-    int subs;                                // tiles that a listed tile of queries may need
-    int group_tiles;                         // row tiles of the groups at most
+    uint32_t hpc_magic;                      // ceil(2^16 / hpc): row / hpc is (row * hpc_magic) >> 16 for the rows of a tile
     int vec_q;
     int32_t* status;
     unsigned polls;
@@ -45,8 +53,12 @@ struct StArgs {
 // What a CTA does.
 struct StItem {
     int tok0, nq, slot, g, h0;               // rows: nq tokens from tok0 on x hpc heads from h0 on, of kv head g
+    int pos0;                                // position of the first token where the others follow it, -1: their positions are looked up
     int key0, key1, which;                   // keys, and the record that takes the result
 };
+
+__device__ __forceinline__ int st_token(const StArgs& sa, int row) { return (int)((uint32_t)row * sa.hpc_magic >> 16); }
+__device__ __forceinline__ int st_pos(const StArgs& sa, const StItem& it, int token) { return it.pos0 >= 0 ? it.pos0 + token : sa.a.b.tok_pos[it.tok0 + token]; }
 
 __device__ __forceinline__ void st_ld16(uint32_t taddr, uint32_t* o) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -58,17 +70,21 @@ __device__ __forceinline__ void st_ld16(uint32_t taddr, uint32_t* o) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) asm volatile("" : "+r"(o[e]));
 }
-// whether one of the eight bf16 values is infinite or NaN
-__device__ __forceinline__ bool st_odd(const uint4& v) {
-    auto two = [](uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u; };
-    return two(v.x) || two(v.y) || two(v.z) || two(v.w);
+// Two bf16 values times zero, added up: zero as long as all were numbers, NaN where one was infinite or NaN.
+__device__ __forceinline__ void st_times_zero(uint32_t& sum, uint32_t x) { asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u)); }
+__device__ __forceinline__ void st_times_zero(uint32_t& sum, const uint4& v) {
+    st_times_zero(sum, v.x);
+    st_times_zero(sum, v.y);
+    st_times_zero(sum, v.z);
+    st_times_zero(sum, v.w);
 }
+__device__ __forceinline__ bool st_odd(uint32_t sum) { return (sum & 0x7fff7fffu) != 0; }
 __device__ __forceinline__ uint32_t st_without(uint32_t x) {            // the pair with those replaced by zero
     return ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u) | ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu);
 }
 __device__ __forceinline__ uint4 st_without(const uint4& v) { return make_uint4(st_without(v.x), st_without(v.y), st_without(v.z), st_without(v.w)); }
 
-// ---- few rows: eight warps -------------------------------------------------------------------------------------------------------------------------------------------------------------
+// ---- few rows: four warps -------------------------------------------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t st_turned(uint32_t x) {              // 8 x 8 values of 16 bits, transposed over the warp
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -79,35 +95,39 @@ template <int HD>
 __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
     const SharedArgs& p = sa.a;
     constexpr int kSteps = HD / 32, kHalves = HD / 64, kTiles = HD / 16;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_rows = it.nq * sa.hpc;
+    const int team = threadIdx.x / (32 * kStTeam), warp = threadIdx.x / 32 % kStTeam, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_rows = it.nq * sa.hpc;
+    auto together = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(3 + team) : "memory"); };
+    smem += team * (kStTeam * 8 * (HD + 2));
     const uint16_t *kp = reinterpret_cast<const uint16_t*>(p.k_pool), *vp = reinterpret_cast<const uint16_t*>(p.v_pool);
+    const int start = it.key0 / 16 * 16 + 16 * warp;
     for (int r0 = 0; r0 < n_rows; r0 += 8) {
+        int next_in = 0, next_page = start < it.key1 ? sh_page(p, it.slot, start, next_in) : -1;
         // columns of the products: rows r0 .. r0 + 7. As an operand a lane has row g, as a result rows 2t and 2t + 1
         uint32_t q[kSteps][4];
         {
             const int r = min(r0 + g, n_rows - 1);
-            const float* src = p.q + (size_t)(it.tok0 + r / sa.hpc) * p.ldq + (size_t)(it.h0 + r % sa.hpc) * HD + 8 * t;
+            const int qi = st_token(sa, r);
+            const float* src = p.q + (size_t)(it.tok0 + qi) * p.ldq + (size_t)(it.h0 + r - qi * sa.hpc) * HD + 8 * t;
+            if (sa.vec_q) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                float x[8];
-                if (sa.vec_q) {
+                for (int s = 0; s < kSteps; ++s) {
                     const float4 a = *reinterpret_cast<const float4*>(src + 32 * s), b = *reinterpret_cast<const float4*>(src + 32 * s + 4);
-                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = src[32 * s + e];
+                    q[s][0] = pack_bf16(a.x, a.y); q[s][1] = pack_bf16(a.z, a.w); q[s][2] = pack_bf16(b.x, b.y); q[s][3] = pack_bf16(b.z, b.w);
                 }
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) q[s][e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[s][e] = pack_bf16(src[32 * s + 2 * e], src[32 * s + 2 * e + 1]);
             }
         }
         int pos[2];
         float slope[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kTiles][4] = {};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 2 * t + i;
-            pos[i] = r < n_rows ? p.b.tok_pos[it.tok0 + r / sa.hpc] : -1;
-            slope[i] = p.slopes && r < n_rows ? p.slopes[it.h0 + r % sa.hpc] * kStLog2e : 0.0f;
+            const int r = r0 + 2 * t + i, qi = st_token(sa, r);
+            pos[i] = r < n_rows ? st_pos(sa, it, qi) : -1;
+            slope[i] = p.slopes && r < n_rows ? p.slopes[it.h0 + r - qi * sa.hpc] * kStLog2e : 0.0f;
         }
         // the keys that any of the rows sees: up to the last position, and from the oldest of a window
         int last = max(pos[0], pos[1]), least = min(pos[0] < 0 ? INT_MAX : pos[0], pos[1] < 0 ? INT_MAX : pos[1]);
@@ -117,26 +137,24 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
             least = min(least, __shfl_xor_sync(0xffffffffu, least, w));
         }
         const int end = min(it.key1, last + 1), oldest = p.window > least ? 0 : least - p.window + 1;
-        for (int j0 = it.key0 / 16 * 16 + 16 * warp; j0 < end; j0 += 16 * kStWarps) {
-            if (j0 + 16 <= oldest && j0 >= p.keep_first) continue;
-            const int page = sh_page(p, it.slot, j0), in_page = j0 % p.b.page_len;            // (pages are a multiple of 32 positions)
-            if (page < 0) continue;
+        for (int j0 = start; j0 < end; j0 += 16 * kStTeam) {
+            const int page = next_page, in_page = next_in;                                    // (pages are a multiple of 32 positions)
+            if (j0 + 16 * kStTeam < end) next_page = sh_page(p, it.slot, j0 + 16 * kStTeam, next_in);
+            if (page < 0 || (j0 + 16 <= oldest && j0 >= p.keep_first)) continue;
             const uint16_t* kr = kp + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD) + 8 * t;
             const uint16_t* vr = vp + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD) + 8 * g;
             auto mine = [&](int key) { return key >= it.key0 && key < end; };
-            const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+            // All sixteen rows are the page's, so nothing is asked before they are loaded: a condition around a load made each wait for the one before (13000 clocks a tile). Scores of keys that are not
+            // the share's are replaced, their values taken out below.
             uint4 k[kSteps][2], v[kHalves][4];
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) k[s][i] = mine(j0 + g + 8 * i) ? ld_stream(kr + (g + 8 * i) * HD + 32 * s) : none;
+                for (int i = 0; i < 2; ++i) k[s][i] = ld_stream(kr + (g + 8 * i) * HD + 32 * s);
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-                    v[h][i] = mine(j0 + key) ? ld_stream(vr + key * HD + 64 * h) : none;
-                }
+                for (int i = 0; i < 4; ++i) v[h][i] = ld_stream(vr + (2 * t + (i & 1) + 8 * (i >> 1)) * HD + 64 * h);
             float s[4] = {};                 // (key g, rows 2t and 2t + 1), (key g + 8, the same)
 #pragma unroll
             for (int e = 0; e < kSteps; ++e) {
@@ -161,7 +179,8 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
                 top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
             }
             if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-                const float f0 = top[0] == m[0] ? 1.0f : tc_exp2(m[0] - top[0]), f1 = top[1] == m[1] ? 1.0f : tc_exp2(m[1] - top[1]);
+                // (never zero: an infinity that has come in stays one)
+                const float f0 = top[0] == m[0] ? 1.0f : fmaxf(tc_exp2(m[0] - top[0]), FLT_MIN), f1 = top[1] == m[1] ? 1.0f : fmaxf(tc_exp2(m[1] - top[1]), FLT_MIN);
                 l[0] *= f0;
                 l[1] *= f1;
 #pragma unroll
@@ -182,12 +201,22 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
             for (int x = 0; x < 3; ++x)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) b[x][i] = st_turned(b[x][i]);
-            bool odd = false;                // a value that is no number: it goes by itself to the rows that see its key
+            if (j0 < it.key0 || j0 + 16 > end) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = mine(j0 + 2 * t + (i & 1) + 8 * (i >> 1));
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) {
+                        v[h][i].x = in ? v[h][i].x : 0u; v[h][i].y = in ? v[h][i].y : 0u; v[h][i].z = in ? v[h][i].z : 0u; v[h][i].w = in ? v[h][i].w : 0u;
+                    }
+                }
+            }
+            uint32_t odd = 0;                // a value that is no number goes by itself to the rows that see its key
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) odd |= st_odd(v[h][i]);
-            if (__any_sync(0xffffffffu, odd)) {
+                for (int i = 0; i < 4; ++i) st_times_zero(odd, v[h][i]);
+            if (__any_sync(0xffffffffu, st_odd(odd))) {
 #pragma unroll 1
                 for (int key = 0; key < 16; ++key) {
                     if (!mine(j0 + key)) continue;
@@ -223,8 +252,8 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
             l[1] += __shfl_xor_sync(0xffffffffu, l[1], w);
         }
         // the warps' parts: [warp][row][columns], then references and sums
-        float *part = smem, *ref = part + kStWarps * 8 * HD, *sum = ref + kStWarps * 8;
-        __syncthreads();                     // the rows before these have been read
+        float *part = smem, *ref = part + kStTeam * 8 * HD, *sum = ref + kStTeam * 8;
+        if (r0 > 0) together();              // the rows before these have been read
 #pragma unroll
         for (int c = 0; c < kTiles; ++c)
 #pragma unroll
@@ -237,19 +266,19 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
                 sum[warp * 8 + 2 * t + i] = l[i];
             }
         }
-        __syncthreads();
-        const int r = r0 + warp;             // a warp puts one row together
-        if (r < n_rows) {
-            float mx = -INFINITY, all = 0.0f, f[kStWarps];
+        together();
+        for (int i = warp; i < min(8, n_rows - r0); i += kStTeam) {      // a warp puts a row together
+            float mx = -INFINITY, all = 0.0f, f[kStTeam];
 #pragma unroll
-            for (int w = 0; w < kStWarps; ++w) mx = fmaxf(mx, ref[w * 8 + warp]);
+            for (int w = 0; w < kStTeam; ++w) mx = fmaxf(mx, ref[w * 8 + i]);
 #pragma unroll
-            for (int w = 0; w < kStWarps; ++w) {
-                const float y = sum[w * 8 + warp];
-                f[w] = ref[w * 8 + warp] == -INFINITY && y == 0.0f ? 0.0f : tc_exp2(ref[w * 8 + warp] - mx);
+            for (int w = 0; w < kStTeam; ++w) {
+                const float y = sum[w * 8 + i];
+                f[w] = ref[w * 8 + i] == -INFINITY && y == 0.0f ? 0.0f : fmaxf(tc_exp2(ref[w * 8 + i] - mx), FLT_MIN);
                 all = fmaf(f[w], y, all);
             }
-            float* rec = sh_record(p, it.tok0 + r / sa.hpc, it.h0 + r % sa.hpc, it.which);
+            const int qi = st_token(sa, r0 + i);
+            float* rec = sh_record(p, it.tok0 + qi, it.h0 + r0 + i - qi * sa.hpc, it.which);
             if (lane == 0) {
                 rec[0] = mx;
                 rec[1] = all;
@@ -257,15 +286,31 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
             if (4 * lane < HD) {
                 float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kStWarps; ++w) {
-                    if (f[w] == 0.0f) continue;
-                    const float4 x = *reinterpret_cast<const float4*>(part + (w * 8 + warp) * HD + 4 * lane);
+                for (int w = 0; w < kStTeam; ++w) {      // (a part without keys is zeros)
+                    const float4 x = *reinterpret_cast<const float4*>(part + (w * 8 + i) * HD + 4 * lane);
                     y.x = fmaf(f[w], x.x, y.x); y.y = fmaf(f[w], x.y, y.y); y.z = fmaf(f[w], x.z, y.z); y.w = fmaf(f[w], x.w, y.w);
                 }
                 *reinterpret_cast<float4*>(rec + kShHead + 4 * lane) = y;
             }
         }
     }
+}
+
+// behind the barriers: the flag of a wait that was given up, then what an item needs beside it, then the TMEM address
+template <int HD>
+__device__ __forceinline__ int* st_gave_up(uint8_t* smem) { return reinterpret_cast<int*>(smem + StShape<HD>::kBars + 448); }
+
+// the barriers, in the order in which st_many has them
+template <int HD>
+__device__ __forceinline__ void st_barriers(uint8_t* smem) {
+    constexpr int ST = StShape<HD>::kStages;
+    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + StShape<HD>::kBars);
+    for (int i = 0; i < 4 * ST; ++i) mb_init(bar++, 1);          // keys full, keys empty, values full, values empty
+    for (int i = 0; i < ST; ++i) mb_init(bar++, 2);              // values ready
+    mb_init(bar++, 128);                                         // queries ready
+    mb_init(bar++, 1);                                           // scores full
+    mb_init(bar++, 128);                                         // weights ready
+    mb_init(bar, 1);                                             // O done
 }
 
 // ---- many rows: tcgen05 ----------------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -283,53 +328,80 @@ struct StTiles {
 };
 
 template <int HD, bool kOpts>
-__device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const StArgs& sa, const StItem& it, uint8_t* smem) {
+__device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const StArgs& sa, const StItem& it, uint8_t* smem, uint32_t tmem, uint32_t& done, uint32_t turn) {
     using Sh = StShape<HD>;
     constexpr int ST = Sh::kStages;
     const SharedArgs& p = sa.a;
     uint8_t *sK = smem, *sV = sK + ST * Sh::kTile, *sQ = sV + ST * Sh::kTile;
-    uint64_t* kfull = reinterpret_cast<uint64_t*>(sQ + Sh::kQBytes);
-    uint64_t *kempty = kfull + ST, *vfull = kempty + ST, *vready = vfull + ST, *vempty = vready + ST, *qready = vempty + ST, *sfull = qready + 1, *pready = sfull + 1, *odone = pready + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(odone + 1);
-    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* extent = reinterpret_cast<int*>(tmem_slot + 2);         // the rows' least and largest position; whether values were taken out
+    uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + Sh::kBars);
+    uint64_t *kempty = kfull + ST, *vfull = kempty + ST, *vempty = vfull + ST, *vready = vempty + ST, *qready = vready + ST, *sfull = qready + 1, *pready = sfull + 1, *odone = pready + 1;
+    volatile int* gave_up = st_gave_up<HD>(smem);
+    int* extent = st_gave_up<HD>(smem) + 1 + 3 * (turn & 1);     // the rows' least and largest position; whether values were taken out
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_rows = it.nq * sa.hpc;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < ST; ++i) { mb_init(kfull + i, 1); mb_init(kempty + i, 1); mb_init(vfull + i, 1); mb_init(vready + i, 2); mb_init(vempty + i, 1); }
-        mb_init(qready, 128); mb_init(sfull, 1); mb_init(pready, 128); mb_init(odone, 1);
-        *gave_up = 0;
-        extent[0] = INT_MAX;
-        extent[1] = -1;
-        extent[2] = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    const int row = threadIdx.x, qi = min(st_token(sa, row), it.nq - 1), h = it.h0 + min(row - st_token(sa, row) * sa.hpc, sa.hpc - 1);      // (of the first four warps)
+    const bool live = row < n_rows;
+    if (threadIdx.x == 0) {                  // the next item's
+        int* other = st_gave_up<HD>(smem) + 1 + 3 * (~turn & 1);
+        other[0] = INT_MAX;
+        other[1] = -1;
+        other[2] = 0;
     }
-    if (warp == 5) tc_alloc(tmem_slot, kStTmem);
-    tc_fence_before();
-    __syncthreads();
-    if (warp < 4) {
-        const int pos = threadIdx.x < it.nq ? p.b.tok_pos[it.tok0 + threadIdx.x] : -1;       // (a tile has at most 128 tokens)
-        const int most = __reduce_max_sync(0xffffffffu, pos), least = __reduce_min_sync(0xffffffffu, pos < 0 ? INT_MAX : pos);
+    if (warp >= 4) {                         // (a tile has at most 128 tokens)
+        const int i = threadIdx.x - 128, pos = i < it.nq ? st_pos(sa, it, i) : -1;
+        const int high = __reduce_max_sync(0xffffffffu, pos), low = __reduce_min_sync(0xffffffffu, pos < 0 ? INT_MAX : pos);
         if (lane == 0) {
-            atomicMax(extent + 1, most);
-            atomicMin(extent, least);
+            atomicMax(extent + 1, high);
+            atomicMin(extent, low);
         }
+        asm volatile("bar.sync 1, 128;" ::: "memory");           // the producer need not wait for the queries
+        asm volatile("bar.arrive 2, 256;" ::: "memory");
+    } else {
+        // the warp's 32 rows of queries, one row (or two) per load so that neighbouring lanes read neighbouring columns; sixteen loads on their way before the first of them is stored. Where a
+        // row lies its own lane knows
+        constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 16;
+        const int col = (lane % kLanes) * 4;
+        const float* from = p.q + (size_t)it.tok0 * p.ldq + (size_t)it.h0 * HD + col;
+        auto queries = [&](auto load) {
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += kPer * kAhead) {
+                uint4 x[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k)     // (rows of no token are some other row's: nothing asks for their results)
+                {
+                    const int r = min(warp * 32 + r0 + k * kPer + lane / kLanes, n_rows - 1), token = st_token(sa, r);
+                    x[k] = load(from + (size_t)token * p.ldq + (r - token * sa.hpc) * HD);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int r = warp * 32 + r0 + k * kPer + lane / kLanes;
+                    *reinterpret_cast<uint2*>(sQ + (col / 64) * Sh::kQBlock + r * 128 + ((((col % 64) / 8) ^ (r & 7)) << 4) + (col % 8) * 2) =
+                        make_uint2(tc_pack(__uint_as_float(x[k].x), __uint_as_float(x[k].y)), tc_pack(__uint_as_float(x[k].z), __uint_as_float(x[k].w)));
+                }
+            }
+        };
+        if (sa.vec_q) queries([](const float* src) { return ld_stream(src); });      // (left to itself the compiler had each load wait for the one before: 20000 clocks)
+        else queries([](const float* src) { return make_uint4(__float_as_uint(src[0]), __float_as_uint(src[1]), __float_as_uint(src[2]), __float_as_uint(src[3])); });
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mb_arrive(qready);
+        asm volatile("bar.sync 2, 256;" ::: "memory");
     }
-    __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
     const int least = extent[0], most = extent[1], key1 = min(it.key1, most + 1);
     const StTiles tiles(it.key0, key1, p.window > least ? 0 : least - p.window + 1, p.keep_first);
     const int n = tiles.n;
+    const uint32_t was = done;               // key tiles of the items before: the barriers' phases go on from there
+    done += n;
     if (warp == 4) {
         if (elect_one()) {   // ===== TMA producer =====
             for (int i = 0; i < n; ++i) {
-                const int s = i % ST, j0 = tiles.tile_of(i) * kStKeys;
-                const uint32_t ph = (uint32_t)(i / ST) & 1;
+                const int j0 = tiles.tile_of(i) * kStKeys;
+                const uint32_t s = (was + i) % ST, ph = (was + i) / ST & 1;
                 int at[2], row[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const int pos = j0 + x * kStBox, page = pos < key1 && pos + kStBox > it.key0 ? sh_page(p, it.slot, pos) : -1;
-                    at[x] = page >= 0 ? pos % p.b.page_len : p.b.page_len;                     // outside the map: zeros
+                    int in_page;
+                    const int pos = j0 + x * kStBox, page = pos < key1 && pos + kStBox > it.key0 ? sh_page(p, it.slot, pos, in_page) : -1;
+                    at[x] = page >= 0 ? in_page : p.b.page_len;                     // outside the map: zeros
                     row[x] = page >= 0 ? page * p.kv_heads + it.g : 0;
                 }
                 if (!tc_wait(kempty + s, ph ^ 1, gave_up, sa.polls)) break;
@@ -350,30 +422,31 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             constexpr uint32_t idesc_s = umma_idesc_bf16(kStRows, kStKeys), idesc_o = umma_idesc_bf16(kStRows, HD) | (1u << 16);      // B MN-major
             const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, Sh::kKBlock);  // + bytes / 16: another place
             auto scores = [&](int i) {
-                const uint64_t k = k_desc + (uint32_t)(i % ST) * (Sh::kTile / 16);
+                const uint64_t k = k_desc + (was + i) % ST * (Sh::kTile / 16);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks)
                     tc_mma_bf16(tmem, q_desc + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kKBlock / 16) + 2 * (ks % 4)), idesc_s, ks != 0);
                 tc_commit(sfull);
-                tc_commit(kempty + i % ST);
+                tc_commit(kempty + (was + i) % ST);
             };
-            bool ok = n > 0 && tc_wait(qready, 0, gave_up, sa.polls) && tc_wait(kfull, 0, gave_up, sa.polls);
+            bool ok = n > 0 && tc_wait(qready, turn & 1, gave_up, sa.polls) && tc_wait(kfull + was % ST, was / ST & 1, gave_up, sa.polls);
             if (ok) {
                 tc_fence_after();
                 scores(0);
             }
             for (int i = 0; ok && i < n; ++i) {
-                ok = tc_wait(vready + i % ST, (uint32_t)(i / ST) & 1, gave_up, sa.polls) && tc_wait(pready, (uint32_t)i & 1, gave_up, sa.polls);
+                const uint32_t at = was + i;
+                ok = tc_wait(vready + at % ST, at / ST & 1, gave_up, sa.polls) && tc_wait(pready, at & 1, gave_up, sa.polls);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t v = v_desc + (uint32_t)(i % ST) * (Sh::kTile / 16);
+                const uint64_t v = v_desc + at % ST * (Sh::kTile / 16);
 #pragma unroll
                 for (int ks = 0; ks < 3 * kStKeys / 16; ++ks)                    // first terms, then second ones, then third ones, against the same values
                     tc_mma_bf16_ts(tmem + 128, tmem + 8 * ks, v + (uint32_t)((ks % (kStKeys / 16)) * 128), idesc_o, (i % kStFlush | ks) != 0);
                 tc_commit(odone);
-                tc_commit(vempty + i % ST);
+                tc_commit(vempty + at % ST);
                 if (i + 1 < n) {        // the next scores land where the weights lie that this product is still reading
-                    ok = tc_wait(kfull + (i + 1) % ST, (uint32_t)((i + 1) / ST) & 1, gave_up, sa.polls) && tc_wait(odone, (uint32_t)i & 1, gave_up, sa.polls);
+                    ok = tc_wait(kfull + (at + 1) % ST, (at + 1) / ST & 1, gave_up, sa.polls) && tc_wait(odone, at & 1, gave_up, sa.polls);
                     if (!ok) break;
                     tc_fence_after();
                     scores(i + 1);
@@ -383,17 +456,20 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
         __syncwarp();
     } else if (warp >= 6) {   // ===== values that are not the share's, or no numbers =====
         for (int i = 0; i < n; ++i) {
-            const int s = i % ST, j0 = tiles.tile_of(i) * kStKeys, from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
-            if (!tc_wait_warp(vfull + s, (uint32_t)(i / ST) & 1, gave_up, sa.polls)) break;
+            const uint32_t s = (was + i) % ST;
+            const int j0 = tiles.tile_of(i) * kStKeys, from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
+            if (!tc_wait_warp(vfull + s, (was + i) / ST & 1, gave_up, sa.polls)) break;
             bool odd = false;
 #pragma unroll 8
             for (int x = (warp - 6) * 32 + lane; x < kStKeys * 8 * Sh::kBlocks; x += 64) {      // (the rows of a block of 64 columns lie one behind the other)
                 const int r = x / 8 % kStKeys;
                 uint4* at = reinterpret_cast<uint4*>(sV + s * Sh::kTile + x * 16);
                 const uint4 v = *at;
+                uint32_t sum = 0;
+                st_times_zero(sum, v);
                 if (r < from || r >= to) {
                     *at = make_uint4(0u, 0u, 0u, 0u);
-                } else if (st_odd(v)) {
+                } else if (st_odd(sum)) {
                     *at = st_without(v);
                     odd = true;
                 }
@@ -406,35 +482,9 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
     }
     bool ok = true;
     float ref = -INFINITY, l = 0.0f;         // what the weights are relative to; their sum
-    const int row = threadIdx.x, qi = min(row / sa.hpc, it.nq - 1), h = it.h0 + row % sa.hpc;
-    const bool live = row < n_rows;          // (of the first four warps)
     float* place = sh_record(p, it.tok0 + qi, h, it.which) + kShHead;
     if (warp < 4) {   // ===== softmax: row = warp * 32 + lane = token * hpc + head =====
-        const int qpos = live ? p.b.tok_pos[it.tok0 + qi] : -1;
-        {   // the warp's 32 rows, one row (or two) per load so that neighbouring lanes read neighbouring columns; sixteen loads on their way before the first of them is stored
-            constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 16;
-            const int col = (lane % kLanes) * 4;
-#pragma unroll 1
-            for (int r0 = 0; r0 < 32; r0 += kPer * kAhead) {
-                float4 x[kAhead];
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    const int r = warp * 32 + r0 + k * kPer + lane / kLanes;
-                    const float* src = p.q + (size_t)(it.tok0 + min(r / sa.hpc, it.nq - 1)) * p.ldq + (size_t)(it.h0 + r % sa.hpc) * HD + col;
-                    if (r >= n_rows) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    else if (sa.vec_q) x[k] = *reinterpret_cast<const float4*>(src);
-                    else x[k] = make_float4(src[0], src[1], src[2], src[3]);
-                }
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    const int r = warp * 32 + r0 + k * kPer + lane / kLanes;
-                    *reinterpret_cast<uint2*>(sQ + (col / 64) * Sh::kQBlock + r * 128 + ((((col % 64) / 8) ^ (r & 7)) << 4) + (col % 8) * 2) =
-                        make_uint2(tc_pack(x[k].x, x[k].y), tc_pack(x[k].z, x[k].w));
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mb_arrive(qready);
-        }
+        const int qpos = live ? st_pos(sa, it, qi) : -1;
         const uint32_t s_tmem = tmem + ((uint32_t)(warp * 32) << 16), o_tmem = s_tmem + 128;
         const float slope = kOpts && p.slopes && live ? p.slopes[h] : 0.0f;
         const bool plain = !kOpts;           // weights are 2^(score * mul - ref): one rounding between a score and its exponential. Without caps or charges mul holds the scale, too
@@ -462,9 +512,10 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             // keys of the tile that are in the share and in a page
             const int from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
             uint64_t have = (to >= 64 ? ~0ull : (1ull << to) - 1) & ~((1ull << from) - 1);
-            if (sh_page(p, it.slot, j0) < 0) have &= ~0xffffffffull;
-            if (to > kStBox && sh_page(p, it.slot, j0 + kStBox) < 0) have &= 0xffffffffull;
-            ok = tc_wait_warp(sfull, (uint32_t)i & 1, gave_up, sa.polls);
+            int in_page;
+            if (sh_page(p, it.slot, j0, in_page) < 0) have &= ~0xffffffffull;
+            if (to > kStBox && sh_page(p, it.slot, j0 + kStBox, in_page) < 0) have &= 0xffffffffull;
+            ok = tc_wait_warp(sfull, (was + i) & 1, gave_up, sa.polls);
             if (!ok) break;
             tc_fence_after();
             uint32_t s[64];
@@ -583,14 +634,18 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             tc_fence_before();
             mb_arrive(pready);
         }
-        if (ok && n > 0) ok = tc_wait_warp(odone, (uint32_t)(n - 1) & 1, gave_up, sa.polls);
+        if (ok && n > 0) ok = tc_wait_warp(odone, (was + n - 1) & 1, gave_up, sa.polls);
         tc_fence_after();
         if (ok && live) {
             place[-kShHead] = ref;
             place[1 - kShHead] = l;
         }
-        float* mine = reinterpret_cast<float*>(smem) + warp * (32 * 33);        // the rings' place: every tile has been read
-        const int rows = min(32, n_rows - warp * 32);
+        // A pair of lanes writes the even lane's row first, then the odd one's, 32 bytes each time: 16 bytes into each of 32 rows would be half sectors, and through shared memory, whole lines, it took
+        // 7000 clocks.
+        const bool odd = lane & 1, peer = __shfl_xor_sync(0xffffffffu, live, 1);
+        float* other = reinterpret_cast<float*>(__shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), 1));
+        float *even_row = (odd ? other : place) + (odd ? 4 : 0), *odd_row = (odd ? place : other) + (odd ? 4 : 0);
+        const bool even_live = odd ? peer : live, odd_live = odd ? live : peer;
 #pragma unroll 1
         for (int c = 0; ok && c < HD; c += 32) {
             uint32_t o[32];
@@ -605,35 +660,28 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 add_flushed(o, c);
                 add_flushed(o + 16, c + 16);
             }
-            __syncwarp();        // through shared memory, so that a store covers neighbouring columns of one row
-#pragma unroll
-            for (int e = 0; e < 32; ++e) mine[lane * 33 + e] = __uint_as_float(o[e]);
             __syncwarp();
-#pragma unroll 1
-            for (int r0 = 0; r0 < rows; r0 += 16) {
-                float x[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) x[k] = mine[(r0 + k) * 33 + lane];
+            for (int e = 0; e < 32; e += 8) {
+                uint32_t got[4];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const int rr = warp * 32 + r0 + k;
-                    if (r0 + k < rows) sh_record(p, it.tok0 + rr / sa.hpc, it.h0 + rr % sa.hpc, it.which)[kShHead + c + lane] = x[k];
-                }
+                for (int i = 0; i < 4; ++i) got[i] = __shfl_xor_sync(0xffffffffu, odd ? o[e + i] : o[e + 4 + i], 1);
+                if (even_live) *reinterpret_cast<uint4*>(even_row + c + e) = odd ? make_uint4(got[0], got[1], got[2], got[3]) : make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                if (odd_live) *reinterpret_cast<uint4*>(odd_row + c + e) = odd ? make_uint4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]) : make_uint4(got[0], got[1], got[2], got[3]);
             }
-            __syncwarp();
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (*gave_up) tc_gave_up(sa.status);
     if (extent[2] && warp < 4 && live) {     // infinities and NaN that were taken out of the values: back to the rows that see them (columns of this row alone, written behind the barrier)
-        const int qpos = p.b.tok_pos[it.tok0 + qi];
+        const int qpos = st_pos(sa, it, qi);
         for (int i = 0; i < n; ++i) {
             const int j0 = tiles.tile_of(i) * kStKeys;
             for (int key = max(j0, it.key0); key < min(j0 + kStKeys, key1); ++key) {
-                const int page = sh_page(p, it.slot, key);
+                int in_page;
+                const int page = sh_page(p, it.slot, key, in_page);
                 if (page < 0 || !seq_sees(qpos, key, p.window, p.keep_first)) continue;
-                const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v_pool) + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, key % p.b.page_len, HD);
+                const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v_pool) + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD);
                 for (int c = 0; c < HD; ++c) {
                     const float x = seq_ld(v, c);
                     if (!(fabsf(x) <= FLT_MAX)) place[c] += x;
@@ -641,10 +689,34 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             }
         }
     }
-    if (warp == 5) {
-        tc_fence_after();
-        tc_dealloc(tmem, kStTmem);
+}
+
+// Keys of a share of the shared positions: by what all groups have (row tiles x key tiles), such that the shares are a round of the grid or a few, and none so short that its beginning and end (as
+// long as some three key tiles) count for more than the rest. Thirty-two lengths about the even one are tried, a lane each. group(g, tiles, keys): row tiles and key tiles of a group. By one warp.
+template <class F>
+__device__ __forceinline__ int st_least(const SharedArgs& p, int all_sets, F group) {
+    const int lane = threadIdx.x & 31, ctas = (int)gridDim.x;
+    long long units = 0, items = 0;
+    for (int g = lane; g < p.n_groups; g += 32) {
+        int tiles, keys;
+        group(g, tiles, keys);
+        units += (long long)tiles * keys;
     }
+    for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+    const long long even = (units * all_sets + ctas - 1) / ctas;
+    const int length = (int)max(4LL, min(1LL << 20, even * (4 + lane) / 16));
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
+        int tiles = 0, keys = 0;
+        if (g0 + lane < p.n_groups) group(g0 + lane, tiles, keys);
+        for (unsigned rest = __ballot_sync(0xffffffffu, tiles > 0 && keys > 0); rest; rest &= rest - 1) {
+            const int who = __ffs(rest) - 1, k = __shfl_sync(0xffffffffu, keys, who);
+            items += (long long)__shfl_sync(0xffffffffu, tiles, who) * min(p.shares, (k + length - 1) / length);
+        }
+    }
+    items *= all_sets;
+    long long cost = ((items + ctas - 1) / ctas) * (length + 3) * 32 + lane;
+    for (int o = 16; o > 0; o >>= 1) cost = min(cost, __shfl_xor_sync(0xffffffffu, cost, o));
+    return __shfl_sync(0xffffffffu, length, (int)(cost & 31)) * kStKeys;
 }
 
 template <int HD, bool kOpts>
@@ -652,50 +724,124 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
     after_previous();        // in front of the allocation of TMEM: a CTA that waits for another kernel must not hold what that kernel's CTAs may be waiting for
     extern __shared__ uint8_t st_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(st_raw) + 1023) & ~(uintptr_t)1023);
+    StPlan& plan = *reinterpret_cast<StPlan*>(smem + StShape<HD>::kPlan);
+    volatile int* gave_up = st_gave_up<HD>(smem);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(st_gave_up<HD>(smem) + 7);
     const SharedArgs& p = sa.a;
-    const int all_sets = p.kv_heads * sa.sets;
-    StItem it;
-    int x = (int)blockIdx.x;
-    if (x < sa.group_tiles * all_sets * p.shares) {      // the group tiles, tiles of one share and head set beside each other
-        int tile = x % sa.group_tiles, first, n;
-        x /= sa.group_tiles;
-        const int z = x % p.shares, set = x / p.shares;
-        const int i = sh_find_group(p, sa.queries, tile, first, n);
-        if (i < 0) return;
-        const int len = max(0, p.group_len[i]), tiles = (len + kStKeys - 1) / kStKeys, cuts = sh_cuts(len, kShLeast, p.shares);
-        if (z >= cuts) return;
-        it.tok0 = first + tile * sa.queries;
-        it.nq = min(sa.queries, n - tile * sa.queries);
-        it.slot = p.b.seg_slot[p.group_start[i]];
-        it.g = set / sa.sets;
-        it.h0 = it.g * (p.heads / p.kv_heads) + set % sa.sets * sa.hpc;
-        it.key0 = tiles * z / cuts * kStKeys;
-        it.key1 = min(len, tiles * (z + 1) / cuts * kStKeys);
-        it.which = z;
-    } else {
-        x -= sa.group_tiles * all_sets * p.shares;
-        const int tile = x % p.b.n_qtiles;
-        x /= p.b.n_qtiles;
-        const int z = x % p.own, sub = x / p.own % sa.subs, set = x / p.own / sa.subs;
-        const int seg = p.b.qt_seg[tile], off = p.b.qt_off[tile], n = min(kBQ, p.b.seg_len[seg] - off);
-        if (sub * sa.queries >= n) return;
-        const int all = p.b.seg_pos0[seg] + off + n, from = min(sh_shared_len(p, seg), all), cuts = sh_cuts(all - from, kShOwnLeast, p.own);
-        if (z >= cuts) return;
-        const int t0 = from / kStKeys, tiles = (all + kStKeys - 1) / kStKeys - t0;
-        it.tok0 = p.b.seg_start[seg] + off + sub * sa.queries;
-        it.nq = min(sa.queries, n - sub * sa.queries);
-        it.slot = p.b.seg_slot[seg];
-        it.g = set / sa.sets;
-        it.h0 = it.g * (p.heads / p.kv_heads) + set % sa.sets * sa.hpc;
-        it.key0 = max(from, (t0 + tiles * z / cuts) * kStKeys);
-        it.key1 = min(all, (t0 + tiles * (z + 1) / cuts) * kStKeys);
-        it.which = p.shares + z;
-        if (it.nq * sa.hpc <= kStFew) {
-            st_few<HD>(sa, it, reinterpret_cast<float*>(smem));
-            return;
-        }
+    const int all_sets = p.kv_heads * sa.sets, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.heads / p.kv_heads;
+    if (threadIdx.x == 0) {
+        st_barriers<HD>(smem);
+        *gave_up = 0;
+        st_gave_up<HD>(smem)[1] = INT_MAX;       // of the first item; each makes those of the next one ready
+        st_gave_up<HD>(smem)[2] = -1;
+        st_gave_up<HD>(smem)[3] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    st_many<HD, kOpts>(tmK, tmV, sa, it, smem);
+    if (warp == 5) tc_alloc(tmem_slot, kStTmem);
+    uint32_t done = 0, turn = 0;             // key tiles and items of the first kind so far
+    long long mine = blockIdx.x;             // the next item of this CTA, counted from the present entries' first
+    const int entries = p.n_groups + p.b.n_qtiles;
+    for (int e0 = 0; e0 < entries; e0 += kStEntries) {
+        {   // an entry a thread
+            const int e = e0 + threadIdx.x, i = threadIdx.x;
+            int tok0 = 0, n = 0, slot = -1, from = 0, end = 0, cuts = 0, tiles = 0, seg = -1;
+            if (e < p.n_groups) {
+                sh_group_tokens(p, e, tok0, n);
+                end = max(0, p.group_len[e]);
+                tiles = (n + sa.queries - 1) / sa.queries;
+                if (n > 0) slot = p.b.seg_slot[p.group_start[e]];
+                plan.n[i] = n; plan.end[i] = end; plan.tiles[i] = tiles; plan.from[i] = p.group_start[e];
+            } else if (e < entries) {
+                const int off = p.b.qt_off[e - p.n_groups];
+                seg = p.b.qt_seg[e - p.n_groups];
+                n = min(kBQ, p.b.seg_len[seg] - off);
+                end = p.b.seg_pos0[seg] + off + n;
+                tok0 = p.b.seg_start[seg] + off;
+                slot = p.b.seg_slot[seg];
+                tiles = n * sa.hpc <= kStFew ? 1 : (n + sa.queries - 1) / sa.queries;
+            }
+            tc_fence_before();
+            __syncthreads();
+            const bool all = p.n_groups <= kStEntries;           // of the first entries: every group is at hand
+            if (e0 == 0 && warp == 0) {
+                const int least = all ? st_least(p, all_sets, [&](int g, int& t, int& k) { t = plan.tiles[g]; k = (plan.end[g] + kStKeys - 1) / kStKeys; })
+                                      : st_least(p, all_sets, [&](int g, int& t, int& k) {
+                                            int first, m;
+                                            sh_group_tokens(p, g, first, m);
+                                            t = (m + sa.queries - 1) / sa.queries;
+                                            k = (max(0, p.group_len[g]) + kStKeys - 1) / kStKeys;
+                                        });
+                if (lane == 0) {
+                    plan.least = least;
+                    if (blockIdx.x == 0) *p.plan = least;
+                }
+            }
+            if (seg >= 0) {
+                int lo = 0, hi = p.n_groups;                     // group_start[lo] <= seg < group_start[hi]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if ((all && e0 == 0 ? plan.from[mid] : p.group_start[mid]) <= seg) lo = mid; else hi = mid;
+                }
+                from = min(all && e0 == 0 ? plan.end[lo] : max(0, p.group_len[lo]), end);
+                cuts = sh_cuts(end - from, p.own_least, p.own);
+            }
+            __syncthreads();
+            if (e < p.n_groups) cuts = sh_cuts(end, plan.least, p.shares);
+            plan.tok0[i] = tok0; plan.n[i] = n; plan.slot[i] = slot; plan.from[i] = from; plan.end[i] = end; plan.cuts[i] = cuts; plan.tiles[i] = tiles;
+            const bool few = seg >= 0 && n * sa.hpc <= kStFew;
+            int upto = few ? (cuts * all_sets + 1) / 2 : tiles * cuts * all_sets;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            if (lane == 31) plan.warp[warp] = upto;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) upto += plan.warp[w];
+            plan.upto[i] = upto;
+            __syncthreads();
+        }
+        tc_fence_after();                    // (the allocation, at the first turn)
+        const uint32_t tmem = *tmem_slot;
+        const int total = plan.upto[kStEntries - 1];
+        for (; mine < total && !*gave_up; mine += gridDim.x) {
+            int e = 0;                       // the first entry that reaches beyond it
+            for (int w = kStEntries / 2; w > 0; w /= 2)
+                if (plan.upto[e + w - 1] <= (int)mine) e += w;
+            int x = (int)mine - (e ? plan.upto[e - 1] : 0);
+            const bool group = e0 + e < p.n_groups;
+            const uint32_t tiles = plan.tiles[e], cuts = plan.cuts[e];
+            const int n = plan.n[e], from = plan.from[e], end = plan.end[e], t0 = from / kStKeys, span = (end + kStKeys - 1) / kStKeys - t0;
+            const bool few = !group && n * sa.hpc <= kStFew;
+            if (few) x = 2 * x + threadIdx.x / (32 * kStTeam);
+            const uint32_t y = (uint32_t)x / tiles, tile = x - y * tiles, z = y / (uint32_t)all_sets, set = y - z * all_sets;
+            StItem it;
+            it.g = sa.sets == 1 ? set : set / (uint32_t)sa.sets;
+            it.tok0 = plan.tok0[e] + tile * sa.queries;
+            it.nq = min(sa.queries, n - (int)tile * sa.queries);
+            it.slot = plan.slot[e];
+            it.pos0 = group ? -1 : end - n + (int)tile * sa.queries;
+            it.h0 = it.g * per + (set - it.g * sa.sets) * sa.hpc;
+            it.key0 = max(from, (int)(t0 + span * z / cuts) * kStKeys);                      // (span * z: 2^25 key tiles at most, 32 shares)
+            it.key1 = min(end, (int)(t0 + span * (z + 1) / cuts) * kStKeys);
+            it.which = (group ? 0 : p.shares) + z;
+            if (few) {
+                if (z < cuts) st_few<HD>(sa, it, reinterpret_cast<float*>(smem));
+            } else {
+                st_many<HD, kOpts>(tmK, tmV, sa, it, smem, tmem, done, turn++);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the next item's copies may land where this one has written
+            __syncthreads();
+        }
+        mine -= total;
+        __syncthreads();                     // the entries have been read
+        if (*gave_up) break;
+    }
+    if (*gave_up) tc_gave_up(sa.status);
+    if (warp == 5) {
+        tc_fence_after();
+        tc_dealloc(*tmem_slot, kStTmem);
+    }
 }
 
 template <int HD, bool kOpts>
@@ -715,8 +861,7 @@ static int st_launch(const SharedArgs& p, cudaStream_t st) {
     for (a.hpc = std::min(per, 16); per % a.hpc; --a.hpc) {}
     a.sets = per / a.hpc;
     a.queries = kStRows / a.hpc;
-    a.subs = p.b.T == p.b.nseg ? 1 : (kBQ + a.queries - 1) / a.queries;
-    a.group_tiles = (p.b.T + a.queries - 1) / a.queries + p.n_groups;
+    a.hpc_magic = (65536u + a.hpc - 1) / a.hpc;
     if (int rc = status_word(&a.status)) return rc;
     a.polls = (unsigned)g_tune_tc_polls;
     a.vec_q = p.ldq % 4 == 0 && ((uintptr_t)p.q % 16) == 0;
@@ -726,9 +871,10 @@ static int st_launch(const SharedArgs& p, cudaStream_t st) {
     const cuuint32_t box[3] = {64, kStBox, 1};
     if (int rc = tc_encode_bf16(&tmK, p.k_pool, 3, dims, strides, box)) return rc;
     if (int rc = tc_encode_bf16(&tmV, p.v_pool, 3, dims, strides, box)) return rc;
-    const long long all_sets = (long long)p.kv_heads * a.sets, grid = all_sets * ((long long)a.group_tiles * p.shares + (long long)p.b.n_qtiles * p.own * a.subs);
-    SLLM_REQUIRE(grid <= 0x7fffffffLL, SLLM_ENOTSUP, "seq_attention_shared: too many tokens or heads");
-    overlapping(kernel)<<<(unsigned)grid, kStThreads, Sh::kSmem, st>>>(tmK, tmV, a);
+    const long long row_tiles = (p.b.T + a.queries - 1) / a.queries + p.n_groups, all_sets = (long long)p.kv_heads * a.sets;
+    SLLM_REQUIRE((row_tiles * p.shares + ((long long)p.b.n_qtiles + row_tiles) * p.own) * all_sets <= 0x7fffffffLL, SLLM_ENOTSUP, "seq_attention_shared: too many tokens or heads");
+    const long long most = (row_tiles * p.shares + (long long)p.b.n_qtiles * ((kBQ + a.queries - 1) / a.queries) * p.own) * all_sets;
+    overlapping(kernel)<<<(unsigned)std::min<long long>(most, 2 * sm_count()), kStThreads, Sh::kSmem, st>>>(tmK, tmV, a);
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
