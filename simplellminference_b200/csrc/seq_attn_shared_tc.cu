@@ -10,7 +10,8 @@
 //   warps 6-7  zero the value rows that are not part of the share, and take infinities and NaN out of the values (0 * NaN is NaN for rows that do not see them, and the terms of a weight times
 //              infinity are NaN for those that do); rows that see them get them back at the end.
 // Where a segment has few rows of its own (a decoding request: the query heads of one token), four warps take 16 keys in turn on mma.sync, 8 rows at a time as the columns: such work is bound by what
-// it reads, and a tile of 128 rows would be empty but for four. A CTA does two items at once, since one is a chain (queries, pages, keys and values, maximum, sums, four parts put together). Keys and values go from the pool to registers as the products take them, 16 bytes a load: the columns of a head are contracted in
+// it reads, and a tile of 128 rows would be empty but for four. A CTA does two items at once, since one is a chain (queries, pages, keys and values,
+// maximum, sums, four parts put together), and the next keys and values are on their way to shared memory meanwhile. Keys and values go from the pool to registers as the products take them, 16 bytes a load: the columns of a head are contracted in
 // an order of the kernel's own, and those of the values are dealt to the tiles of O so that a lane's eight neighbours are rows of four of them.
 #include <cfloat>
 
@@ -22,7 +23,7 @@ namespace sllm {
 constexpr int kStRows = 128, kStKeys = 64, kStThreads = 256, kStBox = 32, kStWarps = kStThreads / 32;
 constexpr int kStFlush = 12;
 constexpr uint32_t kStTmem = 256;            // scores at 0 .. 63, then the weights' terms at 0 .. 95, O at 128; two CTAs share an SM's 512 columns
-constexpr int kStFew = 16, kStTeam = 4;      // rows of a segment up to which its own positions are a team's work; warps of a team, of which a CTA has two
+constexpr int kStFew = 16, kStTeam = 4, kStTeams = kStWarps / kStTeam;      // rows of a segment up to which its own positions are a team's work; warps of a team
 constexpr float kStLog2e = 1.4426950408889634f;
 
 template <int HD>
@@ -92,35 +93,17 @@ __device__ __forceinline__ uint32_t st_turned(uint32_t x) {              // 8 x 
 }
 
 template <int HD>
-__device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
+__device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8_t* smem) {
     const SharedArgs& p = sa.a;
-    constexpr int kSteps = HD / 32, kHalves = HD / 64, kTiles = HD / 16;
+    constexpr int kSteps = HD / 32, kHalves = HD / 64, kTiles = HD / 16, kStage = 64 * HD;       // bytes of a warp: 16 keys, 16 values
     const int team = threadIdx.x / (32 * kStTeam), warp = threadIdx.x / 32 % kStTeam, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_rows = it.nq * sa.hpc;
     auto together = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(3 + team) : "memory"); };
-    smem += team * (kStTeam * 8 * (HD + 2));
+    auto area = [&](int w) { return smem + (team * kStTeam + w) * kStage; };
+    // what a lane copies it reads itself, 16 bytes beside its neighbours' 16 bytes
+    uint8_t *k_stage = area(warp) + lane * 16, *v_stage = k_stage + kStage / 2;
     const uint16_t *kp = reinterpret_cast<const uint16_t*>(p.k_pool), *vp = reinterpret_cast<const uint16_t*>(p.v_pool);
-    const int start = it.key0 / 16 * 16 + 16 * warp;
     for (int r0 = 0; r0 < n_rows; r0 += 8) {
-        int next_in = 0, next_page = start < it.key1 ? sh_page(p, it.slot, start, next_in) : -1;
         // columns of the products: rows r0 .. r0 + 7. As an operand a lane has row g, as a result rows 2t and 2t + 1
-        uint32_t q[kSteps][4];
-        {
-            const int r = min(r0 + g, n_rows - 1);
-            const int qi = st_token(sa, r);
-            const float* src = p.q + (size_t)(it.tok0 + qi) * p.ldq + (size_t)(it.h0 + r - qi * sa.hpc) * HD + 8 * t;
-            if (sa.vec_q) {
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    const float4 a = *reinterpret_cast<const float4*>(src + 32 * s), b = *reinterpret_cast<const float4*>(src + 32 * s + 4);
-                    q[s][0] = pack_bf16(a.x, a.y); q[s][1] = pack_bf16(a.z, a.w); q[s][2] = pack_bf16(b.x, b.y); q[s][3] = pack_bf16(b.z, b.w);
-                }
-            } else {
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) q[s][e] = pack_bf16(src[32 * s + 2 * e], src[32 * s + 2 * e + 1]);
-            }
-        }
         int pos[2];
         float slope[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kTiles][4] = {};
 #pragma unroll
@@ -137,40 +120,75 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
             least = min(least, __shfl_xor_sync(0xffffffffu, least, w));
         }
         const int end = min(it.key1, last + 1), oldest = p.window > least ? 0 : least - p.window + 1;
-        for (int j0 = start; j0 < end; j0 += 16 * kStTeam) {
-            const int page = next_page, in_page = next_in;                                    // (pages are a multiple of 32 positions)
-            if (j0 + 16 * kStTeam < end) next_page = sh_page(p, it.slot, j0 + 16 * kStTeam, next_in);
-            if (page < 0 || (j0 + 16 <= oldest && j0 >= p.keep_first)) continue;
-            const uint16_t* kr = kp + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD) + 8 * t;
-            const uint16_t* vr = vp + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD) + 8 * g;
-            auto mine = [&](int key) { return key >= it.key0 && key < end; };
-            // All sixteen rows are the page's, so nothing is asked before they are loaded: a condition around a load made each wait for the one before (13000 clocks a tile). Scores of keys that are not
-            // the share's are replaced, their values taken out below.
-            uint4 k[kSteps][2], v[kHalves][4];
+        auto mine = [&](int key) { return key >= it.key0 && key < end; };
+        if (r0 > 0) together();              // the rows before these have been read
+        // the warp's next sixteen keys that there are, and their page
+        int page = -1, in_page = 0;
+        auto next = [&](int j) {
+            for (; j < end; j += 16 * kStTeam) {
+                if (j + 16 <= oldest && j >= p.keep_first) continue;
+                page = sh_page(p, it.slot, j, in_page);              // (pages are a multiple of 32 positions)
+                if (page >= 0) break;
+            }
+            return j;
+        };
+        // All sixteen rows are the page's, whatever part of them is the share's: scores of the others are replaced, their values taken out below.
+        auto fetch_keys = [&](bool there) {
+            if (there) {
+                const uint16_t* kr = kp + seq_pool_row(page, p.kv_heads, it.g, p.b.page_len, in_page, HD) + g * HD + 8 * t;
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
+                for (int i = 0; i < 2 * kSteps; ++i) cp_async16(k_stage + i * 512, kr + (i & 1) * 8 * HD + 32 * (i >> 1), 16);
+            }
+            cp_async_commit();
+        };
+        auto value_row = [&](int pg, int in) { return vp + seq_pool_row(pg, p.kv_heads, it.g, p.b.page_len, in, HD) + 8 * g; };
+        auto fetch_values = [&](bool there) {
+            if (there) {
+                const uint16_t* vr = value_row(page, in_page) + 2 * t * HD;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) k[s][i] = ld_stream(kr + (g + 8 * i) * HD + 32 * s);
+                for (int i = 0; i < 4 * kHalves; ++i) cp_async16(v_stage + i * 512, vr + ((i & 1) + 8 * ((i >> 1) & 1)) * HD + 64 * (i >> 2), 16);
+            }
+            cp_async_commit();
+        };
+        int j0 = next(it.key0 / 16 * 16 + 16 * warp);
+        fetch_keys(j0 < end);
+        fetch_values(j0 < end);
+        uint32_t q[kSteps][4];
+        {
+            const int r = min(r0 + g, n_rows - 1), qi = st_token(sa, r);
+            const float* src = p.q + (size_t)(it.tok0 + qi) * p.ldq + (size_t)(it.h0 + r - qi * sa.hpc) * HD + 8 * t;
+            if (sa.vec_q) {
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h)
+                for (int s = 0; s < kSteps; ++s) {
+                    const float4 a = *reinterpret_cast<const float4*>(src + 32 * s), b = *reinterpret_cast<const float4*>(src + 32 * s + 4);
+                    q[s][0] = pack_bf16(a.x, a.y); q[s][1] = pack_bf16(a.z, a.w); q[s][2] = pack_bf16(b.x, b.y); q[s][3] = pack_bf16(b.z, b.w);
+                }
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[h][i] = ld_stream(vr + (2 * t + (i & 1) + 8 * (i >> 1)) * HD + 64 * h);
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[s][e] = pack_bf16(src[32 * s + 2 * e], src[32 * s + 2 * e + 1]);
+            }
+        }
+        while (j0 < end) {
+            const int at_page = page, at_in = in_page, j1 = next(j0 + 16 * kStTeam);
+            cp_async_wait<1>();              // the keys, not the values
             float s[4] = {};                 // (key g, rows 2t and 2t + 1), (key g + 8, the same)
 #pragma unroll
             for (int e = 0; e < kSteps; ++e) {
-                const uint32_t a0[4] = {k[e][0].x, k[e][1].x, k[e][0].y, k[e][1].y}, a1[4] = {k[e][0].z, k[e][1].z, k[e][0].w, k[e][1].w};
+                const uint4 k0 = *reinterpret_cast<const uint4*>(k_stage + (2 * e) * 512), k1 = *reinterpret_cast<const uint4*>(k_stage + (2 * e + 1) * 512);
+                const uint32_t a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
                 mma_bf16_16816(s, a0, q[e][0], q[e][1]);
                 mma_bf16_16816(s, a1, q[e][2], q[e][3]);
             }
-            bool sees[4];
+            fetch_keys(j1 < end);
             float top[2] = {m[0], m[1]};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = j0 + g + 8 * (i >> 1), row = i & 1;
-                sees[i] = mine(key) && seq_sees(pos[row], key, p.window, p.keep_first);
                 float x = s[i] * p.scale;
                 if (p.softcap > 0.0f) x = p.softcap * tc_tanh(x / p.softcap);
-                s[i] = sees[i] ? fmaf(-slope[row], (float)(pos[row] - key), x * kStLog2e) : -INFINITY;
+                s[i] = mine(key) && seq_sees(pos[row], key, p.window, p.keep_first) ? fmaf(-slope[row], (float)(pos[row] - key), x * kStLog2e) : -INFINITY;
                 top[row] = fmaxf(top[row], s[i]);
             }
 #pragma unroll
@@ -201,80 +219,82 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
             for (int x = 0; x < 3; ++x)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) b[x][i] = st_turned(b[x][i]);
-            if (j0 < it.key0 || j0 + 16 > end) {
+            cp_async_wait<1>();              // the values, not the next keys
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool in = mine(j0 + 2 * t + (i & 1) + 8 * (i >> 1));
+            for (int h = 0; h < kHalves; ++h) {
+                uint4 v[4];
+                uint32_t odd = 0;            // a value that is no number goes by itself to the rows that see its key
 #pragma unroll
-                    for (int h = 0; h < kHalves; ++h) {
-                        v[h][i].x = in ? v[h][i].x : 0u; v[h][i].y = in ? v[h][i].y : 0u; v[h][i].z = in ? v[h][i].z : 0u; v[h][i].w = in ? v[h][i].w : 0u;
-                    }
+                for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(v_stage + (4 * h + i) * 512);
+                if (j0 < it.key0 || j0 + 16 > end) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!mine(j0 + 2 * t + (i & 1) + 8 * (i >> 1))) v[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
-            }
-            uint32_t odd = 0;                // a value that is no number goes by itself to the rows that see its key
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st_times_zero(odd, v[h][i]);
-            if (__any_sync(0xffffffffu, st_odd(odd))) {
+                for (int i = 0; i < 4; ++i) st_times_zero(odd, v[i]);
+                if (__any_sync(0xffffffffu, st_odd(odd))) {
+                    const uint16_t* vr = value_row(at_page, at_in);
 #pragma unroll 1
-                for (int key = 0; key < 16; ++key) {
-                    if (!mine(j0 + key)) continue;
-                    const bool s0 = seq_sees(pos[0], j0 + key, p.window, p.keep_first), s1 = seq_sees(pos[1], j0 + key, p.window, p.keep_first);
+                    for (int key = 0; key < 16; ++key) {
+                        if (!mine(j0 + key)) continue;
+                        const bool s0 = seq_sees(pos[0], j0 + key, p.window, p.keep_first), s1 = seq_sees(pos[1], j0 + key, p.window, p.keep_first);
 #pragma unroll
-                    for (int c = 0; c < kTiles; ++c)
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {          // columns 64 (c / 4) + 8 g + 2 (c % 4) + i, rows 2t and 2t + 1
-                            const float x = seq_ld(vr + key * HD, 64 * (c / 4) + 2 * (c % 4) + i);
-                            if (fabsf(x) <= FLT_MAX) continue;
-                            if (s0) o[c][2 * i] += x;
-                            if (s1) o[c][2 * i + 1] += x;
-                        }
+                            for (int i = 0; i < 2; ++i) {      // columns 64 h + 8 g + 2 c + i, rows 2t and 2t + 1
+                                const float x = seq_ld(vr + key * HD, 64 * h + 2 * c + i);
+                                if (fabsf(x) <= FLT_MAX) continue;
+                                if (s0) o[4 * h + c][2 * i] += x;
+                                if (s1) o[4 * h + c][2 * i + 1] += x;
+                            }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = st_without(v[i]);
                 }
-#pragma unroll
-                for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[h][i] = st_without(v[h][i]);
-            }
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    auto word = [&](int i) { return e == 0 ? v[h][i].x : e == 1 ? v[h][i].y : e == 2 ? v[h][i].z : v[h][i].w; };
+                    auto word = [&](int i) { return e == 0 ? v[i].x : e == 1 ? v[i].y : e == 2 ? v[i].z : v[i].w; };
                     const uint32_t a[4] = {__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(0), word(1), 0x7632), __byte_perm(word(2), word(3), 0x5410), __byte_perm(word(2), word(3), 0x7632)};
 #pragma unroll
                     for (int x = 0; x < 3; ++x) mma_bf16_16816(o[4 * h + e], a, b[x][0], b[x][1]);
                 }
+            }
+            fetch_values(j1 < end);
+            j0 = j1;
         }
+        cp_async_wait<0>();
 #pragma unroll
         for (int w = 4; w < 32; w *= 2) {
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], w);
             l[1] += __shfl_xor_sync(0xffffffffu, l[1], w);
         }
-        // the warps' parts: [warp][row][columns], then references and sums
-        float *part = smem, *ref = part + kStTeam * 8 * HD, *sum = ref + kStTeam * 8;
-        if (r0 > 0) together();              // the rows before these have been read
+        // the warps' parts, each in its own area: [row][columns], then references and sums
+        __syncwarp();
+        float* part = reinterpret_cast<float*>(area(warp));
 #pragma unroll
         for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                *reinterpret_cast<float2*>(part + (warp * 8 + 2 * t + i) * HD + 64 * (c / 4) + 8 * g + 2 * (c % 4)) = make_float2(o[c][i], o[c][2 + i]);
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(part + (2 * t + i) * HD + 64 * (c / 4) + 8 * g + 2 * (c % 4)) = make_float2(o[c][i], o[c][2 + i]);
         if (g == 0) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                ref[warp * 8 + 2 * t + i] = m[i];
-                sum[warp * 8 + 2 * t + i] = l[i];
+                part[8 * HD + 2 * t + i] = m[i];
+                part[8 * HD + 8 + 2 * t + i] = l[i];
             }
         }
         together();
         for (int i = warp; i < min(8, n_rows - r0); i += kStTeam) {      // a warp puts a row together
             float mx = -INFINITY, all = 0.0f, f[kStTeam];
 #pragma unroll
-            for (int w = 0; w < kStTeam; ++w) mx = fmaxf(mx, ref[w * 8 + i]);
+            for (int w = 0; w < kStTeam; ++w) {
+                f[w] = reinterpret_cast<const float*>(area(w))[8 * HD + i];
+                mx = fmaxf(mx, f[w]);
+            }
 #pragma unroll
             for (int w = 0; w < kStTeam; ++w) {
-                const float y = sum[w * 8 + i];
-                f[w] = ref[w * 8 + i] == -INFINITY && y == 0.0f ? 0.0f : fmaxf(tc_exp2(ref[w * 8 + i] - mx), FLT_MIN);
+                const float y = reinterpret_cast<const float*>(area(w))[8 * HD + 8 + i];
+                f[w] = f[w] == -INFINITY && y == 0.0f ? 0.0f : fmaxf(tc_exp2(f[w] - mx), FLT_MIN);
                 all = fmaf(f[w], y, all);
             }
             const int qi = st_token(sa, r0 + i);
@@ -287,7 +307,7 @@ __device__ void st_few(const StArgs& sa, const StItem& it, float* smem) {
                 float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < kStTeam; ++w) {      // (a part without keys is zeros)
-                    const float4 x = *reinterpret_cast<const float4*>(part + (w * 8 + i) * HD + 4 * lane);
+                    const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(area(w)) + i * HD + 4 * lane);
                     y.x = fmaf(f[w], x.x, y.x); y.y = fmaf(f[w], x.y, y.y); y.z = fmaf(f[w], x.z, y.z); y.w = fmaf(f[w], x.w, y.w);
                 }
                 *reinterpret_cast<float4*>(rec + kShHead + 4 * lane) = y;
@@ -789,7 +809,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             if (e < p.n_groups) cuts = sh_cuts(end, plan.least, p.shares);
             plan.tok0[i] = tok0; plan.n[i] = n; plan.slot[i] = slot; plan.from[i] = from; plan.end[i] = end; plan.cuts[i] = cuts; plan.tiles[i] = tiles;
             const bool few = seg >= 0 && n * sa.hpc <= kStFew;
-            int upto = few ? (cuts * all_sets + 1) / 2 : tiles * cuts * all_sets;
+            int upto = few ? (cuts * all_sets + kStTeams - 1) / kStTeams : tiles * cuts * all_sets;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int x = __shfl_up_sync(0xffffffffu, upto, o);
@@ -813,7 +833,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             const uint32_t tiles = plan.tiles[e], cuts = plan.cuts[e];
             const int n = plan.n[e], from = plan.from[e], end = plan.end[e], t0 = from / kStKeys, span = (end + kStKeys - 1) / kStKeys - t0;
             const bool few = !group && n * sa.hpc <= kStFew;
-            if (few) x = 2 * x + threadIdx.x / (32 * kStTeam);
+            if (few) x = kStTeams * x + threadIdx.x / (32 * kStTeam);
             const uint32_t y = (uint32_t)x / tiles, tile = x - y * tiles, z = y / (uint32_t)all_sets, set = y - z * all_sets;
             StItem it;
             it.g = sa.sets == 1 ? set : set / (uint32_t)sa.sets;
@@ -826,7 +846,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             it.key1 = min(end, (int)(t0 + span * (z + 1) / cuts) * kStKeys);
             it.which = (group ? 0 : p.shares) + z;
             if (few) {
-                if (z < cuts) st_few<HD>(sa, it, reinterpret_cast<float*>(smem));
+                if (z < cuts) st_few<HD>(sa, it, smem);
             } else {
                 st_many<HD, kOpts>(tmK, tmV, sa, it, smem, tmem, done, turn++);
             }
@@ -847,7 +867,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
 template <int HD, bool kOpts>
 static int st_launch(const SharedArgs& p, cudaStream_t st) {
     using Sh = StShape<HD>;
-    static_assert(Sh::kSmem - 1024 >= kStWarps * 8 * (HD + 2) * 4, "the warps' parts");
+    static_assert(Sh::kBars >= kStWarps * 64 * HD && 64 * HD >= (8 * HD + 16) * 4, "the warps' areas");
     auto* kernel = seq_attention_shared_tc_kernel<HD, kOpts>;
     static OncePerDevice ready;
     if (int rc = ready([&] {

@@ -2,18 +2,21 @@
 //
 //   s_t = max(max_k |x_tk| / 127, 2^-126),  a_tk = round(x_tk / s_t);   C_tn = (sum_k a_tk w_nk) * s_t * v_n + bias_n
 // Sums of codes are exact in 32 bits (127 * 127 * 131072 < 2^31), so a result is three roundings of fp32 away from the formula and does not depend on how a product is cut.
+#include <type_traits>
+
 #include "seq_common.cuh"
 #include "tcgen05.cuh"
 
 namespace sllm {
 
 // ---- rows to codes --------------------------------------------------------------------------------------------------------------------------------------------------------------------
-// A row belongs to blockDim.x threads, which keep kQzValues of its values each in registers (longer rows are read a second time). The largest magnitude is taken over the values' bits, in
-// whose order infinity and NaN come last: a row that has one gets the scale NaN and zeros.
-// The quotient has to be the IEEE one, but a division costs some ten instructions: x times the inverse of the scale is off by less than two units of the last place (2^-16 at 127), so only quotients
-// within 2^-14 of a border between two whole numbers are divided out.
-constexpr int kQzValues = 16, kQzThreads = 1024;
+// A row belongs to a team of warps, which keeps it in registers as it was loaded, up to eight loads of 16 bytes a thread (longer rows are read a second time); a CTA has several teams. The largest
+// magnitude is taken over the values' bits, in whose order infinity and NaN come last: a row that has one gets the scale NaN and zeros.
+// The quotient has to be the IEEE one, but a division costs some ten instructions: x times the inverse of the scale is off by less than two units of the last place (2^-16 at 127), so only where one
+// of a load's quotients is within 2^-14 of a border between two whole numbers are they divided out.
+constexpr int kQzLoads = 8, kQzFewLoads = 2, kQzThreads = 256, kQzWide = 1024;
 constexpr float kQzLeast = 1.17549435e-38f;      // 2^-126
+constexpr float kQzMagic = 12582912.0f;          // 1.5 * 2^23: a sum with it is rounded to a whole number, which the low bits hold
 
 struct QuantiseArgs {
     const void* x;
@@ -23,57 +26,69 @@ struct QuantiseArgs {
     int T, K;
 };
 
-__device__ __forceinline__ int qz_code(float x, float inv, float scale) {
-    constexpr float magic = 12582912.0f;         // 1.5 * 2^23: a sum with it is rounded to a whole number, which the low bits hold
-    const float r = x * inv, whole = r + magic, rest = fabsf(r - (whole - magic));
-    if (rest > 0.5f - 6.103515625e-05f) return __float_as_int(__fdiv_rn(x, scale) + magic);
-    return __float_as_int(whole);
-}
 __device__ __forceinline__ uint32_t qz_pack(int a, int b, int c, int d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-
-// value j of thread i of a row: eight neighbours (bf16) or four (fp32) to a load where rows allow that (kVec), else every blockDim.x-th value
-template <bool kBf16, bool kVec>
-__global__ void __launch_bounds__(kQzThreads) quantise_rows_kernel(QuantiseArgs p) {
-    after_previous();
-    __shared__ uint32_t s_top[kQzThreads / 32];
-    constexpr int kRun = !kVec ? 1 : kBf16 ? 8 : 4;
-    const int row = blockIdx.x * blockDim.y + threadIdx.y, i = threadIdx.x, n = blockDim.x, per = n * kQzValues;
-    const bool live = row < p.T;
-    const size_t from = (size_t)(live ? row : 0) * p.ldx;
-    float v[kQzValues];
-    auto column = [&](int base, int j) { return base + (j / kRun * n + i) * kRun + j % kRun; };
-    auto load = [&](int base) {
+template <int N>
+__device__ __forceinline__ void qz_codes(const float (&x)[N], float inv, float scale, int (&q)[N]) {
+    float near = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kQzValues; j += kRun) {
-            const int c = column(base, j);
-            const bool take = live && c < p.K;
-            if constexpr (kRun == 8) {
-                const uint4 q = take ? ld_stream(reinterpret_cast<const uint16_t*>(p.x) + from + c) : make_uint4(0u, 0u, 0u, 0u);
-                v[j] = bf16_lo(q.x); v[j + 1] = bf16_hi(q.x); v[j + 2] = bf16_lo(q.y); v[j + 3] = bf16_hi(q.y);
-                v[j + 4] = bf16_lo(q.z); v[j + 5] = bf16_hi(q.z); v[j + 6] = bf16_lo(q.w); v[j + 7] = bf16_hi(q.w);
-            } else if constexpr (kRun == 4) {
-                const uint4 q = take ? ld_stream(reinterpret_cast<const float*>(p.x) + from + c) : make_uint4(0u, 0u, 0u, 0u);
-                v[j] = __uint_as_float(q.x); v[j + 1] = __uint_as_float(q.y); v[j + 2] = __uint_as_float(q.z); v[j + 3] = __uint_as_float(q.w);
-            } else if constexpr (kBf16) {
-                v[j] = take ? seq_ld(reinterpret_cast<const uint16_t*>(p.x), from + c) : 0.0f;
-            } else {
-                v[j] = take ? reinterpret_cast<const float*>(p.x)[from + c] : 0.0f;
-            }
+    for (int e = 0; e < N; ++e) {
+        const float r = x[e] * inv, whole = r + kQzMagic;
+        near = fmaxf(near, fabsf(r - (whole - kQzMagic)));
+        q[e] = __float_as_int(whole);
+    }
+    if (near > 0.5f - 6.103515625e-05f) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) q[e] = __float_as_int(__fdiv_rn(x[e], scale) + kQzMagic);
+    }
+}
+// the floats of a load: eight bf16 or four fp32 values
+__device__ __forceinline__ void qz_floats(const uint4& v, float (&x)[8]) {
+    x[0] = bf16_lo(v.x); x[1] = bf16_hi(v.x); x[2] = bf16_lo(v.y); x[3] = bf16_hi(v.y); x[4] = bf16_lo(v.z); x[5] = bf16_hi(v.z); x[6] = bf16_lo(v.w); x[7] = bf16_hi(v.w);
+}
+__device__ __forceinline__ void qz_floats(const uint4& v, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+}
+
+// blockDim.x threads a row, blockDim.y rows. kVec: rows start at multiples of 16 bytes and are a number of whole loads; else a "load" is one value
+template <bool kBf16, bool kVec, int kMost, int kLoads>
+__global__ void __launch_bounds__(kMost) quantise_rows_kernel(QuantiseArgs p) {
+    after_previous();
+    __shared__ uint32_t s_top[kMost / 32];
+    constexpr int kRun = !kVec ? 1 : kBf16 ? 8 : 4;
+    const int row = blockIdx.x * blockDim.y + threadIdx.y, i = threadIdx.x, n = blockDim.x, per = n * kLoads * kRun;
+    const bool live = row < p.T;
+    const size_t from = (size_t)(live ? row : p.T - 1) * p.ldx;
+    uint4 v[kLoads];
+    auto load = [&](int base) {              // every address is inside the row, so that nothing is asked before a load; what is behind the end counts as the value that is there
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const size_t c = from + min(base + (j * n + i) * kRun, p.K - kRun);
+            if constexpr (kVec) v[j] = kBf16 ? ld_stream(reinterpret_cast<const uint16_t*>(p.x) + c) : ld_stream(reinterpret_cast<const float*>(p.x) + c);
+            else v[j].x = kBf16 ? (uint32_t)reinterpret_cast<const uint16_t*>(p.x)[c] << 16 : __float_as_uint(reinterpret_cast<const float*>(p.x)[c]);
         }
     };
     uint32_t top = 0;
     for (int base = 0; base < p.K; base += per) {
         load(base);
 #pragma unroll
-        for (int j = 0; j < kQzValues; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+        for (int j = 0; j < kLoads; ++j) {
+            if constexpr (!kVec) {
+                top = max(top, v[j].x & 0x7fffffffu);
+            } else {
+                const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = kBf16 ? max(top, max(w[e] << 16 & 0x7fff0000u, w[e] & 0x7fff0000u)) : max(top, w[e] & 0x7fffffffu);
+            }
+        }
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    if (n > 32) {
+    if (n > 32) {                            // the row's warps, by a barrier of their own where the CTA has several rows
         const int warp = (threadIdx.y * n + i) >> 5, first = threadIdx.y * n >> 5;
         if ((i & 31) == 0) s_top[warp] = top;
-        __syncthreads();
+        if (blockDim.y == 1) __syncthreads();
+        else asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(n) : "memory");
         for (int w = 0; w < n / 32; ++w) top = max(top, s_top[first + w]);
     }
     if (!live) return;
@@ -84,12 +99,14 @@ __global__ void __launch_bounds__(kQzThreads) quantise_rows_kernel(QuantiseArgs 
     for (int base = 0; base < p.K; base += per) {
         if (p.K > per) load(base);
 #pragma unroll
-        for (int j = 0; j < kQzValues; j += kRun) {
-            const int c = column(base, j);
-            if (c >= p.K) continue;
-            int q[kRun];
-#pragma unroll
-            for (int e = 0; e < kRun; ++e) q[e] = finite ? qz_code(v[j + e], inv, scale) : 0;
+        for (int j = 0; j < kLoads; ++j) {
+            const int c = base + (j * n + i) * kRun;
+            if (c >= p.K) break;
+            float x[kRun];
+            int q[kRun] = {};
+            if constexpr (kVec) qz_floats(v[j], x);
+            else x[0] = __uint_as_float(v[j].x);
+            if (finite) qz_codes(x, inv, scale, q);
             if constexpr (kRun == 8) *reinterpret_cast<uint2*>(to + c) = make_uint2(qz_pack(q[0], q[1], q[2], q[3]), qz_pack(q[4], q[5], q[6], q[7]));
             else if constexpr (kRun == 4) *reinterpret_cast<uint32_t*>(to + c) = qz_pack(q[0], q[1], q[2], q[3]);
             else to[c] = (int8_t)q[0];
@@ -387,19 +404,30 @@ extern "C" {
 
 int sllm_seq_quantise_rows(const void* x, int32_t x_bf16, int64_t ldx, void* codes, int64_t ldc, float* scales, int32_t T, int32_t K, sllm_stream_t stream) {
     SLLM_REQUIRE(x && codes && scales && T > 0 && K > 0, SLLM_EINVAL, "seq_quantise_rows: null pointer, no rows or no columns");
+    SLLM_REQUIRE(K <= 1 << 30, SLLM_ENOTSUP, "seq_quantise_rows: %d columns", K);
     SLLM_REQUIRE(ldx >= K && ldc >= K, SLLM_EINVAL, "seq_quantise_rows: rows of %d values lie %lld and %lld apart", K, (long long)ldx, (long long)ldc);
     const int size = x_bf16 ? 2 : 4, run = x_bf16 ? 8 : 4;
     SLLM_REQUIRE((uintptr_t)x % size == 0, SLLM_EINVAL, "seq_quantise_rows: values are not aligned");
     const bool vec = K % run == 0 && ldx % run == 0 && ((uintptr_t)x % 16) == 0 && ldc % run == 0 && ((uintptr_t)codes % run) == 0;
     QuantiseArgs p{x, (int8_t*)codes, scales, ldx, ldc, T, K};
-    // threads of a row: enough to keep it in registers; short rows share a CTA
-    const int threads = std::min(kQzThreads, std::max(32, (K + kQzValues - 1) / kQzValues + 31) / 32 * 32), rows = std::max(1, 128 / threads);
+    // threads of a row: where there are rows enough, as few as keep it in registers, so that each has eight loads on their way; else four times as many. us, few | many: 14336 rows of 4096 in bf16
+    // QZA, one row of 4096 in fp32 QZB
+    const int loads = vec ? K / run : K;
+    const bool many = (long long)T * loads >= 4096LL * sm_count();
+    const int each = many ? kQzLoads : kQzFewLoads, threads = (std::min(kQzWide, (loads + each - 1) / each) + 31) / 32 * 32, rows = threads >= kQzThreads ? 1 : kQzThreads / threads;
     const dim3 grid((T + rows - 1) / rows), block(threads, rows);
     cudaStream_t st = as_stream(stream);
-    if (x_bf16 && vec) overlapping(quantise_rows_kernel<true, true>)<<<grid, block, 0, st>>>(p);
-    else if (x_bf16) overlapping(quantise_rows_kernel<true, false>)<<<grid, block, 0, st>>>(p);
-    else if (vec) overlapping(quantise_rows_kernel<false, true>)<<<grid, block, 0, st>>>(p);
-    else overlapping(quantise_rows_kernel<false, false>)<<<grid, block, 0, st>>>(p);
+    auto launch = [&](auto bf16, auto whole) {
+        if (!many) overlapping(quantise_rows_kernel<bf16.value, whole.value, kQzWide, kQzFewLoads>)<<<grid, block, 0, st>>>(p);
+        else if (threads > kQzThreads) overlapping(quantise_rows_kernel<bf16.value, whole.value, kQzWide, kQzLoads>)<<<grid, block, 0, st>>>(p);
+        else overlapping(quantise_rows_kernel<bf16.value, whole.value, kQzThreads, kQzLoads>)<<<grid, block, 0, st>>>(p);
+    };
+    using yes = std::true_type;
+    using no = std::false_type;
+    if (x_bf16 && vec) launch(yes{}, yes{});
+    else if (x_bf16) launch(yes{}, no{});
+    else if (vec) launch(no{}, yes{});
+    else launch(no{}, no{});
     ++g_launches;
     SLLM_LAUNCH_CHECK();
     return SLLM_OK;
