@@ -8,13 +8,19 @@
 // bound (hundreds of equal logits, nearly everything banned) are searched `top` times for the next one instead. Nothing depends on the order of threads but the fp32 sums' fixed tree.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "seq_common.cuh"
 
 namespace sllm {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpValues = 32, kLpChunk = kLpThreads * kLpValues, kLpCluster = 8;
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpCluster = 8;
+#ifndef LPV
+#define LPV 32
+#endif
+constexpr int kLpMany = LPV;
 constexpr int kLpTop = 32, kLpFew = 1024;        // alternatives at most; logits that are put in order by counting
 constexpr float kLpLog2e = 1.4426950408889634f;
 
@@ -43,6 +49,20 @@ __device__ __forceinline__ float lp_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float lp_max3(float a, float b, float c) {    // NaN if one of them is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// two fp32 operations at once, each rounded as the single one
+__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) { uint64_t d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ uint64_t lp_mul2(uint64_t a, uint64_t b) { uint64_t d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ void lp_split(uint64_t v, float& lo, float& hi) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    lo = __uint_as_float(a);
+    hi = __uint_as_float(b);
+}
 
 // The sum of exp(x - M) over all logits but those that are M, and of the same times (x - M); how many are M; logits in front of the token.
 struct LpSums {
@@ -51,14 +71,14 @@ struct LpSums {
 };
 
 struct alignas(16) LpShared {
-    uint64_t few[kLpFew], list[kLpTop], next[kLpTop];
+    uint64_t few[kLpFew], list[2][kLpTop];
     uint64_t all[kLpCluster * kLpTop];           // of the first CTA: every CTA's list
     LpSums sums[kLpCluster];                     // and sums
     uint64_t warp64[kLpWarps];
-    float warp_top[kLpWarps], warp_second[kLpWarps], part[2][kLpWarps];
+    float warp_top[2][kLpWarps], warp_second[2][kLpWarps], rest[kLpWarps], spread[kLpWarps];
     int before[kLpWarps], has[kLpWarps];
-    int count;
-    float log_sum;
+    int count[2];
+    float log_sum, largest;
 };
 
 // The sums from one reference to a larger one: the logits that were the largest come in.
@@ -76,9 +96,11 @@ __device__ __forceinline__ void lp_move(float& rest, float& spread, int& has, fl
     has = 0;
 }
 
-template <bool kVec>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(LogprobArgs p) {
+// kValues: logits a thread takes at a time. kVec: rows start at multiples of 16 bytes, four neighbours a load; else every kLpThreads-th logit
+template <bool kVec, int kValues>
+__global__ void __launch_bounds__(kLpThreads, kValues == 32 ? 2 : 3) token_logprobs_kernel(LogprobArgs p) {
     after_previous();
+    constexpr int kGroup = 4 * kLpThreads, kGroups = kValues / 4;        // four of a thread's logits, and the CTA's neighbouring ones with them
     __shared__ LpShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.barrier_arrive();
@@ -89,122 +111,138 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(LogprobAr
     const bool known = tok >= 0 && tok < p.n;
     const float mine = known ? x[tok] : NAN;
     // logits in front of the token: those above a bound, which for indices before the token's is the next float below
-    const bool plain = known && mine == mine;
-    const float just_below = !plain || mine == -INFINITY ? mine : mine == 0.0f ? -1.4012984643e-45f : __uint_as_float(__float_as_uint(mine) + (mine > 0.0f ? -1 : 1));
+    const bool plain = known && mine == mine && mine != -INFINITY;
+    const float just_below = mine == 0.0f ? -1.4012984643e-45f : __uint_as_float(__float_as_uint(mine) + (mine > 0.0f ? -1 : 1));
     const int lo = min(p.n, rank * p.slice), hi = min(p.n, lo + p.slice);
-    const int second = p.top > kLpWarps;         // two logits of every warp are needed for `top` of them
+    const bool second = p.top > kLpWarps;        // two logits of every warp are needed for `top` of them
     float largest = -INFINITY, rest = 0.0f, spread = 0.0f;
-    int before = 0, has = 0, listed = 0;
-    if (tid < kLpTop) sh.list[tid] = 0;
-    for (int at = lo; at < hi; at += kLpChunk) {
-        const int groups = (min(hi - at, kLpChunk) + 4 * kLpThreads - 1) / (4 * kLpThreads);
-        auto index = [&](int k, int e) { return kVec ? at + (k * kLpThreads + tid) * 4 + e : at + (4 * k + e) * kLpThreads + tid; };
-        float v[kLpValues];
+    int before = 0, has = 0, listed = 0, turn = 0;
+    if (tid < kLpTop) sh.list[0][tid] = sh.list[1][tid] = 0;
+    if (tid < 2) sh.count[tid] = 0;
+    for (int at = lo; at < hi; at += kLpThreads * kValues, turn ^= 1) {
+        auto index = [&](int k, int e) { return kVec ? at + k * kGroup + tid * 4 + e : at + k * kGroup + e * kLpThreads + tid; };
+        float v[kValues];
+        // every address is one of the row's, so that nothing is asked before a load (behind a condition each waited for the one before); what is behind the end is replaced afterwards
 #pragma unroll
-        for (int k = 0; k < kLpValues / 4; ++k) {
-            if (kVec && index(k, 3) < hi) {
-                const uint4 q = ld_stream(x + index(k, 0));
+        for (int k = 0; k < kGroups; ++k) {
+            if constexpr (kVec) {
+                const uint4 q = ld_stream(x + min(index(k, 0), (hi & ~3) - 4));
                 v[4 * k] = __uint_as_float(q.x); v[4 * k + 1] = __uint_as_float(q.y); v[4 * k + 2] = __uint_as_float(q.z); v[4 * k + 3] = __uint_as_float(q.w);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * k + e] = k < groups && index(k, e) < hi ? x[index(k, e)] : -INFINITY;
+                for (int e = 0; e < 4; ++e) v[4 * k + e] = x[min(index(k, e), hi - 1)];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+            if (at + (k + 1) * kGroup <= hi) continue;
+            const bool part = kVec && index(k, 0) < hi && index(k, 3) >= hi;                 // the row's last one to three
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (index(k, e) >= hi) v[4 * k + e] = -INFINITY;
+                else if (part) v[4 * k + e] = x[index(k, e)];
             }
         }
         float own = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kLpValues; ++k) own = fmaxf(own, v[k]);
+        for (int k = 0; k < kValues; k += 2) own = lp_max3(own, v[k], v[k + 1]);
+        if (own != own) rest = own;              // NaN: so are this row's sums
         const float top = warp_max(own);
-        const unsigned who = __ballot_sync(0xffffffffu, own == top);
-        const float below = second ? warp_max(who && lane == __ffs(who) - 1 ? -INFINITY : own) : top;
-        __syncthreads();                         // the last turn's readers are through
+        float below = top;
+        if (second) below = warp_max(lane == __ffs(__ballot_sync(0xffffffffu, own == top)) - 1 ? -INFINITY : own);
         if (lane == 0) {
-            sh.warp_top[warp] = top;
-            sh.warp_second[warp] = below;
+            sh.warp_top[turn][warp] = top;
+            sh.warp_second[turn][warp] = below;
         }
-        if (tid == 0) sh.count = 0;
         __syncthreads();
-        float m = largest, bound = INFINITY;
-#pragma unroll
-        for (int w = 0; w < kLpWarps; ++w) {
-            m = fmaxf(m, sh.warp_top[w]);
-            bound = fminf(bound, sh.warp_second[w]);
-        }
+        const float m = fmaxf(largest, warp_max(sh.warp_top[turn][lane & (kLpWarps - 1)]));
+        float bound = -warp_max(-sh.warp_second[turn][lane & (kLpWarps - 1)]);
         lp_move(rest, spread, has, largest, m);
         largest = m;
-        const float ref = m == -INFINITY ? 0.0f : m;
-        auto add = [&](float y) {                // -infinity adds nothing, NaN makes everything NaN
-            const float z = y - ref, e = lp_exp2(z * kLpLog2e);
-            rest += e;
-            spread = fmaf(e, fmaxf(z, -300.0f), spread);
-        };
-        if (own == m) {                          // few threads: the others need not look
+        if (p.top > 0) {
+            if (listed == p.top) bound = fmaxf(bound, lp_value(sh.list[turn][p.top - 1]));
 #pragma unroll
-            for (int k = 0; k < kLpValues; ++k) {
-                if (v[k] == m) ++has;
-                else add(v[k]);
+            for (int k = 0; k < kGroups; ++k) {
+                if (!(fmaxf(fmaxf(v[4 * k], v[4 * k + 1]), fmaxf(v[4 * k + 2], v[4 * k + 3])) >= bound)) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (v[4 * k + e] >= bound && index(k, e) < hi) {
+                        const int to = atomicAdd(&sh.count[turn], 1);
+                        if (to < kLpFew) sh.few[to] = lp_entry(v[4 * k + e], index(k, e));
+                    }
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < kLpValues; ++k) add(v[k]);
         }
         if (plain) {
 #pragma unroll
-            for (int k = 0; k < kLpValues / 4; ++k) {
-                if (kVec) {
-                    const float above = index(k, 3) < tok ? just_below : mine;
+            for (int k = 0; k < kGroups; ++k) {
+                const int first = at + k * kGroup;
+                if (first + kGroup <= tok || first > tok) {              // a group before the token or behind it
+                    const float above = first > tok ? mine : just_below;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) before += v[4 * k + e] > above;
-                    if (index(k, 0) < tok && index(k, 3) >= tok) {
-#pragma unroll
-                        for (int e = 0; e < 3; ++e) before += index(k, e) < min(tok, hi) && v[4 * k + e] == mine;
-                    }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) before += v[4 * k + e] > mine || (v[4 * k + e] == mine && index(k, e) < min(tok, hi));
+                    for (int e = 0; e < 4; ++e) before += v[4 * k + e] > mine || (v[4 * k + e] == mine && index(k, e) < tok);
                 }
             }
-            if (kVec && mine == -INFINITY) {     // nothing is below it: equal ones are counted one by one
+        } else if (known) {                      // -infinity, behind which there is NaN alone; NaN, behind which there is nothing
 #pragma unroll
-                for (int k = 0; k < kLpValues; ++k) before += index(k / 4, k % 4) < min(hi, tok) && index(k / 4, 3) < tok && v[k] == mine;
+            for (int k = 0; k < kValues; ++k) {
+                const int i = index(k / 4, k % 4);
+                before += i < hi && (mine == mine ? v[k] > mine || (v[k] == mine && i < tok) : v[k] == v[k] || i < tok);
             }
-        } else if (known) {                      // NaN comes behind everything else
-#pragma unroll
-            for (int k = 0; k < kLpValues; ++k) before += index(k / 4, k % 4) < hi && (v[k] == v[k] || index(k / 4, k % 4) < tok);
         }
+        // sums. A thread that has one of the largest leaves it out
+        const float ref = m == -INFINITY ? 0.0f : m;
+        if (own == m) {
+#pragma unroll
+            for (int k = 0; k < kValues; ++k) {
+                if (v[k] == m) {
+                    ++has;
+                    v[k] = -INFINITY;
+                }
+            }
+        }
+        uint64_t rest2 = 0, spread2 = 0;
+        const uint64_t ref2 = pair_f32(-ref, -ref), log2e2 = pair_f32(kLpLog2e, kLpLog2e);
+#pragma unroll
+        for (int k = 0; k < kValues; k += 2) {   // -infinity adds nothing
+            float z0, z1, t0, t1;
+            lp_split(lp_add2(pair_f32(v[k], v[k + 1]), ref2), z0, z1);
+            const uint64_t z = pair_f32(fmaxf(z0, -300.0f), fmaxf(z1, -300.0f));
+            lp_split(lp_mul2(z, log2e2), t0, t1);
+            const uint64_t e = pair_f32(lp_exp2(t0), lp_exp2(t1));
+            rest2 = lp_add2(rest2, e);
+            fma_pair(spread2, e, z);
+        }
+        rest += pair_sum(rest2);
+        spread += pair_sum(spread2);
         if (p.top == 0) continue;
-        if (listed == p.top) bound = fmaxf(bound, lp_value(sh.list[p.top - 1]));
-#pragma unroll
-        for (int k = 0; k < kLpValues / 4; ++k) {
-            if (fmaxf(fmaxf(v[4 * k], v[4 * k + 1]), fmaxf(v[4 * k + 2], v[4 * k + 3])) < bound) continue;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (v[4 * k + e] >= bound && index(k, e) < hi) {
-                    const int to = atomicAdd(&sh.count, 1);
-                    if (to < kLpFew) sh.few[to] = lp_entry(v[4 * k + e], index(k, e));
-                }
-        }
         __syncthreads();
-        const int found = sh.count, want = min(p.top, listed + min(hi - at, kLpChunk));
+        const int found = sh.count[turn], want = min(p.top, listed + min(hi - at, kLpThreads * kValues));
+        uint64_t* to = sh.list[turn ^ 1];
         if (found + listed <= kLpFew && found + listed >= want) {
-            if (tid < kLpTop) sh.next[tid] = 0;
-            if (tid < listed) sh.few[found + tid] = sh.list[tid];
-            __syncthreads();
+            if (listed > 0) {
+                if (tid < listed) sh.few[found + tid] = sh.list[turn][tid];
+                __syncthreads();
+            }
             for (int i = tid; i < found + listed; i += kLpThreads) {
                 const uint64_t e = sh.few[i];
                 int ahead = 0;
+#pragma unroll 8
                 for (int j = 0; j < found + listed; ++j) ahead += sh.few[j] > e;
-                if (ahead < p.top) sh.next[ahead] = e;
+                if (ahead < p.top) to[ahead] = e;
             }
-            __syncthreads();
         } else {
+            // (the logits once more: the largest have been taken out)
             uint64_t last = ~0ull;
             for (int i = 0; i < p.top; ++i) {    // the largest one below the last
                 uint64_t best = 0;
-                if (tid < listed && sh.list[tid] < last) best = sh.list[tid];
+                if (tid < listed && sh.list[turn][tid] < last) best = sh.list[turn][tid];
 #pragma unroll
-                for (int k = 0; k < kLpValues; ++k) {
+                for (int k = 0; k < kValues; ++k) {
                     if (index(k / 4, k % 4) >= hi) continue;
-                    const uint64_t e = lp_entry(v[k], index(k / 4, k % 4));
+                    const uint64_t e = lp_entry(own == m && v[k] == -INFINITY ? x[index(k / 4, k % 4)] : v[k], index(k / 4, k % 4));
                     if (e < last && e > best) best = e;
                 }
 #pragma unroll
@@ -216,77 +254,71 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(LogprobAr
                 __syncthreads();
                 best = 0;
                 for (int w = 0; w < kLpWarps; ++w) best = sh.warp64[w] > best ? sh.warp64[w] : best;
-                if (tid == 0) sh.next[i] = best;
+                if (tid == 0) to[i] = best;
                 last = best;                     // 0: there is none left, now or later
                 __syncthreads();
             }
         }
-        if (tid < p.top) sh.list[tid] = sh.next[tid];
         listed = want;
-        __syncthreads();
+        if (at + kLpThreads * kValues < hi) {    // there is another turn
+            __syncthreads();
+            if (tid < kLpTop) sh.list[turn][tid] = 0;
+            if (tid == 0) sh.count[turn] = 0;
+        }
     }
     // this CTA's sums
     rest = warp_sum(rest);
     spread = warp_sum(spread);
-    for (int o = 16; o > 0; o >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-        has += __shfl_xor_sync(0xffffffffu, has, o);
-    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    has = __reduce_add_sync(0xffffffffu, has);
     if (lane == 0) {
-        sh.part[0][warp] = rest;
-        sh.part[1][warp] = spread;
+        sh.rest[warp] = rest;
+        sh.spread[warp] = spread;
         sh.before[warp] = before;
         sh.has[warp] = has;
     }
     __syncthreads();
-    cluster.barrier_wait();    // every CTA of the cluster runs
+    cluster.barrier_wait();                      // every CTA of the cluster runs
     LpShared* first = cluster.map_shared_rank(&sh, 0);
     if (warp == 0) {
-        LpSums s{largest, warp_sum(lane < kLpWarps ? sh.part[0][lane] : 0.0f), warp_sum(lane < kLpWarps ? sh.part[1][lane] : 0.0f), lane < kLpWarps ? sh.before[lane] : 0,
-                 lane < kLpWarps ? sh.has[lane] : 0};
-        for (int o = 16; o > 0; o >>= 1) {
-            s.before += __shfl_xor_sync(0xffffffffu, s.before, o);
-            s.has += __shfl_xor_sync(0xffffffffu, s.has, o);
-        }
+        const bool in = lane < kLpWarps;
+        const LpSums s{largest, warp_sum(in ? sh.rest[lane] : 0.0f), warp_sum(in ? sh.spread[lane] : 0.0f), __reduce_add_sync(0xffffffffu, in ? sh.before[lane] : 0),
+                       __reduce_add_sync(0xffffffffu, in ? sh.has[lane] : 0)};
         if (lane == 0) first->sums[rank] = s;
     }
-    if (tid >= 32 && tid < 32 + p.top) first->all[rank * p.top + tid - 32] = sh.list[tid - 32];
-    cluster.sync();
+    if (tid >= 32 && tid < 32 + p.top) first->all[rank * p.top + tid - 32] = sh.list[turn][tid - 32];
+    if (size == 1) __syncthreads(); else cluster.sync();
     if (rank != 0) return;
-    if (tid == 0) {
-        float m = -INFINITY;
-        for (int i = 0; i < size; ++i) m = fmaxf(m, sh.sums[i].largest);
-        float r = 0.0f, s = 0.0f;
-        int ahead = 0, tops = 0;
-        for (int i = 0; i < size; ++i) {
-            LpSums a = sh.sums[i];
-            lp_move(a.rest, a.spread, a.has, a.largest, m);
-            r += a.rest;
-            s += a.spread;
-            tops += a.has;
-            ahead += a.before;
+    if (warp == 0) {                             // a lane a CTA
+        LpSums a = lane < size ? sh.sums[lane] : LpSums{-INFINITY, 0.0f, 0.0f, 0, 0};
+        const float m = warp_max(a.largest);
+        lp_move(a.rest, a.spread, a.has, a.largest, m);
+        const int tops = __reduce_add_sync(0xffffffffu, a.has), ahead = __reduce_add_sync(0xffffffffu, a.before);
+        const float r = warp_sum(a.rest) + (float)(tops - 1), s = warp_sum(a.spread);
+        if (lane == 0) {
+            float log_sum = log1pf(r), entropy = log_sum - s / (1.0f + r);
+            if (m == -INFINITY) log_sum = entropy = NAN;
+            if (p.entropy) p.entropy[row] = entropy;
+            if (p.rank) p.rank[row] = known ? ahead : -1;
+            if (p.logprob) p.logprob[row] = (mine == m ? 0.0f : mine - m) - log_sum;
+            sh.log_sum = log_sum;
+            sh.largest = m;
         }
-        r += (float)(tops - 1);
-        float log_sum = log1pf(r), entropy = log_sum - s / (1.0f + r);
-        if (m == -INFINITY) log_sum = entropy = NAN;
-        if (p.entropy) p.entropy[row] = entropy;
-        if (p.rank) p.rank[row] = known ? ahead : -1;
-        if (p.logprob) p.logprob[row] = (mine == m ? 0.0f : mine - m) - log_sum;
-        sh.log_sum = log_sum;
-        sh.part[0][0] = m;
+    }
+    if (p.top == 0) return;
+    // of the lists together
+    const int i = tid - 32;
+    const uint64_t e = i >= 0 && i < size * p.top ? sh.all[i] : 0;
+    int ahead = 0;
+    if (e != 0) {
+#pragma unroll 8
+        for (int j = 0; j < size * p.top; ++j) ahead += sh.all[j] > e;
     }
     __syncthreads();
-    const float log_sum = sh.log_sum, m = sh.part[0][0];
-    for (int i = tid; i < size * p.top; i += kLpThreads) {
-        const uint64_t e = sh.all[i];
-        if (e == 0) continue;
-        int ahead = 0;
-        for (int j = 0; j < size * p.top; ++j) ahead += sh.all[j] > e;
-        if (ahead < p.top) {
-            const float z = lp_value(e);
-            p.top_idx[row * p.top + ahead] = lp_index(e);
-            if (p.top_logprob) p.top_logprob[row * p.top + ahead] = (z == m ? 0.0f : z - m) - log_sum;
-        }
+    if (e != 0 && ahead < p.top) {
+        const float z = lp_value(e);
+        p.top_idx[row * p.top + ahead] = lp_index(e);
+        if (p.top_logprob) p.top_logprob[row * p.top + ahead] = (z == sh.largest ? 0.0f : z - sh.largest) - sh.log_sum;
     }
 }
 
@@ -305,11 +337,12 @@ extern "C" int sllm_token_logprobs(const float* logits, int64_t ld, int32_t rows
     SLLM_REQUIRE(logprob || entropy || rank || top, SLLM_EINVAL, "token_logprobs: nothing is asked for");
     // CTAs of a row: as many as leave one no more than it holds in registers, and more while the machine has room and they have 2048 logits each
     int cs = 1;
-    while (cs < kLpCluster && ((n + cs - 1) / cs > kLpChunk || ((long long)rows * cs < 2 * sm_count() && n / cs >= 4096))) cs *= 2;
+    while (cs < kLpCluster && ((n + cs - 1) / cs > 16384 || ((long long)rows * cs < 2 * sm_count() && n / cs >= 4096))) cs *= 2;
     SLLM_REQUIRE((long long)rows * cs <= 0x7fffffffLL, SLLM_ENOTSUP, "token_logprobs: too many rows");
-    const int slice = (int)(((int64_t)n + cs - 1) / cs + 3) / 4 * 4;
+    const int64_t each = ((int64_t)n + cs - 1) / cs;
+    const bool vec = each >= 4 * kLpThreads && ld % 4 == 0 && ((uintptr_t)logits % 16) == 0;
+    const int slice = (int)(vec ? (each + 4 * kLpThreads - 1) / (4 * kLpThreads) * (4 * kLpThreads) : each);      // whole groups: only the last CTA has a part of one
     LogprobArgs p{logits, token, logprob, entropy, top_logprob, rank, top_idx, ld, n, top, slice};
-    const bool vec = slice >= 4 * kLpThreads && ld % 4 == 0 && ((uintptr_t)logits % 16) == 0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * cs));
     cfg.blockDim = dim3(kLpThreads);
@@ -320,8 +353,11 @@ extern "C" int sllm_token_logprobs(const float* logits, int64_t ld, int32_t rows
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (vec) SLLM_CUDA(cudaLaunchKernelEx(&cfg, overlapping(token_logprobs_kernel<true>), p));
-    else SLLM_CUDA(cudaLaunchKernelEx(&cfg, overlapping(token_logprobs_kernel<false>), p));
+    auto launch = [&](auto whole, auto values) { return cudaLaunchKernelEx(&cfg, overlapping(token_logprobs_kernel<whole.value, values.value>), p); };
+    using yes = std::true_type;
+    using no = std::false_type;
+    if (slice <= 8 * kLpThreads) SLLM_CUDA(vec ? launch(yes{}, std::integral_constant<int, 8>{}) : launch(no{}, std::integral_constant<int, 8>{}));
+    else SLLM_CUDA(vec ? launch(yes{}, std::integral_constant<int, kLpMany>{}) : launch(no{}, std::integral_constant<int, kLpMany>{}));
     ++g_launches;
     SLLM_LAUNCH_CHECK();
     return SLLM_OK;
