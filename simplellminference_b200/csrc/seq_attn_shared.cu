@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
 
 static int sh_merge(const SharedArgs& p, cudaStream_t st) {
     const int most = (p.b.T == p.b.nseg ? p.heads : kBQ * p.heads) / 4 + 1;
-    overlapping(seq_attention_shared_merge_kernel)<<<dim3(p.b.n_qtiles, std::min(most, 256)), 128, 0, st>>>(p);
+    LaunchCfg lc(dim3(p.b.n_qtiles, std::min(most, 256)), dim3(128), 0, st, true);
+    SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(seq_attention_shared_merge_kernel), p));
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;

@@ -143,17 +143,7 @@ __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args 
     for (int r = 0; r < kL8Rows; ++r) w[r] = p.w + (size_t)min(n0 + r, p.N - 1) * p.ldw;
 #pragma unroll
     for (int t = 0; t < kT; ++t) a[t] = p.a + (size_t)min(t, p.T - 1) * p.lda;
-#pragma unroll 4
-    for (int c = lane * 16; c < p.K; c += 512) {
-        uint4 x[kL8Rows];
-#pragma unroll
-        for (int r = 0; r < kL8Rows; ++r) x[r] = ld_stream(w[r] + c);
-        if (c + 16 > p.K) {                      // columns behind the last one: whatever the rows hold there does not count
-            const int have = p.K - c;
-            auto keep = [&](uint32_t v, int first) { return have >= first + 4 ? v : have <= first ? 0u : v & ((1u << 8 * (have - first)) - 1); };
-#pragma unroll
-            for (int r = 0; r < kL8Rows; ++r) x[r] = make_uint4(keep(x[r].x, 0), keep(x[r].y, 4), keep(x[r].z, 8), keep(x[r].w, 12));
-        }
+    auto products = [&](const uint4 (&x)[kL8Rows], int c) {
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             const uint4 y = *reinterpret_cast<const uint4*>(a[t] + c);
@@ -161,6 +151,25 @@ __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args 
             for (int r = 0; r < kL8Rows; ++r)
                 sum[r][t] = __dp4a((int)x[r].w, (int)y.w, __dp4a((int)x[r].z, (int)y.z, __dp4a((int)x[r].y, (int)y.y, __dp4a((int)x[r].x, (int)y.x, sum[r][t]))));
         }
+    };
+    const int whole = p.K & ~511;                // up to there every lane has sixteen codes
+#pragma unroll 4
+    for (int c = lane * 16; c < whole; c += 512) {
+        uint4 x[kL8Rows];
+#pragma unroll
+        for (int r = 0; r < kL8Rows; ++r) x[r] = ld_stream(w[r] + c);
+        products(x, c);
+    }
+    if (const int c = whole + lane * 16; c < p.K) {
+        uint4 x[kL8Rows];
+#pragma unroll
+        for (int r = 0; r < kL8Rows; ++r) x[r] = ld_stream(w[r] + c);
+        // columns behind the last one: whatever the rows hold there does not count
+        const int have = p.K - c;
+        auto keep = [&](uint32_t v, int first) { return have >= first + 4 ? v : have <= first ? 0u : v & ((1u << 8 * (have - first)) - 1); };
+#pragma unroll
+        for (int r = 0; r < kL8Rows; ++r) x[r] = make_uint4(keep(x[r].x, 0), keep(x[r].y, 4), keep(x[r].z, 8), keep(x[r].w, 12));
+        products(x, c);
     }
 #pragma unroll
     for (int r = 0; r < kL8Rows; ++r)
@@ -171,11 +180,13 @@ __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args 
         }
 }
 
-// From kL8Few tokens on: tcgen05, products of 8-bit integers with sums in TMEM. The rows of W are the rows of a tile and the tokens its columns, however few there are: a tile is 128 rows of W by up
+// Above kL8Few tokens: tcgen05, products of 8-bit integers with sums in TMEM. The rows of W are the rows of a tile and the tokens its columns, however few there are: a tile is 128 rows of W by up
 // to 256 tokens, and the results of a token, neighbours in memory, lie in neighbouring lanes of a warp.
 //   warp 0 (one lane)  TMA producer: 128 bytes of K of the rows and of the tokens a stage (zeros behind the last of either);
 //   warp 1 (one lane)  MMA issuer, four products of 32 values of K a stage;
 //   warps 2-5          the sums out of TMEM, scales and bias, rows out, while the issuer fills the second accumulator.
+// Where there are many tiles (kPair), the two SMs of a pair share one of 256 rows by up to 256 tokens, each with 128 rows and half of the tokens: what a stage brings in from L2 is what bounds
+// one SM (48 KB for the 512 clocks of its products; 32 KB like this).
 // Where rows and tokens make fewer tiles than the machine has SMs, a cluster shares a tile: its CTAs take a part of K each, leave their sums in shared memory and add up a part of the tokens each
 // (whole numbers: the order does not matter).
 constexpr int kL8TcThreads = 192, kL8Block = 128, kL8Stages = 12;
@@ -186,100 +197,105 @@ struct Linear8Tc {
     Linear8Args a;
     int bn, t_tiles, units, blocks, stages, split, cols;      // tokens of a tile; tiles of tokens and in all; blocks of K; CTAs of a tile; TMEM columns of an accumulator
     int32_t* status;
-    unsigned polls;
+    long long wait_clocks;
 };
 
 __device__ __forceinline__ int l8_peer(const void* local, uint32_t cta) {      // a word of another CTA of the cluster
-    uint32_t at;
     int v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(s_addr(local)), "r"(cta));
-    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(local, cta)) : "memory");
     return v;
 }
-__device__ __forceinline__ void l8_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
+template <bool kPair>
 __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const Linear8Tc p) {
     after_previous();        // in front of the allocation of TMEM: a CTA that waits for another kernel must not hold what that kernel's CTAs may be waiting for
     extern __shared__ uint8_t l8_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(l8_raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t a_bytes = (uint32_t)p.bn * kL8Block, stage_bytes = kL8RowBytes + a_bytes;
+    constexpr int kRows = kPair ? 256 : 128;
+    const int a_rows = kPair ? p.bn / 2 : p.bn;              // tokens that this CTA brings in
+    const uint32_t stage_bytes = kL8RowBytes + (uint32_t)a_rows * kL8Block;
     const int ST = p.stages;
     uint64_t *full = reinterpret_cast<uint64_t*>(smem + kL8Ring), *empty = full + kL8Stages, *tfull = empty + kL8Stages, *tempty = tfull + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = kPair ? cluster_ctarank() : 0u;    // 0 issues the pair's products
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tmW);
         tma_prefetch_desc(&tmA);
         for (int i = 0; i < ST; ++i) { mb_init(full + i, 1); mb_init(empty + i, 1); }
-        for (int i = 0; i < 2; ++i) { mb_init(tfull + i, 1); mb_init(tempty + i, 4); }
-        *gave_up = 0;
+        for (int i = 0; i < 2; ++i) { mb_init(tfull + i, 1); mb_init(tempty + i, kPair ? 8 : 4); }
+        *gave_up = p.wait_clocks == 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tc_alloc(tmem_slot, 2 * p.cols);
+    if (kPair) cluster_sync_all();       // the pair's forms of alloc and dealloc act on both CTAs: whoever issues one has to know that the peer runs (and, at the end, that it is still there)
+    if (warp == 1) { if (kPair) tc_alloc_pair(tmem_slot, 2 * p.cols); else tc_alloc(tmem_slot, 2 * p.cols); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int part = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, step = (int)gridDim.x / p.split;
+    const int group = kPair ? 2 : p.split, part = kPair ? 0 : (int)blockIdx.x % p.split, first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
     const int k0 = p.blocks * part / p.split, k1 = p.blocks * (part + 1) / p.split;
     if (warp == 0) {
         if (elect_one()) {
+            const uint32_t full_at = kPair ? mapa_u32(full, 0) : s_addr(full), ring = s_addr(smem);      // pair: both CTAs' bytes are counted on the first one's barriers
             int stage = 0;
             uint32_t phase = 0;
-            bool ok = true;
+            bool ok = p.wait_clocks != 0;
             for (int unit = first; ok && unit < p.units; unit += step) {
-                const int n0 = unit / p.t_tiles * 128, t0 = unit % p.t_tiles * p.bn;
+                const int n0 = unit / p.t_tiles * kRows + (int)rank * 128, t0 = unit % p.t_tiles * p.bn + (int)rank * a_rows;
                 for (int k = k0; k < k1; ++k) {
-                    ok = tc_wait(empty + stage, phase ^ 1, gave_up, p.polls);
+                    ok = pf_wait<kPair>(empty + stage, phase ^ 1, gave_up, p.wait_clocks);
                     if (!ok) break;
-                    uint8_t* at = smem + (uint32_t)stage * stage_bytes;
-                    mb_expect(full + stage, stage_bytes);
-                    tma_load_2d(at, &tmW, k * kL8Block, n0, full + stage);
-                    tma_load_2d(at + kL8RowBytes, &tmA, k * kL8Block, t0, full + stage);
+                    const uint32_t at = ring + (uint32_t)stage * stage_bytes, bar = full_at + 8 * stage;
+                    if (!kPair) mb_expect(full + stage, stage_bytes);
+                    else if (rank == 0) mb_expect(full + stage, 2 * stage_bytes);
+                    pf_load_2d<kPair>(at, &tmW, k * kL8Block, n0, bar);
+                    pf_load_2d<kPair>(at + kL8RowBytes, &tmA, k * kL8Block, t0, bar);
                     if (++stage == ST) { stage = 0; phase ^= 1; }
                 }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (elect_one()) {
-            const uint32_t idesc = umma_idesc_i8(128, p.bn);
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = umma_idesc_i8(kRows, p.bn);
             const uint64_t w_desc = umma_desc_sw128(smem), a_desc = umma_desc_sw128(smem + kL8RowBytes);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
-            bool ok = true;
+            bool ok = p.wait_clocks != 0;
             for (int unit = first; ok && unit < p.units; unit += step) {
-                ok = tc_wait(tempty + acc, acc_phase ^ 1, gave_up, p.polls);
+                ok = pf_wait<kPair>(tempty + acc, acc_phase ^ 1, gave_up, p.wait_clocks);
                 if (!ok) break;
                 tc_fence_after();
                 for (int k = k0; k < k1; ++k) {
-                    ok = tc_wait(full + stage, phase, gave_up, p.polls);
+                    ok = pf_wait<kPair>(full + stage, phase, gave_up, p.wait_clocks);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t off = (uint64_t)((uint32_t)stage * (stage_bytes >> 4));
 #pragma unroll
-                    for (int i = 0; i < kL8Block / 32; ++i) tc_mma_i8(tmem + (uint32_t)(acc * p.cols), w_desc + off + 2 * i, a_desc + off + 2 * i, idesc, k > k0 || i);
-                    tc_commit(empty + stage);
+                    for (int i = 0; i < kL8Block / 32; ++i) {
+                        if (kPair) tc_mma_i8_pair(tmem + (uint32_t)(acc * p.cols), w_desc + off + 2 * i, a_desc + off + 2 * i, idesc, k > k0 || i);
+                        else tc_mma_i8(tmem + (uint32_t)(acc * p.cols), w_desc + off + 2 * i, a_desc + off + 2 * i, idesc, k > k0 || i);
+                    }
+                    if (kPair) tc_commit_pair(empty + stage); else tc_commit(empty + stage);
                     if (++stage == ST) { stage = 0; phase ^= 1; }
                 }
                 if (!ok) break;
-                tc_commit(tfull + acc);
+                if (kPair) tc_commit_pair(tfull + acc); else tc_commit(tfull + acc);
                 if (++acc == 2) { acc = 0; acc_phase ^= 1; }
             }
         }
         __syncwarp();
     } else {
         const int quad = warp & 3;
+        const uint32_t drained[2] = {kPair ? mapa_u32(tempty, 0) : 0u, kPair ? mapa_u32(tempty + 1, 0) : 0u};
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int unit = first; unit < p.units; unit += step) {
-            if (!tc_wait_warp(tfull + acc, acc_phase, gave_up, p.polls)) break;
+        for (int unit = first; p.wait_clocks != 0 && unit < p.units; unit += step) {
+            if (!__all_sync(0xffffffffu, pf_wait<kPair>(tfull + acc, acc_phase, gave_up, p.wait_clocks))) break;
             tc_fence_after();
-            const int n = unit / p.t_tiles * 128 + quad * 32 + lane, t0 = unit % p.t_tiles * p.bn;
+            const int n = unit / p.t_tiles * kRows + (int)rank * 128 + quad * 32 + lane, t0 = unit % p.t_tiles * p.bn;
             const bool live = n < p.a.N;
             const float ws = live ? p.a.w_scale[n] : 0.0f, bias = live && p.a.bias ? p.a.bias[n] : 0.0f;
             const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * p.cols);
@@ -291,7 +307,7 @@ __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __gri
                 if (c + 32 >= p.bn) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mb_arrive(tempty + acc);
+                    if (lane == 0) { if (kPair) mb_arrive_cluster(drained[acc]); else mb_arrive(tempty + acc); }
                 }
                 if (p.split > 1) {               // (every stage has been read: the ring is free)
 #pragma unroll
@@ -315,9 +331,9 @@ __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __gri
         }
         __syncwarp();
     }
-    if (p.split > 1) {                           // one tile a cluster
-        l8_cluster_sync();
-        const int unit = first, n = unit / p.t_tiles * 128 + (warp & 3) * 32 + lane, t0 = unit % p.t_tiles * p.bn;
+    if (!kPair && p.split > 1) {                 // one tile a cluster
+        cluster_sync_all();
+        const int n = first / p.t_tiles * 128 + (warp & 3) * 32 + lane, t0 = first % p.t_tiles * p.bn;
         if (warp >= 2 && n < p.a.N) {
             for (int j = part; j < p.bn && t0 + j < p.a.T; j += p.split) {
                 int sum = 0;
@@ -325,72 +341,81 @@ __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __gri
                 l8_store(p.a, t0 + j, n, sum);
             }
         }
-        l8_cluster_sync();                       // nobody leaves while its sums are being read
+        cluster_sync_all();                      // nobody leaves while its sums are being read
     }
     tc_fence_before();
-    __syncthreads();
+    if (kPair) cluster_sync_all(); else __syncthreads();      // pair: nobody leaves while the peer may still signal its barriers or read its operands
     if (*gave_up) tc_gave_up(p.status);
     if (warp == 1) {
         tc_fence_after();
-        tc_dealloc(tmem, 2 * p.cols);
+        if (kPair) tc_dealloc_pair(tmem, 2 * p.cols); else tc_dealloc(tmem, 2 * p.cols);
     }
+    if (kPair) cluster_sync_all();
 }
 
-// Tokens of a tile and CTAs that share one: the cheapest of all, a stage reckoned at what its products or its bytes take (clocks), a wave of tiles at its beginning and end beside its stages.
-struct Linear8Plan { int bn, split; };
+// Tokens of a tile, SMs (or CTAs of K) that share one: the cheapest of all, a stage reckoned at what its products or its bytes take (clocks), a wave of tiles at its beginning and end beside its
+// stages. us without and with pairs, the rows' quantisation aside: 2000 x 4096 x 14336 90 | L8A.
+struct Linear8Plan { int bn, split, pair; };
 static Linear8Plan l8_plan(int T, int N, int K) {
-    const int sms = sm_count(), w_tiles = (N + 127) / 128, blocks = (K + kL8Block - 1) / kL8Block, most = std::min(256, (T + 15) / 16 * 16);
-    Linear8Plan best{16, 1};
+    const int sms = sm_count(), blocks = (K + kL8Block - 1) / kL8Block, most = std::min(256, (T + 15) / 16 * 16);
+    Linear8Plan best{16, 1, 0};
     double least = 1e30;
-    for (int bn = 16; bn <= most; bn += 16)
-        for (int split = 1; split <= 8 && split <= blocks; split *= 2) {
-            if (split > 1 && bn > 128) break;
-            const double units = (double)w_tiles * ((T + bn - 1) / bn), waves = (double)(((long long)units * split + sms - 1) / sms);
-            const double stage = std::max(2.0 * bn, (kL8RowBytes + bn * kL8Block) / 50.0);
-            const double cost = waves * (((blocks + split - 1) / split) * stage + (split > 1 ? 4000.0 : 1500.0 + 4.0 * bn));
-            if (cost < least - 1e-9) { least = cost; best = {bn, split}; }
-        }
+    for (int pair = 0; pair < 2; ++pair)
+        for (int bn = pair ? 32 : 16; bn <= (pair ? std::min(256, (T + 31) / 32 * 32) : most); bn += pair ? 32 : 16)
+            for (int split = 1; split <= (pair ? 1 : 8) && split <= blocks; split *= 2) {
+                if (split > 1 && bn > 128) break;
+                const long long units = (long long)((N + (pair ? 255 : 127)) / (pair ? 256 : 128)) * ((T + bn - 1) / bn) * split, workers = pair ? sms / 2 : sms;
+                const double stage = std::max(2.0 * bn, (kL8RowBytes + (pair ? bn / 2 : bn) * kL8Block) / 60.0);
+                const double cost = (double)((units + workers - 1) / workers) * (((blocks + split - 1) / split) * stage + (split > 1 ? 4000.0 : 1500.0 + 4.0 * bn));
+                if (cost < least - 1e-9) { least = cost; best = {bn, split, pair}; }
+            }
     return best;
 }
 
 static int l8_tc(const Linear8Args& a, cudaStream_t st) {
     static OncePerDevice ready;
     if (int rc = ready([&] {
-            SLLM_CUDA(cudaFuncSetAttribute(linear8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kL8Smem));
+            SLLM_CUDA(cudaFuncSetAttribute(linear8_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kL8Smem));
+            SLLM_CUDA(cudaFuncSetAttribute(linear8_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kL8Smem));
             return SLLM_OK;
         }))
         return rc;
     const Linear8Plan pl = l8_plan(a.T, a.N, a.K);
+    const int rows = pl.pair ? 256 : 128, a_rows = pl.pair ? pl.bn / 2 : pl.bn;
     Linear8Tc p{};
     p.a = a;
     p.bn = pl.bn;
     p.split = pl.split;
     p.t_tiles = (a.T + pl.bn - 1) / pl.bn;
-    const long long units = (long long)((a.N + 127) / 128) * p.t_tiles;
+    const long long units = (long long)((a.N + rows - 1) / rows) * p.t_tiles;
     SLLM_REQUIRE(units * pl.split <= 0x7fffffffLL, SLLM_ENOTSUP, "seq_linear8: %d rows for %d tokens", a.N, a.T);
     p.units = (int)units;
     p.blocks = (a.K + kL8Block - 1) / kL8Block;
-    p.stages = std::min(kL8Stages, kL8Ring / ((int)kL8RowBytes + pl.bn * kL8Block));
+    p.stages = std::min(kL8Stages, kL8Ring / ((int)kL8RowBytes + a_rows * kL8Block));
     p.cols = 32;
     while (p.cols < pl.bn) p.cols *= 2;
     if (int rc = status_check()) return rc;
     if (int rc = status_word(&p.status)) return rc;
-    p.polls = (unsigned)g_tune_tc_polls;
+    p.wait_clocks = kPollClocks * g_tune_tc_polls;
     CUtensorMap tmW, tmA;
     if (int rc = tc_encode_rows(&tmW, a.w, (uint64_t)a.N, a.K, a.ldw, 128)) return rc;
-    if (int rc = tc_encode_rows(&tmA, a.a, (uint64_t)a.T, a.K, a.lda, pl.bn)) return rc;
+    if (int rc = tc_encode_rows(&tmA, a.a, (uint64_t)a.T, a.K, a.lda, a_rows)) return rc;
+    const int workers = pl.pair ? std::max(1, sm_count() / 2) : sm_count(), cluster = pl.pair ? 2 : pl.split;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(pl.split > 1 ? (unsigned)(p.units * pl.split) : (unsigned)std::min(p.units, sm_count()));
+    cfg.gridDim = dim3((unsigned)cluster * (pl.split > 1 ? p.units : std::min(p.units, workers)));
     cfg.blockDim = dim3(kL8TcThreads);
     cfg.dynamicSmemBytes = kL8Smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = pl.split;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pl.split > 1 ? 1 : 0;
-    SLLM_CUDA(cudaLaunchKernelEx(&cfg, overlapping(linear8_tc_kernel), tmW, tmA, p));
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    if (pl.pair) SLLM_CUDA(cudaLaunchKernelEx(&cfg, overlapping(linear8_tc_kernel<true>), tmW, tmA, p));
+    else SLLM_CUDA(cudaLaunchKernelEx(&cfg, overlapping(linear8_tc_kernel<false>), tmW, tmA, p));
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
@@ -442,11 +467,10 @@ int sllm_seq_linear8(const void* a, int64_t lda, const float* a_scale, const voi
     Linear8Args p{(const int8_t*)a, (const int8_t*)w, a_scale, w_scale, bias, C, lda, ldw, ldc, T, N, K, accumulate != 0};
     cudaStream_t st = as_stream(stream);
     if (T > kL8Few) return l8_tc(p, st);
-    const int per = T > 2 ? kL8Few : T;
-    const dim3 grid((N + kL8Warps * kL8Rows - 1) / (kL8Warps * kL8Rows));
-    if (per == 1) overlapping(linear8_few_kernel<1>)<<<grid, kL8Warps * 32, 0, st>>>(p);
-    else if (per == 2) overlapping(linear8_few_kernel<2>)<<<grid, kL8Warps * 32, 0, st>>>(p);
-    else overlapping(linear8_few_kernel<kL8Few>)<<<grid, kL8Warps * 32, 0, st>>>(p);
+    LaunchCfg lc(dim3((N + kL8Warps * kL8Rows - 1) / (kL8Warps * kL8Rows)), dim3(kL8Warps * 32), 0, st, true);
+    if (T == 1) SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<1>), p));
+    else if (T == 2) SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<2>), p));
+    else SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<kL8Few>), p));
     ++g_launches;
     SLLM_LAUNCH_CHECK();
     return SLLM_OK;
