@@ -123,11 +123,12 @@ struct Linear8Args {
     int T, N, K, accumulate;
 };
 
+// every rounding by itself: a result does not depend on where a compiler contracts, so not on which kernel it comes from
+__device__ __forceinline__ float l8_value(int sum, float s, float w, float bias) { return __fadd_rn(__fmul_rn(__fmul_rn((float)sum, s), w), bias); }
 __device__ __forceinline__ void l8_store(const Linear8Args& p, int t, int n, int sum) {
-    float v = (float)sum * p.a_scale[t] * p.w_scale[n];
-    if (p.bias) v += p.bias[n];
+    const float v = l8_value(sum, p.a_scale[t], p.w_scale[n], p.bias ? p.bias[n] : 0.0f);
     float* to = p.out + (size_t)t * p.ldc + n;
-    *to = p.accumulate ? *to + v : v;
+    *to = p.accumulate ? __fadd_rn(*to, v) : v;
 }
 
 // A warp takes two rows of W and kT tokens: sixteen codes a load, four products an instruction.
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args 
 // (whole numbers: the order does not matter).
 constexpr int kL8TcThreads = 192, kL8Block = 128, kL8Stages = 12;
 constexpr uint32_t kL8RowBytes = 128 * kL8Block;
-constexpr int kL8Ring = 192 * 1024, kL8Smem = 1024 + kL8Ring + 512;
+constexpr int kL8Ring = 192 * 1024, kL8Smem = 1024 + kL8Ring + 512 + 4 * 256 * 4;      // operands, barriers, the tokens' scales for each of the four warps that store
 
 struct Linear8Tc {
     Linear8Args a;
@@ -292,10 +293,15 @@ __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __gri
         const uint32_t drained[2] = {kPair ? mapa_u32(tempty, 0) : 0u, kPair ? mapa_u32(tempty + 1, 0) : 0u};
         int acc = 0;
         uint32_t acc_phase = 0;
+        float* scales = reinterpret_cast<float*>(smem + kL8Ring + 512) + quad * 256;
         for (int unit = first; p.wait_clocks != 0 && unit < p.units; unit += step) {
+            const int t0 = unit % p.t_tiles * p.bn;
+            __syncwarp();
+            for (int i = lane; i < p.bn; i += 32) scales[i] = p.a.a_scale[min(t0 + i, p.a.T - 1)];
+            __syncwarp();
             if (!__all_sync(0xffffffffu, pf_wait<kPair>(tfull + acc, acc_phase, gave_up, p.wait_clocks))) break;
             tc_fence_after();
-            const int n = unit / p.t_tiles * kRows + (int)rank * 128 + quad * 32 + lane, t0 = unit % p.t_tiles * p.bn;
+            const int n = unit / p.t_tiles * kRows + (int)rank * 128 + quad * 32 + lane;
             const bool live = n < p.a.N;
             const float ws = live ? p.a.w_scale[n] : 0.0f, bias = live && p.a.bias ? p.a.bias[n] : 0.0f;
             const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * p.cols);
@@ -314,17 +320,25 @@ __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __gri
                     for (int j = 0; j < 32; ++j)
                         if (c + j < p.bn) reinterpret_cast<int*>(smem)[(c + j) * 128 + quad * 32 + lane] = (int)v[j];
                 } else {
-                    const int t = t0 + c, have = min(32, min(p.bn - c, p.a.T - t));
-                    const float s = lane < have ? p.a.a_scale[t + lane] : 0.0f;
-                    float* to = p.a.out + (size_t)t * p.a.ldc + n;
+                    // (no shuffles between the stores: behind each of them the next one waited, 2000 clocks for the 32)
+                    const int have = live ? min(32, min(p.bn - c, p.a.T - t0 - c)) : 0;
+                    float* to = p.a.out + (size_t)(t0 + c) * p.a.ldc + n;
+                    float y[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float y = (float)(int)v[j] * __shfl_sync(0xffffffffu, s, j) * ws;
-                        if (j >= have || !live) continue;
-                        if (p.a.bias) y += bias;
-                        float* at = to + (size_t)j * p.a.ldc;
-                        *at = p.a.accumulate ? *at + y : y;
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 s = *reinterpret_cast<const float4*>(scales + c + j);
+                        const float t[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[j + e] = l8_value((int)v[j + e], t[e], ws, bias);
                     }
+                    if (p.a.accumulate) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (j < have) y[j] = __fadd_rn(to[(size_t)j * p.a.ldc], y[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j < have) to[(size_t)j * p.a.ldc] = y[j];
                 }
             }
             if (++acc == 2) { acc = 0; acc_phase ^= 1; }

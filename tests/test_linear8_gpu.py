@@ -140,10 +140,11 @@ def test_a_product_does_not_depend_on_the_other_tokens():
     a = torch.randint(-127, 128, (300, 4096), generator=g, dtype=torch.int8).cuda()
     w = torch.randint(-127, 128, (777, 4096), generator=g, dtype=torch.int8).cuda()
     sa, sw = torch.rand(300, generator=g).cuda(), torch.rand(777, generator=g).cuda()
+    bias = torch.randn(777, generator=g).cuda()
     ops, outs = _ops(), {}
     for first, T in ((0, 300), (200, 1), (199, 3), (170, 40), (100, 128)):
         c = torch.zeros(T, 777, device="cuda")
-        ops.linear8(a[first:].data_ptr(), 4096, sa[first:], w, 4096, sw, None, c.data_ptr(), 777, T, 777, 4096, _st())
+        ops.linear8(a[first:].data_ptr(), 4096, sa[first:], w, 4096, sw, bias, c.data_ptr(), 777, T, 777, 4096, _st())
         torch.cuda.synchronize()
         outs[first, T] = c[200 - first].cpu()
     assert all(torch.equal(v, outs[0, 300]) for v in outs.values())
