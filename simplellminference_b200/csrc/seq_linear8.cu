@@ -131,49 +131,50 @@ __device__ __forceinline__ void l8_store(const Linear8Args& p, int t, int n, int
     *to = p.accumulate ? __fadd_rn(*to, v) : v;
 }
 
-// A warp takes two rows of W and kT tokens: sixteen codes a load, four products an instruction.
-constexpr int kL8Warps = 8, kL8Rows = 2, kL8Few = 4;
-template <int kT>
+// One or two tokens: a warp takes kRows rows of W, sixteen codes a load, four products an instruction, eight loads of W on their way. Bound: what those bring in. us, one token, 1 | 2 | 4 rows a warp:
+// 4096 x 4096 5.6 | 6.5 | 8.7, 4096 x 14336 14.7 | 17.8 | 24.5 (3.9 TB/s), 14336 x 4096 14.1 | 13.2 | 12.0 (4.9 TB/s). Two tokens 14.0; four of them 19.5, where tcgen05 takes 13.6.
+constexpr int kL8Warps = 8, kL8Few = 2, kL8Wide = 8192;
+template <int kT, int kRows>
 __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args p) {
     after_previous();
-    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * kL8Warps + (threadIdx.x >> 5)) * kL8Rows;
+    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * kL8Warps + (threadIdx.x >> 5)) * kRows;
     if (n0 >= p.N) return;
-    int sum[kL8Rows][kT] = {};
-    const int8_t *w[kL8Rows], *a[kT];
+    int sum[kRows][kT] = {};
+    const int8_t *w[kRows], *a[kT];
 #pragma unroll
-    for (int r = 0; r < kL8Rows; ++r) w[r] = p.w + (size_t)min(n0 + r, p.N - 1) * p.ldw;
+    for (int r = 0; r < kRows; ++r) w[r] = p.w + (size_t)min(n0 + r, p.N - 1) * p.ldw;
 #pragma unroll
     for (int t = 0; t < kT; ++t) a[t] = p.a + (size_t)min(t, p.T - 1) * p.lda;
-    auto products = [&](const uint4 (&x)[kL8Rows], int c) {
+    auto products = [&](const uint4 (&x)[kRows], int c) {
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             const uint4 y = *reinterpret_cast<const uint4*>(a[t] + c);
 #pragma unroll
-            for (int r = 0; r < kL8Rows; ++r)
+            for (int r = 0; r < kRows; ++r)
                 sum[r][t] = __dp4a((int)x[r].w, (int)y.w, __dp4a((int)x[r].z, (int)y.z, __dp4a((int)x[r].y, (int)y.y, __dp4a((int)x[r].x, (int)y.x, sum[r][t]))));
         }
     };
     const int whole = p.K & ~511;                // up to there every lane has sixteen codes
-#pragma unroll 4
+#pragma unroll 8 / kRows
     for (int c = lane * 16; c < whole; c += 512) {
-        uint4 x[kL8Rows];
+        uint4 x[kRows];
 #pragma unroll
-        for (int r = 0; r < kL8Rows; ++r) x[r] = ld_stream(w[r] + c);
+        for (int r = 0; r < kRows; ++r) x[r] = ld_stream(w[r] + c);
         products(x, c);
     }
     if (const int c = whole + lane * 16; c < p.K) {
-        uint4 x[kL8Rows];
+        uint4 x[kRows];
 #pragma unroll
-        for (int r = 0; r < kL8Rows; ++r) x[r] = ld_stream(w[r] + c);
+        for (int r = 0; r < kRows; ++r) x[r] = ld_stream(w[r] + c);
         // columns behind the last one: whatever the rows hold there does not count
         const int have = p.K - c;
         auto keep = [&](uint32_t v, int first) { return have >= first + 4 ? v : have <= first ? 0u : v & ((1u << 8 * (have - first)) - 1); };
 #pragma unroll
-        for (int r = 0; r < kL8Rows; ++r) x[r] = make_uint4(keep(x[r].x, 0), keep(x[r].y, 4), keep(x[r].z, 8), keep(x[r].w, 12));
+        for (int r = 0; r < kRows; ++r) x[r] = make_uint4(keep(x[r].x, 0), keep(x[r].y, 4), keep(x[r].z, 8), keep(x[r].w, 12));
         products(x, c);
     }
 #pragma unroll
-    for (int r = 0; r < kL8Rows; ++r)
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             const int v = __reduce_add_sync(0xffffffffu, sum[r][t]);
@@ -349,11 +350,33 @@ __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __gri
         cluster_sync_all();
         const int n = first / p.t_tiles * 128 + (warp & 3) * 32 + lane, t0 = first % p.t_tiles * p.bn;
         if (warp >= 2 && n < p.a.N) {
-            for (int j = part; j < p.bn && t0 + j < p.a.T; j += p.split) {
-                int sum = 0;
-                for (int r = 0; r < p.split; ++r) sum += l8_peer(reinterpret_cast<int*>(smem) + j * 128 + (warp & 3) * 32 + lane, (uint32_t)r);
-                l8_store(p.a, t0 + j, n, sum);
-            }
+            const int* mine = reinterpret_cast<int*>(smem) + (warp & 3) * 32 + lane;
+            const int have = min(p.bn, p.a.T - t0);
+            const float ws = p.a.w_scale[n], bias = p.a.bias ? p.a.bias[n] : 0.0f;
+            auto join = [&](auto ctas) {         // of four tokens at a time all parts are on their way before the first is added
+                constexpr int S = ctas.value;
+                for (int j0 = part; j0 < have; j0 += 4 * S) {
+                    int v[4][S];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int r = 0; r < S; ++r) v[e][r] = l8_peer(mine + min(j0 + e * S, have - 1) * 128, (uint32_t)r);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        int sum = 0;
+#pragma unroll
+                        for (int r = 0; r < S; ++r) sum += v[e][r];
+                        const int t = t0 + j0 + e * S;
+                        if (j0 + e * S >= have) break;
+                        float* to = p.a.out + (size_t)t * p.a.ldc + n;
+                        const float y = l8_value(sum, p.a.a_scale[t], ws, bias);
+                        *to = p.a.accumulate ? __fadd_rn(*to, y) : y;
+                    }
+                }
+            };
+            if (p.split == 2) join(std::integral_constant<int, 2>{});
+            else if (p.split == 4) join(std::integral_constant<int, 4>{});
+            else join(std::integral_constant<int, 8>{});
         }
         cluster_sync_all();                      // nobody leaves while its sums are being read
     }
@@ -481,10 +504,10 @@ int sllm_seq_linear8(const void* a, int64_t lda, const float* a_scale, const voi
     Linear8Args p{(const int8_t*)a, (const int8_t*)w, a_scale, w_scale, bias, C, lda, ldw, ldc, T, N, K, accumulate != 0};
     cudaStream_t st = as_stream(stream);
     if (T > kL8Few) return l8_tc(p, st);
-    LaunchCfg lc(dim3((N + kL8Warps * kL8Rows - 1) / (kL8Warps * kL8Rows)), dim3(kL8Warps * 32), 0, st, true);
-    if (T == 1) SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<1>), p));
-    else if (T == 2) SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<2>), p));
-    else SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<kL8Few>), p));
+    const int rows = N < kL8Wide ? 1 : T == 1 ? 4 : 2;       // of a warp
+    LaunchCfg lc(dim3((N + kL8Warps * rows - 1) / (kL8Warps * rows)), dim3(kL8Warps * 32), 0, st, true);
+    if (rows == 1) SLLM_CUDA(T == 1 ? cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<1, 1>), p) : cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<2, 1>), p));
+    else SLLM_CUDA(T == 1 ? cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<1, 4>), p) : cudaLaunchKernelEx(&lc.cfg, overlapping(linear8_few_kernel<2, 2>), p));
     ++g_launches;
     SLLM_LAUNCH_CHECK();
     return SLLM_OK;
