@@ -161,8 +161,10 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
     } else {
         if (z >= p.own) return;
         const int x = blockIdx.x - group_tiles, seg = p.b.qt_seg[x], off = p.b.qt_off[x];
-        const int n = min(kBQ, p.b.seg_len[seg] - off), end = p.b.seg_pos0[seg] + off + n, from = min(sh_shared_len(p, seg), end);
+        const int n = min(kBQ, p.b.seg_len[seg] - off), end = p.b.seg_pos0[seg] + off + n;
+        const int shared = sh_shared_len(p, seg), from = min(shared, end);
         const int t0 = from / kShKeys, tiles = (end + kShKeys - 1) / kShKeys - t0, cuts = sh_cuts(end - from, p.own_least, p.own);
+        if (g == 0 && z == 0 && threadIdx.x == 0) p.plan[x] = sh_cuts(shared, p.least, p.shares) | cuts << 16;
         if (z >= cuts) return;
         sp.tok0 = p.b.seg_start[seg] + off;
         sp.n_rows = n * per;
@@ -174,31 +176,49 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
     sh_rows<T, kRw>(p, sp, g, sh_smem);
 }
 
-// The records of a (token, head) put together: a warp each.
+// The records of a (token, head) put together: a warp each. Bound: three loads one behind the other (the tile, references and sums, values eight records at a time).
+template <bool kVec>         // results 16 bytes at a time
 __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedArgs p) {
     after_previous();
-    const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], n = min(kBQ, p.b.seg_len[seg] - off), lane = threadIdx.x & 31;
-    const int shared = sh_shared_len(p, seg), end = p.b.seg_pos0[seg] + off + n;
-    const int first = sh_cuts(shared, p.least ? p.least : *p.plan, p.shares), count = first + sh_cuts(end - min(shared, end), p.own_least, p.own);
+    const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], cuts = p.plan[blockIdx.x], lane = threadIdx.x & 31;
+    const int n = min(kBQ, p.b.seg_len[seg] - off), t0 = p.b.seg_start[seg] + off, first = cuts & 0xffff, count = first + (cuts >> 16), step = p.dv + kShHead;
     for (int i = blockIdx.y * 4 + (threadIdx.x >> 5); i < n * p.heads; i += gridDim.y * 4) {
-        const int t = p.b.seg_start[seg] + off + i / p.heads, h = i % p.heads;
-        float top = -INFINITY;
-        for (int k = lane; k < count; k += 32) top = fmaxf(top, sh_record(p, t, h, k < first ? k : p.shares + k - first)[0]);
-        top = warp_max(top);
-        float sum = 0.0f, o[2][4] = {};
-#pragma unroll 4
-        for (int k = 0; k < count; ++k) {
-            const float* rec = sh_record(p, t, h, k < first ? k : p.shares + k - first);
-            const float m = rec[0], l = rec[1];
+        const int t = t0 + i / p.heads, h = i % p.heads;
+        const float* recs = sh_record(p, t, h, 0);
+        auto place = [&](int k) { return recs + (size_t)(k < first ? k : p.shares + k - first) * step; };
+        // at most 48 records: references and sums two a lane
+        float2 head[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int k = lane + 32 * x;
+            head[x] = *reinterpret_cast<const float2*>(place(min(k, max(count, 1) - 1)));
+            if (k >= count) head[x] = make_float2(-INFINITY, 0.0f);
+        }
+        const float top = warp_max(fmaxf(head[0].x, head[1].x));
+        float f[2], sum = 0.0f, o[2][4] = {};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
             // nothing seen: nothing (a sum of NaN goes on); else never zero, so that an infinity stays one
-            const float f = m == -INFINITY && l == 0.0f ? 0.0f : fmaxf(exp2f(m - top), FLT_MIN);
-            sum = fmaf(f, l, sum);
+            f[x] = head[x].x == -INFINITY && head[x].y == 0.0f ? 0.0f : fmaxf(exp2f(head[x].x - top), FLT_MIN);
+            sum = fmaf(f[x], head[x].y, sum);
+        }
+        sum = warp_sum(sum);
+        for (int k0 = 0; k0 < count; k0 += 8) {
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = k0 + k < count ? __shfl_sync(0xffffffffu, k0 < 32 ? f[0] : f[1], (k0 + k) & 31) : 0.0f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int col = c * 128 + 4 * lane;
-                if (col >= p.dv) break;
-                const float4 x = *reinterpret_cast<const float4*>(rec + kShHead + col);
-                o[c][0] = fmaf(f, x.x, o[c][0]); o[c][1] = fmaf(f, x.y, o[c][1]); o[c][2] = fmaf(f, x.z, o[c][2]); o[c][3] = fmaf(f, x.w, o[c][3]);
+                if (c * 128 >= p.dv) break;
+                float4 x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = *reinterpret_cast<const float4*>(place(min(k0 + k, count - 1)) + kShHead + min(col, p.dv - 4));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (k0 + k >= count) break;
+                    o[c][0] = fmaf(w[k], x[k].x, o[c][0]); o[c][1] = fmaf(w[k], x[k].y, o[c][1]); o[c][2] = fmaf(w[k], x[k].z, o[c][2]); o[c][3] = fmaf(w[k], x[k].w, o[c][3]);
+                }
             }
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -206,11 +226,25 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
         for (int c = 0; c < 2; ++c) {
             const int col = c * 128 + 4 * lane;
             if (col >= p.dv) break;
+            const float y[4] = {o[c][0] * inv, o[c][1] * inv, o[c][2] * inv, o[c][3] * inv};
+            if (p.out) {
+                float* to = p.out + (size_t)t * p.ldo + (size_t)h * p.dv + col;
+                if constexpr (kVec) {
+                    *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+                } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float y = o[c][e] * inv;
-                if (p.out) p.out[(size_t)t * p.ldo + (size_t)h * p.dv + col + e] = y;
-                if (p.out16) p.out16[((size_t)t * p.heads + h) * p.dv + col + e] = f32_to_bf16_bits(y);
+                    for (int e = 0; e < 4; ++e) to[e] = y[e];
+                }
+            }
+            if (p.out16) {
+                uint16_t* to = p.out16 + ((size_t)t * p.heads + h) * p.dv + col;
+                if constexpr (kVec) {
+                    *reinterpret_cast<uint2*>(to) = make_uint2((uint32_t)f32_to_bf16_bits(y[0]) | (uint32_t)f32_to_bf16_bits(y[1]) << 16,
+                                                               (uint32_t)f32_to_bf16_bits(y[2]) | (uint32_t)f32_to_bf16_bits(y[3]) << 16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[e] = f32_to_bf16_bits(y[e]);
+                }
             }
         }
     }
@@ -218,8 +252,9 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
 
 static int sh_merge(const SharedArgs& p, cudaStream_t st) {
     const int most = (p.b.T == p.b.nseg ? p.heads : kBQ * p.heads) / 4 + 1;
+    const bool vec = p.ldo % 4 == 0 && ((uintptr_t)p.out % 16) == 0 && ((uintptr_t)p.out16 % 8) == 0;
     LaunchCfg lc(dim3(p.b.n_qtiles, std::min(most, 256)), dim3(128), 0, st, true);
-    SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, overlapping(seq_attention_shared_merge_kernel), p));
+    SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, vec ? overlapping(seq_attention_shared_merge_kernel<true>) : overlapping(seq_attention_shared_merge_kernel<false>), p));
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
@@ -262,7 +297,7 @@ int64_t sllm_seq_attention_shared_ws_bytes(const sllm_seq_batch* b, int32_t n_gr
                  "seq_attention_shared_ws_bytes: bad argument");
     int shares, own;
     shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &shares, &own);
-    return (int64_t)b->T * heads * (shares + own) * (dv + kShHead) * (int64_t)sizeof(float) + kShPlan;
+    return (int64_t)b->T * heads * (shares + own) * (dv + kShHead) * (int64_t)sizeof(float) + sh_plan_bytes(b->n_qtiles);
 }
 
 int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const int32_t* group_start, const int32_t* group_len, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads,
@@ -288,7 +323,7 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
                  "seq_attention_shared: values in keys, charges on the logarithm of the distance, values of every head and chunks are not part of this form");
     SharedArgs p{*b, n_groups, group_start, group_len, q, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, INT_MAX, 0, 0.0f, nullptr, 0, 0,
                  (uint32_t)(((1ull << 32) + b->page_len - 1) / b->page_len), 0, 0, (int*)ws,
-                 (float*)((char*)ws + kShPlan), out, ldo, (uint16_t*)out16};
+                 (float*)((char*)ws + sh_plan_bytes(b->n_qtiles)), out, ldo, (uint16_t*)out16};
     if (opts) {
         if (opts->window > 0) {
             p.window = opts->window;
@@ -301,7 +336,7 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     if (int rc = status_check()) return rc;
     cudaStream_t st = as_stream(stream);
     const bool tc = kv_dtype == SLLM_BF16 && dk == dv && (dk == 64 || dk == 128);
-    p.least = tc ? 0 : 64;
+    p.least = 64;
     p.own_least = tc ? 512 : 64;
     const int rc = tc ? launch_attention_shared_tc(p, st) : kv_dtype == SLLM_F32 ? sh_launch<float, 4>(p, st) : sh_launch<uint16_t, 4>(p, st);
     return rc ? rc : sh_merge(p, st);

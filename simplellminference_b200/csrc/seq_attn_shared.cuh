@@ -23,8 +23,8 @@ struct SharedArgs {
     const float* slopes;
     int shares, own;                     // records of a (token, head) at most: of the shared positions, of its own
     uint32_t page_magic;                 // ceil(2^32 / page_len): the page of a position without a division (page_of)
-    int least, own_least;                // keys of a share at least; least 0: as the plan at the workspace's beginning has it
-    int* plan;
+    int least, own_least;                // keys of a share at least (least: of the kernel that does not plan it itself)
+    int* plan;                           // of every listed tile: its records of shared positions, and its own ones << 16
     float* ws;
     float* out;
     int ldo;
@@ -34,7 +34,8 @@ struct SharedArgs {
 // What a CTA leaves of the keys it has seen, for a (token, head): the reference of the weights as a power of two, their sum, and the weighted sum of the values. Records lie
 // [token][head][shares + own][dv + 4].
 constexpr int kShHead = 4;               // floats in front of the values (16 bytes, so that these are aligned)
-constexpr int kShPlan = 64;              // bytes in front of the records: the plan, one number
+// bytes in front of the records: the plan
+inline int64_t sh_plan_bytes(int n_qtiles) { return ((int64_t)n_qtiles * 4 + 15) / 16 * 16; }
 
 #ifdef __CUDACC__
 

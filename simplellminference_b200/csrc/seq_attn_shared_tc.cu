@@ -30,17 +30,18 @@ template <int HD>
 struct StShape {
     static constexpr int kBlocks = HD / 64, kQBlock = kStRows * 128, kQBytes = kBlocks * kQBlock, kKBlock = kStKeys * 128, kTile = kBlocks * kKBlock;
     static constexpr int kStages = HD == 128 ? 2 : 4;
-    static constexpr int kBars = kQBytes + 2 * kStages * kTile, kPlan = kBars + 512, kSmem = 1024 + kPlan + 10 * 1024;
+    static constexpr int kBars = kQBytes + 2 * kStages * kTile, kPlan = kBars + 512, kSmem = 1024 + kPlan + 11 * 1024;
 };
 
 // The step's work as a CTA sees it: entries (groups, then listed tiles of queries), as many at a time as it has threads, and how many items each and those before it are.
 constexpr int kStEntries = kStThreads;
 struct StPlan {
     int tok0[kStEntries], n[kStEntries], slot[kStEntries], from[kStEntries], end[kStEntries], cuts[kStEntries], tiles[kStEntries], upto[kStEntries];
+    int low[kStEntries], high[kStEntries];       // positions of a group's listed tokens
     int warp[kStWarps];
     int least, total;
 };
-static_assert(sizeof(StPlan) <= 10 * 1024, "its place");
+static_assert(sizeof(StPlan) <= 11 * 1024, "its place");
 
 struct StArgs {
     SharedArgs a;
@@ -56,6 +57,7 @@ struct StItem {
     int tok0, nq, slot, g, h0;               // rows: nq tokens from tok0 on x hpc heads from h0 on, of kv head g
     int pos0;                                // position of the first token where the others follow it, -1: their positions are looked up
     int key0, key1, which;                   // keys, and the record that takes the result
+    int low, high;                           // no token of the rows lies before the one or behind the other position
 };
 
 __device__ __forceinline__ int st_token(const StArgs& sa, int row) { return (int)((uint32_t)row * sa.hpc_magic >> 16); }
@@ -356,26 +358,17 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + Sh::kBars);
     uint64_t *kempty = kfull + ST, *vfull = kempty + ST, *vempty = vfull + ST, *vready = vempty + ST, *qready = vready + ST, *sfull = qready + 1, *pready = sfull + 1, *odone = pready + 1;
     volatile int* gave_up = st_gave_up<HD>(smem);
-    int* extent = st_gave_up<HD>(smem) + 1 + 3 * (turn & 1);     // the rows' least and largest position; whether values were taken out
+    int* taken = st_gave_up<HD>(smem) + 1 + (turn & 1);          // whether values were taken out
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_rows = it.nq * sa.hpc;
     const int row = threadIdx.x, qi = min(st_token(sa, row), it.nq - 1), h = it.h0 + min(row - st_token(sa, row) * sa.hpc, sa.hpc - 1);      // (of the first four warps)
     const bool live = row < n_rows;
-    if (threadIdx.x == 0) {                  // the next item's
-        int* other = st_gave_up<HD>(smem) + 1 + 3 * (~turn & 1);
-        other[0] = INT_MAX;
-        other[1] = -1;
-        other[2] = 0;
-    }
-    if (warp >= 4) {                         // (a tile has at most 128 tokens)
-        const int i = threadIdx.x - 128, pos = i < it.nq ? st_pos(sa, it, i) : -1;
-        const int high = __reduce_max_sync(0xffffffffu, pos), low = __reduce_min_sync(0xffffffffu, pos < 0 ? INT_MAX : pos);
-        if (lane == 0) {
-            atomicMax(extent + 1, high);
-            atomicMin(extent, low);
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");           // the producer need not wait for the queries
-        asm volatile("bar.arrive 2, 256;" ::: "memory");
-    } else {
+    if (threadIdx.x == 0) st_gave_up<HD>(smem)[1 + (~turn & 1)] = 0;      // the next item's
+    const int key1 = min(it.key1, it.high + 1);
+    const StTiles tiles(it.key0, key1, p.window > it.low ? 0 : it.low - p.window + 1, p.keep_first);
+    const int n = tiles.n;
+    const uint32_t was = done;               // key tiles of the items before: the barriers' phases go on from there
+    done += n;
+    if (warp < 4) {
         // the warp's 32 rows of queries, one row (or two) per load so that neighbouring lanes read neighbouring columns; sixteen loads on their way before the first of them is stored. Where a
         // row lies its own lane knows
         constexpr int kLanes = HD / 4, kPer = 32 / kLanes, kAhead = 16;
@@ -403,14 +396,8 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
         else queries([](const float* src) { return make_uint4(__float_as_uint(src[0]), __float_as_uint(src[1]), __float_as_uint(src[2]), __float_as_uint(src[3])); });
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mb_arrive(qready);
-        asm volatile("bar.sync 2, 256;" ::: "memory");
     }
-    tc_fence_after();
-    const int least = extent[0], most = extent[1], key1 = min(it.key1, most + 1);
-    const StTiles tiles(it.key0, key1, p.window > least ? 0 : least - p.window + 1, p.keep_first);
-    const int n = tiles.n;
-    const uint32_t was = done;               // key tiles of the items before: the barriers' phases go on from there
-    done += n;
+
     if (warp == 4) {
         if (elect_one()) {   // ===== TMA producer =====
             for (int i = 0; i < n; ++i) {
@@ -494,7 +481,7 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                     odd = true;
                 }
             }
-            if (odd) extent[2] = 1;
+            if (odd) *taken = 1;
             if (from > 0 || to < kStKeys || __any_sync(0xffffffffu, odd)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mb_arrive(vready + s);
@@ -583,10 +570,13 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
 #pragma unroll
                 for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(fmaf(-slope, d0 - (float)e, __uint_as_float(s[e])));
             }
-            if (!all) {
+            if (!all) {          // the keys of the tile that this row sees, a bit each: up to its own position, and from the window's oldest on or among the first
+                auto below = [&](int key) { return key <= j0 ? 0ull : key >= j0 + 64 ? ~0ull : (1ull << (key - j0)) - 1; };
+                const uint64_t sees = have & below(qpos + 1) & (~below(p.window > qpos ? 0 : qpos - p.window + 1) | below(p.keep_first));
+                const uint32_t seen[2] = {(uint32_t)sees, (uint32_t)(sees >> 32)};
 #pragma unroll
                 for (int e = 0; e < 64; ++e)
-                    if (!(have >> e & 1) || !seq_sees(qpos, j0 + e, p.window, p.keep_first)) s[e] = 0xff800000u;       // -inf
+                    if (!(seen[e / 32] >> (e % 32) & 1)) s[e] = 0xff800000u;       // -inf
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -681,19 +671,20 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 add_flushed(o + 16, c + 16);
             }
             __syncwarp();
+            uint32_t got[16];        // (all of them before the first store: behind a store each shuffle waited)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) got[e] = __shfl_xor_sync(0xffffffffu, odd ? o[(e & ~3) * 2 + (e & 3)] : o[(e & ~3) * 2 + 4 + (e & 3)], 1);
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
-                uint32_t got[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) got[i] = __shfl_xor_sync(0xffffffffu, odd ? o[e + i] : o[e + 4 + i], 1);
-                if (even_live) *reinterpret_cast<uint4*>(even_row + c + e) = odd ? make_uint4(got[0], got[1], got[2], got[3]) : make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                if (odd_live) *reinterpret_cast<uint4*>(odd_row + c + e) = odd ? make_uint4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]) : make_uint4(got[0], got[1], got[2], got[3]);
+                const uint4 g = make_uint4(got[e / 2], got[e / 2 + 1], got[e / 2 + 2], got[e / 2 + 3]);
+                if (even_live) *reinterpret_cast<uint4*>(even_row + c + e) = odd ? g : make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                if (odd_live) *reinterpret_cast<uint4*>(odd_row + c + e) = odd ? make_uint4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]) : g;
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (extent[2] && warp < 4 && live) {     // infinities and NaN that were taken out of the values: back to the rows that see them (columns of this row alone, written behind the barrier)
+    if (*taken && warp < 4 && live) {     // infinities and NaN that were taken out of the values: back to the rows that see them (columns of this row alone, written behind the barrier)
         const int qpos = st_pos(sa, it, qi);
         for (int i = 0; i < n; ++i) {
             const int j0 = tiles.tile_of(i) * kStKeys;
@@ -750,11 +741,11 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
     const SharedArgs& p = sa.a;
     const int all_sets = p.kv_heads * sa.sets, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.heads / p.kv_heads;
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
         st_barriers<HD>(smem);
         *gave_up = 0;
-        st_gave_up<HD>(smem)[1] = INT_MAX;       // of the first item; each makes those of the next one ready
-        st_gave_up<HD>(smem)[2] = -1;
-        st_gave_up<HD>(smem)[3] = 0;
+        st_gave_up<HD>(smem)[1] = 0;             // of the first item; each makes that of the next one ready
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 5) tc_alloc(tmem_slot, kStTmem);
@@ -764,13 +755,13 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
     for (int e0 = 0; e0 < entries; e0 += kStEntries) {
         {   // an entry a thread
             const int e = e0 + threadIdx.x, i = threadIdx.x;
-            int tok0 = 0, n = 0, slot = -1, from = 0, end = 0, cuts = 0, tiles = 0, seg = -1;
+            int tok0 = 0, n = 0, slot = -1, from = 0, end = 0, cuts = 0, tiles = 0, seg = -1, shared = 0;
             if (e < p.n_groups) {
                 sh_group_tokens(p, e, tok0, n);
                 end = max(0, p.group_len[e]);
                 tiles = (n + sa.queries - 1) / sa.queries;
                 if (n > 0) slot = p.b.seg_slot[p.group_start[e]];
-                plan.n[i] = n; plan.end[i] = end; plan.tiles[i] = tiles; plan.from[i] = p.group_start[e];
+                plan.n[i] = n; plan.end[i] = end; plan.tiles[i] = tiles; plan.from[i] = p.group_start[e]; plan.low[i] = INT_MAX; plan.high[i] = -1;
             } else if (e < entries) {
                 const int off = p.b.qt_off[e - p.n_groups];
                 seg = p.b.qt_seg[e - p.n_groups];
@@ -791,10 +782,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
                                             t = (m + sa.queries - 1) / sa.queries;
                                             k = (max(0, p.group_len[g]) + kStKeys - 1) / kStKeys;
                                         });
-                if (lane == 0) {
-                    plan.least = least;
-                    if (blockIdx.x == 0) *p.plan = least;
-                }
+                if (lane == 0) plan.least = least;
             }
             if (seg >= 0) {
                 int lo = 0, hi = p.n_groups;                     // group_start[lo] <= seg < group_start[hi]
@@ -804,9 +792,16 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
                 }
                 from = min(all && e0 == 0 ? plan.end[lo] : max(0, p.group_len[lo]), end);
                 cuts = sh_cuts(end - from, p.own_least, p.own);
+                shared = all && e0 == 0 ? plan.end[lo] : max(0, p.group_len[lo]);
+                if (all && e0 == 0) {
+                    atomicMin(&plan.low[lo], end - n);
+                    atomicMax(&plan.high[lo], end - 1);
+                }
             }
             __syncthreads();
             if (e < p.n_groups) cuts = sh_cuts(end, plan.least, p.shares);
+            else if (blockIdx.x == 0 && seg >= 0) p.plan[e - p.n_groups] = sh_cuts(shared, plan.least, p.shares) | cuts << 16;
+            if (e < p.n_groups && entries > kStEntries) { plan.low[i] = 0; plan.high[i] = INT_MAX - 1; }      // not all of its tiles are here
             plan.tok0[i] = tok0; plan.n[i] = n; plan.slot[i] = slot; plan.from[i] = from; plan.end[i] = end; plan.cuts[i] = cuts; plan.tiles[i] = tiles;
             const bool few = seg >= 0 && n * sa.hpc <= kStFew;
             int upto = few ? (cuts * all_sets + kStTeams - 1) / kStTeams : tiles * cuts * all_sets;
@@ -845,6 +840,8 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             it.key0 = max(from, (int)(t0 + span * z / cuts) * kStKeys);                      // (span * z: 2^25 key tiles at most, 32 shares)
             it.key1 = min(end, (int)(t0 + span * (z + 1) / cuts) * kStKeys);
             it.which = (group ? 0 : p.shares) + z;
+            it.low = group ? plan.low[e] : it.pos0;
+            it.high = group ? plan.high[e] : it.pos0 + it.nq - 1;
             if (few) {
                 if (z < cuts) st_few<HD>(sa, it, smem);
             } else {
