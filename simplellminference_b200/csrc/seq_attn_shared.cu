@@ -18,6 +18,26 @@ struct ShSpan {                          // rows and keys of a CTA
     int which;                           // of the records
 };
 
+// load(i) for the CTA's i < n in turn, kAhead of a thread on their way before the first is handed to store(i, value)
+template <int kAhead, class L, class S>
+__device__ __forceinline__ void sh_stage(int n, L load, S store) {
+    constexpr int kThreads = kShWarps * 32;
+    for (int i0 = threadIdx.x; i0 < n; i0 += kAhead * kThreads) {
+        decltype(load(0)) x[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) x[k] = load(min(i0 + k * kThreads, n - 1));
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (i0 + k * kThreads < n) store(i0 + k * kThreads, x[k]);
+    }
+}
+__device__ __forceinline__ void sh_floats(const uint4& v, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void sh_floats(const uint4& v, float (&x)[8]) {
+    x[0] = bf16_lo(v.x); x[1] = bf16_hi(v.x); x[2] = bf16_lo(v.y); x[3] = bf16_hi(v.y); x[4] = bf16_lo(v.z); x[5] = bf16_hi(v.z); x[6] = bf16_lo(v.w); x[7] = bf16_hi(v.w);
+}
+
 template <typename T, int kRw>
 __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, int g, float* smem) {
     constexpr int kRows = kShWarps * kRw, kPer = 16 / sizeof(T);
@@ -26,15 +46,15 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
     float *s_q = smem, *s_k = s_q + kRows * p.dk, *s_v = s_k + kShKeys * ldk, *s_p = s_v + kShKeys * p.dv;      // s_p: [warp][key][row]
     for (int r0 = 0; r0 < sp.n_rows; r0 += kRows) {
         __syncthreads();
-        for (int i = threadIdx.x; i < kRows * p.dk; i += kShWarps * 32) {
-            const int r = r0 + i / p.dk, c = i % p.dk;
-            float x = 0.0f;
-            if (r < sp.n_rows) {
-                x = p.q[(size_t)(sp.tok0 + r / per) * p.ldq + (size_t)(g * per + r % per) * p.dk + c];
-                if (sizeof(T) == 2) x = seq_round_bf16(x);               // as the products on the tensor cores take it
-            }
-            s_q[i] = x;
-        }
+        // (rows behind the last one are the last one again; nothing asks for their results)
+        sh_stage<4>(kRows * p.dk / 4, [&](int i) {
+            const int r = min(r0 + 4 * i / p.dk, sp.n_rows - 1), c = 4 * i % p.dk;
+            const float* src = p.q + (size_t)(sp.tok0 + r / per) * p.ldq + (size_t)(g * per + r % per) * p.dk + c;
+            return make_float4(src[0], src[1], src[2], src[3]);
+        }, [&](int i, const float4& x) {
+            // as the products on the tensor cores take it
+            *reinterpret_cast<float4*>(s_q + 4 * i) = sizeof(T) == 2 ? make_float4(seq_round_bf16(x.x), seq_round_bf16(x.y), seq_round_bf16(x.z), seq_round_bf16(x.w)) : x;
+        });
         int pos[kRw];
         float m[kRw], l[kRw], o[kRw][2][4], slope[kRw];
 #pragma unroll
@@ -55,24 +75,30 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
 #pragma unroll
             for (int i = 0; i < kRw; ++i) seen |= pos[i] >= j0 && (pos[i] - (j0 + kShKeys - 1) < p.window || j0 < p.keep_first);
             if (!__syncthreads_or(seen && page >= 0)) continue;          // (behind it the last tile has been read, and the queries are there)
+            // All rows of the tile are the page's, whatever part of them is the share's: nothing is asked before they are loaded. Scores of the others are hidden, their values zeros.
             int odd = 0;                                                 // a value that is infinite or NaN
-            for (int i = threadIdx.x; i < kShKeys * (p.dk / kPer); i += kShWarps * 32) {
-                const int k = i / (p.dk / kPer), c = i % (p.dk / kPer) * kPer;
+            const T *kr = reinterpret_cast<const T*>(p.k_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page, p.dk);
+            const T *vr = reinterpret_cast<const T*>(p.v_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page, p.dv);
+            sh_stage<4>(kShKeys * p.dk / kPer, [&](int i) { return ld_stream(kr + i * kPer); }, [&](int i, const uint4& v) {
+                const int at = i * kPer, k = at / p.dk;
                 float x[kPer];
-                seq_ld16(reinterpret_cast<const T*>(p.k_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page + k, p.dk) + c, j0 + k >= sp.key0 && j0 + k < sp.key1, x);
+                sh_floats(v, x);
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) s_k[k * ldk + c + e] = x[e];
-            }
-            for (int i = threadIdx.x; i < kShKeys * (p.dv / kPer); i += kShWarps * 32) {
-                const int k = i / (p.dv / kPer), c = i % (p.dv / kPer) * kPer;
+                for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(s_k + k * ldk + at - k * p.dk + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+            });
+            sh_stage<4>(kShKeys * p.dv / kPer, [&](int i) { return ld_stream(vr + i * kPer); }, [&](int i, const uint4& v) {
+                const int at = i * kPer, k = j0 + at / p.dv;
+                const bool in = k >= sp.key0 && k < sp.key1;
                 float x[kPer];
-                seq_ld16(reinterpret_cast<const T*>(p.v_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page + k, p.dv) + c, j0 + k >= sp.key0 && j0 + k < sp.key1, x);
+                sh_floats(v, x);
 #pragma unroll
                 for (int e = 0; e < kPer; ++e) {
-                    s_v[k * p.dv + c + e] = x[e];
+                    x[e] = in ? x[e] : 0.0f;
                     odd |= !(fabsf(x[e]) <= FLT_MAX);
                 }
-            }
+#pragma unroll
+                for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(s_v + at + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+            });
             odd = __syncthreads_or(odd);
             const int key = j0 + lane;
             float s[kRw] = {};

@@ -706,28 +706,36 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
 // long as some three key tiles) count for more than the rest. Thirty-two lengths about the even one are tried, a lane each. group(g, tiles, keys): row tiles and key tiles of a group. By one warp.
 template <class F>
 __device__ __forceinline__ int st_least(const SharedArgs& p, int all_sets, F group) {
-    const int lane = threadIdx.x & 31, ctas = (int)gridDim.x;
-    long long units = 0, items = 0;
+    const int lane = threadIdx.x & 31;
+    const float inv = 1.0f / (float)gridDim.x;       // (these are estimates: whole-number divisions of 64 bits took 1000 clocks)
+    float units = 0.0f, items = 0.0f;
     for (int g = lane; g < p.n_groups; g += 32) {
         int tiles, keys;
         group(g, tiles, keys);
-        units += (long long)tiles * keys;
+        units += (float)tiles * (float)keys;
     }
-    for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-    const long long even = (units * all_sets + ctas - 1) / ctas;
-    const int length = (int)max(4LL, min(1LL << 20, even * (4 + lane) / 16));
+    const float even = ceilf(warp_sum(units) * (float)all_sets * inv);
+    const int length = (int)fmaxf(4.0f, fminf(1048576.0f, even * (float)(4 + lane) * (1.0f / 16.0f)));
+    const float per = 1.0f / (float)length;
     for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
         int tiles = 0, keys = 0;
         if (g0 + lane < p.n_groups) group(g0 + lane, tiles, keys);
         for (unsigned rest = __ballot_sync(0xffffffffu, tiles > 0 && keys > 0); rest; rest &= rest - 1) {
-            const int who = __ffs(rest) - 1, k = __shfl_sync(0xffffffffu, keys, who);
-            items += (long long)__shfl_sync(0xffffffffu, tiles, who) * min(p.shares, (k + length - 1) / length);
+            const int who = __ffs(rest) - 1;
+            const float k = (float)__shfl_sync(0xffffffffu, keys, who);
+            items += (float)__shfl_sync(0xffffffffu, tiles, who) * fminf((float)p.shares, ceilf(k * per));
         }
     }
-    items *= all_sets;
-    long long cost = ((items + ctas - 1) / ctas) * (length + 3) * 32 + lane;
-    for (int o = 16; o > 0; o >>= 1) cost = min(cost, __shfl_xor_sync(0xffffffffu, cost, o));
-    return __shfl_sync(0xffffffffu, length, (int)(cost & 31)) * kStKeys;
+    const float cost = ceilf(items * (float)all_sets * inv) * (float)(length + 3), least = -warp_max(-cost);
+    return __shfl_sync(0xffffffffu, length, __ffs(__ballot_sync(0xffffffffu, cost == least)) - 1) * kStKeys;
+}
+
+// x / d for numbers below 2^24, the estimate put right
+__device__ __forceinline__ uint32_t st_div(uint32_t x, uint32_t d) {
+    uint32_t q = (uint32_t)__fdividef((float)x, (float)d);
+    if (q * d > x) --q;
+    else if (x - q * d >= d) ++q;
+    return q;
 }
 
 template <int HD, bool kOpts>
@@ -829,7 +837,9 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             const int n = plan.n[e], from = plan.from[e], end = plan.end[e], t0 = from / kStKeys, span = (end + kStKeys - 1) / kStKeys - t0;
             const bool few = !group && n * sa.hpc <= kStFew;
             if (few) x = kStTeams * x + threadIdx.x / (32 * kStTeam);
-            const uint32_t y = (uint32_t)x / tiles, tile = x - y * tiles, z = y / (uint32_t)all_sets, set = y - z * all_sets;
+            // (item numbers may be larger than st_div takes; what is left of them by then is not)
+            const uint32_t y = tiles == 1 ? (uint32_t)x : (uint32_t)x < 1u << 24 ? st_div(x, tiles) : (uint32_t)x / tiles, tile = x - y * tiles;
+            const uint32_t z = y < 1u << 24 ? st_div(y, all_sets) : y / (uint32_t)all_sets, set = y - z * all_sets;
             StItem it;
             it.g = sa.sets == 1 ? set : set / (uint32_t)sa.sets;
             it.tok0 = plan.tok0[e] + tile * sa.queries;
@@ -837,8 +847,9 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             it.slot = plan.slot[e];
             it.pos0 = group ? -1 : end - n + (int)tile * sa.queries;
             it.h0 = it.g * per + (set - it.g * sa.sets) * sa.hpc;
-            it.key0 = max(from, (int)(t0 + span * z / cuts) * kStKeys);                      // (span * z: 2^25 key tiles at most, 32 shares)
-            it.key1 = min(end, (int)(t0 + span * (z + 1) / cuts) * kStKeys);
+            auto cut = [&](uint32_t k) { return cuts == 1 ? span * k : span * k < 1u << 24 ? st_div(span * k, cuts) : span * k / cuts; };      // (2^25 key tiles at most, 32 shares)
+            it.key0 = max(from, (int)(t0 + cut(z)) * kStKeys);
+            it.key1 = min(end, (int)(t0 + cut(z + 1)) * kStKeys);
             it.which = (group ? 0 : p.shares) + z;
             it.low = group ? plan.low[e] : it.pos0;
             it.high = group ? plan.high[e] : it.pos0 + it.nq - 1;
