@@ -21,7 +21,7 @@
 namespace sllm {
 
 constexpr int kStRows = 128, kStKeys = 64, kStThreads = 256, kStBox = 32, kStWarps = kStThreads / 32;
-constexpr int kStFlush = 12;
+constexpr int kStFlush = 12, kStEnds = 8;
 constexpr uint32_t kStTmem = 256;            // scores at 0 .. 63, then the weights' terms at 0 .. 95, O at 128; two CTAs share an SM's 512 columns
 constexpr int kStFew = 16, kStTeam = 4, kStTeams = kStWarps / kStTeam;      // rows of a segment up to which its own positions are a team's work; warps of a team
 constexpr float kStLog2e = 1.4426950408889634f;
@@ -520,8 +520,7 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             const int from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
             uint64_t have = (to >= 64 ? ~0ull : (1ull << to) - 1) & ~((1ull << from) - 1);
             int in_page;
-            if (sh_page(p, it.slot, j0, in_page) < 0) have &= ~0xffffffffull;
-            if (to > kStBox && sh_page(p, it.slot, j0 + kStBox, in_page) < 0) have &= 0xffffffffull;
+            const int page0 = sh_page(p, it.slot, j0, in_page), page1 = sh_page(p, it.slot, min(j0 + kStBox, key1 - 1), in_page);      // (on their way while the scores are made)
             ok = tc_wait_warp(sfull, (was + i) & 1, gave_up, sa.polls);
             if (!ok) break;
             tc_fence_after();
@@ -530,6 +529,8 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             tc_ld32_async(s_tmem + 32, s + 32);
             tc_arrived(s);
             tc_arrived(s + 32);
+            if (page0 < 0) have &= ~0xffffffffull;
+            if (page1 < 0) have &= 0xffffffffull;
             // every key of the tile is visible to every row of the warp
             const bool all = have == ~0ull && __all_sync(0xffffffffu, !live || (j0 + kStKeys - 1 <= qpos && (qpos - j0 < p.window || j0 + kStKeys <= p.keep_first)));
             if (kOpts && p.softcap > 0.0f) {
@@ -702,13 +703,13 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
     }
 }
 
-// Keys of a share of the shared positions: by what all groups have (row tiles x key tiles), such that the shares are a round of the grid or a few, and none so short that its beginning and end (as
-// long as some three key tiles) count for more than the rest. Thirty-two lengths about the even one are tried, a lane each. group(g, tiles, keys): row tiles and key tiles of a group. By one warp.
+// Keys of a share of the shared positions: by what all groups have (row tiles x key tiles), such that the shares are a round of the grid or a few, their beginnings and ends counted
+// as kStEnds key tiles. Thirty-two lengths about the even one are tried, a lane each. group(g, tiles, keys): row tiles and key tiles of a group. By one warp.
 template <class F>
 __device__ __forceinline__ int st_least(const SharedArgs& p, int all_sets, F group) {
     const int lane = threadIdx.x & 31;
     const float inv = 1.0f / (float)gridDim.x;       // (these are estimates: whole-number divisions of 64 bits took 1000 clocks)
-    float units = 0.0f, items = 0.0f;
+    float units = 0.0f, items = 0.0f, longest = 0.0f;
     for (int g = lane; g < p.n_groups; g += 32) {
         int tiles, keys;
         group(g, tiles, keys);
@@ -722,11 +723,12 @@ __device__ __forceinline__ int st_least(const SharedArgs& p, int all_sets, F gro
         if (g0 + lane < p.n_groups) group(g0 + lane, tiles, keys);
         for (unsigned rest = __ballot_sync(0xffffffffu, tiles > 0 && keys > 0); rest; rest &= rest - 1) {
             const int who = __ffs(rest) - 1;
-            const float k = (float)__shfl_sync(0xffffffffu, keys, who);
-            items += (float)__shfl_sync(0xffffffffu, tiles, who) * fminf((float)p.shares, ceilf(k * per));
+            const float k = (float)__shfl_sync(0xffffffffu, keys, who), cuts = fminf((float)p.shares, ceilf(k * per));
+            items += (float)__shfl_sync(0xffffffffu, tiles, who) * cuts;
+            longest = fmaxf(longest, ceilf(__fdividef(k, cuts)));
         }
     }
-    const float cost = ceilf(items * (float)all_sets * inv) * (float)(length + 3), least = -warp_max(-cost);
+    const float cost = ceilf(items * (float)all_sets * inv) * (longest + (float)kStEnds), least = -warp_max(-cost);
     return __shfl_sync(0xffffffffu, length, __ffs(__ballot_sync(0xffffffffu, cost == least)) - 1) * kStKeys;
 }
 
