@@ -323,7 +323,7 @@ int64_t sllm_seq_attention_shared_ws_bytes(const sllm_seq_batch* b, int32_t n_gr
                  "seq_attention_shared_ws_bytes: bad argument");
     int shares, own;
     shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &shares, &own);
-    return (int64_t)b->T * heads * (shares + own) * (dv + kShHead) * (int64_t)sizeof(float) + sh_plan_bytes(b->n_qtiles);
+    return ((int64_t)b->T * heads * (shares + own) * (dv + kShHead) + attention_shared_tc_flush_floats(dk, dv)) * (int64_t)sizeof(float) + sh_plan_bytes(b->n_qtiles);
 }
 
 int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const int32_t* group_start, const int32_t* group_len, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads,
@@ -349,7 +349,7 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
                  "seq_attention_shared: values in keys, charges on the logarithm of the distance, values of every head and chunks are not part of this form");
     SharedArgs p{*b, n_groups, group_start, group_len, q, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, INT_MAX, 0, 0.0f, nullptr, 0, 0,
                  (uint32_t)(((1ull << 32) + b->page_len - 1) / b->page_len), 0, 0, (int*)ws,
-                 (float*)((char*)ws + sh_plan_bytes(b->n_qtiles)), out, ldo, (uint16_t*)out16};
+                 (float*)((char*)ws + sh_plan_bytes(b->n_qtiles)), nullptr, out, ldo, (uint16_t*)out16};
     if (opts) {
         if (opts->window > 0) {
             p.window = opts->window;
@@ -359,6 +359,7 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
         p.slopes = opts->slopes;
     }
     shared_plan(b->T, b->n_qtiles, n_groups, heads, kv_heads, &p.shares, &p.own);
+    p.flush = p.ws + (int64_t)b->T * heads * (p.shares + p.own) * (dv + kShHead);
     if (int rc = status_check()) return rc;
     cudaStream_t st = as_stream(stream);
     const bool tc = kv_dtype == SLLM_BF16 && dk == dv && (dk == 64 || dk == 128);

@@ -7,6 +7,7 @@ namespace sllm {
 // the kernel for pools in bf16 and heads of 64 or 128 (seq_attn_shared_tc.cu)
 struct SharedArgs;
 int launch_attention_shared_tc(const SharedArgs& p, cudaStream_t st);
+int64_t attention_shared_tc_flush_floats(int dk, int dv);      // what its CTAs need to move their accumulators to
 
 // A step whose segments come in groups: the first group_len[g] positions of all segments group_start[g] .. group_start[g + 1] - 1 are the same and are read through the block table of the group's
 // first segment; the positions behind them through each segment's own.
@@ -26,6 +27,7 @@ struct SharedArgs {
     int least, own_least;                // keys of a share at least (least: of the kernel that does not plan it itself)
     int* plan;                           // of every listed tile: its records of shared positions, and its own ones << 16
     float* ws;
+    float* flush;                        // of the kernel on the tensor cores: what its CTAs' accumulators held, a tile of rows each
     float* out;
     int ldo;
     uint16_t* out16;

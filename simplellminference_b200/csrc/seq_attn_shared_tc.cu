@@ -4,7 +4,8 @@
 // neighbouring tokens, on tcgen05, against a share of the keys, 64 at a time:
 //   warps 0-3  softmax, a thread per row: queries to bf16 rows in shared memory; per key tile the scores from TMEM, capped, charged and masked, fp32 maximum and sum; the weights go back to TMEM as
 //              THREE bf16 terms (24 bits; two leave 2^-18 of a weight, which is more than all the rest). O stays in TMEM, rescaled only where a maximum has grown by more than 2^8; the
-//              tensor core truncates as it adds, so every kStFlush tiles O moves on to the row's record;
+//              tensor core truncates as it adds, so every kStFlush tiles O moves on to the CTA's own place in the workspace, [columns / 4][rows] so that whole lines are read and written (in the rows'
+//              records, 16 bytes of a row a lane, a move took six times as long: 290 us instead of 227 for the mixed step);
 //   warp 4     (one lane) TMA producer: boxes of 32 positions, looked up in the block table; what is behind the last position or in no page reads as zeros;
 //   warp 5     (one lane) MMA issuer: S = Q K^T, O += (hi + mid + lo) V with the weights read from TMEM, V as it lies;
 //   warps 6-7  zero the value rows that are not part of the share, and take infinities and NaN out of the values (0 * NaN is NaN for rows that do not see them, and the terms of a weight times
@@ -21,7 +22,7 @@
 namespace sllm {
 
 constexpr int kStRows = 128, kStKeys = 64, kStThreads = 256, kStBox = 32, kStWarps = kStThreads / 32;
-constexpr int kStFlush = 12, kStEnds = 8;
+constexpr int kStFlush = 7, kStEnds = 8;
 constexpr uint32_t kStTmem = 256;            // scores at 0 .. 63, then the weights' terms at 0 .. 95, O at 128; two CTAs share an SM's 512 columns
 constexpr int kStFew = 16, kStTeam = 4, kStTeams = kStWarps / kStTeam;      // rows of a segment up to which its own positions are a team's work; warps of a team
 constexpr float kStLog2e = 1.4426950408889634f;
@@ -107,7 +108,7 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
     for (int r0 = 0; r0 < n_rows; r0 += 8) {
         // columns of the products: rows r0 .. r0 + 7. As an operand a lane has row g, as a result rows 2t and 2t + 1
         int pos[2];
-        float slope[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kTiles][4] = {};
+        float slope[2], m[2] = {-INFINITY, -INFINITY}, l[4] = {}, o[kTiles][4] = {};      // l: of rows 2t, 2t + 1, twice
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = r0 + 2 * t + i, qi = st_token(sa, r);
@@ -201,8 +202,7 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
             if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
                 // (never zero: an infinity that has come in stays one)
                 const float f0 = top[0] == m[0] ? 1.0f : fmaxf(tc_exp2(m[0] - top[0]), FLT_MIN), f1 = top[1] == m[1] ? 1.0f : fmaxf(tc_exp2(m[1] - top[1]), FLT_MIN);
-                l[0] *= f0;
-                l[1] *= f1;
+                l[0] *= f0; l[1] *= f1; l[2] *= f0; l[3] *= f1;
 #pragma unroll
                 for (int c = 0; c < kTiles; ++c) { o[c][0] *= f0; o[c][1] *= f1; o[c][2] *= f0; o[c][3] *= f1; }
                 m[0] = top[0];
@@ -210,10 +210,7 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
             }
             float w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = s[i] == -INFINITY ? 0.0f : tc_exp2(s[i] - m[i & 1]);
-                l[i & 1] += w[i];
-            }
+            for (int i = 0; i < 4; ++i) w[i] = s[i] == -INFINITY ? 0.0f : tc_exp2(s[i] - m[i & 1]);
             uint32_t b[3][2];
             split3_bf16(w[0], w[1], b[0][0], b[1][0], b[2][0]);
             split3_bf16(w[2], w[3], b[0][1], b[1][1], b[2][1]);
@@ -221,6 +218,11 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
             for (int x = 0; x < 3; ++x)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) b[x][i] = st_turned(b[x][i]);
+            {       // the weights' sum by the products that O comes from, so that it is truncated like it
+                const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+                for (int x = 0; x < 3; ++x) mma_bf16_16816(l, ones, b[x][0], b[x][1]);
+            }
             cp_async_wait<1>();              // the values, not the next keys
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
@@ -266,11 +268,6 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
             j0 = j1;
         }
         cp_async_wait<0>();
-#pragma unroll
-        for (int w = 4; w < 32; w *= 2) {
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], w);
-            l[1] += __shfl_xor_sync(0xffffffffu, l[1], w);
-        }
         // the warps' parts, each in its own area: [row][columns], then references and sums
         __syncwarp();
         float* part = reinterpret_cast<float*>(area(warp));
@@ -496,18 +493,15 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
         const float slope = kOpts && p.slopes && live ? p.slopes[h] : 0.0f;
         const bool plain = !kOpts;           // weights are 2^(score * mul - ref): one rounding between a score and its exponential. Without caps or charges mul holds the scale, too
         const float mul = plain ? p.scale * kStLog2e : kStLog2e;
-        float flushed = -INFINITY;           // the reference of what has been flushed
-        auto store_flushed = [&](const uint32_t* o, int c) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(place + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        };
-        auto add_flushed = [&](uint32_t* o, int c) {        // carried over to the present reference
+        float flushed = -INFINITY, lw = 0.0f;        // the reference of what has been flushed; the weights' sum since then
+        float4* const flush = reinterpret_cast<float4*>(p.flush) + (size_t)blockIdx.x * (kStRows * HD / 4) + row;      // [columns / 4][rows]: a warp reads and writes whole lines
+        auto add_flushed = [&](uint32_t* o, int c) {        // thirty-two columns, carried over to the present reference
             const float f = flushed == ref ? 1.0f : tc_exp2(flushed - ref);
-            float4 w[4];
+            float4 w[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const float4*>(place + c + 4 * e);
+            for (int e = 0; e < 8; ++e) w[e] = __ldcg(flush + (size_t)(c / 4 + e) * kStRows);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 8; ++e) {
                 o[4 * e] = __float_as_uint(fmaf(w[e].x, f, __uint_as_float(o[4 * e])));
                 o[4 * e + 1] = __float_as_uint(fmaf(w[e].y, f, __uint_as_float(o[4 * e + 1])));
                 o[4 * e + 2] = __float_as_uint(fmaf(w[e].z, f, __uint_as_float(o[4 * e + 2])));
@@ -524,6 +518,20 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             ok = tc_wait_warp(sfull, (was + i) & 1, gave_up, sa.polls);
             if (!ok) break;
             tc_fence_after();
+            if (i % kStFlush == 0 && i > 0) {           // the product before this tile has completed: these scores follow it
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    tc_ld32_async(o_tmem + c, o);
+                    tc_arrived(o);
+                    if (i > kStFlush) add_flushed(o, c);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) __stcg(flush + (size_t)(c / 4 + e) * kStRows, make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3])));
+                }
+                l += lw;
+                lw = 0.0f;
+                flushed = ref;
+            }
             uint32_t s[64];
             tc_ld32_async(s_tmem, s);
             tc_ld32_async(s_tmem + 32, s + 32);
@@ -583,24 +591,12 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
 #pragma unroll
             for (int e = 0; e < 64; e += 2) m[(e / 2) & 3] = tc_max3(m[(e / 2) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
             const float mx = tc_max3(fmaxf(m[0], m[1]), m[2], m[3]) * mul;
-            if (i % kStFlush == 0 && i > 0) {           // the product before this tile has completed: these scores follow it
-#pragma unroll 1
-                for (int c = 0; c < HD; c += 16) {
-                    uint32_t o[16];
-                    st_ld16(o_tmem + c, o);
-                    if (live) {
-                        if (i > kStFlush) add_flushed(o, c);
-                        store_flushed(o, c);
-                    }
-                    __syncwarp();
-                }
-                flushed = ref;
-            }
             if (i == 0) {
                 ref = mx;
             } else if (__any_sync(0xffffffffu, mx > ref + 8.0f)) {
                 const float nr = fmaxf(ref, mx), f = nr == ref ? 1.0f : tc_exp2(ref - nr);
                 l *= f;
+                lw *= f;
                 ref = nr;
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 16) {
@@ -611,7 +607,7 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                     tc_st16(o_tmem + c, o);
                 }
             }
-            uint64_t sum = 0;                                                   // (0, 0)
+            uint64_t sum[4] = {};                                               // of a product's sixteen keys each
             const float base = ref == -INFINITY ? 0.0f : ref;                   // nothing seen yet: every weight is exp(-inf) = 0
             const uint64_t mul2 = tc_two(__float_as_uint(mul), __float_as_uint(mul)), base2 = tc_two(__float_as_uint(-base), __float_as_uint(-base));
             const uint64_t less = tc_two(__float_as_uint(-1.0f), __float_as_uint(-1.0f));
@@ -626,7 +622,7 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                     x = tc_exp2(x);
                     y = tc_exp2(y);
                     const uint64_t w = tc_two(__float_as_uint(x), __float_as_uint(y));
-                    sum = tc_add2(sum, w);
+                    sum[2 * half + e / 8] = tc_add2(sum[2 * half + e / 8], w);
                     hi[e] = tc_pack(x, y);
                     const uint64_t r = tc_fma2(terms(hi[e]), less, w);          // what the first terms leave: exact
                     tc_split(r, x, y);
@@ -638,13 +634,23 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 tc_st16(s_tmem + 32 + half * 16, mid);
                 tc_st16(s_tmem + 64 + half * 16, lo);
             }
-            float l0, l1;
-            tc_split(sum, l0, l1);
-            l += l0 + l1;
+            // The tensor core truncates as it adds: each of a tile's twelve products (four of first terms, four of second, four of third ones) loses half a unit of O's last place on average. The
+            // weights' sum is added up in the same twelve steps, truncated too, so that the quotient keeps a fraction of the loss only: with plain additions it was 2.6e-7 too small a tile.
+            float part[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float a, b;
+                tc_split(sum[k], a, b);
+                part[k] = a + b;
+            }
+            constexpr float k9 = 1.0f / 512, k18 = k9 * k9;                     // what is left of a weight behind its first term, behind its second: at most, to which the steps' sizes need not be exact
+#pragma unroll
+            for (int k = 0; k < 12; ++k) lw = __fadd_rz(lw, part[k % 4] * (k < 4 ? 1.0f - k9 : k < 8 ? k9 - k18 : k18));
             tc_wait_st();
             tc_fence_before();
             mb_arrive(pready);
         }
+        l += lw;
         if (ok && n > 0) ok = tc_wait_warp(odone, (was + n - 1) & 1, gave_up, sa.polls);
         tc_fence_after();
         if (ok && live) {
@@ -667,10 +673,7 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = 0u;
             }
-            if (n > kStFlush && live) {
-                add_flushed(o, c);
-                add_flushed(o + 16, c + 16);
-            }
+            if (n > kStFlush) add_flushed(o, c);
             __syncwarp();
             uint32_t got[16];        // (all of them before the first store: behind a store each shuffle waited)
 #pragma unroll
@@ -909,6 +912,8 @@ static int st_launch(const SharedArgs& p, cudaStream_t st) {
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
 }
+
+int64_t attention_shared_tc_flush_floats(int dk, int dv) { return dk == dv && (dk == 64 || dk == 128) ? 2LL * sm_count() * kStRows * dv : 0; }
 
 int launch_attention_shared_tc(const SharedArgs& p, cudaStream_t st) {
     const bool opts = p.softcap > 0.0f || p.slopes;
