@@ -21,17 +21,17 @@
 
 namespace sllm {
 
-constexpr int kStRows = 128, kStKeys = 64, kStThreads = 256, kStBox = 32, kStWarps = kStThreads / 32;
-constexpr int kStFlush = 7, kStEnds = 8;
-constexpr uint32_t kStTmem = 256;            // scores at 0 .. 63, then the weights' terms at 0 .. 95, O at 128; two CTAs share an SM's 512 columns
+constexpr int kStRows = 128, kStKeys = 48, kStThreads = 256, kStBox = 16, kStBoxes = kStKeys / kStBox, kStWarps = kStThreads / 32;
+constexpr int kStFlush = 9, kStEnds = 10;
+constexpr uint32_t kStTmem = 256, kStTerms = 48;       // scores at 0 .. 47, the weights' terms at 48, 72 and 96, O at 128; two CTAs share an SM's 512 columns
 constexpr int kStFew = 16, kStTeam = 4, kStTeams = kStWarps / kStTeam;      // rows of a segment up to which its own positions are a team's work; warps of a team
 constexpr float kStLog2e = 1.4426950408889634f;
 
 template <int HD>
 struct StShape {
     static constexpr int kBlocks = HD / 64, kQBlock = kStRows * 128, kQBytes = kBlocks * kQBlock, kKBlock = kStKeys * 128, kTile = kBlocks * kKBlock;
-    static constexpr int kStages = HD == 128 ? 2 : 4;
-    static constexpr int kBars = kQBytes + 2 * kStages * kTile, kPlan = kBars + 512, kSmem = 1024 + kPlan + 11 * 1024;
+    static constexpr int kKeyStages = HD == 128 ? 2 : 4, kValueStages = HD == 128 ? 3 : 4;      // tiles of keys and of values on their way or in use
+    static constexpr int kBars = kQBytes + (kKeyStages + kValueStages) * kTile, kPlan = kBars + 512, kSmem = 1024 + kPlan + 11 * 1024;
 };
 
 // The step's work as a CTA sees it: entries (groups, then listed tiles of queries), as many at a time as it has threads, and how many items each and those before it are.
@@ -64,12 +64,19 @@ struct StItem {
 __device__ __forceinline__ int st_token(const StArgs& sa, int row) { return (int)((uint32_t)row * sa.hpc_magic >> 16); }
 __device__ __forceinline__ int st_pos(const StArgs& sa, const StItem& it, int token) { return it.pos0 >= 0 ? it.pos0 + token : sa.a.b.tok_pos[it.tok0 + token]; }
 
-__device__ __forceinline__ void st_ld16(uint32_t taddr, uint32_t* o) {
+// columns of TMEM from registers and to registers; complete behind tc_wait_st and tc_wait_ld
+__device__ __forceinline__ void st_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void st_ld16_async(uint32_t taddr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]),
-                   "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15])
                  : "r"(taddr)
                  : "memory");
+}
+__device__ __forceinline__ void st_ld16(uint32_t taddr, uint32_t* o) {
+    st_ld16_async(taddr, o);
     tc_wait_ld();
 #pragma unroll
     for (int e = 0; e < 16; ++e) asm volatile("" : "+r"(o[e]));
@@ -322,13 +329,14 @@ __device__ __forceinline__ int* st_gave_up(uint8_t* smem) { return reinterpret_c
 // the barriers, in the order in which st_many has them
 template <int HD>
 __device__ __forceinline__ void st_barriers(uint8_t* smem) {
-    constexpr int ST = StShape<HD>::kStages;
+    constexpr int KS = StShape<HD>::kKeyStages, VS = StShape<HD>::kValueStages;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + StShape<HD>::kBars);
-    for (int i = 0; i < 4 * ST; ++i) mb_init(bar++, 1);          // keys full, keys empty, values full, values empty
-    for (int i = 0; i < ST; ++i) mb_init(bar++, 2);              // values ready
+    for (int i = 0; i < 2 * (KS + VS); ++i) mb_init(bar++, 1);          // keys full, keys empty, values full, values empty
+    for (int i = 0; i < VS; ++i) mb_init(bar++, 2);              // values ready
     mb_init(bar++, 128);                                         // queries ready
     mb_init(bar++, 1);                                           // scores full
     mb_init(bar++, 128);                                         // weights ready
+    mb_init(bar++, 128);                                         // scores read
     mb_init(bar, 1);                                             // O done
 }
 
@@ -349,11 +357,11 @@ struct StTiles {
 template <int HD, bool kOpts>
 __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const StArgs& sa, const StItem& it, uint8_t* smem, uint32_t tmem, uint32_t& done, uint32_t turn) {
     using Sh = StShape<HD>;
-    constexpr int ST = Sh::kStages;
+    constexpr int KS = Sh::kKeyStages, VS = Sh::kValueStages;
     const SharedArgs& p = sa.a;
-    uint8_t *sK = smem, *sV = sK + ST * Sh::kTile, *sQ = sV + ST * Sh::kTile;
+    uint8_t *sK = smem, *sV = sK + KS * Sh::kTile, *sQ = sV + VS * Sh::kTile;
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + Sh::kBars);
-    uint64_t *kempty = kfull + ST, *vfull = kempty + ST, *vempty = vfull + ST, *vready = vempty + ST, *qready = vready + ST, *sfull = qready + 1, *pready = sfull + 1, *odone = pready + 1;
+    uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *vready = vempty + VS, *qready = vready + VS, *sfull = qready + 1, *pready = sfull + 1, *sread = pready + 1, *odone = sread + 1;
     volatile int* gave_up = st_gave_up<HD>(smem);
     int* taken = st_gave_up<HD>(smem) + 1 + (turn & 1);          // whether values were taken out
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_rows = it.nq * sa.hpc;
@@ -399,25 +407,25 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
         if (elect_one()) {   // ===== TMA producer =====
             for (int i = 0; i < n; ++i) {
                 const int j0 = tiles.tile_of(i) * kStKeys;
-                const uint32_t s = (was + i) % ST, ph = (was + i) / ST & 1;
-                int at[2], row[2];
+                const uint32_t ks = (was + i) % KS, kph = (was + i) / KS & 1, vs = (was + i) % VS, vph = (was + i) / VS & 1;
+                int at[kStBoxes], row[kStBoxes];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < kStBoxes; ++x) {
                     int in_page;
                     const int pos = j0 + x * kStBox, page = pos < key1 && pos + kStBox > it.key0 ? sh_page(p, it.slot, pos, in_page) : -1;
                     at[x] = page >= 0 ? in_page : p.b.page_len;                     // outside the map: zeros
                     row[x] = page >= 0 ? page * p.kv_heads + it.g : 0;
                 }
-                if (!tc_wait(kempty + s, ph ^ 1, gave_up, sa.polls)) break;
-                mb_expect(kfull + s, Sh::kTile);
+                if (!tc_wait(kempty + ks, kph ^ 1, gave_up, sa.polls)) break;
+                mb_expect(kfull + ks, Sh::kTile);
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    for (int c = 0; c < Sh::kBlocks; ++c) tma_load_3d(sK + s * Sh::kTile + c * Sh::kKBlock + x * kStBox * 128, &tmK, 64 * c, at[x], row[x], kfull + s);
-                if (!tc_wait(vempty + s, ph ^ 1, gave_up, sa.polls)) break;
-                mb_expect(vfull + s, Sh::kTile);
+                for (int x = 0; x < kStBoxes; ++x)
+                    for (int c = 0; c < Sh::kBlocks; ++c) tma_load_3d(sK + ks * Sh::kTile + c * Sh::kKBlock + x * kStBox * 128, &tmK, 64 * c, at[x], row[x], kfull + ks);
+                if (!tc_wait(vempty + vs, vph ^ 1, gave_up, sa.polls)) break;
+                mb_expect(vfull + vs, Sh::kTile);
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    for (int c = 0; c < Sh::kBlocks; ++c) tma_load_3d(sV + s * Sh::kTile + c * Sh::kKBlock + x * kStBox * 128, &tmV, 64 * c, at[x], row[x], vfull + s);
+                for (int x = 0; x < kStBoxes; ++x)
+                    for (int c = 0; c < Sh::kBlocks; ++c) tma_load_3d(sV + vs * Sh::kTile + c * Sh::kKBlock + x * kStBox * 128, &tmV, 64 * c, at[x], row[x], vfull + vs);
             }
         }
         __syncwarp();
@@ -426,60 +434,69 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
             constexpr uint32_t idesc_s = umma_idesc_bf16(kStRows, kStKeys), idesc_o = umma_idesc_bf16(kStRows, HD) | (1u << 16);      // B MN-major
             const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sK), v_desc = umma_desc_mn_sw128(sV, Sh::kKBlock);  // + bytes / 16: another place
             auto scores = [&](int i) {
-                const uint64_t k = k_desc + (was + i) % ST * (Sh::kTile / 16);
+                const uint64_t k = k_desc + (was + i) % KS * (Sh::kTile / 16);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks)
                     tc_mma_bf16(tmem, q_desc + (uint32_t)((ks / 4) * (Sh::kQBlock / 16) + 2 * (ks % 4)), k + (uint32_t)((ks / 4) * (Sh::kKBlock / 16) + 2 * (ks % 4)), idesc_s, ks != 0);
                 tc_commit(sfull);
-                tc_commit(kempty + (was + i) % ST);
+                tc_commit(kempty + (was + i) % KS);
             };
-            bool ok = n > 0 && tc_wait(qready, turn & 1, gave_up, sa.polls) && tc_wait(kfull + was % ST, was / ST & 1, gave_up, sa.polls);
+            bool ok = n > 0 && tc_wait(qready, turn & 1, gave_up, sa.polls) && tc_wait(kfull + was % KS, was / KS & 1, gave_up, sa.polls);
             if (ok) {
                 tc_fence_after();
                 scores(0);
             }
             for (int i = 0; ok && i < n; ++i) {
                 const uint32_t at = was + i;
-                ok = tc_wait(vready + at % ST, at / ST & 1, gave_up, sa.polls) && tc_wait(pready, at & 1, gave_up, sa.polls);
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t v = v_desc + at % ST * (Sh::kTile / 16);
-#pragma unroll
-                for (int ks = 0; ks < 3 * kStKeys / 16; ++ks)                    // first terms, then second ones, then third ones, against the same values
-                    tc_mma_bf16_ts(tmem + 128, tmem + 8 * ks, v + (uint32_t)((ks % (kStKeys / 16)) * 128), idesc_o, (i % kStFlush | ks) != 0);
-                tc_commit(odone);
-                tc_commit(vempty + at % ST);
-                if (i + 1 < n) {        // the next scores land where the weights lie that this product is still reading
-                    ok = tc_wait(kfull + (at + 1) % ST, (at + 1) / ST & 1, gave_up, sa.polls) && tc_wait(odone, at & 1, gave_up, sa.polls);
+                if (i + 1 < n) {        // the next scores, as soon as these have been read
+                    ok = tc_wait(kfull + (at + 1) % KS, (at + 1) / KS & 1, gave_up, sa.polls) && tc_wait(sread, at & 1, gave_up, sa.polls);
                     if (!ok) break;
                     tc_fence_after();
                     scores(i + 1);
                 }
+                ok = tc_wait(vready + at % VS, at / VS & 1, gave_up, sa.polls) && tc_wait(pready, at & 1, gave_up, sa.polls);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t v = v_desc + at % VS * (Sh::kTile / 16);
+#pragma unroll
+                for (int ks = 0; ks < 3 * kStKeys / 16; ++ks)                    // first terms, then second ones, then third ones, against the same values
+                    tc_mma_bf16_ts(tmem + 128, tmem + kStTerms + 8 * ks, v + (uint32_t)((ks % (kStKeys / 16)) * 128), idesc_o, (i % kStFlush | ks) != 0);
+                tc_commit(odone);
+                tc_commit(vempty + at % VS);
             }
         }
         __syncwarp();
     } else if (warp >= 6) {   // ===== values that are not the share's, or no numbers =====
         for (int i = 0; i < n; ++i) {
-            const uint32_t s = (was + i) % ST;
+            const uint32_t s = (was + i) % VS;
             const int j0 = tiles.tile_of(i) * kStKeys, from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
-            if (!tc_wait_warp(vfull + s, (was + i) / ST & 1, gave_up, sa.polls)) break;
-            bool odd = false;
-#pragma unroll 8
-            for (int x = (warp - 6) * 32 + lane; x < kStKeys * 8 * Sh::kBlocks; x += 64) {      // (the rows of a block of 64 columns lie one behind the other)
-                const int r = x / 8 % kStKeys;
-                uint4* at = reinterpret_cast<uint4*>(sV + s * Sh::kTile + x * 16);
-                const uint4 v = *at;
-                uint32_t sum = 0;
-                st_times_zero(sum, v);
-                if (r < from || r >= to) {
-                    *at = make_uint4(0u, 0u, 0u, 0u);
-                } else if (st_odd(sum)) {
-                    *at = st_without(v);
-                    odd = true;
+            if (!tc_wait_warp(vfull + s, (was + i) / VS & 1, gave_up, sa.polls)) break;
+            constexpr int kLoads = kStKeys * 8 * Sh::kBlocks / 64;                       // 16 bytes each, all on their way before the first is looked at
+            uint4* const at = reinterpret_cast<uint4*>(sV + s * Sh::kTile) + (warp - 6) * 32 + lane;      // (the rows of a block of 64 columns lie one behind the other)
+            uint4 v[kLoads];
+            uint32_t sum[4] = {};
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x) v[x] = at[64 * x];
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x) st_times_zero(sum[x % 4], v[x]);
+            bool odd = st_odd(sum[0]) || st_odd(sum[1]) || st_odd(sum[2]) || st_odd(sum[3]);
+            if (from > 0 || to < kStKeys || __any_sync(0xffffffffu, odd)) {
+                odd = false;
+#pragma unroll
+                for (int x = 0; x < kLoads; ++x) {
+                    const int r = (x * 64 + (warp - 6) * 32 + lane) / 8 % kStKeys;
+                    uint32_t one = 0;
+                    st_times_zero(one, v[x]);
+                    if (r < from || r >= to) {
+                        at[64 * x] = make_uint4(0u, 0u, 0u, 0u);
+                    } else if (st_odd(one)) {
+                        at[64 * x] = st_without(v[x]);
+                        odd = true;
+                    }
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             if (odd) *taken = 1;
-            if (from > 0 || to < kStKeys || __any_sync(0xffffffffu, odd)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mb_arrive(vready + s);
         }
@@ -508,17 +525,28 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 o[4 * e + 3] = __float_as_uint(fmaf(w[e].w, f, __uint_as_float(o[4 * e + 3])));
             }
         };
+        constexpr uint64_t kAll = (1ull << kStKeys) - 1;
+        // what the block table has for a tile's first key and its last (pages are a multiple of 32 positions: two of them at most), a tile ahead and not looked at before then: a lookup that is looked at holds everything up until it has arrived
+        auto entry = [&](int pos) {
+            int in_page;
+            const int at = page_of(pos, p.b.page_len, p.page_magic, in_page);
+            return it.slot >= 0 && at < p.b.max_pages ? p.b.block_table[(size_t)it.slot * p.b.max_pages + at] : -1;
+        };
+        int next0 = -1, next1 = -1;
+        if (n > 0) {
+            const int j0 = tiles.tile_of(0) * kStKeys;
+            next0 = entry(j0);
+            next1 = entry(min(j0 + kStKeys, key1) - 1);
+        }
         for (int i = 0; i < n; ++i) {
             const int j0 = tiles.tile_of(i) * kStKeys;
-            // keys of the tile that are in the share and in a page
-            const int from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
-            uint64_t have = (to >= 64 ? ~0ull : (1ull << to) - 1) & ~((1ull << from) - 1);
-            int in_page;
-            const int page0 = sh_page(p, it.slot, j0, in_page), page1 = sh_page(p, it.slot, min(j0 + kStBox, key1 - 1), in_page);      // (on their way while the scores are made)
             ok = tc_wait_warp(sfull, (was + i) & 1, gave_up, sa.polls);
             if (!ok) break;
             tc_fence_after();
-            if (i % kStFlush == 0 && i > 0) {           // the product before this tile has completed: these scores follow it
+            if (i % kStFlush == 0 && i > 0) {
+                ok = tc_wait_warp(odone, (was + i - 1) & 1, gave_up, sa.polls);
+                if (!ok) break;
+                tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t o[32];
@@ -532,21 +560,37 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 lw = 0.0f;
                 flushed = ref;
             }
-            uint32_t s[64];
+            const bool page0 = (unsigned)next0 < (unsigned)p.n_pages, page1 = (unsigned)next1 < (unsigned)p.n_pages;
+            if (i + 1 < n) {
+                const int j1 = tiles.tile_of(i + 1) * kStKeys;
+                next0 = entry(j1);
+                next1 = entry(min(j1 + kStKeys, key1) - 1);
+            }
+            uint32_t s[kStKeys];
             tc_ld32_async(s_tmem, s);
-            tc_ld32_async(s_tmem + 32, s + 32);
+            st_ld16_async(s_tmem + 32, s + 32);
             tc_arrived(s);
-            tc_arrived(s + 32);
-            if (page0 < 0) have &= ~0xffffffffull;
-            if (page1 < 0) have &= 0xffffffffull;
-            // every key of the tile is visible to every row of the warp
-            const bool all = have == ~0ull && __all_sync(0xffffffffu, !live || (j0 + kStKeys - 1 <= qpos && (qpos - j0 < p.window || j0 + kStKeys <= p.keep_first)));
+#pragma unroll
+            for (int e = 32; e < kStKeys; ++e) asm volatile("" : "+r"(s[e]));
+            tc_fence_before();
+            mb_arrive(sread);
+            // whether every row of the tile sees every key: as a rule the positions of the rows say so at once
+            uint64_t have = kAll;
+            bool all = j0 >= it.key0 && j0 + kStKeys <= key1 && page0 && page1 && j0 + kStKeys - 1 <= it.low && (it.high - j0 < p.window || j0 + kStKeys <= p.keep_first);
+            if (!all) {          // keys of the tile that are in the share and in a page
+                const int from = max(0, it.key0 - j0), to = min(kStKeys, key1 - j0);
+                int in_page;
+                page_of(j0, p.b.page_len, p.page_magic, in_page);
+                const uint64_t first = (1ull << min(kStKeys, p.b.page_len - in_page)) - 1;
+                have = ((1ull << to) - 1) & ~((1ull << from) - 1) & ((page0 ? first : 0ull) | (page1 ? ~first : 0ull));
+                all = have == kAll && __all_sync(0xffffffffu, !live || (j0 + kStKeys - 1 <= qpos && (qpos - j0 < p.window || j0 + kStKeys <= p.keep_first)));
+            }
             if (kOpts && p.softcap > 0.0f) {
                 const float inv = p.scale / p.softcap;
                 const uint64_t inv2 = tc_two(__float_as_uint(inv), __float_as_uint(inv));
                 float top0 = 0.0f, top1 = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 64; e += 2) {
+                for (int e = 0; e < kStKeys; e += 2) {
                     float x, y;
                     tc_split(tc_mul2(tc_two(s[e], s[e + 1]), inv2), x, y);
                     s[e] = __float_as_uint(x);
@@ -557,12 +601,12 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 // scores within a quarter of the cap, as nearly all are: the series that tc_tanh takes for them, two at a time
                 if (__any_sync(0xffffffffu, fmaxf(top0, top1) >= 0.25f)) {
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(p.softcap * tc_tanh(__uint_as_float(s[e])));
+                    for (int e = 0; e < kStKeys; ++e) s[e] = __float_as_uint(p.softcap * tc_tanh(__uint_as_float(s[e])));
                 } else {
                     auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
                     const uint64_t c4 = both(62.0f / 2835.0f), c3 = both(-17.0f / 315.0f), c2 = both(2.0f / 15.0f), c1 = both(-1.0f / 3.0f), c0 = both(1.0f), cap2 = both(p.softcap);
 #pragma unroll
-                    for (int e = 0; e < 64; e += 2) {
+                    for (int e = 0; e < kStKeys; e += 2) {
                         const uint64_t x = tc_two(s[e], s[e + 1]), x2 = tc_mul2(x, x);
                         float a, c;
                         tc_split(tc_mul2(cap2, tc_mul2(x, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, tc_fma2(x2, c4, c3), c2), c1), c0))), a, c);
@@ -572,28 +616,31 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 }
             } else if (!plain) {
 #pragma unroll
-                for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * p.scale);
+                for (int e = 0; e < kStKeys; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * p.scale);
             }
             if (kOpts && p.slopes) {
                 const float d0 = (float)(qpos - j0);
 #pragma unroll
-                for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(fmaf(-slope, d0 - (float)e, __uint_as_float(s[e])));
+                for (int e = 0; e < kStKeys; ++e) s[e] = __float_as_uint(fmaf(-slope, d0 - (float)e, __uint_as_float(s[e])));
             }
             if (!all) {          // the keys of the tile that this row sees, a bit each: up to its own position, and from the window's oldest on or among the first
-                auto below = [&](int key) { return key <= j0 ? 0ull : key >= j0 + 64 ? ~0ull : (1ull << (key - j0)) - 1; };
+                auto below = [&](int key) { return key <= j0 ? 0ull : key >= j0 + kStKeys ? ~0ull : (1ull << (key - j0)) - 1; };
                 const uint64_t sees = have & below(qpos + 1) & (~below(p.window > qpos ? 0 : qpos - p.window + 1) | below(p.keep_first));
                 const uint32_t seen[2] = {(uint32_t)sees, (uint32_t)(sees >> 32)};
 #pragma unroll
-                for (int e = 0; e < 64; ++e)
+                for (int e = 0; e < kStKeys; ++e)
                     if (!(seen[e / 32] >> (e % 32) & 1)) s[e] = 0xff800000u;       // -inf
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 64; e += 2) m[(e / 2) & 3] = tc_max3(m[(e / 2) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            for (int e = 0; e < kStKeys; e += 2) m[(e / 2) & 3] = tc_max3(m[(e / 2) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
             const float mx = tc_max3(fmaxf(m[0], m[1]), m[2], m[3]) * mul;
             if (i == 0) {
                 ref = mx;
             } else if (__any_sync(0xffffffffu, mx > ref + 8.0f)) {
+                ok = tc_wait_warp(odone, (was + i - 1) & 1, gave_up, sa.polls);
+                if (!ok) break;
+                tc_fence_after();
                 const float nr = fmaxf(ref, mx), f = nr == ref ? 1.0f : tc_exp2(ref - nr);
                 l *= f;
                 lw *= f;
@@ -607,22 +654,22 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                     tc_st16(o_tmem + c, o);
                 }
             }
-            uint64_t sum[4] = {};                                               // of a product's sixteen keys each
             const float base = ref == -INFINITY ? 0.0f : ref;                   // nothing seen yet: every weight is exp(-inf) = 0
             const uint64_t mul2 = tc_two(__float_as_uint(mul), __float_as_uint(mul)), base2 = tc_two(__float_as_uint(-base), __float_as_uint(-base));
             const uint64_t less = tc_two(__float_as_uint(-1.0f), __float_as_uint(-1.0f));
             auto terms = [](uint32_t w) { return tc_two(w << 16, w & 0xffff0000u); };
+            uint64_t sum[kStKeys / 16] = {};                                    // of a product's sixteen keys each
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t hi[16], mid[16], lo[16];
+            for (int part = 0; part < kStKeys / 16; ++part) {
+                uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < 8; ++e) {
                     float x, y;
-                    tc_split(tc_fma2(tc_two(s[half * 32 + 2 * e], s[half * 32 + 2 * e + 1]), mul2, base2), x, y);
+                    tc_split(tc_fma2(tc_two(s[part * 16 + 2 * e], s[part * 16 + 2 * e + 1]), mul2, base2), x, y);
                     x = tc_exp2(x);
                     y = tc_exp2(y);
                     const uint64_t w = tc_two(__float_as_uint(x), __float_as_uint(y));
-                    sum[2 * half + e / 8] = tc_add2(sum[2 * half + e / 8], w);
+                    sum[part] = tc_add2(sum[part], w);
                     hi[e] = tc_pack(x, y);
                     const uint64_t r = tc_fma2(terms(hi[e]), less, w);          // what the first terms leave: exact
                     tc_split(r, x, y);
@@ -630,25 +677,31 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                     tc_split(tc_fma2(terms(mid[e]), less, r), x, y);
                     lo[e] = tc_pack(x, y);
                 }
-                tc_st16(s_tmem + half * 16, hi);
-                tc_st16(s_tmem + 32 + half * 16, mid);
-                tc_st16(s_tmem + 64 + half * 16, lo);
+                if (part == 0 && i > 0) {            // the product before this one still reads where the weights go
+                    ok = tc_wait_warp(odone, (was + i - 1) & 1, gave_up, sa.polls);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                st_st8(s_tmem + kStTerms + part * 8, hi);
+                st_st8(s_tmem + kStTerms + kStKeys / 2 + part * 8, mid);
+                st_st8(s_tmem + kStTerms + kStKeys + part * 8, lo);
             }
-            // The tensor core truncates as it adds: each of a tile's twelve products (four of first terms, four of second, four of third ones) loses half a unit of O's last place on average. The
-            // weights' sum is added up in the same twelve steps, truncated too, so that the quotient keeps a fraction of the loss only: with plain additions it was 2.6e-7 too small a tile.
-            float part[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float a, b;
-                tc_split(sum[k], a, b);
-                part[k] = a + b;
-            }
-            constexpr float k9 = 1.0f / 512, k18 = k9 * k9;                     // what is left of a weight behind its first term, behind its second: at most, to which the steps' sizes need not be exact
-#pragma unroll
-            for (int k = 0; k < 12; ++k) lw = __fadd_rz(lw, part[k % 4] * (k < 4 ? 1.0f - k9 : k < 8 ? k9 - k18 : k18));
+            if (!ok) break;
             tc_wait_st();
             tc_fence_before();
             mb_arrive(pready);
+            // The tensor core truncates as it adds: each of a tile's nine products (three of first terms, three of second, three of third ones) loses half a unit of O's last place on average. The
+            // weights' sum is added up in the same nine steps, truncated too, so that the quotient keeps a fraction of the loss only: with plain additions it was 2e-7 too small a tile.
+            constexpr float k9 = 1.0f / 512, k18 = k9 * k9;                     // what is left of a weight behind its first term, behind its second: at most, to which the steps' sizes need not be exact
+            float steps[kStKeys / 16];
+#pragma unroll
+            for (int k = 0; k < kStKeys / 16; ++k) {
+                float a, b;
+                tc_split(sum[k], a, b);
+                steps[k] = a + b;
+            }
+#pragma unroll
+            for (int k = 0; k < 3 * kStKeys / 16; ++k) lw = __fadd_rz(lw, steps[k % (kStKeys / 16)] * (k < kStKeys / 16 ? 1.0f - k9 : k < kStKeys / 8 ? k9 - k18 : k18));
         }
         l += lw;
         if (ok && n > 0) ok = tc_wait_warp(odone, (was + n - 1) & 1, gave_up, sa.polls);
