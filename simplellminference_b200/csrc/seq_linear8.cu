@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kL8TcThreads, 1) linear8_tc_kernel(const __gri
 }
 
 // Tokens of a tile, SMs (or CTAs of K) that share one: the cheapest of all, a stage reckoned at what its products or its bytes take (clocks), a wave of tiles at its beginning and end beside its
-// stages. us without and with pairs, the rows' quantisation aside: 2000 x 4096 x 14336 90 | L8A.
+// stages. us without and with pairs, the rows' quantisation aside: 2000 x 4096 x 14336 87 | 78, 2000 x 14336 x 4096 95 | 85, 512 x 4096 x 4096 13.4 | 14.5.
 struct Linear8Plan { int bn, split, pair; };
 static Linear8Plan l8_plan(int T, int N, int K) {
     const int sms = sm_count(), blocks = (K + kL8Block - 1) / kL8Block, most = std::min(256, (T + 15) / 16 * 16);
@@ -403,7 +403,7 @@ static Linear8Plan l8_plan(int T, int N, int K) {
                 if (split > 1 && bn > 128) break;
                 const long long units = (long long)((N + (pair ? 255 : 127)) / (pair ? 256 : 128)) * ((T + bn - 1) / bn) * split, workers = pair ? sms / 2 : sms;
                 const double stage = std::max(2.0 * bn, (kL8RowBytes + (pair ? bn / 2 : bn) * kL8Block) / 60.0);
-                const double cost = (double)((units + workers - 1) / workers) * (((blocks + split - 1) / split) * stage + (split > 1 ? 4000.0 : 1500.0 + 4.0 * bn));
+                const double cost = (double)((units + workers - 1) / workers) * (((blocks + split - 1) / split) * stage + (split > 1 ? 4000.0 : (pair ? 3500.0 : 1500.0) + 4.0 * bn));
                 if (cost < least - 1e-9) { least = cost; best = {bn, split, pair}; }
             }
     return best;
@@ -473,7 +473,7 @@ int sllm_seq_quantise_rows(const void* x, int32_t x_bf16, int64_t ldx, void* cod
     const bool vec = K % run == 0 && ldx % run == 0 && ((uintptr_t)x % 16) == 0 && ldc % run == 0 && ((uintptr_t)codes % run) == 0;
     QuantiseArgs p{x, (int8_t*)codes, scales, ldx, ldc, T, K};
     // threads of a row: where there are rows enough, as few as keep it in registers, so that each has eight loads on their way; else four times as many. us, few | many: 14336 rows of 4096 in bf16
-    // QZA, one row of 4096 in fp32 QZB
+    // 36 | 54, one row of 4096 in fp32 2.2 | 1.9
     const int loads = vec ? K / run : K;
     const bool many = (long long)T * loads >= 4096LL * sm_count();
     const int each = many ? kQzLoads : kQzFewLoads, threads = (std::min(kQzWide, (loads + each - 1) / each) + 31) / 32 * 32, rows = threads >= kQzThreads ? 1 : kQzThreads / threads;

@@ -253,3 +253,25 @@ def test_waits_that_run_out_are_reported():
         assert lib.sllm_tune(10, 1 << 24) == 0
     assert e.value.code == _lib.ETIMEOUT and lib.sllm_status() == 0
     _close(s.run()[0], s.want())
+
+
+@pytest.mark.parametrize("opts", [{}, {"softcap": 30.0}, {"window": 700, "keep_first": 3}], ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_enough_for_long_shares(dim, opts):
+    """So many rows that a share of the keys is longer than what the tensor core adds up at a time; the scores of later keys are the largest. Scores of up to 40 in size: three times
+    2^-24 * (40 + 16 + 20) over a row's norm, and over the sums of a share the tensor core's truncated additions (nine a tile, nine tiles), a unit of 2^-24 each at most, half of which the weights'
+    sum loses too."""
+    s = SharedStep([(1500, [(0, 400), (7, 200)]), (900, [(0, 1)] * 3)], 32, 8, dim, seed=dim)
+    for at in s.table_np[0, 14:22]:
+        s.k[at] *= 3
+    got, want = s.run(**opts)[0].double(), s.want(window=opts.get("window", 0), keep=opts.get("keep_first", 0), cap=opts.get("softcap", 0.0))
+    assert torch.isfinite(got).all()
+    assert (got - want).norm() <= (3 * 2.0 ** -24 * 76 + 2.0 ** -25 * 81) * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [257, 600])
+def test_many_groups(n, dtype):
+    """More groups than a CTA looks at in one turn."""
+    s = SharedStep([((13 * i) % 150, _owns(1 + (i % 97 == 5) * 3, 60, 1 + (i % 101 == 7) * 20)) for i in range(n)], 4, 2, 64, dtype=dtype)
+    _close(s.run()[0], s.want())
