@@ -11,6 +11,9 @@ namespace sllm {
 
 // Any head width, pools in fp32 or bf16: a CTA takes 4 * kRw rows of a (group or segment, kv head) and a share of the keys, 32 at a time through shared memory; a warp has kRw rows, a lane one
 // key of them for the scores and four columns of the values for the sums; fp32 throughout.
+// Bound: a chain. Four answers of 16 heads of 64 behind 1500 positions 18.6 us with the last kernel, which are, in clocks: whose share it is 2900, queries and pages 3000, for each of its two key
+// tiles keys and values 3800, scores 1600, weights 1800 (the rows' shuffles side by side), sums 2000 (a key's four weights read together, nothing asked in between; with a question per key and row
+// they took 9500).
 constexpr int kShWarps = 4, kShKeys = 32;
 
 struct ShSpan {                          // rows and keys of a CTA
@@ -45,16 +48,7 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
     const int ldk = p.dk + 4, cols = (p.dv + 127) / 128;
     float *s_q = smem, *s_k = s_q + kRows * p.dk, *s_v = s_k + kShKeys * ldk, *s_p = s_v + kShKeys * p.dv;      // s_p: [warp][key][row]
     for (int r0 = 0; r0 < sp.n_rows; r0 += kRows) {
-        __syncthreads();
-        // (rows behind the last one are the last one again; nothing asks for their results)
-        sh_stage<4>(kRows * p.dk / 4, [&](int i) {
-            const int r = min(r0 + 4 * i / p.dk, sp.n_rows - 1), c = 4 * i % p.dk;
-            const float* src = p.q + (size_t)(sp.tok0 + r / per) * p.ldq + (size_t)(g * per + r % per) * p.dk + c;
-            return make_float4(src[0], src[1], src[2], src[3]);
-        }, [&](int i, const float4& x) {
-            // as the products on the tensor cores take it
-            *reinterpret_cast<float4*>(s_q + 4 * i) = sizeof(T) == 2 ? make_float4(seq_round_bf16(x.x), seq_round_bf16(x.y), seq_round_bf16(x.z), seq_round_bf16(x.w)) : x;
-        });
+        int in_page, page = sh_page(p, sp.slot, sp.key0 / kShKeys * kShKeys, in_page);           // (pages are a multiple of 32 positions)
         int pos[kRw];
         float m[kRw], l[kRw], o[kRw][2][4], slope[kRw];
 #pragma unroll
@@ -67,9 +61,18 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
 #pragma unroll
             for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] = 0.0f;
         }
+        __syncthreads();
+        // (rows behind the last one are the last one again; nothing asks for their results)
+        sh_stage<4>(kRows * p.dk / 4, [&](int i) {
+            const int r = min(r0 + 4 * i / p.dk, sp.n_rows - 1), c = 4 * i % p.dk;
+            const float* src = p.q + (size_t)(sp.tok0 + r / per) * p.ldq + (size_t)(g * per + r % per) * p.dk + c;
+            return make_float4(src[0], src[1], src[2], src[3]);
+        }, [&](int i, const float4& x) {
+            // as the products on the tensor cores take it
+            *reinterpret_cast<float4*>(s_q + 4 * i) = sizeof(T) == 2 ? make_float4(seq_round_bf16(x.x), seq_round_bf16(x.y), seq_round_bf16(x.z), seq_round_bf16(x.w)) : x;
+        });
         for (int j0 = sp.key0 / kShKeys * kShKeys; j0 < sp.key1; j0 += kShKeys) {
-            int in_page;
-            const int page = sh_page(p, sp.slot, j0, in_page);           // (pages are a multiple of 32 positions)
+            if (j0 > sp.key0) page = sh_page(p, sp.slot, j0, in_page);
             // hidden from every row of the CTA: before its window, or no page
             int seen = 0;
 #pragma unroll
@@ -79,29 +82,31 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
             int odd = 0;                                                 // a value that is infinite or NaN
             const T *kr = reinterpret_cast<const T*>(p.k_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page, p.dk);
             const T *vr = reinterpret_cast<const T*>(p.v_pool) + seq_pool_row(page, p.kv_heads, g, p.b.page_len, in_page, p.dv);
-            sh_stage<4>(kShKeys * p.dk / kPer, [&](int i) { return ld_stream(kr + i * kPer); }, [&](int i, const uint4& v) {
-                const int at = i * kPer, k = at / p.dk;
+            const int n_k = kShKeys * p.dk / kPer;
+            sh_stage<8>(n_k + kShKeys * p.dv / kPer, [&](int i) { return ld_stream(i < n_k ? kr + i * kPer : vr + (i - n_k) * kPer); }, [&](int i, const uint4& v) {
                 float x[kPer];
                 sh_floats(v, x);
+                float* to;
+                if (i < n_k) {
+                    const int at = i * kPer, k = at / p.dk;
+                    to = s_k + k * ldk + at - k * p.dk;
+                } else {
+                    const int at = (i - n_k) * kPer, k = j0 + at / p.dv;
+                    const bool in = k >= sp.key0 && k < sp.key1;
+                    to = s_v + at;
 #pragma unroll
-                for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(s_k + k * ldk + at - k * p.dk + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-            });
-            sh_stage<4>(kShKeys * p.dv / kPer, [&](int i) { return ld_stream(vr + i * kPer); }, [&](int i, const uint4& v) {
-                const int at = i * kPer, k = j0 + at / p.dv;
-                const bool in = k >= sp.key0 && k < sp.key1;
-                float x[kPer];
-                sh_floats(v, x);
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    x[e] = in ? x[e] : 0.0f;
-                    odd |= !(fabsf(x[e]) <= FLT_MAX);
+                    for (int e = 0; e < kPer; ++e) {
+                        x[e] = in ? x[e] : 0.0f;
+                        odd |= !(fabsf(x[e]) <= FLT_MAX);
+                    }
                 }
 #pragma unroll
-                for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(s_v + at + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
             });
             odd = __syncthreads_or(odd);
             const int key = j0 + lane;
             float s[kRw] = {};
+#pragma unroll 4
             for (int c = 0; c < p.dk; c += 4) {
                 const float4 k = *reinterpret_cast<const float4*>(s_k + lane * ldk + c);
 #pragma unroll
@@ -111,35 +116,50 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
                 }
             }
             unsigned sees[kRw];
+            float top[kRw], f[kRw];
 #pragma unroll
             for (int i = 0; i < kRw; ++i) {
                 const bool here = key >= sp.key0 && key < sp.key1 && seq_sees(pos[i], key, p.window, p.keep_first);
                 sees[i] = __ballot_sync(0xffffffffu, here);
-                const float x = here ? sh_score(s[i] * p.scale, p.softcap, slope[i], pos[i], key) : -INFINITY;
-                const float top = fmaxf(m[i], warp_max(x));
-                const float f = top == -INFINITY ? 1.0f : fmaxf(expf(m[i] - top), FLT_MIN), w = x == -INFINITY ? 0.0f : expf(x - top);
-                m[i] = top;
-                l[i] = l[i] * f + warp_sum(w);
+                s[i] = here ? sh_score(s[i] * p.scale, p.softcap, slope[i], pos[i], key) : -INFINITY;
+                top[i] = s[i];
+            }
 #pragma unroll
-                for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] *= f;
+            for (int d = 16; d > 0; d /= 2)              // (the rows side by side: each step waits for the one before)
+#pragma unroll
+                for (int i = 0; i < kRw; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], d));
+#pragma unroll
+            for (int i = 0; i < kRw; ++i) {
+                top[i] = fmaxf(m[i], top[i]);
+                f[i] = top[i] == -INFINITY ? 1.0f : fmaxf(expf(m[i] - top[i]), FLT_MIN);
+                const float w = s[i] == -INFINITY ? 0.0f : expf(s[i] - top[i]);
+                m[i] = top[i];
+                l[i] = fmaf(l[i], f[i], w);              // of this lane's keys
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] *= f[i];
                 s_p[(warp * kShKeys + lane) * kRw + i] = w;
             }
             __syncwarp();
-            for (int k = 0; k < kShKeys; ++k) {
-                float w[kRw];
+            static_assert(kRw == 4, "a key's weights are read together");
 #pragma unroll
-                for (int i = 0; i < kRw; ++i) w[i] = s_p[(warp * kShKeys + k) * kRw + i];
+            for (int c = 0; c < 2; ++c) {
+                const int col = c * 128 + 4 * lane;
+                if (c >= cols || col >= p.dv) break;
+                auto add = [&](int i, float x, const float4& v) {
+                    o[i][c][0] = fmaf(x, v.x, o[i][c][0]); o[i][c][1] = fmaf(x, v.y, o[i][c][1]); o[i][c][2] = fmaf(x, v.z, o[i][c][2]); o[i][c][3] = fmaf(x, v.w, o[i][c][3]);
+                };
+                if (!odd) {
+#pragma unroll 8
+                    for (int k = 0; k < kShKeys; ++k) {
+                        const float4 w = *reinterpret_cast<const float4*>(s_p + (warp * kShKeys + k) * kRw), v = *reinterpret_cast<const float4*>(s_v + k * p.dv + col);
+                        add(0, w.x, v); add(1, w.y, v); add(2, w.z, v); add(3, w.w, v);
+                    }
+                } else {
+                    for (int k = 0; k < kShKeys; ++k) {
+                        const float4 v = *reinterpret_cast<const float4*>(s_v + k * p.dv + col);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int col = c * 128 + 4 * lane;
-                    if (c >= cols || col >= p.dv) break;
-                    const float4 v = *reinterpret_cast<const float4*>(s_v + k * p.dv + col);
-#pragma unroll
-                    for (int i = 0; i < kRw; ++i) {
-                        if (odd && !(sees[i] >> k & 1)) continue;
-                        const float x = odd ? fmaxf(w[i], FLT_MIN) : w[i];
-                        o[i][c][0] = fmaf(x, v.x, o[i][c][0]); o[i][c][1] = fmaf(x, v.y, o[i][c][1]);
-                        o[i][c][2] = fmaf(x, v.z, o[i][c][2]); o[i][c][3] = fmaf(x, v.w, o[i][c][3]);
+                        for (int i = 0; i < kRw; ++i)
+                            if (sees[i] >> k & 1) add(i, fmaxf(s_p[(warp * kShKeys + k) * kRw + i], FLT_MIN), v);
                     }
                 }
             }
@@ -150,9 +170,10 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
             const int r = r0 + warp * kRw + i;
             if (r >= sp.n_rows) break;
             float* rec = sh_record(p, sp.tok0 + r / per, g * per + r % per, sp.which);
+            const float sum = warp_sum(l[i]);
             if (lane == 0) {
                 rec[0] = m[i] * 1.4426950408889634f;
-                rec[1] = l[i];
+                rec[1] = sum;
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -202,8 +223,8 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
     sh_rows<T, kRw>(p, sp, g, sh_smem);
 }
 
-// The records of a (token, head) put together: a warp each. Bound: three loads one behind the other (the tile, references and sums, values eight records at a time).
-template <bool kVec>         // results 16 bytes at a time
+// The records of a (token, head) put together: a warp each. Bound: loads one behind the other (the tile, its segment, kAhead records at a time).
+template <bool kVec, int kAhead>         // results 16 bytes at a time; records on their way at once
 __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedArgs p) {
     after_previous();
     const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], cuts = p.plan[blockIdx.x], lane = threadIdx.x & 31;
@@ -220,6 +241,13 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
             head[x] = *reinterpret_cast<const float2*>(place(min(k, max(count, 1) - 1)));
             if (k >= count) head[x] = make_float2(-INFINITY, 0.0f);
         }
+        // kAhead records' columns at a time, the first of them on their way while the factors are made
+        float4 x[kAhead];
+        auto fetch = [&](int k0, int c) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) x[k] = *reinterpret_cast<const float4*>(place(min(k0 + k, max(count, 1) - 1)) + kShHead + min(c * 128 + 4 * lane, p.dv - 4));
+        };
+        fetch(0, 0);
         const float top = warp_max(fmaxf(head[0].x, head[1].x));
         float f[2], sum = 0.0f, o[2][4] = {};
 #pragma unroll
@@ -229,19 +257,16 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
             sum = fmaf(f[x], head[x].y, sum);
         }
         sum = warp_sum(sum);
-        for (int k0 = 0; k0 < count; k0 += 8) {
-            float w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = k0 + k < count ? __shfl_sync(0xffffffffu, k0 < 32 ? f[0] : f[1], (k0 + k) & 31) : 0.0f;
+        for (int c = 0; c < 2; ++c) {
+            if (c * 128 >= p.dv) break;
+            for (int k0 = 0; k0 < count; k0 += kAhead) {
+                if (c + k0 > 0) fetch(k0, c);
+                float w[kAhead];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = c * 128 + 4 * lane;
-                if (c * 128 >= p.dv) break;
-                float4 x[8];
+                for (int k = 0; k < kAhead; ++k) w[k] = __shfl_sync(0xffffffffu, k0 < 32 ? f[0] : f[1], (k0 + k) & 31);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = *reinterpret_cast<const float4*>(place(min(k0 + k, count - 1)) + kShHead + min(col, p.dv - 4));
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < kAhead; ++k) {
                     if (k0 + k >= count) break;
                     o[c][0] = fmaf(w[k], x[k].x, o[c][0]); o[c][1] = fmaf(w[k], x[k].y, o[c][1]); o[c][2] = fmaf(w[k], x[k].z, o[c][2]); o[c][3] = fmaf(w[k], x[k].w, o[c][3]);
                 }
@@ -280,7 +305,13 @@ static int sh_merge(const SharedArgs& p, cudaStream_t st) {
     const int most = (p.b.T == p.b.nseg ? p.heads : kBQ * p.heads) / 4 + 1;
     const bool vec = p.ldo % 4 == 0 && ((uintptr_t)p.out % 16) == 0 && ((uintptr_t)p.out16 % 8) == 0;
     LaunchCfg lc(dim3(p.b.n_qtiles, std::min(most, 256)), dim3(128), 0, st, true);
-    SLLM_CUDA(cudaLaunchKernelEx(&lc.cfg, vec ? overlapping(seq_attention_shared_merge_kernel<true>) : overlapping(seq_attention_shared_merge_kernel<false>), p));
+    // records on their way: few rows have many records each and wait for them, many rows few, and CTAs enough to wait beside one another. us of the whole call, 4 | 16: 4 answers behind 1500 positions
+    // in fp32 20.2 | 18.6, 64 behind 8000 62.8 | 60.7, 512 rows behind 4000 110.6 | 119.5
+    const bool few = (long long)p.b.T * p.heads < 16LL * sm_count();
+    auto launch = [&](auto whole, auto ahead) { return cudaLaunchKernelEx(&lc.cfg, overlapping(seq_attention_shared_merge_kernel<whole.value, ahead.value>), p); };
+    using four = std::integral_constant<int, 4>;
+    using sixteen = std::integral_constant<int, 16>;
+    SLLM_CUDA(vec ? few ? launch(std::true_type{}, sixteen{}) : launch(std::true_type{}, four{}) : few ? launch(std::false_type{}, sixteen{}) : launch(std::false_type{}, four{}));
     ++g_launches;
     SLLM_LAUNCH_CHECK_ONLY();
     return SLLM_OK;
