@@ -159,7 +159,12 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
                         const float4 v = *reinterpret_cast<const float4*>(s_v + k * p.dv + col);
 #pragma unroll
                         for (int i = 0; i < kRw; ++i)
-                            if (sees[i] >> k & 1) add(i, fmaxf(s_p[(warp * kShKeys + k) * kRw + i], FLT_MIN), v);
+                            if (sees[i] >> k & 1) {
+                                // (an infinity times a weight that has become zero stays one)
+                                const float w = s_p[(warp * kShKeys + k) * kRw + i], x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[i][c][e] = fmaf(fabsf(x[e]) <= FLT_MAX ? w : fmaxf(w, FLT_MIN), x[e], o[i][c][e]);
+                            }
                     }
                 }
             }

@@ -645,7 +645,7 @@ __device__ void st_many(const CUtensorMap& tmK, const CUtensorMap& tmV, const St
                 ok = tc_wait_warp(odone, (was + i - 1) & 1, gave_up, sa.polls);
                 if (!ok) break;
                 tc_fence_after();
-                const float nr = fmaxf(ref, mx), f = nr == ref ? 1.0f : tc_exp2(ref - nr);
+                const float nr = mx > ref + 8.0f ? mx : ref, f = nr == ref ? 1.0f : tc_exp2(ref - nr);      // (each row by what it sees itself: no other row's keys show in its bits)
                 l *= f;
                 lw *= f;
                 ref = nr;

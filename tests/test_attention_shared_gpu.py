@@ -275,3 +275,22 @@ def test_many_groups(n, dtype):
     """More groups than a CTA looks at in one turn."""
     s = SharedStep([((13 * i) % 150, _owns(1 + (i % 97 == 5) * 3, 60, 1 + (i % 101 == 7) * 20)) for i in range(n)], 4, 2, 64, dtype=dtype)
     _close(s.run()[0], s.want())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_later_keys_show_in_no_bit(dim, softcap, dtype):
+    """A token's results are the same numbers whatever the keys and values behind it hold, although rows beside it see them."""
+    s = SharedStep([(200, [(0, 150), (30, 100)]), (700, [(0, 2)])], 8, 2, dim, dtype=dtype, seed=11)
+    first = s.run(softcap=softcap)[0]
+    for i, at in ((0, 75), (1, 40), (2, 1)):
+        _, pos, n = s.segs[i]
+        for j in range(pos + at, pos + n):
+            page, row = s.table_np[i, j // s.page], j % s.page
+            s.k[page, :, row] *= 30
+            s.v[page, :, row] = math.inf if j % 2 else 3e38
+    again = s.run(softcap=softcap)[0]
+    for rows in (slice(0, 75), slice(150, 190), slice(250, 251)):
+        assert torch.equal(first[rows], again[rows]), rows
+    assert not torch.equal(first, again)
