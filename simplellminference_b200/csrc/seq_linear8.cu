@@ -32,11 +32,23 @@ __device__ __forceinline__ uint32_t qz_pack(int a, int b, int c, int d) {
 template <int N>
 __device__ __forceinline__ void qz_codes(const float (&x)[N], float inv, float scale, int (&q)[N]) {
     float near = 0.0f;
+    if constexpr (N == 1) {
+        const float r = x[0] * inv, whole = r + kQzMagic;
+        near = fabsf(r - (whole - kQzMagic));
+        q[0] = __float_as_int(whole);
+    } else {                                 // two at a time: the instructions are what bounds a matrix of rows
+        auto both = [](float v) { return tc_two(__float_as_uint(v), __float_as_uint(v)); };
+        const uint64_t inv2 = both(inv), magic = both(kQzMagic), less = both(-kQzMagic), minus = both(-1.0f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const float r = x[e] * inv, whole = r + kQzMagic;
-        near = fmaxf(near, fabsf(r - (whole - kQzMagic)));
-        q[e] = __float_as_int(whole);
+        for (int e = 0; e < N; e += 2) {
+            const uint64_t r = tc_mul2(tc_two(__float_as_uint(x[e]), __float_as_uint(x[e + 1])), inv2), whole = tc_add2(r, magic);
+            float a, b;
+            tc_split(tc_fma2(tc_add2(whole, less), minus, r), a, b);
+            near = tc_max3(near, fabsf(a), fabsf(b));
+            tc_split(whole, a, b);
+            q[e] = __float_as_int(a);
+            q[e + 1] = __float_as_int(b);
+        }
     }
     if (near > 0.5f - 6.103515625e-05f) {
 #pragma unroll
@@ -79,10 +91,11 @@ __global__ void __launch_bounds__(kMost) quantise_rows_kernel(QuantiseArgs p) {
             } else {
                 const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top = kBf16 ? max(top, max(w[e] << 16 & 0x7fff0000u, w[e] & 0x7fff0000u)) : max(top, w[e] & 0x7fffffffu);
+                for (int e = 0; e < 4; ++e) top = kBf16 ? __vmaxu2(top, w[e] & 0x7fff7fffu) : max(top, w[e] & 0x7fffffffu);
             }
         }
     }
+    if (kVec && kBf16) top = max(top << 16, top & 0xffff0000u);              // two values' bits beside one another until here
     top = __reduce_max_sync(0xffffffffu, top);
     if (n > 32) {                            // the row's warps, by a barrier of their own where the CTA has several rows
         const int warp = (threadIdx.y * n + i) >> 5, first = threadIdx.y * n >> 5;
