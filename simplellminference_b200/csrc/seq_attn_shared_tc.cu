@@ -844,7 +844,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             tc_fence_before();
             __syncthreads();
             const bool all = p.n_groups <= kStEntries;           // of the first entries: every group is at hand
-            if (e0 == 0 && warp == 0) {
+            if (e0 == 0 && warp == kStWarps - 1) {               // (as a rule without an entry: the others look their groups up meanwhile)
                 const int least = all ? st_least(p, all_sets, [&](int g, int& t, int& k) { t = plan.tiles[g]; k = (plan.end[g] + kStKeys - 1) / kStKeys; })
                                       : st_least(p, all_sets, [&](int g, int& t, int& k) {
                                             int first, m;
