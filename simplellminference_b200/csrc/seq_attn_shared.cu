@@ -400,7 +400,11 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     cudaStream_t st = as_stream(stream);
     const bool tc = kv_dtype == SLLM_BF16 && dk == dv && (dk == 64 || dk == 128);
     p.least = 64;
-    p.own_least = tc ? 512 : 64;
+    // On the tensor cores' kernel a share of a segment's own keys costs as much as some hundred keys at its beginning and end, so it has 512 unless there are too few segments to occupy two CTAs an SM.
+    // us, 512 always | like this: a token behind 2000 positions of its own 29.9 | 17.5, four behind 1000 31.6 | 17.7, 16 behind 500 and 1000 shared ones 32.6 | 28.2, a portion of 512 37.0 | 33.0;
+    // half as long where there are segments enough, that portion took 40.5.
+    const int64_t units = (int64_t)b->n_qtiles * kv_heads;
+    p.own_least = tc ? (int)std::min<int64_t>(512, std::max<int64_t>(128, (512 * units / (2 * sm_count()) + 63) / 64 * 64)) : 64;
     const int rc = tc ? launch_attention_shared_tc(p, st) : kv_dtype == SLLM_F32 ? sh_launch<float, 4>(p, st) : sh_launch<uint16_t, 4>(p, st);
     return rc ? rc : sh_merge(p, st);
 }
