@@ -3,8 +3,6 @@
 //   s_j = scale * (q . k_j),  p = softmax over the visible j,  o = sum_j p_j v_j
 // The keys j below the group's shared length are read once for all tokens of the group: the query heads of a kv head and all the tokens are the rows of one product. The keys from there on are each
 // segment's own. Both leave (reference, sum, weighted values) of every row, and a last kernel puts them together. A hidden key's values may be anything: they reach no row that does not see it.
-#include <cfloat>
-
 #include "seq_attn_shared.cuh"
 
 namespace sllm {
@@ -51,6 +49,7 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
         int in_page, page = sh_page(p, sp.slot, sp.key0 / kShKeys * kShKeys, in_page);           // (pages are a multiple of 32 positions)
         int pos[kRw];
         float m[kRw], l[kRw], o[kRw][2][4], slope[kRw];
+        bool infinite = false;                                           // a tile so far had values that are no numbers
 #pragma unroll
         for (int i = 0; i < kRw; ++i) {
             const int r = r0 + warp * kRw + i;
@@ -104,6 +103,7 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
                 for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
             });
             odd = __syncthreads_or(odd);
+            infinite |= odd != 0;
             const int key = j0 + lane;
             float s[kRw] = {};
 #pragma unroll 4
@@ -131,12 +131,17 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
 #pragma unroll
             for (int i = 0; i < kRw; ++i) {
                 top[i] = fmaxf(m[i], top[i]);
-                f[i] = top[i] == -INFINITY ? 1.0f : fmaxf(expf(m[i] - top[i]), FLT_MIN);
+                f[i] = top[i] == -INFINITY ? 1.0f : expf(m[i] - top[i]);
                 const float w = s[i] == -INFINITY ? 0.0f : expf(s[i] - top[i]);
                 m[i] = top[i];
                 l[i] = fmaf(l[i], f[i], w);              // of this lane's keys
+                if (!infinite) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] *= f[i];
+                    for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] *= f[i];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) o[i][c / 4][c % 4] = sh_carried(o[i][c / 4][c % 4], f[i]);
+                }
                 s_p[(warp * kShKeys + lane) * kRw + i] = w;
             }
             __syncwarp();
@@ -160,10 +165,9 @@ __device__ __forceinline__ void sh_rows(const SharedArgs& p, const ShSpan& sp, i
 #pragma unroll
                         for (int i = 0; i < kRw; ++i)
                             if (sees[i] >> k & 1) {
-                                // (an infinity times a weight that has become zero stays one)
                                 const float w = s_p[(warp * kShKeys + k) * kRw + i], x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) o[i][c][e] = fmaf(fabsf(x[e]) <= FLT_MAX ? w : fmaxf(w, FLT_MIN), x[e], o[i][c][e]);
+                                for (int e = 0; e < 4; ++e) o[i][c][e] = sh_add(o[i][c][e], w, x[e]);
                             }
                     }
                 }
@@ -257,8 +261,7 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
         float f[2], sum = 0.0f, o[2][4] = {};
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            // nothing seen: nothing (a sum of NaN goes on); else never zero, so that an infinity stays one
-            f[x] = head[x].x == -INFINITY && head[x].y == 0.0f ? 0.0f : fmaxf(exp2f(head[x].x - top), FLT_MIN);
+            f[x] = head[x].x == -INFINITY && head[x].y == 0.0f ? 0.0f : exp2f(head[x].x - top);      // nothing seen: nothing (a sum of NaN goes on)
             sum = fmaf(f[x], head[x].y, sum);
         }
         sum = warp_sum(sum);
@@ -274,6 +277,24 @@ __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedA
                 for (int k = 0; k < kAhead; ++k) {
                     if (k0 + k >= count) break;
                     o[c][0] = fmaf(w[k], x[k].x, o[c][0]); o[c][1] = fmaf(w[k], x[k].y, o[c][1]); o[c][2] = fmaf(w[k], x[k].z, o[c][2]); o[c][3] = fmaf(w[k], x[k].w, o[c][3]);
+                }
+            }
+        }
+        // NaN: as a rule an infinity times a factor that 32 bits have no number for, which is to stay an infinity. Once more, asking for each
+        bool none = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) none |= o[e / 4][e % 4] != o[e / 4][e % 4];
+        if (__any_sync(0xffffffffu, none)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e / 4][e % 4] = 0.0f;
+#pragma unroll 1
+            for (int k = 0; k < count; ++k) {
+                const float w = __shfl_sync(0xffffffffu, k < 32 ? f[0] : f[1], k & 31);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    if (c * 128 + 4 * lane >= p.dv) break;
+                    const float4 y = *reinterpret_cast<const float4*>(place(k) + kShHead + c * 128 + 4 * lane);
+                    o[c][0] = sh_add(o[c][0], w, y.x); o[c][1] = sh_add(o[c][1], w, y.y); o[c][2] = sh_add(o[c][2], w, y.z); o[c][3] = sh_add(o[c][3], w, y.w);
                 }
             }
         }

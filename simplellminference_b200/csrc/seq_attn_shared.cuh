@@ -1,5 +1,7 @@
 // csrc/seq_attn_shared.cuh — what the kernels of attention behind shared first positions have in common (seq_attn_shared.cu).
 #pragma once
+#include <cfloat>
+
 #include "seq_attn.cuh"
 
 namespace sllm {
@@ -99,6 +101,10 @@ __device__ __forceinline__ float sh_score(float s, float softcap, float slope, i
     if (softcap > 0.0f) s = softcap * tanhf(s / softcap);
     return fmaf(-slope, (float)(pos - key), s);
 }
+// Weights and the factors that carry sums to another reference are never zero, but 32 bits may hold no more than a zero for one: for finite numbers that is what it is, an infinity (or NaN) stays what
+// it is. (A least weight instead of the zero brought 1e36 times 2^-126 into results of size 1.)
+__device__ __forceinline__ float sh_carried(float sum, float factor) { return fabsf(sum) <= FLT_MAX ? sum * factor : sum; }
+__device__ __forceinline__ float sh_add(float sum, float w, float x) { return fabsf(x) <= FLT_MAX ? fmaf(w, x, sum) : sum + x; }
 
 #endif
 

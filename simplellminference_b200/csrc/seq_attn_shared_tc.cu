@@ -18,8 +18,6 @@
 // it reads, and a tile of 128 rows would be empty but for four. A CTA does two items at once, since one is a chain (queries, pages, keys and values, maximum, sums, four parts put together), and the
 // next keys and values are on their way to shared memory meanwhile. The columns of a head are contracted in an order of the kernel's own, 16 bytes a lane, and those of the values are dealt to the
 // tiles of O so that a lane's eight neighbours are rows of four of them. 64 tokens with 200 positions each of their own 28 us, with 400 40 (4.2 TB/s between the two).
-#include <cfloat>
-
 #include "seq_attn_shared.cuh"
 #include "tcgen05.cuh"
 
@@ -120,6 +118,7 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
         // columns of the products: rows r0 .. r0 + 7. As an operand a lane has row g, as a result rows 2t and 2t + 1
         int pos[2];
         float slope[2], m[2] = {-INFINITY, -INFINITY}, l[4] = {}, o[kTiles][4] = {};      // l: of rows 2t, 2t + 1, twice
+        bool infinite = false;               // a value so far was no number
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = r0 + 2 * t + i, qi = st_token(sa, r);
@@ -211,11 +210,17 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
                 top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
             }
             if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-                // (never zero: an infinity that has come in stays one)
-                const float f0 = top[0] == m[0] ? 1.0f : fmaxf(tc_exp2(m[0] - top[0]), FLT_MIN), f1 = top[1] == m[1] ? 1.0f : fmaxf(tc_exp2(m[1] - top[1]), FLT_MIN);
+                const float f0 = top[0] == m[0] ? 1.0f : tc_exp2(m[0] - top[0]), f1 = top[1] == m[1] ? 1.0f : tc_exp2(m[1] - top[1]);
                 l[0] *= f0; l[1] *= f1; l[2] *= f0; l[3] *= f1;
+                if (!infinite) {
 #pragma unroll
-                for (int c = 0; c < kTiles; ++c) { o[c][0] *= f0; o[c][1] *= f1; o[c][2] *= f0; o[c][3] *= f1; }
+                    for (int c = 0; c < kTiles; ++c) { o[c][0] *= f0; o[c][1] *= f1; o[c][2] *= f0; o[c][3] *= f1; }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[c][i] = sh_carried(o[c][i], i & 1 ? f1 : f0);
+                }
                 m[0] = top[0];
                 m[1] = top[1];
             }
@@ -249,6 +254,7 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
 #pragma unroll
                 for (int i = 0; i < 4; ++i) st_times_zero(odd, v[i]);
                 if (__any_sync(0xffffffffu, st_odd(odd))) {
+                    infinite = true;
                     const uint16_t* vr = value_row(at_page, at_in);
 #pragma unroll 1
                     for (int key = 0; key < 16; ++key) {
@@ -304,7 +310,7 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
 #pragma unroll
             for (int w = 0; w < kStTeam; ++w) {
                 const float y = reinterpret_cast<const float*>(area(w))[8 * HD + 8 + i];
-                f[w] = f[w] == -INFINITY && y == 0.0f ? 0.0f : fmaxf(tc_exp2(f[w] - mx), FLT_MIN);
+                f[w] = f[w] == -INFINITY && y == 0.0f ? 0.0f : tc_exp2(f[w] - mx);
                 all = fmaf(f[w], y, all);
             }
             const int qi = st_token(sa, r0 + i);
@@ -319,6 +325,14 @@ __device__ __forceinline__ void st_few(const StArgs& sa, const StItem& it, uint8
                 for (int w = 0; w < kStTeam; ++w) {      // (a part without keys is zeros)
                     const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(area(w)) + i * HD + 4 * lane);
                     y.x = fmaf(f[w], x.x, y.x); y.y = fmaf(f[w], x.y, y.y); y.z = fmaf(f[w], x.z, y.z); y.w = fmaf(f[w], x.w, y.w);
+                }
+                if (y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w) {      // NaN: as a rule an infinity times a factor that 32 bits have no number for, which is to stay an infinity
+                    y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < kStTeam; ++w) {
+                        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(area(w)) + i * HD + 4 * lane);
+                        y.x = sh_add(y.x, f[w], x.x); y.y = sh_add(y.y, f[w], x.y); y.z = sh_add(y.z, f[w], x.z); y.w = sh_add(y.w, f[w], x.w);
+                    }
                 }
                 *reinterpret_cast<float4*>(rec + kShHead + 4 * lane) = y;
             }
