@@ -828,13 +828,14 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
         st_barriers<HD>(smem);
-        *gave_up = 0;
+        *gave_up = sa.polls == 0;
         st_gave_up<HD>(smem)[1] = 0;             // of the first item; each makes that of the next one ready
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 5) tc_alloc(tmem_slot, kStTmem);
     uint32_t done = 0, turn = 0;             // key tiles and items of the first kind so far
     long long mine = blockIdx.x;             // the next item of this CTA, counted from the present entries' first
+    bool stop = sa.polls == 0;               // a wait was given up: agreed on at an item's end, since a thread that looked at the flag by itself could see what another one set in the next item
     const int entries = p.n_groups + p.b.n_qtiles;
     for (int e0 = 0; e0 < entries; e0 += kStEntries) {
         {   // an entry a thread
@@ -903,7 +904,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
         tc_fence_after();                    // (the allocation, at the first turn)
         const uint32_t tmem = *tmem_slot;
         const int total = plan.upto[kStEntries - 1];
-        for (; mine < total && !*gave_up; mine += gridDim.x) {
+        for (; mine < total && !stop; mine += gridDim.x) {
             int e = 0;                       // the first entry that reaches beyond it
             for (int w = kStEntries / 2; w > 0; w /= 2)
                 if (plan.upto[e + w - 1] <= (int)mine) e += w;
@@ -935,13 +936,13 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
                 st_many<HD, kOpts>(tmK, tmV, sa, it, smem, tmem, done, turn++);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the next item's copies may land where this one has written
-            __syncthreads();
+            stop = __syncthreads_or(*gave_up);
         }
         mine -= total;
         __syncthreads();                     // the entries have been read
-        if (*gave_up) break;
+        if (stop) break;
     }
-    if (*gave_up) tc_gave_up(sa.status);
+    if (stop) tc_gave_up(sa.status);
     if (warp == 5) {
         tc_fence_after();
         tc_dealloc(*tmem_slot, kStTmem);
