@@ -940,7 +940,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
         }
         mine -= total;
         __syncthreads();                     // the entries have been read
-        if (stop) break;
+        if (stop && blockIdx.x > 0) break;   // (the first CTA leaves the plan of every tile, whatever became of the items: the last kernel goes by it)
     }
     if (stop) tc_gave_up(sa.status);
     if (warp == 5) {

@@ -37,3 +37,12 @@ def test_the_whole_cta_stops(groups, polls):
         s = SharedStep(groups, 8, 2, dim)
         reported = _after_waits_of(polls, s, s.want(), 5)
         assert reported == 5 or polls > 0
+
+
+@pytest.mark.parametrize("polls", [0, 1])
+@pytest.mark.parametrize("n", [300, 700])
+def test_more_tiles_than_a_turn_of_the_plan(n, polls):
+    """The plan is made for 256 groups and tiles at a time; the last kernel asks for all of it. The workspace holds ones in every bit before the call."""
+    s = SharedStep([((13 * i) % 150, [((7 * i) % 60, 1 + (i % 101 == 7) * 20)]) for i in range(n // 2)] + [(64, [(i % 50, 1) for i in range(n // 2)])], 8, 2, 64)
+    reported = _after_waits_of(polls, s, s.want(), 3)
+    assert reported == 3 or polls > 0
