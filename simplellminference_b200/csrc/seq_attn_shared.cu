@@ -236,9 +236,9 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
 template <bool kVec, int kAhead>         // results 16 bytes at a time; records on their way at once
 __global__ void __launch_bounds__(128) seq_attention_shared_merge_kernel(SharedArgs p) {
     after_previous();
-    const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], cuts = p.plan[blockIdx.x], lane = threadIdx.x & 31;
-    const int n = min(kBQ, p.b.seg_len[seg] - off), t0 = p.b.seg_start[seg] + off, step = p.dv + kShHead;
-    const int first = min(cuts & 0xffff, p.shares), count = first + min(cuts >> 16 & 0xffff, p.own);      // (no more than there are places for, whatever the plan may say)
+    const int seg = p.b.qt_seg[blockIdx.x], off = p.b.qt_off[blockIdx.x], cuts = (int)__vminu2(p.plan[blockIdx.x], p.shares | p.own << 16), lane = threadIdx.x & 31;
+    // (no more records than there are places for, whatever the plan may say)
+    const int n = min(kBQ, p.b.seg_len[seg] - off), t0 = p.b.seg_start[seg] + off, first = cuts & 0xffff, count = first + (cuts >> 16), step = p.dv + kShHead;
     for (int i = blockIdx.y * 4 + (threadIdx.x >> 5); i < n * p.heads; i += gridDim.y * 4) {
         const int t = t0 + i / p.heads, h = i % p.heads;
         const float* recs = sh_record(p, t, h, 0);

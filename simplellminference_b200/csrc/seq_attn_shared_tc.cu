@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
     if (warp == 5) tc_alloc(tmem_slot, kStTmem);
     uint32_t done = 0, turn = 0;             // key tiles and items of the first kind so far
     long long mine = blockIdx.x;             // the next item of this CTA, counted from the present entries' first
-    bool stop = sa.polls == 0;               // a wait was given up: agreed on at an item's end, since a thread that looked at the flag by itself could see what another one set in the next item
+    bool stop = sa.polls == 0;               // a wait was given up
     const int entries = p.n_groups + p.b.n_qtiles;
     for (int e0 = 0; e0 < entries; e0 += kStEntries) {
         {   // an entry a thread
@@ -936,7 +936,8 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
                 st_many<HD, kOpts>(tmK, tmV, sa, it, smem, tmem, done, turn++);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the next item's copies may land where this one has written
-            stop = __syncthreads_or(*gave_up);
+            stop = *gave_up;                 // (what this item's waits set it to lies behind a barrier, what the next one's do behind the one that follows: all threads see the same)
+            __syncthreads();
         }
         mine -= total;
         __syncthreads();                     // the entries have been read
