@@ -542,7 +542,7 @@ int sllm_seq_attention_out(const sllm_seq_batch* b, const float* q, int32_t ldq,
                            const sllm_seq_attn_opts* opts, float* out, int32_t ldo, void* out16, sllm_stream_t stream);
 /* sllm_seq_attention_out for segments in groups whose first positions are the same. Segments group_start[g] .. group_start[g + 1] - 1 (device arrays; group_start [n_groups + 1] ascends from 0 to
  * nseg) share their positions 0 .. group_len[g] - 1, which are read once for all their tokens, through the block table of the group's first segment; the positions behind them through each
- * segment's own. Segments come in the order of their tokens. 0: nothing is shared; a token sees no position behind its own, whatever group_len says. Pools in fp32 or bf16 (queries are then
+ * segment's own. Segments come in the order of their tokens. 0: nothing is shared; a token sees no position behind its own, whatever group_len says. A table has room for up to 2^31 - 2^26 - 1 positions. Pools in fp32 or bf16 (queries are then
  * rounded to bf16) of n_pages pages: no others are touched, keys whose page the table does not have are hidden, and a token that sees none gives zeros. Options: window, keep_first, softcap,
  * slopes; the others are SLLM_ENOTSUP. Head widths are multiples of 8 up to 256, scale is positive. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16: the fp32 result
  * rounded); rows of tokens in no listed tile stay as they are. ws: at least sllm_seq_attention_shared_ws_bytes bytes, which need no contents; calls that may run at the same time need one each. */

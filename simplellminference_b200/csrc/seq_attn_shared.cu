@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kShWarps * 32) seq_attention_shared_kernel(Sha
         int tile = blockIdx.x, first, n;
         const int i = sh_find_group(p, tokens, tile, first, n);
         if (i < 0) return;
-        const int len = max(0, p.group_len[i]), tiles = (len + kShKeys - 1) / kShKeys, cuts = sh_cuts(len, p.least, p.shares);
+        const int len = sh_group_len(p, i), tiles = (len + kShKeys - 1) / kShKeys, cuts = sh_cuts(len, p.least, p.shares);
         if (z >= cuts) return;
         sp.tok0 = first + tile * tokens;
         sp.n_rows = min(tokens, n - tile * tokens) * per;
@@ -401,6 +401,7 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     SLLM_REQUIRE(kv_heads <= 65535, SLLM_ENOTSUP, "seq_attention_shared: %d kv heads", kv_heads);
     SLLM_REQUIRE(scale > 0.0f && scale <= FLT_MAX, SLLM_EINVAL, "seq_attention_shared: scores need a positive finite scale");
     SLLM_REQUIRE(b->page_len > 0 && b->page_len % kBK == 0, SLLM_ENOTSUP, "seq_attention_shared: pages of a multiple of %d positions", kBK);
+    SLLM_REQUIRE((int64_t)b->max_pages * b->page_len <= kShMostPositions, SLLM_ENOTSUP, "seq_attention_shared: tables of up to %d positions", kShMostPositions);
     SLLM_REQUIRE(ldq >= heads * dk && (!out || ldo >= heads * dv), SLLM_EINVAL, "seq_attention_shared: a row is shorter than its heads");
     SLLM_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) % 16) == 0, SLLM_EINVAL, "seq_attention_shared: pools have to start at a multiple of 16 bytes");
     SLLM_REQUIRE(ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= sllm_seq_attention_shared_ws_bytes(b, n_groups, heads, kv_heads, dk, dv), SLLM_EINVAL,
@@ -409,6 +410,7 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     SLLM_REQUIRE(!opts || (!opts->values_in_keys && !opts->logdist && !opts->cross_values && !opts->chunk), SLLM_ENOTSUP,
                  "seq_attention_shared: values in keys, charges on the logarithm of the distance, values of every head and chunks are not part of this form");
     SharedArgs p{*b, n_groups, group_start, group_len, q, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, INT_MAX, 0, 0.0f, nullptr, 0, 0,
+                 b->max_pages * b->page_len,
                  (uint32_t)(((1ull << 32) + b->page_len - 1) / b->page_len), 0, 0, (int*)ws,
                  (float*)((char*)ws + sh_plan_bytes(b->n_qtiles)), nullptr, out, ldo, (uint16_t*)out16};
     if (opts) {

@@ -25,6 +25,7 @@ struct SharedArgs {
     float softcap;
     const float* slopes;
     int shares, own;                     // records of a (token, head) at most: of the shared positions, of its own
+    int table_len;                       // positions that a row of the block table has room for
     uint32_t page_magic;                 // ceil(2^32 / page_len): the page of a position without a division (page_of)
     int least, own_least;                // keys of a share at least (least: of the kernel that does not plan it itself)
     int* plan;                           // of every listed tile: its records of shared positions, and its own ones << 16
@@ -38,6 +39,8 @@ struct SharedArgs {
 // What a CTA leaves of the keys it has seen, for a (token, head): the reference of the weights as a power of two, their sum, and the weighted sum of the values. Records lie
 // [token][head][shares + own][dv + 4].
 constexpr int kShHead = 4;               // floats in front of the values (16 bytes, so that these are aligned)
+// positions of a table at most: added to the keys of a share, whole tiles and the like, 2^26 at most, they stay within 32 bits
+constexpr int kShMostPositions = 0x7fffffff - (1 << 26);
 // bytes in front of the records: the plan
 inline int64_t sh_plan_bytes(int n_qtiles) { return ((int64_t)n_qtiles * 4 + 15) / 16 * 16; }
 
@@ -61,11 +64,13 @@ __device__ __forceinline__ void sh_group_tokens(const SharedArgs& p, int g, int&
     first = p.b.seg_start[s0];
     n = max(0, min(p.b.seg_start[s1 - 1] + p.b.seg_len[s1 - 1], p.b.T) - first);
 }
+// positions that a group shares, whatever it says: those that a table has room for, since none of the others has a page
+__device__ __forceinline__ int sh_group_len(const SharedArgs& p, int g) { return min(max(0, p.group_len[g]), p.table_len); }
 // positions that segment `seg` shares with its group (by whole warps)
 __device__ __forceinline__ int sh_shared_len(const SharedArgs& p, int seg) {
     int upto = 0;                        // groups that begin at or before the segment
     for (int i = threadIdx.x & 31; i - (int)(threadIdx.x & 31) < p.n_groups; i += 32) upto += __popc(__ballot_sync(0xffffffffu, i < p.n_groups && p.group_start[i] <= seg));
-    return upto > 0 ? max(0, p.group_len[upto - 1]) : 0;
+    return upto > 0 ? sh_group_len(p, upto - 1) : 0;
 }
 // The group that holds row tile `tile` of tiles of `tokens` tokens, group after group, its first token and how many it has; `tile` becomes the tile's number in it (by whole warps). -1: there
 // are not so many.

@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
             int tok0 = 0, n = 0, slot = -1, from = 0, end = 0, cuts = 0, tiles = 0, seg = -1, shared = 0;
             if (e < p.n_groups) {
                 sh_group_tokens(p, e, tok0, n);
-                end = max(0, p.group_len[e]);
+                end = sh_group_len(p, e);
                 tiles = (n + sa.queries - 1) / sa.queries;
                 if (n > 0) slot = p.b.seg_slot[p.group_start[e]];
                 plan.n[i] = n; plan.end[i] = end; plan.tiles[i] = tiles; plan.from[i] = p.group_start[e]; plan.low[i] = INT_MAX; plan.high[i] = -1;
@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
                                             int first, m;
                                             sh_group_tokens(p, g, first, m);
                                             t = (m + sa.queries - 1) / sa.queries;
-                                            k = (max(0, p.group_len[g]) + kStKeys - 1) / kStKeys;
+                                            k = (sh_group_len(p, g) + kStKeys - 1) / kStKeys;
                                         });
                 if (lane == 0) plan.least = least;
             }
@@ -875,9 +875,9 @@ __global__ void __launch_bounds__(kStThreads, 2) seq_attention_shared_tc_kernel(
                     const int mid = (lo + hi) / 2;
                     if ((all && e0 == 0 ? plan.from[mid] : p.group_start[mid]) <= seg) lo = mid; else hi = mid;
                 }
-                from = min(all && e0 == 0 ? plan.end[lo] : max(0, p.group_len[lo]), end);
+                shared = all && e0 == 0 ? plan.end[lo] : sh_group_len(p, lo);
+                from = min(shared, end);
                 cuts = sh_cuts(end - from, p.own_least, p.own);
-                shared = all && e0 == 0 ? plan.end[lo] : max(0, p.group_len[lo]);
                 if (all && e0 == 0) {
                     atomicMin(&plan.low[lo], end - n);
                     atomicMax(&plan.high[lo], end - 1);

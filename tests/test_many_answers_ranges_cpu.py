@@ -1,0 +1,21 @@
+"""Sizes at the ends of their range that the operators of many answers to one prompt refuse on the host, before anything is launched (no device)."""
+import ctypes as C
+
+import pytest
+
+from simplellminference_b200 import _lib
+from test_many_answers_cpu import SHARED, _batch
+
+
+def _shared(b, **change):
+    a = {**SHARED, **change}
+    if a["opts"] is not None:
+        a["opts"] = C.byref(a["opts"])
+    return _lib.load().sllm_seq_attention_shared(C.byref(b), *a.values(), None)
+
+
+@pytest.mark.parametrize("max_pages,page_len", [(1 << 25, 64), (1 << 16, 1 << 15), ((1 << 31) - 1, 32), (32505857, 64)])
+def test_tables_of_more_positions_than_are_counted(max_pages, page_len):
+    """Positions, the keys of a share added to them and whole tiles stay within 32 bits."""
+    assert _shared(_batch(max_pages=max_pages, page_len=page_len)) == _lib.ENOTSUP
+    assert b"positions" in _lib.load().sllm_last_error()
