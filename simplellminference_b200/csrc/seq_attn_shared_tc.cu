@@ -366,7 +366,7 @@ struct StTiles {
         first = key0 / kStKeys;
         const int end = (key1 + kStKeys - 1) / kStKeys;
         lo = min(max(first, oldest / kStKeys), max(end, first));
-        n_keep = max(0, min(lo, (keep_first + kStKeys - 1) / kStKeys) - first);
+        n_keep = max(0, (min(keep_first, lo * kStKeys) + kStKeys - 1) / kStKeys - first);
         n = key1 > key0 ? n_keep + max(0, end - lo) : 0;
     }
     __device__ __forceinline__ int tile_of(int i) const { return i < n_keep ? first + i : lo + i - n_keep; }

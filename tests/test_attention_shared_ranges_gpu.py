@@ -26,3 +26,13 @@ def test_many_groups_of_any_size(dtype):
     """More of them than a CTA looks at in one turn, one request each."""
     s = SharedStep([((13 * i) % 150, [((7 * i) % 60, 1 + (i % 101 == 7) * 20)]) for i in range(300)], 8, 2, 64, dtype=dtype)
     _close(s.run(groups=(s.group_start, torch.full((300,), MOST, dtype=torch.int32, device="cuda")))[0], s.want())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_first_positions_that_stay_visible_without_end(dim, dtype):
+    """Whatever the window, all positions are then seen."""
+    s = SharedStep([(400, [(10, 1), (100, 1)]), (130, [(0, 70)]), (0, [(300, 1), (7, 200)])], 8, 2, dim, dtype=dtype)
+    want = s.want()
+    for window, keep in ((100, MOST), (1, MOST - 40), (MOST, MOST), (60, 1 << 30)):
+        _close(s.run(window=window, keep_first=keep)[0], want)
