@@ -154,7 +154,7 @@ int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, int32_t n, c
 /* How likely tokens are, for all rows in one launch. Row r of `rows`: n logits at logits + r * ld; p = softmax. token [rows] int32 or NULL: logprob [rows] = ln p(token), rank [rows] int32 =
  * how many tokens come before it (larger logits, equal ones of a lower index); a token outside 0 .. n - 1 gives NaN and -1. entropy [rows] = -sum p ln p. top > 0 (32 at most): the most likely
  * tokens in that order, top_idx [rows][top] int32 and top_logprob [rows][top]. Outputs that are not wanted are NULL. A logit of -infinity has no probability; where logits are +infinity, those share
- * it evenly; a row with NaN, or of nothing but -infinity, gives NaN, its ranks and alternatives stay those of the order, in which NaN comes last. Sums are fp32, relative to the largest logit. */
+ * it evenly; a row with NaN, or of nothing but -infinity, gives NaN, its ranks and alternatives stay those of the order, in which NaN comes last. Sums are fp32, relative to the largest logit. Up to 2^30 logits a row. */
 int sllm_token_logprobs(const float* logits, int64_t ld, int32_t rows, int32_t n, const int32_t* token, float* logprob, float* entropy, int32_t* rank, int32_t top, int32_t* top_idx,
                         float* top_logprob, sllm_stream_t stream);
 

@@ -343,6 +343,7 @@ using namespace sllm;
 extern "C" int sllm_token_logprobs(const float* logits, int64_t ld, int32_t rows, int32_t n, const int32_t* token, float* logprob, float* entropy, int32_t* rank, int32_t top, int32_t* top_idx,
                                    float* top_logprob, sllm_stream_t stream) {
     SLLM_REQUIRE(logits && rows > 0 && n > 0, SLLM_EINVAL, "token_logprobs: null pointer, no rows or no logits");
+    SLLM_REQUIRE(n <= 1 << 30, SLLM_ENOTSUP, "token_logprobs: rows of %d logits", n);      // (indices go on to the end of a turn)
     SLLM_REQUIRE(ld >= n, SLLM_EINVAL, "token_logprobs: rows of %d logits lie %lld apart", n, (long long)ld);
     SLLM_REQUIRE(token || (!logprob && !rank), SLLM_EINVAL, "token_logprobs: a log probability and a rank are those of a given token");
     SLLM_REQUIRE(top >= 0 && top <= n, SLLM_EINVAL, "token_logprobs: %d alternatives of %d logits", top, n);

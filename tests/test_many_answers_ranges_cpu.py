@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from simplellminference_b200 import _lib
-from test_many_answers_cpu import SHARED, _batch
+from test_many_answers_cpu import LOGPROB, SHARED, _batch
 
 
 def _shared(b, **change):
@@ -19,3 +19,10 @@ def test_tables_of_more_positions_than_are_counted(max_pages, page_len):
     """Positions, the keys of a share added to them and whole tiles stay within 32 bits."""
     assert _shared(_batch(max_pages=max_pages, page_len=page_len)) == _lib.ENOTSUP
     assert b"positions" in _lib.load().sllm_last_error()
+
+
+@pytest.mark.parametrize("n", [(1 << 30) + 1, (1 << 31) - 1])
+def test_rows_of_more_logits_than_are_counted(n):
+    """Indices of logits go on to the end of a CTA's turn, which has to be a number of 32 bits, too."""
+    assert _lib.load().sllm_token_logprobs(*{**LOGPROB, "n": n, "ld": n}.values(), None) == _lib.ENOTSUP
+    assert b"token_logprobs" in _lib.load().sllm_last_error()
