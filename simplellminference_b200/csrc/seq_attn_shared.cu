@@ -406,7 +406,7 @@ int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const i
     SLLM_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) % 16) == 0, SLLM_EINVAL, "seq_attention_shared: pools have to start at a multiple of 16 bytes");
     SLLM_REQUIRE(ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= sllm_seq_attention_shared_ws_bytes(b, n_groups, heads, kv_heads, dk, dv), SLLM_EINVAL,
                  "seq_attention_shared: the workspace is too small or not aligned");
-    SLLM_REQUIRE(!opts || (opts->window >= 0 && opts->keep_first >= 0 && opts->softcap >= 0.0f), SLLM_EINVAL, "seq_attention_shared: bad options");
+    SLLM_REQUIRE(!opts || (opts->window >= 0 && opts->keep_first >= 0 && opts->softcap >= 0.0f && opts->softcap <= FLT_MAX), SLLM_EINVAL, "seq_attention_shared: bad options");
     SLLM_REQUIRE(!opts || (!opts->values_in_keys && !opts->logdist && !opts->cross_values && !opts->chunk), SLLM_ENOTSUP,
                  "seq_attention_shared: values in keys, charges on the logarithm of the distance, values of every head and chunks are not part of this form");
     SharedArgs p{*b, n_groups, group_start, group_len, q, ldq, heads, kv_heads, dk, dv, scale, k_pool, v_pool, n_pages, INT_MAX, 0, 0.0f, nullptr, 0, 0,

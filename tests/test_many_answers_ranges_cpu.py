@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from simplellminference_b200 import _lib
-from test_many_answers_cpu import LOGPROB, SHARED, _batch
+from test_many_answers_cpu import LOGPROB, SHARED, _batch, _opts
 
 
 def _shared(b, **change):
@@ -26,3 +26,10 @@ def test_rows_of_more_logits_than_are_counted(n):
     """Indices of logits go on to the end of a CTA's turn, which has to be a number of 32 bits, too."""
     assert _lib.load().sllm_token_logprobs(*{**LOGPROB, "n": n, "ld": n}.values(), None) == _lib.ENOTSUP
     assert b"token_logprobs" in _lib.load().sllm_last_error()
+
+
+@pytest.mark.parametrize("cap", [float("inf"), float("nan"), -1.0])
+def test_caps_that_are_no_numbers(cap):
+    """An infinite cap times the tanh of a score divided by it is NaN; a call without a cap is what is meant."""
+    assert _shared(_batch(), opts=_opts(softcap=cap)) == _lib.EINVAL
+    assert b"bad options" in _lib.load().sllm_last_error()
