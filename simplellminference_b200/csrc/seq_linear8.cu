@@ -1,7 +1,7 @@
 // csrc/seq_linear8.cu — products of 8-bit integers with a scale for every token and every output channel, and the rows of codes they read.
 //
 //   s_t = max(max_k |x_tk| / 127, 2^-126),  a_tk = round(x_tk / s_t);   C_tn = (sum_k a_tk w_nk) * s_t * v_n + bias_n
-// Sums of codes are exact in 32 bits (127 * 127 * 131072 < 2^31), so a result is three roundings of fp32 away from the formula and does not depend on how a product is cut.
+// Sums of codes are exact in 32 bits (127 * 127 * 131072 < 2^31; with codes of -128, which no row here gets, 2^14 * 131071 < 2^31), so a result is three roundings of fp32 away from the formula and does not depend on how a product is cut.
 #include <type_traits>
 
 #include "seq_common.cuh"

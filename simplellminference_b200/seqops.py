@@ -84,7 +84,8 @@ class Ops:
         self._ck(self.lib.sllm_seq_quantise_rows(x_ptr, int(bool(x_bf16)), ldx, codes_ptr, ldc, _p(scales), T, K, st))
 
     def linear8(self, a_ptr, lda, a_scale, w, ldw, w_scale, bias, c_ptr, ldc, T, N, K, st, accumulate=False):
-        """C = (a . w^T) * a_scale[t] * w_scale[n] (+ bias) (+ C): int8 codes [T][lda] and [N][ldw], rows at multiples of 16 bytes; sums exact, the result fp32."""
+        """C = (a . w^T) * a_scale[t] * w_scale[n] (+ bias) (+ C): int8 codes (-127 .. 127, as ``quantise_rows`` leaves them) [T][lda] and [N][ldw], rows at multiples of 16 bytes; sums
+        exact, the result fp32."""
         self._ck(self.lib.sllm_seq_linear8(a_ptr, lda, _p(a_scale), _p(w), ldw, _p(w_scale), _p(bias), c_ptr, ldc, T, N, K, int(bool(accumulate)), st))
 
     def linear_grouped(self, a_ptr, a_bf16, w, c_ptr, counts_ptr, groups, cap, rows_hint, N, K, st):
