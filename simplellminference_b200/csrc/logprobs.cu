@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LogprobAr
             if (listed == p.top) {               // the list is full: only what is larger than its last one (an equal one has a higher index), so the next float above
                 const uint64_t last = sh.list[turn][p.top - 1];
                 bound = last >> 32 == 0 ? -INFINITY : lp_unkey((uint32_t)(last >> 32) + 1);         // (NaN, which nothing reaches, above infinity)
-            } else {
+            } else {                             // the first turn: behind it the list is full, or there is no second one
+                static_assert(kTurn >= kLpTop, "a turn fills the list");
                 // `top` logits reach the `top`-th largest of the warps' largest threads, or half (a quarter) as many warps with two (four) each their second (fourth) (NaN is below everything)
                 const int each = p.top <= kLpWarps ? 1 : p.top <= 2 * kLpWarps ? 2 : 4;
                 uint32_t left = key, least = top;
@@ -190,7 +191,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(LogprobAr
                 }
                 const uint32_t reached = __shfl_sync(0xffffffffu, one, __ffs(__ballot_sync(0xffffffffu, ahead == (p.top + each - 1) / each - 1)) - 1);
                 bound = reached ? lp_unkey(reached) : -INFINITY;
-                if (listed > 0) bound = -INFINITY;       // (a short first turn: rare)
             }
             if (own >= bound || own != own) {
 #pragma unroll
