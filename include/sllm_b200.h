@@ -154,7 +154,8 @@ int sllm_sample_rows(const float* logits, int32_t ld, int32_t rows, int32_t n, c
 /* How likely tokens are, for all rows in one launch. Row r of `rows`: n logits at logits + r * ld; p = softmax. token [rows] int32 or NULL: logprob [rows] = ln p(token), rank [rows] int32 =
  * how many tokens come before it (larger logits, equal ones of a lower index); a token outside 0 .. n - 1 gives NaN and -1. entropy [rows] = -sum p ln p. top > 0 (32 at most): the most likely
  * tokens in that order, top_idx [rows][top] int32 and top_logprob [rows][top]. Outputs that are not wanted are NULL. A logit of -infinity has no probability; where logits are +infinity, those share
- * it evenly; a row with NaN, or of nothing but -infinity, gives NaN, its ranks and alternatives stay those of the order, in which NaN comes last. Sums are fp32, relative to the largest logit. Up to 2^30 logits a row. */
+ * it evenly; a row with NaN, or of nothing but -infinity, gives NaN, its ranks and alternatives stay those of the order, in which NaN comes last. Sums are fp32, relative to the largest logit. Up to
+ * 2^30 logits a row. */
 int sllm_token_logprobs(const float* logits, int64_t ld, int32_t rows, int32_t n, const int32_t* token, float* logprob, float* entropy, int32_t* rank, int32_t top, int32_t* top_idx,
                         float* top_logprob, sllm_stream_t stream);
 
@@ -543,10 +544,12 @@ int sllm_seq_attention_out(const sllm_seq_batch* b, const float* q, int32_t ldq,
                            const sllm_seq_attn_opts* opts, float* out, int32_t ldo, void* out16, sllm_stream_t stream);
 /* sllm_seq_attention_out for segments in groups whose first positions are the same. Segments group_start[g] .. group_start[g + 1] - 1 (device arrays; group_start [n_groups + 1] ascends from 0 to
  * nseg) share their positions 0 .. group_len[g] - 1, which are read once for all their tokens, through the block table of the group's first segment; the positions behind them through each
- * segment's own. Segments come in the order of their tokens. 0: nothing is shared; a token sees no position behind its own, whatever group_len says. A table has room for up to 2^31 - 2^26 - 1 positions. Pools in fp32 or bf16 (queries are then
- * rounded to bf16) of n_pages pages: no others are touched, keys whose page the table does not have are hidden, and a token that sees none gives zeros. Options: window, keep_first, softcap,
- * slopes; the others are SLLM_ENOTSUP. Head widths are multiples of 8 up to 256, scale is positive. The result as fp32 [T][ldo] (out) and / or dense bf16 [T][heads * dv] (out16: the fp32 result
- * rounded); rows of tokens in no listed tile stay as they are. ws: at least sllm_seq_attention_shared_ws_bytes bytes, which need no contents; calls that may run at the same time need one each. */
+ * segment's own. Segments come in the order of their tokens. 0: nothing is shared; a token sees no position behind its own, whatever group_len says. A table has room for up to
+ * 2^31 - 2^26 - 1 positions. Pools in fp32 or bf16 (queries are then rounded to bf16) of n_pages pages: no others are touched, keys whose page the table does not have are hidden, and a token that
+ * sees none gives zeros. Weighted sums are fp32 and taken before they are divided: results are numbers where values stay below 2^119 divided by the number of keys a token sees. Options: window,
+ * keep_first, softcap (finite), slopes; the others are SLLM_ENOTSUP. Head widths are multiples of 8 up to 256, scale is positive. The result as fp32 [T][ldo] (out) and / or dense bf16
+ * [T][heads * dv] (out16: the fp32 result rounded); rows of tokens in no listed tile stay as they are. ws: at least sllm_seq_attention_shared_ws_bytes bytes, which need no contents; calls that may
+ * run at the same time need one each. */
 int64_t sllm_seq_attention_shared_ws_bytes(const sllm_seq_batch* b, int32_t n_groups, int32_t heads, int32_t kv_heads, int32_t dk, int32_t dv);
 int sllm_seq_attention_shared(const sllm_seq_batch* b, int32_t n_groups, const int32_t* group_start, const int32_t* group_len, const float* q, int32_t ldq, int32_t heads, int32_t kv_heads,
                               int32_t dk, int32_t dv, float scale, const void* k_pool, const void* v_pool, int32_t kv_dtype, int32_t n_pages, void* ws, int64_t ws_bytes,

@@ -62,3 +62,15 @@ def test_infinite_values_without_weight(dim, dtype, value):
         fine = want.isfinite()
         assert not fine.all() and torch.equal(got[want.isinf()], want[want.isinf()])
         assert ((got - want).abs()[fine] <= 16 * 2.0 ** -24 * want.abs()[fine] + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_values_as_large_as_they_may_be(dim, dtype):
+    """Sums are taken before the division, with weights of up to 2^8: values of 2^119 divided by the number of keys stay numbers. Scores of size 1: 2^-24 * (8 + 16 + 20) of the largest value seen,
+    three times that over the norm."""
+    s = SharedStep([(700, [(0, 1), (200, 1), (10, 60)]), (0, [(900, 1), (0, 300)])], 8, 2, dim, dtype=dtype, seed=9)
+    s.v = (s.v.sign() * 2.0 ** 119 / 1024).to(dtype)
+    got, want = s.run()[0].double(), s.want()
+    assert torch.isfinite(got).all() and (got - want).norm() <= 8e-6 * want.norm()
+    assert (got - want).abs().max() <= 3e-5 * 2.0 ** 109
