@@ -456,10 +456,11 @@ typedef struct {
 int64_t sllm_seq_step_fill(int32_t* out, int64_t capacity, int32_t nseg, const int32_t* segments, const int32_t* tokens, const int32_t* rows, int32_t n_rows,
                            const sllm_kvpages* kp, int32_t tile, int64_t* offsets, int32_t* n_qtiles);
 /* Rows of fp32 (x_bf16 != 0: bf16) values to 8-bit integers with a scale a row: scale = max(max |x| / 127, 2^-126), code = x / scale rounded to fp32 and then to the nearest whole number (of two
- * as near the even one). A row with an infinite value or NaN gets the scale NaN and zeros. x [T][ldx] values, codes [T][ldc] int8 (columns behind K stay as they are), scales [T]. */
+ * as near the even one). A row with an infinite value or NaN gets the scale NaN and zeros. x [T][ldx] values, codes [T][ldc] int8 (columns behind K stay as they are), scales [T];
+ * T and K up to 2^30. */
 int sllm_seq_quantise_rows(const void* x, int32_t x_bf16, int64_t ldx, void* codes, int64_t ldc, float* scales, int32_t T, int32_t K, sllm_stream_t stream);
 /* C[t][n] = (sum_k a[t][k] * w[n][k]) * a_scale[t] * w_scale[n] + bias[n] (+ C[t][n] if accumulate): int8 codes a [T][lda] and w [N][ldw], rows of both at multiples of 16 bytes and readable up to
- * lda and ldw (what lies behind column K does not count), bias [N] or NULL, C fp32 [T][ldc]. Sums are exact for codes of -127 .. 127, as
+ * lda and ldw (what lies behind column K does not count), bias [N] or NULL, C fp32 [T][ldc], T and N up to 2^30. Sums are exact for codes of -127 .. 127, as
  * sllm_seq_quantise_rows leaves them, and K up to 131072 (where codes of -128 meet, up to 131071), then rounded to fp32; the products follow in this order. */
 int sllm_seq_linear8(const void* a, int64_t lda, const float* a_scale, const void* w, int64_t ldw, const float* w_scale, const float* bias, float* C, int64_t ldc, int32_t T, int32_t N, int32_t K,
                      int32_t accumulate, sllm_stream_t stream);

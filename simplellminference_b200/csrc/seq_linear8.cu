@@ -480,7 +480,7 @@ extern "C" {
 
 int sllm_seq_quantise_rows(const void* x, int32_t x_bf16, int64_t ldx, void* codes, int64_t ldc, float* scales, int32_t T, int32_t K, sllm_stream_t stream) {
     SLLM_REQUIRE(x && codes && scales && T > 0 && K > 0, SLLM_EINVAL, "seq_quantise_rows: null pointer, no rows or no columns");
-    SLLM_REQUIRE(K <= 1 << 30, SLLM_ENOTSUP, "seq_quantise_rows: %d columns", K);
+    SLLM_REQUIRE(T <= 1 << 30 && K <= 1 << 30, SLLM_ENOTSUP, "seq_quantise_rows: %d rows of %d columns", T, K);
     SLLM_REQUIRE(ldx >= K && ldc >= K, SLLM_EINVAL, "seq_quantise_rows: rows of %d values lie %lld and %lld apart", K, (long long)ldx, (long long)ldc);
     const int size = x_bf16 ? 2 : 4, run = x_bf16 ? 8 : 4;
     SLLM_REQUIRE((uintptr_t)x % size == 0, SLLM_EINVAL, "seq_quantise_rows: values are not aligned");
@@ -513,6 +513,7 @@ int sllm_seq_linear8(const void* a, int64_t lda, const float* a_scale, const voi
                      int32_t accumulate, sllm_stream_t stream) {
     SLLM_REQUIRE(a && a_scale && w && w_scale && C && T > 0 && N > 0 && K > 0, SLLM_EINVAL, "seq_linear8: null pointer or empty product");
     SLLM_REQUIRE(K <= 131072, SLLM_ENOTSUP, "seq_linear8: sums over %d products do not fit 32 bits", K);
+    SLLM_REQUIRE(T <= 1 << 30 && N <= 1 << 30, SLLM_ENOTSUP, "seq_linear8: %d rows for %d tokens", N, T);
     SLLM_REQUIRE(lda >= K && ldw >= K && ldc >= N, SLLM_EINVAL, "seq_linear8: a row is shorter than its values");
     SLLM_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && (((uintptr_t)a | (uintptr_t)w) % 16) == 0, SLLM_EINVAL, "seq_linear8: rows of codes have to start at multiples of 16 bytes");
     Linear8Args p{(const int8_t*)a, (const int8_t*)w, a_scale, w_scale, bias, C, lda, ldw, ldc, T, N, K, accumulate != 0};

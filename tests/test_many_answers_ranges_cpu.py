@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from simplellminference_b200 import _lib
-from test_many_answers_cpu import LOGPROB, SHARED, _batch, _opts
+from test_many_answers_cpu import LINEAR, LOGPROB, QUANTISE, SHARED, _batch, _opts
 
 
 def _shared(b, **change):
@@ -33,3 +33,15 @@ def test_caps_that_are_no_numbers(cap):
     """An infinite cap times the tanh of a score divided by it is NaN; a call without a cap is what is meant."""
     assert _shared(_batch(), opts=_opts(softcap=cap)) == _lib.EINVAL
     assert b"bad options" in _lib.load().sllm_last_error()
+
+
+MOST = (1 << 31) - 1
+
+
+@pytest.mark.parametrize("size", [(1 << 30) + 1, MOST - 7, MOST])
+def test_more_rows_than_are_counted(size):
+    """Rows are rounded up to whole tiles, which has to stay within 32 bits."""
+    f = _lib.load()
+    assert f.sllm_seq_quantise_rows(*{**QUANTISE, "T": size}.values(), None) == _lib.ENOTSUP and b"seq_quantise_rows" in f.sllm_last_error()
+    for change in ({"T": size}, {"N": size, "ldc": size}, {"N": size, "ldc": size, "T": 1}):
+        assert f.sllm_seq_linear8(*{**LINEAR, **change}.values(), None) == _lib.ENOTSUP and b"seq_linear8" in f.sllm_last_error()
