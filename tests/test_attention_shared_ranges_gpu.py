@@ -36,3 +36,11 @@ def test_first_positions_that_stay_visible_without_end(dim, dtype):
     want = s.want()
     for window, keep in ((100, MOST), (1, MOST - 40), (MOST, MOST), (60, 1 << 30)):
         _close(s.run(window=window, keep_first=keep)[0], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_segments_without_tokens(dtype):
+    """Places of a captured step that are not taken: segments of no tokens, tiles of them among the listed ones, a group of nothing else."""
+    groups = [(100, [(0, 1), (5, 0), (30, 40)]), (64, [(0, 0), (9, 0)]), (70, [(3, 0), (20, 1)]), (0, [(0, 0)])]
+    s = SharedStep(groups, 8, 2, 64, dtype=dtype, tiles=[(0, 0), (1, 0), (2, 32), (2, 0), (3, 0), (4, 0), (5, 0), (6, 0), (7, 0)])
+    _close(s.run()[0], s.want())
