@@ -3,12 +3,13 @@
 //   M = max x,  S = sum exp(x - M);  log p_t = (x_t - M) - log S;  entropy = log S + sum exp(x - M) (M - x) / S;  rank of t: logits in front of it (larger ones, equal ones with a lower
 //   index);  alternatives: the `top` first logits in that order.
 // S is held as 1 + R with the largest logit itself left out of R: log1p(R) and both terms of the entropy, neither of them negative, keep their bits where one token has nearly all the weight.
-// A cluster of up to eight CTAs shares a row; a CTA takes 8192 logits at a time into its registers, so that they are read once. A warp's sums are relative to its own largest so far. The threads'
-// largest logits give a bound that at least `top` logits reach, so that a few dozen of the first turn's are left to be put in order, by counting for each how many are in front of it; after that only
+// A cluster of up to eight CTAs shares a row; a CTA takes 8192 logits at a time into its registers (2048 where its part of the row is no longer than 4096), so that they are read once. A warp's sums
+// are relative to its own largest so far. The threads' largest logits give a bound that at least `top` logits reach, so that a few dozen of the first turn's are left to be put in order, by counting for each how many are in front of it; after that only
 // what is larger than the last of the list. Data that defeat the bound (hundreds of equal logits, nearly everything banned) are searched `top` times for the next one instead. Nothing depends on the
 // order of threads but the fp32 sums' fixed tree.
 // Bound: a turn is a chain (loads 2000 to 3000 clocks, largest and bound 1500, rank 1200, sums 1200, list 2000) that four CTAs an SM hide in part, and a row ends with two barriers of its cluster
-// and 4000 clocks for the lists. One row of 32000 logits 6.2 us (floor 0.02), 64 rows of 128256 with 20 alternatives 19.7 (5.0; the same in one turn of 16384 a CTA 23.5), 1000 rows 114 (78.2: 4.5 TB/s).
+// and 4000 clocks for the lists. One row of 32000 logits, two turns of 2048 a CTA, 6.2 us (floor 0.02), 64 rows of 128256 with 20 alternatives 19.7 (5.0; the same in one turn of 16384 a CTA 23.5),
+// 1000 rows 114 (78.2: 4.5 TB/s). A round of the machine is 592 CTAs: 592 rows of 128256 take 65 us, 600 90, 1184 127, so that some rows more than a round holds are the dearest.
 #include <cooperative_groups.h>
 
 #include <type_traits>

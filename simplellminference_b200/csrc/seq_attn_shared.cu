@@ -9,7 +9,7 @@ namespace sllm {
 
 // Any head width, pools in fp32 or bf16: a CTA takes 4 * kRw rows of a (group or segment, kv head) and a share of the keys, 32 at a time through shared memory; a warp has kRw rows, a lane one
 // key of them for the scores and four columns of the values for the sums; fp32 throughout.
-// Bound: a chain. Four answers of 16 heads of 64 behind 1500 positions 18.6 us with the last kernel, which are, in clocks: whose share it is 2900, queries and pages 3000, for each of its two key
+// Bound: a chain. Four answers of 16 heads of 64 behind 1500 positions 19 us with the last kernel, which are, in clocks: whose share it is 2900, queries and pages 3000, for each of its two key
 // tiles keys and values 3800, scores 1600, weights 1800 (the rows' shuffles side by side), sums 2000 (a key's four weights read together, nothing asked in between; with a question per key and row
 // they took 9500).
 constexpr int kShWarps = 4, kShKeys = 32;

@@ -5,15 +5,18 @@
 // made while these are worked on, and their products while the next are):
 //   warps 0-3  softmax, a thread per row: queries to bf16 rows in shared memory; per key tile the scores from TMEM, capped, charged and masked, fp32 maximum and sum; the weights go back to TMEM as
 //              THREE bf16 terms (24 bits; two leave 2^-18 of a weight, which is more than all the rest). O stays in TMEM, rescaled only where a maximum has grown by more than 2^8; the
-//              tensor core truncates as it adds, so every kStFlush tiles O moves on to the CTA's own place in the workspace, [columns / 4][rows] so that whole lines are read and written (with moves of 16
-//              bytes of a row a lane, to the rows' records, the mixed step took 290 us instead of 227); twelve tiles between two moves instead of seven gave results 1.4e-6 off instead of 9e-7;
+//              tensor core truncates as it adds, so every kStFlush tiles O moves on to the CTA's own place in the workspace, [columns / 4][rows] so that whole lines are read and written
+//              (moves of 16 bytes of a row a lane, to the rows' records, with the tiles of 64 keys that were there before: the mixed step 290 us instead of 223). Between two moves 6 | 9 | 12 | 18
+//              tiles: results of the mixed step 6.5e-7 | 9.0e-7 | 1.15e-6 | 1.6e-6 off (without moves 2.6e-6; the plain form in fp32 1.16e-6), 211 | 206 | 200 | 194 us;
 //   warp 4     (one lane) TMA producer: boxes of 16 positions, looked up in the block table; what is behind the last position or in no page reads as zeros;
 //   warp 5     (one lane) MMA issuer: S = Q K^T, O += (hi + mid + lo) V with the weights read from TMEM, V as it lies;
 //   warps 6-7  zero the value rows that are not part of the share, and take infinities and NaN out of the values (0 * NaN is NaN for rows that do not see them, and the terms of a weight times
 //              infinity are NaN for those that do); rows that see them get them back at the end.
 // Bound of this kind: 148 SMs take a key tile of 128 rows in 1400 clocks each (2100 with a cap). Its products are 800 of them and the rest of the softmax's instructions that two CTAs cannot hide;
-// an item begins with 6000 (its queries) and ends with 7500 (64 KB of records a CTA, all CTAs at once), the step's plan is 9000. 512 rows of 32 heads behind 4000 positions 113 us (71 GFLOP with
-// the weights' terms: 0.63 PFLOP/s); tiles of 64 keys, scores and weights one over the other, took 128, and then one CTA an SM with two such tiles, or two threads a row, no less.
+// an item begins with 6000 (its queries) and ends with 7500 (64 KB of records a CTA, all CTAs at once), the step's plan is 4000 to 6000 for eight answers and 5600 to 8400 for the mixed step.
+// 512 rows of 32 heads behind 4000 positions 111 us (71 GFLOP with the weights' terms: 0.64 PFLOP/s). All 128 registers of a thread are in use, and 40 to 64 bytes a
+// thread spilled (84 for heads of 128 with caps or charges). Tiles of 64 keys, scores and weights one over the other, took 128 us, and then one CTA an SM with two such tiles, or two threads a row, no
+// less.
 // Where a segment has few rows of its own (a decoding request: the query heads of one token), four warps take 16 keys in turn on mma.sync, 8 rows at a time as the columns: such work is bound by what
 // it reads, and a tile of 128 rows would be empty but for four. A CTA does two items at once, since one is a chain (queries, pages, keys and values, maximum, sums, four parts put together), and the
 // next keys and values are on their way to shared memory meanwhile. The columns of a head are contracted in an order of the kernel's own, 16 bytes a lane, and those of the values are dealt to the

@@ -145,8 +145,12 @@ __device__ __forceinline__ void l8_store(const Linear8Args& p, int t, int n, int
     *to = p.accumulate ? __fadd_rn(*to, v) : v;
 }
 
-// One or two tokens: a warp takes kRows rows of W, sixteen codes a load, four products an instruction, eight loads of W on their way. Bound: what those bring in. us, one token, 1 | 2 | 4 rows a warp:
-// 4096 x 4096 5.6 | 6.5 | 8.7, 4096 x 14336 14.7 | 17.8 | 24.5 (3.9 TB/s), 14336 x 4096 14.1 | 13.2 | 12.0 (4.9 TB/s). Two tokens 14.0; four of them 19.5, where tcgen05 takes 13.6.
+// One or two tokens: a warp takes kRows rows of W, sixteen codes a load, four products an instruction, eight loads of W on their way. Bound: what those bring in. us, N x K:
+//   one token, 1 | 2 | 4 rows a warp, tcgen05: 4096 x 4096 5.7 | 6.4 | 8.7, 7.1; 6144 x 4096 6.6 | 7.2 | 9.1, 8.7; 8192 x 4096 10.0 | 8.1 | 9.6, 9.7; 11008 x 4096 10.6 | 9.8 | 10.8, 11.1;
+//     14336 x 4096 14.2 | 13.7 | 12.2, 12.9; 28672 x 4096 24.5 | 21.3 | 22.6, 22.7; 4096 x 14336 14.8 | 17.7 | 24.3, 13.7; 8192 x 14336 28.7 | 22.7 | 26.8, 22.5
+//   two, 1 | 2 rows, tcgen05: 4096 x 4096 6.5 | 6.7, 7.2; 6144 x 4096 11.3 | 7.4, 8.7; 8192 x 4096 11.6 | 8.3, 9.8; 14336 x 4096 16.8 | 13.8, 12.8; 28672 x 4096 29.2 | 25.9, 23.2; 4096 x 14336 17.1 | 18.2, 13.7
+// One row a warp below kL8Wide rows, else four for one token and two for two, is right to a tenth in most places, not in all: two tokens through 6144 rows would be 7.4 with two rows a warp, and long
+// rows are faster on tcgen05 even for one token. Four tokens here took 19.5, where tcgen05 takes 13.6.
 constexpr int kL8Warps = 8, kL8Few = 2, kL8Wide = 8192;
 template <int kT, int kRows>
 __global__ void __launch_bounds__(kL8Warps * 32) linear8_few_kernel(Linear8Args p) {
